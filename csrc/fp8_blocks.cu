@@ -1,0 +1,412 @@
+// bf16 -> the 8-bit form with a scale for each block of 128 (fp8_blocks.cuh): the cast of a matrix, row-major and transposed, the
+// residual's addition and RMSNorm that end in it, and the way back.
+//
+//   cast    q = round8(x 2^-e), e from the largest magnitude of a block: 1 x 128 (activations, gradients) or 128 x 128 (weights, whose two
+//           copies then hold the same values).  A transposed copy of 1 x 128 blocks has blocks of 128 along the rows of x.
+//   norm    t = bf16(x + residual), rstd = 1 / sqrt(mean(t^2) + eps), h = cast(t rstd gain), the products in 32 bits
+//
+// An infinity or a NaN is stored as NaN, and the other values of its block are scaled as if it were not there.
+#include "fp8_blocks.cuh"
+
+namespace kf {
+namespace f8b {
+
+enum Source { PLAIN = 0, NORMED = 1 };  // the matrix itself, or x * rstd[row] * gain[column]
+
+__device__ __forceinline__ float2 pair_at(const uint4& v, int j) { return unpack_bf16(j == 0 ? v.x : j == 1 ? v.y : j == 2 ? v.z : v.w); }
+
+// largest magnitude over the 16 lanes of a half warp
+__device__ __forceinline__ float half_warp_max(float m) {
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) m = max_abs(m, __shfl_xor_sync(0xffffffffu, m, o));
+  return m;
+}
+
+// One 128 x 128 tile per block of 256 threads: 16 threads x 8 columns, 8 rows per thread.
+template <bool E5M2, int SRC, bool SQUARE>
+__global__ void __launch_bounds__(256)
+kf_cast_blocks(const __nv_bfloat16* __restrict__ x, int rows, int cols, long long ldx, const float* __restrict__ rstd,
+               const __nv_bfloat16* __restrict__ gain, uint8_t* __restrict__ out, long long ld_out, uint8_t* __restrict__ scales,
+               long long ld_scales, uint8_t* __restrict__ out_t, long long ld_t, uint8_t* __restrict__ scales_t, long long ld_scales_t) {
+  __shared__ uint32_t tile[128][32];  // bytes of the tile on their way to the transposed copy; first the column maxima
+  __shared__ float col_inv[128];
+  __shared__ uint8_t row_byte[128], col_byte[128];
+  __shared__ float red[8];
+  const int r0 = blockIdx.y * 128, c0 = blockIdx.x * 128;
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  const int c = c0 + tx * 8;
+  const bool wide_in = c + 7 < cols && (ldx & 7) == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0;
+  uint4 v[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int r = r0 + ty + 16 * i;
+    v[i] = make_uint4(0, 0, 0, 0);
+    if (r < rows) {
+      const __nv_bfloat16* p = x + size_t(r) * ldx + c;
+      if (wide_in) {
+        v[i] = *reinterpret_cast<const uint4*>(p);
+      } else {
+        uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (c + e < cols) w[e >> 1] |= uint32_t(*reinterpret_cast<const unsigned short*>(p + e)) << (16 * (e & 1));
+        v[i] = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+    }
+  }
+  float g[8];
+  if (SRC == NORMED) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) g[e] = c + e < cols ? __bfloat162float(gain[c + e]) : 0.f;
+  }
+  // the values of row i, as the norm kernel forms them
+  auto values = [&](int i, float (&f)[8]) {
+    const int r = r0 + ty + 16 * i;
+    const float s = SRC == NORMED && r < rows ? rstd[r] : 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 p = pair_at(v[i], j);
+      f[2 * j] = SRC == NORMED ? mul_full(mul_full(p.x, s), g[2 * j]) : p.x;
+      f[2 * j + 1] = SRC == NORMED ? mul_full(mul_full(p.y, s), g[2 * j + 1]) : p.y;
+    }
+  };
+  float row_max[8], col_max[8];
+  bool any_inf = false;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) col_max[e] = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    float f[8], m = 0.f;
+    values(i, f);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      m = max_abs(m, f[e]);
+      col_max[e] = max_abs(col_max[e], f[e]);
+    }
+    row_max[i] = m;
+    any_inf |= is_inf(m);
+  }
+  any_inf = __syncthreads_or(any_inf);
+  if (any_inf) {  // rare: once more, over the finite values
+#pragma unroll
+    for (int e = 0; e < 8; ++e) col_max[e] = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      float f[8], m = 0.f;
+      values(i, f);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        m = max_abs(m, nan_if_inf(f[e]));
+        col_max[e] = max_abs(col_max[e], nan_if_inf(f[e]));
+      }
+      row_max[i] = m;
+    }
+  }
+  float block_inv = 0.f;
+  uint32_t block_byte = 0;
+  if (SQUARE) {
+    float m = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max_abs(m, row_max[i]);
+    m = half_warp_max(m);
+    m = max_abs(m, __shfl_xor_sync(0xffffffffu, m, 16));
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < 8; ++w) m = max_abs(m, red[w]);
+    block_byte = scale_byte<E5M2>(m);
+    block_inv = inverse_of(block_byte);
+  } else if (out_t) {
+    float(*part)[128] = reinterpret_cast<float(*)[128]>(&tile[0][0]);  // [16][128]
+#pragma unroll
+    for (int e = 0; e < 8; ++e) part[ty][tx * 8 + e] = col_max[e];
+    __syncthreads();
+    if (threadIdx.x < 128) {
+      float m = 0.f;
+#pragma unroll
+      for (int k = 0; k < 16; ++k) m = max_abs(m, part[k][threadIdx.x]);
+      const uint32_t b = scale_byte<E5M2>(m);
+      col_byte[threadIdx.x] = uint8_t(b);
+      col_inv[threadIdx.x] = inverse_of(b);
+    }
+    __syncthreads();
+  }
+  const bool wide_out = c + 7 < cols && (ld_out & 7) == 0 && (reinterpret_cast<uintptr_t>(out) & 7) == 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int rl = ty + 16 * i, r = r0 + rl;
+    float f[8];
+    values(i, f);
+    if (any_inf) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[e] = nan_if_inf(f[e]);
+    }
+    uint32_t q[2] = {0, 0};
+    if (out || SQUARE) {
+      float inv = block_inv;
+      if (!SQUARE) {
+        const uint32_t b = scale_byte<E5M2>(half_warp_max(row_max[i]));
+        inv = inverse_of(b);
+        if (tx == 0) row_byte[rl] = uint8_t(b);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) q[j >> 1] |= to_bytes<E5M2>(f[2 * j], f[2 * j + 1], inv) << (16 * (j & 1));
+    }
+    if (out && r < rows) {
+      uint8_t* o = out + size_t(r) * ld_out + c;
+      if (wide_out) {
+        *reinterpret_cast<uint2*>(o) = make_uint2(q[0], q[1]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (c + e < cols) o[e] = uint8_t(q[e >> 2] >> (8 * (e & 3)));
+      }
+    }
+    if (out_t) {
+      if (!SQUARE) {
+        q[0] = q[1] = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t lo = to_bytes<E5M2>(f[2 * j], 0.f, col_inv[tx * 8 + 2 * j]), hi = to_bytes<E5M2>(f[2 * j + 1], 0.f, col_inv[tx * 8 + 2 * j + 1]);
+          q[j >> 1] |= ((lo & 0xffu) | (hi & 0xffu) << 8) << (16 * (j & 1));
+        }
+      }
+      // word w of row r at w ^ 4 * (r / 16 % 8): the 32 lanes of a transposed read hit 32 different banks
+      *reinterpret_cast<uint2*>(&tile[rl][(tx * 2) ^ (((rl >> 4) & 7) << 2)]) = make_uint2(q[0], q[1]);
+    }
+  }
+  __syncthreads();
+  if (threadIdx.x < 128) {
+    const int r = r0 + threadIdx.x;
+    if (out && r < rows) scales[blockIdx.x * ld_scales + r] = SQUARE ? uint8_t(block_byte) : row_byte[threadIdx.x];
+  } else if (out_t) {
+    const int k = threadIdx.x - 128;
+    if (c0 + k < cols) scales_t[blockIdx.y * ld_scales_t + c0 + k] = SQUARE ? uint8_t(block_byte) : col_byte[k];
+  }
+  if (!out_t) return;
+  const int lane = threadIdx.x & 31;
+  const int rg = lane & 7, cg = (threadIdx.x >> 5) * 4 + (lane >> 3);  // 16 source rows x 4 source columns per thread
+  uint32_t t[4][4];                                                     // [column][word of four rows]
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    uint32_t a[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) a[j] = tile[rg * 16 + i * 4 + j][cg ^ (rg << 2)];
+    const uint32_t p0 = __byte_perm(a[0], a[1], 0x5140), p1 = __byte_perm(a[0], a[1], 0x7362);
+    const uint32_t p2 = __byte_perm(a[2], a[3], 0x5140), p3 = __byte_perm(a[2], a[3], 0x7362);
+    t[0][i] = __byte_perm(p0, p2, 0x5410);
+    t[1][i] = __byte_perm(p0, p2, 0x7632);
+    t[2][i] = __byte_perm(p1, p3, 0x5410);
+    t[3][i] = __byte_perm(p1, p3, 0x7632);
+  }
+  const int r = r0 + rg * 16;
+  const bool wide_t = r + 15 < rows && (ld_t & 15) == 0 && (reinterpret_cast<uintptr_t>(out_t) & 15) == 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int oc = c0 + cg * 4 + j;
+    if (oc >= cols) continue;
+    uint8_t* o = out_t + size_t(oc) * ld_t + r;
+    if (wide_t) {
+      *reinterpret_cast<uint4*>(o) = make_uint4(t[j][0], t[j][1], t[j][2], t[j][3]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        if (r + e < rows) o[e] = uint8_t(t[j][e >> 2] >> (8 * (e & 3)));
+    }
+  }
+}
+
+__device__ __forceinline__ float row_sum(float v, float* red, int threads) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if (threads <= 32) return v;
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = 0.f;
+  for (int w = 0; w < threads / 32; ++w) v += red[w];
+  return v;
+}
+
+// One row per block of THREADS threads, VPT vectors of eight columns per thread held in registers; 16 neighbouring threads have a block
+// of 128 columns between them.  Vector c of a thread is c * THREADS + thread.
+template <int THREADS, int VPT>
+__global__ void __launch_bounds__(THREADS)
+kf_add_rmsnorm_blocks(const __nv_bfloat16* __restrict__ x, const __nv_bfloat16* __restrict__ residual, const __nv_bfloat16* __restrict__ gain,
+                      __nv_bfloat16* __restrict__ t_out, float* __restrict__ rstd_out, uint8_t* __restrict__ out, long long ld_out,
+                      uint8_t* __restrict__ scales, long long ld_scales, int D, float eps) {
+  __shared__ float red[32];
+  const size_t row = blockIdx.x;
+  const int nvec = D >> 3;
+  const __nv_bfloat16* xr = x + row * D;
+  uint4 v[VPT], rv[VPT];
+#pragma unroll
+  for (int c = 0; c < VPT; ++c) {
+    const int i = threadIdx.x + c * THREADS;
+    v[c] = rv[c] = make_uint4(0, 0, 0, 0);
+    if (i < nvec) {
+      v[c] = *reinterpret_cast<const uint4*>(xr + i * 8);
+      if (residual) rv[c] = *reinterpret_cast<const uint4*>(residual + row * D + i * 8);
+    }
+  }
+  float ss = 0.f;
+#pragma unroll
+  for (int c = 0; c < VPT; ++c) {
+    const int i = threadIdx.x + c * THREADS;
+    if (residual) {
+      uint32_t w[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 a = pair_at(v[c], j), b = pair_at(rv[c], j);
+        w[j] = pack_bf16(add_full(a.x, b.x), add_full(a.y, b.y));
+      }
+      v[c] = make_uint4(w[0], w[1], w[2], w[3]);
+      if (i < nvec) *reinterpret_cast<uint4*>(t_out + row * D + i * 8) = v[c];
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 a = pair_at(v[c], j);
+      ss += a.x * a.x;
+      ss += a.y * a.y;
+    }
+  }
+  const float r = rsqrtf(row_sum(ss, red, THREADS) / D + eps);
+  if (threadIdx.x == 0 && rstd_out) rstd_out[row] = r;
+#pragma unroll
+  for (int c = 0; c < VPT; ++c) {
+    const int i = threadIdx.x + c * THREADS;
+    const uint4 gv = i < nvec ? *reinterpret_cast<const uint4*>(gain + i * 8) : make_uint4(0, 0, 0, 0);
+    float f[8], m = 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 a = pair_at(v[c], j), g = pair_at(gv, j);
+      f[2 * j] = mul_full(mul_full(a.x, r), g.x);
+      f[2 * j + 1] = mul_full(mul_full(a.y, r), g.y);
+      m = max_abs(max_abs(m, f[2 * j]), f[2 * j + 1]);
+    }
+    m = half_warp_max(m);
+    if (is_inf(m)) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[e] = nan_if_inf(f[e]);
+    }
+    if (__any_sync(0xffffffffu, is_inf(m))) {  // rare: the largest finite value (a half without an infinity gets the same again)
+      m = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) m = max_abs(m, f[e]);
+      m = half_warp_max(m);
+    }
+    const uint32_t b = scale_byte<false>(m);
+    const float inv = inverse_of(b);
+    if (i < nvec) {
+      uint32_t q[2] = {0, 0};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) q[j >> 1] |= to_bytes<false>(f[2 * j], f[2 * j + 1], inv) << (16 * (j & 1));
+      *reinterpret_cast<uint2*>(out + row * ld_out + i * 8) = make_uint2(q[0], q[1]);
+      if ((i & 15) == 0) scales[(i >> 4) * ld_scales + row] = uint8_t(b);
+    }
+  }
+}
+
+// The values that the bytes stand for, in bf16 (exact where bf16 has them): eight per thread.
+template <bool E5M2>
+__global__ void __launch_bounds__(256)
+kf_blocks_values(const uint8_t* __restrict__ q, long long ld, const uint8_t* __restrict__ scales, long long ld_scales, int rows, int cols,
+                 __nv_bfloat16* __restrict__ out) {
+  const int vecs = (cols + 7) >> 3;
+  const long long i = blockIdx.x * 256LL + threadIdx.x;
+  if (i >= (long long)rows * vecs) return;
+  const int r = int(i / vecs), c = int(i - (long long)r * vecs) * 8;
+  // a factor of 2^-127 (byte 0) has no normal 32-bit number: half of the next one, which subnormal arithmetic keeps
+  const uint32_t b = scales[(c >> 7) * ld_scales + r];
+  const float f = b == 0 ? __uint_as_float(0x400000u) : b == 255 ? __uint_as_float(0x7fffffffu) : __uint_as_float(b << 23);
+  const uint8_t* p = q + r * ld + c;
+  __nv_bfloat16* o = out + (size_t)r * cols + c;
+  const bool whole = c + 7 < cols;
+  uint32_t w[2] = {0, 0};
+  if (whole && (ld & 7) == 0 && (reinterpret_cast<uintptr_t>(q) & 7) == 0) {
+    const uint2 u = *reinterpret_cast<const uint2*>(p);
+    w[0] = u.x;
+    w[1] = u.y;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (c + e < cols) w[e >> 2] |= uint32_t(p[e]) << (8 * (e & 3));
+  }
+  uint32_t packed[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w[j >> 1] >> (16 * (j & 1))), E5M2 ? __NV_E5M2 : __NV_E4M3);
+    packed[j] = pack_bf16(mul_full(__half2float(__half(__half_raw{h.x})), f), mul_full(__half2float(__half(__half_raw{h.y})), f));
+  }
+  if (whole && (cols & 7) == 0) {
+    *reinterpret_cast<uint4*>(o) = make_uint4(packed[0], packed[1], packed[2], packed[3]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (c + e < cols) reinterpret_cast<unsigned short*>(o)[e] = (unsigned short)(packed[e >> 1] >> (16 * (e & 1)));
+  }
+}
+
+static int launched() {
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? 0 : 400 + (int)e;
+}
+
+}  // namespace f8b
+}  // namespace kf
+
+extern "C" {
+
+// Casts bf16 x[rows][cols] (pitch ldx elements), or x * rstd[row] * gain[column] where rstd is given.  out / scales: row-major copy (pitch
+// ld_out) and its (ceil(cols / 128), rows) scale bytes (pitch ld_scales); out_t / scales_t: the transposed one, (cols, rows) and
+// (ceil(rows / 128), cols); either may be null.  square: blocks of 128 x 128.
+int kf_fp8_blocks_cast_bf16(const void* x, int rows, int cols, long long ldx, const void* rstd, const void* gain, int e5m2, int square,
+                            void* out, long long ld_out, void* scales, long long ld_scales, void* out_t, long long ld_t, void* scales_t,
+                            long long ld_scales_t, void* stream) {
+  using namespace kf::f8b;
+  if (rows <= 0 || cols <= 0 || rows > 128 * 65535 || (rstd == nullptr) != (gain == nullptr) || (!out && !out_t) || (rstd && (square || e5m2)))
+    return 5;
+  const dim3 grid((cols + 127) / 128, (rows + 127) / 128);
+  auto kern = rstd ? kf_cast_blocks<false, NORMED, false>
+              : square ? (e5m2 ? kf_cast_blocks<true, PLAIN, true> : kf_cast_blocks<false, PLAIN, true>)
+                       : (e5m2 ? kf_cast_blocks<true, PLAIN, false> : kf_cast_blocks<false, PLAIN, false>);
+  kern<<<grid, 256, 0, (cudaStream_t)stream>>>((const __nv_bfloat16*)x, rows, cols, ldx, (const float*)rstd, (const __nv_bfloat16*)gain,
+                                               (uint8_t*)out, ld_out, (uint8_t*)scales, ld_scales, (uint8_t*)out_t, ld_t,
+                                               (uint8_t*)scales_t, ld_scales_t);
+  return launched();
+}
+
+// t = bf16(x + residual) (x itself, and nothing is written, where residual is null), rstd, and RMSNorm(t) * gain in e4m3.  x, residual, t:
+// contiguous rows of D bf16 values on 16 bytes, D a multiple of 8, at most 32 768; pitch ld_out a multiple of 8.
+int kf_add_rmsnorm_fp8_blocks(const void* x, const void* residual, const void* gain, void* t, void* rstd, void* out, long long ld_out,
+                              void* scales, long long ld_scales, int rows, int D, float eps, void* stream) {
+  using namespace kf::f8b;
+  if (rows <= 0 || D <= 0 || (D & 7) || D > 32768 || (ld_out & 7) ||
+      ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(residual) | reinterpret_cast<uintptr_t>(gain) | reinterpret_cast<uintptr_t>(t)) & 15) ||
+      (reinterpret_cast<uintptr_t>(out) & 7) || (residual && !t))
+    return 5;
+  auto go = [&](auto kern, int threads) {
+    kern<<<rows, threads, 0, (cudaStream_t)stream>>>((const __nv_bfloat16*)x, (const __nv_bfloat16*)residual, (const __nv_bfloat16*)gain,
+                                                     (__nv_bfloat16*)t, (float*)rstd, (uint8_t*)out, ld_out, (uint8_t*)scales, ld_scales, D, eps);
+    return launched();
+  };
+  if (D <= 1024) return go(kf_add_rmsnorm_blocks<32, 4>, 32);
+  if (D <= 4096) return go(kf_add_rmsnorm_blocks<128, 4>, 128);
+  if (D <= 8192) return go(kf_add_rmsnorm_blocks<256, 4>, 256);
+  if (D <= 16384) return go(kf_add_rmsnorm_blocks<512, 4>, 512);
+  return go(kf_add_rmsnorm_blocks<1024, 4>, 1024);
+}
+
+// out[rows][cols] (contiguous bf16) = the values that q (pitch ld) and its scale bytes stand for.
+int kf_fp8_blocks_values_bf16(const void* q, long long ld, const void* scales, long long ld_scales, int rows, int cols, int e5m2, void* out,
+                              void* stream) {
+  using namespace kf::f8b;
+  if (rows <= 0 || cols <= 0 || (reinterpret_cast<uintptr_t>(out) & 15)) return 5;
+  const long long n = (long long)rows * ((cols + 7) / 8);
+  if ((n + 255) / 256 > 0x7fffffffLL) return 5;
+  auto kern = e5m2 ? kf_blocks_values<true> : kf_blocks_values<false>;
+  kern<<<unsigned((n + 255) / 256), 256, 0, (cudaStream_t)stream>>>((const uint8_t*)q, ld, (const uint8_t*)scales, ld_scales, rows, cols,
+                                                                    (__nv_bfloat16*)out);
+  return launched();
+}
+
+}  // extern "C"

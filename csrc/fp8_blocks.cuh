@@ -1,0 +1,54 @@
+// The 8-bit form with a scale for each block of 128: a byte per value (e4m3 or e5m2) and, for every row and 128 columns, a byte b that
+// stands for the factor 2^(b - 127).  Scale bytes are stored block-major, (ceil(cols / 128), rows), so that the 128 rows of a tile read
+// theirs as one line.
+//
+// Why powers of two: the tensor cores multiply such factors into the sum of a block themselves (tcgen05.mma kind::mxf8f6f4), a value's
+// bits do not depend on how its scale was rounded, and what a byte pair stands for is exact in bf16.
+#pragma once
+#include "common.cuh"
+#include <cuda_fp8.h>
+
+namespace kf {
+namespace f8b {
+
+constexpr int BLOCK = 128;
+
+// 32-bit arithmetic that keeps subnormal numbers, which the library's flags would flush
+__device__ __forceinline__ float mul_full(float a, float b) {
+  float r;
+  asm("mul.rn.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float add_full(float a, float b) {
+  float r;
+  asm("add.rn.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float max_abs(float m, float v) {  // NaN counts for nothing
+  float r;
+  asm("{\n\t.reg .f32 t;\n\tabs.f32 t, %2;\n\tmax.f32 %0, %1, t;\n\t}" : "=f"(r) : "f"(m), "f"(v));
+  return r;
+}
+
+// Scale byte of a block whose largest magnitude is a (finite): the least power of two, of at least 2^-126, that brings a to 448 or less
+// (e4m3; 57 344 for e5m2).  Both are 1.75 times a power of two, so the exponent and one comparison of a's bits decide it exactly.
+template <bool E5M2>
+__device__ __forceinline__ uint32_t scale_byte(float a) {
+  const uint32_t u = __float_as_uint(a);
+  const int e = int(u >> 23) - (E5M2 ? 15 : 8) + ((u & 0x7fffffu) > 0x600000u ? 1 : 0);
+  return u == 0 ? 127u : uint32_t(max(e, 1));
+}
+// the factor that divides by the scale: exact, and a normal number for every byte that scale_byte gives (1 .. 247)
+__device__ __forceinline__ float inverse_of(uint32_t byte) { return __uint_as_float((254u - byte) << 23); }
+
+__device__ __forceinline__ bool is_inf(float v) { return (__float_as_uint(v) & 0x7fffffffu) == 0x7f800000u; }
+__device__ __forceinline__ float nan_if_inf(float v) { return is_inf(v) ? __uint_as_float(0x7fffffffu) : v; }
+
+// two values, scaled, as two bytes: nearest, ties to even
+template <bool E5M2>
+__device__ __forceinline__ uint32_t to_bytes(float a, float b, float inv) {
+  return (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(mul_full(a, inv), mul_full(b, inv)), __NV_SATFINITE, E5M2 ? __NV_E5M2 : __NV_E4M3);
+}
+
+}  // namespace f8b
+}  // namespace kf

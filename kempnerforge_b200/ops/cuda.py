@@ -97,6 +97,10 @@ def _declare(L: ctypes.CDLL) -> None:
         "kf_fp8_scale_bf16": [vp, ll, i, vp, vp, vp],
         "kf_gemm_fp8_swiglu": [vp, vp, vp, vp, i, i, i, ll, ll, i, i, vp, vp, vp, vp, i, vp],
         "kf_gemm_fp8_swiglu_bwd": [vp, vp, vp, vp, i, i, i, ll, ll, i, vp, vp, vp, vp, i, vp],
+        "kf_fp8_blocks_cast_bf16": [vp, i, i, ll, vp, vp, i, i, vp, ll, vp, ll, vp, ll, vp, ll, vp],
+        "kf_add_rmsnorm_fp8_blocks": [vp, vp, vp, vp, vp, vp, ll, vp, ll, i, i, f, vp],
+        "kf_fp8_blocks_values_bf16": [vp, ll, vp, ll, i, i, i, vp, vp],
+        "kf_gemm_fp8_blocks": [vp, vp, vp, vp, vp, i, i, i, ll, ll, ll, ll, ll, i, i, i, i, vp],
         "kf_fp8_absmax_bf16": [vp, ll, vp, vp, vp],
         "kf_fp8_cast_bf16": [vp, i, i, ll, vp, i, vp, i, vp, ll, vp, ll, vp],
         "kf_lion": [vp, vp, vp, ll, i, f, f, f, f, vp],
@@ -876,6 +880,60 @@ def gemm_fp8_swiglu_bwd(a8: torch.Tensor, b8: torch.Tensor, sa: torch.Tensor, sb
                                         sa.data_ptr(), sb.data_ptr(), scratch.data_ptr() + 4, ctypes.byref(count), sm_count(), _stream()),
            "kf_gemm_fp8_swiglu_bwd")
     return dgu, PartialMax(scratch, count.value)
+
+
+# --------------------------------------------------------------------------- fp8 with a scale for each block of 128 (ops/fp8_blocks.py)
+def _block_buffers(rows: int, cols: int, device):
+    """(bytes (rows, cols) with rows on 128 bytes, scale bytes (ceil(cols / 128), rows) with rows on 16)."""
+    values = torch.empty((rows, -(-cols // 128) * 128), dtype=torch.uint8, device=device)
+    scales = torch.empty((-(-cols // 128), -(-rows // 16) * 16), dtype=torch.uint8, device=device)
+    return values if values.shape[1] == cols else values[:, :cols], scales if scales.shape[1] == rows else scales[:, :rows]
+
+
+def fp8_blocks_cast(x2: torch.Tensor, e5m2: bool, square: bool, want_row: bool, want_t: bool, rstd: torch.Tensor | None = None,
+                    gain: torch.Tensor | None = None):
+    """(bytes, scale bytes) of the bf16 matrix ``x2``, or of ``x2 * rstd[:, None] * gain``, and of its transpose; None in place of what is
+    not wanted."""
+    rows, cols = x2.shape
+    row = _block_buffers(rows, cols, x2.device) if want_row else (None, None)
+    t = _block_buffers(cols, rows, x2.device) if want_t else (None, None)
+    (q, s), (qt, st) = row, t
+    _check(lib().kf_fp8_blocks_cast_bf16(
+        x2.data_ptr(), rows, cols, x2.stride(0), _ptr(rstd), _ptr(gain), int(e5m2), int(square),
+        _ptr(q), q.stride(0) if want_row else 0, _ptr(s), s.stride(0) if want_row else 0,
+        _ptr(qt), qt.stride(0) if want_t else 0, _ptr(st), st.stride(0) if want_t else 0, _stream()), "kf_fp8_blocks_cast_bf16")
+    return row if want_row else None, t if want_t else None
+
+
+def add_rmsnorm_fp8_blocks(x2: torch.Tensor, r2: torch.Tensor | None, gain: torch.Tensor, eps: float):
+    """(x2 + r2 or None, rstd, (bytes, scale bytes) of its RMSNorm) of contiguous bf16 matrices."""
+    rows, d = x2.shape
+    t = torch.empty_like(x2) if r2 is not None else None
+    rstd = torch.empty(rows, dtype=torch.float32, device=x2.device)
+    q, s = _block_buffers(rows, d, x2.device)
+    _check(lib().kf_add_rmsnorm_fp8_blocks(x2.data_ptr(), _ptr(r2), gain.data_ptr(), _ptr(t), rstd.data_ptr(), q.data_ptr(), q.stride(0),
+                                           s.data_ptr(), s.stride(0), rows, d, eps, _stream()), "kf_add_rmsnorm_fp8_blocks")
+    return t, rstd, (q, s)
+
+
+def fp8_blocks_values(q: torch.Tensor, s: torch.Tensor, e5m2: bool) -> torch.Tensor:
+    """The bf16 values that bytes and scale bytes stand for."""
+    rows, cols = q.shape
+    out = torch.empty((rows, cols), dtype=torch.bfloat16, device=q.device)
+    _check(lib().kf_fp8_blocks_values_bf16(q.data_ptr(), q.stride(0), s.data_ptr(), s.stride(0), rows, cols, int(e5m2), out.data_ptr(),
+                                           _stream()), "kf_fp8_blocks_values_bf16")
+    return out
+
+
+def gemm_fp8_blocks(a: torch.Tensor, sa: torch.Tensor, b: torch.Tensor, sb: torch.Tensor, a_e5m2: bool, b_e5m2: bool, out: torch.Tensor,
+                    accumulate: bool = False) -> torch.Tensor:
+    """out (M, N) bf16 (+)= a (M, K) @ b (N, K)ᵀ of bytes with scale bytes for each block of 128."""
+    m, k = a.shape
+    n = b.shape[0]
+    _check(lib().kf_gemm_fp8_blocks(a.data_ptr(), sa.data_ptr(), b.data_ptr(), sb.data_ptr(), out.data_ptr(), m, n, k, a.stride(0),
+                                    sa.stride(0), b.stride(0), sb.stride(0), out.stride(0), int(a_e5m2), int(b_e5m2), int(accumulate),
+                                    sm_count(), _stream()), "kf_gemm_fp8_blocks")
+    return out
 
 
 # --------------------------------------------------------------------------- attention

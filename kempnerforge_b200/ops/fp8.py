@@ -105,6 +105,33 @@ class _Copies:
         return type(None), ()
 
 
+def weights_state(weights):
+    """What tells kept copies of the weights from those of other values: None while a graph is captured, where none are kept."""
+    state = [0]
+    if weights[0].is_cuda:
+        if torch._C._cuda_isCurrentStreamCapturing():
+            return None
+        state[0] = torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
+    for w in weights:
+        # its version, its address, the writes of kernels, and the version of the flat buffer that it is a view of (binding a
+        # parameter to the buffer leaves it a counter of its own, which a write of the buffer does not move)
+        own = w.__dict__.get
+        flat = own("_kf_flat")
+        state += w._version, w.data_ptr(), own("_kf_writes"), None if flat is None else flat.values_version
+    return state
+
+
+def copies_of(weights, state, row, scale=None) -> _Copies:
+    """Copies to be kept of the weights that ``state`` tells of."""
+    return _Copies(state, [StorageWeakRef(w.untyped_storage()) for w in weights], scale, row)
+
+
+def still_those_of(cached, state) -> bool:
+    """Whether ``cached`` are copies of the weights that ``state`` tells of."""
+    # where the storage that held an address is alive, no other one does
+    return type(cached) is _Copies and cached.state == state and not any([torch.UntypedStorage._expired(ref.cdata) for ref in cached.storages])
+
+
 def quantized_weight(weights, want_t: bool):
     """(scale, row-major fp8, transposed fp8 or None) of the weights stacked along the output dimension.
 
@@ -118,23 +145,14 @@ def quantized_weight(weights, want_t: bool):
     from kempnerforge_b200.ops import functional as F
 
     stacked = lambda: F._stack_weight_rows(weights).detach()  # noqa: E731
-    state = [0]
-    if weights[0].is_cuda:
-        if torch._C._cuda_isCurrentStreamCapturing():
-            return quantize(stacked(), want_t=want_t)
-        state[0] = torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
-    for w in weights:
-        # its version, its address, the writes of kernels, and the version of the flat buffer that it is a view of (binding a
-        # parameter to the buffer leaves it a counter of its own, which a write of the buffer does not move)
-        own = w.__dict__.get
-        flat = own("_kf_flat")
-        state += w._version, w.data_ptr(), own("_kf_writes"), None if flat is None else flat.values_version
+    state = weights_state(weights)
+    if state is None:
+        return quantize(stacked(), want_t=want_t)
     holder = weights[0]
     cached = getattr(holder, "_kf_fp8_cache", None)
-    # where the storage that held an address is alive, no other one does
-    if type(cached) is not _Copies or cached.state != state or any([torch.UntypedStorage._expired(ref.cdata) for ref in cached.storages]):
+    if not still_those_of(cached, state):
         sw, w8, _ = quantize(stacked())
-        cached = holder._kf_fp8_cache = _Copies(state, [StorageWeakRef(w.untyped_storage()) for w in weights], sw, w8)
+        cached = holder._kf_fp8_cache = copies_of(weights, state, w8, sw)
     if want_t and cached.transposed is None:
         cached.transposed = quantize(stacked(), want_row=False, want_t=True, scale=cached.scale)[2]
     return cached.scale, cached.row, cached.transposed

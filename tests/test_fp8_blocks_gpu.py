@@ -1,0 +1,366 @@
+"""The kernels of fp8 with a scale for each block of 128 against plain arithmetic in 64 bits."""
+
+import pytest
+import torch
+
+from kempnerforge_b200.ops import fp8_blocks as fb
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda"
+HALF_BF16 = 2.0**-8        # bf16 has 7 fraction bits: a step at 1 is 2^-7 (torch.finfo(torch.bfloat16).eps), a rounding is off by half of it
+
+
+def _gen(seed):
+    return torch.Generator(device=DEV).manual_seed(seed)
+
+
+def _spread(rows, cols, seed, dtype=torch.bfloat16):
+    """Rows of very different size, some columns large, zeros among them."""
+    g = _gen(seed)
+    x = torch.randn(rows, cols, device=DEV, generator=g) * torch.exp(4 * torch.randn(rows, 1, device=DEV, generator=g))
+    x[:, :: max(2, cols // 3)] *= 50
+    x[torch.rand(rows, cols, device=DEV, generator=g) < 0.05] = 0
+    if rows > 2:
+        x[rows // 2] = 0
+    return x.to(dtype)
+
+
+def _same(a, b):
+    return torch.equal(a.values, b.values) and torch.equal(a.scales, b.scales)
+
+
+def _plain(x2, e5m2, square):
+    return fb._cast_rows(x2.float(), e5m2, square)
+
+
+SHAPES = [(1, 1), (1, 128), (3, 129), (127, 40), (128, 128), (130, 1000), (257, 776), (1, 4096), (1000, 264)]
+
+
+@pytest.mark.parametrize("square", [False, True], ids=["rows", "squares"])
+@pytest.mark.parametrize("e5m2", [False, True], ids=["e4m3", "e5m2"])
+@pytest.mark.parametrize("rows, cols", SHAPES)
+def test_cast_gives_the_defined_bytes_both_ways(native_lib, rows, cols, e5m2, square):
+    x = _spread(rows, cols, rows + cols)
+    row, t = fb.quantize(x, e5m2, square, True, True)
+    assert _same(row, _plain(x, e5m2, square)) and _same(t, _plain(x.t().contiguous(), e5m2, square))
+    assert _same(fb.quantize(x, e5m2, square)[0], row) and _same(fb.quantize(x, e5m2, square, False, True)[1], t)
+    if square:
+        assert torch.equal(row.values, t.values.t())
+    exact = fb._values(row)
+    assert torch.equal(row.dequantize(), exact.bfloat16()) and torch.equal(row.dequantize().float(), exact)
+
+
+def test_cast_reads_pitched_rows_and_writes_nothing_else(native_lib):
+    frame = _spread(70, 400, 1)
+    for view in (frame[:, 8:285], frame[3:, 5:300], frame.t()[:, 1:60], frame[:1].expand(40, 400)):
+        row, t = fb.quantize(view, want_t=True)
+        assert _same(row, _plain(view, False, False)) and _same(t, _plain(view.t().contiguous(), False, False))
+
+
+@pytest.mark.parametrize("e5m2", [False, True], ids=["e4m3", "e5m2"])
+def test_cast_at_borders_of_scales_and_at_the_ends_of_the_range(native_lib, e5m2):
+    top = 57344.0 if e5m2 else 448.0
+    x = torch.zeros(12, 128, device=DEV, dtype=torch.bfloat16)
+    x[0, 5], x[1, 5], x[2, 5] = top, top * (1 + 2**-7), -top * 2.0**-20      # just fits; the next bf16 value does not
+    x[3], x[4, 0] = 2.0**-130, 2.0**-133                                     # subnormal numbers only
+    x[5, 0], x[5, 1] = 3.3e38, 1e-38
+    x[6, 3], x[6, 4] = float("inf"), 2.0
+    x[7, 9], x[7, 8] = float("nan"), -3.0
+    x[8] = float("-inf")
+    x[9] = -0.0
+    x[10, ::2], x[11, 127] = 1.0, 2.0**-140
+    row, t = fb.quantize(x, e5m2, want_t=True)
+    want, want_t = _plain(x, e5m2, False), _plain(x.t().contiguous(), e5m2, False)
+    for got, ref in ((row, want), (t, want_t)):
+        assert torch.equal(got.scales, ref.scales)
+        a, b = fb._values(got), fb._values(ref)
+        assert torch.equal(a.isnan(), b.isnan()) and torch.equal(a.nan_to_num(), b.nan_to_num())
+    assert row.scales[0, 0] == 127 and row.scales[0, 1] == 128 and row.scales[0, 9] == 127
+    assert fb._values(row)[6].isnan().sum() == 1 and fb._values(row)[6, 4] == 2 and fb._values(row)[7, 8] == -3
+
+
+def _mm_case(m, n, k, ea, eb, seed=0):
+    a = fb.quantize(_spread(m, k, seed + 1), ea)[0]
+    b = fb.quantize(_spread(n, k, seed + 2), eb)[0]
+    return a, b, fb._values(a).double(), fb._values(b).double()
+
+
+def _mm_close(got, want, mag, k):
+    """One rounding to bf16, and a sum in 32 bits of k terms (2^-23 of the terms' sum each, for hardware that truncates)."""
+    err = (got.double() - want).abs()
+    return bool((err <= HALF_BF16 * want.abs() * (1 + 2**-7) + (k + 2) * 2.0**-23 * mag + 1e-38).all())
+
+
+MM = [(1, 1, 1), (1, 4096, 512), (2, 24, 136), (16, 128, 128), (17, 1001, 777), (64, 256, 2048), (100, 136, 40), (128, 224, 640),
+      (129, 225, 129), (200, 512, 1536), (256, 448, 256), (257, 300, 1000), (333, 1001, 777), (513, 96, 384), (700, 1792, 520)]
+
+
+@pytest.mark.parametrize("ea, eb", [(False, False), (True, False), (False, True), (True, True)], ids=["e4m3", "e5m2xe4m3", "e4m3xe5m2", "e5m2"])
+@pytest.mark.parametrize("m, n, k", MM)
+def test_product(native_lib, m, n, k, ea, eb):
+    a, b, av, bv = _mm_case(m, n, k, ea, eb)
+    want, mag = av @ bv.t(), av.abs() @ bv.abs().t()
+    got = fb.mm(a, b)
+    assert got.is_contiguous() and got.shape == (m, n)
+    assert _mm_close(got, want, mag, k)
+    assert torch.equal(got, fb.mm(a, b))
+    assert native_lib.read_status() == 0
+
+
+@pytest.mark.parametrize("m, n, k", [(5, 200, 300), (64, 129, 256), (300, 520, 384), (300, 521, 384)])
+def test_product_adds_into_a_pitched_output_and_leaves_the_rest(native_lib, m, n, k):
+    a, b, av, bv = _mm_case(m, n, k, False, False, 7)
+    want, mag = av @ bv.t(), av.abs() @ bv.abs().t()
+    for first, pitch in ((0, -(-n // 8) * 8 + 8), (1, n + 3)):
+        frame = torch.full((m + 2, pitch), 7.0, dtype=torch.bfloat16, device=DEV)
+        out = frame[1 : m + 1, first : first + n]
+        assert fb.mm(a, b, out=out).data_ptr() == out.data_ptr()
+        assert torch.equal(out, fb.mm(a, b))
+        old = _spread(m, n, 3)
+        out.copy_(old)
+        fb.mm(a, b, out=out, accumulate=True)
+        assert _mm_close(out, want + old.double(), mag + old.double().abs(), k)
+        out.fill_(7.0)
+        assert bool((frame == 7.0).all())
+    assert native_lib.read_status() == 0
+
+
+def test_product_of_slices_and_of_scales_at_the_ends(native_lib):
+    a, b, av, bv = _mm_case(40, 72, 512, False, False, 9)
+    part = fb.mm(fb.BlockScaled(a.values[3:20, 128:384], a.scales[1:3, 3:20]), fb.BlockScaled(b.values[5:, 128:384], b.scales[1:3, 5:]))
+    want = av[3:20, 128:384] @ bv[5:, 128:384].t()
+    assert _mm_close(part, want, av[3:20, 128:384].abs() @ bv[5:, 128:384].abs().t(), 256)
+    one = torch.full((1, 128), 0x38, dtype=torch.uint8, device=DEV)          # 1.0 in e4m3
+    for sa, sb, value in ((127, 127, 128.0), (254, 1, 256.0), (1, 200, 0.0), (60, 194, 128.0), (100, 100, 128 * 2.0**-54)):
+        s = lambda v: torch.full((1, 1), v, dtype=torch.uint8, device=DEV)   # noqa: E731
+        got = fb.mm(fb.BlockScaled(one, s(sa)), fb.BlockScaled(one, s(sb)))
+        assert got.item() == (value if value else 128 * 2.0**(1 + 200 - 254)), (sa, sb, got)
+    nan = fb.mm(fb.BlockScaled(one, torch.full((1, 1), 255, dtype=torch.uint8, device=DEV)), fb.BlockScaled(one, torch.full((1, 1), 127, dtype=torch.uint8, device=DEV)))
+    assert nan.isnan().all()
+
+
+def test_what_is_not_finite_stays_in_its_row_and_column(native_lib):
+    x, w = _spread(40, 300, 3), _spread(50, 300, 4)
+    clean = fb.mm(fb.quantize(x)[0], fb.quantize(w)[0])
+    x2, w2 = x.clone(), w.clone()
+    x2[7, 200], w2[11, 5] = float("inf"), float("nan")
+    got = fb.mm(fb.quantize(x2)[0], fb.quantize(w2)[0])
+    bad = torch.zeros_like(got, dtype=torch.bool)
+    bad[7], bad[:, 11] = True, True
+    assert torch.equal(got.isnan(), bad)
+    assert torch.equal(got[~bad], clean[~bad])
+
+
+NORM = [(1, 8), (1, 4096), (3, 136), (5, 1024), (130, 1032), (64, 4104), (33, 8200), (2, 16392), (2, 32768), (1000, 776)]
+
+
+@pytest.mark.parametrize("with_residual", [False, True], ids=["alone", "residual"])
+@pytest.mark.parametrize("rows, d", NORM)
+def test_norm(native_lib, rows, d, with_residual):
+    x, gain = _spread(rows, d, d), (1 + 0.2 * torch.randn(d, device=DEV, generator=_gen(1))).bfloat16()
+    residual = _spread(rows, d, d + 1) if with_residual else None
+    t, rstd, h = fb.add_rmsnorm(x, residual, gain, 1e-5)
+    assert torch.equal(t, x if residual is None else (x.float() + residual.float()).bfloat16())
+    want = (t.double().square().mean(1) + 1e-5).rsqrt()
+    # a sum of d squares (2^-24 each, at most d of them one after another) under a square root, and an approximate one (2^-22)
+    assert bool(((rstd.double() - want).abs() <= want * (d * 2.0**-25 + 2.0**-21)).all())
+    assert _same(h, fb._cast_rows(t.float() * rstd[:, None] * gain.float(), False))
+    normed = fb._normed_t(t, rstd, gain)
+    assert _same(normed, fb._cast_rows((t.float() * rstd[:, None] * gain.float()).t().contiguous(), False))
+    again = fb.add_rmsnorm(x, residual, gain, 1e-5)
+    assert torch.equal(again[1], rstd) and _same(again[2], h)
+
+
+def test_norm_of_rows_with_infinities_and_zeros(native_lib):
+    x = torch.randn(6, 264, device=DEV, generator=_gen(0)).bfloat16()
+    x[1, 3], x[2, 200], x[3] = float("inf"), float("nan"), 0
+    gain = torch.ones(264, device=DEV, dtype=torch.bfloat16)
+    t, rstd, h = fb.add_rmsnorm(x, None, gain)
+    v = fb._values(h)
+    assert rstd[1] == 0 and rstd[2].isnan() and v[1].isnan().sum() == 1 and v[2].isnan().all() and not v[3].any()
+    assert v[[0, 3, 4, 5]].isfinite().all()
+    gain[5] = float("inf")                                       # of one column: NaN there, the rest of its block scaled as without it
+    got = fb.add_rmsnorm(x[4:], None, gain)[2]
+    assert _same(got, fb._cast_rows(x[4:].float() * fb.add_rmsnorm(x[4:], None, gain)[1][:, None] * gain.float(), False))
+    assert fb._values(got).isnan().sum() == 2
+
+
+def _layer(tokens, d, outs, seed=0, grads=True):
+    g = _gen(seed)
+    r = lambda *s, std=1.0: (torch.randn(*s, device=DEV, generator=g) * std).bfloat16()   # noqa: E731
+    x, residual, gain = r(*tokens, d), r(*tokens, d), 1 + r(d, std=0.1)
+    ws = [r(n, d, std=d**-0.5) for n in outs]
+    if grads:
+        for p in (x, residual, gain, *ws):
+            p.requires_grad_()
+    return x, residual, gain, ws, r(*tokens, d, std=0.1), r(*tokens, sum(outs), std=0.1)
+
+
+def _norm_grads64(dh, t, gain, dt, eps):
+    t, gain, dh = t.double(), gain.double(), dh.double()
+    r = (t.square().mean(1, keepdim=True) + eps).rsqrt()
+    g = dh * gain
+    mean = (g * t).mean(1, keepdim=True)
+    mag = (r * g).abs() + t.abs() * r**3 * (g * t).abs().mean(1, keepdim=True) + dt.double().abs()
+    return r * g - t * r**3 * mean + dt.double(), mag, (dh * t * r).sum(0), (dh * t * r).abs().sum(0)
+
+
+@pytest.mark.parametrize("with_residual", [False, True], ids=["alone", "residual"])
+@pytest.mark.parametrize("tokens, d, outs", [((1,), 64, (40,)), ((3, 77), 264, (128, 40, 40)), ((257,), 768, (776,)), ((2, 300), 1024, (512, 512))])
+def test_layer_and_its_gradients(native_lib, tokens, d, outs, with_residual):
+    x, residual, gain, ws, dt, dy = _layer(tokens, d, outs)
+    if not with_residual:
+        residual = None
+    t, y = fb.norm_linear(x, residual, gain, ws, 1e-5)
+    leaves = [p for p in (x, residual, gain, *ws) if p is not None]
+    got = dict(zip(["x"] + ["r"] * with_residual + ["gain"] + [f"w{i}" for i in range(len(ws))], torch.autograd.grad((t, y), leaves, (dt, dy))))
+    rows = x.numel() // d
+    t2, dy2, dt2 = t.detach().view(rows, d), dy.view(rows, -1), dt.view(rows, d)
+    h, w = fb.add_rmsnorm(x.detach().view(rows, d), None if residual is None else residual.detach().view(rows, d), gain.detach()), torch.cat([p.detach() for p in ws])
+    assert torch.equal(t2, h[0])
+    hv, wv, gv = fb._values(h[2]).double(), fb._values(_plain(w, False, True)).double(), fb._values(_plain(dy2, False, False)).double()
+    assert _mm_close(y.detach().view(rows, -1), hv @ wv.t(), hv.abs() @ wv.abs().t(), d)
+    # dh is rounded to bf16 once before the norm's gradient
+    dh, dh_mag = gv @ wv, gv.abs() @ wv.abs()
+    dh_err = HALF_BF16 * dh.abs() * (1 + 2**-7) + (w.shape[0] + 2) * 2.0**-23 * dh_mag
+    dx, mag, dgain, dgain_mag = _norm_grads64(dh, t2, gain.detach(), dt2, 1e-5)
+    _, err, _, gain_err = _norm_grads64(dh_err, t2, gain.detach().abs(), dt2 * 0, 1e-5)
+    # 32-bit sums of d terms and of `rows` terms
+    assert bool(((got["x"].view(rows, d).double() - dx).abs() <= err + HALF_BF16 * (dx.abs() + err) + d * 2.0**-22 * mag + 2.0**-20 * mag).all())
+    if with_residual:
+        assert torch.equal(got["r"], got["x"])
+    assert bool(((got["gain"].double() - dgain).abs() <= gain_err + HALF_BF16 * (dgain.abs() + gain_err) + (rows + 8) * 2.0**-21 * dgain_mag).all())
+    ht = fb._values(fb._cast_rows((t2.float() * h[1][:, None] * gain.detach().float()).t().contiguous(), False)).double()
+    gt = fb._values(_plain(dy2.t().contiguous(), False, False)).double()
+    dw = torch.cat([got[f"w{i}"] for i in range(len(ws))])
+    assert _mm_close(dw, gt @ ht.t(), gt.abs() @ ht.abs().t(), rows)
+    assert native_lib.read_status() == 0
+
+
+@pytest.mark.parametrize("lead", [(5,), (2, 150)])
+def test_linear_and_its_gradients(native_lib, lead):
+    d, outs = 200, (136, 48)
+    x, _, _, ws, _, dy = _layer(lead, d, outs, 3)
+    y = fb.linear(x, ws)
+    dx, *dws = torch.autograd.grad(y, (x, *ws), dy)
+    x2, dy2, w = x.detach().view(-1, d), dy.view(-1, sum(outs)), torch.cat([p.detach() for p in ws])
+    v = lambda m, sq=False: fb._values(_plain(m, False, sq)).double()   # noqa: E731
+    for got, a, b in ((y.detach().view(-1, sum(outs)), v(x2), v(w, True)), (dx.view(-1, d), v(dy2), v(w, True).t()),
+                      (torch.cat(dws), v(dy2.t().contiguous()), v(x2.t().contiguous()))):
+        assert _mm_close(got, a @ b.t(), a.abs() @ b.abs().t(), a.shape[1])
+
+
+def test_gradients_of_a_linear_agree_with_differences(native_lib):
+    """Small whole numbers are exact in 8 bits, so that all that differences of the loss are off by is the rounding of the outputs that the
+    step changes (a row or a column of them; up to 136 * 49, so not all are exact in bf16): half a step of each, times its |c|."""
+    g = _gen(5)
+    whole = lambda *s, top: torch.randint(-top, top + 1, s, device=DEV, generator=g).bfloat16()   # noqa: E731
+    x, w, c = whole(130, 136, top=7).requires_grad_(), whole(72, 136, top=7).requires_grad_(), whole(130, 72, top=2)
+    dx, dw = torch.autograd.grad(fb.linear(x, [w]), (x, w), c)
+    with torch.no_grad():
+        for leaf, grad, other, at in ((x, dx, w, (3, 5)), (x, dx, w, (129, 135)), (w, dw, x, (71, 130)), (w, dw, x, (0, 0))):
+            up, down = leaf.clone(), leaf.clone()
+            up[at] += 1
+            down[at] -= 1
+            ys = [fb.linear(*((v, [other]) if leaf is x else (other, [v]))).double() for v in (up, down)]
+            moved = (lambda v: v[at[0]]) if leaf is x else (lambda v: v[:, at[0]])
+            slope = ((ys[0] - ys[1]) * c.double()).sum().item() / 2
+            off = HALF_BF16 * sum((moved(v).abs() * (1 + 2**-7) * moved(c).double().abs()).sum().item() for v in ys) / 2
+            assert abs(slope - grad[at].item()) <= off + HALF_BF16 * abs(grad[at].item()), (slope, grad[at], off)
+
+
+def test_gradients_of_the_layer_agree_with_differences(native_lib):
+    """Along a gradient the loss changes by its length; what the casts of two calls add to a difference is random: off by at most 2^-4 of
+    a value, 0.03 of it in the mean square, which over the 512 x 256 outputs, each a sum, is 0.05 |c| |y| / sqrt(n) for one of them."""
+    x, residual, gain, ws, _, c = _layer((512,), 256, (256,), 8)
+    loss = lambda a, b, s: (fb.norm_linear(a, b, s, ws)[1].double() * c.double()).sum()   # noqa: E731
+    t, y = fb.norm_linear(x, residual, gain, ws)
+    grads = torch.autograd.grad(y, (x, residual, gain), c)
+    noise = 0.05 * c.double().norm() * y.detach().double().norm() / y.numel() ** 0.5
+    with torch.no_grad():
+        for i, grad in enumerate(grads):
+            leaves = [x, residual, gain]
+            step = 0.05 * leaves[i].double().norm() / grad.double().norm()
+            ends = []
+            for sign in (1, -1):
+                moved = list(leaves)
+                moved[i] = (leaves[i].double() + sign * step * grad.double()).bfloat16()
+                ends.append(loss(*moved))
+            slope = ((ends[0] - ends[1]) / 2).item()
+            want = (step * grad.double().square().sum()).item()
+            # five deviations, and 5 % for the curvature over a step of 5 %
+            assert abs(slope - want) <= 5 * noise.item() + 0.05 * want, (i, slope, want, noise)
+
+
+def test_half_of_the_graph(native_lib):
+    x, residual, gain, ws, dt, dy = _layer((40,), 264, (48,), 2)
+    t, y = fb.norm_linear(x, residual, gain, ws)
+    assert torch.equal(torch.autograd.grad(t, x, dt, retain_graph=True)[0], dt)          # the sum alone
+    both = torch.autograd.grad((t, y), (x, gain, ws[0]), (dt, dy), retain_graph=True)
+    only = torch.autograd.grad(y, (x, gain, ws[0]), dy, retain_graph=True)
+    assert torch.equal(both[1], only[1]) and torch.equal(both[2], only[2])
+    assert torch.equal(torch.autograd.grad(y, ws[0], dy)[0], both[2])
+    for need in range(4):                                                                # one leaf at a time
+        args = [p.detach().requires_grad_(i == need) for i, p in enumerate((x, residual, gain, ws[0]))]
+        t, y = fb.norm_linear(args[0], args[1], args[2], args[3:])
+        got = torch.autograd.grad(y, args[need], dy)[0]
+        assert torch.equal(got, [only[0], only[0], only[1], only[2]][need])
+    with torch.no_grad():
+        quiet = fb.norm_linear(x, residual, gain, ws)
+    assert torch.equal(quiet[1], y) and not quiet[1].requires_grad
+
+
+def test_saved_on_the_host_and_expanded_gradients(native_lib):
+    x, residual, gain, ws, _, dy = _layer((37,), 264, (40,), 4)
+    want = torch.autograd.grad(fb.linear(x, ws), (x, *ws), dy)
+    with torch.autograd.graph.save_on_cpu():
+        y = fb.linear(x, ws)
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(y, (x, *ws), dy), want))
+    y = fb.linear(x, ws)
+    ones = torch.autograd.grad(y.float().sum(), (x, *ws))
+    y = fb.linear(x, ws)
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(y, (x, *ws), torch.ones_like(y)), ones))
+
+
+def test_no_tokens(native_lib):
+    x, residual, gain, ws, _, _ = _layer((0,), 264, (40,), 4)
+    t, y = fb.norm_linear(x, residual, gain, ws)
+    grads = torch.autograd.grad((t.float().sum() + y.float().sum()), (x, residual, gain, *ws))
+    assert y.shape == (0, 40) and grads[0].shape == x.shape and not grads[2].any() and not grads[3].any()
+    y = fb.linear(x, ws)
+    assert y.shape == (0, 40) and not torch.autograd.grad(y.float().sum(), ws[0])[0].any()
+
+
+def test_captured_and_replayed_on_new_inputs_and_weights(native_lib):
+    x, residual, gain, ws, _, _ = _layer((50,), 264, (136,), 6, grads=False)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        fb.norm_linear(x, residual, gain, ws)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        t, y = fb.norm_linear(x, residual, gain, ws)
+    for seed in (11, 12):
+        new = _layer((50,), 264, (136,), seed, grads=False)
+        for old, value in zip((x, residual, gain, *ws), (*new[:3], *new[3])):
+            old.copy_(value)
+        graph.replay()
+        want = fb.norm_linear(*new[:3], new[3])
+        assert torch.equal(t, want[0]) and torch.equal(y, want[1])
+    assert native_lib.read_status() == 0
+
+
+def test_two_streams_at_once(native_lib):
+    cases = [_layer((300,), 512, (520,), s, grads=False) for s in (1, 2)]
+    want = [fb.norm_linear(*c[:3], c[3]) for c in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cases]
+    for _ in range(20):
+        got = []
+        for c, s in zip(cases, streams):
+            with torch.cuda.stream(s):
+                got.append(fb.norm_linear(*c[:3], c[3]))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for g, w in zip(got, want) for a, b in zip(g, w))
