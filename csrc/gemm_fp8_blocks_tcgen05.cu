@@ -7,9 +7,11 @@
 // read the same bytes.  The scales so cost no pass over the accumulators, which would have to be read back, scaled and added outside the
 // tensor cores once per block.
 //
-// Roles of a CTA: warp 0 loads the operands and the stage's scale bytes by TMA, warps 2 .. 5 move the bytes from shared to tensor memory
-// (row r of A's 128 to lane r % 32 of column r / 32, the same in each quarter of the lanes, as the instruction wants them; B's rows likewise),
-// warp 1 issues the instructions, warps 6 .. 9 store the tile before.
+// Roles of a CTA: warp 0 loads the operands by TMA and warp 10 the scale bytes, warps 2 .. 5 move the bytes from shared to tensor memory (row r of
+// A's 128 to lane r % 32 of column r / 32, the same in each quarter of the lanes, as the instruction wants them; B's rows likewise), warp 1
+// issues the instructions, warps 6 .. 9 store the tile before.  Scales travel four blocks at a time, as the four bytes of a word of tensor
+// memory of which an instruction names one: a hand-over for every block, with its wait for the stores and the arrival at the other CTA,
+// took 1600 clocks where the block's instructions take 450 (8192 x 28 672 from 4096: 1569 us, in fours XXX).
 #include "fp8_blocks.cuh"
 #include "gemm_epilogue.cuh"
 #include "pair_common.cuh"
@@ -25,21 +27,26 @@ constexpr int TILE_M = 256;   // rows per CTA pair
 constexpr int MAX_N = 224;    // columns of the widest tile: two accumulators and the scales share 512 columns of tensor memory
 constexpr int BK = BLOCK;     // bytes per row of a stage
 constexpr int UMMA_K = 32;
-constexpr int STAGES = 5;
+constexpr int STAGES = 7;
 constexpr int A_BYTES = CTA_M * BK;
 constexpr int B_BYTES = (MAX_N / 2) * BK;
-constexpr int SF_BYTES = 512;                       // scale bytes of a stage: 128 of A, up to 224 of B
 constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
+constexpr int GROUP = 4;                            // blocks whose scale bytes travel together
+constexpr int SLOTS = 3;                            // groups under way
+constexpr int SFA_BYTES = GROUP * CTA_M;            // [block][row]
+constexpr int SF_BYTES = SFA_BYTES + GROUP * 256;
 constexpr int SF_COLS = 12;                         // their columns of tensor memory: 4 and 8
 constexpr int SF_BASE = 2 * MAX_N;
 constexpr int TMEM_COLS = 512;
-static_assert(SF_BASE + STAGES * SF_COLS <= TMEM_COLS && STAGE_BYTES % 1024 == 0, "tensor memory; swizzled tiles start on 1024 bytes");
+static_assert(SF_BASE + SLOTS * SF_COLS <= TMEM_COLS && STAGE_BYTES % 1024 == 0, "tensor memory; swizzled tiles start on 1024 bytes");
 constexpr int GROUP_M = 8;
 constexpr int BOX_BYTES = 2048;  // one staged 32 x 32 box per epilogue warp
-constexpr int THREADS = 320;
-constexpr size_t SMEM = size_t(STAGES) * (STAGE_BYTES + SF_BYTES) + 4 * BOX_BYTES + 1024 + 256;
+constexpr int THREADS = 352;
+constexpr size_t SMEM = size_t(STAGES) * STAGE_BYTES + SLOTS * SF_BYTES + 4 * BOX_BYTES + 1024 + 256;
 
-// Instruction descriptor for kind::mxf8f6f4: formats 0 = e4m3, 1 = e5m2, both K-major, scales as exponent bytes, byte 0 of each word.
+// Instruction descriptor for kind::mxf8f6f4: formats 0 = e4m3, 1 = e5m2, both K-major, scales as exponent bytes, byte 0 of each word; plus
+// b of them, byte b.
+constexpr uint32_t IDESC_NEXT_BYTE = (1u << 4) | (1u << 29);
 __host__ __device__ constexpr uint32_t idesc_blocks(int m, int n, int a_fmt, int b_fmt) {
   return (uint32_t(a_fmt) << 7) | (uint32_t(b_fmt) << 10) | (uint32_t(n >> 3) << 17) | (1u << 23) | (uint32_t(m >> 4) << 24);
 }
@@ -51,6 +58,38 @@ __device__ __forceinline__ void mma_pair_blocks(uint32_t d_tmem, uint64_t adesc,
       "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d_tmem),
       "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
       : "memory");
+}
+// Arrival and wait that hand over tensor memory only: what orders tcgen05.st before another CTA's tcgen05.mma is tcgen05.wait::st, the
+// tcgen05 fences on both sides and this signal.  With release and acquire at cluster scope in their stead a hand-over of four blocks'
+// scales took 2000 ns, whatever the width of the tile (74 x 256 rows, 128 to 224 columns, K 4096, us: 132 to 137, so 109 to 116).
+__device__ __forceinline__ void arrive_relaxed_on_leader(uint32_t bar) {
+  asm volatile(
+      "{\n\t.reg .b32 ra;\n\t"
+      "mapa.shared::cluster.u32 ra, %0, 0;\n\t"
+      "mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [ra];\n\t}" ::"r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ bool mbar_wait_relaxed(uint32_t bar, uint32_t parity, int* status, int code) {
+  const long long t0 = clock64();
+  uint32_t spins = 0;
+  while (true) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred P;\n\t"
+        "mbarrier.try_wait.parity.relaxed.cluster.shared::cta.b64 P, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, P;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    if (ok) return true;
+    if ((++spins & 0x3ff) == 0) {
+      if (*reinterpret_cast<volatile int*>(status) != 0) return false;
+      if (clock64() - t0 > KF_WAIT_CYCLES) {
+        atomicCAS(status, 0, code);
+        return false;
+      }
+    }
+  }
 }
 __device__ __forceinline__ void tmem_st_x4(uint32_t taddr, const uint32_t (&r)[4]) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]) : "memory");
@@ -64,6 +103,11 @@ __device__ __forceinline__ uint32_t lds_u8(uint32_t addr) {
   uint32_t v;
   asm volatile("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
   return v;
+}
+// bytes at addr, addr + step, .. as a word
+__device__ __forceinline__ uint32_t four_bytes(uint32_t addr, uint32_t step) {
+  const uint32_t a = lds_u8(addr), b = lds_u8(addr + step), c = lds_u8(addr + 2 * step), d = lds_u8(addr + 3 * step);
+  return a | b << 8 | c << 16 | d << 24;
 }
 __device__ __forceinline__ unsigned short lds_u16(uint32_t addr) {
   unsigned short v;
@@ -90,17 +134,19 @@ kf_gemm_fp8_blocks_2cta(const __grid_constant__ CUtensorMap map_a, const __grid_
   extern __shared__ uint8_t smem_raw[];
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   const uint32_t sf_smem = smem_base + STAGES * STAGE_BYTES;
-  const uint32_t box_smem = sf_smem + STAGES * SF_BYTES;
+  const uint32_t box_smem = sf_smem + SLOTS * SF_BYTES;
   const uint32_t bar_base = box_smem + 4 * BOX_BYTES;
   auto full_bar = [&](int s) { return bar_base + 8u * s; };                  // the leader's: both CTAs' operands
   auto empty_bar = [&](int s) { return bar_base + 8u * (STAGES + s); };
-  auto sf_full_bar = [&](int s) { return bar_base + 8u * (2 * STAGES + s); };  // this CTA's scale bytes are in shared memory
-  auto sf_ready_bar = [&](int s) { return bar_base + 8u * (3 * STAGES + s); }; // the leader's: both CTAs' are in tensor memory
-  auto tfull_bar = [&](int a) { return bar_base + 8u * (4 * STAGES + a); };
-  auto tempty_bar = [&](int a) { return bar_base + 8u * (4 * STAGES + 2 + a); };
-  const uint32_t drain_bar = bar_base + 8u * (4 * STAGES + 4);
-  const uint32_t tmem_slot = bar_base + 8u * (4 * STAGES + 5);
-  static_assert(8 * (4 * STAGES + 5) + 4 <= 256, "barriers");
+  auto tfull_bar = [&](int a) { return bar_base + 8u * (2 * STAGES + a); };
+  auto tempty_bar = [&](int a) { return bar_base + 8u * (2 * STAGES + 2 + a); };
+  const uint32_t sf_bars = bar_base + 8u * (2 * STAGES + 4);
+  auto sf_full_bar = [&](int g) { return sf_bars + 8u * g; };                 // this CTA's scale bytes are in shared memory
+  auto sf_ready_bar = [&](int g) { return sf_bars + 8u * (SLOTS + g); };      // the leader's: both CTAs' are in tensor memory
+  auto sf_empty_bar = [&](int g) { return sf_bars + 8u * (2 * SLOTS + g); };  // shared bytes and columns may be overwritten
+  const uint32_t drain_bar = sf_bars + 8u * (3 * SLOTS);
+  const uint32_t tmem_slot = drain_bar + 8u;
+  static_assert(8 * (2 * STAGES + 4 + 3 * SLOTS + 1) + 4 <= 256, "barriers");
   volatile uint32_t* tmem_slot_ptr = reinterpret_cast<volatile uint32_t*>(smem_raw + (tmem_slot - smem_u32(smem_raw)));
 
   const int warp = warp_index();
@@ -112,14 +158,17 @@ kf_gemm_fp8_blocks_2cta(const __grid_constant__ CUtensorMap map_a, const __grid_
   const int m_blocks = (M + TILE_M - 1) / TILE_M;
   const int n_blocks = (N + tile_n - 1) / tile_n;
   const int num_tiles = m_blocks * n_blocks;
-  const int k_blocks = (K + BK - 1) / BK;
+  const int k_blocks = (K + BK - 1) / BK, groups = (k_blocks + GROUP - 1) / GROUP;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(full_bar(s), 1);
       mbar_init(empty_bar(s), 1);
-      mbar_init(sf_full_bar(s), 1);
-      mbar_init(sf_ready_bar(s), 8);  // four warps of both CTAs
+    }
+    for (int g = 0; g < SLOTS; ++g) {
+      mbar_init(sf_full_bar(g), 1);
+      mbar_init(sf_ready_bar(g), 8);  // four warps of both CTAs
+      mbar_init(sf_empty_bar(g), 5);  // the instructions, and four warps that have read the shared bytes
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(tfull_bar(a), 1);
@@ -150,33 +199,49 @@ kf_gemm_fp8_blocks_2cta(const __grid_constant__ CUtensorMap map_a, const __grid_
       for (int t = pair; t < num_tiles && ok; t += num_pairs) {
         int tm, tn;
         tilemath::raster(t, m_blocks, n_blocks, GROUP_M, tm, tn);
-        const int m0 = tm * TILE_M + int(rank) * CTA_M, n0 = tn * tile_n;
+        const int m0 = tm * TILE_M + int(rank) * CTA_M, n0 = tn * tile_n + int(rank) * half_n;
         for (int kb = 0; kb < k_blocks; ++kb, ++it) {
           const int s = it % STAGES;
           const uint32_t ph = (it / STAGES) & 1;
           if (!mbar_wait(empty_bar(s), ph ^ 1, status, KF_ERR_WAIT_EMPTY)) { ok = false; break; }
-          const uint32_t a_dst = smem_base + s * STAGE_BYTES, sf_dst = sf_smem + s * SF_BYTES;
+          const uint32_t a_dst = smem_base + s * STAGE_BYTES;
           const uint32_t lead_full = full_bar(s) & PEER_BIT_MASK;
-          mbar_expect_tx(sf_full_bar(s), CTA_M + tile_n);
-          tma_load_2d(sf_dst, &map_sa, sf_full_bar(s), m0, kb);
-          tma_load_2d(sf_dst + CTA_M, &map_sb, sf_full_bar(s), n0, kb);
           if (leader) mbar_expect_tx(full_bar(s), 2 * (A_BYTES + half_n * BK));
           tma_load_2d_pair(a_dst, &map_a, lead_full, kb * BK, m0);
-          tma_load_2d_pair(a_dst + A_BYTES, &map_b, lead_full, kb * BK, n0 + int(rank) * half_n);
+          tma_load_2d_pair(a_dst + A_BYTES, &map_b, lead_full, kb * BK, n0);
         }
       }
       // copies into this CTA's shared memory are complete once their stages were consumed or, on the error path, once
-      // the leader's full barrier flipped and the scales have landed
-      for (int j = max(0, it - STAGES); j < it; ++j) {
-        mbar_wait(sf_full_bar(j % STAGES), (j / STAGES) & 1, status, KF_ERR_WAIT_DRAIN);
-        if (leader) mbar_wait(full_bar(j % STAGES), (j / STAGES) & 1, status, KF_ERR_WAIT_DRAIN);
+      // the leader's full barrier flipped
+      if (leader)
+        for (int j = max(0, it - STAGES); j < it; ++j)
+          mbar_wait(full_bar(j % STAGES), (j / STAGES) & 1, status, KF_ERR_WAIT_DRAIN);
+    }
+  } else if (warp == 10) {
+    // ------------------------------------------------------------ TMA producer of the scale bytes, ahead of the operands' ring
+    if (elect_one()) {
+      int gi = 0;
+      bool ok = true;
+      for (int t = pair; t < num_tiles && ok; t += num_pairs) {
+        int tm, tn;
+        tilemath::raster(t, m_blocks, n_blocks, GROUP_M, tm, tn);
+        const int m0 = tm * TILE_M + int(rank) * CTA_M, n0 = tn * tile_n;
+        for (int i = 0; i < groups; ++i, ++gi) {
+          const int g = gi % SLOTS;
+          if (!mbar_wait(sf_empty_bar(g), ((gi / SLOTS) & 1) ^ 1, status, KF_ERR_WAIT_EMPTY)) { ok = false; break; }
+          mbar_expect_tx(sf_full_bar(g), GROUP * (CTA_M + tile_n));
+          tma_load_2d(sf_smem + g * SF_BYTES, &map_sa, sf_full_bar(g), m0, i * GROUP);
+          tma_load_2d(sf_smem + g * SF_BYTES + SFA_BYTES, &map_sb, sf_full_bar(g), n0, i * GROUP);
+        }
       }
+      for (int j = max(0, gi - SLOTS); j < gi; ++j)
+        mbar_wait(sf_full_bar(j % SLOTS), (j / SLOTS) & 1, status, KF_ERR_WAIT_DRAIN);
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer (leader CTA only)
     if (leader && elect_one()) {
       const uint32_t idesc = idesc_blocks(TILE_M, tile_n, a_fmt, b_fmt);
-      int it = 0, tile_iter = 0;
+      int it = 0, gi = 0, tile_iter = 0;
       bool ok = true;
       for (int t = pair; t < num_tiles && ok; t += num_pairs, ++tile_iter) {
         const int acc = tile_iter & 1;
@@ -187,19 +252,22 @@ kf_gemm_fp8_blocks_2cta(const __grid_constant__ CUtensorMap map_a, const __grid_
         for (int kb = 0; kb < k_blocks; ++kb, ++it) {
           const int s = it % STAGES;
           const uint32_t ph = (it / STAGES) & 1;
-          if (!mbar_wait_cluster(sf_ready_bar(s), ph, status, KF_ERR_WAIT_FULL) || !mbar_wait(full_bar(s), ph, status, KF_ERR_WAIT_FULL)) {
-            ok = false;
-            break;
-          }
+          const int b = kb % GROUP, g = gi % SLOTS;
+          if (b == 0 && !mbar_wait_relaxed(sf_ready_bar(g), (gi / SLOTS) & 1, status, KF_ERR_WAIT_FULL)) { ok = false; break; }
+          if (!mbar_wait(full_bar(s), ph, status, KF_ERR_WAIT_FULL)) { ok = false; break; }
           tc_fence_after();
           const uint32_t a_src = smem_base + s * STAGE_BYTES;
           const uint32_t b_src = a_src + A_BYTES;
-          const uint32_t sfa = tmem_base + SF_BASE + s * SF_COLS, sfb = sfa + 4;
+          const uint32_t sfa = tmem_base + SF_BASE + g * SF_COLS, sfb = sfa + 4;
 #pragma unroll
           for (int k = 0; k < BK / UMMA_K; ++k)
-            mma_pair_blocks(d_tmem, umma_desc_sw128(a_src + k * UMMA_K, 16, 1024), umma_desc_sw128(b_src + k * UMMA_K, 16, 1024), idesc,
-                            sfa, sfb, (kb | k) != 0);
+            mma_pair_blocks(d_tmem, umma_desc_sw128(a_src + k * UMMA_K, 16, 1024), umma_desc_sw128(b_src + k * UMMA_K, 16, 1024),
+                            idesc + b * IDESC_NEXT_BYTE, sfa, sfb, (kb | k) != 0);
           commit_pair(empty_bar(s));
+          if (b == GROUP - 1 || kb == k_blocks - 1) {
+            commit_pair(sf_empty_bar(g));
+            ++gi;
+          }
         }
         if (ok) commit_pair(tfull_bar(acc));
       }
@@ -210,27 +278,30 @@ kf_gemm_fp8_blocks_2cta(const __grid_constant__ CUtensorMap map_a, const __grid_
     }
   } else if (warp < 6) {
     // ------------------------------------------------------------ scale bytes: shared -> tensor memory
-    // A stage's bytes land only after the instructions that read the columns of its slot before have retired (empty_bar).
+    // A slot's bytes land only after the instructions that read its columns before have retired (sf_empty_bar).
     const uint32_t t_lane = tmem_base + (uint32_t((warp & 3) * 32) << 16) + SF_BASE;
-    int it = 0;
+    int gi = 0;
     bool ok = true;
     for (int t = pair; t < num_tiles && ok; t += num_pairs) {
-      for (int kb = 0; kb < k_blocks; ++kb, ++it) {
-        const int s = it % STAGES;
-        if (!mbar_wait(sf_full_bar(s), (it / STAGES) & 1, status, KF_ERR_WAIT_FULL)) { ok = false; break; }
+      for (int i = 0; i < groups; ++i, ++gi) {
+        const int g = gi % SLOTS;
+        if (!mbar_wait(sf_full_bar(g), (gi / SLOTS) & 1, status, KF_ERR_WAIT_FULL)) { ok = false; break; }
         tc_fence_after();
-        const uint32_t src = sf_smem + s * SF_BYTES + lane;
+        const uint32_t a_src = sf_smem + g * SF_BYTES + lane, b_src = a_src + SFA_BYTES;
         uint32_t a[4], b[8];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) a[c] = lds_u8(src + c * 32);
+        for (int c = 0; c < 4; ++c) a[c] = four_bytes(a_src + c * 32, CTA_M);
 #pragma unroll
-        for (int c = 0; c < 8; ++c) b[c] = c * 32 < tile_n ? lds_u8(src + CTA_M + c * 32) : 0u;
-        tmem_st_x4(t_lane + s * SF_COLS, a);
-        tmem_st_x8(t_lane + s * SF_COLS + 4, b);
+        for (int c = 0; c < 8; ++c) b[c] = c * 32 < tile_n ? four_bytes(b_src + c * 32, tile_n) : 0u;
+        tmem_st_x4(t_lane + g * SF_COLS, a);
+        tmem_st_x8(t_lane + g * SF_COLS + 4, b);
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) arrive_release_on_cta(sf_ready_bar(s), 0);
+        if (lane == 0) {
+          mbar_arrive(sf_empty_bar(g));
+          arrive_relaxed_on_leader(sf_ready_bar(g));
+        }
       }
     }
   } else {
@@ -343,8 +414,8 @@ int kf_gemm_fp8_blocks(const void* A, const void* sa, const void* B, const void*
   int rc;
   if ((rc = make_map_u8(&ma, A, M, K, lda, BK, CTA_M, true))) return 100 + rc;
   if ((rc = make_map_u8(&mb, B, N, K, ldb, BK, tile_n / 2, true))) return 200 + rc;
-  if ((rc = make_map_u8(&msa, sa, k_blocks, M, ldsa, CTA_M, 1, false))) return 100 + rc;
-  if ((rc = make_map_u8(&msb, sb, k_blocks, N, ldsb, tile_n, 1, false))) return 200 + rc;
+  if ((rc = make_map_u8(&msa, sa, k_blocks, M, ldsa, CTA_M, GROUP, false))) return 100 + rc;
+  if ((rc = make_map_u8(&msb, sb, k_blocks, N, ldsb, tile_n, GROUP, false))) return 200 + rc;
   static bool attr_set[64] = {};
   int dev = 0;
   cudaGetDevice(&dev);
