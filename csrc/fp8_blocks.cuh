@@ -50,5 +50,35 @@ __device__ __forceinline__ uint32_t to_bytes(float a, float b, float inv) {
   return (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(mul_full(a, inv), mul_full(b, inv)), __NV_SATFINITE, E5M2 ? __NV_E5M2 : __NV_E4M3);
 }
 
+// ------------------------------------------------------------------ tcgen05
+// Instruction descriptor for kind::mxf8f6f4: formats 0 = e4m3, 1 = e5m2, both K-major, scales as exponent bytes, byte 0 of each word; plus
+// b of them, byte b.
+constexpr uint32_t IDESC_NEXT_BYTE = (1u << 4) | (1u << 29);
+__host__ __device__ constexpr uint32_t idesc_blocks(int m, int n, int a_fmt, int b_fmt) {
+  return (uint32_t(a_fmt) << 7) | (uint32_t(b_fmt) << 10) | (uint32_t(n >> 3) << 17) | (1u << 23) | (uint32_t(m >> 4) << 24);
+}
+__device__ __forceinline__ void tmem_st_x4(uint32_t taddr, const uint32_t (&r)[4]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]) : "memory");
+}
+__device__ __forceinline__ void tmem_st_x8(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]),
+               "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+// rows x cols bytes, pitch ld -> tensor map with (box_cols x box_rows) boxes
+inline int make_map_u8(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols, uint64_t ld, uint32_t box_cols, uint32_t box_rows,
+                       bool swizzled) {
+  EncodeTiledFn fn = encode_tiled_fn();
+  if (!fn) return -1;
+  cuuint64_t dims[2] = {cols, rows};
+  cuuint64_t strides[1] = {ld};
+  cuuint32_t box[2] = {box_cols, box_rows};
+  cuuint32_t estr[2] = {1, 1};
+  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  swizzled ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? 0 : (int)r;
+}
+
 }  // namespace f8b
 }  // namespace kf

@@ -44,12 +44,6 @@ constexpr int BOX_BYTES = 2048;  // one staged 32 x 32 box per epilogue warp
 constexpr int THREADS = 352;
 constexpr size_t SMEM = size_t(STAGES) * STAGE_BYTES + SLOTS * SF_BYTES + 4 * BOX_BYTES + 1024 + 256;
 
-// Instruction descriptor for kind::mxf8f6f4: formats 0 = e4m3, 1 = e5m2, both K-major, scales as exponent bytes, byte 0 of each word; plus
-// b of them, byte b.
-constexpr uint32_t IDESC_NEXT_BYTE = (1u << 4) | (1u << 29);
-__host__ __device__ constexpr uint32_t idesc_blocks(int m, int n, int a_fmt, int b_fmt) {
-  return (uint32_t(a_fmt) << 7) | (uint32_t(b_fmt) << 10) | (uint32_t(n >> 3) << 17) | (1u << 23) | (uint32_t(m >> 4) << 24);
-}
 __device__ __forceinline__ void mma_pair_blocks(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t sfa, uint32_t sfb,
                                                 uint32_t accumulate) {
   asm volatile(
@@ -91,22 +85,9 @@ __device__ __forceinline__ bool mbar_wait_relaxed(uint32_t bar, uint32_t parity,
     }
   }
 }
-__device__ __forceinline__ void tmem_st_x4(uint32_t taddr, const uint32_t (&r)[4]) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]) : "memory");
-}
-__device__ __forceinline__ void tmem_st_x8(uint32_t taddr, const uint32_t (&r)[8]) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]),
-               "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
-               : "memory");
-}
-__device__ __forceinline__ uint32_t lds_u8(uint32_t addr) {
-  uint32_t v;
-  asm volatile("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
-  return v;
-}
-// bytes at addr, addr + step, .. as a word
-__device__ __forceinline__ uint32_t four_bytes(uint32_t addr, uint32_t step) {
-  const uint32_t a = lds_u8(addr), b = lds_u8(addr + step), c = lds_u8(addr + 2 * step), d = lds_u8(addr + 3 * step);
+// bytes at p, p + step, .. as a word
+__device__ __forceinline__ uint32_t four_bytes(const uint8_t* p, int step) {
+  const uint32_t a = p[0], b = p[step], c = p[2 * step], d = p[3 * step];
   return a | b << 8 | c << 16 | d << 24;
 }
 __device__ __forceinline__ unsigned short lds_u16(uint32_t addr) {
@@ -287,7 +268,8 @@ kf_gemm_fp8_blocks_2cta(const __grid_constant__ CUtensorMap map_a, const __grid_
         const int g = gi % SLOTS;
         if (!mbar_wait(sf_full_bar(g), (gi / SLOTS) & 1, status, KF_ERR_WAIT_FULL)) { ok = false; break; }
         tc_fence_after();
-        const uint32_t a_src = sf_smem + g * SF_BYTES + lane, b_src = a_src + SFA_BYTES;
+        const uint8_t* a_src = smem_raw + (sf_smem - smem_u32(smem_raw)) + g * SF_BYTES + lane;
+        const uint8_t* b_src = a_src + SFA_BYTES;
         uint32_t a[4], b[8];
 #pragma unroll
         for (int c = 0; c < 4; ++c) a[c] = four_bytes(a_src + c * 32, CTA_M);
@@ -359,21 +341,6 @@ kf_gemm_fp8_blocks_2cta(const __grid_constant__ CUtensorMap map_a, const __grid_
   }
 }
 
-// rows x cols bytes, pitch ld -> tensor map with (box_cols x box_rows) boxes
-static int make_map_u8(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols, uint64_t ld, uint32_t box_cols, uint32_t box_rows,
-                       bool swizzled) {
-  EncodeTiledFn fn = encode_tiled_fn();
-  if (!fn) return -1;
-  cuuint64_t dims[2] = {cols, rows};
-  cuuint64_t strides[1] = {ld};
-  cuuint32_t box[2] = {box_cols, box_rows};
-  cuuint32_t estr[2] = {1, 1};
-  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                  swizzled ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  return r == CUDA_SUCCESS ? 0 : (int)r;
-}
-
 // Tile width of a launch: rounds of tiles over the pairs times the columns of a tile, narrow ones at a surcharge for the operand bytes
 // that they need per clock (pair_tile_width has the figures).
 static int tile_width(int M, int N, int pairs) {
@@ -393,6 +360,11 @@ static int tile_width(int M, int N, int pairs) {
   return best;
 }
 
+// gemm_fp8_blocks_skinny.cu
+int gemm_blocks_skinny(const void* A, const void* sa, const void* B, const void* sb, void* C, int M, int N, int K, long long lda,
+                       long long ldsa, long long ldb, long long ldsb, long long ldc, int a_fmt, int b_fmt, int accumulate, int num_sms,
+                       int* status, void* stream);
+
 }  // namespace f8b
 }  // namespace kf
 
@@ -407,6 +379,9 @@ int kf_gemm_fp8_blocks(const void* A, const void* sa, const void* B, const void*
                        void* stream) {
   using namespace kf::f8b;
   if (((lda | ldb | ldsa | ldsb) & 15) || M <= 0 || N <= 0 || K <= 0 || num_sms < 2) return 5;
+  int* status = reinterpret_cast<int*>(kf_status_device_ptr());
+  if (M <= 256)
+    return gemm_blocks_skinny(A, sa, B, sb, C, M, N, K, lda, ldsa, ldb, ldsb, ldc, a_fmt, b_fmt, accumulate, num_sms, status, stream);
   int pairs = num_sms / 2;
   const int tile_n = tile_width(M, N, pairs);
   const int k_blocks = (K + BK - 1) / BK;
@@ -428,8 +403,7 @@ int kf_gemm_fp8_blocks(const void* A, const void* sa, const void* B, const void*
   if (tiles > 0x7fffffffLL) return 5;
   if (tiles < pairs) pairs = (int)tiles;
   kf_gemm_fp8_blocks_2cta<<<pairs * 2, THREADS, SMEM, (cudaStream_t)stream>>>(ma, mb, msa, msb, reinterpret_cast<__nv_bfloat16*>(C), M, N, K,
-                                                                             ldc, accumulate, a_fmt, b_fmt, tile_n,
-                                                                             reinterpret_cast<int*>(kf_status_device_ptr()));
+                                                                             ldc, accumulate, a_fmt, b_fmt, tile_n, status);
   cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? 0 : 400 + (int)e;
 }
