@@ -57,19 +57,19 @@ __device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
   return v;
 }
 
-// The scale bytes of COLS x 32 rows and four blocks, in the lane's words: row c * 32 + lane in word c.  Rows and blocks that do not exist
-// are 0 (their values are).
+// The scale bytes of COLS x 32 rows and four blocks, in the lane's words: row c * 32 + lane in word c.  All loads leave before the first is
+// waited for (one after another, as behind a test of each row, they took 7 us); in the place of rows and blocks that do not exist the
+// last one's are read, for accumulators that nobody reads.
 template <int COLS>
 __device__ __forceinline__ void load_scales(const uint8_t* __restrict__ s, long long ld, int row0, int rows, int kb0, int kb1, int lane,
                                             uint32_t (&w)[COLS]) {
+  uint8_t v[COLS][GROUP];
 #pragma unroll
-  for (int c = 0; c < COLS; ++c) {
-    const int r = row0 + c * 32 + lane;
-    w[c] = 0;
+  for (int c = 0; c < COLS; ++c)
 #pragma unroll
-    for (int b = 0; b < GROUP; ++b)
-      if (r < rows && kb0 + b < kb1) w[c] |= uint32_t(s[(long long)(kb0 + b) * ld + r]) << (8 * b);
-  }
+    for (int b = 0; b < GROUP; ++b) v[c][b] = __ldg(s + (long long)min(kb0 + b, kb1 - 1) * ld + min(row0 + c * 32 + lane, rows - 1));
+#pragma unroll
+  for (int c = 0; c < COLS; ++c) w[c] = uint32_t(v[c][0]) | uint32_t(v[c][1]) << 8 | uint32_t(v[c][2]) << 16 | uint32_t(v[c][3]) << 24;
 }
 
 struct Args {
@@ -79,6 +79,48 @@ struct Args {
   long long ldo;       // elements between rows of out
   int M, N, K, accumulate, x_fmt, w_fmt;
 };
+
+// This CTA's share of the tile: the sum of the SPLITS partial tiles at `red_addr` of each CTA, eight columns of a token per thread and step,
+// their loads all at once.
+template <int SPLITS>
+__device__ __forceinline__ void add_and_store(const Args& a, uint32_t red_addr, int row0, int rank, bool wide) {
+  const int valid = min(WROWS, a.N - row0);
+  for (int i = rank * THREADS + threadIdx.x; i < a.M * (WROWS / 8); i += SPLITS * THREADS) {
+    const int t = i / (WROWS / 8), n = (i % (WROWS / 8)) * 8;
+    if (n >= valid) continue;
+    const uint32_t off = red_addr + uint32_t(t * WROWS + n) * 4u;
+    float4 u[SPLITS], v[SPLITS];
+#pragma unroll
+    for (int r = 0; r < SPLITS; ++r) {
+      const uint32_t src = mapa_shared(off, r);
+      u[r] = ld_cluster_f4(src);
+      v[r] = ld_cluster_f4(src + 16);
+    }
+    float f[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+    for (int r = 0; r < SPLITS; ++r) {
+      f[0] += u[r].x; f[1] += u[r].y; f[2] += u[r].z; f[3] += u[r].w;
+      f[4] += v[r].x; f[5] += v[r].y; f[6] += v[r].z; f[7] += v[r].w;
+    }
+    __nv_bfloat16* p = a.out + (long long)t * a.ldo + row0 + n;
+    if (wide) {
+      uint4 o = make_uint4(0, 0, 0, 0);
+      if (a.accumulate) o = *reinterpret_cast<const uint4*>(p);
+      const uint32_t w[4] = {o.x, o.y, o.z, o.w};
+      uint32_t q[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 old = a.accumulate ? unpack_bf16(w[j]) : make_float2(0.f, 0.f);
+        q[j] = pack_bf16(f[2 * j] + old.x, f[2 * j + 1] + old.y);
+      }
+      *reinterpret_cast<uint4*>(p) = make_uint4(q[0], q[1], q[2], q[3]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (n + e < valid) p[e] = __float2bfloat16(a.accumulate ? f[e] + __bfloat162float(p[e]) : f[e]);
+    }
+  }
+}
 
 template <int NT>
 __global__ void __launch_bounds__(THREADS)
@@ -224,38 +266,11 @@ kf_gemm_fp8_blocks_skinny(const __grid_constant__ CUtensorMap map_x, const __gri
   }
 
   // ------------------------------------------------------------ sum over the splits (fixed order), store
-  const int valid = min(WROWS, a.N - row0);
-  for (int i = rank * THREADS + threadIdx.x; i < a.M * (WROWS / 8); i += splits * THREADS) {
-    const int t = i / (WROWS / 8), n = (i % (WROWS / 8)) * 8;
-    if (n >= valid) continue;
-    float f[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] = 0.f;
-    const uint32_t off = smem_base + uint32_t(t * WROWS + n) * 4u;
-#pragma unroll 1
-    for (int r = 0; r < splits; ++r) {
-      const uint32_t src = mapa_shared(off, r);
-      const float4 u = ld_cluster_f4(src), v = ld_cluster_f4(src + 16);
-      f[0] += u.x; f[1] += u.y; f[2] += u.z; f[3] += u.w;
-      f[4] += v.x; f[5] += v.y; f[6] += v.z; f[7] += v.w;
-    }
-    __nv_bfloat16* p = a.out + (long long)t * a.ldo + row0 + n;
-    if (wide) {
-      uint4 o = make_uint4(0, 0, 0, 0);
-      if (a.accumulate) o = *reinterpret_cast<const uint4*>(p);
-      const uint32_t w[4] = {o.x, o.y, o.z, o.w};
-      uint32_t q[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float2 old = a.accumulate ? unpack_bf16(w[j]) : make_float2(0.f, 0.f);
-        q[j] = pack_bf16(f[2 * j] + old.x, f[2 * j + 1] + old.y);
-      }
-      *reinterpret_cast<uint4*>(p) = make_uint4(q[0], q[1], q[2], q[3]);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (n + e < valid) p[e] = __float2bfloat16(a.accumulate ? f[e] + __bfloat162float(p[e]) : f[e]);
-    }
+  switch (splits) {
+    case 1: add_and_store<1>(a, smem_base, row0, rank, wide); break;
+    case 2: add_and_store<2>(a, smem_base, row0, rank, wide); break;
+    case 4: add_and_store<4>(a, smem_base, row0, rank, wide); break;
+    default: add_and_store<8>(a, smem_base, row0, rank, wide); break;
   }
   cluster_sync_all();  // the buffers stay valid until every CTA of the cluster has read them
 }
