@@ -147,6 +147,12 @@ kf_gemm_fp8_blocks_skinny(const __grid_constant__ CUtensorMap map_x, const __gri
   const int kb0 = k_blocks * rank / splits, kb1 = k_blocks * (rank + 1) / splits;
   const int n_kb = kb1 - kb0;
 
+  // the first scale bytes are asked for before the ring's first fill (up to 100 KB per CTA) stands in line at the memory
+  uint32_t sw[4], sx[C::SFX_COLS];
+  if (warp >= 2) {
+    load_scales<4>(a.sw, a.ldsw, row0, a.N, kb0, kb1, lane, sw);
+    load_scales<C::SFX_COLS>(a.sx, a.ldsx, 0, a.M, kb0, kb1, lane, sx);
+  }
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::STAGES; ++s) {
       mbar_init(full_bar(s), 1);
@@ -214,9 +220,6 @@ kf_gemm_fp8_blocks_skinny(const __grid_constant__ CUtensorMap map_x, const __gri
     const int quarter = warp & 3;
     const uint32_t t_lane = tmem_base + (uint32_t(quarter * 32) << 16);
     // ------------------------------------------------------------ scale bytes: global -> tensor memory
-    uint32_t sw[4], sx[C::SFX_COLS];
-    load_scales<4>(a.sw, a.ldsw, row0, a.N, kb0, kb1, lane, sw);
-    load_scales<C::SFX_COLS>(a.sx, a.ldsx, 0, a.M, kb0, kb1, lane, sx);
     for (int gi = 0; gi * GROUP < n_kb; ++gi) {
       const int g = gi % SLOTS;
       if (!mbar_wait(sf_empty_bar(g), ((gi / SLOTS) & 1) ^ 1, status, KF_ERR_WAIT_EMPTY)) { ok = false; break; }

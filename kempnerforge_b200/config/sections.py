@@ -190,6 +190,7 @@ class ActivationCheckpointing(StrEnum):
 
 
 _PRECISIONS = ("bf16", "fp16", "fp32", "fp8")
+_FP8_SCALINGS = ("tensor", "block128")
 
 
 @dataclass
@@ -203,6 +204,7 @@ class TrainConfig:
     data_seed: int | None = None
     compile_model: bool = True  # accepted for preset compatibility; no tracing compiler here
     mixed_precision: Literal["bf16", "fp16", "fp32", "fp8"] = "bf16"
+    fp8_scaling: Literal["tensor", "block128"] = "tensor"  # with mixed_precision "fp8": values that share a scale
     activation_checkpointing: ActivationCheckpointing = ActivationCheckpointing.none
     loss_fn: str = "cross_entropy"
     z_loss_weight: float = 0.0
@@ -215,6 +217,7 @@ class TrainConfig:
         for name in ("batch_size", "seq_len", "max_steps", "grad_accum_steps", "grad_clip_norm"):
             _require(getattr(self, name) > 0, f"{name} must be positive")
         _require(self.mixed_precision in _PRECISIONS, f"mixed_precision must be one of {_PRECISIONS}")
+        _require(self.fp8_scaling in _FP8_SCALINGS, f"fp8_scaling must be one of {_FP8_SCALINGS}")
 
     @property
     def param_dtype(self):

@@ -23,7 +23,10 @@ class SwiGLUMLP(nn.Module):
         self.down_proj = nn.Linear(hidden_dim, dim, bias=False)
         self.tp = None  # TPContext when gate/up are column-sharded and down row-sharded
 
-    def forward(self, x: torch.Tensor) -> torch.Tensor:
+    def forward(self, x: torch.Tensor, gate_up: torch.Tensor | None = None) -> torch.Tensor:
+        """``gate_up``: the two projections (.., gate | up) of ``x`` where the caller has them already."""
+        if gate_up is not None:
+            return F.linear(F.swiglu_stacked(gate_up), self.down_proj.weight)
         if self.tp is not None:
             gu = self.tp.column_linear(x, [self.gate_proj.weight, self.up_proj.weight])
             return self.tp.row_linear(F.swiglu_stacked(gu), self.down_proj.weight)

@@ -31,7 +31,7 @@ from kempnerforge_b200.config.sections import ModelConfig
 from kempnerforge_b200.models.attention import Attention, KVCache
 from kempnerforge_b200.models.embedding import OutputHead, TokenEmbedding
 from kempnerforge_b200.models.init import init_weights
-from kempnerforge_b200.models.mlp import build_mlp
+from kempnerforge_b200.models.mlp import SwiGLUMLP, build_mlp
 from kempnerforge_b200.models.modality import ModalityContext
 from kempnerforge_b200.models.moe import MoEMLP, build_moe
 from kempnerforge_b200.models.norm import build_norm
@@ -40,6 +40,11 @@ from kempnerforge_b200.ops import functional as F
 
 
 _FUSED_BLOCK_OFF = bool(os.environ.get("KF_DISABLE_FUSED_BLOCK"))
+
+
+def _unhooked(mod: nn.Module) -> bool:
+    """Nothing watches what goes into the module or stands in for its forward."""
+    return not (mod._forward_hooks or mod._forward_pre_hooks or mod._backward_hooks or mod._backward_pre_hooks or "forward" in mod.__dict__)
 
 
 class TransformerBlock(nn.Module):
@@ -78,12 +83,33 @@ class TransformerBlock(nn.Module):
             self.attention_norm(x), cos, sin, kv_cache=kv_cache, doc_ids=doc_ids, key_padding_mask=key_padding_mask
         )
 
+    def _fp8_qkv(self, x):
+        """(x, q | k | v of its norm) with the normalised activation in 8 bits (block-scaled fp8), or None."""
+        att = self.attention
+        if not getattr(self, "_kf_fp8_norms", False) or type(att) is not Attention or att.tp is not None or not _unhooked(att):
+            return None
+        from kempnerforge_b200.ops import fp8_blocks
+
+        return fp8_blocks.norm_linear_of(self.attention_norm, x, None, [att.q_proj.weight, att.k_proj.weight, att.v_proj.weight])
+
+    def _fp8_gate_up(self, x, attn):
+        """(x + attn, gate | up of its norm), likewise."""
+        mlp = self.mlp
+        if not getattr(self, "_kf_fp8_norms", False) or type(mlp) is not SwiGLUMLP or mlp.tp is not None or not _unhooked(mlp):
+            return None
+        from kempnerforge_b200.ops import fp8_blocks
+
+        return fp8_blocks.norm_linear_of(self.mlp_norm, x, attn, [mlp.gate_proj.weight, mlp.up_proj.weight])
+
     def _body(self, x, cos, sin, kv_cache, doc_ids, key_padding_mask):
         if self.ac_mode == "selective" and self.training and torch.is_grad_enabled() and kv_cache is None:
             attn = checkpoint(
                 self._attn_branch, x, cos, sin, None, doc_ids, key_padding_mask, use_reentrant=False,
                 context_fn=checkpoint_contexts,
             )
+        elif (pair := self._fp8_qkv(x)) is not None:
+            x, qkv = pair
+            attn = self.attention(x, cos, sin, kv_cache=kv_cache, doc_ids=doc_ids, key_padding_mask=key_padding_mask, qkv=qkv)
         else:
             if x.is_cuda and not _FUSED_BLOCK_OFF and F.use_native(x):
                 from kempnerforge_b200.ops import fused_block
@@ -94,6 +120,9 @@ class TransformerBlock(nn.Module):
                     x = fused_block.attn_half(self, x, cos, sin)
                     return x + self.mlp(self.mlp_norm(x))
             attn = self._attn_branch(x, cos, sin, kv_cache, doc_ids, key_padding_mask)
+        if (pair := self._fp8_gate_up(x, attn)) is not None:
+            x, gate_up = pair
+            return x + self.mlp(x, gate_up=gate_up)
         x = x + attn
         return x + self.mlp(self.mlp_norm(x))
 

@@ -34,8 +34,15 @@ def _eligible(linear: nn.Linear) -> bool:
     return linear.in_features % 16 == 0 and linear.out_features % 16 == 0
 
 
-def convert_model(model: nn.Module, skip: tuple[str, ...] = ("experts", "shared_expert", "router")) -> int:
-    """Tag every eligible ``nn.Linear`` outside ``skip`` for fp8 GEMMs.  Returns the number tagged."""
+SCALINGS = ("tensor", "block128")
+
+
+def convert_model(model: nn.Module, skip: tuple[str, ...] = ("experts", "shared_expert", "router"), scaling: str = "tensor") -> int:
+    """Tag every eligible ``nn.Linear`` outside ``skip`` for fp8 GEMMs, with one scale per tensor or (``scaling="block128"``,
+    :mod:`kempnerforge_b200.ops.fp8_blocks`) one for each block of 128.  Returns the number tagged."""
+    if scaling not in SCALINGS:
+        raise ValueError(f"fp8 scaling must be one of {SCALINGS}, got {scaling!r}")
+    blocks = scaling == "block128"
     n = 0
     for name, mod in model.named_modules():
         if not isinstance(mod, nn.Linear) or any(part in skip for part in name.split(".")):
@@ -45,16 +52,22 @@ def convert_model(model: nn.Module, skip: tuple[str, ...] = ("experts", "shared_
         if not _eligible(mod):
             continue
         mod.weight._kf_fp8 = True
+        mod.weight._kf_fp8_blocks = blocks
         n += 1
     for m in model.modules():
         if hasattr(m, "ac_mode"):
             m._kf_fp8_block = True  # the fused bf16 block node is bypassed
-    log.info("fp8: %d Linear layers use e4m3/e5m2 tensor-core GEMMs", n)
+            m._kf_fp8_norms = blocks  # a norm before such a Linear may write 8 bits
+    log.info("fp8: %d Linear layers use e4m3/e5m2 tensor-core GEMMs, one scale per %s", n, "block of 128" if blocks else "tensor")
     return n
 
 
 def is_fp8_weight(w: torch.Tensor) -> bool:
     return bool(getattr(w, "_kf_fp8", False))
+
+
+def has_block_scales(w: torch.Tensor) -> bool:
+    return bool(getattr(w, "_kf_fp8_blocks", False))
 
 
 # --------------------------------------------------------------------------- quantisation
@@ -256,7 +269,7 @@ def swiglu_mlp(x: torch.Tensor, wg: torch.Tensor, wu: torch.Tensor, wd: torch.Te
     """A SwiGLU feed-forward whose three weights are tagged for fp8 and that the node covers, else None."""
     from kempnerforge_b200.ops import functional as F
 
-    if (not F.use_native(x) or x.numel() == 0 or not supported(x, [wg, wu, wd]) or wg.shape != wu.shape
+    if (not F.use_native(x) or x.numel() == 0 or has_block_scales(wg) or not supported(x, [wg, wu, wd]) or wg.shape != wu.shape
             or wd.shape[1] != wg.shape[0] or wg.shape[1] != x.shape[-1] or any(not w.is_cuda or w.dtype != torch.bfloat16 for w in (wg, wu, wd))):
         return None
     return _Fp8SwiGLUFn.apply(x, wg, wu, wd, torch.is_grad_enabled())
@@ -264,10 +277,17 @@ def swiglu_mlp(x: torch.Tensor, wg: torch.Tensor, wu: torch.Tensor, wd: torch.Te
 
 def linear(x: torch.Tensor, weights: list[torch.Tensor]) -> torch.Tensor:
     """fp8 Linear against one weight or several weights stacked along the output dimension."""
+    if has_block_scales(weights[0]):
+        from kempnerforge_b200.ops import fp8_blocks
+
+        return fp8_blocks.linear(x, weights)
     return _Fp8LinearFn.apply(x, *weights)
 
 
 def supported(x: torch.Tensor, weights: list[torch.Tensor]) -> bool:
+    if has_block_scales(weights[0]):   # any number of tokens
+        return (x.dtype == torch.bfloat16 and x.dim() > 0
+                and all(has_block_scales(w) and w.dtype == torch.bfloat16 and w.shape[1] == x.shape[-1] and w.device == x.device for w in weights))
     t = x.numel() // x.shape[-1]
     return (x.dtype == torch.bfloat16 and t % 16 == 0 and all(is_fp8_weight(w) for w in weights)
             and all(w.shape[0] % 16 == 0 and w.shape[1] % 16 == 0 for w in weights))

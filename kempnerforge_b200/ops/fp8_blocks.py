@@ -269,12 +269,11 @@ class _BlocksLinearFn(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        *x8t, = ctx.saved_tensors[:2]
-        weights = ctx.saved_tensors[2:]
+        q8t, s8t, *weights = ctx.saved_tensors
         need_dx, need_dw = ctx.needs_input_grad[0], any(ctx.needs_input_grad[1:])
         g8, g8t = quantize(_rows(dy), want_row=need_dx, want_t=need_dw)
         dx = mm(g8, quantized_weight(weights, want_t=True)[1]).view(ctx.x_shape) if need_dx else None
-        wgrads = _weight_grads(weights, ctx.needs_input_grad[1:], g8t, BlockScaled(*x8t)) if need_dw else [None] * len(weights)
+        wgrads = _weight_grads(weights, ctx.needs_input_grad[1:], g8t, BlockScaled(q8t, s8t)) if need_dw else [None] * len(weights)
         return dx, *wgrads
 
 
@@ -356,6 +355,23 @@ def _normed_t(t, rstd, gain) -> BlockScaled:
         with _on(t):
             return BlockScaled(*_cuda().fp8_blocks_cast(t, False, False, False, True, rstd, _aligned(gain))[1])
     return _cast_rows((t.float() * rstd[:, None] * gain.float()).t().contiguous(), False)
+
+
+def norm_linear_of(norm, x: torch.Tensor, residual: torch.Tensor | None, weights):
+    """:func:`norm_linear` in place of the module ``norm`` and the product with ``weights``, or None where that is something else: another
+    norm, hooks that want its output, weights that are not tagged for block scales."""
+    from torch.nn.modules import module
+
+    from kempnerforge_b200.models.norm import RMSNorm
+
+    if (type(norm) is not RMSNorm or norm._forward_hooks or norm._forward_pre_hooks or norm._backward_hooks or norm._backward_pre_hooks
+            or "forward" in norm.__dict__ or module._has_any_global_hook() or not fp8.supported(x, weights)
+            or not fp8.has_block_scales(weights[0])):
+        return None
+    d = x.shape[-1]
+    if d % 8 or not 0 < d <= 32768 or norm.weight.dtype != _BF16 or norm.weight.device != x.device or (residual is not None and residual.dtype != _BF16):
+        return None
+    return norm_linear(x, residual, norm.weight, weights, norm.eps)
 
 
 def norm_linear(x: torch.Tensor, residual: torch.Tensor | None, norm_weight: torch.Tensor, weights, eps: float = 1e-5):

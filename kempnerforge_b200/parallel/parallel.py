@@ -68,12 +68,12 @@ def apply_ac(model: nn.Module, mode: str = "full") -> None:
     log.info("activation checkpointing = %s on %d blocks", mode, n)
 
 
-def apply_float8(model: nn.Module, enable_fsdp_float8_all_gather: bool = True) -> int:
-    """Switch the dense Linear call sites to tensor-wise scaled fp8 GEMMs; experts, shared experts and routers
-    keep bf16 (same module filter as the reference).  Returns the number of converted modules."""
+def apply_float8(model: nn.Module, enable_fsdp_float8_all_gather: bool = True, scaling: str = "tensor") -> int:
+    """Switch the dense Linear call sites to fp8 GEMMs, scaled per tensor or (``"block128"``) per block of 128; experts, shared experts
+    and routers keep bf16 (same module filter as the reference).  Returns the number of converted modules."""
     from kempnerforge_b200.ops import fp8
 
-    return fp8.convert_model(model, skip=("experts", "shared_expert", "router"))
+    return fp8.convert_model(model, skip=("experts", "shared_expert", "router"), scaling=scaling)
 
 
 def _wants_sharded_params(model: nn.Module, world: int, mode: str | None) -> bool:
@@ -196,6 +196,7 @@ def build_parallel_model(
     mp_policy: MixedPrecisionPolicy | None = None,
     frames_per_clip: int = 1,
     param_sharding: str | None = None,
+    fp8_scaling: str = "tensor",
     **model_kwargs,
 ) -> nn.Module:
     """Build the registered model and apply TP -> EP -> FP8 -> AC -> sharded DP.
@@ -236,7 +237,7 @@ def build_parallel_model(
         if ep_size > 1:
             apply_expert_parallel(model, ep_pg, ep_in_dp)
     if fp8:
-        apply_float8(model)
+        apply_float8(model, scaling=fp8_scaling)
     if ac_mode and str(ac_mode) != "none":
         apply_ac(model, str(ac_mode))
     apply_fsdp2(model, device_mesh, transport=transport, param_sharding=param_sharding)

@@ -306,7 +306,7 @@ def build_pipeline(config, device: torch.device, mesh, transport: str | None = N
 
         apply_tensor_parallel(module, mesh)
     if tc.is_fp8:
-        apply_float8(module)
+        apply_float8(module, scaling=tc.fp8_scaling)
     if str(tc.activation_checkpointing) != "none":
         apply_ac(module, str(tc.activation_checkpointing))
     apply_fsdp2(module, mesh, transport=transport)

@@ -127,7 +127,7 @@ class Trainer:
             self.model = build_parallel_model(
                 config.model, self.device, self.mesh,
                 ac_mode=str(tc.activation_checkpointing), param_dtype=tc.param_dtype,
-                fp8=tc.is_fp8, compile_model=False, transport=transport,
+                fp8=tc.is_fp8, fp8_scaling=tc.fp8_scaling, compile_model=False, transport=transport,
                 ep_in_dp=config.distributed.ep_in_dp and config.distributed.ep > 1,
                 param_sharding=getattr(config.distributed, "param_sharding", None),
             )
