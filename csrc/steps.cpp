@@ -17,6 +17,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <optional>
 #include <vector>
 
 namespace {
@@ -294,7 +295,18 @@ PyObject* configure(PyObject*, PyObject* args) {
   Py_RETURN_NONE;
 }
 
+}  // namespace
+
+#include "fp8_blocks_calls.h"
+
+namespace {
+
 PyMethodDef methods[] = {
+    {"fp8_mm", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(fp8_mm)), METH_FASTCALL, "product of block-scaled fp8 matrices"},
+    {"fp8_add_rmsnorm", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(fp8_add_rmsnorm)), METH_FASTCALL, "RMSNorm in block-scaled fp8"},
+    {"fp8_cast", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(fp8_cast)), METH_FASTCALL, "a matrix in block-scaled fp8"},
+    {"fp8_values", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(fp8_values)), METH_FASTCALL, "its values in bf16"},
+    {"fp8_configure", fp8_configure, METH_VARARGS, "the native entries of the block-scaled operators"},
     {"decode", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(decode)), METH_FASTCALL, "one new token per sequence through blocks"},
     {"configure", configure, METH_VARARGS, "classes and the native entry"},
     {nullptr, nullptr, 0, nullptr},

@@ -503,6 +503,8 @@ def _load_steps():
     spec.loader.exec_module(mod)
     mod.configure(Attention, SwiGLUMLP, RMSNorm, KVCache, torch.nn.Parameter,
                   ctypes.cast(lib().kf_blocks_decode_bf16, c_void_p).value, SKINNY_MAX_ROWS, lib().kf_skinny_norm_rows())
+    mod.fp8_configure(*(ctypes.cast(getattr(lib(), name), c_void_p).value for name in (
+        "kf_gemm_fp8_blocks", "kf_add_rmsnorm_fp8_blocks", "kf_fp8_blocks_cast_bf16", "kf_fp8_blocks_values_bf16")))
     _steps = mod
     return mod
 
@@ -883,6 +885,36 @@ def gemm_fp8_swiglu_bwd(a8: torch.Tensor, b8: torch.Tensor, sa: torch.Tensor, sb
 
 
 # --------------------------------------------------------------------------- fp8 with a scale for each block of 128 (ops/fp8_blocks.py)
+def _step(name: str, *args):
+    """The answer of a call of ``csrc/fp8_blocks_calls.h`` on the current device's stream; None where the call is not plainly covered."""
+    global LAUNCH_COUNT
+    steps = _load_steps() if _steps is None else _steps
+    if not steps:
+        return None
+    device = torch._C._cuda_getDevice()
+    r = getattr(steps, name)(*args, device, torch._C._cuda_getCurrentRawStream(device))
+    if type(r) is int:
+        raise NativeKernelError(f"{name} failed with code {r}")
+    if r is not None:
+        LAUNCH_COUNT += 1
+    return r
+
+
+def fp8_blocks_mm(a, b) -> torch.Tensor | None:
+    """:func:`gemm_fp8_blocks` of two (values, scales, e5m2), checked as well; None where Python's checks have to look."""
+    global LAUNCH_COUNT
+    steps = _load_steps() if _steps is None else _steps
+    if not steps:
+        return None
+    device = torch._C._cuda_getDevice()
+    r = steps.fp8_mm(*a, *b, device, torch._C._cuda_getCurrentRawStream(device), sm_count())
+    if type(r) is int:
+        raise NativeKernelError(f"kf_gemm_fp8_blocks failed with code {r}")
+    if r is not None:
+        LAUNCH_COUNT += 1
+    return r
+
+
 def _block_buffers(rows: int, cols: int, device):
     """(bytes (rows, cols) with rows on 128 bytes, scale bytes (ceil(cols / 128), rows) with rows on 16)."""
     values = torch.empty((rows, -(-cols // 128) * 128), dtype=torch.uint8, device=device)

@@ -64,6 +64,8 @@ class BlockScaled(NamedTuple):
 
     def dequantize(self) -> torch.Tensor:
         """The values as bf16, which has them exactly (down to 2^-133)."""
+        if self.values.is_cuda and (out := _cuda()._step("fp8_values", *self)) is not None:
+            return out
         _check_operand(self, "matrix")
         if self.values.numel() == 0:
             return torch.empty(self.values.shape, dtype=_BF16, device=self.values.device)
@@ -128,6 +130,9 @@ def quantize(x2: torch.Tensor, e5m2: bool = False, square: bool = False, want_ro
              want_t: bool = False) -> tuple[BlockScaled | None, BlockScaled | None]:
     """(``x2`` in 8 bits or None, its transpose in 8 bits or None) of a bf16 matrix.  ``square``: blocks of 128 x 128, so that both hold
     the same values; else each has blocks of 128 along its own columns."""
+    if x2.is_cuda and (r := _cuda()._step("fp8_cast", x2, e5m2, square, want_row, want_t)) is not None:
+        q, s, qt, st = r
+        return None if q is None else BlockScaled(q, s, e5m2), None if qt is None else BlockScaled(qt, st, e5m2)
     _check_matrix(x2)
     rows, cols = x2.shape
     if not (want_row or want_t):
@@ -146,6 +151,8 @@ def quantize(x2: torch.Tensor, e5m2: bool = False, square: bool = False, want_ro
 
 def mm(a: BlockScaled, b: BlockScaled, out: torch.Tensor | None = None, accumulate: bool = False) -> torch.Tensor:
     """bf16 (M, N) = a (M, K) @ b (N, K)ᵀ, accumulated in fp32 and rounded once; with ``accumulate`` added to ``out`` before that."""
+    if out is None and a.values.is_cuda and (y := _cuda().fp8_blocks_mm(a, b)) is not None:
+        return y
     _check_operand(a, "a")
     _check_operand(b, "b")
     (m, k), n = a.values.shape, b.values.shape[0]
@@ -182,6 +189,9 @@ def add_rmsnorm(x: torch.Tensor, residual: torch.Tensor | None, weight: torch.Te
     """(t, rstd, h) of bf16 matrices (rows, d), d a multiple of 8 up to 32 768: t = x + residual rounded to bf16 (x itself without one),
     rstd = 1 / sqrt(mean(t²) + eps) as fp32 (rows,), h = t * rstd * weight in 8 bits, never rounded to 16.  Not differentiable by itself:
     :func:`norm_linear` is."""
+    if x.is_cuda and (r := _cuda()._step("fp8_add_rmsnorm", x, residual, weight, eps)) is not None:
+        t, rstd, q, s = r
+        return x.detach() if t is None else t, rstd, BlockScaled(q, s)
     _check_norm(x, residual, weight)
     _check_matrix(x)
     x, residual, weight = x.detach(), None if residual is None else residual.detach(), weight.detach()
