@@ -1,8 +1,8 @@
 // Calls of the block-scaled fp8 operators (fp8_blocks.cu, gemm_fp8_blocks_tcgen05.cu) from Python: the checks of their arguments, the
 // output's memory and the launch in one native call.  In Python the checks of a product took 11 us and its ctypes call 5, more than most
-// products of few tokens take on the GPU: 19 us with the output's memory, and 6 so; a norm 21 and 9, a cast 15 and 7.  What is not plainly covered (another device than
-// the current one, pitches that need a copy, sizes of zero, arguments that are wrong) is answered with None and left to the Python path
-// (ops/fp8_blocks.py), which holds the rules; nothing is remembered between calls.
+// products of few tokens take on the GPU: 19 us with the output's memory, and 6 so; a norm 21 and 9, a cast 15 and 7.  What is not plainly
+// covered (another device than the current one, pitches that need a copy, sizes of zero, arguments that are wrong) is answered with None and
+// left to the Python path (ops/fp8_blocks.py), which holds the rules; nothing is remembered between calls.
 //
 // Included by steps.cpp, whose `tensor` tells plain tensors from wrappers.
 #pragma once
@@ -16,6 +16,8 @@ struct Fp8Blocks {
   int (*cast)(const void*, int, int, long long, const void*, const void*, int, int, void*, long long, void*, long long, void*, long long, void*,
               long long, void*) = nullptr;
   int (*values)(const void*, long long, const void*, long long, int, int, int, void*, void*) = nullptr;
+  int (*norm_bwd)(const void*, const void*, const void*, const void*, void*, void*, void*, void*, int, int, const void*, void*) = nullptr;
+  int (*norm_bwd_blocks)(int) = nullptr;
 } f8;
 
 constexpr long long kLargest = 0x7fffffff;
@@ -71,25 +73,29 @@ struct Buffers {
   long long scale_pitch() const { return scales_all.size(1); }
 };
 
-// fp8_mm(a values, a scales, a e5m2, b values, b scales, b e5m2, device, stream, sms) -> bf16 (M, N)
+// fp8_mm(a values, a scales, a e5m2, b values, b scales, b e5m2, out or None, accumulate, sms, device, stream) -> out, bf16 (M, N)
 PyObject* fp8_mm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   long device = 0;
   void* stream = nullptr;
-  if (nargs != 9 || !f8.gemm || !where(args + 6, &device, &stream)) return PyErr_Occurred() ? nullptr : Py_NewRef(Py_None);
+  if (nargs != 11 || !f8.gemm || !where(args + 9, &device, &stream)) return PyErr_Occurred() ? nullptr : Py_NewRef(Py_None);
   const long sms = PyLong_AsLong(args[8]);
   if (PyErr_Occurred()) return nullptr;
   const at::Tensor *qa, *sa, *qb, *sb;
-  int ea = 0, eb = 0;
+  int ea = 0, eb = 0, accumulate = 0;
   if (!operand(args[0], args[1], device, qa, sa) || !operand(args[3], args[4], device, qb, sb) || qa->size(1) != qb->size(1) ||
-      !flag(args[2], &ea) || !flag(args[5], &eb))
+      !flag(args[2], &ea) || !flag(args[5], &eb) || !flag(args[7], &accumulate))
+    Py_RETURN_NONE;
+  const at::Tensor* to = args[6] == Py_None ? nullptr : dense(args[6], at::kBFloat16, 2, device);
+  if (args[6] == Py_None ? accumulate != 0
+                         : !to || to->size(0) != qa->size(0) || to->size(1) != qb->size(0) || to->stride(1) != 1 || to->stride(0) < to->size(1))
     Py_RETURN_NONE;
   HANDLE_TH_ERRORS
-  at::Tensor out = at::empty({qa->size(0), qb->size(0)}, qa->options().dtype(at::kBFloat16));
+  at::Tensor out = to ? *to : at::empty({qa->size(0), qb->size(0)}, qa->options().dtype(at::kBFloat16));
   const int rc = issued([&] {
     return f8.gemm(qa->const_data_ptr(), sa->const_data_ptr(), qb->const_data_ptr(), sb->const_data_ptr(), at_(out), int(qa->size(0)), int(qb->size(0)),
-                   int(qa->size(1)), qa->stride(0), sa->stride(0), qb->stride(0), sb->stride(0), out.size(1), ea, eb, 0, int(sms), stream);
+                   int(qa->size(1)), qa->stride(0), sa->stride(0), qb->stride(0), sb->stride(0), out.stride(0), ea, eb, accumulate, int(sms), stream);
   });
-  return rc ? PyLong_FromLong(rc) : THPVariable_Wrap(std::move(out));
+  return rc ? PyLong_FromLong(rc) : to ? Py_NewRef(args[6]) : THPVariable_Wrap(std::move(out));
   END_HANDLE_TH_ERRORS
 }
 
@@ -122,23 +128,31 @@ PyObject* fp8_add_rmsnorm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
-// fp8_cast(x, e5m2, square, want_row, want_t, device, stream) -> (values, scales, transposed values, transposed scales), None where not wanted
+// fp8_cast(x, e5m2, square, want_row, want_t, rstd or None, gain or None, device, stream) -> (values, scales, transposed values, transposed
+// scales), None where not wanted; with rstd and gain of x * rstd[:, None] * gain
 PyObject* fp8_cast(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   long device = 0;
   void* stream = nullptr;
-  if (nargs != 7 || !f8.cast || !where(args + 5, &device, &stream)) return PyErr_Occurred() ? nullptr : Py_NewRef(Py_None);
+  if (nargs != 9 || !f8.cast || !where(args + 7, &device, &stream)) return PyErr_Occurred() ? nullptr : Py_NewRef(Py_None);
   int e5m2, square, row, tr;
   const at::Tensor* x = dense(args[0], at::kBFloat16, 2, device);
   if (!x || !flag(args[1], &e5m2) || !flag(args[2], &square) || !flag(args[3], &row) || !flag(args[4], &tr)) Py_RETURN_NONE;
   const int64_t rows = x->size(0), cols = x->size(1);
   if ((!row && !tr) || rows < 1 || cols < 1 || rows > 128 * 65535 || cols > kLargest || x->stride(1) != 1 || x->stride(0) < cols) Py_RETURN_NONE;
+  const at::Tensor *rstd = nullptr, *gain = nullptr;
+  if (args[5] != Py_None) {
+    rstd = dense(args[5], at::kFloat, 1, device);
+    gain = dense(args[6], at::kBFloat16, 1, device);
+    if (!rstd || !gain || square || e5m2 || rstd->size(0) != rows || gain->size(0) != cols || !rstd->is_contiguous() || !gain->is_contiguous()) Py_RETURN_NONE;
+  }
   HANDLE_TH_ERRORS
   const at::TensorOptions o = x->options().dtype(at::kByte);
   std::optional<Buffers> a, b;
   if (row) a.emplace(rows, cols, o);
   if (tr) b.emplace(cols, rows, o);
   const int rc = issued([&] {
-    return f8.cast(x->const_data_ptr(), int(rows), int(cols), x->stride(0), nullptr, nullptr, e5m2, square, a ? at_(a->values_all) : nullptr,
+    return f8.cast(x->const_data_ptr(), int(rows), int(cols), x->stride(0), rstd ? rstd->const_data_ptr() : nullptr,
+                   gain ? gain->const_data_ptr() : nullptr, e5m2, square, a ? at_(a->values_all) : nullptr,
                    a ? a->pitch() : 0, a ? at_(a->scales_all) : nullptr, a ? a->scale_pitch() : 0, b ? at_(b->values_all) : nullptr, b ? b->pitch() : 0,
                    b ? at_(b->scales_all) : nullptr, b ? b->scale_pitch() : 0, stream);
   });
@@ -167,10 +181,39 @@ PyObject* fp8_values(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
-// fp8_configure(addresses of kf_gemm_fp8_blocks, kf_add_rmsnorm_fp8_blocks, kf_fp8_blocks_cast_bf16, kf_fp8_blocks_values_bf16)
+// norm_grads(dh, t, gain, rstd, dt or None, device, stream) -> (dt + RMSNorm'(dh), gradient of the gain), both bf16
+PyObject* norm_grads(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  long device = 0;
+  void* stream = nullptr;
+  if (nargs != 7 || !f8.norm_bwd || !where(args + 5, &device, &stream)) return PyErr_Occurred() ? nullptr : Py_NewRef(Py_None);
+  const bool add = args[4] != Py_None;
+  const at::Tensor *dh = dense(args[0], at::kBFloat16, 2, device), *t = dense(args[1], at::kBFloat16, 2, device);
+  const at::Tensor *gain = dense(args[2], at::kBFloat16, 1, device), *rstd = dense(args[3], at::kFloat, 1, device);
+  const at::Tensor* dt = add ? dense(args[4], at::kBFloat16, 2, device) : nullptr;
+  if (!dh || !t || !gain || !rstd || (add && !dt)) Py_RETURN_NONE;
+  const int64_t rows = t->size(0), d = t->size(1);
+  if (rows < 1 || rows > kLargest || d < 8 || d % 8 || d > 32768 || dh->sizes() != t->sizes() || gain->size(0) != d || rstd->size(0) != rows ||
+      !dh->is_contiguous() || !t->is_contiguous() || !gain->is_contiguous() || !rstd->is_contiguous() || !address(*dh) || !address(*t) ||
+      !address(*gain) || (add && (dt->sizes() != t->sizes() || !dt->is_contiguous() || !address(*dt))))
+    Py_RETURN_NONE;
+  HANDLE_TH_ERRORS
+  at::Tensor partial = at::empty({f8.norm_bwd_blocks(int(rows)) * d}, rstd->options()), dx = at::empty({rows, d}, t->options());
+  at::Tensor dgain = at::empty({d}, t->options());
+  const int rc = issued([&] {
+    return f8.norm_bwd(dh->const_data_ptr(), t->const_data_ptr(), gain->const_data_ptr(), rstd->const_data_ptr(), at_(dx), at_(partial), at_(dgain),
+                       nullptr, int(rows), int(d), add ? dt->const_data_ptr() : nullptr, stream);
+  });
+  return rc ? PyLong_FromLong(rc) : Py_BuildValue("(NN)", THPVariable_Wrap(std::move(dx)), THPVariable_Wrap(std::move(dgain)));
+  END_HANDLE_TH_ERRORS
+}
+
+// fp8_configure(addresses of kf_gemm_fp8_blocks, kf_add_rmsnorm_fp8_blocks, kf_fp8_blocks_cast_bf16, kf_fp8_blocks_values_bf16,
+// kf_rmsnorm_bwd_bf16, kf_rmsnorm_bwd_blocks)
 PyObject* fp8_configure(PyObject*, PyObject* args) {
-  unsigned long long gemm = 0, norm = 0, cast = 0, values = 0;
-  if (!PyArg_ParseTuple(args, "KKKK", &gemm, &norm, &cast, &values)) return nullptr;
+  unsigned long long gemm = 0, norm = 0, cast = 0, values = 0, bwd = 0, bwd_blocks = 0;
+  if (!PyArg_ParseTuple(args, "KKKKKK", &gemm, &norm, &cast, &values, &bwd, &bwd_blocks)) return nullptr;
+  f8.norm_bwd = reinterpret_cast<decltype(f8.norm_bwd)>(bwd);
+  f8.norm_bwd_blocks = reinterpret_cast<decltype(f8.norm_bwd_blocks)>(bwd_blocks);
   f8.gemm = reinterpret_cast<decltype(f8.gemm)>(gemm);
   f8.norm = reinterpret_cast<decltype(f8.norm)>(norm);
   f8.cast = reinterpret_cast<decltype(f8.cast)>(cast);

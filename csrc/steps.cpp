@@ -306,6 +306,7 @@ PyMethodDef methods[] = {
     {"fp8_add_rmsnorm", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(fp8_add_rmsnorm)), METH_FASTCALL, "RMSNorm in block-scaled fp8"},
     {"fp8_cast", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(fp8_cast)), METH_FASTCALL, "a matrix in block-scaled fp8"},
     {"fp8_values", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(fp8_values)), METH_FASTCALL, "its values in bf16"},
+    {"norm_grads", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(norm_grads)), METH_FASTCALL, "gradients of an RMSNorm and its gain"},
     {"fp8_configure", fp8_configure, METH_VARARGS, "the native entries of the block-scaled operators"},
     {"decode", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(decode)), METH_FASTCALL, "one new token per sequence through blocks"},
     {"configure", configure, METH_VARARGS, "classes and the native entry"},

@@ -504,7 +504,8 @@ def _load_steps():
     mod.configure(Attention, SwiGLUMLP, RMSNorm, KVCache, torch.nn.Parameter,
                   ctypes.cast(lib().kf_blocks_decode_bf16, c_void_p).value, SKINNY_MAX_ROWS, lib().kf_skinny_norm_rows())
     mod.fp8_configure(*(ctypes.cast(getattr(lib(), name), c_void_p).value for name in (
-        "kf_gemm_fp8_blocks", "kf_add_rmsnorm_fp8_blocks", "kf_fp8_blocks_cast_bf16", "kf_fp8_blocks_values_bf16")))
+        "kf_gemm_fp8_blocks", "kf_add_rmsnorm_fp8_blocks", "kf_fp8_blocks_cast_bf16", "kf_fp8_blocks_values_bf16",
+        "kf_rmsnorm_bwd_bf16", "kf_rmsnorm_bwd_blocks")))
     _steps = mod
     return mod
 
@@ -885,7 +886,7 @@ def gemm_fp8_swiglu_bwd(a8: torch.Tensor, b8: torch.Tensor, sa: torch.Tensor, sb
 
 
 # --------------------------------------------------------------------------- fp8 with a scale for each block of 128 (ops/fp8_blocks.py)
-def _step(name: str, *args):
+def _step(name: str, *args, launches: int = 1):
     """The answer of a call of ``csrc/fp8_blocks_calls.h`` on the current device's stream; None where the call is not plainly covered."""
     global LAUNCH_COUNT
     steps = _load_steps() if _steps is None else _steps
@@ -896,23 +897,19 @@ def _step(name: str, *args):
     if type(r) is int:
         raise NativeKernelError(f"{name} failed with code {r}")
     if r is not None:
-        LAUNCH_COUNT += 1
+        LAUNCH_COUNT += launches
     return r
 
 
-def fp8_blocks_mm(a, b) -> torch.Tensor | None:
+def fp8_blocks_mm(a, b, out: torch.Tensor | None, accumulate: bool) -> torch.Tensor | None:
     """:func:`gemm_fp8_blocks` of two (values, scales, e5m2), checked as well; None where Python's checks have to look."""
-    global LAUNCH_COUNT
-    steps = _load_steps() if _steps is None else _steps
-    if not steps:
-        return None
-    device = torch._C._cuda_getDevice()
-    r = steps.fp8_mm(*a, *b, device, torch._C._cuda_getCurrentRawStream(device), sm_count())
-    if type(r) is int:
-        raise NativeKernelError(f"kf_gemm_fp8_blocks failed with code {r}")
-    if r is not None:
-        LAUNCH_COUNT += 1
-    return r
+    return _step("fp8_mm", *a, *b, out, accumulate, sm_count())
+
+
+def norm_grads(dh, t, gain, rstd, dt) -> tuple[torch.Tensor, torch.Tensor]:
+    """:func:`rmsnorm_bwd` of contiguous matrices, ``dt`` (or None) added."""
+    r = _step("norm_grads", dh, t, gain, rstd, dt, launches=3)
+    return rmsnorm_bwd(dh, t, gain, rstd, residual_grad=dt) if r is None else r
 
 
 def _block_buffers(rows: int, cols: int, device):

@@ -130,7 +130,7 @@ def quantize(x2: torch.Tensor, e5m2: bool = False, square: bool = False, want_ro
              want_t: bool = False) -> tuple[BlockScaled | None, BlockScaled | None]:
     """(``x2`` in 8 bits or None, its transpose in 8 bits or None) of a bf16 matrix.  ``square``: blocks of 128 x 128, so that both hold
     the same values; else each has blocks of 128 along its own columns."""
-    if x2.is_cuda and (r := _cuda()._step("fp8_cast", x2, e5m2, square, want_row, want_t)) is not None:
+    if x2.is_cuda and (r := _cuda()._step("fp8_cast", x2, e5m2, square, want_row, want_t, None, None)) is not None:
         q, s, qt, st = r
         return None if q is None else BlockScaled(q, s, e5m2), None if qt is None else BlockScaled(qt, st, e5m2)
     _check_matrix(x2)
@@ -151,7 +151,7 @@ def quantize(x2: torch.Tensor, e5m2: bool = False, square: bool = False, want_ro
 
 def mm(a: BlockScaled, b: BlockScaled, out: torch.Tensor | None = None, accumulate: bool = False) -> torch.Tensor:
     """bf16 (M, N) = a (M, K) @ b (N, K)ᵀ, accumulated in fp32 and rounded once; with ``accumulate`` added to ``out`` before that."""
-    if out is None and a.values.is_cuda and (y := _cuda().fp8_blocks_mm(a, b)) is not None:
+    if a.values.is_cuda and (y := _cuda().fp8_blocks_mm(a, b, out, accumulate)) is not None:
         return y
     _check_operand(a, "a")
     _check_operand(b, "b")
@@ -338,7 +338,7 @@ def _norm_grads(dh, t, gain, rstd, dt):
         return torch.empty_like(t), torch.zeros_like(gain)
     if t.is_cuda:
         with _on(t):
-            return _cuda().rmsnorm_bwd(dh, t, _aligned(gain), rstd, residual_grad=None if dt is None else _aligned(dt))
+            return _cuda().norm_grads(dh, t, _aligned(gain), rstd, None if dt is None else _aligned(dt))
     tf, g, r = t.float(), dh.float() * gain.float(), rstd[:, None]
     d = r * g - tf * (r * r * r * (g * tf).mean(1, keepdim=True))
     return (d if dt is None else d + dt.float()).to(_BF16), (dh.float() * tf * r).sum(0).to(gain.dtype)
@@ -362,6 +362,9 @@ def _normed_t(t, rstd, gain) -> BlockScaled:
     if t.numel() == 0:
         return _empty(t.shape[1], t.shape[0], t.device, False)
     if t.is_cuda:
+        r = _cuda()._step("fp8_cast", t, False, False, False, True, rstd, gain)
+        if r is not None:
+            return BlockScaled(r[2], r[3])
         with _on(t):
             return BlockScaled(*_cuda().fp8_blocks_cast(t, False, False, False, True, rstd, _aligned(gain))[1])
     return _cast_rows((t.float() * rstd[:, None] * gain.float()).t().contiguous(), False)
