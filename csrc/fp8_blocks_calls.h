@@ -62,15 +62,12 @@ int issued(Call&& call) {
 
 void* at_(const at::Tensor& t) { return t.mutable_data_ptr(); }
 
+// Values with rows on 128 bytes, scale bytes with rows on 16.
 struct Buffers {
-  at::Tensor values, scales, values_all, scales_all;
+  at::Tensor values, scales;
   Buffers(int64_t rows, int64_t cols, const at::TensorOptions& o)
-      : values_all(at::empty({rows, (cols + 127) / 128 * 128}, o)), scales_all(at::empty({(cols + 127) / 128, (rows + 15) / 16 * 16}, o)) {
-    values = values_all.size(1) == cols ? values_all : values_all.narrow(1, 0, cols);
-    scales = scales_all.size(1) == rows ? scales_all : scales_all.narrow(1, 0, rows);
-  }
-  long long pitch() const { return values_all.size(1); }
-  long long scale_pitch() const { return scales_all.size(1); }
+      : values(at::empty_strided({rows, cols}, {(cols + 127) / 128 * 128, 1}, o)),
+        scales(at::empty_strided({(cols + 127) / 128, rows}, {(rows + 15) / 16 * 16, 1}, o)) {}
 };
 
 // fp8_mm(a values, a scales, a e5m2, b values, b scales, b e5m2, out or None, accumulate, sms, device, stream) -> out, bf16 (M, N)
@@ -119,8 +116,8 @@ PyObject* fp8_add_rmsnorm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if (add) t = at::empty({rows, d}, x->options());
   Buffers h(rows, d, x->options().dtype(at::kByte));
   const int rc = issued([&] {
-    return f8.norm(x->const_data_ptr(), add ? r->const_data_ptr() : nullptr, gain->const_data_ptr(), add ? at_(t) : nullptr, at_(rstd), at_(h.values_all),
-                   h.pitch(), at_(h.scales_all), h.scale_pitch(), int(rows), int(d), float(eps), stream);
+    return f8.norm(x->const_data_ptr(), add ? r->const_data_ptr() : nullptr, gain->const_data_ptr(), add ? at_(t) : nullptr, at_(rstd), at_(h.values),
+                   h.values.stride(0), at_(h.scales), h.scales.stride(0), int(rows), int(d), float(eps), stream);
   });
   if (rc) return PyLong_FromLong(rc);
   PyObject* first = add ? THPVariable_Wrap(std::move(t)) : Py_NewRef(Py_None);
@@ -152,9 +149,9 @@ PyObject* fp8_cast(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if (tr) b.emplace(cols, rows, o);
   const int rc = issued([&] {
     return f8.cast(x->const_data_ptr(), int(rows), int(cols), x->stride(0), rstd ? rstd->const_data_ptr() : nullptr,
-                   gain ? gain->const_data_ptr() : nullptr, e5m2, square, a ? at_(a->values_all) : nullptr,
-                   a ? a->pitch() : 0, a ? at_(a->scales_all) : nullptr, a ? a->scale_pitch() : 0, b ? at_(b->values_all) : nullptr, b ? b->pitch() : 0,
-                   b ? at_(b->scales_all) : nullptr, b ? b->scale_pitch() : 0, stream);
+                   gain ? gain->const_data_ptr() : nullptr, e5m2, square, a ? at_(a->values) : nullptr,
+                   a ? a->values.stride(0) : 0, a ? at_(a->scales) : nullptr, a ? a->scales.stride(0) : 0, b ? at_(b->values) : nullptr,
+                   b ? b->values.stride(0) : 0, b ? at_(b->scales) : nullptr, b ? b->scales.stride(0) : 0, stream);
   });
   if (rc) return PyLong_FromLong(rc);
   auto give = [](std::optional<Buffers>& v, bool scales) {

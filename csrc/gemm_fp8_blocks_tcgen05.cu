@@ -18,6 +18,8 @@
 #include "pair_common.cuh"
 #include "tile_math.h"
 
+#include <utility>
+
 namespace kf {
 namespace f8b {
 
@@ -57,12 +59,32 @@ __device__ __forceinline__ void mma_pair_blocks(uint32_t d_tmem, uint64_t adesc,
 // Arrival and wait that hand over tensor memory only: what orders tcgen05.st before another CTA's tcgen05.mma is tcgen05.wait::st, the
 // tcgen05 fences on both sides and this signal.  With release and acquire at cluster scope in their stead a hand-over of four blocks'
 // scales took 2000 ns, whatever the width of the tile (74 x 256 rows, 128 to 224 columns, K 4096, us: 132 to 137, so 109 to 116).
-__device__ __forceinline__ void arrive_relaxed_on_leader(uint32_t bar) {
+__device__ __forceinline__ void arrive_relaxed_on_cta(uint32_t bar, uint32_t cta) {
   asm volatile(
       "{\n\t.reg .b32 ra;\n\t"
-      "mapa.shared::cluster.u32 ra, %0, 0;\n\t"
-      "mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [ra];\n\t}" ::"r"(bar)
+      "mapa.shared::cluster.u32 ra, %0, %1;\n\t"
+      "mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [ra];\n\t}" ::"r"(bar),
+      "r"(cta)
       : "memory");
+}
+// Arrival on the barrier at the same place in the CTAs of the mask once all instructions issued by this thread have retired.
+__device__ __forceinline__ void commit_to(uint32_t bar, uint16_t mask) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"(mask)
+      : "memory");
+}
+__device__ __forceinline__ void st_cluster_f4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+__device__ __forceinline__ uint32_t cluster_nctaid() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t mapa_shared(uint32_t addr, uint32_t cta) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(cta));
+  return r;
 }
 __device__ __forceinline__ bool mbar_wait_relaxed(uint32_t bar, uint32_t parity, int* status, int code) {
   const long long t0 = clock64();
@@ -97,22 +119,73 @@ __device__ __forceinline__ unsigned short lds_u16(uint32_t addr) {
   return v;
 }
 
-// 32 x 32 values of a warp (a row per lane) into a matrix whose rows do not start on 16 bytes: through the box, 64 contiguous bytes of one
-// row per instruction.
-__device__ __forceinline__ void store_rows32_any(uint32_t box, int lane, const Rows32& own, __nv_bfloat16* dst, size_t ld, int rows, int cols) {
-  __syncwarp();
-#pragma unroll
-  for (int q = 0; q < 4; ++q) sts128(box_row_chunk(box, lane, q), own.q[q]);
-  __syncwarp();
-  for (int r = 0; r < rows; ++r)
-    if (lane < cols) reinterpret_cast<unsigned short*>(dst)[r * ld + lane] = lds_u16(box_row_chunk(box, r, lane >> 3) + (lane & 7) * 2);
-}
+// Where a product goes: C[row * ld + column], or with `turned` (A's rows are C's columns) C[column * ld + row].
+struct Output {
+  __nv_bfloat16* C;
+  long long ld;
+  int turned, accumulate;
+  bool wide;  // rows of C start on 16 bytes and hold a multiple of eight values
 
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
+  // 32 x 32 values of a warp at (row0, col0), a row per lane, of which rows x cols exist; box: 2 KB of the warp's own
+  __device__ __forceinline__ void put(uint32_t box, int lane, const uint32_t (&v)[32], int row0, int col0, int rows, int cols) const {
+    if (turned) {
+      __nv_bfloat16* dst = C + (long long)col0 * ld + row0;
+      if (wide && !accumulate) {
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 32; ++i) sts_bf16(box_row_chunk(box, i, lane >> 3) + (lane & 7) * 2, __uint_as_float(v[i]));
+        copy_box(box, lane, dst, cols, rows);
+      } else if (lane < rows) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+          if (i < cols) add_or_set(dst + i * ld + lane, __uint_as_float(v[i]));
+      }
+      return;
+    }
+    __nv_bfloat16* dst = C + (long long)row0 * ld + col0;
+    if (!accumulate) {
+      const Rows32 own = pack_row32(v);
+      __syncwarp();
+#pragma unroll
+      for (int q = 0; q < 4; ++q) sts128(box_row_chunk(box, lane, q), own.q[q]);
+      if (wide) {
+        copy_box(box, lane, dst, rows, cols);
+      } else {  // 64 contiguous bytes of one row per instruction
+        __syncwarp();
+        for (int r = 0; r < rows; ++r)
+          if (lane < cols) reinterpret_cast<unsigned short*>(dst)[r * ld + lane] = lds_u16(box_row_chunk(box, r, lane >> 3) + (lane & 7) * 2);
+      }
+    } else if (lane < rows) {
+      dst += lane * ld;
+      if (wide) {
+        store_chunk<__nv_bfloat16>(dst, v, cols, true, nullptr);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+          if (i < cols) add_or_set(dst + i, __uint_as_float(v[i]));
+      }
+    }
+  }
+
+ private:
+  __device__ __forceinline__ void add_or_set(__nv_bfloat16* p, float v) const { *p = __float2bfloat16(accumulate ? __bfloat162float(*p) + v : v); }
+  static __device__ __forceinline__ void sts_bf16(uint32_t addr, float v) {
+    asm volatile("st.shared.u16 [%0], %1;" ::"r"(addr), "h"(__bfloat16_as_ushort(__float2bfloat16(v))) : "memory");
+  }
+  __device__ __forceinline__ void copy_box(uint32_t box, int lane, __nv_bfloat16* dst, int rows, int cols) const {
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int row = i * 8 + (lane >> 2), ch = lane & 3;
+      if (row < rows && ch * 8 < cols) *reinterpret_cast<uint4*>(dst + row * ld + ch * 8) = lds128(box_row_chunk(box, row, ch));
+    }
+  }
+};
+
+__global__ void __launch_bounds__(THREADS, 1)
 kf_gemm_fp8_blocks_2cta(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                         const __grid_constant__ CUtensorMap map_sa, const __grid_constant__ CUtensorMap map_sb,
-                        __nv_bfloat16* __restrict__ C, int M, int N, int K, long long ldc, int accumulate, int a_fmt, int b_fmt, int tile_n,
-                        int* status) {
+                        const Output out, int M, int N, int K, int a_fmt, int b_fmt, int tile_n, int* status) {
   extern __shared__ uint8_t smem_raw[];
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   const uint32_t sf_smem = smem_base + STAGES * STAGE_BYTES;
@@ -133,14 +206,19 @@ kf_gemm_fp8_blocks_2cta(const __grid_constant__ CUtensorMap map_a, const __grid_
 
   const int warp = warp_index();
   const int lane = threadIdx.x & 31;
-  const uint32_t rank = cluster_ctarank();
+  // A cluster is `splits` pairs that divide the reduction of a tile; with one pair it walks over its share of the tiles.
+  const uint32_t cta = cluster_ctarank(), rank = cta & 1, lead = cta & ~1u;
+  const uint16_t pair_mask = uint16_t(3u << lead);
   const bool leader = rank == 0;
-  const int pair = blockIdx.x >> 1, num_pairs = gridDim.x >> 1;
+  const int splits = int(cluster_nctaid()) >> 1, split = int(cta) >> 1;
+  const int pair = int(blockIdx.x) / (2 * splits), num_pairs = int(gridDim.x) / (2 * splits);
   const int half_n = tile_n >> 1;
   const int m_blocks = (M + TILE_M - 1) / TILE_M;
   const int n_blocks = (N + tile_n - 1) / tile_n;
   const int num_tiles = m_blocks * n_blocks;
-  const int k_blocks = (K + BK - 1) / BK, groups = (k_blocks + GROUP - 1) / GROUP;
+  const int all_blocks = (K + BK - 1) / BK;
+  const int kb0 = all_blocks * split / splits, k_blocks = all_blocks * (split + 1) / splits - kb0;  // this pair's
+  const int groups = (k_blocks + GROUP - 1) / GROUP;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
@@ -173,6 +251,9 @@ kf_gemm_fp8_blocks_2cta(const __grid_constant__ CUtensorMap map_a, const __grid_
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot_ptr;
 
+  const int quarter = warp & 3;
+  const uint32_t box = box_smem + uint32_t((warp - 6) & 3) * BOX_BYTES, t_row = tmem_base + (uint32_t(quarter * 32) << 16);
+
   if (warp == 0) {
     // ------------------------------------------------------------ TMA producer (one per CTA)
     if (elect_one()) {
@@ -189,8 +270,8 @@ kf_gemm_fp8_blocks_2cta(const __grid_constant__ CUtensorMap map_a, const __grid_
           const uint32_t a_dst = smem_base + s * STAGE_BYTES;
           const uint32_t lead_full = full_bar(s) & PEER_BIT_MASK;
           if (leader) mbar_expect_tx(full_bar(s), 2 * (A_BYTES + half_n * BK));
-          tma_load_2d_pair(a_dst, &map_a, lead_full, kb * BK, m0);
-          tma_load_2d_pair(a_dst + A_BYTES, &map_b, lead_full, kb * BK, n0);
+          tma_load_2d_pair(a_dst, &map_a, lead_full, (kb0 + kb) * BK, m0);
+          tma_load_2d_pair(a_dst + A_BYTES, &map_b, lead_full, (kb0 + kb) * BK, n0);
         }
       }
       // copies into this CTA's shared memory are complete once their stages were consumed or, on the error path, once
@@ -212,8 +293,8 @@ kf_gemm_fp8_blocks_2cta(const __grid_constant__ CUtensorMap map_a, const __grid_
           const int g = gi % SLOTS;
           if (!mbar_wait(sf_empty_bar(g), ((gi / SLOTS) & 1) ^ 1, status, KF_ERR_WAIT_EMPTY)) { ok = false; break; }
           mbar_expect_tx(sf_full_bar(g), GROUP * (CTA_M + tile_n));
-          tma_load_2d(sf_smem + g * SF_BYTES, &map_sa, sf_full_bar(g), m0, i * GROUP);
-          tma_load_2d(sf_smem + g * SF_BYTES + SFA_BYTES, &map_sb, sf_full_bar(g), n0, i * GROUP);
+          tma_load_2d(sf_smem + g * SF_BYTES, &map_sa, sf_full_bar(g), m0, kb0 + i * GROUP);
+          tma_load_2d(sf_smem + g * SF_BYTES + SFA_BYTES, &map_sb, sf_full_bar(g), n0, kb0 + i * GROUP);
         }
       }
       for (int j = max(0, gi - SLOTS); j < gi; ++j)
@@ -245,13 +326,13 @@ kf_gemm_fp8_blocks_2cta(const __grid_constant__ CUtensorMap map_a, const __grid_
           for (int k = 0; k < BK / UMMA_K; ++k)
             mma_pair_blocks(d_tmem, umma_desc_sw128(a_src + k * UMMA_K, 16, 1024), umma_desc_sw128(b_src + k * UMMA_K, 16, 1024),
                             idesc + b * IDESC_NEXT_BYTE, sfa, sfb, (kb | k) != 0);
-          commit_pair(empty_bar(s));
+          commit_to(empty_bar(s), pair_mask);
           if (b == GROUP - 1 || kb == k_blocks - 1) {
-            commit_pair(sf_empty_bar(g));
+            commit_to(sf_empty_bar(g), pair_mask);
             ++gi;
           }
         }
-        if (ok) commit_pair(tfull_bar(acc));
+        if (ok) commit_to(tfull_bar(acc), pair_mask);
       }
       // every MMA must have retired before either CTA gives up its shared or tensor memory
       asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(drain_bar)
@@ -283,56 +364,90 @@ kf_gemm_fp8_blocks_2cta(const __grid_constant__ CUtensorMap map_a, const __grid_
         __syncwarp();
         if (lane == 0) {
           mbar_arrive(sf_empty_bar(g));
-          arrive_relaxed_on_leader(sf_ready_bar(g));
+          arrive_relaxed_on_cta(sf_ready_bar(g), lead);
         }
       }
     }
   } else {
     // ------------------------------------------------------------ epilogue (warps 6 .. 9 of both CTAs)
-    const int quarter = warp & 3;
-    const uint32_t box = box_smem + uint32_t(warp - 6) * BOX_BYTES;
-    const bool wide = ((ldc | N) & 7) == 0 && (reinterpret_cast<uintptr_t>(C) & 15) == 0;
     int tile_iter = 0;
     bool ok = true;
     for (int t = pair; t < num_tiles && ok; t += num_pairs, ++tile_iter) {
+      const int acc = tile_iter & 1;
+      if (!mbar_wait(tfull_bar(acc), (tile_iter >> 1) & 1, status, KF_ERR_WAIT_TMEM_FULL)) { ok = false; break; }
+      tc_fence_after();
+      if (splits > 1) break;  // the only tile: below, together with the other pairs
       int tm, tn;
       tilemath::raster(t, m_blocks, n_blocks, GROUP_M, tm, tn);
-      const int acc = tile_iter & 1;
-      const uint32_t acc_ph = (tile_iter >> 1) & 1;
-      if (!mbar_wait(tfull_bar(acc), acc_ph, status, KF_ERR_WAIT_TMEM_FULL)) { ok = false; break; }
-      tc_fence_after();
       const int row0 = tm * TILE_M + int(rank) * CTA_M + quarter * 32;  // this warp's rows, and how many exist
       const int rows = max(0, min(32, M - row0));
       const int col0 = tn * tile_n, width = min(tile_n, N - col0);
-      const uint32_t t_row = tmem_base + (uint32_t(quarter * 32) << 16) + acc * MAX_N;
-      __nv_bfloat16* c0 = C + size_t(row0) * ldc + col0;
 #pragma unroll 1
       for (int c = 0; c * 32 < width; ++c) {
         uint32_t v[32];
-        tmem_ld_32x32(t_row + c * 32, v);
+        tmem_ld_32x32(t_row + acc * MAX_N + c * 32, v);
         tmem_ld_wait();
-        const int valid = min(32, width - c * 32);
-        __nv_bfloat16* dst = c0 + c * 32;
-        if (!accumulate) {
-          if (wide) store_rows32(box, lane, pack_row32(v), dst, ldc, rows, valid);
-          else store_rows32_any(box, lane, pack_row32(v), dst, ldc, rows, valid);
-        } else if (lane < rows) {
-          dst += size_t(lane) * ldc;
-          if (wide) {
-            store_chunk<__nv_bfloat16>(dst, v, valid, true, nullptr);
-          } else {
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (i < valid) dst[i] = __float2bfloat16(__bfloat162float(dst[i]) + __uint_as_float(v[i]));
-          }
-        }
+        out.put(box, lane, v, row0, col0 + c * 32, rows, min(32, width - c * 32));
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) arrive_on_cta(tempty_bar(acc), 0);
+      if (lane == 0) arrive_on_cta(tempty_bar(acc), lead);
     }
   }
 
+  if (splits > 1) {
+    // ------------------------------------------------------------ sum over the pairs of the cluster
+    // Chunk c of 32 columns belongs to pair c % splits.  Every pair hands the other chunks of its accumulator to their owners' shared memory
+    // (16 bytes of a lane's row after 16 of its neighbour's), where the rings are idle once all instructions have retired, and the owner adds
+    // them in the order of the pairs, in 32 bits.
+    constexpr uint32_t CHUNK_BYTES = CTA_M * 32 * 4, WARP_BYTES = 32 * 32 * 4;
+    int tm, tn;
+    tilemath::raster(pair, m_blocks, n_blocks, GROUP_M, tm, tn);
+    const int row0 = tm * TILE_M + int(rank) * CTA_M + quarter * 32, rows = max(0, min(32, M - row0));
+    const int col0 = tn * tile_n, width = min(tile_n, N - col0);
+    const uint32_t mine = smem_base + uint32_t(quarter) * WARP_BYTES + uint32_t(lane) * 16;
+    __syncwarp();
+    cluster_sync_all();
+    if (warp >= 6 && warp < 10) {
+#pragma unroll 1
+      for (int c = 0; c * 32 < width; ++c) {
+        const int owner = c % splits;
+        if (owner == split) continue;
+        uint32_t v[32];
+        tmem_ld_32x32(t_row + c * 32, v);
+        tmem_ld_wait();
+        const uint32_t at = mapa_shared(mine + uint32_t((c / splits) * (splits - 1) + (split < owner ? split : split - 1)) * CHUNK_BYTES, 2 * owner + rank);
+#pragma unroll
+        for (int q = 0; q < 8; ++q) st_cluster_f4(at + q * 512, v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+      }
+    }
+    __syncwarp();
+    cluster_sync_all();
+    if (warp >= 6 && warp < 10) {
+#pragma unroll 1
+      for (int c = split; c * 32 < width; c += splits) {
+        uint32_t own[32], v[32];
+        tmem_ld_32x32(t_row + c * 32, own);
+        tmem_ld_wait();
+        const uint32_t at = mine + uint32_t((c / splits) * (splits - 1)) * CHUNK_BYTES;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] = 0u;
+#pragma unroll 1
+        for (int j = 0; j < splits; ++j) {
+#pragma unroll
+          for (int q = 0; q < 8; ++q) {
+            uint4 u = make_uint4(own[4 * q], own[4 * q + 1], own[4 * q + 2], own[4 * q + 3]);
+            if (j != split) u = lds128(at + uint32_t(j < split ? j : j - 1) * CHUNK_BYTES + q * 512);
+            v[4 * q] = __float_as_uint(__uint_as_float(v[4 * q]) + __uint_as_float(u.x));
+            v[4 * q + 1] = __float_as_uint(__uint_as_float(v[4 * q + 1]) + __uint_as_float(u.y));
+            v[4 * q + 2] = __float_as_uint(__uint_as_float(v[4 * q + 2]) + __uint_as_float(u.z));
+            v[4 * q + 3] = __float_as_uint(__uint_as_float(v[4 * q + 3]) + __uint_as_float(u.w));
+          }
+        }
+        out.put(box, lane, v, row0, col0 + c * 32, rows, min(32, width - c * 32));
+      }
+    }
+  }
   tc_fence_before();
   __syncthreads();
   cluster_sync_all();
@@ -342,29 +457,42 @@ kf_gemm_fp8_blocks_2cta(const __grid_constant__ CUtensorMap map_a, const __grid_
   }
 }
 
-// Tile width of a launch: rounds of tiles over the pairs times the columns of a tile, narrow ones at a surcharge for the operand bytes
-// that they need per clock (pair_tile_width has the figures).
-static int tile_width(int M, int N, int pairs) {
-  const int m_blocks = (M + TILE_M - 1) / TILE_M;
-  int best = MAX_N;
+// How a product is cut: which matrix gives the rows of 256, the columns of a tile, the pairs that divide its reduction.
+struct Cut {
+  int turned, tile_n, splits;
+};
+// The cheapest by what was measured, in ns: a block of 128 takes 0.66 (columns + 250) on a pair while all of them ask for operands (64 columns
+// 207, 128 250, 192 300, 224 313), the last tile's way out 4.5 a column, and the sum over a cluster its barriers and its copies.  Of 74 pairs
+// 33 clusters of two fit, and 15 of four.  us, graph of launches on weights in turn, cut by columns only -> so: 200 x 4096 from 14 336 36.5 ->
+// 21.1, 64 x 4096 from 4096 12.5 -> 10.4, 1554 x 7168 from 5120 50.9 -> 45.0, 2000 x 2048 from 2048 14.9 -> 12.3, 120 x 1304 from 952 6.6 -> 6.0.
+static Cut cut_of(int M, int N, int K, int num_sms) {
+  const int pairs = num_sms / 2, k_blocks = (K + BK - 1) / BK;
+  Cut best{0, MAX_N, 1};
   float best_cost = 3.4e38f;
-  for (int tn = MAX_N; tn >= 128; tn -= 32) {
-    const long long tiles = (long long)m_blocks * ((N + tn - 1) / tn);
-    const long long rounds = (tiles + pairs - 1) / pairs;
-    const float bytes_per_clk = (128.f + 0.5f * tn) * 64.f / tn;
-    const float cost = float(rounds) * tn * (1.f + 0.1f * (bytes_per_clk - 64.f) / 32.f);
-    if (cost < best_cost) {
-      best = tn;
-      best_cost = cost;
+  for (int turned = 0; turned < 2; ++turned) {
+    const int m = turned ? N : M, n = turned ? M : N, m_blocks = (m + TILE_M - 1) / TILE_M;
+    for (int tn = MAX_N; tn >= 32; tn -= 32) {
+      if (tn - 32 >= n) continue;
+      const long long tiles = (long long)m_blocks * ((n + tn - 1) / tn);
+      for (int splits = 1; splits <= 4; splits *= 2) {
+        if (splits > 1 && (tiles * splits > pairs - (splits == 2 ? 8 : 14) || k_blocks < splits)) break;
+        const long long rounds = splits > 1 ? 1 : (tiles + pairs - 1) / pairs;
+        const float cost = float(rounds * ((k_blocks + splits - 1) / splits)) * 0.66f * float(tn + 250) + 4.5f * float(tn) +
+                           (splits == 1 ? 0.f : splits == 2 ? 600.f + 13.f * float(tn) : 1200.f + 20.f * float(tn));
+        if (cost < best_cost) {
+          best = {turned, tn, splits};
+          best_cost = cost;
+        }
+      }
     }
   }
   return best;
 }
 
-// gemm_fp8_blocks_skinny.cu
-int gemm_blocks_skinny(const void* A, const void* sa, const void* B, const void* sb, void* C, int M, int N, int K, long long lda,
-                       long long ldsa, long long ldb, long long ldsb, long long ldc, int a_fmt, int b_fmt, int accumulate, int num_sms,
-                       int* status, void* stream);
+// gemm_fp8_blocks_few.cu
+bool few_serves(int M, int N, int K);
+int gemm_blocks_few(const void* A, const void* sa, const void* B, const void* sb, void* C, int M, int N, int K, long long lda, long long ldsa,
+                    long long ldb, long long ldsb, long long ldc, int a_fmt, int b_fmt, int accumulate, int num_sms, void* stream);
 
 }  // namespace f8b
 }  // namespace kf
@@ -381,11 +509,20 @@ int kf_gemm_fp8_blocks(const void* A, const void* sa, const void* B, const void*
   using namespace kf::f8b;
   if (((lda | ldb | ldsa | ldsb) & 15) || M <= 0 || N <= 0 || K <= 0 || num_sms < 2) return 5;
   int* status = reinterpret_cast<int*>(kf_status_device_ptr());
-  if (M <= 256)
-    return gemm_blocks_skinny(A, sa, B, sb, C, M, N, K, lda, ldsa, ldb, ldsb, ldc, a_fmt, b_fmt, accumulate, num_sms, status, stream);
-  int pairs = num_sms / 2;
-  const int tile_n = tile_width(M, N, pairs);
-  const int k_blocks = (K + BK - 1) / BK;
+  if (few_serves(M, N, K)) return gemm_blocks_few(A, sa, B, sb, C, M, N, K, lda, ldsa, ldb, ldsb, ldc, a_fmt, b_fmt, accumulate, num_sms, stream);
+  const Cut cut = cut_of(M, N, K, num_sms);
+  const bool wide = ((ldc | N) & 7) == 0 && (reinterpret_cast<uintptr_t>(C) & 15) == 0;
+  if (cut.turned) {
+    std::swap(A, B);
+    std::swap(sa, sb);
+    std::swap(lda, ldb);
+    std::swap(ldsa, ldsb);
+    std::swap(M, N);
+    std::swap(a_fmt, b_fmt);
+  }
+  const int tile_n = cut.tile_n, k_blocks = (K + BK - 1) / BK;
+  const long long tiles = (long long)((M + TILE_M - 1) / TILE_M) * ((N + tile_n - 1) / tile_n);
+  if (tiles > 0x7fffffffLL) return 5;
   CUtensorMap ma, mb, msa, msb;
   int rc;
   if ((rc = make_map_u8(&ma, A, M, K, lda, BK, CTA_M, true))) return 100 + rc;
@@ -400,12 +537,20 @@ int kf_gemm_fp8_blocks(const void* A, const void* sa, const void* B, const void*
     if (e != cudaSuccess) return 300 + (int)e;
     if (dev < 64) attr_set[dev] = true;
   }
-  const long long tiles = (long long)((M + TILE_M - 1) / TILE_M) * ((N + tile_n - 1) / tile_n);
-  if (tiles > 0x7fffffffLL) return 5;
-  if (tiles < pairs) pairs = (int)tiles;
-  kf_gemm_fp8_blocks_2cta<<<pairs * 2, THREADS, SMEM, (cudaStream_t)stream>>>(ma, mb, msa, msb, reinterpret_cast<__nv_bfloat16*>(C), M, N, K,
-                                                                             ldc, accumulate, a_fmt, b_fmt, tile_n, status);
-  cudaError_t e = cudaGetLastError();
+  const int clusters = cut.splits > 1 ? (int)tiles : (int)(tiles < num_sms / 2 ? tiles : num_sms / 2);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(unsigned(clusters * 2 * cut.splits));
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = SMEM;
+  cfg.stream = (cudaStream_t)stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = unsigned(2 * cut.splits);
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const Output out{reinterpret_cast<__nv_bfloat16*>(C), ldc, cut.turned, accumulate, wide};
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kf_gemm_fp8_blocks_2cta, ma, mb, msa, msb, out, M, N, K, a_fmt, b_fmt, tile_n, status);
   return e == cudaSuccess ? 0 : 400 + (int)e;
 }
 

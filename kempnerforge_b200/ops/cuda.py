@@ -914,9 +914,8 @@ def norm_grads(dh, t, gain, rstd, dt) -> tuple[torch.Tensor, torch.Tensor]:
 
 def _block_buffers(rows: int, cols: int, device):
     """(bytes (rows, cols) with rows on 128 bytes, scale bytes (ceil(cols / 128), rows) with rows on 16)."""
-    values = torch.empty((rows, -(-cols // 128) * 128), dtype=torch.uint8, device=device)
-    scales = torch.empty((-(-cols // 128), -(-rows // 16) * 16), dtype=torch.uint8, device=device)
-    return values if values.shape[1] == cols else values[:, :cols], scales if scales.shape[1] == rows else scales[:, :rows]
+    return (torch.empty_strided((rows, cols), (-(-cols // 128) * 128, 1), dtype=torch.uint8, device=device),
+            torch.empty_strided((-(-cols // 128), rows), (-(-rows // 16) * 16, 1), dtype=torch.uint8, device=device))
 
 
 def fp8_blocks_cast(x2: torch.Tensor, e5m2: bool, square: bool, want_row: bool, want_t: bool, rstd: torch.Tensor | None = None,

@@ -93,7 +93,8 @@ def _mm_close(got, want, mag, k):
 
 
 MM = [(1, 1, 1), (1, 4096, 512), (2, 24, 136), (16, 128, 128), (17, 1001, 777), (64, 256, 2048), (100, 136, 40), (128, 224, 640),
-      (129, 225, 129), (200, 512, 1536), (256, 448, 256), (257, 300, 1000), (333, 1001, 777), (513, 96, 384), (700, 1792, 520)]
+      (129, 225, 129), (200, 512, 1536), (256, 448, 256), (257, 300, 1000), (333, 1001, 777), (513, 96, 384), (700, 1792, 520),
+      (300, 200, 4096), (260, 1000, 8200), (2001, 72, 2048), (72, 2001, 2048), (1300, 1304, 900), (5000, 40, 1000), (3000, 2999, 136)]
 
 
 @pytest.mark.parametrize("ea, eb", [(False, False), (True, False), (False, True), (True, True)], ids=["e4m3", "e5m2xe4m3", "e4m3xe5m2", "e5m2"])
@@ -108,7 +109,7 @@ def test_product(native_lib, m, n, k, ea, eb):
     assert native_lib.read_status() == 0
 
 
-@pytest.mark.parametrize("m, n, k", [(5, 200, 300), (64, 129, 256), (300, 520, 384), (300, 521, 384)])
+@pytest.mark.parametrize("m, n, k", [(5, 200, 300), (64, 129, 256), (300, 520, 384), (300, 521, 384), (264, 1000, 4096), (261, 1000, 4096), (1304, 296, 4096), (1300, 297, 2048)])
 def test_product_adds_into_a_pitched_output_and_leaves_the_rest(native_lib, m, n, k):
     a, b, av, bv = _mm_case(m, n, k, False, False, 7)
     want, mag = av @ bv.t(), av.abs() @ bv.abs().t()
