@@ -8,6 +8,8 @@
 // An infinity or a NaN is stored as NaN, and the other values of its block are scaled as if it were not there.
 #include "fp8_blocks.cuh"
 
+#include <type_traits>
+
 namespace kf {
 namespace f8b {
 
@@ -21,25 +23,38 @@ __device__ __forceinline__ float half_warp_max(float m) {
   for (int o = 8; o > 0; o >>= 1) m = max_abs(m, __shfl_xor_sync(0xffffffffu, m, o));
   return m;
 }
+// of pairs of bf16 (a NaN counts for nothing)
+__device__ __forceinline__ uint32_t max_abs2(uint32_t m, uint32_t v) {
+  const __nv_bfloat162 r = __hmax2(*reinterpret_cast<const __nv_bfloat162*>(&m), __habs2(*reinterpret_cast<const __nv_bfloat162*>(&v)));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
 
-// One 128 x 128 tile per block of 256 threads: 16 threads x 8 columns, 8 rows per thread.
-template <bool E5M2, int SRC, bool SQUARE>
-__global__ void __launch_bounds__(256)
+// One 128 x 128 tile per block of 512 threads: 16 threads x 8 columns, rows ty, ty + 32, ty + 64 and ty + 96 of a thread.
+//
+// Bound by memory: 2 bytes in, 1 or 2 out per element, and all of them pass through registers, so what counts is how many blocks an SM
+// holds while others wait (registers: two to four) and how little is done per value: maxima of bf16 values are taken in pairs as they
+// are, and infinities have a path of their own.  16 384 x 4096, us (at the copy rate): row-major 35 (31), transposed 41 (31), both 57 (41),
+// squares both 49 (41), normed 54 (31); with 256 threads, two blocks on an SM and a look at each value for infinities 60, 68, 84, 59 and 128.
+template <bool E5M2, int SRC, bool SQUARE, bool ROW, bool T>
+__global__ void __launch_bounds__(512, ROW && !T ? 4 : SRC == NORMED ? 2 : 3)
 kf_cast_blocks(const __nv_bfloat16* __restrict__ x, int rows, int cols, long long ldx, const float* __restrict__ rstd,
                const __nv_bfloat16* __restrict__ gain, uint8_t* __restrict__ out, long long ld_out, uint8_t* __restrict__ scales,
                long long ld_scales, uint8_t* __restrict__ out_t, long long ld_t, uint8_t* __restrict__ scales_t, long long ld_scales_t) {
-  __shared__ uint32_t tile[128][32];  // bytes of the tile on their way to the transposed copy; first the column maxima
+  constexpr int PER = 4;  // rows of a thread
+  __shared__ uint32_t tile[T ? 128 : 1][32];               // bytes of the tile on their way to the transposed copy
+  __shared__ float part[T && !SQUARE ? 16 : 1][128];       // column maxima of each warp
   __shared__ float col_inv[128];
   __shared__ uint8_t row_byte[128], col_byte[128];
-  __shared__ float red[8];
+  __shared__ float red[16];
   const int r0 = blockIdx.y * 128, c0 = blockIdx.x * 128;
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   const int c = c0 + tx * 8;
   const bool wide_in = c + 7 < cols && (ldx & 7) == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0;
-  uint4 v[8];
+  uint4 v[PER];
+  float s[PER];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int r = r0 + ty + 16 * i;
+  for (int i = 0; i < PER; ++i) {
+    const int r = r0 + ty + 32 * i;
     v[i] = make_uint4(0, 0, 0, 0);
     if (r < rows) {
       const __nv_bfloat16* p = x + size_t(r) * ldx + c;
@@ -53,73 +68,110 @@ kf_cast_blocks(const __nv_bfloat16* __restrict__ x, int rows, int cols, long lon
         v[i] = make_uint4(w[0], w[1], w[2], w[3]);
       }
     }
+    if (SRC == NORMED) s[i] = rstd[min(r, rows - 1)];
   }
   float g[8];
   if (SRC == NORMED) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) g[e] = c + e < cols ? __bfloat162float(gain[c + e]) : 0.f;
+    for (int e = 0; e < 8; ++e) g[e] = __bfloat162float(gain[min(c + e, cols - 1)]);
   }
-  // the values of row i, as the norm kernel forms them
-  auto values = [&](int i, float (&f)[8]) {
-    const int r = r0 + ty + 16 * i;
-    const float s = SRC == NORMED && r < rows ? rstd[r] : 0.f;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float2 p = pair_at(v[i], j);
-      f[2 * j] = SRC == NORMED ? mul_full(mul_full(p.x, s), g[2 * j]) : p.x;
-      f[2 * j + 1] = SRC == NORMED ? mul_full(mul_full(p.y, s), g[2 * j + 1]) : p.y;
-    }
+  // two neighbouring values, as the norm kernel forms them
+  auto value2 = [&](int i, int j) {
+    float2 p = pair_at(v[i], j);
+    if (SRC == NORMED) p = make_float2(mul_full(mul_full(p.x, s[i]), g[2 * j]), mul_full(mul_full(p.y, s[i]), g[2 * j + 1]));
+    return p;
   };
-  float row_max[8], col_max[8];
-  bool any_inf = false;
+  // maxima of the thread's part of each row, and of its columns
+  float row_max[PER], col_max[8];
+  if (SRC == PLAIN) {
+    uint32_t rm[PER], cm[4] = {0, 0, 0, 0};
 #pragma unroll
-  for (int e = 0; e < 8; ++e) col_max[e] = 0.f;
+    for (int i = 0; i < PER; ++i) {
+      rm[i] = 0;
+      const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    float f[8], m = 0.f;
-    values(i, f);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      m = max_abs(m, f[e]);
-      col_max[e] = max_abs(col_max[e], f[e]);
+      for (int j = 0; j < 4; ++j) {
+        if (ROW || SQUARE) rm[i] = max_abs2(rm[i], w[j]);
+        if (T && !SQUARE) cm[j] = max_abs2(cm[j], w[j]);
+      }
     }
-    row_max[i] = m;
-    any_inf |= is_inf(m);
+    if (ROW || SQUARE) {  // two rows to a word
+#pragma unroll
+      for (int i = 0; i < PER; i += 2) {
+        uint32_t m = max_abs2(__byte_perm(rm[i], rm[i + 1], 0x5410), __byte_perm(rm[i], rm[i + 1], 0x7632));
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) m = max_abs2(m, __shfl_xor_sync(0xffffffffu, m, o));
+        const float2 f = unpack_bf16(m);
+        row_max[i] = f.x;
+        row_max[i + 1] = f.y;
+      }
+    }
+    if (T && !SQUARE) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 f = unpack_bf16(max_abs2(cm[j], __shfl_xor_sync(0xffffffffu, cm[j], 16)));
+        col_max[2 * j] = f.x;
+        col_max[2 * j + 1] = f.y;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) col_max[e] = 0.f;
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 f = value2(i, j);
+        col_max[2 * j] = max_abs(col_max[2 * j], f.x);
+        col_max[2 * j + 1] = max_abs(col_max[2 * j + 1], f.y);
+      }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) col_max[e] = max_abs(col_max[e], __shfl_xor_sync(0xffffffffu, col_max[e], 16));
+  }
+  bool any_inf = false;
+  if (ROW || SQUARE) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) any_inf |= is_inf(row_max[i]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) any_inf |= is_inf(col_max[e]);
   }
   any_inf = __syncthreads_or(any_inf);
   if (any_inf) {  // rare: once more, over the finite values
 #pragma unroll
     for (int e = 0; e < 8; ++e) col_max[e] = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      float f[8], m = 0.f;
-      values(i, f);
+    for (int i = 0; i < PER; ++i) {
+      float m = 0.f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        m = max_abs(m, nan_if_inf(f[e]));
-        col_max[e] = max_abs(col_max[e], nan_if_inf(f[e]));
+      for (int j = 0; j < 4; ++j) {
+        float2 f = value2(i, j);
+        f = make_float2(nan_if_inf(f.x), nan_if_inf(f.y));
+        m = max_abs(max_abs(m, f.x), f.y);
+        col_max[2 * j] = max_abs(col_max[2 * j], f.x);
+        col_max[2 * j + 1] = max_abs(col_max[2 * j + 1], f.y);
       }
-      row_max[i] = m;
+      row_max[i] = half_warp_max(m);
     }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) col_max[e] = max_abs(col_max[e], __shfl_xor_sync(0xffffffffu, col_max[e], 16));
   }
   float block_inv = 0.f;
   uint32_t block_byte = 0;
   if (SQUARE) {
-    float m = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) m = max_abs(m, row_max[i]);
-    m = half_warp_max(m);
+    float m = max_abs(max_abs(row_max[0], row_max[1]), max_abs(row_max[2], row_max[3]));
     m = max_abs(m, __shfl_xor_sync(0xffffffffu, m, 16));
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
+    if (lane == 0) red[warp] = m;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < 8; ++w) m = max_abs(m, red[w]);
+    for (int w = 0; w < 16; ++w) m = max_abs(m, red[w]);
     block_byte = scale_byte<E5M2>(m);
     block_inv = inverse_of(block_byte);
-  } else if (out_t) {
-    float(*part)[128] = reinterpret_cast<float(*)[128]>(&tile[0][0]);  // [16][128]
-#pragma unroll
-    for (int e = 0; e < 8; ++e) part[ty][tx * 8 + e] = col_max[e];
+  } else if (T) {
+    if (lane < 16) {
+      *reinterpret_cast<float4*>(&part[warp][tx * 8]) = make_float4(col_max[0], col_max[1], col_max[2], col_max[3]);
+      *reinterpret_cast<float4*>(&part[warp][tx * 8 + 4]) = make_float4(col_max[4], col_max[5], col_max[6], col_max[7]);
+    }
     __syncthreads();
     if (threadIdx.x < 128) {
       float m = 0.f;
@@ -131,67 +183,64 @@ kf_cast_blocks(const __nv_bfloat16* __restrict__ x, int rows, int cols, long lon
     }
     __syncthreads();
   }
+  float ci[8];
+  if (T && !SQUARE) {
+    const float4 lo = *reinterpret_cast<const float4*>(&col_inv[tx * 8]), hi = *reinterpret_cast<const float4*>(&col_inv[tx * 8 + 4]);
+    ci[0] = lo.x; ci[1] = lo.y; ci[2] = lo.z; ci[3] = lo.w;
+    ci[4] = hi.x; ci[5] = hi.y; ci[6] = hi.z; ci[7] = hi.w;
+  }
   const bool wide_out = c + 7 < cols && (ld_out & 7) == 0 && (reinterpret_cast<uintptr_t>(out) & 7) == 0;
+  // with_inf: infinities are looked for, which costs as much again as all that is done otherwise
+  auto give = [&](auto with_inf) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int rl = ty + 16 * i, r = r0 + rl;
-    float f[8];
-    values(i, f);
-    if (any_inf) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) f[e] = nan_if_inf(f[e]);
-    }
-    uint32_t q[2] = {0, 0};
-    if (out || SQUARE) {
+    for (int i = 0; i < PER; ++i) {
+      const int rl = ty + 32 * i, r = r0 + rl;
+      uint32_t q[2] = {0, 0}, qt[2] = {0, 0};
       float inv = block_inv;
-      if (!SQUARE) {
-        const uint32_t b = scale_byte<E5M2>(half_warp_max(row_max[i]));
+      if (ROW && !SQUARE) {
+        const uint32_t b = scale_byte<E5M2>(row_max[i]);
         inv = inverse_of(b);
         if (tx == 0) row_byte[rl] = uint8_t(b);
       }
 #pragma unroll
-      for (int j = 0; j < 4; ++j) q[j >> 1] |= to_bytes<E5M2>(f[2 * j], f[2 * j + 1], inv) << (16 * (j & 1));
-    }
-    if (out && r < rows) {
-      uint8_t* o = out + size_t(r) * ld_out + c;
-      if (wide_out) {
-        *reinterpret_cast<uint2*>(o) = make_uint2(q[0], q[1]);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (c + e < cols) o[e] = uint8_t(q[e >> 2] >> (8 * (e & 3)));
+      for (int j = 0; j < 4; ++j) {
+        float2 f = value2(i, j);
+        if (decltype(with_inf)::value) f = make_float2(nan_if_inf(f.x), nan_if_inf(f.y));
+        if (ROW || SQUARE) q[j >> 1] |= to_bytes<E5M2>(mul_full(f.x, inv), mul_full(f.y, inv)) << (16 * (j & 1));
+        if (T && !SQUARE) qt[j >> 1] |= to_bytes<E5M2>(mul_full(f.x, ci[2 * j]), mul_full(f.y, ci[2 * j + 1])) << (16 * (j & 1));
       }
-    }
-    if (out_t) {
-      if (!SQUARE) {
-        q[0] = q[1] = 0;
+      if (ROW && r < rows) {
+        uint8_t* o = out + size_t(r) * ld_out + c;
+        if (wide_out) {
+          *reinterpret_cast<uint2*>(o) = make_uint2(q[0], q[1]);
+        } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint32_t lo = to_bytes<E5M2>(f[2 * j], 0.f, col_inv[tx * 8 + 2 * j]), hi = to_bytes<E5M2>(f[2 * j + 1], 0.f, col_inv[tx * 8 + 2 * j + 1]);
-          q[j >> 1] |= ((lo & 0xffu) | (hi & 0xffu) << 8) << (16 * (j & 1));
+          for (int e = 0; e < 8; ++e)
+            if (c + e < cols) o[e] = uint8_t(q[e >> 2] >> (8 * (e & 3)));
         }
       }
-      // word w of row r at w ^ 4 * (r / 16 % 8): the 32 lanes of a transposed read hit 32 different banks
-      *reinterpret_cast<uint2*>(&tile[rl][(tx * 2) ^ (((rl >> 4) & 7) << 2)]) = make_uint2(q[0], q[1]);
+      // word w of row r at w ^ 2 * (r / 8 % 16): the 32 lanes of a transposed read hit 32 different banks
+      if (T) *reinterpret_cast<uint2*>(&tile[rl][(tx * 2) ^ (((rl >> 3) & 15) << 1)]) = SQUARE ? make_uint2(q[0], q[1]) : make_uint2(qt[0], qt[1]);
     }
-  }
+  };
+  if (any_inf) give(std::true_type{});
+  else give(std::false_type{});
   __syncthreads();
-  if (threadIdx.x < 128) {
+  if (ROW && threadIdx.x < 128) {
     const int r = r0 + threadIdx.x;
-    if (out && r < rows) scales[blockIdx.x * ld_scales + r] = SQUARE ? uint8_t(block_byte) : row_byte[threadIdx.x];
-  } else if (out_t) {
+    if (r < rows) scales[blockIdx.x * ld_scales + r] = SQUARE ? uint8_t(block_byte) : row_byte[threadIdx.x];
+  } else if (T && threadIdx.x >= 128 && threadIdx.x < 256) {
     const int k = threadIdx.x - 128;
     if (c0 + k < cols) scales_t[blockIdx.y * ld_scales_t + c0 + k] = SQUARE ? uint8_t(block_byte) : col_byte[k];
   }
-  if (!out_t) return;
-  const int lane = threadIdx.x & 31;
-  const int rg = lane & 7, cg = (threadIdx.x >> 5) * 4 + (lane >> 3);  // 16 source rows x 4 source columns per thread
-  uint32_t t[4][4];                                                     // [column][word of four rows]
+  if (!T) return;
+  const int rg = lane & 15, cg = warp * 2 + (lane >> 4);  // 8 source rows x 4 source columns per thread
+  uint32_t t[4][2];                                       // [column][word of four rows]
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < 2; ++i) {
     uint32_t a[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) a[j] = tile[rg * 16 + i * 4 + j][cg ^ (rg << 2)];
+    for (int j = 0; j < 4; ++j) a[j] = tile[rg * 8 + i * 4 + j][cg ^ (rg << 1)];
     const uint32_t p0 = __byte_perm(a[0], a[1], 0x5140), p1 = __byte_perm(a[0], a[1], 0x7362);
     const uint32_t p2 = __byte_perm(a[2], a[3], 0x5140), p3 = __byte_perm(a[2], a[3], 0x7362);
     t[0][i] = __byte_perm(p0, p2, 0x5410);
@@ -199,18 +248,18 @@ kf_cast_blocks(const __nv_bfloat16* __restrict__ x, int rows, int cols, long lon
     t[2][i] = __byte_perm(p1, p3, 0x5410);
     t[3][i] = __byte_perm(p1, p3, 0x7632);
   }
-  const int r = r0 + rg * 16;
-  const bool wide_t = r + 15 < rows && (ld_t & 15) == 0 && (reinterpret_cast<uintptr_t>(out_t) & 15) == 0;
+  const int r = r0 + rg * 8;
+  const bool wide_t = r + 7 < rows && (ld_t & 7) == 0 && (reinterpret_cast<uintptr_t>(out_t) & 7) == 0;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const int oc = c0 + cg * 4 + j;
     if (oc >= cols) continue;
     uint8_t* o = out_t + size_t(oc) * ld_t + r;
     if (wide_t) {
-      *reinterpret_cast<uint4*>(o) = make_uint4(t[j][0], t[j][1], t[j][2], t[j][3]);
+      *reinterpret_cast<uint2*>(o) = make_uint2(t[j][0], t[j][1]);
     } else {
 #pragma unroll
-      for (int e = 0; e < 16; ++e)
+      for (int e = 0; e < 8; ++e)
         if (r + e < rows) o[e] = uint8_t(t[j][e >> 2] >> (8 * (e & 3)));
     }
   }
@@ -299,49 +348,47 @@ kf_add_rmsnorm_blocks(const __nv_bfloat16* __restrict__ x, const __nv_bfloat16* 
     if (i < nvec) {
       uint32_t q[2] = {0, 0};
 #pragma unroll
-      for (int j = 0; j < 4; ++j) q[j >> 1] |= to_bytes<false>(f[2 * j], f[2 * j + 1], inv) << (16 * (j & 1));
+      for (int j = 0; j < 4; ++j) q[j >> 1] |= to_bytes<false>(mul_full(f[2 * j], inv), mul_full(f[2 * j + 1], inv)) << (16 * (j & 1));
       *reinterpret_cast<uint2*>(out + row * ld_out + i * 8) = make_uint2(q[0], q[1]);
       if ((i & 15) == 0) scales[(i >> 4) * ld_scales + row] = uint8_t(b);
     }
   }
 }
 
-// The values that the bytes stand for, in bf16 (exact where bf16 has them): eight per thread.
+// The values that the bytes stand for, in bf16 (exact where bf16 has them): sixteen per thread, blocks of 16 x 16 threads on 256 columns.
 template <bool E5M2>
 __global__ void __launch_bounds__(256)
 kf_blocks_values(const uint8_t* __restrict__ q, long long ld, const uint8_t* __restrict__ scales, long long ld_scales, int rows, int cols,
                  __nv_bfloat16* __restrict__ out) {
-  const int vecs = (cols + 7) >> 3;
-  const long long i = blockIdx.x * 256LL + threadIdx.x;
-  if (i >= (long long)rows * vecs) return;
-  const int r = int(i / vecs), c = int(i - (long long)r * vecs) * 8;
-  // a factor of 2^-127 (byte 0) has no normal 32-bit number: half of the next one, which subnormal arithmetic keeps
-  const uint32_t b = scales[(c >> 7) * ld_scales + r];
-  const float f = b == 0 ? __uint_as_float(0x400000u) : b == 255 ? __uint_as_float(0x7fffffffu) : __uint_as_float(b << 23);
+  const int c = blockIdx.y * 256 + (threadIdx.x & 15) * 16, r = blockIdx.x * 16 + (threadIdx.x >> 4);
+  if (c >= cols || r >= rows) return;
   const uint8_t* p = q + r * ld + c;
   __nv_bfloat16* o = out + (size_t)r * cols + c;
-  const bool whole = c + 7 < cols;
-  uint32_t w[2] = {0, 0};
-  if (whole && (ld & 7) == 0 && (reinterpret_cast<uintptr_t>(q) & 7) == 0) {
-    const uint2 u = *reinterpret_cast<const uint2*>(p);
-    w[0] = u.x;
-    w[1] = u.y;
+  const bool whole = c + 15 < cols;
+  uint32_t w[4] = {0, 0, 0, 0};
+  const uint32_t b = scales[(c >> 7) * ld_scales + r];
+  if (whole && (ld & 15) == 0 && (reinterpret_cast<uintptr_t>(q) & 15) == 0) {
+    const uint4 u = *reinterpret_cast<const uint4*>(p);
+    w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
   } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
+    for (int e = 0; e < 16; ++e)
       if (c + e < cols) w[e >> 2] |= uint32_t(p[e]) << (8 * (e & 3));
   }
-  uint32_t packed[4];
+  // a factor of 2^-127 (byte 0) has no normal 32-bit number: half of the next one, which subnormal arithmetic keeps
+  const float f = b == 0 ? __uint_as_float(0x400000u) : b == 255 ? __uint_as_float(0x7fffffffu) : __uint_as_float(b << 23);
+  uint32_t packed[8];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
+  for (int j = 0; j < 8; ++j) {
     const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w[j >> 1] >> (16 * (j & 1))), E5M2 ? __NV_E5M2 : __NV_E4M3);
     packed[j] = pack_bf16(mul_full(__half2float(__half(__half_raw{h.x})), f), mul_full(__half2float(__half(__half_raw{h.y})), f));
   }
   if (whole && (cols & 7) == 0) {
     *reinterpret_cast<uint4*>(o) = make_uint4(packed[0], packed[1], packed[2], packed[3]);
+    *reinterpret_cast<uint4*>(o + 8) = make_uint4(packed[4], packed[5], packed[6], packed[7]);
   } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
+    for (int e = 0; e < 16; ++e)
       if (c + e < cols) reinterpret_cast<unsigned short*>(o)[e] = (unsigned short)(packed[e >> 1] >> (16 * (e & 1)));
   }
 }
@@ -356,23 +403,29 @@ static int launched() {
 
 extern "C" {
 
-// Casts bf16 x[rows][cols] (pitch ldx elements), or x * rstd[row] * gain[column] where rstd is given.  out / scales: row-major copy (pitch
+// Casts bf16 x[rows][cols] (pitch ldx elements), or x * rstd[row] * gain[column] where rstd is given (the transposed copy in e4m3 only).  out / scales: row-major copy (pitch
 // ld_out) and its (ceil(cols / 128), rows) scale bytes (pitch ld_scales); out_t / scales_t: the transposed one, (cols, rows) and
 // (ceil(rows / 128), cols); either may be null.  square: blocks of 128 x 128.
 int kf_fp8_blocks_cast_bf16(const void* x, int rows, int cols, long long ldx, const void* rstd, const void* gain, int e5m2, int square,
                             void* out, long long ld_out, void* scales, long long ld_scales, void* out_t, long long ld_t, void* scales_t,
                             long long ld_scales_t, void* stream) {
   using namespace kf::f8b;
-  if (rows <= 0 || cols <= 0 || rows > 128 * 65535 || (rstd == nullptr) != (gain == nullptr) || (!out && !out_t) || (rstd && (square || e5m2)))
+  if (rows <= 0 || cols <= 0 || rows > 128 * 65535 || (rstd == nullptr) != (gain == nullptr) || (!out && !out_t) ||
+      (rstd && (square || e5m2 || out)))
     return 5;
-  const dim3 grid((cols + 127) / 128, (rows + 127) / 128);
-  auto kern = rstd ? kf_cast_blocks<false, NORMED, false>
-              : square ? (e5m2 ? kf_cast_blocks<true, PLAIN, true> : kf_cast_blocks<false, PLAIN, true>)
-                       : (e5m2 ? kf_cast_blocks<true, PLAIN, false> : kf_cast_blocks<false, PLAIN, false>);
-  kern<<<grid, 256, 0, (cudaStream_t)stream>>>((const __nv_bfloat16*)x, rows, cols, ldx, (const float*)rstd, (const __nv_bfloat16*)gain,
-                                               (uint8_t*)out, ld_out, (uint8_t*)scales, ld_scales, (uint8_t*)out_t, ld_t,
-                                               (uint8_t*)scales_t, ld_scales_t);
-  return launched();
+  auto go = [&](auto kern) {
+    kern<<<dim3((cols + 127) / 128, (rows + 127) / 128), 512, 0, (cudaStream_t)stream>>>(
+        (const __nv_bfloat16*)x, rows, cols, ldx, (const float*)rstd, (const __nv_bfloat16*)gain, (uint8_t*)out, ld_out, (uint8_t*)scales,
+        ld_scales, (uint8_t*)out_t, ld_t, (uint8_t*)scales_t, ld_scales_t);
+    return launched();
+  };
+  auto copies = [&](auto e5, auto sq) {
+    constexpr bool E = decltype(e5)::value, S = decltype(sq)::value;
+    return !out_t ? go(kf_cast_blocks<E, PLAIN, S, true, false>) : !out ? go(kf_cast_blocks<E, PLAIN, S, false, true>) : go(kf_cast_blocks<E, PLAIN, S, true, true>);
+  };
+  if (rstd) return go(kf_cast_blocks<false, NORMED, false, false, true>);
+  if (square) return e5m2 ? copies(std::true_type{}, std::true_type{}) : copies(std::false_type{}, std::true_type{});
+  return e5m2 ? copies(std::true_type{}, std::false_type{}) : copies(std::false_type{}, std::false_type{});
 }
 
 // t = bf16(x + residual) (x itself, and nothing is written, where residual is null), rstd, and RMSNorm(t) * gain in e4m3.  x, residual, t:
@@ -401,11 +454,10 @@ int kf_fp8_blocks_values_bf16(const void* q, long long ld, const void* scales, l
                               void* stream) {
   using namespace kf::f8b;
   if (rows <= 0 || cols <= 0 || (reinterpret_cast<uintptr_t>(out) & 15)) return 5;
-  const long long n = (long long)rows * ((cols + 7) / 8);
-  if ((n + 255) / 256 > 0x7fffffffLL) return 5;
+  if ((cols + 255) / 256 > 65535) return 5;
   auto kern = e5m2 ? kf_blocks_values<true> : kf_blocks_values<false>;
-  kern<<<unsigned((n + 255) / 256), 256, 0, (cudaStream_t)stream>>>((const uint8_t*)q, ld, (const uint8_t*)scales, ld_scales, rows, cols,
-                                                                    (__nv_bfloat16*)out);
+  kern<<<dim3((rows + 15) / 16, (cols + 255) / 256), 256, 0, (cudaStream_t)stream>>>((const uint8_t*)q, ld, (const uint8_t*)scales, ld_scales, rows,
+                                                                                    cols, (__nv_bfloat16*)out);
   return launched();
 }
 

@@ -44,10 +44,10 @@ __device__ __forceinline__ float inverse_of(uint32_t byte) { return __uint_as_fl
 __device__ __forceinline__ bool is_inf(float v) { return (__float_as_uint(v) & 0x7fffffffu) == 0x7f800000u; }
 __device__ __forceinline__ float nan_if_inf(float v) { return is_inf(v) ? __uint_as_float(0x7fffffffu) : v; }
 
-// two values, scaled, as two bytes: nearest, ties to even
+// two values as two bytes: nearest, ties to even
 template <bool E5M2>
-__device__ __forceinline__ uint32_t to_bytes(float a, float b, float inv) {
-  return (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(mul_full(a, inv), mul_full(b, inv)), __NV_SATFINITE, E5M2 ? __NV_E5M2 : __NV_E4M3);
+__device__ __forceinline__ uint32_t to_bytes(float a, float b) {
+  return (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, E5M2 ? __NV_E5M2 : __NV_E4M3);
 }
 
 // ------------------------------------------------------------------ tcgen05
