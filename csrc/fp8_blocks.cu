@@ -50,6 +50,8 @@ kf_cast_blocks(const __nv_bfloat16* __restrict__ x, int rows, int cols, long lon
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   const int c = c0 + tx * 8;
   const bool wide_in = c + 7 < cols && (ldx & 7) == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0;
+  wait_for_previous();
+  let_next_in();
   uint4 v[PER];
   float s[PER];
 #pragma unroll
@@ -287,6 +289,8 @@ kf_add_rmsnorm_blocks(const __nv_bfloat16* __restrict__ x, const __nv_bfloat16* 
   const size_t row = blockIdx.x;
   const int nvec = D >> 3;
   const __nv_bfloat16* xr = x + row * D;
+  wait_for_previous();
+  let_next_in();
   uint4 v[VPT], rv[VPT];
 #pragma unroll
   for (int c = 0; c < VPT; ++c) {
@@ -318,7 +322,8 @@ kf_add_rmsnorm_blocks(const __nv_bfloat16* __restrict__ x, const __nv_bfloat16* 
       ss += a.y * a.y;
     }
   }
-  const float r = rsqrtf(row_sum(ss, red, THREADS) / D + eps);
+  // both rounded to the nearest: an approximate one sends three times as many values to the other neighbour in the cast
+  const float r = __frsqrt_rn(__fadd_rn(__fdiv_rn(row_sum(ss, red, THREADS), float(D)), eps));
   if (threadIdx.x == 0 && rstd_out) rstd_out[row] = r;
 #pragma unroll
   for (int c = 0; c < VPT; ++c) {
@@ -361,6 +366,8 @@ __global__ void __launch_bounds__(256)
 kf_blocks_values(const uint8_t* __restrict__ q, long long ld, const uint8_t* __restrict__ scales, long long ld_scales, int rows, int cols,
                  __nv_bfloat16* __restrict__ out) {
   const int c = blockIdx.y * 256 + (threadIdx.x & 15) * 16, r = blockIdx.x * 16 + (threadIdx.x >> 4);
+  wait_for_previous();
+  let_next_in();
   if (c >= cols || r >= rows) return;
   const uint8_t* p = q + r * ld + c;
   __nv_bfloat16* o = out + (size_t)r * cols + c;
@@ -393,11 +400,6 @@ kf_blocks_values(const uint8_t* __restrict__ q, long long ld, const uint8_t* __r
   }
 }
 
-static int launched() {
-  const cudaError_t e = cudaGetLastError();
-  return e == cudaSuccess ? 0 : 400 + (int)e;
-}
-
 }  // namespace f8b
 }  // namespace kf
 
@@ -414,10 +416,9 @@ int kf_fp8_blocks_cast_bf16(const void* x, int rows, int cols, long long ldx, co
       (rstd && (square || e5m2 || out)))
     return 5;
   auto go = [&](auto kern) {
-    kern<<<dim3((cols + 127) / 128, (rows + 127) / 128), 512, 0, (cudaStream_t)stream>>>(
-        (const __nv_bfloat16*)x, rows, cols, ldx, (const float*)rstd, (const __nv_bfloat16*)gain, (uint8_t*)out, ld_out, (uint8_t*)scales,
-        ld_scales, (uint8_t*)out_t, ld_t, (uint8_t*)scales_t, ld_scales_t);
-    return launched();
+    return launch_programmatic(kern, dim3((cols + 127) / 128, (rows + 127) / 128), 512, 0, 1, (cudaStream_t)stream, (const __nv_bfloat16*)x, rows, cols,
+                               ldx, (const float*)rstd, (const __nv_bfloat16*)gain, (uint8_t*)out, ld_out, (uint8_t*)scales, ld_scales,
+                               (uint8_t*)out_t, ld_t, (uint8_t*)scales_t, ld_scales_t);
   };
   auto copies = [&](auto e5, auto sq) {
     constexpr bool E = decltype(e5)::value, S = decltype(sq)::value;
@@ -438,9 +439,8 @@ int kf_add_rmsnorm_fp8_blocks(const void* x, const void* residual, const void* g
       (reinterpret_cast<uintptr_t>(out) & 7) || (residual && !t))
     return 5;
   auto go = [&](auto kern, int threads) {
-    kern<<<rows, threads, 0, (cudaStream_t)stream>>>((const __nv_bfloat16*)x, (const __nv_bfloat16*)residual, (const __nv_bfloat16*)gain,
-                                                     (__nv_bfloat16*)t, (float*)rstd, (uint8_t*)out, ld_out, (uint8_t*)scales, ld_scales, D, eps);
-    return launched();
+    return launch_programmatic(kern, dim3(unsigned(rows)), threads, 0, 1, (cudaStream_t)stream, (const __nv_bfloat16*)x, (const __nv_bfloat16*)residual,
+                               (const __nv_bfloat16*)gain, (__nv_bfloat16*)t, (float*)rstd, (uint8_t*)out, ld_out, (uint8_t*)scales, ld_scales, D, eps);
   };
   if (D <= 1024) return go(kf_add_rmsnorm_blocks<32, 4>, 32);
   if (D <= 4096) return go(kf_add_rmsnorm_blocks<128, 4>, 128);
@@ -456,9 +456,8 @@ int kf_fp8_blocks_values_bf16(const void* q, long long ld, const void* scales, l
   if (rows <= 0 || cols <= 0 || (reinterpret_cast<uintptr_t>(out) & 15)) return 5;
   if ((cols + 255) / 256 > 65535) return 5;
   auto kern = e5m2 ? kf_blocks_values<true> : kf_blocks_values<false>;
-  kern<<<dim3((rows + 15) / 16, (cols + 255) / 256), 256, 0, (cudaStream_t)stream>>>((const uint8_t*)q, ld, (const uint8_t*)scales, ld_scales, rows,
-                                                                                    cols, (__nv_bfloat16*)out);
-  return launched();
+  return launch_programmatic(kern, dim3((rows + 15) / 16, (cols + 255) / 256), 256, 0, 1, (cudaStream_t)stream, (const uint8_t*)q, ld,
+                             (const uint8_t*)scales, ld_scales, rows, cols, (__nv_bfloat16*)out);
 }
 
 }  // extern "C"

@@ -50,6 +50,32 @@ __device__ __forceinline__ uint32_t to_bytes(float a, float b) {
   return (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, E5M2 ? __NV_E5M2 : __NV_E4M3);
 }
 
+// ------------------------------------------------------------------ programmatic launches
+// A kernel so launched sets itself up while the one before it drains.  It waits before it reads or writes global memory, and lets the next
+// one in only after that: whatever starts early finds every kernel but its immediate predecessor complete.
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void let_next_in() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+// kernel<<<grid, block, smem, stream>>>(args ..), in clusters of `cluster` blocks, as a programmatic launch
+template <class... P, class... A>
+int launch_programmatic(void (*kernel)(P...), dim3 grid, int block, size_t smem, int cluster, cudaStream_t stream, A&&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(unsigned(block));
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = unsigned(cluster);
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+  return e == cudaSuccess ? 0 : 400 + (int)e;
+}
+
 // ------------------------------------------------------------------ tcgen05
 // Instruction descriptor for kind::mxf8f6f4: formats 0 = e4m3, 1 = e5m2, both K-major, scales as exponent bytes, byte 0 of each word; plus
 // b of them, byte b.

@@ -82,6 +82,8 @@ kf_gemm_fp8_blocks_few(const Args a) {
   const int warp = threadIdx.x >> 5, warps = blockDim.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int n0 = blockIdx.x * ROWS, k_blocks = (a.K + BLOCK - 1) / BLOCK;
   // rows and tokens that do not exist stand for the last one: nobody reads what comes of them
+  wait_for_previous();
+  let_next_in();
   const int row[2] = {min(n0 + g, a.N - 1), min(n0 + 8 + g, a.N - 1)};
   float total[TILES][4] = {};
   uint32_t nan_w[2] = {}, nan_x[TILES] = {};
@@ -178,9 +180,7 @@ template <int TILES>
 static int launch(const Args& a, int a_fmt, int b_fmt, int warps, cudaStream_t stream) {
   auto kern = b_fmt ? (a_fmt ? kf_gemm_fp8_blocks_few<TILES, true, true> : kf_gemm_fp8_blocks_few<TILES, true, false>)
                     : (a_fmt ? kf_gemm_fp8_blocks_few<TILES, false, true> : kf_gemm_fp8_blocks_few<TILES, false, false>);
-  kern<<<(a.N + ROWS - 1) / ROWS, 32 * warps, 0, stream>>>(a);
-  const cudaError_t e = cudaGetLastError();
-  return e == cudaSuccess ? 0 : 400 + (int)e;
+  return launch_programmatic(kern, dim3((a.N + ROWS - 1) / ROWS), 32 * warps, 0, 1, stream, a);
 }
 
 }  // namespace few

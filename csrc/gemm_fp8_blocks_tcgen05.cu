@@ -250,6 +250,8 @@ kf_gemm_fp8_blocks_2cta(const __grid_constant__ CUtensorMap map_a, const __grid_
   cluster_sync_all();  // both CTAs' barriers exist before anyone signals across the pair
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot_ptr;
+  wait_for_previous();
+  let_next_in();
 
   const int quarter = warp & 3;
   const uint32_t box = box_smem + uint32_t((warp - 6) & 3) * BOX_BYTES, t_row = tmem_base + (uint32_t(quarter * 32) << 16);
@@ -538,20 +540,9 @@ int kf_gemm_fp8_blocks(const void* A, const void* sa, const void* B, const void*
     if (dev < 64) attr_set[dev] = true;
   }
   const int clusters = cut.splits > 1 ? (int)tiles : (int)(tiles < num_sms / 2 ? tiles : num_sms / 2);
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(unsigned(clusters * 2 * cut.splits));
-  cfg.blockDim = dim3(THREADS);
-  cfg.dynamicSmemBytes = SMEM;
-  cfg.stream = (cudaStream_t)stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = unsigned(2 * cut.splits);
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
   const Output out{reinterpret_cast<__nv_bfloat16*>(C), ldc, cut.turned, accumulate, wide};
-  cudaError_t e = cudaLaunchKernelEx(&cfg, kf_gemm_fp8_blocks_2cta, ma, mb, msa, msb, out, M, N, K, a_fmt, b_fmt, tile_n, status);
-  return e == cudaSuccess ? 0 : 400 + (int)e;
+  return launch_programmatic(kf_gemm_fp8_blocks_2cta, dim3(unsigned(clusters * 2 * cut.splits)), THREADS, SMEM, 2 * cut.splits, (cudaStream_t)stream,
+                             ma, mb, msa, msb, out, M, N, K, a_fmt, b_fmt, tile_n, status);
 }
 
 }  // extern "C"
