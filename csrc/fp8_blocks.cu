@@ -3,7 +3,11 @@
 //
 //   cast    q = round8(x 2^-e), e from the largest magnitude of a block: 1 x 128 (activations, gradients) or 128 x 128 (weights, whose two
 //           copies then hold the same values).  A transposed copy of 1 x 128 blocks has blocks of 128 along the rows of x.
-//   norm    t = bf16(x + residual), rstd = 1 / sqrt(mean(t^2) + eps), h = cast(t rstd gain), the products in 32 bits
+//   norm    t = bf16(x + residual), rstd = 1 / sqrt(mean(t^2) + eps), h = cast(t gain rstd), the products in 32 bits
+//   norm's gradients  dx = dt + rstd (dh gain - t rstd^2 mean(dh gain t)), dgain = sum over rows of dh t rstd, of dh in 32 bits
+//
+// The kernels are programmatic launches, so no pointer is promised to be the only one to its memory: a load under that promise may be moved
+// before the wait for the kernel that writes it.
 //
 // An infinity or a NaN is stored as NaN, and the other values of its block are scaled as if it were not there.
 #include "fp8_blocks.cuh"
@@ -37,9 +41,9 @@ __device__ __forceinline__ uint32_t max_abs2(uint32_t m, uint32_t v) {
 // squares both 49 (41), normed 54 (31); with 256 threads, two blocks on an SM and a look at each value for infinities 60, 68, 84, 59 and 128.
 template <bool E5M2, int SRC, bool SQUARE, bool ROW, bool T>
 __global__ void __launch_bounds__(512, ROW && !T ? 4 : SRC == NORMED ? 2 : 3)
-kf_cast_blocks(const __nv_bfloat16* __restrict__ x, int rows, int cols, long long ldx, const float* __restrict__ rstd,
-               const __nv_bfloat16* __restrict__ gain, uint8_t* __restrict__ out, long long ld_out, uint8_t* __restrict__ scales,
-               long long ld_scales, uint8_t* __restrict__ out_t, long long ld_t, uint8_t* __restrict__ scales_t, long long ld_scales_t) {
+kf_cast_blocks(const __nv_bfloat16* x, int rows, int cols, long long ldx, const float* rstd,
+               const __nv_bfloat16* gain, uint8_t* out, long long ld_out, uint8_t* scales,
+               long long ld_scales, uint8_t* out_t, long long ld_t, uint8_t* scales_t, long long ld_scales_t) {
   constexpr int PER = 4;  // rows of a thread
   __shared__ uint32_t tile[T ? 128 : 1][32];               // bytes of the tile on their way to the transposed copy
   __shared__ float part[T && !SQUARE ? 16 : 1][128];       // column maxima of each warp
@@ -80,7 +84,7 @@ kf_cast_blocks(const __nv_bfloat16* __restrict__ x, int rows, int cols, long lon
   // two neighbouring values, as the norm kernel forms them
   auto value2 = [&](int i, int j) {
     float2 p = pair_at(v[i], j);
-    if (SRC == NORMED) p = make_float2(mul_full(mul_full(p.x, s[i]), g[2 * j]), mul_full(mul_full(p.y, s[i]), g[2 * j + 1]));
+    if (SRC == NORMED) p = make_float2(mul_full(mul_full(p.x, g[2 * j]), s[i]), mul_full(mul_full(p.y, g[2 * j + 1]), s[i]));
     return p;
   };
   // maxima of the thread's part of each row, and of its columns
@@ -267,14 +271,17 @@ kf_cast_blocks(const __nv_bfloat16* __restrict__ x, int rows, int cols, long lon
   }
 }
 
-__device__ __forceinline__ float row_sum(float v, float* red, int threads) {
+// Sum over the threads of a block, in T; `red` is free again for the block after the next barrier.
+template <int THREADS, class T>
+__device__ __forceinline__ T block_sum(T v, T* red) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  if (threads <= 32) return v;
+  if (THREADS <= 32) return v;
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
   __syncthreads();
-  v = 0.f;
-  for (int w = 0; w < threads / 32; ++w) v += red[w];
+  v = 0;
+#pragma unroll
+  for (int w = 0; w < THREADS / 32; ++w) v += red[w];
   return v;
 }
 
@@ -282,10 +289,10 @@ __device__ __forceinline__ float row_sum(float v, float* red, int threads) {
 // of 128 columns between them.  Vector c of a thread is c * THREADS + thread.
 template <int THREADS, int VPT>
 __global__ void __launch_bounds__(THREADS)
-kf_add_rmsnorm_blocks(const __nv_bfloat16* __restrict__ x, const __nv_bfloat16* __restrict__ residual, const __nv_bfloat16* __restrict__ gain,
-                      __nv_bfloat16* __restrict__ t_out, float* __restrict__ rstd_out, uint8_t* __restrict__ out, long long ld_out,
-                      uint8_t* __restrict__ scales, long long ld_scales, int D, float eps) {
-  __shared__ float red[32];
+kf_add_rmsnorm_blocks(const __nv_bfloat16* x, const __nv_bfloat16* residual, const __nv_bfloat16* gain,
+                      __nv_bfloat16* t_out, float* rstd_out, uint8_t* out, long long ld_out,
+                      uint8_t* scales, long long ld_scales, int D, float eps) {
+  __shared__ double red[32];
   const size_t row = blockIdx.x;
   const int nvec = D >> 3;
   const __nv_bfloat16* xr = x + row * D;
@@ -322,8 +329,9 @@ kf_add_rmsnorm_blocks(const __nv_bfloat16* __restrict__ x, const __nv_bfloat16* 
       ss += a.y * a.y;
     }
   }
-  // both rounded to the nearest: an approximate one sends three times as many values to the other neighbour in the cast
-  const float r = __frsqrt_rn(__fadd_rn(__fdiv_rn(row_sum(ss, red, THREADS), float(D)), eps));
+  // What the 24th bit of rstd says decides, next to a border, which of two 8-bit neighbours all values of a row go to: threads' sums are added
+  // in 64 bits, and division and root are those that round to the nearest.
+  const float r = __frsqrt_rn(__fadd_rn(__fdiv_rn(float(block_sum<THREADS>(double(ss), red)), float(D)), eps));
   if (threadIdx.x == 0 && rstd_out) rstd_out[row] = r;
 #pragma unroll
   for (int c = 0; c < VPT; ++c) {
@@ -333,8 +341,8 @@ kf_add_rmsnorm_blocks(const __nv_bfloat16* __restrict__ x, const __nv_bfloat16* 
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const float2 a = pair_at(v[c], j), g = pair_at(gv, j);
-      f[2 * j] = mul_full(mul_full(a.x, r), g.x);
-      f[2 * j + 1] = mul_full(mul_full(a.y, r), g.y);
+      f[2 * j] = mul_full(mul_full(a.x, g.x), r);  // the first product is exact: 16 bits
+      f[2 * j + 1] = mul_full(mul_full(a.y, g.y), r);
       m = max_abs(max_abs(m, f[2 * j]), f[2 * j + 1]);
     }
     m = half_warp_max(m);
@@ -360,11 +368,98 @@ kf_add_rmsnorm_blocks(const __nv_bfloat16* __restrict__ x, const __nv_bfloat16* 
   }
 }
 
+// Gradients of RMSNorm from dh in 32 bits, one pass: a block walks over rows, keeps its columns' part of the gain's gradient in registers and
+// leaves it in partial[block][column] for kf_column_sums.  dh as a product leaves it, unrounded: rounded to 16 bits on the way it moves the
+// gain's gradient, a sum over thousands of rows that cancel, by as much as the gradient's own rounding does.
+template <int THREADS, int VPT>
+__global__ void __launch_bounds__(THREADS)
+kf_norm_grads(const float* dh, const __nv_bfloat16* t, const __nv_bfloat16* gain, const float* rstd, const __nv_bfloat16* dt, __nv_bfloat16* dx,
+              float* partial, int rows, int D) {
+  __shared__ float red[2][32];
+  const int nvec = D >> 3;
+  wait_for_previous();
+  let_next_in();
+  float sum[VPT][8] = {};
+  int turn = 0;
+  for (int row = blockIdx.x; row < rows; row += gridDim.x, turn ^= 1) {
+    const size_t at = size_t(row) * D;
+    float4 a[VPT][2];
+    uint4 tv[VPT], iv[VPT], gv[VPT];
+#pragma unroll
+    for (int c = 0; c < VPT; ++c) {
+      const int i = threadIdx.x + c * THREADS;
+      a[c][0] = a[c][1] = make_float4(0.f, 0.f, 0.f, 0.f);
+      tv[c] = iv[c] = gv[c] = make_uint4(0, 0, 0, 0);
+      if (i < nvec) {
+        a[c][0] = *reinterpret_cast<const float4*>(dh + at + i * 8);
+        a[c][1] = *reinterpret_cast<const float4*>(dh + at + i * 8 + 4);
+        tv[c] = *reinterpret_cast<const uint4*>(t + at + i * 8);
+        if (dt) iv[c] = *reinterpret_cast<const uint4*>(dt + at + i * 8);
+        gv[c] = *reinterpret_cast<const uint4*>(gain + i * 8);
+      }
+    }
+    const float r = rstd[row];
+    float dot = 0.f;
+#pragma unroll
+    for (int c = 0; c < VPT; ++c) {
+      const float d[8] = {a[c][0].x, a[c][0].y, a[c][0].z, a[c][0].w, a[c][1].x, a[c][1].y, a[c][1].z, a[c][1].w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 x = pair_at(tv[c], j), g = pair_at(gv[c], j);
+        dot += d[2 * j] * (g.x * x.x);
+        dot += d[2 * j + 1] * (g.y * x.y);
+        sum[c][2 * j] += d[2 * j] * (x.x * r);
+        sum[c][2 * j + 1] += d[2 * j + 1] * (x.y * r);
+      }
+    }
+    const float coef = block_sum<THREADS>(dot, red[turn]) / float(D) * r * r * r;
+#pragma unroll
+    for (int c = 0; c < VPT; ++c) {
+      const int i = threadIdx.x + c * THREADS;
+      const float d[8] = {a[c][0].x, a[c][0].y, a[c][0].z, a[c][0].w, a[c][1].x, a[c][1].y, a[c][1].z, a[c][1].w};
+      uint32_t w[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 x = pair_at(tv[c], j), g = pair_at(gv[c], j), in = pair_at(iv[c], j);
+        w[j] = pack_bf16(in.x + (r * (d[2 * j] * g.x) - x.x * coef), in.y + (r * (d[2 * j + 1] * g.y) - x.y * coef));
+      }
+      if (i < nvec) *reinterpret_cast<uint4*>(dx + at + i * 8) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < VPT; ++c) {
+    const int i = threadIdx.x + c * THREADS;
+    if (i < nvec) {
+      float* p = partial + size_t(blockIdx.x) * D + i * 8;
+      *reinterpret_cast<float4*>(p) = make_float4(sum[c][0], sum[c][1], sum[c][2], sum[c][3]);
+      *reinterpret_cast<float4*>(p + 4) = make_float4(sum[c][4], sum[c][5], sum[c][6], sum[c][7]);
+    }
+  }
+}
+
+// out[column] = sum over parts of partial[part][column], 32 columns per block and every eighth part per warp, in a fixed order
+__global__ void __launch_bounds__(256) kf_column_sums(const float* partial, int parts, int D, __nv_bfloat16* out) {
+  __shared__ float red[8][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
+  wait_for_previous();
+  let_next_in();
+  float v = 0.f;
+  if (c < D)
+    for (int p = warp; p < parts; p += 8) v += partial[size_t(p) * D + c];
+  red[warp][lane] = v;
+  __syncthreads();
+  if (warp == 0 && c < D) {
+#pragma unroll
+    for (int w = 1; w < 8; ++w) v += red[w][lane];
+    out[c] = __float2bfloat16(v);
+  }
+}
+
 // The values that the bytes stand for, in bf16 (exact where bf16 has them): sixteen per thread, blocks of 16 x 16 threads on 256 columns.
 template <bool E5M2>
 __global__ void __launch_bounds__(256)
-kf_blocks_values(const uint8_t* __restrict__ q, long long ld, const uint8_t* __restrict__ scales, long long ld_scales, int rows, int cols,
-                 __nv_bfloat16* __restrict__ out) {
+kf_blocks_values(const uint8_t* q, long long ld, const uint8_t* scales, long long ld_scales, int rows, int cols,
+                 __nv_bfloat16* out) {
   const int c = blockIdx.y * 256 + (threadIdx.x & 15) * 16, r = blockIdx.x * 16 + (threadIdx.x >> 4);
   wait_for_previous();
   let_next_in();
@@ -447,6 +542,32 @@ int kf_add_rmsnorm_fp8_blocks(const void* x, const void* residual, const void* g
   if (D <= 8192) return go(kf_add_rmsnorm_blocks<256, 4>, 256);
   if (D <= 16384) return go(kf_add_rmsnorm_blocks<512, 4>, 512);
   return go(kf_add_rmsnorm_blocks<1024, 4>, 1024);
+}
+
+// Blocks of kf_norm_grads_f32, each of which leaves D floats in `partial`.
+int kf_norm_grads_blocks(int rows, int D, int num_sms) {
+  const int per_sm = D <= 1024 ? 16 : D <= 4096 ? 4 : 2;
+  return rows < num_sms * per_sm ? (rows < 1 ? 1 : rows) : num_sms * per_sm;
+}
+
+// dx (bf16) = dt (or 0 where null) + the gradient of RMSNorm at t for dh (fp32); dgain (bf16) of its gain.  Contiguous rows on 16 bytes, D a
+// multiple of 8, at most 8192.
+int kf_norm_grads_f32(const void* dh, const void* t, const void* gain, const void* rstd, const void* dt, void* dx, void* partial, void* dgain, int rows,
+                      int D, int num_sms, void* stream) {
+  using namespace kf::f8b;
+  if (rows <= 0 || D <= 0 || (D & 7) || D > 8192 ||
+      ((reinterpret_cast<uintptr_t>(dh) | reinterpret_cast<uintptr_t>(t) | reinterpret_cast<uintptr_t>(gain) | reinterpret_cast<uintptr_t>(dt) |
+        reinterpret_cast<uintptr_t>(dx) | reinterpret_cast<uintptr_t>(partial)) & 15))
+    return 5;
+  const int blocks = kf_norm_grads_blocks(rows, D, num_sms);
+  cudaStream_t st = (cudaStream_t)stream;
+  auto go = [&](auto kern, int threads) {
+    return launch_programmatic(kern, dim3(unsigned(blocks)), threads, 0, 1, st, (const float*)dh, (const __nv_bfloat16*)t, (const __nv_bfloat16*)gain,
+                               (const float*)rstd, (const __nv_bfloat16*)dt, (__nv_bfloat16*)dx, (float*)partial, rows, D);
+  };
+  const int rc = D <= 1024 ? go(kf_norm_grads<32, 4>, 32) : D <= 4096 ? go(kf_norm_grads<256, 2>, 256) : go(kf_norm_grads<512, 2>, 512);
+  if (rc) return rc;
+  return launch_programmatic(kf_column_sums, dim3((D + 31) / 32), 256, 0, 1, st, (const float*)partial, blocks, D, (__nv_bfloat16*)dgain);
 }
 
 // out[rows][cols] (contiguous bf16) = the values that q (pitch ld) and its scale bytes stand for.

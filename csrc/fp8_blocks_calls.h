@@ -11,13 +11,13 @@ namespace {
 
 struct Fp8Blocks {
   int (*gemm)(const void*, const void*, const void*, const void*, void*, int, int, int, long long, long long, long long, long long, long long, int,
-              int, int, int, void*) = nullptr;
+              int, int, int, int, void*) = nullptr;
   int (*norm)(const void*, const void*, const void*, void*, void*, void*, long long, void*, long long, int, int, float, void*) = nullptr;
   int (*cast)(const void*, int, int, long long, const void*, const void*, int, int, void*, long long, void*, long long, void*, long long, void*,
               long long, void*) = nullptr;
   int (*values)(const void*, long long, const void*, long long, int, int, int, void*, void*) = nullptr;
-  int (*norm_bwd)(const void*, const void*, const void*, const void*, void*, void*, void*, void*, int, int, const void*, void*) = nullptr;
-  int (*norm_bwd_blocks)(int) = nullptr;
+  int (*norm_grads)(const void*, const void*, const void*, const void*, const void*, void*, void*, void*, int, int, int, void*) = nullptr;
+  int (*norm_grads_blocks)(int, int, int) = nullptr;
 } f8;
 
 constexpr long long kLargest = 0x7fffffff;
@@ -70,27 +70,28 @@ struct Buffers {
         scales(at::empty_strided({(cols + 127) / 128, rows}, {(rows + 15) / 16 * 16, 1}, o)) {}
 };
 
-// fp8_mm(a values, a scales, a e5m2, b values, b scales, b e5m2, out or None, accumulate, sms, device, stream) -> out, bf16 (M, N)
+// fp8_mm(a values, a scales, a e5m2, b values, b scales, b e5m2, out or None, accumulate, f32, sms, device, stream) -> out (M, N), bf16 or fp32
 PyObject* fp8_mm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   long device = 0;
   void* stream = nullptr;
-  if (nargs != 11 || !f8.gemm || !where(args + 9, &device, &stream)) return PyErr_Occurred() ? nullptr : Py_NewRef(Py_None);
-  const long sms = PyLong_AsLong(args[8]);
+  if (nargs != 12 || !f8.gemm || !where(args + 10, &device, &stream)) return PyErr_Occurred() ? nullptr : Py_NewRef(Py_None);
+  const long sms = PyLong_AsLong(args[9]);
   if (PyErr_Occurred()) return nullptr;
   const at::Tensor *qa, *sa, *qb, *sb;
-  int ea = 0, eb = 0, accumulate = 0;
+  int ea = 0, eb = 0, accumulate = 0, f32 = 0;
   if (!operand(args[0], args[1], device, qa, sa) || !operand(args[3], args[4], device, qb, sb) || qa->size(1) != qb->size(1) ||
-      !flag(args[2], &ea) || !flag(args[5], &eb) || !flag(args[7], &accumulate))
+      !flag(args[2], &ea) || !flag(args[5], &eb) || !flag(args[7], &accumulate) || !flag(args[8], &f32))
     Py_RETURN_NONE;
-  const at::Tensor* to = args[6] == Py_None ? nullptr : dense(args[6], at::kBFloat16, 2, device);
+  const at::ScalarType type = f32 ? at::kFloat : at::kBFloat16;
+  const at::Tensor* to = args[6] == Py_None ? nullptr : dense(args[6], type, 2, device);
   if (args[6] == Py_None ? accumulate != 0
                          : !to || to->size(0) != qa->size(0) || to->size(1) != qb->size(0) || to->stride(1) != 1 || to->stride(0) < to->size(1))
     Py_RETURN_NONE;
   HANDLE_TH_ERRORS
-  at::Tensor out = to ? *to : at::empty({qa->size(0), qb->size(0)}, qa->options().dtype(at::kBFloat16));
+  at::Tensor out = to ? *to : at::empty({qa->size(0), qb->size(0)}, qa->options().dtype(type));
   const int rc = issued([&] {
     return f8.gemm(qa->const_data_ptr(), sa->const_data_ptr(), qb->const_data_ptr(), sb->const_data_ptr(), at_(out), int(qa->size(0)), int(qb->size(0)),
-                   int(qa->size(1)), qa->stride(0), sa->stride(0), qb->stride(0), sb->stride(0), out.stride(0), ea, eb, accumulate, int(sms), stream);
+                   int(qa->size(1)), qa->stride(0), sa->stride(0), qb->stride(0), sb->stride(0), out.stride(0), f32, ea, eb, accumulate, int(sms), stream);
   });
   return rc ? PyLong_FromLong(rc) : to ? Py_NewRef(args[6]) : THPVariable_Wrap(std::move(out));
   END_HANDLE_TH_ERRORS
@@ -178,43 +179,45 @@ PyObject* fp8_values(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
-// norm_grads(dh, t, gain, rstd, dt or None, device, stream) -> (dt + RMSNorm'(dh), gradient of the gain), both bf16
+// norm_grads(dh (fp32), t, gain, rstd, dt or None, sms, device, stream) -> (dt + RMSNorm'(dh), gradient of the gain), both bf16
 PyObject* norm_grads(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   long device = 0;
   void* stream = nullptr;
-  if (nargs != 7 || !f8.norm_bwd || !where(args + 5, &device, &stream)) return PyErr_Occurred() ? nullptr : Py_NewRef(Py_None);
+  if (nargs != 8 || !f8.norm_grads || !where(args + 6, &device, &stream)) return PyErr_Occurred() ? nullptr : Py_NewRef(Py_None);
+  const long sms = PyLong_AsLong(args[5]);
+  if (PyErr_Occurred()) return nullptr;
   const bool add = args[4] != Py_None;
-  const at::Tensor *dh = dense(args[0], at::kBFloat16, 2, device), *t = dense(args[1], at::kBFloat16, 2, device);
+  const at::Tensor *dh = dense(args[0], at::kFloat, 2, device), *t = dense(args[1], at::kBFloat16, 2, device);
   const at::Tensor *gain = dense(args[2], at::kBFloat16, 1, device), *rstd = dense(args[3], at::kFloat, 1, device);
   const at::Tensor* dt = add ? dense(args[4], at::kBFloat16, 2, device) : nullptr;
   if (!dh || !t || !gain || !rstd || (add && !dt)) Py_RETURN_NONE;
   const int64_t rows = t->size(0), d = t->size(1);
-  if (rows < 1 || rows > kLargest || d < 8 || d % 8 || d > 32768 || dh->sizes() != t->sizes() || gain->size(0) != d || rstd->size(0) != rows ||
+  if (rows < 1 || rows > kLargest || d < 8 || d % 8 || d > 8192 || dh->sizes() != t->sizes() || gain->size(0) != d || rstd->size(0) != rows ||
       !dh->is_contiguous() || !t->is_contiguous() || !gain->is_contiguous() || !rstd->is_contiguous() || !address(*dh) || !address(*t) ||
       !address(*gain) || (add && (dt->sizes() != t->sizes() || !dt->is_contiguous() || !address(*dt))))
     Py_RETURN_NONE;
   HANDLE_TH_ERRORS
-  at::Tensor partial = at::empty({f8.norm_bwd_blocks(int(rows)) * d}, rstd->options()), dx = at::empty({rows, d}, t->options());
+  at::Tensor partial = at::empty({f8.norm_grads_blocks(int(rows), int(d), int(sms)), d}, rstd->options()), dx = at::empty({rows, d}, t->options());
   at::Tensor dgain = at::empty({d}, t->options());
   const int rc = issued([&] {
-    return f8.norm_bwd(dh->const_data_ptr(), t->const_data_ptr(), gain->const_data_ptr(), rstd->const_data_ptr(), at_(dx), at_(partial), at_(dgain),
-                       nullptr, int(rows), int(d), add ? dt->const_data_ptr() : nullptr, stream);
+    return f8.norm_grads(dh->const_data_ptr(), t->const_data_ptr(), gain->const_data_ptr(), rstd->const_data_ptr(), add ? dt->const_data_ptr() : nullptr,
+                         at_(dx), at_(partial), at_(dgain), int(rows), int(d), int(sms), stream);
   });
   return rc ? PyLong_FromLong(rc) : Py_BuildValue("(NN)", THPVariable_Wrap(std::move(dx)), THPVariable_Wrap(std::move(dgain)));
   END_HANDLE_TH_ERRORS
 }
 
 // fp8_configure(addresses of kf_gemm_fp8_blocks, kf_add_rmsnorm_fp8_blocks, kf_fp8_blocks_cast_bf16, kf_fp8_blocks_values_bf16,
-// kf_rmsnorm_bwd_bf16, kf_rmsnorm_bwd_blocks)
+// kf_norm_grads_f32, kf_norm_grads_blocks)
 PyObject* fp8_configure(PyObject*, PyObject* args) {
-  unsigned long long gemm = 0, norm = 0, cast = 0, values = 0, bwd = 0, bwd_blocks = 0;
-  if (!PyArg_ParseTuple(args, "KKKKKK", &gemm, &norm, &cast, &values, &bwd, &bwd_blocks)) return nullptr;
-  f8.norm_bwd = reinterpret_cast<decltype(f8.norm_bwd)>(bwd);
-  f8.norm_bwd_blocks = reinterpret_cast<decltype(f8.norm_bwd_blocks)>(bwd_blocks);
+  unsigned long long gemm = 0, norm = 0, cast = 0, values = 0, grads = 0, grads_blocks = 0;
+  if (!PyArg_ParseTuple(args, "KKKKKK", &gemm, &norm, &cast, &values, &grads, &grads_blocks)) return nullptr;
   f8.gemm = reinterpret_cast<decltype(f8.gemm)>(gemm);
   f8.norm = reinterpret_cast<decltype(f8.norm)>(norm);
   f8.cast = reinterpret_cast<decltype(f8.cast)>(cast);
   f8.values = reinterpret_cast<decltype(f8.values)>(values);
+  f8.norm_grads = reinterpret_cast<decltype(f8.norm_grads)>(grads);
+  f8.norm_grads_blocks = reinterpret_cast<decltype(f8.norm_grads_blocks)>(grads_blocks);
   Py_RETURN_NONE;
 }
 

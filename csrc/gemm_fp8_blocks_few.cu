@@ -25,14 +25,18 @@ constexpr int MAX_TOKENS = 16;
 struct Args {
   const uint8_t *x, *w, *sx, *sw;
   long long ldx, ldw, ldsx, ldsw;
-  __nv_bfloat16* out;
+  void* out;
   long long ldo;
-  int M, N, K, accumulate;
+  int M, N, K, f32, accumulate;
 };
 
-// factor of a scale byte: 2^(b - 127), NaN for 255
-__device__ __forceinline__ float factor(uint32_t b) {
-  return b == 0 ? __uint_as_float(0x400000u) : b == 255 ? __uint_as_float(0x7fffffffu) : __uint_as_float(b << 23);
+// v 2^(a + b - 254 + UP), NaN where a scale byte is 255: by two factors of half the exponent, since one of 2^(a - 127) could send beyond the range
+// what the other brings back.  (A sum below -252, whose factors have no normal number, leaves nothing of a block's sum of at most 2^33.)
+template <int UP>
+__device__ __forceinline__ float scaled(float v, uint32_t a, uint32_t b) {
+  const int e = int(a + b) - 254 + UP, h = e >> 1;
+  const float lo = __uint_as_float(uint32_t(max(h + 127, 0)) << 23), hi = __uint_as_float(uint32_t(max(e - h + 127, 0)) << 23);
+  return a == 255 || b == 255 ? __uint_as_float(0x7fffffffu) : mul_full(mul_full(v, lo), hi);
 }
 
 __device__ __forceinline__ void mma16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -61,10 +65,10 @@ __device__ __forceinline__ uint32_t word(const uint4& v, int i) { return i == 0 
 
 // 16 bytes of a row at column k; LAST: zeros past K
 template <bool LAST>
-__device__ __forceinline__ uint4 piece(const uint8_t* __restrict__ row, int k, int K) {
-  if (!LAST) return __ldg(reinterpret_cast<const uint4*>(row + k));
+__device__ __forceinline__ uint4 piece(const uint8_t* row, int k, int K) {
+  if (!LAST) return *reinterpret_cast<const uint4*>(row + k);
   if (k >= K) return make_uint4(0, 0, 0, 0);
-  const uint4 v = __ldg(reinterpret_cast<const uint4*>(row + k));
+  const uint4 v = *reinterpret_cast<const uint4*>(row + k);
   uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -92,7 +96,7 @@ kf_gemm_fp8_blocks_few(const Args a) {
     constexpr bool LAST = decltype(last)::value;
     const int k = kb * BLOCK + t * 16;
     uint4 wv[2][2], xv[TILES][2];  // [row g or g + 8][half of the block]
-    float fw[2], fx[TILES][2];
+    uint32_t sw[2], sx[TILES][2];
 #pragma unroll
     for (int r = 0; r < 2; ++r)
 #pragma unroll
@@ -103,10 +107,10 @@ kf_gemm_fp8_blocks_few(const Args a) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) xv[i][h] = piece<LAST>(a.x + m * a.ldx, k + 64 * h, a.K);
 #pragma unroll
-      for (int e = 0; e < 2; ++e) fx[i][e] = factor(__ldg(a.sx + kb * a.ldsx + min(c + e, a.M - 1)));
+      for (int e = 0; e < 2; ++e) sx[i][e] = a.sx[kb * a.ldsx + min(c + e, a.M - 1)];
     }
 #pragma unroll
-    for (int r = 0; r < 2; ++r) fw[r] = factor(__ldg(a.sw + kb * a.ldsw + row[r]));
+    for (int r = 0; r < 2; ++r) sw[r] = a.sw[kb * a.ldsw + row[r]];
     float d[TILES][4] = {};
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -127,11 +131,11 @@ kf_gemm_fp8_blocks_few(const Args a) {
         }
       }
     }
-    constexpr float up = (W5 ? 1.f : 256.f) * (X5 ? 1.f : 256.f);  // what moving the bytes took away
+    constexpr int UP = (W5 ? 0 : 8) + (X5 ? 0 : 8);  // what moving the bytes took away
 #pragma unroll
     for (int i = 0; i < TILES; ++i)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) total[i][e] += mul_full(mul_full(d[i][e] * up, fw[e >> 1]), fx[i][e & 1]);
+      for (int e = 0; e < 4; ++e) total[i][e] = add_full(total[i][e], scaled<UP>(d[i][e], sw[e >> 1], sx[i][e & 1]));
   };
   const int whole = a.K / BLOCK;
   int kb = warp;
@@ -171,8 +175,13 @@ kf_gemm_fp8_blocks_few(const Args a) {
     if (m >= a.M || n >= a.N) continue;
     float v = 0.f;
     for (int w = 0; w < warps; ++w) v += red[w][i];
-    __nv_bfloat16* p = a.out + m * a.ldo + n;
-    *p = __float2bfloat16(a.accumulate ? v + __bfloat162float(*p) : v);
+    if (a.f32) {
+      float* p = static_cast<float*>(a.out) + m * a.ldo + n;
+      *p = a.accumulate ? v + *p : v;
+    } else {
+      __nv_bfloat16* p = static_cast<__nv_bfloat16*>(a.out) + m * a.ldo + n;
+      *p = __float2bfloat16(a.accumulate ? v + __bfloat162float(*p) : v);
+    }
   }
 }
 
@@ -192,9 +201,9 @@ bool few_serves(int M, int N, int K) { return M <= few::MAX_TOKENS && (long long
 
 // The call of kf_gemm_fp8_blocks that few_serves.
 int gemm_blocks_few(const void* A, const void* sa, const void* B, const void* sb, void* C, int M, int N, int K, long long lda, long long ldsa,
-                    long long ldb, long long ldsb, long long ldc, int a_fmt, int b_fmt, int accumulate, int num_sms, void* stream) {
-  const few::Args a{(const uint8_t*)A, (const uint8_t*)B, (const uint8_t*)sa, (const uint8_t*)sb, lda, ldb, ldsa, ldsb, (__nv_bfloat16*)C, ldc, M, N, K,
-                    accumulate};
+                    long long ldb, long long ldsb, long long ldc, int f32, int a_fmt, int b_fmt, int accumulate, int num_sms, void* stream) {
+  const few::Args a{(const uint8_t*)A, (const uint8_t*)B, (const uint8_t*)sa, (const uint8_t*)sb, lda, ldb, ldsa, ldsb, C, ldc, M, N, K,
+                    f32, accumulate};
   if (((reinterpret_cast<uintptr_t>(A) | reinterpret_cast<uintptr_t>(B)) & 15) != 0) return 5;
   const int k_blocks = (K + BLOCK - 1) / BLOCK;
   int warps = (N + few::ROWS - 1) / few::ROWS <= num_sms ? 16 : 8;  // 2048 x 2048, 8 tokens 4.4 / 4.9 us; 4096 x 4096, one token 10.6 / 9.1

@@ -122,12 +122,29 @@ __device__ __forceinline__ unsigned short lds_u16(uint32_t addr) {
 // Where a product goes: C[row * ld + column], or with `turned` (A's rows are C's columns) C[column * ld + row].
 struct Output {
   __nv_bfloat16* C;
+  float* F;  // C in 32 bits instead, or null
   long long ld;
   int turned, accumulate;
   bool wide;  // rows of C start on 16 bytes and hold a multiple of eight values
 
   // 32 x 32 values of a warp at (row0, col0), a row per lane, of which rows x cols exist; box: 2 KB of the warp's own
   __device__ __forceinline__ void put(uint32_t box, int lane, const uint32_t (&v)[32], int row0, int col0, int rows, int cols) const {
+    if (F) {
+      float* dst = F + (turned ? (long long)col0 * ld + row0 + lane : (long long)(row0 + lane) * ld + col0);
+      const long long step = turned ? ld : 1;
+      if (lane < rows) {
+        if (wide && !turned && !accumulate) {
+#pragma unroll
+          for (int q = 0; q < 8; ++q)
+            if (4 * q < cols) *reinterpret_cast<uint4*>(dst + 4 * q) = make_uint4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (i < cols) dst[i * step] = accumulate ? dst[i * step] + __uint_as_float(v[i]) : __uint_as_float(v[i]);
+        }
+      }
+      return;
+    }
     if (turned) {
       __nv_bfloat16* dst = C + (long long)col0 * ld + row0;
       if (wide && !accumulate) {
@@ -494,7 +511,7 @@ static Cut cut_of(int M, int N, int K, int num_sms) {
 // gemm_fp8_blocks_few.cu
 bool few_serves(int M, int N, int K);
 int gemm_blocks_few(const void* A, const void* sa, const void* B, const void* sb, void* C, int M, int N, int K, long long lda, long long ldsa,
-                    long long ldb, long long ldsb, long long ldc, int a_fmt, int b_fmt, int accumulate, int num_sms, void* stream);
+                    long long ldb, long long ldsb, long long ldc, int f32, int a_fmt, int b_fmt, int accumulate, int num_sms, void* stream);
 
 }  // namespace f8b
 }  // namespace kf
@@ -504,14 +521,14 @@ extern "C" void* kf_status_device_ptr();
 extern "C" {
 
 // C[M,N] (+)= A8[M,K] B8[N,K]^T with the scales of blocks of 128 along K: sa (ceil(K / 128), M), sb (ceil(K / 128), N) bytes.  Pitches
-// lda, ldb, ldsa, ldsb in bytes, multiples of 16 (bases too), ldc in elements.  a_fmt / b_fmt: 0 = e4m3, 1 = e5m2.
+// lda, ldb, ldsa, ldsb in bytes, multiples of 16 (bases too), ldc in elements.  C is bf16, or fp32 with f32.  a_fmt / b_fmt: 0 = e4m3, 1 = e5m2.
 int kf_gemm_fp8_blocks(const void* A, const void* sa, const void* B, const void* sb, void* C, int M, int N, int K, long long lda,
-                       long long ldsa, long long ldb, long long ldsb, long long ldc, int a_fmt, int b_fmt, int accumulate, int num_sms,
-                       void* stream) {
+                       long long ldsa, long long ldb, long long ldsb, long long ldc, int f32, int a_fmt, int b_fmt, int accumulate,
+                       int num_sms, void* stream) {
   using namespace kf::f8b;
   if (((lda | ldb | ldsa | ldsb) & 15) || M <= 0 || N <= 0 || K <= 0 || num_sms < 2) return 5;
   int* status = reinterpret_cast<int*>(kf_status_device_ptr());
-  if (few_serves(M, N, K)) return gemm_blocks_few(A, sa, B, sb, C, M, N, K, lda, ldsa, ldb, ldsb, ldc, a_fmt, b_fmt, accumulate, num_sms, stream);
+  if (few_serves(M, N, K)) return gemm_blocks_few(A, sa, B, sb, C, M, N, K, lda, ldsa, ldb, ldsb, ldc, f32, a_fmt, b_fmt, accumulate, num_sms, stream);
   const Cut cut = cut_of(M, N, K, num_sms);
   const bool wide = ((ldc | N) & 7) == 0 && (reinterpret_cast<uintptr_t>(C) & 15) == 0;
   if (cut.turned) {
@@ -540,7 +557,7 @@ int kf_gemm_fp8_blocks(const void* A, const void* sa, const void* B, const void*
     if (dev < 64) attr_set[dev] = true;
   }
   const int clusters = cut.splits > 1 ? (int)tiles : (int)(tiles < num_sms / 2 ? tiles : num_sms / 2);
-  const Output out{reinterpret_cast<__nv_bfloat16*>(C), ldc, cut.turned, accumulate, wide};
+  const Output out{reinterpret_cast<__nv_bfloat16*>(C), f32 ? reinterpret_cast<float*>(C) : nullptr, ldc, cut.turned, accumulate, wide};
   return launch_programmatic(kf_gemm_fp8_blocks_2cta, dim3(unsigned(clusters * 2 * cut.splits)), THREADS, SMEM, 2 * cut.splits, (cudaStream_t)stream,
                              ma, mb, msa, msb, out, M, N, K, a_fmt, b_fmt, tile_n, status);
 }

@@ -100,7 +100,9 @@ def _declare(L: ctypes.CDLL) -> None:
         "kf_fp8_blocks_cast_bf16": [vp, i, i, ll, vp, vp, i, i, vp, ll, vp, ll, vp, ll, vp, ll, vp],
         "kf_add_rmsnorm_fp8_blocks": [vp, vp, vp, vp, vp, vp, ll, vp, ll, i, i, f, vp],
         "kf_fp8_blocks_values_bf16": [vp, ll, vp, ll, i, i, i, vp, vp],
-        "kf_gemm_fp8_blocks": [vp, vp, vp, vp, vp, i, i, i, ll, ll, ll, ll, ll, i, i, i, i, vp],
+        "kf_norm_grads_blocks": [i, i, i],
+        "kf_norm_grads_f32": [vp, vp, vp, vp, vp, vp, vp, vp, i, i, i, vp],
+        "kf_gemm_fp8_blocks": [vp, vp, vp, vp, vp, i, i, i, ll, ll, ll, ll, ll, i, i, i, i, i, vp],
         "kf_fp8_absmax_bf16": [vp, ll, vp, vp, vp],
         "kf_fp8_cast_bf16": [vp, i, i, ll, vp, i, vp, i, vp, ll, vp, ll, vp],
         "kf_lion": [vp, vp, vp, ll, i, f, f, f, f, vp],
@@ -505,7 +507,7 @@ def _load_steps():
                   ctypes.cast(lib().kf_blocks_decode_bf16, c_void_p).value, SKINNY_MAX_ROWS, lib().kf_skinny_norm_rows())
     mod.fp8_configure(*(ctypes.cast(getattr(lib(), name), c_void_p).value for name in (
         "kf_gemm_fp8_blocks", "kf_add_rmsnorm_fp8_blocks", "kf_fp8_blocks_cast_bf16", "kf_fp8_blocks_values_bf16",
-        "kf_rmsnorm_bwd_bf16", "kf_rmsnorm_bwd_blocks")))
+        "kf_norm_grads_f32", "kf_norm_grads_blocks")))
     _steps = mod
     return mod
 
@@ -901,15 +903,27 @@ def _step(name: str, *args, launches: int = 1):
     return r
 
 
-def fp8_blocks_mm(a, b, out: torch.Tensor | None, accumulate: bool) -> torch.Tensor | None:
+def fp8_blocks_mm(a, b, out: torch.Tensor | None, accumulate: bool, f32: bool) -> torch.Tensor | None:
     """:func:`gemm_fp8_blocks` of two (values, scales, e5m2), checked as well; None where Python's checks have to look."""
-    return _step("fp8_mm", *a, *b, out, accumulate, sm_count())
+    return _step("fp8_mm", *a, *b, out, accumulate, f32, sm_count())
 
 
-def norm_grads(dh, t, gain, rstd, dt) -> tuple[torch.Tensor, torch.Tensor]:
-    """:func:`rmsnorm_bwd` of contiguous matrices, ``dt`` (or None) added."""
-    r = _step("norm_grads", dh, t, gain, rstd, dt, launches=3)
-    return rmsnorm_bwd(dh, t, gain, rstd, residual_grad=dt) if r is None else r
+# Widest rows of which norm_grads keeps the gradient of the gain in registers.
+NORM_GRADS_MAX_DIM = 8192
+
+
+def norm_grads(dh: torch.Tensor, t: torch.Tensor, gain: torch.Tensor, rstd: torch.Tensor, dt: torch.Tensor | None):
+    """(dt + gradient of t, gradient of the gain), bf16, of an RMSNorm of rows of up to NORM_GRADS_MAX_DIM values; ``dh`` is fp32, and all
+    are contiguous and on 16 bytes."""
+    r = _step("norm_grads", dh, t, gain, rstd, dt, sm_count(), launches=2)
+    if r is not None:
+        return r
+    rows, d = t.shape
+    partial = torch.empty((lib().kf_norm_grads_blocks(rows, d, sm_count()), d), dtype=torch.float32, device=t.device)
+    dx, dgain = torch.empty_like(t), torch.empty(d, dtype=torch.bfloat16, device=t.device)
+    _check(lib().kf_norm_grads_f32(dh.data_ptr(), t.data_ptr(), gain.data_ptr(), rstd.data_ptr(), _ptr(dt), dx.data_ptr(), partial.data_ptr(),
+                                   dgain.data_ptr(), rows, d, sm_count(), _stream()), "kf_norm_grads_f32", 2)
+    return dx, dgain
 
 
 def _block_buffers(rows: int, cols: int, device):
@@ -920,7 +934,7 @@ def _block_buffers(rows: int, cols: int, device):
 
 def fp8_blocks_cast(x2: torch.Tensor, e5m2: bool, square: bool, want_row: bool, want_t: bool, rstd: torch.Tensor | None = None,
                     gain: torch.Tensor | None = None):
-    """(bytes, scale bytes) of the bf16 matrix ``x2``, or of ``x2 * rstd[:, None] * gain``, and of its transpose; None in place of what is
+    """(bytes, scale bytes) of the bf16 matrix ``x2``, or of ``x2 * gain * rstd[:, None]``, and of its transpose; None in place of what is
     not wanted."""
     rows, cols = x2.shape
     row = _block_buffers(rows, cols, x2.device) if want_row else (None, None)
@@ -955,11 +969,11 @@ def fp8_blocks_values(q: torch.Tensor, s: torch.Tensor, e5m2: bool) -> torch.Ten
 
 def gemm_fp8_blocks(a: torch.Tensor, sa: torch.Tensor, b: torch.Tensor, sb: torch.Tensor, a_e5m2: bool, b_e5m2: bool, out: torch.Tensor,
                     accumulate: bool = False) -> torch.Tensor:
-    """out (M, N) bf16 (+)= a (M, K) @ b (N, K)ᵀ of bytes with scale bytes for each block of 128."""
+    """out (M, N), bf16 or fp32, (+)= a (M, K) @ b (N, K)ᵀ of bytes with scale bytes for each block of 128."""
     m, k = a.shape
     n = b.shape[0]
     _check(lib().kf_gemm_fp8_blocks(a.data_ptr(), sa.data_ptr(), b.data_ptr(), sb.data_ptr(), out.data_ptr(), m, n, k, a.stride(0),
-                                    sa.stride(0), b.stride(0), sb.stride(0), out.stride(0), int(a_e5m2), int(b_e5m2), int(accumulate),
+                                    sa.stride(0), b.stride(0), sb.stride(0), out.stride(0), int(out.dtype == torch.float32), int(a_e5m2), int(b_e5m2), int(accumulate),
                                     sm_count(), _stream()), "kf_gemm_fp8_blocks")
     return out
 

@@ -17,7 +17,7 @@ if it were not there.
     norm_linear    differentiable x + residual -> RMSNorm -> Linear, the normalised activation in 8 bits only
 
     forward   y  = q(h) q(W)ᵀ                 q over 128 values of k, W over squares
-    backward  dh = q(dy) q(W)                 q over 128 values of n
+    backward  dh = q(dy) q(W)                 q over 128 values of n; of a norm_linear kept in 32 bits for the norm's gradients
               dW = q(dyᵀ) q(hᵀ)ᵀ              q over 128 tokens
 
 ``train.fp8_scaling = "block128"`` has the fp8 Linear layers take this path.  CUDA tensors run the kernels of ``csrc/fp8_blocks.cu`` and
@@ -149,9 +149,12 @@ def quantize(x2: torch.Tensor, e5m2: bool = False, square: bool = False, want_ro
     return _cast_rows(v, e5m2, square) if want_row else None, _cast_rows(v.t().contiguous(), e5m2, square) if want_t else None
 
 
-def mm(a: BlockScaled, b: BlockScaled, out: torch.Tensor | None = None, accumulate: bool = False) -> torch.Tensor:
-    """bf16 (M, N) = a (M, K) @ b (N, K)ᵀ, accumulated in fp32 and rounded once; with ``accumulate`` added to ``out`` before that."""
-    if a.values.is_cuda and (y := _cuda().fp8_blocks_mm(a, b, out, accumulate)) is not None:
+def mm(a: BlockScaled, b: BlockScaled, out: torch.Tensor | None = None, accumulate: bool = False, dtype: torch.dtype | None = None) -> torch.Tensor:
+    """(M, N) = a (M, K) @ b (N, K)ᵀ, accumulated in fp32 and rounded once to ``dtype``: that of ``out``, else bf16 unless fp32 is asked for;
+    with ``accumulate`` added to ``out`` before the rounding."""
+    if dtype is None:
+        dtype = _BF16 if out is None else out.dtype
+    if a.values.is_cuda and (y := _cuda().fp8_blocks_mm(a, b, out, accumulate, dtype is torch.float32)) is not None:
         return y
     _check_operand(a, "a")
     _check_operand(b, "b")
@@ -161,10 +164,12 @@ def mm(a: BlockScaled, b: BlockScaled, out: torch.Tensor | None = None, accumula
     dev = a.values.device
     if b.values.device != dev:
         raise ValueError(f"operands on {dev} and {b.values.device}")
+    if dtype not in (_BF16, torch.float32):
+        raise ValueError(f"products are bf16 or fp32, got {dtype}")
     if out is None:
-        out, accumulate = torch.empty((m, n), dtype=_BF16, device=dev), False
-    elif out.shape != (m, n) or out.dtype != _BF16 or out.device != dev or (n > 1 and out.stride(1) != 1) or (m > 1 and out.stride(0) < n):
-        raise ValueError(f"out: a bf16 ({m}, {n}) matrix on {dev} with contiguous columns is wanted")
+        out, accumulate = torch.empty((m, n), dtype=dtype, device=dev), False
+    elif out.shape != (m, n) or out.dtype != dtype or out.device != dev or (n > 1 and out.stride(1) != 1) or (m > 1 and out.stride(0) < n):
+        raise ValueError(f"out: a {dtype} ({m}, {n}) matrix on {dev} with contiguous columns is wanted")
     if m == 0 or n == 0 or k == 0:
         return out if accumulate else out.zero_()
     if not a.values.is_cuda:
@@ -187,7 +192,7 @@ def _pitched(t: torch.Tensor) -> torch.Tensor:
 
 def add_rmsnorm(x: torch.Tensor, residual: torch.Tensor | None, weight: torch.Tensor, eps: float = 1e-5):
     """(t, rstd, h) of bf16 matrices (rows, d), d a multiple of 8 up to 32 768: t = x + residual rounded to bf16 (x itself without one),
-    rstd = 1 / sqrt(mean(t²) + eps) as fp32 (rows,), h = t * rstd * weight in 8 bits, never rounded to 16.  Not differentiable by itself:
+    rstd = 1 / sqrt(mean(t²) + eps) as fp32 (rows,), h = (t * weight) * rstd in 8 bits, never rounded to 16.  Not differentiable by itself:
     :func:`norm_linear` is."""
     if x.is_cuda and (r := _cuda()._step("fp8_add_rmsnorm", x, residual, weight, eps)) is not None:
         t, rstd, q, s = r
@@ -201,7 +206,7 @@ def add_rmsnorm(x: torch.Tensor, residual: torch.Tensor | None, weight: torch.Te
     if not x.is_cuda:
         t = x if residual is None else (x.float() + residual.float()).to(_BF16)
         rstd = torch.rsqrt(t.float().square().mean(1) + eps)
-        return t, rstd, _cast_rows(t.float() * rstd[:, None] * weight.float(), False)
+        return t, rstd, _cast_rows(t.float() * weight.float() * rstd[:, None], False)
     x, residual, weight = _aligned(x), residual if residual is None else _aligned(residual), _aligned(weight)
     with _on(x):
         t, rstd, h = _cuda().add_rmsnorm_fp8_blocks(x, residual, weight, eps)
@@ -323,7 +328,7 @@ class _NormLinearFn(torch.autograd.Function):
             need_h = need_x or need_r or need_g
             g8, g8t = quantize(_rows(dy), want_row=need_h, want_t=any(need_w))
             if need_h:
-                dh = mm(g8, quantized_weight(weights, want_t=True)[1])
+                dh = mm(g8, quantized_weight(weights, want_t=True)[1], dtype=torch.float32)
                 dx, dgain = _norm_grads(dh, t, gain, rstd, None if dt is None else _rows(dt))
                 dx = dx.view(ctx.x_shape)
                 dgain = _gain_grad(gain, dgain) if need_g else None
@@ -337,11 +342,15 @@ def _norm_grads(dh, t, gain, rstd, dt):
     if t.numel() == 0:
         return torch.empty_like(t), torch.zeros_like(gain)
     if t.is_cuda:
+        cu = _cuda()
+        gain, dt = _aligned(gain), None if dt is None else _aligned(dt)
         with _on(t):
-            return _cuda().norm_grads(dh, t, _aligned(gain), rstd, None if dt is None else _aligned(dt))
-    tf, g, r = t.float(), dh.float() * gain.float(), rstd[:, None]
+            if t.shape[1] > cu.NORM_GRADS_MAX_DIM:
+                return cu.rmsnorm_bwd(dh.to(_BF16), t, gain, rstd, residual_grad=dt)
+            return cu.norm_grads(dh, t, gain, rstd, dt)
+    tf, g, r = t.float(), dh * gain.float(), rstd[:, None]
     d = r * g - tf * (r * r * r * (g * tf).mean(1, keepdim=True))
-    return (d if dt is None else d + dt.float()).to(_BF16), (dh.float() * tf * r).sum(0).to(gain.dtype)
+    return (d if dt is None else d + dt.float()).to(_BF16), (dh * tf * r).sum(0).to(gain.dtype)
 
 
 def _gain_grad(gain, dgain):
@@ -358,7 +367,7 @@ def _gain_grad(gain, dgain):
 
 
 def _normed_t(t, rstd, gain) -> BlockScaled:
-    """The transpose of t * rstd * gain in 8 bits."""
+    """The transpose of (t * gain) * rstd in 8 bits."""
     if t.numel() == 0:
         return _empty(t.shape[1], t.shape[0], t.device, False)
     if t.is_cuda:
@@ -367,7 +376,7 @@ def _normed_t(t, rstd, gain) -> BlockScaled:
             return BlockScaled(r[2], r[3])
         with _on(t):
             return BlockScaled(*_cuda().fp8_blocks_cast(t, False, False, False, True, rstd, _aligned(gain))[1])
-    return _cast_rows((t.float() * rstd[:, None] * gain.float()).t().contiguous(), False)
+    return _cast_rows((t.float() * gain.float() * rstd[:, None]).t().contiguous(), False)
 
 
 def norm_linear_of(norm, x: torch.Tensor, residual: torch.Tensor | None, weights):

@@ -109,6 +109,22 @@ def test_product(native_lib, m, n, k, ea, eb):
     assert native_lib.read_status() == 0
 
 
+@pytest.mark.parametrize("m, n, k", [(1, 1000, 700), (9, 129, 4096), (20, 256, 300), (300, 521, 384), (300, 200, 4096), (72, 2001, 2048), (700, 1792, 520)])
+def test_product_in_32_bits(native_lib, m, n, k):
+    a, b, av, bv = _mm_case(m, n, k, False, True, 5)
+    want, mag = av @ bv.t(), av.abs() @ bv.abs().t()
+    got = fb.mm(a, b, dtype=torch.float32)
+    bound = (k + 2) * 2.0**-23 * mag + 1e-38
+    assert got.dtype == torch.float32 and bool(((got.double() - want).abs() <= bound).all())
+    frame = torch.full((m + 1, n + 5), 7.0, device=DEV)
+    old = _spread(m, n, 3, torch.float32)
+    frame[:m, 1 : n + 1] = old
+    fb.mm(a, b, out=frame[:m, 1 : n + 1], accumulate=True)
+    assert bool(((frame[:m, 1 : n + 1].double() - want - old.double()).abs() <= bound + 2.0**-23 * (old.double().abs() + want.abs())).all())
+    assert bool((frame[m] == 7).all()) and bool((frame[:, 0] == 7).all()) and bool((frame[:, n + 1 :] == 7).all())
+    assert native_lib.read_status() == 0
+
+
 @pytest.mark.parametrize("m, n, k", [(5, 200, 300), (64, 129, 256), (300, 520, 384), (300, 521, 384), (264, 1000, 4096), (261, 1000, 4096), (1304, 296, 4096), (1300, 297, 2048)])
 def test_product_adds_into_a_pitched_output_and_leaves_the_rest(native_lib, m, n, k):
     a, b, av, bv = _mm_case(m, n, k, False, False, 7)
@@ -132,13 +148,16 @@ def test_product_of_slices_and_of_scales_at_the_ends(native_lib):
     part = fb.mm(fb.BlockScaled(a.values[3:20, 128:384], a.scales[1:3, 3:20]), fb.BlockScaled(b.values[5:, 128:384], b.scales[1:3, 5:]))
     want = av[3:20, 128:384] @ bv[5:, 128:384].t()
     assert _mm_close(part, want, av[3:20, 128:384].abs() @ bv[5:, 128:384].abs().t(), 256)
-    one = torch.full((1, 128), 0x38, dtype=torch.uint8, device=DEV)          # 1.0 in e4m3
-    for sa, sb, value in ((127, 127, 128.0), (254, 1, 256.0), (1, 200, 0.0), (60, 194, 128.0), (100, 100, 128 * 2.0**-54)):
-        s = lambda v: torch.full((1, 1), v, dtype=torch.uint8, device=DEV)   # noqa: E731
-        got = fb.mm(fb.BlockScaled(one, s(sa)), fb.BlockScaled(one, s(sb)))
-        assert got.item() == (value if value else 128 * 2.0**(1 + 200 - 254)), (sa, sb, got)
-    nan = fb.mm(fb.BlockScaled(one, torch.full((1, 1), 255, dtype=torch.uint8, device=DEV)), fb.BlockScaled(one, torch.full((1, 1), 127, dtype=torch.uint8, device=DEV)))
-    assert nan.isnan().all()
+    for rows in (1, 9, 40, 300):                                              # of each kernel
+        one = torch.full((rows, 128), 0x38, dtype=torch.uint8, device=DEV)    # 1.0 in e4m3
+        s = lambda v, pitch=-(-rows // 16) * 16: torch.full((1, pitch), v, dtype=torch.uint8, device=DEV)[:, :rows]   # noqa: E731, B023
+        for sa, sb in ((127, 127), (254, 1), (1, 254), (254, 0), (0, 254), (1, 200), (60, 194), (194, 60), (100, 100), (254, 100), (120, 120)):
+            for a8, b8 in ((False, False), (False, True), (True, False)):
+                v = one if not a8 else torch.full_like(one, 0x3C), one if not b8 else torch.full_like(one, 0x3C)      # 1.0 in e5m2
+                got = fb.mm(fb.BlockScaled(v[0], s(sa), a8), fb.BlockScaled(v[1], s(sb), b8))
+                assert bool((got.double() == 128 * 2.0 ** (sa + sb - 254)).all()), (rows, sa, sb, got)
+        for sa, sb in ((255, 127), (127, 255), (255, 0)):
+            assert fb.mm(fb.BlockScaled(one, s(sa)), fb.BlockScaled(one, s(sb))).isnan().all()
 
 
 def test_what_is_not_finite_stays_in_its_row_and_column(native_lib):
@@ -166,9 +185,9 @@ def test_norm(native_lib, rows, d, with_residual):
     want = (t.double().square().mean(1) + 1e-5).rsqrt()
     # a sum of d squares (2^-24 each, at most d of them one after another) under a square root, and an approximate one (2^-22)
     assert bool(((rstd.double() - want).abs() <= want * (d * 2.0**-25 + 2.0**-21)).all())
-    assert _same(h, fb._cast_rows(t.float() * rstd[:, None] * gain.float(), False))
+    assert _same(h, fb._cast_rows(t.float() * gain.float() * rstd[:, None], False))
     normed = fb._normed_t(t, rstd, gain)
-    assert _same(normed, fb._cast_rows((t.float() * rstd[:, None] * gain.float()).t().contiguous(), False))
+    assert _same(normed, fb._cast_rows((t.float() * gain.float() * rstd[:, None]).t().contiguous(), False))
     again = fb.add_rmsnorm(x, residual, gain, 1e-5)
     assert torch.equal(again[1], rstd) and _same(again[2], h)
 
@@ -183,7 +202,7 @@ def test_norm_of_rows_with_infinities_and_zeros(native_lib):
     assert v[[0, 3, 4, 5]].isfinite().all()
     gain[5] = float("inf")                                       # of one column: NaN there, the rest of its block scaled as without it
     got = fb.add_rmsnorm(x[4:], None, gain)[2]
-    assert _same(got, fb._cast_rows(x[4:].float() * fb.add_rmsnorm(x[4:], None, gain)[1][:, None] * gain.float(), False))
+    assert _same(got, fb._cast_rows(x[4:].float() * gain.float() * fb.add_rmsnorm(x[4:], None, gain)[1][:, None], False))
     assert fb._values(got).isnan().sum() == 2
 
 
@@ -222,9 +241,9 @@ def test_layer_and_its_gradients(native_lib, tokens, d, outs, with_residual):
     assert torch.equal(t2, h[0])
     hv, wv, gv = fb._values(h[2]).double(), fb._values(_plain(w, False, True)).double(), fb._values(_plain(dy2, False, False)).double()
     assert _mm_close(y.detach().view(rows, -1), hv @ wv.t(), hv.abs() @ wv.abs().t(), d)
-    # dh is rounded to bf16 once before the norm's gradient
+    # dh stays in 32 bits
     dh, dh_mag = gv @ wv, gv.abs() @ wv.abs()
-    dh_err = HALF_BF16 * dh.abs() * (1 + 2**-7) + (w.shape[0] + 2) * 2.0**-23 * dh_mag
+    dh_err = (w.shape[0] + 2) * 2.0**-23 * dh_mag
     dx, mag, dgain, dgain_mag = _norm_grads64(dh, t2, gain.detach(), dt2, 1e-5)
     _, err, _, gain_err = _norm_grads64(dh_err, t2, gain.detach().abs(), dt2 * 0, 1e-5)
     # 32-bit sums of d terms and of `rows` terms
@@ -232,11 +251,29 @@ def test_layer_and_its_gradients(native_lib, tokens, d, outs, with_residual):
     if with_residual:
         assert torch.equal(got["r"], got["x"])
     assert bool(((got["gain"].double() - dgain).abs() <= gain_err + HALF_BF16 * (dgain.abs() + gain_err) + (rows + 8) * 2.0**-21 * dgain_mag).all())
-    ht = fb._values(fb._cast_rows((t2.float() * h[1][:, None] * gain.detach().float()).t().contiguous(), False)).double()
+    ht = fb._values(fb._cast_rows((t2.float() * gain.detach().float() * h[1][:, None]).t().contiguous(), False)).double()
     gt = fb._values(_plain(dy2.t().contiguous(), False, False)).double()
     dw = torch.cat([got[f"w{i}"] for i in range(len(ws))])
     assert _mm_close(dw, gt @ ht.t(), gt.abs() @ ht.abs().t(), rows)
     assert native_lib.read_status() == 0
+
+
+@pytest.mark.parametrize("rows, d", [(1, 8), (3, 136), (3000, 1024), (130, 1032), (1000, 4096), (70, 4104), (33, 8192), (20, 8200)])
+def test_gradients_of_the_norm(native_lib, rows, d):
+    g = _gen(d)
+    r = lambda *s: torch.randn(*s, device=DEV, generator=g)   # noqa: E731
+    t, gain, dt, dh = (2 * r(rows, d)).bfloat16(), (1 + 0.2 * r(d)).bfloat16(), r(rows, d).bfloat16(), r(rows, d)
+    rstd = (t.double().square().mean(1) + 1e-5).rsqrt().float()
+    # rows too wide for the kernel of 32 bits: a rounding of dh to bf16, and a kernel that rounds less carefully
+    err = dh.double().abs() * (HALF_BF16 if d > 8192 else 0)
+    for with_dt in (dt, None):
+        dx, dgain = fb._norm_grads(dh, t, gain, rstd, with_dt)
+        want, mag, want_gain, gain_mag = _norm_grads64(dh, t, gain, dt if with_dt is not None else dt * 0, 1e-5)
+        _, more, _, more_gain = _norm_grads64(err, t, gain.abs(), dt * 0, 1e-5)
+        assert bool(((dx.double() - want).abs() <= more + HALF_BF16 * (want.abs() + more) + d * 2.0**-22 * mag).all())
+        assert bool(((dgain.double() - want_gain).abs() <= more_gain + HALF_BF16 * (want_gain.abs() + more_gain) + (rows + 8) * 2.0**-22 * gain_mag).all())
+        again = fb._norm_grads(dh, t, gain, rstd, with_dt)
+        assert torch.equal(again[0], dx) and torch.equal(again[1], dgain)
 
 
 @pytest.mark.parametrize("lead", [(5,), (2, 150)])
