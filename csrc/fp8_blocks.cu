@@ -371,8 +371,11 @@ kf_add_rmsnorm_blocks(const __nv_bfloat16* x, const __nv_bfloat16* residual, con
 // Gradients of RMSNorm from dh in 32 bits, one pass: a block walks over rows, keeps its columns' part of the gain's gradient in registers and
 // leaves it in partial[block][column] for kf_column_sums.  dh as a product leaves it, unrounded: rounded to 16 bits on the way it moves the
 // gain's gradient, a sum over thousands of rows that cancel, by as much as the gradient's own rounding does.
-template <int THREADS, int VPT>
-__global__ void __launch_bounds__(THREADS)
+// Bound by memory, 10 bytes an element (dt given), and by the wait of a row for its own sum: three blocks on an SM take turns (four of 64
+// registers spill, and gain nothing).  us (at the copy rate; the two passes that there were over dh in 16 bits): 16 384 x 4096 120 (103; 159),
+// 4096 x 4096 37 (26; 49), 16 384 x 768 28 (19; 74), 999 x 768 8.2 (1.2; 11.7).
+template <int THREADS, int VPT, int BLOCKS>
+__global__ void __launch_bounds__(THREADS, BLOCKS)
 kf_norm_grads(const float* dh, const __nv_bfloat16* t, const __nv_bfloat16* gain, const float* rstd, const __nv_bfloat16* dt, __nv_bfloat16* dx,
               float* partial, int rows, int D) {
   __shared__ float red[2][32];
@@ -437,22 +440,23 @@ kf_norm_grads(const float* dh, const __nv_bfloat16* t, const __nv_bfloat16* gain
   }
 }
 
-// out[column] = sum over parts of partial[part][column], 32 columns per block and every eighth part per warp, in a fixed order
-__global__ void __launch_bounds__(256) kf_column_sums(const float* partial, int parts, int D, __nv_bfloat16* out) {
-  __shared__ float red[8][32];
+// out[column] = sum over parts of partial[part][column], 32 columns per block and every 32nd part per warp, in a fixed order
+__global__ void __launch_bounds__(1024) kf_column_sums(const float* partial, int parts, int D, __nv_bfloat16* out) {
+  __shared__ float red[32][33];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
   wait_for_previous();
   let_next_in();
   float v = 0.f;
-  if (c < D)
-    for (int p = warp; p < parts; p += 8) v += partial[size_t(p) * D + c];
+  if (c < D) {
+#pragma unroll 8
+    for (int p = warp; p < parts; p += 32) v += partial[size_t(p) * D + c];
+  }
   red[warp][lane] = v;
   __syncthreads();
-  if (warp == 0 && c < D) {
+  v = red[lane][warp];  // a warp per column
 #pragma unroll
-    for (int w = 1; w < 8; ++w) v += red[w][lane];
-    out[c] = __float2bfloat16(v);
-  }
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if (lane == 0 && blockIdx.x * 32 + warp < D) out[blockIdx.x * 32 + warp] = __float2bfloat16(v);
 }
 
 // The values that the bytes stand for, in bf16 (exact where bf16 has them): sixteen per thread, blocks of 16 x 16 threads on 256 columns.
@@ -544,10 +548,11 @@ int kf_add_rmsnorm_fp8_blocks(const void* x, const void* residual, const void* g
   return go(kf_add_rmsnorm_blocks<1024, 4>, 1024);
 }
 
-// Blocks of kf_norm_grads_f32, each of which leaves D floats in `partial`.
+// Blocks of kf_norm_grads_f32, each of which leaves D floats in `partial`: what the SMs hold, of four rows at least where that fills them.
 int kf_norm_grads_blocks(int rows, int D, int num_sms) {
-  const int per_sm = D <= 1024 ? 16 : D <= 4096 ? 4 : 2;
-  return rows < num_sms * per_sm ? (rows < 1 ? 1 : rows) : num_sms * per_sm;
+  int blocks = num_sms * (D <= 1024 ? 8 : D <= 4096 ? 3 : 2);
+  if (blocks > rows / 4) blocks = rows / 4 > num_sms ? rows / 4 : num_sms;
+  return rows < 1 ? 1 : rows < blocks ? rows : blocks;
 }
 
 // dx (bf16) = dt (or 0 where null) + the gradient of RMSNorm at t for dh (fp32); dgain (bf16) of its gain.  Contiguous rows on 16 bytes, D a
@@ -565,9 +570,9 @@ int kf_norm_grads_f32(const void* dh, const void* t, const void* gain, const voi
     return launch_programmatic(kern, dim3(unsigned(blocks)), threads, 0, 1, st, (const float*)dh, (const __nv_bfloat16*)t, (const __nv_bfloat16*)gain,
                                (const float*)rstd, (const __nv_bfloat16*)dt, (__nv_bfloat16*)dx, (float*)partial, rows, D);
   };
-  const int rc = D <= 1024 ? go(kf_norm_grads<32, 4>, 32) : D <= 4096 ? go(kf_norm_grads<256, 2>, 256) : go(kf_norm_grads<512, 2>, 512);
+  const int rc = D <= 1024 ? go(kf_norm_grads<128, 1, 8>, 128) : D <= 4096 ? go(kf_norm_grads<256, 2, 3>, 256) : go(kf_norm_grads<512, 2, 2>, 512);
   if (rc) return rc;
-  return launch_programmatic(kf_column_sums, dim3((D + 31) / 32), 256, 0, 1, st, (const float*)partial, blocks, D, (__nv_bfloat16*)dgain);
+  return launch_programmatic(kf_column_sums, dim3((D + 31) / 32), 1024, 0, 1, st, (const float*)partial, blocks, D, (__nv_bfloat16*)dgain);
 }
 
 // out[rows][cols] (contiguous bf16) = the values that q (pitch ld) and its scale bytes stand for.
