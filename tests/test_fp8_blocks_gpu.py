@@ -402,3 +402,65 @@ def test_two_streams_at_once(native_lib):
                 got.append(fb.norm_linear(*c[:3], c[3]))
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for g, w in zip(got, want) for a, b in zip(g, w))
+
+
+def test_a_captured_step_gives_the_gradients_of_each_replay(native_lib):
+    d, outs = 264, (136, 48)
+    x, residual, gain, ws, dt, dy = _layer((70,), d, outs, 6)
+    leaves = (x, residual, gain, *ws)
+
+    def step():
+        t, y = fb.norm_linear(x, residual, gain, ws)
+        return t, y, *torch.autograd.grad((t, y), leaves, (dt, dy))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step()
+    torch.cuda.current_stream().wait_stream(side)
+    graphs = []
+    for _ in range(2):                                     # two graphs of the same step share nothing but their inputs
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = step()
+        graphs.append((graph, got))
+    for seed in (21, 22):
+        new = _layer((70,), d, outs, seed)
+        with torch.no_grad():
+            for old, value in zip((*leaves, dt, dy), (*new[:3], *new[3], *new[4:])):
+                old.copy_(value)
+        for graph, got in graphs:
+            for v in got:
+                v.detach().fill_(7.0)
+        for graph, _ in graphs:
+            graph.replay()
+        want = step()
+        for _, got in graphs:
+            for a, b in zip(got, want):
+                assert torch.equal(a, b)
+    assert native_lib.read_status() == 0
+
+
+@pytest.mark.parametrize("m", [3, 70, 700])
+def test_products_right_after_what_they_read_and_before_what_overwrites_it(native_lib, m):
+    """Launches that overlap their predecessor's end: each cast, product and overwrite in a row sees what stands before it in the stream."""
+    n, k, rounds = 520, 1040, 12
+    xs, w = [_spread(m, k, s) for s in range(rounds)], fb.quantize(_spread(n, k, 99), square=True)[0]
+    want = [fb.mm(fb.quantize(x)[0], w) for x in xs]
+    torch.cuda.synchronize()
+    x, out = torch.empty_like(xs[0]), torch.empty_like(want[0])
+    a = fb.quantize(xs[0])[0]
+    kept = []
+    for v in xs:
+        x.copy_(v)
+        q = fb.quantize(x)[0]
+        a.values.copy_(q.values)
+        a.scales.copy_(q.scales)
+        fb.mm(a, w, out=out)
+        kept.append(out.clone())
+        a.values.fill_(0x7F)                              # NaN: nothing may read it any more
+        x.fill_(float("nan"))
+        out.fill_(float("nan"))
+    assert all(torch.equal(p, q) for p, q in zip(kept, want))
+    assert native_lib.read_status() == 0
