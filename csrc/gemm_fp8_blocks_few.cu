@@ -194,10 +194,10 @@ static int launch(const Args& a, int a_fmt, int b_fmt, int warps, cudaStream_t s
 
 }  // namespace few
 
-// Whether this kernel is the quicker one.  us, this / the tensor-memory kernel, graphs of launches on weights in turn: one token 256 x 256 2.2 /
-// 4.9, 1024 x 1024 2.9 / 6.0, 4096 x 4096 9.1 / 10.0, 6144 x 4096 12.6 / 11.0; 16 tokens 1024 x 1024 3.1 / 6.0, 4096 x 2048 6.8 / 8.2, 4096 x 4096
-// 10.8 / 10.1; 32 tokens in fours of eight 1024 x 1024 4.5 / 6.1, 1304 x 952 6.5 / 6.0, so not built.
-bool few_serves(int M, int N, int K) { return M <= few::MAX_TOKENS && (long long)N * K * ((M + 7) / 8) <= 20LL << 20; }
+// Whether this kernel is the quicker one.  us, this / the tensor-memory kernel, graphs of launches on weights in turn: one token 256 x 256 1.9 /
+// 4.0, 1024 x 1024 2.4 / 4.6, 2048 x 2048 3.9 / 6.3, 4096 x 2048 5.8 / 6.6, 4096 x 4096 9.3 / 8.5, 1024 x 14 336 14.1 / 11.1; 16 tokens 1304 x 952
+// 3.5 / 4.5, 2048 x 2048 4.5 / 6.3, 4096 x 2048 6.7 / 6.7.  In fours of eight tokens it gains little (32 x 1304 from 952 6.5 / 6.0): not built.
+bool few_serves(int M, int N, int K) { return M <= few::MAX_TOKENS && (long long)N * K * ((M + 7) / 8) <= 12LL << 20; }
 
 // The call of kf_gemm_fp8_blocks that few_serves.
 int gemm_blocks_few(const void* A, const void* sa, const void* B, const void* sb, void* C, int M, int N, int K, long long lda, long long ldsa,
@@ -206,7 +206,7 @@ int gemm_blocks_few(const void* A, const void* sa, const void* B, const void* sb
                     f32, accumulate};
   if (((reinterpret_cast<uintptr_t>(A) | reinterpret_cast<uintptr_t>(B)) & 15) != 0) return 5;
   const int k_blocks = (K + BLOCK - 1) / BLOCK;
-  int warps = (N + few::ROWS - 1) / few::ROWS <= num_sms ? 16 : 8;  // 2048 x 2048, 8 tokens 4.4 / 4.9 us; 4096 x 4096, one token 10.6 / 9.1
+  int warps = (N + few::ROWS - 1) / few::ROWS <= num_sms ? 16 : 8;  // 2048 x 2048, 8 tokens 4.4 / 4.9 us with 16 / 8; 4096 x 4096, one token 10.6 / 9.1
   if (warps > k_blocks) warps = k_blocks;
   cudaStream_t st = (cudaStream_t)stream;
   return M <= 8 ? few::launch<1>(a, a_fmt, b_fmt, warps, st) : few::launch<2>(a, a_fmt, b_fmt, warps, st);
