@@ -306,6 +306,9 @@ PyMethodDef methods[] = {
     {"fp8_add_rmsnorm", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(fp8_add_rmsnorm)), METH_FASTCALL, "RMSNorm in block-scaled fp8"},
     {"fp8_cast", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(fp8_cast)), METH_FASTCALL, "a matrix in block-scaled fp8"},
     {"fp8_values", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(fp8_values)), METH_FASTCALL, "its values in bf16"},
+    {"fp8_norm_linear", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(fp8_norm_linear)), METH_FASTCALL, "norm and product of a layer"},
+    {"fp8_norm_linear_grads", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(fp8_norm_linear_grads)), METH_FASTCALL, "its gradients"},
+    {"fp8_linear_grads", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(fp8_linear_grads)), METH_FASTCALL, "gradients of a product with a weight"},
     {"norm_grads", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(norm_grads)), METH_FASTCALL, "gradients of an RMSNorm and its gain"},
     {"fp8_configure", fp8_configure, METH_VARARGS, "the native entries of the block-scaled operators"},
     {"decode", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(decode)), METH_FASTCALL, "one new token per sequence through blocks"},

@@ -264,10 +264,10 @@ def _rows(x: torch.Tensor) -> torch.Tensor:
     return x2 if x2.is_contiguous() else x2.contiguous()
 
 
-def _weight_grads(weights, needs, g8t: BlockScaled, h8t: BlockScaled):
+def _deposit(weights, needs, compute):
     from kempnerforge_b200.ops import functional as F
 
-    return F._deposit_stacked_weight_grads(weights, needs, lambda out, acc: mm(g8t, h8t, out=out, accumulate=acc))
+    return F._deposit_stacked_weight_grads(weights, needs, compute)
 
 
 class _BlocksLinearFn(torch.autograd.Function):
@@ -286,10 +286,30 @@ class _BlocksLinearFn(torch.autograd.Function):
     def backward(ctx, dy):
         q8t, s8t, *weights = ctx.saved_tensors
         need_dx, need_dw = ctx.needs_input_grad[0], any(ctx.needs_input_grad[1:])
-        g8, g8t = quantize(_rows(dy), want_row=need_dx, want_t=need_dw)
-        dx = mm(g8, quantized_weight(weights, want_t=True)[1]).view(ctx.x_shape) if need_dx else None
-        wgrads = _weight_grads(weights, ctx.needs_input_grad[1:], g8t, BlockScaled(q8t, s8t)) if need_dw else [None] * len(weights)
-        return dx, *wgrads
+        dy2 = _rows(dy)
+        w8t = quantized_weight(weights, want_t=True)[1] if need_dx else None
+        dx = None
+
+        def run(out=None, accumulate=False):
+            nonlocal dx
+            if dy2.is_cuda:
+                r = _cuda()._step("fp8_linear_grads", dy2, *(w8t[:2] if need_dx else (None, None)), q8t, s8t, out, accumulate, _cuda().sm_count(),
+                                  launches=1 + need_dx + need_dw)
+                if r is not None:
+                    dx = r if need_dx else None
+                    return
+            g8, g8t = quantize(dy2, want_row=need_dx, want_t=need_dw)
+            if need_dx:
+                dx = mm(g8, w8t)
+            if need_dw:
+                mm(g8t, BlockScaled(q8t, s8t), out=out, accumulate=accumulate)
+
+        wgrads = [None] * len(weights)
+        if need_dw:
+            wgrads = _deposit(weights, ctx.needs_input_grad[1:], run)
+        elif need_dx:
+            run()
+        return dx.view(ctx.x_shape) if need_dx else None, *wgrads
 
 
 def linear(x: torch.Tensor, weights) -> torch.Tensor:
@@ -306,10 +326,15 @@ class _NormLinearFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, gain, eps, *weights):
         ctx.set_materialize_grads(False)
-        r2 = None if residual is None else _rows(residual)
-        t, rstd, h8 = add_rmsnorm(_rows(x), r2, gain, eps)
+        x2, r2 = _rows(x), None if residual is None else _rows(residual)
         w8, _ = quantized_weight(weights, want_t=any(ctx.needs_input_grad[:3]))
-        y = mm(h8, w8)
+        r = _cuda()._step("fp8_norm_linear", x2, r2, gain, eps, *w8[:2], _cuda().sm_count(), launches=2) if x.is_cuda else None
+        if r is not None:
+            t, rstd, y = r
+            t = x2.detach() if t is None else t
+        else:
+            t, rstd, h8 = add_rmsnorm(x2, r2, gain, eps)
+            y = mm(h8, w8)
         ctx.save_for_backward(t, rstd, gain, *weights)
         ctx.x_shape = x.shape
         # without a residual the sum is x itself: its gradient comes in here and is added where the norm's is written
@@ -325,15 +350,31 @@ class _NormLinearFn(torch.autograd.Function):
         if dy is None:
             dx = dt
         else:
-            need_h = need_x or need_r or need_g
-            g8, g8t = quantize(_rows(dy), want_row=need_h, want_t=any(need_w))
+            need_h, any_w = need_x or need_r or need_g, any(need_w)
+            dy2, dt2 = _rows(dy), None if dt is None else _rows(dt)
+            w8t = quantized_weight(weights, want_t=True)[1] if need_h else None
+
+            def run(out=None, accumulate=False):
+                nonlocal dx, dgain
+                if dy2.is_cuda:
+                    r = _cuda()._step("fp8_norm_linear_grads", dy2, dt2, t, gain, rstd, *(w8t[:2] if need_h else (None, None)), out, accumulate,
+                                      _cuda().sm_count(), launches=1 + 3 * need_h + 2 * any_w)
+                    if r is not None:
+                        dx, dgain = r
+                        return
+                g8, g8t = quantize(dy2, want_row=need_h, want_t=any_w)
+                if need_h:
+                    dx, dgain = _norm_grads(mm(g8, w8t, dtype=torch.float32), t, gain, rstd, dt2)
+                if any_w:
+                    mm(g8t, _normed_t(t, rstd, gain), out=out, accumulate=accumulate)
+
+            if any_w:
+                wgrads = _deposit(weights, need_w, run)
+            elif need_h:
+                run()
             if need_h:
-                dh = mm(g8, quantized_weight(weights, want_t=True)[1], dtype=torch.float32)
-                dx, dgain = _norm_grads(dh, t, gain, rstd, None if dt is None else _rows(dt))
                 dx = dx.view(ctx.x_shape)
                 dgain = _gain_grad(gain, dgain) if need_g else None
-            if any(need_w):
-                wgrads = _weight_grads(weights, need_w, g8t, _normed_t(t, rstd, gain))
         return dx if need_x else None, dx if need_r else None, dgain, None, *wgrads
 
 
