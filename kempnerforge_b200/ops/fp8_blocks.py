@@ -39,10 +39,21 @@ _BF16 = torch.bfloat16
 _NOTHING = contextlib.nullcontext()
 
 
-def _cuda():
-    from kempnerforge_b200.ops import cuda as cu
+_modules = None
 
-    return cu
+
+def _others():
+    """(ops.cuda, ops.functional), imported when first wanted."""
+    global _modules
+    if _modules is None:
+        from kempnerforge_b200.ops import cuda, functional
+
+        _modules = cuda, functional
+    return _modules
+
+
+def _cuda():
+    return _others()[0]
 
 
 def _on(t: torch.Tensor):
@@ -214,12 +225,12 @@ def add_rmsnorm(x: torch.Tensor, residual: torch.Tensor | None, weight: torch.Te
 
 
 def _check_norm(x, residual, weight) -> None:
-    d = x.shape[-1] if x.dim() else 0
-    if x.dtype != _BF16 or weight.dtype != _BF16 or (residual is not None and residual.dtype != _BF16):
+    d, device = x.size(-1) if x.dim() else 0, x.device
+    if x.dtype is not _BF16 or weight.dtype is not _BF16 or (residual is not None and residual.dtype is not _BF16):
         raise ValueError("x, residual and weight are bf16")
-    if weight.shape != (d,) or (residual is not None and residual.shape != x.shape):
+    if weight.dim() != 1 or weight.size(0) != d or (residual is not None and residual.shape != x.shape):
         raise ValueError(f"shapes: x {tuple(x.shape)}, residual {None if residual is None else tuple(residual.shape)}, weight {tuple(weight.shape)}")
-    if weight.device != x.device or (residual is not None and residual.device != x.device):
+    if weight.device != device or (residual is not None and residual.device != device):
         raise ValueError("x, residual and weight are on one device")
     if d % 8 or not 0 < d <= 32768:
         raise ValueError(f"rows of {d} values: a multiple of 8 up to 32768 is wanted")
@@ -235,9 +246,7 @@ def _aligned(t: torch.Tensor) -> torch.Tensor:
 def quantized_weight(weights, want_t: bool) -> tuple[BlockScaled, BlockScaled | None]:
     """(the weights stacked along the output dimension in 8 bits, the transpose of that or None), in squares of 128 x 128.  Kept on the
     first weight and reused under the conditions of :func:`kempnerforge_b200.ops.fp8.quantized_weight`."""
-    from kempnerforge_b200.ops import functional as F
-
-    stacked = lambda: F._stack_weight_rows(weights).detach()  # noqa: E731
+    stacked = lambda: _others()[1]._stack_weight_rows(weights).detach()  # noqa: E731
     state = fp8.weights_state(weights)
     if state is None:
         return quantize(stacked(), square=True, want_t=want_t)
@@ -252,22 +261,17 @@ def quantized_weight(weights, want_t: bool) -> tuple[BlockScaled, BlockScaled | 
 
 
 def _check_weights(x: torch.Tensor, weights) -> None:
-    if x.dtype != _BF16 or not x.dim() or not weights:
+    if x.dtype is not _BF16 or not x.dim() or not weights:
         raise ValueError("x is bf16 and has at least one weight")
+    k, device = x.size(-1), x.device
     for w in weights:
-        if w.dtype != _BF16 or w.dim() != 2 or w.shape[1] != x.shape[-1] or w.device != x.device:
-            raise ValueError(f"weights are bf16 (out, {x.shape[-1]}) matrices on {x.device}, got {w.dtype} {tuple(w.shape)} on {w.device}")
+        if w.dtype is not _BF16 or w.dim() != 2 or w.size(1) != k or w.device != device:
+            raise ValueError(f"weights are bf16 (out, {k}) matrices on {device}, got {w.dtype} {tuple(w.shape)} on {w.device}")
 
 
 def _rows(x: torch.Tensor) -> torch.Tensor:
-    x2 = x.reshape(-1, x.shape[-1])
+    x2 = x if x.dim() == 2 else x.reshape(-1, x.size(-1))
     return x2 if x2.is_contiguous() else x2.contiguous()
-
-
-def _deposit(weights, needs, compute):
-    from kempnerforge_b200.ops import functional as F
-
-    return F._deposit_stacked_weight_grads(weights, needs, compute)
 
 
 class _BlocksLinearFn(torch.autograd.Function):
@@ -306,7 +310,7 @@ class _BlocksLinearFn(torch.autograd.Function):
 
         wgrads = [None] * len(weights)
         if need_dw:
-            wgrads = _deposit(weights, ctx.needs_input_grad[1:], run)
+            wgrads = _others()[1]._deposit_stacked_weight_grads(weights, ctx.needs_input_grad[1:], run)
         elif need_dx:
             run()
         return dx.view(ctx.x_shape) if need_dx else None, *wgrads
@@ -369,7 +373,7 @@ class _NormLinearFn(torch.autograd.Function):
                     mm(g8t, _normed_t(t, rstd, gain), out=out, accumulate=accumulate)
 
             if any_w:
-                wgrads = _deposit(weights, need_w, run)
+                wgrads = _others()[1]._deposit_stacked_weight_grads(weights, need_w, run)
             elif need_h:
                 run()
             if need_h:
