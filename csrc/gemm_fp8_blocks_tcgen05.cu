@@ -406,12 +406,19 @@ kf_gemm_fp8_blocks_2cta(const __grid_constant__ CUtensorMap map_a, const __grid_
       const int row0 = tm * TILE_M + int(rank) * CTA_M + quarter * 32;  // this warp's rows, and how many exist
       const int rows = max(0, min(32, M - row0));
       const int col0 = tn * tile_n, width = min(tile_n, N - col0);
+      // the next 32 columns are under way while these are stored
+      const uint32_t from = t_row + acc * MAX_N;
+      uint32_t v[32], w[32];
+      tmem_ld_32x32(from, v);
 #pragma unroll 1
-      for (int c = 0; c * 32 < width; ++c) {
-        uint32_t v[32];
-        tmem_ld_32x32(t_row + acc * MAX_N + c * 32, v);
+      for (int c = 0; c < width; c += 64) {
         tmem_ld_wait();
-        out.put(box, lane, v, row0, col0 + c * 32, rows, min(32, width - c * 32));
+        if (c + 32 < width) tmem_ld_32x32(from + c + 32, w);
+        out.put(box, lane, v, row0, col0 + c, rows, min(32, width - c));
+        if (c + 32 >= width) break;
+        tmem_ld_wait();
+        if (c + 64 < width) tmem_ld_32x32(from + c + 64, v);
+        out.put(box, lane, w, row0, col0 + c + 32, rows, min(32, width - c - 32));
       }
       tc_fence_before();
       __syncwarp();
@@ -431,12 +438,19 @@ kf_gemm_fp8_blocks_2cta(const __grid_constant__ CUtensorMap map_a, const __grid_
     const int col0 = tn * tile_n, width = min(tile_n, N - col0);
     const uint32_t mine = smem_base + uint32_t(quarter) * WARP_BYTES + uint32_t(lane) * 16;
     __syncwarp();
-    cluster_sync_all();
-    if (warp >= 6 && warp < 10) {
+    cluster_meet();
+    tc_fence_after();
+    // warps 2 .. 5, which have no scales to move any more, take every other chunk; their boxes lie behind what arrives
+    const bool works = warp >= 2 && warp < 10;
+    const int half = warp < 6;
+    const uint32_t my_box = half ? smem_base + 6 * CHUNK_BYTES + uint32_t(warp - 2) * BOX_BYTES : box;
+    static_assert(6 * CHUNK_BYTES + 4 * BOX_BYTES <= STAGES * STAGE_BYTES, "at most two chunks of three pairs, or four of one, then the boxes");
+    if (works) {
+      int turn = 0;
 #pragma unroll 1
       for (int c = 0; c * 32 < width; ++c) {
         const int owner = c % splits;
-        if (owner == split) continue;
+        if (owner == split || (turn++ & 1) != half) continue;
         uint32_t v[32];
         tmem_ld_32x32(t_row + c * 32, v);
         tmem_ld_wait();
@@ -447,9 +461,9 @@ kf_gemm_fp8_blocks_2cta(const __grid_constant__ CUtensorMap map_a, const __grid_
     }
     __syncwarp();
     cluster_sync_all();
-    if (warp >= 6 && warp < 10) {
+    if (works) {
 #pragma unroll 1
-      for (int c = split; c * 32 < width; c += splits) {
+      for (int c = split + half * splits; c * 32 < width; c += 2 * splits) {
         uint32_t own[32], v[32];
         tmem_ld_32x32(t_row + c * 32, own);
         tmem_ld_wait();
@@ -468,10 +482,11 @@ kf_gemm_fp8_blocks_2cta(const __grid_constant__ CUtensorMap map_a, const __grid_
             v[4 * q + 3] = __float_as_uint(__uint_as_float(v[4 * q + 3]) + __uint_as_float(u.w));
           }
         }
-        out.put(box, lane, v, row0, col0 + c * 32, rows, min(32, width - c * 32));
+        out.put(my_box, lane, v, row0, col0 + c * 32, rows, min(32, width - c * 32));
       }
     }
   }
+
   tc_fence_before();
   __syncthreads();
   cluster_meet();  // neither CTA's tensor memory is in use
