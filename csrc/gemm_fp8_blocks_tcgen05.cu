@@ -18,6 +18,7 @@
 #include "pair_common.cuh"
 #include "tile_math.h"
 
+#include <type_traits>
 #include <utility>
 
 namespace kf {
@@ -118,6 +119,12 @@ __device__ __forceinline__ uint32_t four_bytes(const uint8_t* p, int step) {
   const uint32_t a = p[0], b = p[step], c = p[2 * step], d = p[3 * step];
   return a | b << 8 | c << 16 | d << 24;
 }
+__device__ __forceinline__ void sts32(uint32_t addr, uint32_t v) { asm volatile("st.shared.b32 [%0], %1;" ::"r"(addr), "r"(v) : "memory"); }
+__device__ __forceinline__ uint32_t lds32(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
 __device__ __forceinline__ unsigned short lds_u16(uint32_t addr) {
   unsigned short v;
   asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(addr) : "memory");
@@ -125,47 +132,33 @@ __device__ __forceinline__ unsigned short lds_u16(uint32_t addr) {
 }
 
 // Where a product goes: C[row * ld + column], or with `turned` (A's rows are C's columns) C[column * ld + row].
+// One of the four kinds (bf16 or fp32, set or added to) to a kernel: with all of them in one, the registers and the instructions of the others
+// cost bf16 outputs up to a fifth (us, 14 336 x 4096 from 2048: 96 -> 108).
+template <typename T, bool ADD>
 struct Output {
-  __nv_bfloat16* C;
-  float* F;  // C in 32 bits instead, or null
+  T* C;
   long long ld;
-  int turned, accumulate;
+  int turned;
   bool wide;  // rows of C start on 16 bytes and hold a multiple of eight values
 
   // 32 x 32 values of a warp at (row0, col0), a row per lane, of which rows x cols exist; box: 2 KB of the warp's own
   __device__ __forceinline__ void put(uint32_t box, int lane, const uint32_t (&v)[32], int row0, int col0, int rows, int cols) const {
-    if (F) {
-      float* dst = F + (turned ? (long long)col0 * ld + row0 + lane : (long long)(row0 + lane) * ld + col0);
-      const long long step = turned ? ld : 1;
-      if (lane < rows) {
-        if (wide && !turned && !accumulate) {
+    constexpr bool BF16 = sizeof(T) == 2;
+    T* dst = C + (turned ? (long long)col0 * ld + row0 : (long long)row0 * ld + col0);
+    if (turned) {
+      if constexpr (BF16 && !ADD) {
+        if (wide) {
+          __syncwarp();
 #pragma unroll
-          for (int q = 0; q < 8; ++q)
-            if (4 * q < cols) *reinterpret_cast<uint4*>(dst + 4 * q) = make_uint4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (i < cols) dst[i * step] = accumulate ? dst[i * step] + __uint_as_float(v[i]) : __uint_as_float(v[i]);
+          for (int i = 0; i < 32; ++i) sts_bf16(box_row_chunk(box, i, lane >> 3) + (lane & 7) * 2, __uint_as_float(v[i]));
+          copy_box(box, lane, dst, cols, rows);
+          return;
         }
       }
+      if (lane < rows) put_each(dst + lane, v, cols);
       return;
     }
-    if (turned) {
-      __nv_bfloat16* dst = C + (long long)col0 * ld + row0;
-      if (wide && !accumulate) {
-        __syncwarp();
-#pragma unroll
-        for (int i = 0; i < 32; ++i) sts_bf16(box_row_chunk(box, i, lane >> 3) + (lane & 7) * 2, __uint_as_float(v[i]));
-        copy_box(box, lane, dst, cols, rows);
-      } else if (lane < rows) {
-#pragma unroll
-        for (int i = 0; i < 32; ++i)
-          if (i < cols) add_or_set(dst + i * ld + lane, __uint_as_float(v[i]));
-      }
-      return;
-    }
-    __nv_bfloat16* dst = C + (long long)row0 * ld + col0;
-    if (!accumulate) {
+    if constexpr (BF16 && !ADD) {
       const Rows32 own = pack_row32(v);
       __syncwarp();
 #pragma unroll
@@ -177,20 +170,68 @@ struct Output {
         for (int r = 0; r < rows; ++r)
           if (lane < cols) reinterpret_cast<unsigned short*>(dst)[r * ld + lane] = lds_u16(box_row_chunk(box, r, lane >> 3) + (lane & 7) * 2);
       }
+    } else if (!wide || (ADD && !BF16)) {
+      put_rows(box, lane, dst, v, rows, cols);
     } else if (lane < rows) {
-      dst += lane * ld;
-      if (wide) {
-        store_chunk<__nv_bfloat16>(dst, v, cols, true, nullptr);
+      if constexpr (BF16) {
+        store_chunk<T>(dst + lane * ld, v, cols, true, nullptr);
       } else {
 #pragma unroll
-        for (int i = 0; i < 32; ++i)
-          if (i < cols) add_or_set(dst + i, __uint_as_float(v[i]));
+        for (int q = 0; q < 8; ++q)
+          if (4 * q < cols) *reinterpret_cast<uint4*>(dst + lane * ld + 4 * q) = make_uint4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
       }
     }
   }
 
  private:
-  __device__ __forceinline__ void add_or_set(__nv_bfloat16* p, float v) const { *p = __float2bfloat16(accumulate ? __bfloat162float(*p) + v : v); }
+  static __device__ __forceinline__ float sum(float old, uint32_t v) { return ADD ? old + __uint_as_float(v) : __uint_as_float(v); }
+  static __device__ __forceinline__ float read(const T* p) {
+    if constexpr (sizeof(T) == 2) return __bfloat162float(*p);
+    else return *p;
+  }
+  static __device__ __forceinline__ void write(T* p, float v) {
+    if constexpr (sizeof(T) == 2) *p = __float2bfloat16(v);
+    else *p = v;
+  }
+  // What is added to is read ahead of the stores, 16 at once: behind a store that might be to the same place each read would wait for the
+  // one before (us, added to 14 336 x 4096 from 2048: 1492 -> 202, all 32 at once, which spills, 314).
+  //
+  // Rows of the output, 32 neighbours from the warp's lanes
+  __device__ __forceinline__ void put_each(T* dst, const uint32_t (&v)[32], int cols) const {
+#pragma unroll
+    for (int h = 0; h < 32; h += 16) {
+      float old[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) old[i] = ADD && h + i < cols ? read(dst + (h + i) * ld) : 0.f;
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (h + i < cols) write(dst + (h + i) * ld, sum(old[i], v[h + i]));
+    }
+  }
+  // A row of the output from a lane: 16 columns at a time go through the warp's box, so that an instruction writes 16 neighbours of two rows.
+  // The word of a row is permuted by its number, which keeps both ways through the box free of bank conflicts.  (us, added to 1001 x 4097 from
+  // 1024 110 -> 32, a row per lane with the reads ahead 332; 4096 x 4096 in fp32 from 4096 222 -> 93, in words of 16 bytes per lane 290.)
+  __device__ __forceinline__ void put_rows(uint32_t box, int lane, T* dst, const uint32_t (&v)[32], int rows, int cols) const {
+    const int half = lane >> 4, c = lane & 15;
+#pragma unroll
+    for (int h = 0; h < 32; h += 16) {
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < 16; ++i) sts32(box + lane * 64 + ((i ^ (lane >> 1)) << 2), v[h + i]);
+      __syncwarp();
+#pragma unroll 1
+      for (int r0 = half; r0 < rows; r0 += 16) {
+        float old[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) old[j] = ADD && r0 + 2 * j < rows && h + c < cols ? read(dst + (r0 + 2 * j) * ld + h + c) : 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int r = r0 + 2 * j;
+          if (r < rows && h + c < cols) write(dst + r * ld + h + c, sum(old[j], lds32(box + r * 64 + ((c ^ (r >> 1)) << 2))));
+        }
+      }
+    }
+  }
   static __device__ __forceinline__ void sts_bf16(uint32_t addr, float v) {
     asm volatile("st.shared.u16 [%0], %1;" ::"r"(addr), "h"(__bfloat16_as_ushort(__float2bfloat16(v))) : "memory");
   }
@@ -204,10 +245,11 @@ struct Output {
   }
 };
 
+template <typename T, bool ADD>
 __global__ void __launch_bounds__(THREADS, 1)
 kf_gemm_fp8_blocks_2cta(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                         const __grid_constant__ CUtensorMap map_sa, const __grid_constant__ CUtensorMap map_sb,
-                        const Output out, int M, int N, int K, int a_fmt, int b_fmt, int tile_n, int* status) {
+                        const Output<T, ADD> out, int M, int N, int K, int a_fmt, int b_fmt, int tile_n, int* status) {
   extern __shared__ uint8_t smem_raw[];
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   const uint32_t sf_smem = smem_base + STAGES * STAGE_BYTES;
@@ -502,7 +544,8 @@ struct Cut {
 };
 // The cheapest by what was measured, in ns: a block of 128 takes 0.66 (columns + 250) on a pair while all of them ask for operands (64 columns
 // 207, 128 250, 192 300, 224 313), the last tile's way out 4.5 a column, and the sum over a cluster its barriers and its copies.  Of 74 pairs
-// 33 clusters of two fit, and 15 of four.  us, graph of launches on weights in turn, cut by columns only -> so: 200 x 4096 from 14 336 36.5 ->
+// 33 clusters of two fit, and 15 of four; one is left free, since the last of a launch right behind another had to wait (13.3 us for 339 x 576 from
+// 8064 in 33 clusters, in 12 of four 9.9).  us, graph of launches on weights in turn, cut by columns only -> so: 200 x 4096 from 14 336 36.5 ->
 // 21.1, 64 x 4096 from 4096 12.5 -> 10.4, 1554 x 7168 from 5120 50.9 -> 45.0, 2000 x 2048 from 2048 14.9 -> 12.3, 120 x 1304 from 952 6.6 -> 6.0.
 static Cut cut_of(int M, int N, int K, int num_sms) {
   const int pairs = num_sms / 2, k_blocks = (K + BK - 1) / BK;
@@ -514,7 +557,7 @@ static Cut cut_of(int M, int N, int K, int num_sms) {
       if (tn - 32 >= n) continue;
       const long long tiles = (long long)m_blocks * ((n + tn - 1) / tn);
       for (int splits = 1; splits <= 4; splits *= 2) {
-        if (splits > 1 && (tiles * splits > pairs - (splits == 2 ? 8 : 14) || k_blocks < splits)) break;
+        if (splits > 1 && (tiles * splits > pairs - (splits == 2 ? 10 : 18) || k_blocks < splits)) break;
         const long long rounds = splits > 1 ? 1 : (tiles + pairs - 1) / pairs;
         const float cost = float(rounds * ((k_blocks + splits - 1) / splits)) * 0.66f * float(tn + 250) + 4.5f * float(tn) +
                            (splits == 1 ? 0.f : splits == 2 ? 600.f + 13.f * float(tn) : 1200.f + 20.f * float(tn));
@@ -526,6 +569,21 @@ static Cut cut_of(int M, int N, int K, int num_sms) {
     }
   }
   return best;
+}
+
+template <typename T, bool ADD>
+static int launch_blocks(const Output<T, ADD>& out, int clusters, int splits, cudaStream_t stream, const CUtensorMap& ma, const CUtensorMap& mb,
+                         const CUtensorMap& msa, const CUtensorMap& msb, int M, int N, int K, int a_fmt, int b_fmt, int tile_n, int* status) {
+  static bool attr_set[64] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev >= 64 || !attr_set[dev]) {
+    cudaError_t e = cudaFuncSetAttribute(kf_gemm_fp8_blocks_2cta<T, ADD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM);
+    if (e != cudaSuccess) return 300 + (int)e;
+    if (dev < 64) attr_set[dev] = true;
+  }
+  return launch_programmatic(kf_gemm_fp8_blocks_2cta<T, ADD>, dim3(unsigned(clusters * 2 * splits)), THREADS, SMEM, 2 * splits, stream, ma, mb, msa,
+                             msb, out, M, N, K, a_fmt, b_fmt, tile_n, status);
 }
 
 // gemm_fp8_blocks_few.cu
@@ -568,18 +626,13 @@ int kf_gemm_fp8_blocks(const void* A, const void* sa, const void* B, const void*
   if ((rc = make_map_u8(&mb, B, N, K, ldb, BK, tile_n / 2, true))) return 200 + rc;
   if ((rc = make_map_u8(&msa, sa, k_blocks, M, ldsa, CTA_M, GROUP, false))) return 100 + rc;
   if ((rc = make_map_u8(&msb, sb, k_blocks, N, ldsb, tile_n, GROUP, false))) return 200 + rc;
-  static bool attr_set[64] = {};
-  int dev = 0;
-  cudaGetDevice(&dev);
-  if (dev >= 64 || !attr_set[dev]) {
-    cudaError_t e = cudaFuncSetAttribute(kf_gemm_fp8_blocks_2cta, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM);
-    if (e != cudaSuccess) return 300 + (int)e;
-    if (dev < 64) attr_set[dev] = true;
-  }
   const int clusters = cut.splits > 1 ? (int)tiles : (int)(tiles < num_sms / 2 ? tiles : num_sms / 2);
-  const Output out{reinterpret_cast<__nv_bfloat16*>(C), f32 ? reinterpret_cast<float*>(C) : nullptr, ldc, cut.turned, accumulate, wide};
-  return launch_programmatic(kf_gemm_fp8_blocks_2cta, dim3(unsigned(clusters * 2 * cut.splits)), THREADS, SMEM, 2 * cut.splits, (cudaStream_t)stream,
-                             ma, mb, msa, msb, out, M, N, K, a_fmt, b_fmt, tile_n, status);
+  auto launch = [&](auto* c, auto add) {
+    using Out = Output<std::remove_pointer_t<decltype(c)>, decltype(add)::value>;
+    return launch_blocks(Out{c, ldc, cut.turned, wide}, clusters, cut.splits, (cudaStream_t)stream, ma, mb, msa, msb, M, N, K, a_fmt, b_fmt, tile_n, status);
+  };
+  if (f32) return accumulate ? launch((float*)C, std::true_type{}) : launch((float*)C, std::false_type{});
+  return accumulate ? launch((__nv_bfloat16*)C, std::true_type{}) : launch((__nv_bfloat16*)C, std::false_type{});
 }
 
 }  // extern "C"

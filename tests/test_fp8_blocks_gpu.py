@@ -143,6 +143,21 @@ def test_product_adds_into_a_pitched_output_and_leaves_the_rest(native_lib, m, n
     assert native_lib.read_status() == 0
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("m, n, k", [(40, 4104, 300), (300, 520, 384), (1304, 296, 4096), (72, 2008, 2048), (2008, 72, 520), (1800, 7256, 136)])
+def test_product_adds_into_a_contiguous_output(native_lib, m, n, k, dtype):
+    a, b, av, bv = _mm_case(m, n, k, False, False, 17)
+    want, mag = av @ bv.t(), av.abs() @ bv.abs().t()
+    old = _spread(m, n, 3, dtype)
+    out = fb.mm(a, b, out=old.clone(), accumulate=True)
+    total, size = want + old.double(), mag + old.double().abs()
+    if dtype == torch.bfloat16:
+        assert _mm_close(out, total, size, k)
+    else:
+        assert bool(((out.double() - total).abs() <= (k + 4) * 2.0**-23 * size + 1e-38).all())
+    assert native_lib.read_status() == 0
+
+
 def test_product_of_slices_and_of_scales_at_the_ends(native_lib):
     a, b, av, bv = _mm_case(40, 72, 512, False, False, 9)
     part = fb.mm(fb.BlockScaled(a.values[3:20, 128:384], a.scales[1:3, 3:20]), fb.BlockScaled(b.values[5:, 128:384], b.scales[1:3, 5:]))
