@@ -3,7 +3,7 @@
 //
 //   cast    q = round8(x 2^-e), e from the largest magnitude of a block: 1 x 128 (activations, gradients) or 128 x 128 (weights, whose two
 //           copies then hold the same values).  A transposed copy of 1 x 128 blocks has blocks of 128 along the rows of x.
-//   norm    t = bf16(x + residual), rstd = 1 / sqrt(mean(t^2) + eps), h = cast(t gain rstd), the products in 32 bits
+//   norm    t = bf16(x + residual), rstd = 1 / sqrt(mean(t^2) + eps), h = cast(t gain rstd), rounded once
 //   norm's gradients  dx = dt + rstd (dh gain - t rstd^2 mean(dh gain t)), dgain = sum over rows of dh t rstd, of dh in 32 bits
 //
 // The kernels are programmatic launches, so no pointer is promised to be the only one to its memory: a load under that promise may be moved
@@ -285,13 +285,32 @@ __device__ __forceinline__ T block_sum(T v, T* red) {
   return v;
 }
 
+// the square of a bf16's magnitude (the low 16 bits of w, or the high ones) in 64 bits; subnormal numbers and zeros count as 2^-127 or a little
+// more, whose squares are nothing in the 32 bits that a sum ends in, infinities and NaN as 2^128
+__device__ __forceinline__ double square64(uint32_t w, bool high) {
+  const uint32_t u = high ? (w >> 3) & 0x0fffe000u : (w & 0x7fffu) << 13;
+  const double a = __hiloint2double(int(u + (uint32_t(1023 - 127) << 20)), 0);
+  return a * a;
+}
+// p (hi + lo) on its way to 8 bits: towards zero, and odd where anything was cut off, which tells any shorter rounding on which side of a border
+// the product is.  p has 16 bits, hi + lo 48, so only a hi of up to 8 bits without a lo can be exact (cut = 0).
+__device__ __forceinline__ float times_odd(float p, float hi, float lo, uint32_t cut) {
+  float r;
+  asm("fma.rz.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(p), "f"(hi), "f"(mul_full(p, lo)));
+  return __uint_as_float(__float_as_uint(r) | cut);
+}
+
 // One row per block of THREADS threads, VPT vectors of eight columns per thread held in registers; 16 neighbouring threads have a block
 // of 128 columns between them.  Vector c of a thread is c * THREADS + thread.
+//
+// Bound by memory: 4 bytes an element in, 3 out.  us (at the copy rate): 16 384 x 4096 74 (72), 4096 x 4096 23 (18), 777 x 5120 9.2 (4.3), one row
+// 3.2.  The sum and rstd in 64 bits and the products that keep what they cut off cost 2 to 7 % of that (73, 21.5, 8.6, 3.0 in 32 bits, where one byte in
+// two million was the neighbour of the right one).
 template <int THREADS, int VPT>
 __global__ void __launch_bounds__(THREADS)
 kf_add_rmsnorm_blocks(const __nv_bfloat16* x, const __nv_bfloat16* residual, const __nv_bfloat16* gain,
                       __nv_bfloat16* t_out, float* rstd_out, uint8_t* out, long long ld_out,
-                      uint8_t* scales, long long ld_scales, int D, float eps) {
+                      uint8_t* scales, long long ld_scales, int D, double per_D, double eps) {
   __shared__ double red[32];
   const size_t row = blockIdx.x;
   const int nvec = D >> 3;
@@ -308,7 +327,7 @@ kf_add_rmsnorm_blocks(const __nv_bfloat16* x, const __nv_bfloat16* residual, con
       if (residual) rv[c] = *reinterpret_cast<const uint4*>(residual + row * D + i * 8);
     }
   }
-  float ss = 0.f;
+  double sum = 0.;
 #pragma unroll
   for (int c = 0; c < VPT; ++c) {
     const int i = threadIdx.x + c * THREADS;
@@ -322,17 +341,43 @@ kf_add_rmsnorm_blocks(const __nv_bfloat16* x, const __nv_bfloat16* residual, con
       v[c] = make_uint4(w[0], w[1], w[2], w[3]);
       if (i < nvec) *reinterpret_cast<uint4*>(t_out + row * D + i * 8) = v[c];
     }
+    if (i < nvec) {
+      const uint32_t w[4] = {v[c].x, v[c].y, v[c].z, v[c].w};
+      double even = 0., odd = 0.;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float2 a = pair_at(v[c], j);
-      ss += a.x * a.x;
-      ss += a.y * a.y;
+      for (int j = 0; j < 4; ++j) {
+        even += square64(w[j], false);
+        odd += square64(w[j], true);
+      }
+      sum += even + odd;
     }
   }
-  // What the 24th bit of rstd says decides, next to a border, which of two 8-bit neighbours all values of a row go to: threads' sums are added
-  // in 64 bits, and division and root are those that round to the nearest.
-  const float r = __frsqrt_rn(__fadd_rn(__fdiv_rn(float(block_sum<THREADS>(double(ss), red)), float(D)), eps));
+  // rstd = r + lo: its 24th bit says, for values next to a border, which of two 8-bit neighbours they go to, and with it they go where the
+  // formula says.  One step of Newton's iteration for 1 / sqrt from the nearest 32-bit number.
+  double mean = block_sum<THREADS>(sum, red) * per_D + eps;
+  if (mean > 3.4e38) {  // infinities, NaN and sums that 32 bits do not hold: as they are there
+    float ss = 0.f;
+#pragma unroll
+    for (int c = 0; c < VPT; ++c)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 a = pair_at(v[c], j);
+        ss += a.x * a.x + a.y * a.y;
+      }
+    __syncthreads();
+    mean = block_sum<THREADS>(double(ss), red);
+  }
+  const float first = __frsqrt_rn(float(mean));
+  float r = first, lo = 0.f;
+  if (first > 0.f && first <= 3.4e38f) {
+    const double y = first;
+    lo = first * (0.5f * float(1. - mean * (y * y)));
+    r = add_full(first, lo);
+    lo = add_full(lo, add_full(first, -r));
+  }
+  const uint32_t cut = lo == 0.f && (__float_as_uint(r) & 0xffffu) == 0 ? 0u : 1u;
   if (threadIdx.x == 0 && rstd_out) rstd_out[row] = r;
+  const float largest = __uint_as_float(0x7f7fffffu);
 #pragma unroll
   for (int c = 0; c < VPT; ++c) {
     const int i = threadIdx.x + c * THREADS;
@@ -341,21 +386,22 @@ kf_add_rmsnorm_blocks(const __nv_bfloat16* x, const __nv_bfloat16* residual, con
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const float2 a = pair_at(v[c], j), g = pair_at(gv, j);
-      f[2 * j] = mul_full(mul_full(a.x, g.x), r);  // the first product is exact: 16 bits
-      f[2 * j + 1] = mul_full(mul_full(a.y, g.y), r);
+      f[2 * j] = times_odd(mul_full(a.x, g.x), r, lo, cut);  // the first product is exact: 16 bits
+      f[2 * j + 1] = times_odd(mul_full(a.y, g.y), r, lo, cut);
       m = max_abs(max_abs(m, f[2 * j]), f[2 * j + 1]);
     }
     m = half_warp_max(m);
-    if (is_inf(m)) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) f[e] = nan_if_inf(f[e]);
-    }
-    if (__any_sync(0xffffffffu, is_inf(m))) {  // rare: the largest finite value (a half without an infinity gets the same again)
+    // rare: towards zero, what 32 bits do not hold ends on their largest number.  (A half warp without one gets the same maximum again.)
+    if (__any_sync(0xffffffffu, m >= largest)) {
       m = 0.f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) m = max_abs(m, f[e]);
+      for (int e = 0; e < 8; ++e) {
+        if (fabsf(f[e]) >= largest) f[e] = __uint_as_float(0x7fffffffu);
+        m = max_abs(m, f[e]);
+      }
       m = half_warp_max(m);
     }
+    if (__float_as_uint(m) <= 1u) m = 0.f;  // zeros with their last bit set
     const uint32_t b = scale_byte<false>(m);
     const float inv = inverse_of(b);
     if (i < nvec) {
@@ -539,7 +585,7 @@ int kf_add_rmsnorm_fp8_blocks(const void* x, const void* residual, const void* g
     return 5;
   auto go = [&](auto kern, int threads) {
     return launch_programmatic(kern, dim3(unsigned(rows)), threads, 0, 1, (cudaStream_t)stream, (const __nv_bfloat16*)x, (const __nv_bfloat16*)residual,
-                               (const __nv_bfloat16*)gain, (__nv_bfloat16*)t, (float*)rstd, (uint8_t*)out, ld_out, (uint8_t*)scales, ld_scales, D, eps);
+                               (const __nv_bfloat16*)gain, (__nv_bfloat16*)t, (float*)rstd, (uint8_t*)out, ld_out, (uint8_t*)scales, ld_scales, D, 1. / D, double(eps));
   };
   if (D <= 1024) return go(kf_add_rmsnorm_blocks<32, 4>, 32);
   if (D <= 4096) return go(kf_add_rmsnorm_blocks<128, 4>, 128);

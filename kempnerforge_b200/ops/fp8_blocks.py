@@ -203,8 +203,9 @@ def _pitched(t: torch.Tensor) -> torch.Tensor:
 
 def add_rmsnorm(x: torch.Tensor, residual: torch.Tensor | None, weight: torch.Tensor, eps: float = 1e-5):
     """(t, rstd, h) of bf16 matrices (rows, d), d a multiple of 8 up to 32 768: t = x + residual rounded to bf16 (x itself without one),
-    rstd = 1 / sqrt(mean(t²) + eps) as fp32 (rows,), h = (t * weight) * rstd in 8 bits, never rounded to 16.  Not differentiable by itself:
-    :func:`norm_linear` is."""
+    rstd = 1 / sqrt(mean(t²) + eps) as fp32 (rows,), h = (t * weight) * rstd in 8 bits, never rounded to 16 (on a GPU not to 32
+    either: rstd has more bits there than are returned, and h is the 8-bit number next to the formula's value).  Not differentiable by
+    itself: :func:`norm_linear` is."""
     if x.is_cuda and (r := _cuda()._step("fp8_add_rmsnorm", x, residual, weight, eps)) is not None:
         t, rstd, q, s = r
         return x.detach() if t is None else t, rstd, BlockScaled(q, s)

@@ -187,6 +187,17 @@ def test_what_is_not_finite_stays_in_its_row_and_column(native_lib):
     assert torch.equal(got[~bad], clean[~bad])
 
 
+def _cast64(v):
+    """Bytes and block-major scales of finite `v` (rows, k) in 64 bits, e4m3, from the definition."""
+    rows, k = v.shape
+    blocks = torch.nn.functional.pad(v, (0, -k % 128)).view(rows, -1, 128)
+    mant, ex = torch.frexp(blocks.abs().amax(2))
+    e = torch.where(mant > 0, (ex - 9 + (mant > 0.875)).clamp_min(-126), 0)
+    q = blocks * torch.exp2(-e.double())[:, :, None]
+    step = torch.exp2((torch.frexp(q)[1] - 1).clamp_min(-6).double() - 3)
+    return (torch.round(q / step) * step).view(rows, -1)[:, :k].float().to(torch.float8_e4m3fn).view(torch.uint8), (e + 127).t().to(torch.uint8)
+
+
 NORM = [(1, 8), (1, 4096), (3, 136), (5, 1024), (130, 1032), (64, 4104), (33, 8200), (2, 16392), (2, 32768), (1000, 776)]
 
 
@@ -200,7 +211,8 @@ def test_norm(native_lib, rows, d, with_residual):
     want = (t.double().square().mean(1) + 1e-5).rsqrt()
     # a sum of d squares (2^-24 each, at most d of them one after another) under a square root, and an approximate one (2^-22)
     assert bool(((rstd.double() - want).abs() <= want * (d * 2.0**-25 + 2.0**-21)).all())
-    assert _same(h, fb._cast_rows(t.float() * gain.float() * rstd[:, None], False))
+    q, scales = _cast64(t.double() * gain.double() / (t.double().square().mean(1) + torch.tensor(1e-5).double()).sqrt()[:, None])
+    assert torch.equal(h.scales, scales) and torch.equal(h.values, q)
     normed = fb._normed_t(t, rstd, gain)
     assert _same(normed, fb._cast_rows((t.float() * gain.float() * rstd[:, None]).t().contiguous(), False))
     again = fb.add_rmsnorm(x, residual, gain, 1e-5)
@@ -219,6 +231,27 @@ def test_norm_of_rows_with_infinities_and_zeros(native_lib):
     got = fb.add_rmsnorm(x[4:], None, gain)[2]
     assert _same(got, fb._cast_rows(x[4:].float() * gain.float() * fb.add_rmsnorm(x[4:], None, gain)[1][:, None], False))
     assert fb._values(got).isnan().sum() == 2
+
+
+def test_norm_of_rows_at_the_ends_of_the_types(native_lib):
+    one = lambda *s: torch.ones(*s, device=DEV, dtype=torch.bfloat16)   # noqa: E731
+    # rstd a power of two: products are exact, and halfway between two 8-bit numbers they go to the even one
+    gain = torch.tensor([1, 1.0625, 1.1875, 1.9375, 448, 416, 1.4375, -1.0625], device=DEV).bfloat16()
+    for size in (1.0, 2.0**-12, 2.0**30):
+        t, rstd, h = fb.add_rmsnorm(size * one(3, 8), None, gain, 0.0)
+        assert bool((rstd == 1 / size).all())
+        assert fb._values(h).tolist() == [[1, 1, 1.25, 2, 448, 416, 1.5, -1]] * 3
+    # a product that 32 bits do not hold is NaN, the rest of its block scaled as if it were not there
+    x, big = 2.0**-10 * one(1, 8), torch.full((8,), 3.3e38, device=DEV).bfloat16()
+    x[0, 2], big[5] = 2.0**-8, 0
+    v = fb._values(fb.add_rmsnorm(x, None, big, 0.0)[2])[0]
+    want = big.double()[0] / (x.double().square().mean()).sqrt() * 2.0**-10
+    assert v[2].isnan() and v[5] == 0 and bool(((v[[0, 1, 3, 4, 6, 7]].double() - want).abs() <= want * 2.0**-4).all())
+    # squares that 32 bits do not hold: rstd is 0, and so are the finite values; a row of zeros without eps has none
+    t, rstd, h = fb.add_rmsnorm(torch.cat([1e30 * one(1, 8), -1e30 * one(1, 8), 0 * one(1, 8)]), None, one(8), 0.0)
+    assert rstd[:2].tolist() == [0, 0] and not fb._values(h)[:2].any() and h.scales[:, :2].tolist() == [[127, 127]]
+    assert rstd[2].isinf() and fb._values(h)[2].isnan().all()
+    assert native_lib.read_status() == 0
 
 
 def _layer(tokens, d, outs, seed=0, grads=True):
