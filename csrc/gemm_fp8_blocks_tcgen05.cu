@@ -155,6 +155,9 @@ struct Output {
           return;
         }
       }
+      if constexpr (!(BF16 && !ADD)) {
+        if (wide) return put_words<true>(box, lane, dst, v, cols, rows);
+      }
       if (lane < rows) put_each(dst + lane, v, cols);
       return;
     }
@@ -170,16 +173,10 @@ struct Output {
         for (int r = 0; r < rows; ++r)
           if (lane < cols) reinterpret_cast<unsigned short*>(dst)[r * ld + lane] = lds_u16(box_row_chunk(box, r, lane >> 3) + (lane & 7) * 2);
       }
-    } else if (!wide || (ADD && !BF16)) {
+    } else if (!wide) {
       put_rows(box, lane, dst, v, rows, cols);
-    } else if (lane < rows) {
-      if constexpr (BF16) {
-        store_chunk<T>(dst + lane * ld, v, cols, true, nullptr);
-      } else {
-#pragma unroll
-        for (int q = 0; q < 8; ++q)
-          if (4 * q < cols) *reinterpret_cast<uint4*>(dst + lane * ld + 4 * q) = make_uint4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
-      }
+    } else {
+      put_words<false>(box, lane, dst, v, rows, cols);
     }
   }
 
@@ -193,8 +190,8 @@ struct Output {
     if constexpr (sizeof(T) == 2) *p = __float2bfloat16(v);
     else *p = v;
   }
-  // What is added to is read ahead of the stores, 16 at once: behind a store that might be to the same place each read would wait for the
-  // one before (us, added to 14 336 x 4096 from 2048: 1492 -> 202, all 32 at once, which spills, 314).
+  // What is added to is read ahead of the stores: behind a store that might be to the same place each read would wait for the one before (us,
+  // added to 1001 x 4097 from 1024 in bf16 110 -> 28, 777 x 1001 from 999 in fp32 31 -> 9.4).
   //
   // Rows of the output, 32 neighbours from the warp's lanes
   __device__ __forceinline__ void put_each(T* dst, const uint32_t (&v)[32], int cols) const {
@@ -209,8 +206,8 @@ struct Output {
     }
   }
   // A row of the output from a lane: 16 columns at a time go through the warp's box, so that an instruction writes 16 neighbours of two rows.
-  // The word of a row is permuted by its number, which keeps both ways through the box free of bank conflicts.  (us, added to 1001 x 4097 from
-  // 1024 110 -> 32, a row per lane with the reads ahead 332; 4096 x 4096 in fp32 from 4096 222 -> 93, in words of 16 bytes per lane 290.)
+  // The word of a row is permuted by its number, which keeps both ways through the box free of bank conflicts.  (A row per lane with the reads
+  // ahead: 332 us for those 28.)
   __device__ __forceinline__ void put_rows(uint32_t box, int lane, T* dst, const uint32_t (&v)[32], int rows, int cols) const {
     const int half = lane >> 4, c = lane & 15;
 #pragma unroll
@@ -231,6 +228,60 @@ struct Output {
         }
       }
     }
+  }
+  // rows x cols of the output in words of 16 bytes, each row's by neighbouring lanes; with TURNED v holds columns of it.  Half of the values go
+  // through the box at a time, as 32 rows of 16 or 16 rows of 32, with 16-byte words permuted so that no way through it has bank conflicts.
+  // A word per lane's own row fills half a sector at a time, single values are many instructions (us, 4096 x 4096 from 6144 in fp32 92 -> 83; from
+  // 4096 64 -> 55, added to 222 -> 65, in bf16 70 -> 57), and with all that is added to read first its way is waited for once (added to 14 336 x 4096
+  // from 2048, bf16, 1492 -> 134, in fp32 1499 -> 154).
+  template <bool TURNED>
+  __device__ __forceinline__ void put_words(uint32_t box, int lane, T* dst, const uint32_t (&v)[32], int rows, int cols) const {
+    constexpr int PER = 16 / sizeof(T), W = TURNED ? 32 : 16, LANES = W / PER, STEP = 32 / LANES, N = 16 / PER;
+    const int r0 = lane / LANES, c = lane % LANES * PER;
+    auto at = [&](int row, int word) { return box + row * (4 * W) + ((word ^ (TURNED ? row & 1 : (row >> 1) & 3)) << 4); };
+    const long long step = STEP * ld, half = TURNED ? 16 * ld : 16;
+    T* const to = dst + r0 * ld + c;
+    // row i and half h of this lane's words exist
+    auto exists = [&](int i, int h) { return r0 + (TURNED ? h : 0) + i * STEP < rows && (TURNED ? 0 : h) + c < cols; };
+    uint4 old[2][N];
+    if constexpr (ADD) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+          if (exists(i, 16 * h)) old[h][i] = *reinterpret_cast<const uint4*>(to + h * half + i * step);
+    }
+#pragma unroll
+    for (int h = 0; h < 32; h += 16) {
+      __syncwarp();
+      if constexpr (TURNED) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sts32(at(i, lane >> 2) + (lane & 3) * 4, v[h + i]);
+      } else {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) sts128(at(lane, q), make_uint4(v[h + 4 * q], v[h + 4 * q + 1], v[h + 4 * q + 2], v[h + 4 * q + 3]));
+      }
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int r = r0 + i * STEP;
+        const uint4 a = lds128(at(r, c >> 2));
+        const uint4 o = old[h >> 4][i];
+        uint4 w;
+        if constexpr (PER == 4) {
+          w = make_uint4(plus(o.x, a.x), plus(o.y, a.y), plus(o.z, a.z), plus(o.w, a.w));
+        } else {
+          const uint4 b = lds128(at(r, (c >> 2) + 1));
+          w = make_uint4(plus2(o.x, a.x, a.y), plus2(o.y, a.z, a.w), plus2(o.z, b.x, b.y), plus2(o.w, b.z, b.w));
+        }
+        if (exists(i, h)) *reinterpret_cast<uint4*>(to + (h >> 4) * half + i * step) = w;
+      }
+    }
+  }
+  static __device__ __forceinline__ uint32_t plus(uint32_t old, uint32_t v) { return __float_as_uint(sum(__uint_as_float(old), v)); }
+  static __device__ __forceinline__ uint32_t plus2(uint32_t old, uint32_t v, uint32_t w) {
+    const float2 o = unpack_bf16(old);
+    return pack_bf16(sum(o.x, v), sum(o.y, w));
   }
   static __device__ __forceinline__ void sts_bf16(uint32_t addr, float v) {
     asm volatile("st.shared.u16 [%0], %1;" ::"r"(addr), "h"(__bfloat16_as_ushort(__float2bfloat16(v))) : "memory");
@@ -448,12 +499,21 @@ kf_gemm_fp8_blocks_2cta(const __grid_constant__ CUtensorMap map_a, const __grid_
       const int row0 = tm * TILE_M + int(rank) * CTA_M + quarter * 32;  // this warp's rows, and how many exist
       const int rows = max(0, min(32, M - row0));
       const int col0 = tn * tile_n, width = min(tile_n, N - col0);
-      // the next 32 columns are under way while these are stored
+      // the next 32 columns are under way while these are stored; where the output is read too, its values need the registers
       const uint32_t from = t_row + acc * MAX_N;
       uint32_t v[32], w[32];
-      tmem_ld_32x32(from, v);
+      if constexpr (ADD) {
 #pragma unroll 1
-      for (int c = 0; c < width; c += 64) {
+        for (int c = 0; c < width; c += 32) {
+          tmem_ld_32x32(from + c, v);
+          tmem_ld_wait();
+          out.put(box, lane, v, row0, col0 + c, rows, min(32, width - c));
+        }
+      } else {
+        tmem_ld_32x32(from, v);
+      }
+#pragma unroll 1
+      for (int c = ADD ? width : 0; c < width; c += 64) {
         tmem_ld_wait();
         if (c + 32 < width) tmem_ld_32x32(from + c + 32, w);
         out.put(box, lane, v, row0, col0 + c, rows, min(32, width - c));
