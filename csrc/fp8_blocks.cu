@@ -365,7 +365,7 @@ kf_add_rmsnorm_blocks(const __nv_bfloat16* x, const __nv_bfloat16* residual, con
         ss += a.x * a.x + a.y * a.y;
       }
     __syncthreads();
-    mean = block_sum<THREADS>(double(ss), red);
+    mean = block_sum<THREADS>(double(ss), red) * per_D + eps;
   }
   const float first = __frsqrt_rn(float(mean));
   float r = first, lo = 0.f;
@@ -577,7 +577,7 @@ int kf_fp8_blocks_cast_bf16(const void* x, int rows, int cols, long long ldx, co
 // t = bf16(x + residual) (x itself, and nothing is written, where residual is null), rstd, and RMSNorm(t) * gain in e4m3.  x, residual, t:
 // contiguous rows of D bf16 values on 16 bytes, D a multiple of 8, at most 32 768; pitch ld_out a multiple of 8.
 int kf_add_rmsnorm_fp8_blocks(const void* x, const void* residual, const void* gain, void* t, void* rstd, void* out, long long ld_out,
-                              void* scales, long long ld_scales, int rows, int D, float eps, void* stream) {
+                              void* scales, long long ld_scales, int rows, int D, double eps, void* stream) {
   using namespace kf::f8b;
   if (rows <= 0 || D <= 0 || (D & 7) || D > 32768 || (ld_out & 7) ||
       ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(residual) | reinterpret_cast<uintptr_t>(gain) | reinterpret_cast<uintptr_t>(t)) & 15) ||
@@ -585,7 +585,8 @@ int kf_add_rmsnorm_fp8_blocks(const void* x, const void* residual, const void* g
     return 5;
   auto go = [&](auto kern, int threads) {
     return launch_programmatic(kern, dim3(unsigned(rows)), threads, 0, 1, (cudaStream_t)stream, (const __nv_bfloat16*)x, (const __nv_bfloat16*)residual,
-                               (const __nv_bfloat16*)gain, (__nv_bfloat16*)t, (float*)rstd, (uint8_t*)out, ld_out, (uint8_t*)scales, ld_scales, D, 1. / D, double(eps));
+                               (const __nv_bfloat16*)gain, (__nv_bfloat16*)t, (float*)rstd, (uint8_t*)out, ld_out, (uint8_t*)scales, ld_scales, D, 1. / D,
+                               eps);
   };
   if (D <= 1024) return go(kf_add_rmsnorm_blocks<32, 4>, 32);
   if (D <= 4096) return go(kf_add_rmsnorm_blocks<128, 4>, 128);

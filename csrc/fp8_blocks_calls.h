@@ -14,7 +14,7 @@ namespace {
 struct Fp8Blocks {
   int (*gemm)(const void*, const void*, const void*, const void*, void*, int, int, int, long long, long long, long long, long long, long long, int,
               int, int, int, int, void*) = nullptr;
-  int (*norm)(const void*, const void*, const void*, void*, void*, void*, long long, void*, long long, int, int, float, void*) = nullptr;
+  int (*norm)(const void*, const void*, const void*, void*, void*, void*, long long, void*, long long, int, int, double, void*) = nullptr;
   int (*cast)(const void*, int, int, long long, const void*, const void*, int, int, void*, long long, void*, long long, void*, long long, void*,
               long long, void*) = nullptr;
   int (*values)(const void*, long long, const void*, long long, int, int, int, void*, void*) = nullptr;
@@ -22,7 +22,7 @@ struct Fp8Blocks {
   int (*norm_grads_blocks)(int, int, int) = nullptr;
 } f8;
 
-constexpr long long kLargest = 0x7fffffff;
+constexpr long long kLargest = 0x7fff0000;  // kernels add a few blocks to an index in 32 bits
 
 // A plain dense CUDA tensor of this type and rank on the given device.
 const at::Tensor* dense(PyObject* o, at::ScalarType type, long rank, long device) {
@@ -96,7 +96,7 @@ int norm(const at::Tensor& x, const at::Tensor* residual, const at::Tensor& gain
          void* stream) {
   return issued([&] {
     return f8.norm(x.const_data_ptr(), residual ? residual->const_data_ptr() : nullptr, gain.const_data_ptr(), t ? at_(*t) : nullptr, at_(rstd),
-                   at_(h.values), h.values.stride(0), at_(h.scales), h.scales.stride(0), int(x.size(0)), int(x.size(1)), float(eps), stream);
+                   at_(h.values), h.values.stride(0), at_(h.scales), h.scales.stride(0), int(x.size(0)), int(x.size(1)), eps, stream);
   });
 }
 

@@ -98,7 +98,7 @@ def _declare(L: ctypes.CDLL) -> None:
         "kf_gemm_fp8_swiglu": [vp, vp, vp, vp, i, i, i, ll, ll, i, i, vp, vp, vp, vp, i, vp],
         "kf_gemm_fp8_swiglu_bwd": [vp, vp, vp, vp, i, i, i, ll, ll, i, vp, vp, vp, vp, i, vp],
         "kf_fp8_blocks_cast_bf16": [vp, i, i, ll, vp, vp, i, i, vp, ll, vp, ll, vp, ll, vp, ll, vp],
-        "kf_add_rmsnorm_fp8_blocks": [vp, vp, vp, vp, vp, vp, ll, vp, ll, i, i, f, vp],
+        "kf_add_rmsnorm_fp8_blocks": [vp, vp, vp, vp, vp, vp, ll, vp, ll, i, i, ctypes.c_double, vp],
         "kf_fp8_blocks_values_bf16": [vp, ll, vp, ll, i, i, i, vp, vp],
         "kf_norm_grads_blocks": [i, i, i],
         "kf_norm_grads_f32": [vp, vp, vp, vp, vp, vp, vp, vp, i, i, i, vp],

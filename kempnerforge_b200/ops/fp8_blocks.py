@@ -35,6 +35,7 @@ from torch.autograd.function import once_differentiable
 from kempnerforge_b200.ops import fp8
 
 BLOCK = 128
+_LARGEST = 2**31 - 2**16  # rows or columns: indices of kernels have 32 bits, and a few blocks are added to them
 _BF16 = torch.bfloat16
 _NOTHING = contextlib.nullcontext()
 
@@ -91,6 +92,8 @@ def _check_operand(a: BlockScaled, name: str) -> None:
     if q.dtype != torch.uint8 or s.dtype != torch.uint8 or q.dim() != 2 or s.dim() != 2 or q.device != s.device:
         raise ValueError(f"{name}: values and scales are uint8 matrices on one device")
     rows, k = q.shape
+    if max(rows, k) > _LARGEST:
+        raise ValueError(f"{name}: {rows} rows of {k} values, at most {_LARGEST} of either are covered")
     if s.shape != (-(-k // BLOCK), rows):
         raise ValueError(f"{name}: {rows} rows of {k} values have scales of shape {(-(-k // BLOCK), rows)}, got {tuple(s.shape)}")
     if q.numel() and ((k > 1 and q.stride(1) != 1) or (rows > 1 and s.stride(1) != 1)):
@@ -100,6 +103,8 @@ def _check_operand(a: BlockScaled, name: str) -> None:
 def _check_matrix(x2: torch.Tensor, name: str = "x") -> None:
     if x2.dim() != 2 or x2.dtype != _BF16:
         raise ValueError(f"{name}: a bf16 matrix is wanted, got {x2.dtype} of shape {tuple(x2.shape)}")
+    if max(x2.shape) > _LARGEST:
+        raise ValueError(f"{name}: shape {tuple(x2.shape)}, at most {_LARGEST} rows or columns are covered")
 
 
 # --------------------------------------------------------------------------- plain arithmetic (CPU)

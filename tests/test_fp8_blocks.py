@@ -117,6 +117,9 @@ def _ok(k=200, rows=6):
     lambda: fb.mm(_ok(), _ok(), out=torch.empty(1, 6, dtype=torch.bfloat16).expand(6, 6)),        # rows on one another
     lambda: fb.mm(_ok(), fb.BlockScaled(*(t.to("meta") for t in _ok()[:2]))),                     # another device
     lambda: fb.BlockScaled(_ok().values, _ok().scales.int()).dequantize(),
+    lambda: fb.BlockScaled(*(torch.empty(s, device="meta", dtype=torch.uint8) for s in ((2**31, 1), (1, 2**31)))).dequantize(),   # too many rows
+    lambda: fb.quantize(torch.empty(1, 2**32 + 1, device="meta", dtype=torch.bfloat16)),
+    lambda: fb.add_rmsnorm(torch.empty(2**32 + 1, 8, device="meta", dtype=torch.bfloat16), None, torch.empty(8, device="meta", dtype=torch.bfloat16)),
     lambda: fb.add_rmsnorm(torch.randn(4, 12).bfloat16(), None, torch.ones(12).bfloat16()),       # rows of 12
     lambda: fb.add_rmsnorm(torch.randn(4, 32776).bfloat16(), None, torch.ones(32776).bfloat16()),
     lambda: fb.add_rmsnorm(torch.randn(2, 4, 16).bfloat16(), None, torch.ones(16).bfloat16()),

@@ -211,7 +211,7 @@ def test_norm(native_lib, rows, d, with_residual):
     want = (t.double().square().mean(1) + 1e-5).rsqrt()
     # a sum of d squares (2^-24 each, at most d of them one after another) under a square root, and an approximate one (2^-22)
     assert bool(((rstd.double() - want).abs() <= want * (d * 2.0**-25 + 2.0**-21)).all())
-    q, scales = _cast64(t.double() * gain.double() / (t.double().square().mean(1) + torch.tensor(1e-5).double()).sqrt()[:, None])
+    q, scales = _cast64(t.double() * gain.double() / (t.double().square().mean(1) + 1e-5).sqrt()[:, None])
     assert torch.equal(h.scales, scales) and torch.equal(h.values, q)
     normed = fb._normed_t(t, rstd, gain)
     assert _same(normed, fb._cast_rows((t.float() * gain.float() * rstd[:, None]).t().contiguous(), False))
@@ -571,3 +571,40 @@ def test_operands_in_odd_places_of_memory(native_lib):
     a, b = fb.quantize(x)[0], fb.quantize(ws[0])[0]
     odd = lambda q: fb.BlockScaled(torch.nn.functional.pad(q.values, (3, 2), value=0x7F)[:, 3:267], torch.nn.functional.pad(q.scales, (1, 1), value=255)[:, 1:-1])   # noqa: E731
     assert torch.equal(fb.mm(odd(a), odd(b)), fb.mm(a, b)) and torch.equal(odd(a).dequantize(), a.dequantize())
+
+
+def test_offsets_past_32_bits(native_lib):
+    rows, d = (1 << 20) + 1030, 4096                              # 4.3 G values: matrices of 2, 1 and 4 bytes a value all end behind 2^32 bytes
+    tail, last = slice(rows - 300, rows), 300
+    x = torch.zeros(rows, d, device=DEV, dtype=torch.bfloat16)
+    x[tail], x[:300] = _spread(last, d, 1), _spread(last, d, 2)
+    gain = (1 + 0.2 * torch.randn(d, device=DEV, generator=_gen(1))).bfloat16()
+    q, qt = fb.quantize(x, want_t=True)
+    assert _same(fb.BlockScaled(q.values[tail], q.scales[:, tail]), fb.quantize(x[tail])[0])
+    first = (rows - 300) // 128 * 128                             # transposed blocks of whole 128 rows start there
+    part = fb.quantize(x[first:], want_row=False, want_t=True)[1]
+    assert torch.equal(qt.values[:, first:], part.values) and torch.equal(qt.scales[first // 128 :], part.scales)
+    assert torch.equal(q.dequantize()[tail], fb.BlockScaled(q.values[tail], q.scales[:, tail]).dequantize())
+    del qt, part
+    t, rstd, h = fb.add_rmsnorm(x, x, gain)
+    want = fb.add_rmsnorm(x[tail], x[tail], gain)
+    assert torch.equal(t[tail], want[0]) and torch.equal(rstd[tail], want[1]) and _same(fb.BlockScaled(h.values[tail], h.scales[:, tail]), want[2])
+    del t, h
+    # a tall operand, in either place, and an output whose rows lie far apart
+    w, _, wv, _ = _mm_case(40, 40, d, False, False, 3)
+    qv = fb._values(fb.BlockScaled(q.values[tail], q.scales[:, tail])).double()
+    exact, mag = qv @ wv.t(), qv.abs() @ wv.abs().t()
+    assert _mm_close(fb.mm(q, w)[tail], exact, mag, d) and _mm_close(fb.mm(w, q)[:, tail], exact.t(), mag.t(), d)
+    frame = torch.zeros(rows, d, device=DEV, dtype=torch.bfloat16)
+    fb.mm(q, w, out=frame[:, 8:48])
+    assert _mm_close(frame[tail, 8:48], exact, mag, d) and not frame[tail, :8].any() and not frame[tail, 48:].any()
+    del q, frame
+    dh = torch.zeros(rows, d, device=DEV)
+    dh[tail] = _spread(last, d, 4, torch.float32)
+    dx, dgain = fb._norm_grads(dh, x, gain, rstd, x)
+    small, small_gain = fb._norm_grads(dh[tail].clone(), x[tail].clone(), gain, rstd[tail].clone(), x[tail].clone())
+    assert torch.equal(dx[tail], small)
+    # sums of the same 300 terms and zeros, in another order (2^-24 a term) before the rounding
+    size = (dh[tail].double() * x[tail].double() * rstd[tail].double()[:, None]).abs().sum(0)
+    assert bool(((dgain.double() - small_gain.double()).abs() <= 2 * HALF_BF16 * dgain.double().abs() + 600 * 2.0**-24 * size).all())
+    assert native_lib.read_status() == 0
