@@ -6,10 +6,13 @@
 // tensor memory, no copies through shared memory): a warp reads rows of W in 16-byte pieces straight into fragments, multiplies a block's
 // sum by its two factors and adds that up in 32 bits.  The warps of a block divide K and add up in a fixed order.
 //
-// The products are those of 16-bit halves (mma.sync.m16n8k16): an e4m3 byte moved to the exponent and fraction bits of a half is its value
-// times 2^-8, an e5m2 byte is the upper byte of one, and four bytes become two pairs with seven shifts and masks.  NaN has no place in that
-// move, so e4m3 operands are looked through for it.  The order of k within a fragment is free as long as both operands have the same: lane (g, t) takes bytes 16 t .. 16 t + 15 of
-// rows g and g + 8 of each 64, and of a word the bytes 0 and 2, then 1 and 3.
+// The products are those of 16-bit halves (mma.sync.m16n8k16), which have every e4m3 and e5m2 value.  The order of k within a fragment is free as
+// long as both operands have the same: lane (g, t) takes bytes 16 t .. 16 t + 15 of rows g and g + 8 of each 64, and a word's four bytes make a pair
+// of each of a fragment's two.
+//
+// One token, graph of launches on weights in turn, us (at the copy rate): 1024 x 1024 2.2 (0.2), 2048 x 2048 3.7 (0.6); the tensor-memory kernel 5.2
+// and 6.0.  Two to four blocks of K under way per warp instead of the next one change little (2048 x 2048 3.8 - 4.5, 4096 x 4096 8.1 - 9.6 for 8.2): per
+// block of 2 KB a warp has 300 instructions to issue, and that and the wait for the next take turns.
 #include "fp8_blocks.cuh"
 
 #include <type_traits>
@@ -30,11 +33,10 @@ struct Args {
   int M, N, K, f32, accumulate;
 };
 
-// v 2^(a + b - 254 + UP), NaN where a scale byte is 255: by two factors of half the exponent, since one of 2^(a - 127) could send beyond the range
-// what the other brings back.  (A sum below -252, whose factors have no normal number, leaves nothing of a block's sum of at most 2^33.)
-template <int UP>
+// v 2^(a + b - 254), NaN where a scale byte is 255: by two factors of half the exponent, since one of 2^(a - 127) could send beyond the range
+// what the other brings back.  (A sum below -252, whose factors have no normal number, leaves nothing of a block's sum of at most 2^39.)
 __device__ __forceinline__ float scaled(float v, uint32_t a, uint32_t b) {
-  const int e = int(a + b) - 254 + UP, h = e >> 1;
+  const int e = int(a + b) - 254, h = e >> 1;
   const float lo = __uint_as_float(uint32_t(max(h + 127, 0)) << 23), hi = __uint_as_float(uint32_t(max(e - h + 127, 0)) << 23);
   return a == 255 || b == 255 ? __uint_as_float(0x7fffffffu) : mul_full(mul_full(v, lo), hi);
 }
@@ -44,22 +46,13 @@ __device__ __forceinline__ void mma16(float (&d)[4], uint32_t a0, uint32_t a1, u
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// bytes 0 and 2, bytes 1 and 3 of a word as halves; e4m3 values times 2^-8, and NaN as something else: nan_in tells of it
+// bytes 0 and 1, bytes 2 and 3 of a word as halves
 template <bool E5M2>
-__device__ __forceinline__ void halves(uint32_t w, uint32_t& even, uint32_t& odd) {
-  if (E5M2) {
-    even = (w << 8) & 0xff00ff00u;
-    odd = w & 0xff00ff00u;
-  } else {
-    even = ((w << 8) & 0x80008000u) | ((w << 7) & 0x3f803f80u);
-    odd = (w & 0x80008000u) | ((w >> 1) & 0x3f803f80u);
-  }
-}
-template <bool E5M2>
-__device__ __forceinline__ uint32_t nan_in(const uint4& v) {
-  if (E5M2) return 0;  // a half has it
-  auto in = [](uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; };
-  return in(v.x) | in(v.y) | in(v.z) | in(v.w);
+__device__ __forceinline__ void halves(uint32_t w, uint32_t& low, uint32_t& high) {
+  const __half2_raw a = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w & 0xffffu), E5M2 ? __NV_E5M2 : __NV_E4M3);
+  const __half2_raw b = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w >> 16), E5M2 ? __NV_E5M2 : __NV_E4M3);
+  low = uint32_t(a.x) | uint32_t(a.y) << 16;
+  high = uint32_t(b.x) | uint32_t(b.y) << 16;
 }
 __device__ __forceinline__ uint32_t word(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
 
@@ -90,76 +83,62 @@ kf_gemm_fp8_blocks_few(const Args a) {
   let_next_in();
   const int row[2] = {min(n0 + g, a.N - 1), min(n0 + 8 + g, a.N - 1)};
   float total[TILES][4] = {};
-  uint32_t nan_w[2] = {}, nan_x[TILES] = {};
+  struct Loaded {
+    uint4 w[2][2], x[TILES][2];  // [row g or g + 8][half of the block]
+    uint32_t sw[2], sx[TILES][2];
+  };
   // all loads of a block leave before the first is used: none stands behind a test
-  auto block = [&](int kb, auto last) {
+  auto load = [&](Loaded& v, int kb, auto last) {
     constexpr bool LAST = decltype(last)::value;
     const int k = kb * BLOCK + t * 16;
-    uint4 wv[2][2], xv[TILES][2];  // [row g or g + 8][half of the block]
-    uint32_t sw[2], sx[TILES][2];
 #pragma unroll
     for (int r = 0; r < 2; ++r)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) wv[r][h] = piece<LAST>(a.w + row[r] * a.ldw, k + 64 * h, a.K);
+      for (int h = 0; h < 2; ++h) v.w[r][h] = piece<LAST>(a.w + row[r] * a.ldw, k + 64 * h, a.K);
 #pragma unroll
     for (int i = 0; i < TILES; ++i) {
       const int m = min(8 * i + g, a.M - 1), c = 8 * i + 2 * t;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) xv[i][h] = piece<LAST>(a.x + m * a.ldx, k + 64 * h, a.K);
+      for (int h = 0; h < 2; ++h) v.x[i][h] = piece<LAST>(a.x + m * a.ldx, k + 64 * h, a.K);
 #pragma unroll
-      for (int e = 0; e < 2; ++e) sx[i][e] = a.sx[kb * a.ldsx + min(c + e, a.M - 1)];
+      for (int e = 0; e < 2; ++e) v.sx[i][e] = a.sx[kb * a.ldsx + min(c + e, a.M - 1)];
     }
 #pragma unroll
-    for (int r = 0; r < 2; ++r) sw[r] = a.sw[kb * a.ldsw + row[r]];
+    for (int r = 0; r < 2; ++r) v.sw[r] = a.sw[kb * a.ldsw + row[r]];
+  };
+  auto add = [&](const Loaded& v) {
     float d[TILES][4] = {};
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-#pragma unroll
-      for (int i = 0; i < TILES; ++i) nan_x[i] |= nan_in<X5>(xv[i][h]);
-#pragma unroll
-      for (int r = 0; r < 2; ++r) nan_w[r] |= nan_in<W5>(wv[r][h]);
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         uint32_t a0, a1, a2, a3;
-        halves<W5>(word(wv[0][h], q), a0, a2);
-        halves<W5>(word(wv[1][h], q), a1, a3);
+        halves<W5>(word(v.w[0][h], q), a0, a2);
+        halves<W5>(word(v.w[1][h], q), a1, a3);
 #pragma unroll
         for (int i = 0; i < TILES; ++i) {
           uint32_t b0, b1;
-          halves<X5>(word(xv[i][h], q), b0, b1);
+          halves<X5>(word(v.x[i][h], q), b0, b1);
           mma16(d[i], a0, a1, a2, a3, b0, b1);
         }
       }
-    }
-    constexpr int UP = (W5 ? 0 : 8) + (X5 ? 0 : 8);  // what moving the bytes took away
 #pragma unroll
     for (int i = 0; i < TILES; ++i)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) total[i][e] = add_full(total[i][e], scaled<UP>(d[i][e], sw[e >> 1], sx[i][e & 1]));
+      for (int e = 0; e < 4; ++e) total[i][e] = add_full(total[i][e], scaled(d[i][e], v.sw[e >> 1], v.sx[i][e & 1]));
   };
   const int whole = a.K / BLOCK;
   int kb = warp;
-#pragma unroll 2
-  for (; kb < whole; kb += warps) block(kb, std::false_type{});
-  if (kb < k_blocks) block(kb, std::true_type{});
-  // a NaN among a row's or a token's values: in all that they take part in
-  uint32_t any = nan_w[0] | nan_w[1];
-#pragma unroll
-  for (int i = 0; i < TILES; ++i) any |= nan_x[i];
-  if (__any_sync(0xffffffffu, any != 0)) {
-    const float nan = __uint_as_float(0x7fffffffu);
-    auto over_t = [](uint32_t v) {
-      v |= __shfl_xor_sync(0xffffffffu, v, 1);
-      return v | __shfl_xor_sync(0xffffffffu, v, 2);
-    };
-#pragma unroll
-    for (int i = 0; i < TILES; ++i) {
-      const uint32_t token = over_t(nan_x[i]);  // of token g, in its four lanes
-      const uint32_t tok[2] = {__shfl_sync(0xffffffffu, token, 8 * t), __shfl_sync(0xffffffffu, token, 8 * t + 4)};
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (over_t(nan_w[e >> 1]) | tok[e & 1]) total[i][e] = nan;
-    }
+  Loaded v;
+  if (kb < whole) load(v, kb, std::false_type{});
+  while (kb < whole) {
+    add(v);
+    kb += warps;
+    if (kb < whole) load(v, kb, std::false_type{});
+  }
+  if (kb < k_blocks) {
+    load(v, kb, std::true_type{});
+    add(v);
   }
 #pragma unroll
   for (int i = 0; i < TILES; ++i) {
@@ -195,8 +174,8 @@ static int launch(const Args& a, int a_fmt, int b_fmt, int warps, cudaStream_t s
 }  // namespace few
 
 // Whether this kernel is the quicker one.  us, this / the tensor-memory kernel, graphs of launches on weights in turn: one token 256 x 256 1.9 /
-// 4.0, 1024 x 1024 2.4 / 4.6, 2048 x 2048 3.9 / 6.3, 4096 x 2048 5.8 / 6.6, 4096 x 4096 9.3 / 8.5, 1024 x 14 336 14.1 / 11.1; 16 tokens 1304 x 952
-// 3.5 / 4.5, 2048 x 2048 4.5 / 6.3, 4096 x 2048 6.7 / 6.7.  In fours of eight tokens it gains little (32 x 1304 from 952 6.5 / 6.0): not built.
+// 3.1, 1024 x 1024 2.2 / 5.2, 2048 x 2048 3.7 / 6.0, 4096 x 4096 8.2 / 8.3, 6144 x 4096 12.6 / 9.0; 16 tokens 1304 x 952 3.4 / 4.6, 4096 x 2048
+// 6.3 / 6.3.  In fours of eight tokens it gains little (32 x 1304 from 952 6.5 / 6.0): not built.
 bool few_serves(int M, int N, int K) { return M <= few::MAX_TOKENS && (long long)N * K * ((M + 7) / 8) <= 12LL << 20; }
 
 // The call of kf_gemm_fp8_blocks that few_serves.
@@ -206,7 +185,7 @@ int gemm_blocks_few(const void* A, const void* sa, const void* B, const void* sb
                     f32, accumulate};
   if (((reinterpret_cast<uintptr_t>(A) | reinterpret_cast<uintptr_t>(B)) & 15) != 0) return 5;
   const int k_blocks = (K + BLOCK - 1) / BLOCK;
-  int warps = (N + few::ROWS - 1) / few::ROWS <= num_sms ? 16 : 8;  // 2048 x 2048, 8 tokens 4.4 / 4.9 us with 16 / 8; 4096 x 4096, one token 10.6 / 9.1
+  int warps = (N + few::ROWS - 1) / few::ROWS <= num_sms ? 16 : 8;  // us with 16 / 8: 2048 x 2048, 8 tokens 3.7 / 4.3; 4096 x 2048, 16 tokens 8.2 / 6.3
   if (warps > k_blocks) warps = k_blocks;
   cudaStream_t st = (cudaStream_t)stream;
   return M <= 8 ? few::launch<1>(a, a_fmt, b_fmt, warps, st) : few::launch<2>(a, a_fmt, b_fmt, warps, st);
