@@ -3,7 +3,7 @@
 // products of few tokens take on the GPU: 19 us with the output's memory, and 6 so; a norm 21 and 9, a cast 15 and 7.  What is not plainly
 // covered (another device than the current one, pitches that need a copy, sizes of zero, arguments that are wrong) is answered with None and
 // left to the Python path (ops/fp8_blocks.py), which holds the rules; nothing is remembered between calls.  A layer's forward pass and its
-// gradients are one call each: 999 tokens of 768 columns to 2304 with all gradients took 240 us call by call, and 215 so (84 of them are those of
+// gradients are one call each: 999 tokens of 768 columns to 2304 with all gradients took 240 us call by call, and 205 so (84 of them are those of
 // a node that does nothing, between autograd's threads).
 //
 // Included by steps.cpp, whose `tensor` tells plain tensors from wrappers.
