@@ -303,10 +303,14 @@ __device__ __forceinline__ float times_odd(float p, float hi, float lo, uint32_t
 // One row per block of THREADS threads, VPT vectors of eight columns per thread held in registers; 16 neighbouring threads have a block
 // of 128 columns between them.  Vector c of a thread is c * THREADS + thread.
 //
-// Bound by memory: 4 bytes an element in, 3 out.  us (at the copy rate): 16 384 x 4096 74 (72), 4096 x 4096 23 (18), 777 x 5120 9.2 (4.3), one row
-// 3.2.  The sum and rstd in 64 bits and the products that keep what they cut off cost 2 to 7 % of that (73, 21.5, 8.6, 3.0 in 32 bits, where one byte in
-// two million was the neighbour of the right one).
-template <int THREADS, int VPT>
+// Bound by memory, 4 bytes an element in and 3 out, and by the instructions (82 % of the issue slots); few rows by the chain load - sum - store.
+// EARLY reads the gain with the row instead of after the sum, for 20 more registers: us, with / without, 1 x 4096 2.5 / 3.2, 777 x 5120 8.3 / 8.9,
+// 2048 x 2048 7.6 / 8.8, 4096 x 4096 22.6 / 22.9, 777 x 6144 9.3 / 9.2, 8192 x 5120 53 / 50, 16 384 x 4096 77 / 73 (at the copy rate 0.01, 4.3, 4.5, 18,
+// 5, 45, 72).  A row has as many warps as hold it: with 256 threads for 5120 columns 777 rows are 9.2, with 128 for 2048 columns 2048 rows 9.7, for
+// 2560 8192 rows 33 (29 so).  The sum and rstd in 64 bits and the products that keep what they cut off cost 2 to 7 % (16 384 x 4096 72.6, 777 x
+// 5120 8.6 in 32 bits, where one byte in two million was the neighbour of the right one).
+constexpr long long EARLY_THREADS = 1 << 18;  // rows x threads that the SMs hold at once
+template <int THREADS, int VPT, bool EARLY>
 __global__ void __launch_bounds__(THREADS)
 kf_add_rmsnorm_blocks(const __nv_bfloat16* x, const __nv_bfloat16* residual, const __nv_bfloat16* gain,
                       __nv_bfloat16* t_out, float* rstd_out, uint8_t* out, long long ld_out,
@@ -317,16 +321,19 @@ kf_add_rmsnorm_blocks(const __nv_bfloat16* x, const __nv_bfloat16* residual, con
   const __nv_bfloat16* xr = x + row * D;
   wait_for_previous();
   let_next_in();
-  uint4 v[VPT], rv[VPT];
+  uint4 v[VPT], rv[VPT], gv[VPT];
 #pragma unroll
   for (int c = 0; c < VPT; ++c) {
     const int i = threadIdx.x + c * THREADS;
-    v[c] = rv[c] = make_uint4(0, 0, 0, 0);
+    v[c] = rv[c] = gv[c] = make_uint4(0, 0, 0, 0);
     if (i < nvec) {
       v[c] = *reinterpret_cast<const uint4*>(xr + i * 8);
       if (residual) rv[c] = *reinterpret_cast<const uint4*>(residual + row * D + i * 8);
     }
   }
+#pragma unroll
+  for (int c = 0; c < VPT; ++c)
+    if (const int i = threadIdx.x + c * THREADS; EARLY && i < nvec) gv[c] = *reinterpret_cast<const uint4*>(gain + i * 8);
   double sum = 0.;
 #pragma unroll
   for (int c = 0; c < VPT; ++c) {
@@ -381,11 +388,11 @@ kf_add_rmsnorm_blocks(const __nv_bfloat16* x, const __nv_bfloat16* residual, con
 #pragma unroll
   for (int c = 0; c < VPT; ++c) {
     const int i = threadIdx.x + c * THREADS;
-    const uint4 gv = i < nvec ? *reinterpret_cast<const uint4*>(gain + i * 8) : make_uint4(0, 0, 0, 0);
+    if (!EARLY && i < nvec) gv[c] = *reinterpret_cast<const uint4*>(gain + i * 8);
     float f[8], m = 0.f;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const float2 a = pair_at(v[c], j), g = pair_at(gv, j);
+      const float2 a = pair_at(v[c], j), g = pair_at(gv[c], j);
       f[2 * j] = times_odd(mul_full(a.x, g.x), r, lo, cut);  // the first product is exact: 16 bits
       f[2 * j + 1] = times_odd(mul_full(a.y, g.y), r, lo, cut);
       m = max_abs(max_abs(m, f[2 * j]), f[2 * j + 1]);
@@ -588,11 +595,22 @@ int kf_add_rmsnorm_fp8_blocks(const void* x, const void* residual, const void* g
                                (const __nv_bfloat16*)gain, (__nv_bfloat16*)t, (float*)rstd, (uint8_t*)out, ld_out, (uint8_t*)scales, ld_scales, D, 1. / D,
                                eps);
   };
-  if (D <= 1024) return go(kf_add_rmsnorm_blocks<32, 4>, 32);
-  if (D <= 4096) return go(kf_add_rmsnorm_blocks<128, 4>, 128);
-  if (D <= 8192) return go(kf_add_rmsnorm_blocks<256, 4>, 256);
-  if (D <= 16384) return go(kf_add_rmsnorm_blocks<512, 4>, 512);
-  return go(kf_add_rmsnorm_blocks<1024, 4>, 1024);
+  // as many warps as hold a row
+  auto pick = [&](auto threads) {
+    constexpr int N = decltype(threads)::value;
+    return (long long)rows * N <= EARLY_THREADS ? go(kf_add_rmsnorm_blocks<N, 4, true>, N) : go(kf_add_rmsnorm_blocks<N, 4, false>, N);
+  };
+  const int warps = (D / 8 + 4 * 32 - 1) / (4 * 32);
+  switch (warps) {
+    case 1: return pick(std::integral_constant<int, 32>{});
+    case 2: return pick(std::integral_constant<int, 64>{});
+    case 3: return pick(std::integral_constant<int, 96>{});
+    case 4: return pick(std::integral_constant<int, 128>{});
+    case 5: return pick(std::integral_constant<int, 160>{});
+    case 6: return pick(std::integral_constant<int, 192>{});
+  }
+  return warps <= 8 ? pick(std::integral_constant<int, 256>{})
+                    : warps <= 16 ? pick(std::integral_constant<int, 512>{}) : pick(std::integral_constant<int, 1024>{});
 }
 
 // Blocks of kf_norm_grads_f32, each of which leaves D floats in `partial`: what the SMs hold, of four rows at least where that fills them.

@@ -198,7 +198,7 @@ def _cast64(v):
     return (torch.round(q / step) * step).view(rows, -1)[:, :k].float().to(torch.float8_e4m3fn).view(torch.uint8), (e + 127).t().to(torch.uint8)
 
 
-NORM = [(1, 8), (1, 4096), (3, 136), (5, 1024), (130, 1032), (64, 4104), (33, 8200), (2, 16392), (2, 32768), (1000, 776)]
+NORM = [(1, 8), (1, 4096), (3, 136), (5, 1024), (130, 1032), (64, 4104), (33, 8200), (50, 2056), (700, 2560), (700, 2056), (20, 5128), (70, 4864), (2000, 6144), (8200, 264), (2, 16392), (2, 32768), (1000, 776)]
 
 
 @pytest.mark.parametrize("with_residual", [False, True], ids=["alone", "residual"])
