@@ -604,9 +604,10 @@ struct Cut {
 };
 // The cheapest by what was measured, in ns: a block of 128 takes 0.66 (columns + 250) on a pair while all of them ask for operands (64 columns
 // 207, 128 250, 192 300, 224 313), the last tile's way out 4.5 a column, and the sum over a cluster its barriers and its copies.  Of 74 pairs
-// 33 clusters of two fit, and 15 of four; one is left free, since the last of a launch right behind another had to wait (13.3 us for 339 x 576 from
-// 8064 in 33 clusters, in 12 of four 9.9).  us, graph of launches on weights in turn, cut by columns only -> so: 200 x 4096 from 14 336 36.5 ->
-// 21.1, 64 x 4096 from 4096 12.5 -> 10.4, 1554 x 7168 from 5120 50.9 -> 45.0, 2000 x 2048 from 2048 14.9 -> 12.3, 120 x 1304 from 952 6.6 -> 6.0.
+// 33 clusters of two fit, 22 of three and 15 of four; some are left free, since the last of a launch right behind another had to wait (13.3 us for
+// 339 x 576 from 8064 in 33 clusters of two, in 12 of four 9.9; 24 of three where 22 fit take 15.0 for 9.0).  us, graph of launches on weights in
+// turn, cut by columns only -> so: 200 x 4096 from 14 336 36.5 -> 18.0, 64 x 4096 from 4096 12.5 -> 8.4, 1554 x 7168 from 5120 50.9 -> 43.2, 2000 x
+// 2048 from 2048 14.9 -> 12.3, 120 x 1304 from 952 6.6 -> 6.0; by powers of two only -> by three, too: 1 x 4096 from 14 336 16.6 -> 14.5.
 static Cut cut_of(int M, int N, int K, int num_sms) {
   const int pairs = num_sms / 2, k_blocks = (K + BK - 1) / BK;
   Cut best{0, MAX_N, 1};
@@ -616,11 +617,12 @@ static Cut cut_of(int M, int N, int K, int num_sms) {
     for (int tn = MAX_N; tn >= 32; tn -= 32) {
       if (tn - 32 >= n) continue;
       const long long tiles = (long long)m_blocks * ((n + tn - 1) / tn);
-      for (int splits = 1; splits <= 4; splits *= 2) {
-        if (splits > 1 && (tiles * splits > pairs - (splits == 2 ? 10 : 18) || k_blocks < splits)) break;
+      for (int splits = 1; splits <= 4; ++splits) {
+        const int left = splits == 2 ? 14 : splits == 3 ? 8 : 18;  // pairs that such clusters leave idle
+        if (splits > 1 && (tiles * splits > pairs - left || k_blocks < splits)) break;
         const long long rounds = splits > 1 ? 1 : (tiles + pairs - 1) / pairs;
         const float cost = float(rounds * ((k_blocks + splits - 1) / splits)) * 0.66f * float(tn + 250) + 4.5f * float(tn) +
-                           (splits == 1 ? 0.f : splits == 2 ? 600.f + 13.f * float(tn) : 1200.f + 20.f * float(tn));
+                           (splits == 1 ? 0.f : splits == 2 ? 600.f + 9.f * float(tn) : splits == 3 ? 900.f + 12.f * float(tn) : 1200.f + 16.f * float(tn));
         if (cost < best_cost) {
           best = {turned, tn, splits};
           best_cost = cost;

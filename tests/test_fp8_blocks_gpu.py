@@ -94,7 +94,8 @@ def _mm_close(got, want, mag, k):
 
 MM = [(1, 1, 1), (1, 4096, 512), (2, 24, 136), (16, 128, 128), (17, 1001, 777), (64, 256, 2048), (100, 136, 40), (128, 224, 640),
       (129, 225, 129), (200, 512, 1536), (256, 448, 256), (257, 300, 1000), (333, 1001, 777), (513, 96, 384), (700, 1792, 520),
-      (300, 200, 4096), (260, 1000, 8200), (2001, 72, 2048), (72, 2001, 2048), (1300, 1304, 900), (5000, 40, 1000), (3000, 2999, 136)]
+      (300, 200, 4096), (260, 1000, 8200), (2001, 72, 2048), (72, 2001, 2048), (1300, 1304, 900), (5000, 40, 1000), (3000, 2999, 136),
+      (5, 4096, 4097), (619, 1080, 5316), (200, 4096, 14300), (1300, 190, 6000)]
 
 
 @pytest.mark.parametrize("ea, eb", [(False, False), (True, False), (False, True), (True, True)], ids=["e4m3", "e5m2xe4m3", "e4m3xe5m2", "e5m2"])
