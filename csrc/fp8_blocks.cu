@@ -557,9 +557,9 @@ kf_blocks_values(const uint8_t* q, long long ld, const uint8_t* scales, long lon
 
 extern "C" {
 
-// Casts bf16 x[rows][cols] (pitch ldx elements), or x * rstd[row] * gain[column] where rstd is given (the transposed copy in e4m3 only).  out / scales: row-major copy (pitch
-// ld_out) and its (ceil(cols / 128), rows) scale bytes (pitch ld_scales); out_t / scales_t: the transposed one, (cols, rows) and
-// (ceil(rows / 128), cols); either may be null.  square: blocks of 128 x 128.
+// Casts bf16 x[rows][cols] (pitch ldx elements), or x * rstd[row] * gain[column] where rstd is given (the transposed copy in e4m3 only).  out /
+// scales: row-major copy (pitch ld_out) and its (ceil(cols / 128), rows) scale bytes (pitch ld_scales); out_t / scales_t: the transposed one, (cols,
+// rows) and (ceil(rows / 128), cols); either may be null.  square: blocks of 128 x 128.
 int kf_fp8_blocks_cast_bf16(const void* x, int rows, int cols, long long ldx, const void* rstd, const void* gain, int e5m2, int square,
                             void* out, long long ld_out, void* scales, long long ld_scales, void* out_t, long long ld_t, void* scales_t,
                             long long ld_scales_t, void* stream) {
@@ -574,7 +574,8 @@ int kf_fp8_blocks_cast_bf16(const void* x, int rows, int cols, long long ldx, co
   };
   auto copies = [&](auto e5, auto sq) {
     constexpr bool E = decltype(e5)::value, S = decltype(sq)::value;
-    return !out_t ? go(kf_cast_blocks<E, PLAIN, S, true, false>) : !out ? go(kf_cast_blocks<E, PLAIN, S, false, true>) : go(kf_cast_blocks<E, PLAIN, S, true, true>);
+    if (!out_t) return go(kf_cast_blocks<E, PLAIN, S, true, false>);
+    return out ? go(kf_cast_blocks<E, PLAIN, S, true, true>) : go(kf_cast_blocks<E, PLAIN, S, false, true>);
   };
   if (rstd) return go(kf_cast_blocks<false, NORMED, false, false, true>);
   if (square) return e5m2 ? copies(std::true_type{}, std::true_type{}) : copies(std::false_type{}, std::true_type{});
