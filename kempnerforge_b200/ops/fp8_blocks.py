@@ -170,6 +170,8 @@ def mm(a: BlockScaled, b: BlockScaled, out: torch.Tensor | None = None, accumula
     with ``accumulate`` added to ``out`` before the rounding."""
     if dtype is None:
         dtype = _BF16 if out is None else out.dtype
+    if dtype is not _BF16 and dtype is not torch.float32:   # first: the native call knows these two only
+        raise ValueError(f"products are bf16 or fp32, got {dtype}")
     if a.values.is_cuda and (y := _cuda().fp8_blocks_mm(a, b, out, accumulate, dtype is torch.float32)) is not None:
         return y
     _check_operand(a, "a")
@@ -180,8 +182,6 @@ def mm(a: BlockScaled, b: BlockScaled, out: torch.Tensor | None = None, accumula
     dev = a.values.device
     if b.values.device != dev:
         raise ValueError(f"operands on {dev} and {b.values.device}")
-    if dtype not in (_BF16, torch.float32):
-        raise ValueError(f"products are bf16 or fp32, got {dtype}")
     if out is None:
         out, accumulate = torch.empty((m, n), dtype=dtype, device=dev), False
     elif out.shape != (m, n) or out.dtype != dtype or out.device != dev or (n > 1 and out.stride(1) != 1) or (m > 1 and out.stride(0) < n):

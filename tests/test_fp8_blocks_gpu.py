@@ -609,3 +609,15 @@ def test_offsets_past_32_bits(native_lib):
     size = (dh[tail].double() * x[tail].double() * rstd[tail].double()[:, None]).abs().sum(0)
     assert bool(((dgain.double() - small_gain.double()).abs() <= 2 * HALF_BF16 * dgain.double().abs() + 600 * 2.0**-24 * size).all())
     assert native_lib.read_status() == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float64, torch.int32])
+def test_products_of_other_types_are_refused(native_lib, dtype):
+    q = fb.quantize(torch.randn(6, 200, device=DEV).bfloat16())[0]
+    for out in (None, torch.full((6, 6), 7.0, dtype=torch.bfloat16, device=DEV), torch.full((6, 6), 7.0, device=DEV)):
+        with pytest.raises(ValueError):
+            fb.mm(q, q, out=out, dtype=dtype)
+        assert out is None or bool((out == 7).all())
+    for out, other in ((torch.bfloat16, torch.float32), (torch.float32, torch.bfloat16)):
+        with pytest.raises(ValueError):
+            fb.mm(q, q, out=torch.empty(6, 6, dtype=out, device=DEV), dtype=other)
