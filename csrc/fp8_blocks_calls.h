@@ -154,7 +154,11 @@ PyObject* fp8_mm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
   at::Tensor out = to ? *to : at::empty({qa->size(0), qb->size(0)}, qa->options().dtype(type));
   const int rc = product(*qa, *sa, ea, *qb, *sb, eb, out, accumulate, sms, stream);
-  return rc ? PyLong_FromLong(rc) : to ? Py_NewRef(args[6]) : THPVariable_Wrap(std::move(out));
+  if (rc) return PyLong_FromLong(rc);
+  if (!to) return THPVariable_Wrap(std::move(out));
+  // what is kept by a tensor's version (saved for a gradient, 8-bit copies of a weight) learns of the write
+  if (!to->is_inference()) to->unsafeGetTensorImpl()->bump_version();
+  return Py_NewRef(args[6]);
   END_HANDLE_TH_ERRORS
 }
 

@@ -167,7 +167,7 @@ def quantize(x2: torch.Tensor, e5m2: bool = False, square: bool = False, want_ro
 
 def mm(a: BlockScaled, b: BlockScaled, out: torch.Tensor | None = None, accumulate: bool = False, dtype: torch.dtype | None = None) -> torch.Tensor:
     """(M, N) = a (M, K) @ b (N, K)ᵀ, accumulated in fp32 and rounded once to ``dtype``: that of ``out``, else bf16 unless fp32 is asked for;
-    with ``accumulate`` added to ``out`` before the rounding."""
+    with ``accumulate`` added to ``out`` before the rounding.  A write of ``out`` moves its version, as a tensor operation's does."""
     if dtype is None:
         dtype = _BF16 if out is None else out.dtype
     if dtype is not _BF16 and dtype is not torch.float32:   # first: the native call knows these two only
@@ -192,8 +192,9 @@ def mm(a: BlockScaled, b: BlockScaled, out: torch.Tensor | None = None, accumula
         y = _values(a) @ _values(b).t()
         return out.copy_(out.float() + y if accumulate else y)
     with _on(out):
-        return _cuda().gemm_fp8_blocks(_pitched(a.values), _pitched(a.scales), _pitched(b.values), _pitched(b.scales), a.e5m2, b.e5m2, out,
-                                       accumulate)
+        _cuda().gemm_fp8_blocks(_pitched(a.values), _pitched(a.scales), _pitched(b.values), _pitched(b.scales), a.e5m2, b.e5m2, out, accumulate)
+    torch.autograd.graph.increment_version(out)   # which a kernel's write does not do
+    return out
 
 
 def _pitched(t: torch.Tensor) -> torch.Tensor:

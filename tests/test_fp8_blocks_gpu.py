@@ -621,3 +621,28 @@ def test_products_of_other_types_are_refused(native_lib, dtype):
     for out, other in ((torch.bfloat16, torch.float32), (torch.float32, torch.bfloat16)):
         with pytest.raises(ValueError):
             fb.mm(q, q, out=torch.empty(6, 6, dtype=out, device=DEV), dtype=other)
+
+
+@pytest.mark.parametrize("native", [True, False], ids=["native", "python"])
+@pytest.mark.parametrize("m, n, k", [(6, 40, 200), (300, 264, 200)])
+def test_a_product_moves_the_version_of_what_it_writes(native_lib, monkeypatch, m, n, k, native):
+    if not native:
+        monkeypatch.setattr(native_lib, "_steps", False)
+    a, b = fb.quantize(_spread(m, k, 1))[0], fb.quantize(_spread(n, k, 2))[0]
+    for accumulate in (False, True):
+        out = torch.ones(m, n, device=DEV, dtype=torch.bfloat16)
+        other = torch.ones(m, n, device=DEV, dtype=torch.bfloat16, requires_grad=True)
+        y = out * other                                      # keeps `out` for its gradient
+        fb.mm(a, b, out=out, accumulate=accumulate)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.sum().backward()
+    # a weight that is written so has 8-bit copies of its new values
+    w = torch.nn.Parameter(torch.randn(m, n, device=DEV).bfloat16())
+    fb.quantized_weight([w], want_t=True)
+    with torch.no_grad():
+        fb.mm(a, b, out=w)
+    kept, fresh = fb.quantized_weight([w], want_t=True), fb.quantize(w.detach(), square=True, want_t=True)
+    assert all(_same(p, q) for p, q in zip(kept, fresh))
+    with torch.inference_mode():
+        quiet = torch.empty(m, n, device=DEV, dtype=torch.bfloat16)    # has no version
+    assert torch.equal(fb.mm(a, b, out=quiet), w)
