@@ -95,7 +95,10 @@ def scaled_mm(a8, b8, sa, sb, a_e5m2=False, b_e5m2=False, out=None, accumulate=F
     from kempnerforge_b200.ops import cuda as cu
 
     if a8.is_cuda:
-        return cu.gemm_fp8(a8, b8, sa, sb, a_e5m2, b_e5m2, out=out, accumulate=accumulate)
+        y = cu.gemm_fp8(a8, b8, sa, sb, a_e5m2, b_e5m2, out=out, accumulate=accumulate)
+        if out is not None:
+            torch.autograd.graph.increment_version(out)   # which a kernel's write does not do
+        return y
     y = (a8.float() @ b8.float().t()) / (sa * sb)
     if out is None:
         return y.to(torch.bfloat16)

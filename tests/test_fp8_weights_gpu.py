@@ -106,3 +106,16 @@ def test_a_kept_graph_still_runs_after_a_native_update(native_lib, how):
     x.grad = None
     y.sum().backward()
     assert torch.allclose(x.grad.float(), lin.weight.detach().float().sum(0).expand(64, -1), rtol=2**-7, atol=2**-5)
+
+
+def test_a_tensorwise_product_moves_the_version_of_what_it_writes(native_lib):
+    from kempnerforge_b200.ops import fp8
+
+    a, b = torch.randn(32, 64, device=DEV).bfloat16(), torch.randn(48, 64, device=DEV).bfloat16()
+    (sa, a8, _), (sb, b8, _) = fp8.quantize(a), fp8.quantize(b)
+    w = torch.nn.Parameter(torch.randn(32, 48, device=DEV).bfloat16())
+    fp8.quantized_weight([w], want_t=False)
+    with torch.no_grad():
+        fp8.scaled_mm(a8, b8, sa, sb, out=w)
+    kept, fresh = fp8.quantized_weight([w], want_t=False), fp8.quantize(w.detach())
+    assert torch.equal(kept[0], fresh[0]) and torch.equal(kept[1], fresh[1])
