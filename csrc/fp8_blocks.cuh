@@ -12,6 +12,7 @@ namespace kf {
 namespace f8b {
 
 constexpr int BLOCK = 128;
+constexpr int LARGEST = 0x7fff0000;  // rows or columns: kernels add a few blocks to an index in 32 bits
 
 // 32-bit arithmetic that keeps subnormal numbers, which the library's flags would flush
 __device__ __forceinline__ float mul_full(float a, float b) {

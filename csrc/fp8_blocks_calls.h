@@ -114,7 +114,7 @@ int gradients(const at::Tensor& dh, const at::Tensor& t, const at::Tensor& gain,
 // ------------------------------------------------------------------ checks
 // A matrix that the cast takes as it is.
 bool castable(const at::Tensor* x) {
-  return x && x->size(0) > 0 && x->size(1) > 0 && x->size(0) <= 128 * 65535 && x->size(1) <= kLargest && x->stride(1) == 1 && x->stride(0) >= x->size(1);
+  return x && x->size(0) > 0 && x->size(1) > 0 && x->size(0) <= kLargest && x->size(1) <= kLargest && x->stride(1) == 1 && x->stride(0) >= x->size(1);
 }
 // Rows that the norm's kernels take as they are, and a gain for them.
 bool rows_of(const at::Tensor* x, const at::Tensor* gain, int64_t widest) {

@@ -646,3 +646,57 @@ def test_a_product_moves_the_version_of_what_it_writes(native_lib, monkeypatch, 
     with torch.inference_mode():
         quiet = torch.empty(m, n, device=DEV, dtype=torch.bfloat16)    # has no version
     assert torch.equal(fb.mm(a, b, out=quiet), w)
+
+
+@pytest.mark.parametrize("native", [True, False], ids=["native", "python"])
+def test_more_tiles_than_one_dimension_of_a_grid_holds(native_lib, monkeypatch, native):
+    if not native:
+        monkeypatch.setattr(native_lib, "_steps", False)
+    first = 128 * 65535 + 256                                  # of the rows that are not zero: further tiles than 65 535
+    rows, last = first + 300, slice(first, first + 300)
+    x = torch.zeros(rows, 24, device=DEV, dtype=torch.bfloat16)
+    x[last] = _spread(300, 24, 1)
+    for square in (False, True):
+        q, qt = fb.quantize(x, square=square, want_t=True)
+        want, want_t = fb.quantize(x[last], square=square, want_t=True)
+        assert _same(fb.BlockScaled(q.values[last], q.scales[:, last]), want)
+        assert torch.equal(qt.values[:, last], want_t.values) and torch.equal(qt.scales[first // 128 :], want_t.scales)
+        assert not q.values[:first].any() and bool((q.scales[:, :first] == 127).all())
+        assert not qt.values[:, :first].any() and bool((qt.scales[: first // 128] == 127).all())
+        alone = fb.quantize(x, square=square, want_row=False, want_t=True)[1]
+        assert _same(alone, qt)
+        del q, qt, alone
+    # a layer's gradients cast as many rows; small whole numbers are exact in 8 bits and in sums of 32, in any order
+    g = _gen(2)
+    whole = lambda *s: torch.randint(-7, 8, s, device=DEV, generator=g).bfloat16()   # noqa: E731
+    gain, w = torch.ones(24, device=DEV, dtype=torch.bfloat16), whole(16, 24).requires_grad_()
+    dy = torch.zeros(rows, 16, device=DEV, dtype=torch.bfloat16)
+    x[last], dy[last] = whole(300, 24), whole(300, 16)
+    x.requires_grad_()
+    small = x.detach()[last].clone().requires_grad_()
+    for normed in (False, True):
+        layer = (lambda v: fb.norm_linear(v, None, gain, [w])[1]) if normed else (lambda v: fb.linear(v, [w]))   # noqa: B023
+        dx, dw = torch.autograd.grad(layer(x), (x, w), dy)
+        want, want_w = torch.autograd.grad(layer(small), (small, w), dy[last])
+        assert torch.equal(dx[last], want) and not dx[:first].any()
+        # normalised values: the same 300 terms, at most 7 * sqrt(24) each, in another order, and a rounding of both
+        off = 2 * HALF_BF16 * want_w.double().abs() + 302 * 2.0**-23 * 300 * 35 if normed else 0
+        assert bool(((dw.double() - want_w.double()).abs() <= off).all())
+        del dx, dw
+    assert native_lib.read_status() == 0
+
+
+@pytest.mark.parametrize("native", [True, False], ids=["native", "python"])
+def test_values_of_more_columns_than_one_dimension_of_a_grid_holds(native_lib, monkeypatch, native):
+    if not native:
+        monkeypatch.setattr(native_lib, "_steps", False)
+    first = 256 * 65535 + 512
+    x = torch.zeros(3, first + 300, device=DEV, dtype=torch.bfloat16)
+    x[:, first:] = _spread(3, 300, 4)
+    x[1, :300] = 1.0
+    q = fb.quantize(x)[0]
+    v = q.dequantize()
+    part = fb.BlockScaled(q.values[:, first:], q.scales[first // 128 :])
+    assert torch.equal(v[:, first:].float(), fb._values(part)) and bool((v[1, :300] == 1).all())
+    assert not v[0, :first].any() and not v[2, :first].any() and not v[1, 300:first].any()
+    assert native_lib.read_status() == 0
