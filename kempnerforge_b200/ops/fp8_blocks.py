@@ -283,9 +283,10 @@ def _rows(x: torch.Tensor) -> torch.Tensor:
 
 class _BlocksLinearFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, *weights):
-        x8, x8t = quantize(_rows(x), want_t=any(ctx.needs_input_grad[1:]))
-        w8, _ = quantized_weight(weights, want_t=ctx.needs_input_grad[0])
+    def forward(ctx, x, recording, *weights):
+        # what a backward reads is made where one is recorded: needs_input_grad tells of the leaves only
+        x8, x8t = quantize(_rows(x), want_t=recording and any(ctx.needs_input_grad[2:]))
+        w8, _ = quantized_weight(weights, want_t=recording and ctx.needs_input_grad[0])
         y = mm(x8, w8)
         # the transposed copy is all that the gradient of the weights reads of x: half of its bytes
         ctx.save_for_backward(*(x8t[:2] if x8t is not None else (None, None)), *weights)
@@ -296,7 +297,7 @@ class _BlocksLinearFn(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dy):
         q8t, s8t, *weights = ctx.saved_tensors
-        need_dx, need_dw = ctx.needs_input_grad[0], any(ctx.needs_input_grad[1:])
+        need_dx, need_dw = ctx.needs_input_grad[0], any(ctx.needs_input_grad[2:])
         dy2 = _rows(dy)
         w8t = quantized_weight(weights, want_t=True)[1] if need_dx else None
         dx = None
@@ -317,17 +318,17 @@ class _BlocksLinearFn(torch.autograd.Function):
 
         wgrads = [None] * len(weights)
         if need_dw:
-            wgrads = _others()[1]._deposit_stacked_weight_grads(weights, ctx.needs_input_grad[1:], run)
+            wgrads = _others()[1]._deposit_stacked_weight_grads(weights, ctx.needs_input_grad[2:], run)
         elif need_dx:
             run()
-        return dx.view(ctx.x_shape) if need_dx else None, *wgrads
+        return dx.view(ctx.x_shape) if need_dx else None, None, *wgrads
 
 
 def linear(x: torch.Tensor, weights) -> torch.Tensor:
     """x (..., K) bf16 against one or several (out_i, K) bf16 weights stacked along the output: y (..., sum out_i)."""
     weights = list(weights)
     _check_weights(x, weights)
-    return _BlocksLinearFn.apply(x, *weights)
+    return _BlocksLinearFn.apply(x, torch.is_grad_enabled(), *weights)
 
 
 class _NormLinearFn(torch.autograd.Function):
@@ -335,10 +336,10 @@ class _NormLinearFn(torch.autograd.Function):
     normalised activation once more, along the tokens."""
 
     @staticmethod
-    def forward(ctx, x, residual, gain, eps, *weights):
+    def forward(ctx, x, residual, gain, eps, recording, *weights):
         ctx.set_materialize_grads(False)
         x2, r2 = _rows(x), None if residual is None else _rows(residual)
-        w8, _ = quantized_weight(weights, want_t=any(ctx.needs_input_grad[:3]))
+        w8, _ = quantized_weight(weights, want_t=recording and any(ctx.needs_input_grad[:3]))
         r = _cuda()._step("fp8_norm_linear", x2, r2, gain, eps, *w8[:2], _cuda().sm_count(), launches=2) if x.is_cuda else None
         if r is not None:
             t, rstd, y = r
@@ -355,7 +356,7 @@ class _NormLinearFn(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dt, dy):
         t, rstd, gain, *weights = ctx.saved_tensors
-        need_x, need_r, need_g, _, *need_w = ctx.needs_input_grad
+        need_x, need_r, need_g, _, _, *need_w = ctx.needs_input_grad
         dx = dgain = None
         wgrads = [None] * len(weights)
         if dy is None:
@@ -386,7 +387,7 @@ class _NormLinearFn(torch.autograd.Function):
             if need_h:
                 dx = dx.view(ctx.x_shape)
                 dgain = _gain_grad(gain, dgain) if need_g else None
-        return dx if need_x else None, dx if need_r else None, dgain, None, *wgrads
+        return dx if need_x else None, dx if need_r else None, dgain, None, None, *wgrads
 
 
 def _norm_grads(dh, t, gain, rstd, dt):
@@ -454,4 +455,4 @@ def norm_linear(x: torch.Tensor, residual: torch.Tensor | None, norm_weight: tor
     weights = list(weights)
     _check_weights(x, weights)
     _check_norm(x, residual, norm_weight)
-    return _NormLinearFn.apply(x, residual, norm_weight, eps, *weights)
+    return _NormLinearFn.apply(x, residual, norm_weight, eps, torch.is_grad_enabled(), *weights)

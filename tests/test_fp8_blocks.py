@@ -143,3 +143,21 @@ def test_no_rows():
     y.float().sum().backward()
     assert y.shape == (0, 8) and w.grad.shape == (8, 16) and not w.grad.any() and not gain.grad.any()
     assert fb.mm(fb.quantize(torch.randn(3, 0).bfloat16())[0], fb.quantize(torch.randn(2, 0).bfloat16())[0]).tolist() == [[0, 0]] * 3
+
+
+def test_without_gradients_nothing_is_made_for_a_backward(monkeypatch):
+    """A transposed copy serves a gradient only: weights that want one do not bring it where none is recorded."""
+    wanted, real = [], fb.quantize
+    monkeypatch.setattr(fb, "quantize", lambda x2, *a, **kw: wanted.append(kw.get("want_t", False)) or real(x2, *a, **kw))
+    x, gain = torch.randn(4, 64).bfloat16().requires_grad_(), torch.ones(64).bfloat16().requires_grad_()
+    for quiet in (torch.no_grad, torch.inference_mode):
+        ws = [torch.randn(8, 64).bfloat16().requires_grad_() for _ in range(2)]
+        with quiet():
+            fb.linear(x, ws[:1])
+            fb.norm_linear(x, None, gain, ws[1:])
+        assert len(wanted) == 3 and not any(wanted) and all(w._kf_fp8_block_cache.transposed is None for w in ws)
+        wanted.clear()
+    y, (_, z) = fb.linear(x, ws[:1]), fb.norm_linear(x, None, gain, ws[1:])
+    assert wanted == [True, True, True]        # x, and the transposed copies of the kept weights
+    (y.float().sum() + z.float().sum()).backward()
+    assert all(p.grad is not None and bool(p.grad.any()) for p in (x, gain, *ws))
