@@ -493,6 +493,90 @@ kf_norm_grads(const float* dh, const __nv_bfloat16* t, const __nv_bfloat16* gain
   }
 }
 
+// The same of rows of more than 16 384 columns, whose data registers do not hold: the gain's sums are in shared memory, each column's with the one
+// thread that has it, and a row is read twice, the second time from L2.  us (at the copy rate): 2048 x 32 768 142 (103).  (1024 threads with the
+// data in registers serve up to 16 384 columns: 4096 x 12 288 124 (77), 4096 x 16 384 136 (103).  Rounding dh to bf16 for the two passes over such
+// values, as the layers did for more than 8192 columns, lost what cancels in the gain's gradient and took 167, 216 and 245.)
+__global__ void __launch_bounds__(1024)
+kf_norm_grads_wide(const float* dh, const __nv_bfloat16* t, const __nv_bfloat16* gain, const float* rstd, const __nv_bfloat16* dt, __nv_bfloat16* dx,
+                   float* partial, int rows, int D) {
+  extern __shared__ float4 sums[];  // [half of a vector of eight][vector]
+  __shared__ float red[2][32];
+  const int nvec = D >> 3;
+  for (int i = threadIdx.x; i < nvec; i += 1024) sums[i] = sums[nvec + i] = make_float4(0.f, 0.f, 0.f, 0.f);
+  wait_for_previous();
+  let_next_in();
+  int turn = 0;
+  for (int row = blockIdx.x; row < rows; row += gridDim.x, turn ^= 1) {
+    const size_t at = size_t(row) * D;
+    const float r = rstd[row];
+    float4 a[2][2];
+    uint4 tv[2], gv[2], iv[2];
+    // two vectors of this thread, dt's too where it is asked for
+    auto load = [&](int i0, const __nv_bfloat16* in) {
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const int i = i0 + c * 1024;
+        a[c][0] = a[c][1] = make_float4(0.f, 0.f, 0.f, 0.f);
+        tv[c] = gv[c] = iv[c] = make_uint4(0, 0, 0, 0);
+        if (i < nvec) {
+          a[c][0] = *reinterpret_cast<const float4*>(dh + at + i * 8);
+          a[c][1] = *reinterpret_cast<const float4*>(dh + at + i * 8 + 4);
+          tv[c] = *reinterpret_cast<const uint4*>(t + at + i * 8);
+          gv[c] = *reinterpret_cast<const uint4*>(gain + i * 8);
+          if (in) iv[c] = *reinterpret_cast<const uint4*>(in + at + i * 8);
+        }
+      }
+    };
+    float dot = 0.f;
+#pragma unroll 1
+    for (int i0 = threadIdx.x; i0 < nvec; i0 += 2048) {
+      load(i0, nullptr);
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const int i = i0 + c * 1024;
+        const float d[8] = {a[c][0].x, a[c][0].y, a[c][0].z, a[c][0].w, a[c][1].x, a[c][1].y, a[c][1].z, a[c][1].w};
+        float s[8];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float2 x = pair_at(tv[c], j), g = pair_at(gv[c], j);
+          dot += d[2 * j] * (g.x * x.x);
+          dot += d[2 * j + 1] * (g.y * x.y);
+          s[2 * j] = d[2 * j] * (x.x * r);
+          s[2 * j + 1] = d[2 * j + 1] * (x.y * r);
+        }
+        if (i < nvec) {
+          const float4 lo = sums[i], hi = sums[nvec + i];
+          sums[i] = make_float4(lo.x + s[0], lo.y + s[1], lo.z + s[2], lo.w + s[3]);
+          sums[nvec + i] = make_float4(hi.x + s[4], hi.y + s[5], hi.z + s[6], hi.w + s[7]);
+        }
+      }
+    }
+    const float coef = block_sum<1024>(dot, red[turn]) / float(D) * r * r * r;
+#pragma unroll 1
+    for (int i0 = threadIdx.x; i0 < nvec; i0 += 2048) {
+      load(i0, dt);
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const int i = i0 + c * 1024;
+        const float d[8] = {a[c][0].x, a[c][0].y, a[c][0].z, a[c][0].w, a[c][1].x, a[c][1].y, a[c][1].z, a[c][1].w};
+        uint32_t w[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float2 x = pair_at(tv[c], j), g = pair_at(gv[c], j), in = pair_at(iv[c], j);
+          w[j] = pack_bf16(in.x + (r * (d[2 * j] * g.x) - x.x * coef), in.y + (r * (d[2 * j + 1] * g.y) - x.y * coef));
+        }
+        if (i < nvec) *reinterpret_cast<uint4*>(dx + at + i * 8) = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+    }
+  }
+  for (int i = threadIdx.x; i < nvec; i += 1024) {
+    float* p = partial + size_t(blockIdx.x) * D + i * 8;
+    *reinterpret_cast<float4*>(p) = sums[i];
+    *reinterpret_cast<float4*>(p + 4) = sums[nvec + i];
+  }
+}
+
 // out[column] = sum over parts of partial[part][column], 32 columns per block and every 32nd part per warp, in a fixed order
 __global__ void __launch_bounds__(1024) kf_column_sums(const float* partial, int parts, int D, __nv_bfloat16* out) {
   __shared__ float red[32][33];
@@ -626,27 +710,42 @@ int kf_add_rmsnorm_fp8_blocks(const void* x, const void* residual, const void* g
 
 // Blocks of kf_norm_grads_f32, each of which leaves D floats in `partial`: what the SMs hold, of four rows at least where that fills them.
 int kf_norm_grads_blocks(int rows, int D, int num_sms) {
-  int blocks = num_sms * (D <= 1024 ? 8 : D <= 4096 ? 3 : 2);
+  int blocks = num_sms * (D <= 1024 ? 8 : D <= 4096 ? 3 : D <= 8192 ? 2 : 1);
   if (blocks > rows / 4) blocks = rows / 4 > num_sms ? rows / 4 : num_sms;
   return rows < 1 ? 1 : rows < blocks ? rows : blocks;
 }
 
 // dx (bf16) = dt (or 0 where null) + the gradient of RMSNorm at t for dh (fp32); dgain (bf16) of its gain.  Contiguous rows on 16 bytes, D a
-// multiple of 8, at most 8192.
+// multiple of 8, at most 32 768.
 int kf_norm_grads_f32(const void* dh, const void* t, const void* gain, const void* rstd, const void* dt, void* dx, void* partial, void* dgain, int rows,
                       int D, int num_sms, void* stream) {
   using namespace kf::f8b;
-  if (rows <= 0 || D <= 0 || (D & 7) || D > 8192 ||
+  if (rows <= 0 || D <= 0 || (D & 7) || D > 32768 ||
       ((reinterpret_cast<uintptr_t>(dh) | reinterpret_cast<uintptr_t>(t) | reinterpret_cast<uintptr_t>(gain) | reinterpret_cast<uintptr_t>(dt) |
         reinterpret_cast<uintptr_t>(dx) | reinterpret_cast<uintptr_t>(partial)) & 15))
     return 5;
   const int blocks = kf_norm_grads_blocks(rows, D, num_sms);
   cudaStream_t st = (cudaStream_t)stream;
+  const size_t wide = D > 16384 ? size_t(D) * 4 : 0;  // bytes of shared memory
+  if (wide) {
+    static bool attr_set[64] = {};
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev >= 64 || !attr_set[dev]) {
+      const cudaError_t e = cudaFuncSetAttribute(kf_norm_grads_wide, cudaFuncAttributeMaxDynamicSharedMemorySize, 32768 * 4);
+      if (e != cudaSuccess) return 300 + (int)e;
+      if (dev < 64) attr_set[dev] = true;
+    }
+  }
   auto go = [&](auto kern, int threads) {
-    return launch_programmatic(kern, dim3(unsigned(blocks)), threads, 0, 1, st, (const float*)dh, (const __nv_bfloat16*)t, (const __nv_bfloat16*)gain,
+    return launch_programmatic(kern, dim3(unsigned(blocks)), threads, wide, 1, st, (const float*)dh, (const __nv_bfloat16*)t, (const __nv_bfloat16*)gain,
                                (const float*)rstd, (const __nv_bfloat16*)dt, (__nv_bfloat16*)dx, (float*)partial, rows, D);
   };
-  const int rc = D <= 1024 ? go(kf_norm_grads<128, 1, 8>, 128) : D <= 4096 ? go(kf_norm_grads<256, 2, 3>, 256) : go(kf_norm_grads<512, 2, 2>, 512);
+  const int rc = D <= 1024    ? go(kf_norm_grads<128, 1, 8>, 128)
+                 : D <= 4096  ? go(kf_norm_grads<256, 2, 3>, 256)
+                 : D <= 8192  ? go(kf_norm_grads<512, 2, 2>, 512)
+                 : D <= 16384 ? go(kf_norm_grads<1024, 2, 1>, 1024)
+                              : go(kf_norm_grads_wide, 1024);
   if (rc) return rc;
   return launch_programmatic(kf_column_sums, dim3((D + 31) / 32), 1024, 0, 1, st, (const float*)partial, blocks, D, (__nv_bfloat16*)dgain);
 }

@@ -117,10 +117,10 @@ bool castable(const at::Tensor* x) {
   return x && x->size(0) > 0 && x->size(1) > 0 && x->size(0) <= kLargest && x->size(1) <= kLargest && x->stride(1) == 1 && x->stride(0) >= x->size(1);
 }
 // Rows that the norm's kernels take as they are, and a gain for them.
-bool rows_of(const at::Tensor* x, const at::Tensor* gain, int64_t widest) {
+bool rows_of(const at::Tensor* x, const at::Tensor* gain) {
   if (!x || !gain) return false;
   const int64_t rows = x->size(0), d = x->size(1);
-  return rows > 0 && rows <= kLargest && d > 0 && d % 8 == 0 && d <= widest && gain->size(0) == d && x->is_contiguous() && gain->is_contiguous() &&
+  return rows > 0 && rows <= kLargest && d > 0 && d % 8 == 0 && d <= 32768 && gain->size(0) == d && x->is_contiguous() && gain->is_contiguous() &&
          address(*x) && address(*gain);
 }
 bool like(const at::Tensor* a, const at::Tensor& x) { return a && a->sizes() == x.sizes() && a->is_contiguous() && address(*a); }
@@ -172,7 +172,7 @@ PyObject* fp8_add_rmsnorm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   const bool add = args[1] != Py_None;
   const at::Tensor *x = dense(args[0], at::kBFloat16, 2, device), *r = add ? dense(args[1], at::kBFloat16, 2, device) : nullptr;
   const at::Tensor* gain = dense(args[2], at::kBFloat16, 1, device);
-  if (!rows_of(x, gain, 32768) || (add && !like(r, *x))) return none();
+  if (!rows_of(x, gain) || (add && !like(r, *x))) return none();
   HANDLE_TH_ERRORS
   at::Tensor t, rstd = at::empty({x->size(0)}, x->options().dtype(at::kFloat));
   if (add) t = at::empty(x->sizes(), x->options());
@@ -239,7 +239,7 @@ PyObject* norm_grads(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   const at::Tensor *dh = dense(args[0], at::kFloat, 2, device), *t = dense(args[1], at::kBFloat16, 2, device);
   const at::Tensor *gain = dense(args[2], at::kBFloat16, 1, device), *rstd = dense(args[3], at::kFloat, 1, device);
   const at::Tensor* dt = add ? dense(args[4], at::kBFloat16, 2, device) : nullptr;
-  if (!rows_of(t, gain, 8192) || !like(dh, *t) || !rstd || rstd->size(0) != t->size(0) || !rstd->is_contiguous() || (add && !like(dt, *t))) return none();
+  if (!rows_of(t, gain) || !like(dh, *t) || !rstd || rstd->size(0) != t->size(0) || !rstd->is_contiguous() || (add && !like(dt, *t))) return none();
   HANDLE_TH_ERRORS
   at::Tensor dx = at::empty(t->sizes(), t->options()), dgain = at::empty({t->size(1)}, t->options());
   const int rc = gradients(*dh, *t, *gain, *rstd, dt, dx, dgain, sms, stream);
@@ -259,7 +259,7 @@ PyObject* fp8_norm_linear(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   const bool add = args[1] != Py_None;
   const at::Tensor *x = dense(args[0], at::kBFloat16, 2, device), *r = add ? dense(args[1], at::kBFloat16, 2, device) : nullptr;
   const at::Tensor *gain = dense(args[2], at::kBFloat16, 1, device), *qw, *sw;
-  if (!rows_of(x, gain, 32768) || (add && !like(r, *x)) || !operand(args[4], args[5], device, qw, sw) || qw->size(1) != x->size(1)) return none();
+  if (!rows_of(x, gain) || (add && !like(r, *x)) || !operand(args[4], args[5], device, qw, sw) || qw->size(1) != x->size(1)) return none();
   HANDLE_TH_ERRORS
   at::Tensor t, rstd = at::empty({x->size(0)}, x->options().dtype(at::kFloat)), y = at::empty({x->size(0), qw->size(0)}, x->options());
   if (add) t = at::empty(x->sizes(), x->options());
@@ -283,7 +283,7 @@ PyObject* fp8_norm_linear_grads(PyObject*, PyObject* const* args, Py_ssize_t nar
   const at::Tensor *t = dense(args[2], at::kBFloat16, 2, device), *gain = dense(args[3], at::kBFloat16, 1, device);
   const at::Tensor *rstd = dense(args[4], at::kFloat, 1, device), *qw = nullptr, *sw = nullptr, *dw = nullptr;
   int accumulate = 0;
-  if (!castable(dy) || !rows_of(t, gain, 8192) || !castable(t) || t->size(0) != dy->size(0) || !rstd || rstd->size(0) != t->size(0) ||
+  if (!castable(dy) || !rows_of(t, gain) || !castable(t) || t->size(0) != dy->size(0) || !rstd || rstd->size(0) != t->size(0) ||
       !rstd->is_contiguous() || (add && !like(dt, *t)) || !(need_h || need_w) || !flag(args[8], &accumulate) ||
       (need_h && (!operand(args[5], args[6], device, qw, sw) || qw->size(0) != t->size(1) || qw->size(1) != dy->size(1))) ||
       !output(args[7], at::kBFloat16, dy->size(1), t->size(1), device, dw))

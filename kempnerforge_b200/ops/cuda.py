@@ -908,13 +908,9 @@ def fp8_blocks_mm(a, b, out: torch.Tensor | None, accumulate: bool, f32: bool) -
     return _step("fp8_mm", *a, *b, out, accumulate, f32, sm_count())
 
 
-# Widest rows of which norm_grads keeps the gradient of the gain in registers.
-NORM_GRADS_MAX_DIM = 8192
-
-
 def norm_grads(dh: torch.Tensor, t: torch.Tensor, gain: torch.Tensor, rstd: torch.Tensor, dt: torch.Tensor | None):
-    """(dt + gradient of t, gradient of the gain), bf16, of an RMSNorm of rows of up to NORM_GRADS_MAX_DIM values; ``dh`` is fp32, and all
-    are contiguous and on 16 bytes."""
+    """(dt + gradient of t, gradient of the gain), bf16, of an RMSNorm of rows of up to 32 768 values; ``dh`` is fp32, and all are
+    contiguous and on 16 bytes."""
     r = _step("norm_grads", dh, t, gain, rstd, dt, sm_count(), launches=2)
     if r is not None:
         return r

@@ -395,12 +395,8 @@ def _norm_grads(dh, t, gain, rstd, dt):
     if t.numel() == 0:
         return torch.empty_like(t), torch.zeros_like(gain)
     if t.is_cuda:
-        cu = _cuda()
-        gain, dt = _aligned(gain), None if dt is None else _aligned(dt)
         with _on(t):
-            if t.shape[1] > cu.NORM_GRADS_MAX_DIM:
-                return cu.rmsnorm_bwd(dh.to(_BF16), t, gain, rstd, residual_grad=dt)
-            return cu.norm_grads(dh, t, gain, rstd, dt)
+            return _cuda().norm_grads(dh, t, _aligned(gain), rstd, None if dt is None else _aligned(dt))
     tf, g, r = t.float(), dh * gain.float(), rstd[:, None]
     d = r * g - tf * (r * r * r * (g * tf).mean(1, keepdim=True))
     return (d if dt is None else d + dt.float()).to(_BF16), (dh * tf * r).sum(0).to(gain.dtype)

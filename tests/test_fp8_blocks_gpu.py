@@ -700,3 +700,57 @@ def test_values_of_more_columns_than_one_dimension_of_a_grid_holds(native_lib, m
     assert torch.equal(v[:, first:].float(), fb._values(part)) and bool((v[1, :300] == 1).all())
     assert not v[0, :first].any() and not v[2, :first].any() and not v[1, 300:first].any()
     assert native_lib.read_status() == 0
+
+
+@pytest.mark.parametrize("d", [8192, 8200, 16392, 32768])
+def test_gradients_of_a_norm_keep_their_32_bits_at_any_width(native_lib, d):
+    """256 and 257 in turn, of changing sign from row to row: all sums are exact in 32 bits, and 16 bits have no 257."""
+    rows, dev = 300, dict(device=DEV)
+    r, c = torch.arange(rows, **dev)[:, None], torch.arange(d, **dev)[None]
+    dh = (256.0 + (r + c) % 2) * (1 - 2 * (r % 2))
+    one = torch.ones(rows, d, dtype=torch.bfloat16, **dev)
+    dx, dgain = fb._norm_grads(dh, one, one[0].clone(), torch.ones(rows, **dev), None)
+    assert torch.equal(dx.float(), dh - dh.mean(1, keepdim=True)) and bool((dx.float().abs() == 0.5).all())
+    assert torch.equal(dgain.float(), dh.sum(0)) and bool((dgain.float().abs() == rows / 2).all())
+
+
+@pytest.mark.parametrize("rows, d", [(1, 8200), (20, 8200), (700, 8200), (33, 12296), (150, 16392), (449, 20000), (7, 24584), (2, 32768), (320, 32768)])
+def test_gradients_of_wide_norms(native_lib, rows, d):
+    g = _gen(d)
+    r = lambda *s: torch.randn(*s, device=DEV, generator=g)   # noqa: E731
+    t, gain, dt, dh = (2 * r(rows, d)).bfloat16(), (1 + 0.2 * r(d)).bfloat16(), r(rows, d).bfloat16(), r(rows, d)
+    rstd = (t.double().square().mean(1) + 1e-5).rsqrt().float()
+    for with_dt in (dt, None):
+        dx, dgain = fb._norm_grads(dh, t, gain, rstd, with_dt)
+        want, mag, want_gain, gain_mag = _norm_grads64(dh, t, gain, dt if with_dt is not None else dt * 0, 1e-5)
+        assert bool(((dx.double() - want).abs() <= HALF_BF16 * want.abs() + d * 2.0**-22 * mag).all())
+        assert bool(((dgain.double() - want_gain).abs() <= HALF_BF16 * want_gain.abs() + (rows + 8) * 2.0**-22 * gain_mag).all())
+        again = fb._norm_grads(dh, t, gain, rstd, with_dt)
+        assert torch.equal(again[0], dx) and torch.equal(again[1], dgain)
+
+
+@pytest.mark.parametrize("d", [8200, 32768])
+def test_a_wide_layer_through_both_ways_of_checks(native_lib, monkeypatch, d):
+    x, residual, gain, ws, dt, dy = _layer((40,), d, (72,), 3)
+
+    def step():
+        t, y = fb.norm_linear(x, residual, gain, ws)
+        return torch.autograd.grad((t, y), (x, gain, ws[0]), (dt, dy))
+
+    native, before = step(), native_lib.LAUNCH_COUNT
+    step()
+    launches = native_lib.LAUNCH_COUNT - before
+    # the product before the norm's gradients is in 32 bits: all that dx and the gain's gradient are off by is its sums and one rounding
+    t, rstd, _ = fb.add_rmsnorm(x.detach(), residual.detach(), gain.detach())
+    gv, wv = fb._values(fb.quantize(dy)[0]).double(), fb._values(fb.quantize(ws[0].detach(), square=True)[0]).double()
+    dh, dh_err = gv @ wv, 74 * 2.0**-23 * (gv.abs() @ wv.abs())
+    want, mag, want_gain, gain_mag = _norm_grads64(dh, t, gain.detach(), dt, 1e-5)
+    _, err, _, gain_err = _norm_grads64(dh_err, t, gain.detach().abs(), dt * 0, 1e-5)
+    assert bool(((native[0].double() - want).abs() <= err + HALF_BF16 * (want.abs() + err) + d * 2.0**-22 * mag).all())
+    assert bool(((native[1].double() - want_gain).abs() <= gain_err + HALF_BF16 * (want_gain.abs() + gain_err) + 48 * 2.0**-21 * gain_mag).all())
+    monkeypatch.setattr(native_lib, "_steps", False)
+    before = native_lib.LAUNCH_COUNT
+    plain = step()
+    assert native_lib.LAUNCH_COUNT - before == launches > 0
+    assert all(torch.equal(a, b) for a, b in zip(native, plain))
+    assert native_lib.read_status() == 0
