@@ -92,6 +92,13 @@ class TransformerBlock(nn.Module):
 
         return fp8_blocks.norm_linear_of(self.attention_norm, x, None, [att.q_proj.weight, att.k_proj.weight, att.v_proj.weight])
 
+    def _recomputed_attn_branch(self, x, cos, sin, doc_ids, key_padding_mask):
+        """The attention branch with the norm that :meth:`_body` takes without recomputation."""
+        if (pair := self._fp8_qkv(x)) is None:
+            return self._attn_branch(x, cos, sin, None, doc_ids, key_padding_mask)
+        x, qkv = pair
+        return self.attention(x, cos, sin, doc_ids=doc_ids, key_padding_mask=key_padding_mask, qkv=qkv)
+
     def _fp8_gate_up(self, x, attn):
         """(x + attn, gate | up of its norm), likewise."""
         mlp = self.mlp
@@ -104,7 +111,7 @@ class TransformerBlock(nn.Module):
     def _body(self, x, cos, sin, kv_cache, doc_ids, key_padding_mask):
         if self.ac_mode == "selective" and self.training and torch.is_grad_enabled() and kv_cache is None:
             attn = checkpoint(
-                self._attn_branch, x, cos, sin, None, doc_ids, key_padding_mask, use_reentrant=False,
+                self._recomputed_attn_branch, x, cos, sin, doc_ids, key_padding_mask, use_reentrant=False,
                 context_fn=checkpoint_contexts,
             )
         elif (pair := self._fp8_qkv(x)) is not None:

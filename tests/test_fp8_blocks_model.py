@@ -205,3 +205,27 @@ def test_the_trainer_builds_and_steps_it(tmp_path):
     before = trainer.model.layers["0"].mlp.gate_proj.weight.detach().clone()
     trainer.train_step([{"input_ids": tok[:, :-1], "labels": tok[:, 1:]}])
     assert not torch.equal(before, trainer.model.layers["0"].mlp.gate_proj.weight)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_selective_recomputation_takes_the_same_norms(device, monkeypatch):
+    """The attention's norm writes 8 bits inside of a recomputed branch too: outputs and losses are those of the other modes."""
+    losses, grads = [], []
+    for mode in ("none", "selective", "full"):
+        model, tokens = _model(device, ac=mode)
+        calls = _count(monkeypatch)
+        loss = model.train().compute_loss(tokens[:, :-1], tokens[:, 1:])
+        assert len(calls) == 4
+        loss.backward()
+        losses.append(loss.detach())
+        grads.append({n: p.grad for n, p in model.named_parameters()})
+        logits = model(tokens)
+        with torch.no_grad():
+            assert torch.equal(logits, model.eval()(tokens))
+        monkeypatch.undo()
+    assert torch.equal(losses[0], losses[1]) and torch.equal(losses[0], losses[2])
+    # the gradient of the last block's first norm is added to the residual's in another node: what is behind it has the same bits
+    for name, g in grads[0].items():
+        assert grads[1][name].isfinite().all()
+        if name.startswith(("layers.1.mlp", "layers.1.attention.o_proj", "norm", "output_head")):
+            assert torch.equal(g, grads[1][name]) and torch.equal(g, grads[2][name]), name
