@@ -253,6 +253,12 @@ def _aligned(t: torch.Tensor) -> torch.Tensor:
 def quantized_weight(weights, want_t: bool) -> tuple[BlockScaled, BlockScaled | None]:
     """(the weights stacked along the output dimension in 8 bits, the transpose of that or None), in squares of 128 x 128.  Kept on the
     first weight and reused under the conditions of :func:`kempnerforge_b200.ops.fp8.quantized_weight`."""
+    # on the weights' device: the stream that copies belong to and whether it is captured are asked of the current one
+    with _on(weights[0]) if weights[0].is_cuda else _NOTHING:
+        return _quantized_weight(weights, want_t)
+
+
+def _quantized_weight(weights, want_t: bool) -> tuple[BlockScaled, BlockScaled | None]:
     stacked = lambda: _others()[1]._stack_weight_rows(weights).detach()  # noqa: E731
     state = fp8.weights_state(weights)
     if state is None:

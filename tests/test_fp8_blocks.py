@@ -161,3 +161,29 @@ def test_without_gradients_nothing_is_made_for_a_backward(monkeypatch):
     assert wanted == [True, True, True]        # x, and the transposed copies of the kept weights
     (y.float().sum() + z.float().sum()).backward()
     assert all(p.grad is not None and bool(p.grad.any()) for p in (x, gain, *ws))
+
+
+def test_kept_weights_of_another_device_go_by_its_stream(monkeypatch):
+    """The stream that copies belong to, and whether a graph is captured, are asked of the weights' device, not of the current one."""
+    import contextlib
+    import types
+
+    current = [0]
+
+    @contextlib.contextmanager
+    def device(d):
+        before, current[0] = current[0], d.index
+        yield
+        current[0] = before
+
+    seen = []
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: current[0], raising=False)
+    monkeypatch.setattr(torch.cuda, "device", device)
+    monkeypatch.setattr(fb.fp8, "weights_state", lambda ws: seen.append(current[0]))
+    monkeypatch.setattr(fb, "quantize", lambda *a, **kw: seen.append(current[0]) or (None, None))
+    monkeypatch.setattr(fb, "_others", lambda: (None, types.SimpleNamespace(_stack_weight_rows=lambda ws: torch.empty(1, 1))))
+    for index in (0, 1):
+        w = types.SimpleNamespace(is_cuda=True, device=torch.device("cuda", index))
+        fb.quantized_weight([w], want_t=False)
+        assert seen == [index, index] and current == [0]
+        seen.clear()
