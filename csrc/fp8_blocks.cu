@@ -3,7 +3,8 @@
 //
 //   cast    q = round8(x 2^-e), e from the largest magnitude of a block: 1 x 128 (activations, gradients) or 128 x 128 (weights, whose two
 //           copies then hold the same values).  A transposed copy of 1 x 128 blocks has blocks of 128 along the rows of x.
-//   norm    t = bf16(x + residual), rstd = 1 / sqrt(mean(t^2) + eps), h = cast(t gain rstd), rounded once
+//   norm    t = bf16(x + residual), rstd = 1 / sqrt(mean(t^2) + eps), h = cast(t gain rstd), rounded once (in the transposed copy that a
+//           backward pass makes of t and rstd twice: to 32 bits, then to 8)
 //   norm's gradients  dx = dt + rstd (dh gain - t rstd^2 mean(dh gain t)), dgain = sum over rows of dh t rstd, of dh in 32 bits
 //
 // The kernels are programmatic launches, so no pointer is promised to be the only one to its memory: a load under that promise may be moved
@@ -81,7 +82,9 @@ kf_cast_blocks(const __nv_bfloat16* x, int rows, int cols, long long ldx, const 
 #pragma unroll
     for (int e = 0; e < 8; ++e) g[e] = __bfloat162float(gain[min(c + e, cols - 1)]);
   }
-  // two neighbouring values, as the norm kernel forms them
+  // Two neighbouring values.  Of normed ones the first product is exact, the second is rounded to 32 bits and taken with the 32 bits of rstd that
+  // are kept, where the norm kernel, which has the row's sum, keeps what is cut off: next to a border of two 8-bit numbers, 17 of 25
+  // million values, the transposed copy has the neighbour of the byte that the formula and the forward pass give.
   auto value2 = [&](int i, int j) {
     float2 p = pair_at(v[i], j);
     if (SRC == NORMED) p = make_float2(mul_full(mul_full(p.x, g[2 * j]), s[i]), mul_full(mul_full(p.y, g[2 * j + 1]), s[i]));

@@ -754,3 +754,14 @@ def test_a_wide_layer_through_both_ways_of_checks(native_lib, monkeypatch, d):
     assert native_lib.LAUNCH_COUNT - before == launches > 0
     assert all(torch.equal(a, b) for a, b in zip(native, plain))
     assert native_lib.read_status() == 0
+
+
+@pytest.mark.parametrize("with_residual", [False, True], ids=["alone", "residual"])
+@pytest.mark.parametrize("rows, d", NORM)
+def test_rstd_is_the_nearest_32_bit_number(native_lib, rows, d, with_residual):
+    """The sum has 64 bits and rstd about 48 before it is rounded: half a step of 32 bits (2^-24 of the value at most) and 2^-40 for what is
+    before it, whatever the width."""
+    x, gain = _spread(rows, d, d), torch.ones(d, device=DEV, dtype=torch.bfloat16)
+    t, rstd, _ = fb.add_rmsnorm(x, _spread(rows, d, d + 1) if with_residual else None, gain, 1e-5)
+    want = (t.double().square().mean(1) + 1e-5).rsqrt()
+    assert bool(((rstd.double() - want).abs() <= want * (2.0**-24 + 2.0**-40)).all())
