@@ -38,8 +38,8 @@ __device__ __forceinline__ uint32_t max_abs2(uint32_t m, uint32_t v) {
 //
 // Bound by memory: 2 bytes in, 1 or 2 out per element, and all of them pass through registers, so what counts is how many blocks an SM
 // holds while others wait (registers: two to four) and how little is done per value: maxima of bf16 values are taken in pairs as they
-// are, and infinities have a path of their own.  16 384 x 4096, us (at the copy rate): row-major 35 (31), transposed 41 (31), both 57 (41),
-// squares both 49 (41), normed 54 (31); with 256 threads, two blocks on an SM and a look at each value for infinities 60, 68, 84, 59 and 128.
+// are, and infinities have a path of their own.  16 384 x 4096, us (at the copy rate): row-major 34 (31), transposed 40 (31), both 56 (41),
+// squares both 48 (41), normed 51 (31); with 256 threads, two blocks on an SM and a look at each value for infinities 60, 68, 84, 59 and 128.
 template <bool E5M2, int SRC, bool SQUARE, bool ROW, bool T>
 __global__ void __launch_bounds__(512, ROW && !T ? 4 : SRC == NORMED ? 2 : 3)
 kf_cast_blocks(const __nv_bfloat16* x, int rows, int cols, long long ldx, const float* rstd,

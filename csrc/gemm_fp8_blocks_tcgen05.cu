@@ -546,7 +546,7 @@ kf_gemm_fp8_blocks_2cta(const __grid_constant__ CUtensorMap map_a, const __grid_
     const bool works = warp >= 2 && warp < 10;
     const int half = warp < 6;
     const uint32_t my_box = half ? smem_base + 6 * CHUNK_BYTES + uint32_t(warp - 2) * BOX_BYTES : box;
-    static_assert(6 * CHUNK_BYTES + 4 * BOX_BYTES <= STAGES * STAGE_BYTES, "at most two chunks of three pairs, or four of one, then the boxes");
+    static_assert(6 * CHUNK_BYTES + 4 * BOX_BYTES <= STAGES * STAGE_BYTES, "at most two chunks of three pairs, three of two, or four of one, then the boxes");
     if (works) {
       int turn = 0;
 #pragma unroll 1
