@@ -1,0 +1,358 @@
+// Attention of the new tokens of many continuations over their own tokens, joined with what the prompt gave (second of two kernels).
+//
+// What a continuation has written itself is its own, so these keys are read by its group of query heads only: a stream as in the generation
+// step of single sequences.  In a beam search the cache of a continuation does not move when beams are exchanged; own_rows says in whose
+// cache each position lies.  Beams share most of their ancestors, so most of these keys come out of L2 for all beams but the first.
+//   * one cluster per (continuation, key head): the group's query heads are the 16 rows of an m16n8k16 MMA, the keys are split over the
+//     cluster's CTAs (up to 8) and over the four warps of each;
+//   * tiles of 64 keys move through a three-stage cp.async ring, 16-byte chunks XOR-swizzled, so that ldmatrix is free of bank conflicts;
+//   * the partial (max, sum, output) triples of the warps, the CTAs and the prompt's partial results are joined in a fixed order.
+// All of it up to that last step runs without the prompt's kernel, and starts on the SMs that it leaves (programmatic launch).
+#include "decode_common.cuh"
+#include "shared_prefix.cuh"
+
+namespace kf {
+namespace shared_prefix {
+
+using namespace kf::decode;
+
+constexpr int OWN_THREADS = 128;
+constexpr int OWN_TILE = 64;     // keys per ring stage, 16 per warp
+constexpr int OWN_STAGES = 3;
+constexpr int OWN_ROWS = 16;     // query heads per cluster (MMA rows)
+
+template <int HD>
+struct OwnCfg {
+  static constexpr int TILE_BYTES = OWN_TILE * HD * 2;
+  static constexpr int RING = OWN_STAGES * 2 * TILE_BYTES;
+  static constexpr int PART = 4 * OWN_ROWS * HD * 4;                 // per-warp partial outputs, alias the ring
+  static constexpr int BODY = RING > PART ? RING : PART;
+  static constexpr int MERGED = OWN_ROWS * HD * 4;                   // the CTA's merged partial
+  static constexpr int STATS = (4 + 1) * OWN_ROWS * 2 * 4;           // (max, sum) per warp and merged
+  static constexpr int SEEN = OWN_STAGES * OWN_TILE;                 // per ring row: holds a visible key
+  static constexpr size_t SMEM = size_t(BODY) + MERGED + STATS + SEEN;
+};
+
+struct Own {
+  const __nv_bfloat16 *q, *k, *v;
+  __nv_bfloat16* o;
+  const uint8_t* rows;                                       // [B][W][S] or null
+  int S, Hkv, group;
+  long long q_b, q_w, q_h, k_b, k_w, k_s, k_h, v_b, v_w, v_s, v_h;   // elements
+  long long r_b, r_w;
+  float scale_log2;
+};
+
+template <int HD>
+__global__ void __launch_bounds__(OWN_THREADS)
+kf_shared_prefix_own(const Own a, const Layout lay, const float* part_o, const float2* part_ml) {
+  using C = OwnCfg<HD>;
+  extern __shared__ __align__(128) uint8_t smem_raw[];
+  const uint32_t ring = smem_u32(smem_raw);
+  float* part = reinterpret_cast<float*>(smem_raw);
+  float* merged = reinterpret_cast<float*>(smem_raw + C::BODY);
+  float* stats = reinterpret_cast<float*>(smem_raw + C::BODY + C::MERGED);  // [5][ROWS][2]
+  uint8_t* seen = smem_raw + C::BODY + C::MERGED + C::STATS;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int splits = int(cluster_nctaid()), rank = int(cluster_ctarank());
+  const int blocks_per_kv = (a.group + OWN_ROWS - 1) / OWN_ROWS;
+  long long unit = blockIdx.x / splits;
+  const int hb = int(unit % blocks_per_kv);
+  unit /= blocks_per_kv;
+  const int hk = int(unit % a.Hkv);
+  unit /= a.Hkv;
+  const int w = int(unit % lay.W), b = int(unit / lay.W);
+  const int n_heads = min(OWN_ROWS, a.group - hb * OWN_ROWS);     // query heads of this cluster
+  const int h0 = hk * a.group + hb * OWN_ROWS;
+
+  const int n_tiles = (a.S + OWN_TILE - 1) / OWN_TILE;
+  const int t0 = int((long long)n_tiles * rank / splits), t1 = int((long long)n_tiles * (rank + 1) / splits);
+  const __nv_bfloat16* kb = a.k + b * a.k_b + hk * a.k_h;
+  const __nv_bfloat16* vb = a.v + b * a.v_b + hk * a.v_h;
+  const uint8_t* table = a.rows ? a.rows + b * a.r_b + w * a.r_w : nullptr;
+
+  constexpr int CHUNKS = HD / 8;                        // 16-byte chunks per row
+  auto issue = [&](int t) {
+    const int st = (t - t0) % OWN_STAGES;
+    const uint32_t ks = ring + uint32_t(st) * 2u * C::TILE_BYTES, vs = ks + C::TILE_BYTES;
+#pragma unroll
+    for (int i = 0; i < OWN_TILE * CHUNKS / OWN_THREADS; ++i) {
+      const int idx = threadIdx.x + i * OWN_THREADS, r = idx / CHUNKS, c = idx % CHUNKS;
+      const int pos = t * OWN_TILE + r;
+      const int slot = pos >= a.S ? lay.W : table ? int(table[pos]) : w;
+      const bool in = slot < lay.W;
+      const long long ko = in ? slot * a.k_w + pos * a.k_s + c * 8 : 0, vo = in ? slot * a.v_w + pos * a.v_s + c * 8 : 0;
+      const uint32_t dst = uint32_t(r * HD * 2 + ((c ^ (r & 7)) << 4));
+      cp_async16(ks + dst, kb + ko, in);
+      cp_async16(vs + dst, vb + vo, in);
+      if (c == 0) seen[st * OWN_TILE + r] = in;
+    }
+  };
+  for (int t = t0; t < t0 + OWN_STAGES - 1; ++t) {
+    if (t < t1) issue(t);
+    cp_commit();
+  }
+
+  // query rows as MMA A fragments (rows past the group are zero)
+  uint32_t qa[HD / 16][4];
+  {
+    const int g = lane >> 2, c = (lane & 3) * 2;
+    const __nv_bfloat16* q0 = a.q + b * a.q_b + w * a.q_w + (h0 + g) * a.q_h;
+    const __nv_bfloat16* q1 = q0 + 8 * a.q_h;
+#pragma unroll
+    for (int kk = 0; kk < HD / 16; ++kk) {
+      qa[kk][0] = g < n_heads ? *reinterpret_cast<const uint32_t*>(q0 + kk * 16 + c) : 0u;
+      qa[kk][1] = g + 8 < n_heads ? *reinterpret_cast<const uint32_t*>(q1 + kk * 16 + c) : 0u;
+      qa[kk][2] = g < n_heads ? *reinterpret_cast<const uint32_t*>(q0 + kk * 16 + 8 + c) : 0u;
+      qa[kk][3] = g + 8 < n_heads ? *reinterpret_cast<const uint32_t*>(q1 + kk * 16 + 8 + c) : 0u;
+    }
+  }
+  float o[HD / 8][4];
+#pragma unroll
+  for (int i = 0; i < HD / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+
+  for (int t = t0; t < t1; ++t) {
+    cp_wait<OWN_STAGES - 2>();
+    __syncthreads();  // tile t has landed for every thread, and the stage refilled below has been consumed
+    if (t + OWN_STAGES - 1 < t1) issue(t + OWN_STAGES - 1);
+    cp_commit();
+    if (t * OWN_TILE + warp * 16 >= a.S) continue;
+    const int st = (t - t0) % OWN_STAGES;
+    const uint32_t ks = ring + uint32_t(st) * 2u * C::TILE_BYTES, vs = ks + C::TILE_BYTES;
+    const int mi = lane >> 3, lr = lane & 7;
+    float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+    {
+      const int r = warp * 16 + lr + (mi >> 1) * 8;
+      const uint32_t row = ks + uint32_t(r * HD * 2);
+#pragma unroll
+      for (int kk = 0; kk < HD / 16; ++kk) {
+        uint32_t f[4];
+        ldsm4(row + uint32_t(((kk * 2 + (mi & 1)) ^ lr) << 4), f);
+        mma16816(s[0], qa[kk], f[0], f[1]);
+        mma16816(s[1], qa[kk], f[2], f[3]);
+      }
+    }
+    const uint8_t* sees = seen + st * OWN_TILE + warp * 16 + (lane & 3) * 2;
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[n][e] = sees[n * 8 + (e & 1)] ? s[n][e] * a.scale_log2 : -INFINITY;
+    uint32_t pa[4];
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf) {
+      float mx = fmaxf(fmaxf(s[0][2 * hf], s[0][2 * hf + 1]), fmaxf(s[1][2 * hf], s[1][2 * hf + 1]));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+      const float mn = fmaxf(m[hf], mx);
+      const float base = mn == -INFINITY ? 0.f : mn;
+      const float alpha = weight(m[hf], base);
+      m[hf] = mn;
+      float p[2][2], sum = 0.f;
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          p[n][e] = fast_exp2(s[n][2 * hf + e] - base);
+          sum += p[n][e];
+        }
+      l[hf] = l[hf] * alpha + sum;  // this thread's four keys; the quad is summed at the end
+      pa[hf] = pack_bf16(p[0][0], p[0][1]);
+      pa[2 + hf] = pack_bf16(p[1][0], p[1][1]);
+#pragma unroll
+      for (int i = 0; i < HD / 8; ++i) {
+        o[i][2 * hf] *= alpha;
+        o[i][2 * hf + 1] *= alpha;
+      }
+    }
+    {
+      const int r = warp * 16 + lr + (mi & 1) * 8;
+      const uint32_t row = vs + uint32_t(r * HD * 2);
+#pragma unroll
+      for (int d = 0; d < HD / 16; ++d) {
+        uint32_t f[4];
+        ldsm4_t(row + uint32_t(((d * 2 + (mi >> 1)) ^ lr) << 4), f);
+        mma16816(o[2 * d], pa, f[0], f[1]);
+        mma16816(o[2 * d + 1], pa, f[2], f[3]);
+      }
+    }
+  }
+  cp_wait<0>();
+  __syncthreads();  // the ring is idle: it becomes the partial buffer
+
+  // ---- the warps of this CTA
+#pragma unroll
+  for (int hf = 0; hf < 2; ++hf) {
+    l[hf] += __shfl_xor_sync(0xffffffffu, l[hf], 1);
+    l[hf] += __shfl_xor_sync(0xffffffffu, l[hf], 2);
+    const int r = (lane >> 2) + hf * 8;
+    if ((lane & 3) == 0) {
+      stats[(warp * OWN_ROWS + r) * 2] = m[hf];
+      stats[(warp * OWN_ROWS + r) * 2 + 1] = l[hf];
+    }
+    if (r < n_heads) {
+      float* dst = part + (warp * OWN_ROWS + r) * HD + (lane & 3) * 2;
+#pragma unroll
+      for (int i = 0; i < HD / 8; ++i) *reinterpret_cast<float2*>(dst + i * 8) = make_float2(o[i][2 * hf], o[i][2 * hf + 1]);
+    }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < n_heads * (HD / 4); i += OWN_THREADS) {
+    const int r = i / (HD / 4), d = (i % (HD / 4)) * 4;
+    float top = -INFINITY;
+#pragma unroll
+    for (int x = 0; x < 4; ++x) top = fmaxf(top, stats[(x * OWN_ROWS + r) * 2]);
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    float sum = 0.f;
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const float f = weight(stats[(x * OWN_ROWS + r) * 2], top);
+      const float4 v = *reinterpret_cast<const float4*>(part + (x * OWN_ROWS + r) * HD + d);
+      acc.x += f * v.x; acc.y += f * v.y; acc.z += f * v.z; acc.w += f * v.w;
+      sum += f * stats[(x * OWN_ROWS + r) * 2 + 1];
+    }
+    *reinterpret_cast<float4*>(merged + r * HD + d) = acc;
+    if (d == 0) {
+      stats[(4 * OWN_ROWS + r) * 2] = top;
+      stats[(4 * OWN_ROWS + r) * 2 + 1] = sum;
+    }
+  }
+  // ---- the prompt's partial results: which there are
+  long long before = 0, total = 0;
+  if (part_o != nullptr) {
+    before = tiles_before(lay, b);
+    total = tiles_before(lay, lay.B);
+  }
+  cluster_sync_all();
+  grid_dep_wait();
+  const int u = hk * lay.row_tiles + w / lay.wt;
+  const int nt = part_o != nullptr ? tiles_of(length(lay, b)) : 0;
+  int c0 = 0, c1 = -1;
+  if (nt > 0) {
+    const int ctas = working(lay, total);
+    c0 = cta_of(total, before + (long long)u * nt, ctas);
+    c1 = cta_of(total, before + (long long)(u + 1) * nt - 1, ctas);
+  }
+  const long long slot0 = ((long long)b * lay.per_prompt + u + c0) * TILE_ROWS + (w % lay.wt) * a.group + hb * OWN_ROWS;
+  // ---- the CTAs of the cluster and the prompt, each CTA its share of the output
+  const uint32_t merged_a = ring + C::BODY, stats_a = ring + C::BODY + C::MERGED + 4 * OWN_ROWS * 2 * 4;
+  for (int i = rank * OWN_THREADS + threadIdx.x; i < n_heads * (HD / 4); i += splits * OWN_THREADS) {
+    const int r = i / (HD / 4), d = (i % (HD / 4)) * 4;
+    const float2* ml = part_ml + slot0 + r;
+    float top = -INFINITY;
+    for (int c = 0; c < splits; ++c) top = fmaxf(top, ld_cluster_f1(mapa_shared(stats_a + r * 8, c)));
+    for (int c = 0; c <= c1 - c0; ++c) top = fmaxf(top, ld_after_wait(ml + (long long)c * TILE_ROWS).x);
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    float sum = 0.f;
+    for (int c = 0; c < splits; ++c) {
+      const float f = weight(ld_cluster_f1(mapa_shared(stats_a + r * 8, c)), top);
+      const float4 v = ld_cluster_f4(mapa_shared(merged_a + uint32_t(r * HD + d) * 4u, c));
+      acc.x += f * v.x; acc.y += f * v.y; acc.z += f * v.z; acc.w += f * v.w;
+      sum += f * ld_cluster_f1(mapa_shared(stats_a + r * 8 + 4, c));
+    }
+    for (int c = 0; c <= c1 - c0; ++c) {
+      const float2 x = ld_after_wait(ml + (long long)c * TILE_ROWS);
+      const float f = weight(x.x, top);
+      const float4 v = ld_after_wait(reinterpret_cast<const float4*>(part_o + (slot0 + r + (long long)c * TILE_ROWS) * HD + d));
+      acc.x += f * v.x; acc.y += f * v.y; acc.z += f * v.z; acc.w += f * v.w;
+      sum += f * x.y;
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;   // nothing visible: zeros
+    uint2 out;
+    out.x = pack_bf16(acc.x * inv, acc.y * inv);
+    out.y = pack_bf16(acc.z * inv, acc.w * inv);
+    *reinterpret_cast<uint2*>(a.o + (((long long)b * lay.W + w) * a.Hkv * a.group + h0 + r) * HD + d) = out;
+  }
+  cluster_sync_all();   // no CTA leaves while another reads its shared memory
+}
+
+template <int HD>
+static int launch_own(const Own& a, const Layout& l, const float* part_o, const float2* part_ml, int num_sms, cudaStream_t stream) {
+  using C = OwnCfg<HD>;
+  auto kern = kf_shared_prefix_own<HD>;
+  static bool attr_set[16] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev >= 16 || !attr_set[dev]) {
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::SMEM);
+    if (e != cudaSuccess) return 300 + (int)e;
+    if (dev < 16) attr_set[dev] = true;
+  }
+  const long long units = (long long)l.B * l.W * a.Hkv * ((a.group + OWN_ROWS - 1) / OWN_ROWS);
+  // two CTAs per SM, at least one tile per CTA
+  int splits = 1;
+  while (splits < 8 && units * splits * 2 <= 2LL * num_sms && a.S > splits * OWN_TILE) splits *= 2;
+  if (units * splits > 0x7fffffffLL) return 6;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(units * splits));
+  cfg.blockDim = dim3(OWN_THREADS);
+  cfg.dynamicSmemBytes = C::SMEM;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)splits;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = part_o != nullptr ? 2 : 1;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kern, a, l, part_o, part_ml);
+  return e == cudaSuccess ? 0 : 500 + (int)e;
+}
+
+int launch_prefix(const void* q, const void* k, const void* v, const Layout& l, int H, int Hkv, int hd, const long long* qs, const long long* ks,
+                  const long long* vs, float scale, float* part_o, float2* part_ml, int* status, cudaStream_t stream);
+
+static bool make_layout(Layout& l, const void* lens, int B, int W, int P, int group, int Hkv, int num_sms) {
+  if (group > TILE_ROWS) return false;
+  const int wt = TILE_ROWS / group < W ? TILE_ROWS / group : W;
+  const int row_tiles = (W + wt - 1) / wt;
+  const long long tiles = (long long)tiles_of(P) * Hkv * row_tiles * B;
+  l = Layout{(const int*)lens, B, W, P, Hkv * row_tiles, row_tiles, wt, (int)(tiles < num_sms ? tiles : num_sms)};
+  return (long long)Hkv * row_tiles * B < 0x7fffff00LL;
+}
+
+}  // namespace shared_prefix
+}  // namespace kf
+
+extern "C" void* kf_status_device_ptr();
+
+extern "C" {
+
+// Bytes of scratch that kf_shared_prefix_attn_bf16 needs for these sizes (0: none), negative where it does not take them.
+long long kf_shared_prefix_scratch(int B, int W, int P, int H, int Hkv, int hd, int num_sms) {
+  using namespace kf::shared_prefix;
+  Layout l;
+  if (B < 1 || W < 1 || P < 0 || Hkv < 1 || H % Hkv || (hd != 64 && hd != 128) || !make_layout(l, nullptr, B, W, P, H / Hkv, Hkv, num_sms)) return -1;
+  return P == 0 ? 0 : slots(l) * TILE_ROWS * (hd * 4 + 8);
+}
+
+// o (B, W, H, hd), dense = attention of q (B, W, H, hd) over k, v (B, P, Hkv, hd), of which lens[b] positions count (null: all), and over
+// own_k, own_v (B, W, S, Hkv, hd), where position s of continuation w lies in the cache of continuation rows[b][w][s] (null: w).
+// steps: in elements, of q (prompt, continuation, head), k and v (prompt, position, head), own_k and own_v (prompt, continuation, position,
+// head) and rows (prompt, continuation): 19 numbers.  Head dim 64 or 128, dense; steps multiples of 8 and bases on 16 bytes (rows: any).
+int kf_shared_prefix_attn_bf16(const void* q, const void* k, const void* v, const void* own_k, const void* own_v, const void* lens,
+                               const void* rows, void* o, void* scratch, int B, int W, int P, int S, int H, int Hkv, int hd,
+                               const long long* steps, float scale, int num_sms, void* stream) {
+  using namespace kf::shared_prefix;
+  Layout l;
+  if (kf_shared_prefix_scratch(B, W, P, H, Hkv, hd, num_sms) < 0 || S < 0 || !(scale > 0.f)) return 3;
+  make_layout(l, lens, B, W, P, H / Hkv, Hkv, num_sms);
+  const long long *qs = steps, *ks = steps + 3, *vs = steps + 6, *oks = steps + 9, *ovs = steps + 13, *rs = steps + 17;
+  for (int i = 0; i < 17; ++i)
+    if (steps[i] & 7) return 5;
+  cudaStream_t st = (cudaStream_t)stream;
+  float* part_o = P > 0 ? (float*)scratch : nullptr;
+  float2* part_ml = P > 0 ? (float2*)(part_o + slots(l) * TILE_ROWS * hd) : nullptr;
+  if (P > 0) {
+    const int rc = launch_prefix(q, k, v, l, H, Hkv, hd, qs, ks, vs, scale, part_o, part_ml, (int*)kf_status_device_ptr(), st);
+    if (rc) return rc;
+  }
+  const Own a{(const __nv_bfloat16*)q, (const __nv_bfloat16*)own_k, (const __nv_bfloat16*)own_v, (__nv_bfloat16*)o, (const uint8_t*)rows, S, Hkv,
+              H / Hkv, qs[0], qs[1], qs[2], oks[0], oks[1], oks[2], oks[3], ovs[0], ovs[1], ovs[2], ovs[3], rs[0], rs[1],
+              scale * 1.4426950408889634f};
+  return hd == 128 ? launch_own<128>(a, l, part_o, part_ml, num_sms, st) : launch_own<64>(a, l, part_o, part_ml, num_sms, st);
+}
+
+}  // extern "C"

@@ -1,0 +1,516 @@
+// Attention of the new tokens of many continuations over the prompt that they share: partial results (first of two kernels).
+//
+// The W continuations of a prompt and the query heads of a key head are the rows of one tile, up to 128 of them, so that a key is read
+// once for all and S = Q K^T and O += P V are 128-row products on the tensor cores; one kernel per continuation reads it W times.
+// What bounds it: the keys and values, 4 hd bytes per position and head.  A tile of 128 keys of 128 values is 64 KB, which is 2700 cycles
+// of an SM's share of HBM; its two products take 512, its 16 384 exponentials 1024.  So rows that are not there (a tile is always 128)
+// cost nothing, and all that counts is to keep the copies in flight: three stages each of K and V (192 KB) run ahead of the products.
+//
+//   warp 0     : TMA producer of Q and K
+//   warp 1     : MMA issuer
+//   warp 2     : TMA producer of V (warp 3 only makes the first warpgroup whole)
+//   warps 4-7  : softmax of the even tiles of a unit, one thread per row
+//   warps 8-11 : softmax of the odd tiles
+//   TMEM       : S_even | S_odd | O_even | O_odd   (128 fp32 columns each; bf16 P over the start of its S)
+// The two softmax groups have maxima, sums and accumulators of their own, so neither waits for the other; they are joined where a unit ends.
+//
+// P is rounded to bf16 for the second product (2^-9 of each weight, and the sum of the weights is that of the unrounded ones);
+// maxima, sums and O are fp32, and so are the partial results.
+#include "attention_common.cuh"
+#include "shared_prefix.cuh"
+#include "skinny_common.cuh"
+
+namespace kf {
+namespace shared_prefix {
+
+using namespace kf::attn;
+
+constexpr int THREADS = 384;
+constexpr int REGS_ISSUE = 72, REGS_SOFTMAX = 216;  // per thread; 72 + 2 * 216 = 3 * 168, what the launch gets
+constexpr int TMEM_COLS = 512;
+constexpr int STAGES = 3;
+constexpr float RESCALE_THRESHOLD = 8.0f;           // P up to 2^8 before the accumulator is scaled again
+
+template <int HD>
+struct Cfg {
+  static constexpr int BLOCKS = HD / 64;
+  static constexpr int TILE_BYTES = TILE_KEYS * HD * 2;
+  static constexpr int BLOCK_BYTES = TILE_KEYS * 128;
+  static constexpr int TILES = 1 + 2 * STAGES;      // Q, K ring, V ring
+  static constexpr int STATS = 2 * TILE_ROWS * 8;   // (max, sum) of each group's rows
+  static constexpr int HEAD = 3 * 1024;             // STATS and the barriers, before the tiles, which start on 1024 bytes
+  static constexpr size_t SMEM = HEAD + TILES * size_t(TILE_BYTES);   // all of the 227 KB of a CTA at a head dim of 128
+};
+
+// Where a CTA is in its range.
+struct Walk {
+  int b, u, j, nt;      // prompt, unit of the prompt, tile of the unit, tiles of a unit of this prompt
+  long long left;       // tiles of the range that are still to come
+};
+
+__device__ __forceinline__ void advance(const Layout& l, Walk& w, int n) {
+  w.left -= n;
+  w.j = 0;
+  if (++w.u == l.per_prompt) {
+    w.u = 0;
+    if (w.left > 0) {
+      do {
+        w.nt = tiles_of(length(l, ++w.b));
+      } while (w.nt == 0);
+    }
+  }
+}
+
+__device__ __forceinline__ int segment(const Walk& w) { return int(w.left < w.nt - w.j ? w.left : w.nt - w.j); }
+
+// Start of this CTA's range, by one warp.
+__device__ Walk locate(const Layout& l) {
+  Walk w;
+  const long long total = tiles_before(l, l.B);
+  const int ctas = working(l, total), cta = int(blockIdx.x);
+  const long long t0 = cta < ctas ? range_begin(total, cta, ctas) : 0;
+  w.left = cta < ctas ? range_begin(total, cta + 1, ctas) - t0 : 0;
+  w.b = w.u = w.j = 0;
+  w.nt = 1;
+  if (w.left <= 0) return w;
+  long long before = 0;
+  if (!l.lens) {
+    w.b = int(t0 / ((long long)tiles_of(l.P) * l.per_prompt));
+    before = (long long)tiles_of(l.P) * l.per_prompt * w.b;
+  } else {
+    const int lane = threadIdx.x & 31;
+    for (int base = 0; base < l.B; base += 32) {
+      const long long own = base + lane < l.B ? (long long)tiles_of(length(l, base + lane)) * l.per_prompt : 0;
+      long long upto = own;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long v = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += v;
+      }
+      const uint32_t past = __ballot_sync(0xffffffffu, before + upto > t0);
+      if (past) {
+        const int at = __ffs(past) - 1;
+        w.b = base + at;
+        before += __shfl_sync(0xffffffffu, upto - own, at);
+        break;
+      }
+      before += __shfl_sync(0xffffffffu, upto, 31);
+    }
+  }
+  w.nt = tiles_of(length(l, w.b));
+  w.u = int((t0 - before) / w.nt);
+  w.j = int((t0 - before) % w.nt);
+  return w;
+}
+
+template <int N>
+__device__ __forceinline__ void regs_give() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void regs_take() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+
+template <int HD>
+__global__ void __launch_bounds__(THREADS, 1)
+kf_shared_prefix_tcgen05(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                         const __grid_constant__ CUtensorMap map_v, const Layout lay, int group, float scale_log2, float* __restrict__ part_o,
+                         float2* __restrict__ part_ml, int* status) {
+  using C = Cfg<HD>;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  const uint32_t smem_base = smem_u32(smem_raw) + C::HEAD;
+  uint8_t* smem = smem_raw + C::HEAD;
+  if (smem_base & 1023u) {   // not as declared: nothing is touched
+    if (threadIdx.x == 0) atomicCAS(status, 0, int(KF_ERR_WAIT_DRAIN));
+    return;
+  }
+  const uint32_t q_smem = smem_base, k_smem = q_smem + C::TILE_BYTES, v_smem = k_smem + STAGES * C::TILE_BYTES;
+  float2* stats = reinterpret_cast<float2*>(smem_raw);
+  uint8_t* bar_generic = smem_raw + C::STATS;
+  const uint32_t bar_base = smem_u32(bar_generic);
+  auto k_full = [&](int st) { return bar_base + 8u * st; };
+  auto k_empty = [&](int st) { return bar_base + 8u * (3 + st); };
+  auto v_full = [&](int st) { return bar_base + 8u * (6 + st); };
+  auto v_empty = [&](int st) { return bar_base + 8u * (9 + st); };
+  auto s_full = [&](int g) { return bar_base + 8u * (12 + g); };
+  auto p_half = [&](int g) { return bar_base + 8u * (14 + g); };   // weights of the first 64 keys are in tensor memory
+  auto p_full = [&](int g) { return bar_base + 8u * (16 + g); };
+  auto pv_done = [&](int g) { return bar_base + 8u * (18 + g); };
+  const uint32_t q_full = bar_base + 8u * 20, q_empty = bar_base + 8u * 21;
+  const uint32_t o_final = bar_base + 8u * 22, o_free = bar_base + 8u * 23, drain_bar = bar_base + 8u * 24;
+  volatile uint32_t* tmem_slot_ptr = reinterpret_cast<volatile uint32_t*>(bar_generic + 8 * 25);
+  Walk* start = reinterpret_cast<Walk*>(bar_generic + 8 * 26);
+
+  const int warp = warp_index();
+  const int lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < STAGES; ++i) {
+      mbar_init(k_full(i), 1);
+      mbar_init(k_empty(i), 1);
+      mbar_init(v_full(i), 1);
+      mbar_init(v_empty(i), 1);
+    }
+    for (int g = 0; g < 2; ++g) {
+      mbar_init(s_full(g), 1);
+      mbar_init(p_half(g), 4);
+      mbar_init(p_full(g), 4);
+      mbar_init(pv_done(g), 1);
+    }
+    mbar_init(q_full, 1);
+    mbar_init(q_empty, 1);
+    mbar_init(o_final, 1);
+    mbar_init(o_free, 8);
+    mbar_init(drain_bar, 1);
+    mbar_fence_init();
+    tma_prefetch_desc(&map_q);
+    tma_prefetch_desc(&map_k);
+    tma_prefetch_desc(&map_v);
+  }
+  if (warp == 1) {
+    tmem_alloc(smem_u32(const_cast<uint32_t*>(tmem_slot_ptr)), TMEM_COLS);
+    tmem_relinquish();
+  }
+  if (warp == 2) {
+    const Walk w = locate(lay);
+    if (lane == 0) *start = w;
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  grid_dep_launch();
+  const uint32_t tmem_base = *tmem_slot_ptr;
+  Walk wk = *start;
+  auto s_col = [&](int g) { return tmem_base + uint32_t(g * 128); };
+  auto o_col = [&](int g) { return tmem_base + uint32_t(256 + g * 128); };
+
+  if (warp < 4) {
+    regs_give<REGS_ISSUE>();
+    if (warp == 0) {
+      // ------------------------------------------------------------ TMA producer of Q and K
+      if (elect_one()) {
+        bool ok = true;
+        int i = 0, seg = 0, issued = 0, q_issued = 0;   // i, seg: tiles and units so far
+        while (wk.left > 0 && ok) {
+          const int n = segment(wk), hk = wk.u / lay.row_tiles, rt = wk.u % lay.row_tiles;
+          if (seg > 0 && !mbar_wait(q_empty, (seg - 1) & 1, status, KF_ERR_WAIT_EMPTY)) { ok = false; break; }
+          mbar_expect_tx(q_full, uint32_t(group * lay.wt * HD * 2));
+#pragma unroll
+          for (int c = 0; c < C::BLOCKS; ++c)
+            tma_load_4d(q_smem + c * C::BLOCK_BYTES, &map_q, q_full, 64 * c, hk * group, rt * lay.wt, wk.b);
+          ++q_issued;
+          for (int j = wk.j; j < wk.j + n; ++j, ++i) {
+            const int st = i % STAGES, use = i / STAGES;
+            if (use > 0 && !mbar_wait(k_empty(st), (use - 1) & 1, status, KF_ERR_WAIT_EMPTY)) { ok = false; break; }
+            mbar_expect_tx(k_full(st), C::TILE_BYTES);
+#pragma unroll
+            for (int c = 0; c < C::BLOCKS; ++c)
+              tma_load_4d(k_smem + st * C::TILE_BYTES + c * C::BLOCK_BYTES, &map_k, k_full(st), 64 * c, hk, j * TILE_KEYS, wk.b);
+            ++issued;
+          }
+          advance(lay, wk, n);
+          ++seg;
+        }
+        if (!ok) {
+          if (q_issued > 0) mbar_wait(q_full, (q_issued - 1) & 1, status, KF_ERR_WAIT_DRAIN);
+          for (int j = max(0, issued - STAGES); j < issued; ++j) mbar_wait(k_full(j % STAGES), (j / STAGES) & 1, status, KF_ERR_WAIT_DRAIN);
+        }
+      }
+    } else if (warp == 2) {
+      // ------------------------------------------------------------ TMA producer of V
+      if (elect_one()) {
+        bool ok = true;
+        int i = 0, issued = 0;
+        while (wk.left > 0 && ok) {
+          const int n = segment(wk), hk = wk.u / lay.row_tiles;
+          for (int j = wk.j; j < wk.j + n; ++j, ++i) {
+            const int st = i % STAGES, use = i / STAGES;
+            if (use > 0 && !mbar_wait(v_empty(st), (use - 1) & 1, status, KF_ERR_WAIT_EMPTY)) { ok = false; break; }
+            mbar_expect_tx(v_full(st), C::TILE_BYTES);
+#pragma unroll
+            for (int c = 0; c < C::BLOCKS; ++c)
+              tma_load_4d(v_smem + st * C::TILE_BYTES + c * C::BLOCK_BYTES, &map_v, v_full(st), 64 * c, hk, j * TILE_KEYS, wk.b);
+            ++issued;
+          }
+          advance(lay, wk, n);
+        }
+        if (!ok)
+          for (int j = max(0, issued - STAGES); j < issued; ++j) mbar_wait(v_full(j % STAGES), (j / STAGES) & 1, status, KF_ERR_WAIT_DRAIN);
+      }
+    } else if (warp == 1) {
+      // ------------------------------------------------------------ MMA issuer
+      if (elect_one()) {
+        constexpr uint32_t idesc_s = umma_idesc_bf16(TILE_ROWS, TILE_KEYS, false, false);
+        constexpr uint32_t idesc_o = umma_idesc_bf16(TILE_ROWS, HD, false, true);
+        bool ok = true;
+        int first = 0, seg = 0;        // tiles before this unit, units
+        int done[2] = {0, 0};          // tiles of each group whose P has been read
+        // S_g = Q K^T of the i-th tile of the range
+        auto issue_s = [&](int g, int i) {
+          const int st = i % STAGES;
+          if (!mbar_wait(k_full(st), (i / STAGES) & 1, status, KF_ERR_WAIT_FULL)) return false;
+          tc_fence_after();
+#pragma unroll
+          for (int kk = 0; kk < HD / 16; ++kk) {
+            const uint32_t off = (kk / 4) * C::BLOCK_BYTES + (kk % 4) * 32;
+            tc_mma_f16(s_col(g), umma_desc_sw128(q_smem + off, 16, 1024), umma_desc_sw128(k_smem + st * C::TILE_BYTES + off, 16, 1024),
+                       idesc_s, kk != 0);
+          }
+          tc_commit(s_full(g));
+          tc_commit(k_empty(st));
+          return true;
+        };
+        while (wk.left > 0 && ok) {
+          const int n = segment(wk);
+          ok = mbar_wait(q_full, seg & 1, status, KF_ERR_WAIT_FULL);
+          if (ok) tc_fence_after();
+          for (int i = 0; i < min(n, 2) && ok; ++i) ok = issue_s(i, first + i);
+          if (ok && n <= 2) tc_commit(q_empty);
+          // the accumulators of the unit before have been read
+          if (ok && seg > 0) ok = mbar_wait(o_free, (seg - 1) & 1, status, KF_ERR_WAIT_TMEM_EMPTY);
+          for (int i = 0; i < n && ok; ++i) {
+            const int g = i & 1, st = (first + i) % STAGES;
+            if (!mbar_wait(v_full(st), ((first + i) / STAGES) & 1, status, KF_ERR_WAIT_FULL)) { ok = false; break; }
+            // O_g += P_g V: A = P from tensor memory, B = V with the head dim contiguous, in two halves of the keys
+            if (!mbar_wait(p_half(g), done[g] & 1, status, KF_ERR_WAIT_TMEM_EMPTY)) { ok = false; break; }
+            tc_fence_after();
+#pragma unroll
+            for (int kk = 0; kk < TILE_KEYS / 32; ++kk)
+              tc_mma_f16_ts(o_col(g), s_col(g) + kk * 8, umma_desc_sw128(v_smem + st * C::TILE_BYTES + kk * 2048, C::BLOCK_BYTES, 1024),
+                            idesc_o, i >= 2 || kk != 0);
+            if (!mbar_wait(p_full(g), done[g] & 1, status, KF_ERR_WAIT_TMEM_EMPTY)) { ok = false; break; }
+            tc_fence_after();
+#pragma unroll
+            for (int kk = TILE_KEYS / 32; kk < TILE_KEYS / 16; ++kk)
+              tc_mma_f16_ts(o_col(g), s_col(g) + kk * 8, umma_desc_sw128(v_smem + st * C::TILE_BYTES + kk * 2048, C::BLOCK_BYTES, 1024),
+                            idesc_o, 1u);
+            tc_commit(pv_done(g));
+            tc_commit(v_empty(st));
+            ++done[g];
+            if (i + 1 == n) tc_commit(o_final);
+            // the group's next scores follow at once: the products just issued have read its P before they are written
+            if (i + 2 < n) {
+              ok = issue_s(g, first + i + 2);
+              if (ok && i + 3 == n) tc_commit(q_empty);
+            }
+          }
+          first += n;
+          ++seg;
+          advance(lay, wk, n);
+        }
+        if (!ok) {
+          tc_commit(drain_bar);
+          mbar_wait(drain_bar, 0, status, KF_ERR_WAIT_DRAIN);
+        }
+      }
+    }
+  } else {
+    // ------------------------------------------------------------ softmax: warps 4-7 even tiles, 8-11 odd tiles
+    regs_take<REGS_SOFTMAX>();
+    const int g = (warp >> 2) - 1;
+    const int quarter = warp & 3;
+    const int row = quarter * 32 + lane;
+    const uint32_t lane_off = uint32_t(quarter * 32) << 16;
+    const uint32_t t_s = s_col(g) + lane_off, t_o = o_col(g) + lane_off;
+    const float NEG_INF = -INFINITY;
+    bool ok = true;
+    int first = 0, seg = 0, mine = 0;   // tiles before this unit, units, tiles of this group
+    while (wk.left > 0) {
+      const int n = segment(wk), rt = wk.u % lay.row_tiles;
+      const int rows = min(lay.wt, lay.W - rt * lay.wt) * group;
+      const bool active = quarter * 32 < rows;   // the warp has rows at all
+      const int len = length(lay, wk.b);
+      float m_run = NEG_INF, l_run = 0.f;
+      for (int i = g; i < n; i += 2, ++mine) {
+        const int n0 = (wk.j + i) * TILE_KEYS;
+        if (ok && !mbar_wait(s_full(g), mine & 1, status, KF_ERR_WAIT_TMEM_FULL)) ok = false;
+        tc_fence_after();
+        if (n0 + TILE_KEYS > len && len < lay.P) {
+          // positions behind the prompt hold anything, and 0 times that need not be 0: their values become zeros
+          const int st = (first + i) % STAGES;
+          if (ok && !mbar_wait(v_full(st), ((first + i) / STAGES) & 1, status, KF_ERR_WAIT_FULL)) ok = false;
+          if (ok && n0 + row >= len) {
+#pragma unroll
+            for (int c = 0; c < C::BLOCKS; ++c)
+#pragma unroll
+              for (int e = 0; e < 8; ++e)
+                *reinterpret_cast<uint4*>(smem + (1 + STAGES + st) * C::TILE_BYTES + c * C::BLOCK_BYTES + row * 128 + e * 16) = make_uint4(0, 0, 0, 0);
+          }
+          fence_async_smem();
+        }
+        if (!active) {
+          // rows that are not there: whatever their P is, nobody reads what comes of it
+          __syncwarp();
+          tc_fence_before();
+          if (lane == 0) {
+            mbar_arrive(p_half(g));
+            mbar_arrive(p_full(g));
+          }
+          continue;
+        }
+        uint32_t sv[TILE_KEYS];
+#pragma unroll
+        for (int c = 0; c < TILE_KEYS / 32; ++c) tmem_ld_32x32_at(t_s + c * 32, sv + c * 32);
+        tmem_ld_wait();
+        if (n0 + TILE_KEYS > len) {
+#pragma unroll
+          for (int k = 0; k < TILE_KEYS; ++k) sv[k] = n0 + k < len ? sv[k] : __float_as_uint(NEG_INF);
+        }
+        float mx;
+        {
+          float mx4[4] = {NEG_INF, NEG_INF, NEG_INF, NEG_INF};
+#pragma unroll
+          for (int k = 0; k < TILE_KEYS; k += 8)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) mx4[q] = fmax3(mx4[q], __uint_as_float(sv[k + 2 * q]), __uint_as_float(sv[k + 2 * q + 1]));
+          mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
+        }
+        const float m_new = fmaxf(m_run, mx * scale_log2);
+        const bool grow = m_new > m_run + RESCALE_THRESHOLD;
+        if (__any_sync(0xffffffffu, grow)) {
+          const float alpha = grow ? (m_run == NEG_INF ? 0.f : fast_exp2(m_run - m_new)) : 1.f;
+          if (i >= 2) {
+            if (ok && !mbar_wait(pv_done(g), (mine - 1) & 1, status, KF_ERR_WAIT_TMEM_FULL)) ok = false;
+            tc_fence_after();
+#pragma unroll 1
+            for (int c = 0; c < HD / 32; ++c) {
+              uint32_t o[32];
+              tmem_ld_32x32_at(t_o + c * 32, o);
+              tmem_ld_wait();
+#pragma unroll
+              for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
+              tmem_st_32x32(t_o + c * 32, o);
+            }
+          }
+          if (grow) {
+            l_run *= alpha;
+            m_run = m_new;
+          }
+        }
+        const float m_use = m_run == NEG_INF ? 0.f : m_run;
+        const uint64_t scale2 = pack2(scale_log2, scale_log2), neg_m2 = pack2(-m_use, -m_use);
+        uint64_t lsum[4] = {0ull, 0ull, 0ull, 0ull};
+#pragma unroll
+        for (int c = 0; c < TILE_KEYS / 32; ++c) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int k = 0; k < 16; ++k) {
+            const uint64_t x2 = ffma2(pack2(__uint_as_float(sv[c * 32 + 2 * k]), __uint_as_float(sv[c * 32 + 2 * k + 1])), scale2, neg_m2);
+            float x0, x1;
+            unpack2(x2, x0, x1);
+            const float e0 = fast_exp2(x0), e1 = fast_exp2(x1);
+            lsum[k & 3] = fadd2(lsum[k & 3], pack2(e0, e1));
+            pk[k] = pack_bf16(e0, e1);
+          }
+          tmem_st_32x16(t_s + c * 16, pk);
+          if (c == 1) {
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(p_half(g));
+          }
+        }
+        float a0, a1;
+        unpack2(fadd2(fadd2(lsum[0], lsum[1]), fadd2(lsum[2], lsum[3])), a0, a1);
+        l_run += a0 + a1;
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(p_full(g));
+      }
+      // ---- the unit's partial result: both groups' rows joined, each group writes half of the columns
+      stats[g * TILE_ROWS + row] = make_float2(m_run, l_run);
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      const float2 other = stats[(1 - g) * TILE_ROWS + row];
+      const float top = fmaxf(m_run, other.x);
+      const float f_mine = m_run == NEG_INF ? 0.f : fast_exp2(m_run - top), f_other = other.x == NEG_INF ? 0.f : fast_exp2(other.x - top);
+      const float f0 = g == 0 ? f_mine : f_other, f1 = g == 0 ? f_other : f_mine;
+      if (ok && !mbar_wait(o_final, seg & 1, status, KF_ERR_WAIT_TMEM_FULL)) ok = false;
+      tc_fence_after();
+      if (ok && active) {
+        const long long slot = (long long)wk.b * lay.per_prompt + wk.u + blockIdx.x;
+        float* dst = part_o + (slot * TILE_ROWS + row) * HD;
+#pragma unroll 1
+        for (int c = 0; c < HD / 64; ++c) {
+          const int col = g * (HD / 2) + c * 32;
+          uint32_t o0[32], o1[32];
+          tmem_ld_32x32_at(o_col(0) + lane_off + col, o0);
+          if (n > 1) tmem_ld_32x32_at(o_col(1) + lane_off + col, o1);
+          tmem_ld_wait();
+          if (row < rows) {
+#pragma unroll
+            for (int k = 0; k < 32; k += 4) {
+              float v[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                v[e] = f0 * __uint_as_float(o0[k + e]);
+                if (n > 1) v[e] = __fmaf_rn(f1, __uint_as_float(o1[k + e]), v[e]);
+              }
+              *reinterpret_cast<float4*>(dst + col + k) = make_float4(v[0], v[1], v[2], v[3]);
+            }
+          }
+        }
+        if (g == 0 && row < rows) part_ml[slot * TILE_ROWS + row] = make_float2(top, f_mine * l_run + f_other * other.y);
+      }
+      tc_fence_before();
+      // the accumulators may be written again, and stats by the next unit
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      if (lane == 0) mbar_arrive(o_free);
+      first += n;
+      ++seg;
+      advance(lay, wk, n);
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, TMEM_COLS);
+  }
+}
+
+// bf16 tensor of four dimensions, the last one dense; steps in elements.  A box that reaches over an end is filled with zeros.
+static int make_map_4d(CUtensorMap* map, const void* base, const uint64_t (&size)[4], const long long (&step)[3], const uint32_t (&box_)[4]) {
+  EncodeTiledFn fn = encode_tiled_fn();
+  if (!fn) return -1;
+  cuuint64_t dims[4], strides[3];
+  cuuint32_t box[4], estr[4] = {1, 1, 1, 1};
+  for (int i = 0; i < 4; ++i) dims[i] = size[i], box[i] = box_[i];
+  for (int i = 0; i < 3; ++i) strides[i] = cuuint64_t(size[i + 1] > 1 ? step[i] * 2 : 16);   // of a single entry nothing is stepped over
+  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? 0 : (int)r;
+}
+
+template <int HD>
+static int launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const Layout& l, int group, float scale, float* part_o,
+                  float2* part_ml, int* status, cudaStream_t stream) {
+  auto kern = kf_shared_prefix_tcgen05<HD>;
+  static bool attr_set[16] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev >= 16 || !attr_set[dev]) {
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Cfg<HD>::SMEM);
+    if (e != cudaSuccess) return 300 + (int)e;
+    if (dev < 16) attr_set[dev] = true;
+  }
+  kern<<<(unsigned)l.ctas, THREADS, Cfg<HD>::SMEM, stream>>>(mq, mk, mv, l, group, scale * 1.4426950408889634f, part_o, part_ml, status);
+  cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? 0 : 400 + (int)e;
+}
+
+// Steps in elements: q prompt, continuation, head; k and v prompt, position, head.
+int launch_prefix(const void* q, const void* k, const void* v, const Layout& l, int H, int Hkv, int hd, const long long* qs, const long long* ks,
+                  const long long* vs, float scale, float* part_o, float2* part_ml, int* status, cudaStream_t stream) {
+  const int group = H / Hkv;
+  CUtensorMap mq, mk, mv;
+  int rc = make_map_4d(&mq, q, {(uint64_t)hd, (uint64_t)H, (uint64_t)l.W, (uint64_t)l.B}, {qs[2], qs[1], qs[0]},
+                       {64u, (uint32_t)group, (uint32_t)l.wt, 1u});
+  if (rc) return 1000 + rc;
+  rc = make_map_4d(&mk, k, {(uint64_t)hd, (uint64_t)Hkv, (uint64_t)l.P, (uint64_t)l.B}, {ks[2], ks[1], ks[0]}, {64u, 1u, (uint32_t)TILE_KEYS, 1u});
+  if (rc) return 2000 + rc;
+  rc = make_map_4d(&mv, v, {(uint64_t)hd, (uint64_t)Hkv, (uint64_t)l.P, (uint64_t)l.B}, {vs[2], vs[1], vs[0]}, {64u, 1u, (uint32_t)TILE_KEYS, 1u});
+  if (rc) return 3000 + rc;
+  return hd == 128 ? launch<128>(mq, mk, mv, l, group, scale, part_o, part_ml, status, stream)
+                   : launch<64>(mq, mk, mv, l, group, scale, part_o, part_ml, status, stream);
+}
+
+}  // namespace shared_prefix
+}  // namespace kf

@@ -25,6 +25,19 @@ __device__ __forceinline__ void cluster_sync_all() {
 __device__ __forceinline__ void grid_dep_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void grid_dep_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
+// Loads of what the previous kernel of the stream wrote, after grid_dep_wait.  Plain loads through a pointer that is const and
+// __restrict__ may be moved ahead of the wait, because the compiler takes such memory for constant throughout the kernel.
+__device__ __forceinline__ float2 ld_after_wait(const float2* p) {
+  float2 v;
+  asm volatile("ld.global.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "l"(p) : "memory");
+  return v;
+}
+__device__ __forceinline__ float4 ld_after_wait(const float4* p) {
+  float4 v;
+  asm volatile("ld.global.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(p) : "memory");
+  return v;
+}
+
 // (x, y) rotated by the angle of (c, s), spelled out because which of two products is fused with their sum decides one bf16 value in
 // 10^5, and the compiler chooses differently from kernel to kernel.  This is the choice of the rotary kernel.
 __device__ __forceinline__ void rotate_pair(float x, float y, float c, float s, float& rx, float& ry) {

@@ -298,6 +298,7 @@ PyObject* configure(PyObject*, PyObject* args) {
 }  // namespace
 
 #include "fp8_blocks_calls.h"
+#include "beam_calls.h"
 
 namespace {
 
@@ -310,6 +311,11 @@ PyMethodDef methods[] = {
     {"fp8_norm_linear_grads", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(fp8_norm_linear_grads)), METH_FASTCALL, "its gradients"},
     {"fp8_linear_grads", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(fp8_linear_grads)), METH_FASTCALL, "gradients of a product with a weight"},
     {"norm_grads", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(norm_grads)), METH_FASTCALL, "gradients of an RMSNorm and its gain"},
+    {"beam_select", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(beam_select)), METH_FASTCALL, "a step of beam search"},
+    {"beam_reorder", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(beam_reorder)), METH_FASTCALL, "states follow their parents"},
+    {"shared_prefix_attn", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(shared_prefix_attn)), METH_FASTCALL,
+     "attention of continuations of one prompt"},
+    {"beam_configure", beam_configure, METH_VARARGS, "the native entries of beam search"},
     {"fp8_configure", fp8_configure, METH_VARARGS, "the native entries of the block-scaled operators"},
     {"decode", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(decode)), METH_FASTCALL, "one new token per sequence through blocks"},
     {"configure", configure, METH_VARARGS, "classes and the native entry"},

@@ -139,6 +139,12 @@ def _declare(L: ctypes.CDLL) -> None:
         "kf_symm_pull_bf16": [vp, i, i, vp, vp, vp, vp, i, vp],
         "kf_symm_rs_shard_bf16": [vp, vp, i, i, i, vp, vp, vp, vp, i, i, vp],
         "kf_gemm_gather_bf16": [i, vp, vp, vp, i, i, i, i, i, i, vp, i, i, i, vp, vp, vp, vp, vp, vp, i, i, i, i, vp],
+        "kf_shared_prefix_scratch": [i] * 7,
+        "kf_shared_prefix_attn_bf16": [vp] * 9 + [i] * 7 + [vp, f, i, vp],
+        "kf_beam_splits": [ll, i, i, i],
+        "kf_beam_select": [vp, i, ll, ll, vp, vp, i, i, i, ll, ll, vp, i, vp, vp, vp, vp, vp],
+        "kf_beam_max_states": [],
+        "kf_beam_reorder": [vp, i, i, i, vp, i, i, vp],
         "kf_read_status": [],
         "kf_clear_status": [],
         "kf_status_device_ptr": [],
@@ -148,7 +154,7 @@ def _declare(L: ctypes.CDLL) -> None:
         if fn is None:
             continue
         fn.argtypes = args
-        fn.restype = c_void_p if name == "kf_status_device_ptr" else c_int
+        fn.restype = c_void_p if name == "kf_status_device_ptr" else ll if name == "kf_shared_prefix_scratch" else c_int
     if hasattr(L, "kf_clear_status"):
         L.kf_clear_status.restype = None
 
@@ -508,6 +514,9 @@ def _load_steps():
     mod.fp8_configure(*(ctypes.cast(getattr(lib(), name), c_void_p).value for name in (
         "kf_gemm_fp8_blocks", "kf_add_rmsnorm_fp8_blocks", "kf_fp8_blocks_cast_bf16", "kf_fp8_blocks_values_bf16",
         "kf_norm_grads_f32", "kf_norm_grads_blocks")))
+    mod.beam_configure(*(ctypes.cast(getattr(lib(), name), c_void_p).value for name in (
+        "kf_beam_splits", "kf_beam_select", "kf_beam_reorder", "kf_shared_prefix_scratch", "kf_shared_prefix_attn_bf16")),
+        BEAMS, lib().kf_beam_max_states())
     _steps = mod
     return mod
 
@@ -889,7 +898,7 @@ def gemm_fp8_swiglu_bwd(a8: torch.Tensor, b8: torch.Tensor, sa: torch.Tensor, sb
 
 # --------------------------------------------------------------------------- fp8 with a scale for each block of 128 (ops/fp8_blocks.py)
 def _step(name: str, *args, launches: int = 1):
-    """The answer of a call of ``csrc/fp8_blocks_calls.h`` on the current device's stream; None where the call is not plainly covered."""
+    """The answer of a call of ``csrc/fp8_blocks_calls.h`` or ``csrc/beam_calls.h`` on the current device's stream; None where the call is not plainly covered."""
     global LAUNCH_COUNT
     steps = _load_steps() if _steps is None else _steps
     if not steps:
@@ -1062,6 +1071,110 @@ def attn_fwd(q, k, v, causal: bool, doc_ids, scale: float):
         "kf_attn_fwd2_bf16" if two else "kf_attn_fwd_bf16",
     )
     return out, lse
+
+
+# --------------------------------------------------------------------------- attention over a shared prefix
+def _steps_of(t: torch.Tensor) -> list[int]:
+    """Strides of all dimensions but the last; of one entry nothing is stepped over."""
+    return [s if n > 1 else 0 for n, s in zip(t.shape[:-1], t.stride()[:-1])]
+
+
+def _copies_ok(t: torch.Tensor) -> torch.Tensor:
+    """`t` where 16-byte copies can take it: a dense last dimension, steps and base on 16 bytes; else a copy that is so."""
+    if (t.numel() == 0 or t.stride(-1) == 1 and t.data_ptr() % 16 == 0
+            and all(n == 1 or (s > 0 and s % 8 == 0) for n, s in zip(t.shape[:-1], t.stride()[:-1]))):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def shared_prefix_call(q, k, v, own_k, own_v, prefix_lens, own_rows, scale) -> torch.Tensor | None:
+    """:func:`shared_prefix_attn`, checked as well; None where Python's checks have to look."""
+    global LAUNCH_COUNT
+    out = _step("shared_prefix_attn", q, k, v, own_k, own_v, prefix_lens, own_rows, scale, sm_count())
+    if out is not None and k.shape[1]:
+        LAUNCH_COUNT += 1   # the kernel over the prompts
+    return out
+
+
+def shared_prefix_supported(q: torch.Tensor, k: torch.Tensor) -> bool:
+    b, w, h, hd = q.shape
+    return hd in (64, 128) and h // k.shape[2] <= 128 and b * w * h < 2**27 and k.shape[1] < 2**31 - 2**16
+
+
+def shared_prefix_attn(q, k, v, own_k, own_v, prefix_lens, own_rows, scale: float) -> torch.Tensor:
+    """q (B, W, H, hd), k / v (B, P, Hkv, hd), own_k / own_v (B, W, S, Hkv, hd) bf16, prefix_lens (B,) int32, own_rows (B, W, S) uint8."""
+    q, k, v, own_k, own_v = (_copies_ok(t) for t in (q, k, v, own_k, own_v))
+    b, w, h, hd = q.shape
+    p, hkv, s = k.shape[1], k.shape[2], own_k.shape[2]
+    if own_rows is not None and own_rows.stride(2) != 1:
+        own_rows = own_rows.contiguous()
+    L, sms = lib(), sm_count()
+    scratch = torch.empty(L.kf_shared_prefix_scratch(b, w, p, h, hkv, hd, sms), dtype=torch.uint8, device=q.device)
+    out = torch.empty((b, w, h, hd), dtype=q.dtype, device=q.device)
+    rows = own_rows.stride()[:2] if own_rows is not None else (0, 0)
+    steps = array("q", (*_steps_of(q), *_steps_of(k), *_steps_of(v), *_steps_of(own_k), *_steps_of(own_v), *rows))
+    _check(L.kf_shared_prefix_attn_bf16(q.data_ptr(), k.data_ptr(), v.data_ptr(), own_k.data_ptr(), own_v.data_ptr(), _ptr(prefix_lens),
+                                        _ptr(own_rows), out.data_ptr(), scratch.data_ptr(), b, w, p, s, h, hkv, hd, steps.buffer_info()[0],
+                                        float(scale), sms, _stream()), "kf_shared_prefix_attn_bf16", 2 if p else 1)
+    return out
+
+
+# --------------------------------------------------------------------------- beam search
+BEAMS = 32   # beams of a prompt that the kernels take: a warp's list is one candidate per lane
+_LOGITS = {torch.bfloat16: 0, torch.float32: 1, torch.float16: 2}
+
+
+def beam_select_call(logits, scores, finished, eos_id: int, pad_id: int):
+    """:func:`beam_select`, checked as well; None where Python's checks have to look."""
+    return _step("beam_select", logits, scores, finished, eos_id, pad_id, sm_count(), launches=2)
+
+
+def beam_reorder_call(states: list, parents, length, out: list | None) -> bool:
+    """:func:`beam_reorder` of all states, checked as well; False where Python's checks have to look."""
+    global LAUNCH_COUNT
+    steps = _load_steps() if _steps is None else _steps
+    device = torch._C._cuda_getDevice()
+    n = steps.beam_reorder(states, parents, length, out, sm_count(), device, torch._C._cuda_getCurrentRawStream(device)) if steps else None
+    if n is None:
+        return False
+    if n < 0:
+        raise NativeKernelError(f"beam_reorder failed with code {-n}")
+    LAUNCH_COUNT += n
+    return True
+
+
+def beam_select_supported(logits: torch.Tensor) -> bool:
+    return (logits.dtype in _LOGITS and logits.shape[1] <= BEAMS and logits.stride(2) == 1 and logits.shape[2] < 2**31 - 2**16
+            and logits.shape[0] * logits.shape[1] < 2**27)
+
+
+def beam_select(logits: torch.Tensor, scores: torch.Tensor, finished: torch.Tensor | None, eos_id: int, pad_id: int):
+    """(scores, parents, tokens, finished), (B, W) each, of logits (B, W, V) whose last dimension is dense; the others are contiguous."""
+    b, w, v = logits.shape
+    L, rows = lib(), b * w
+    splits = L.kf_beam_splits(rows, v, logits.element_size(), sm_count())
+    scratch = torch.empty(splits * rows * (16 + 8 * w), dtype=torch.uint8, device=logits.device)
+    out = (torch.empty_like(scores), torch.empty((b, w), dtype=torch.int64, device=logits.device),
+           torch.empty((b, w), dtype=torch.int64, device=logits.device), torch.empty((b, w), dtype=torch.bool, device=logits.device))
+    _check(L.kf_beam_select(logits.data_ptr(), _LOGITS[logits.dtype], logits.stride(0), logits.stride(1), scores.data_ptr(), _ptr(finished),
+                            b, w, v, eos_id, pad_id, scratch.data_ptr(), splits, *(t.data_ptr() for t in out), _stream()), "kf_beam_select", 2)
+    return out
+
+
+def beam_reorder(moves, parents: torch.Tensor) -> None:
+    """``moves``: (source, destination, bytes of a beam that move) of states whose beams are dense; the same tensor, or no overlap."""
+    b, w = parents.shape
+    L = lib()
+    most = L.kf_beam_max_states()
+    for lo in range(0, len(moves), most):
+        part = moves[lo : lo + most]
+        table = array("q")
+        for src, dst, n in part:
+            size = src.element_size()
+            table.extend((src.data_ptr(), dst.data_ptr(), src.stride(0) * size, src.stride(1) * size, dst.stride(0) * size,
+                          dst.stride(1) * size, n))
+        _check(L.kf_beam_reorder(table.buffer_info()[0], len(part), b, w, parents.data_ptr(), int(parents.dtype == torch.int64), sm_count(),
+                                 _stream()), "kf_beam_reorder")
 
 
 # --------------------------------------------------------------------------- Lion / schedule-free AdamW

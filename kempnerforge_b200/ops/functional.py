@@ -14,6 +14,7 @@ the optimizer and the reduce-scatter read the flat buffer directly.
 
 from __future__ import annotations
 
+import contextlib
 import math
 import os
 
@@ -336,6 +337,67 @@ def attention(
         )
         return out.transpose(1, 2)
     return ref.attention(q, k, v, causal, doc_ids, key_padding_mask, scale)
+
+
+def _on_device(t: torch.Tensor):
+    """Kernels go to the current device's stream: that of `t` has to be current."""
+    return contextlib.nullcontext() if t.device.index == torch._C._cuda_getDevice() else torch.cuda.device(t.device)
+
+
+def shared_prefix_attention(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    own_k: torch.Tensor,
+    own_v: torch.Tensor,
+    prefix_lens: torch.Tensor | None = None,
+    own_rows: torch.Tensor | None = None,
+    scale: float | None = None,
+) -> torch.Tensor:
+    """One new token for each of W continuations of B prompts: softmax(q [K | own K]ᵀ * scale) [V | own V] -> (B, W, H, hd).
+
+    q (B, W, H, hd); k, v (B, P, Hkv, hd): the prompts' keys and values, read once for all continuations; own_k, own_v
+    (B, W, S, Hkv, hd): those of each continuation's own tokens, the new one's included.  P or S may be 0.
+
+    ``prefix_lens`` (B,) int32 or int64: how many positions of each prompt count, 0 .. P; what lies behind them is not looked at.
+    ``own_rows`` (B, W, S) uint8: position s of continuation w lies in the own cache of continuation ``own_rows[b, w, s]`` of the same
+    prompt, which lets beams be exchanged without moving their caches; a value that is no continuation hides the position.
+    A continuation that sees nothing gives zeros.  ``scale`` is positive.
+
+    bf16 with heads of 64 or 128 runs ``csrc/shared_prefix_tcgen05.cu`` and ``csrc/shared_prefix_own.cu``; other types and sizes, calls
+    that want gradients, and CPU tensors the formulas of ``ops.ref``.
+    """
+    if q.is_cuda and not _FORCE_REF and _cuda().attn_policy() == "native":
+        out = _cuda().shared_prefix_call(q, k, v, own_k, own_v, prefix_lens, own_rows, scale)
+        if out is not None:
+            return out
+    if q.dim() != 4 or k.dim() != 4 or own_k.dim() != 5:
+        raise ValueError(f"q is (B, W, H, hd), k (B, P, Hkv, hd), own_k (B, W, S, Hkv, hd), not {tuple(q.shape)}, {tuple(k.shape)}, {tuple(own_k.shape)}")
+    b, w, h, hd = q.shape
+    hkv, s = k.shape[2], own_k.shape[2]
+    if (v.shape != k.shape or own_v.shape != own_k.shape or k.shape[0] != b or k.shape[3] != hd or own_k.shape != (b, w, s, hkv, hd)
+            or hkv == 0 or h % hkv or h == 0 or hd == 0):
+        raise ValueError(f"shapes do not belong together: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}, own_k {tuple(own_k.shape)}, "
+                         f"own_v {tuple(own_v.shape)}")
+    for t in (k, v, own_k, own_v):
+        if t.dtype != q.dtype or t.device != q.device:
+            raise ValueError(f"q is {q.dtype} on {q.device}, a cache {t.dtype} on {t.device}")
+    if prefix_lens is not None and (prefix_lens.shape != (b,) or prefix_lens.dtype not in (torch.int32, torch.int64) or prefix_lens.device != q.device):
+        raise ValueError(f"prefix_lens is ({b},) int32 or int64 on {q.device}, not {tuple(prefix_lens.shape)} {prefix_lens.dtype} on {prefix_lens.device}")
+    if own_rows is not None and (own_rows.shape != (b, w, s) or own_rows.dtype != torch.uint8 or own_rows.device != q.device):
+        raise ValueError(f"own_rows is {(b, w, s)} uint8 on {q.device}, not {tuple(own_rows.shape)} {own_rows.dtype} on {own_rows.device}")
+    scale = 1.0 / math.sqrt(hd) if scale is None else float(scale)
+    if not 0.0 < scale < math.inf:
+        raise ValueError(f"scale {scale} is not positive")
+    needs_grad = torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, own_k, own_v))
+    if b * w and use_native(q) and not needs_grad and _cuda().attn_policy() == "native" and _cuda().shared_prefix_supported(q, k):
+        with _on_device(q):
+            if prefix_lens is not None:
+                if prefix_lens.dtype != torch.int32:
+                    prefix_lens = prefix_lens.clamp(0, k.shape[1]).to(torch.int32)
+                prefix_lens = prefix_lens.contiguous()
+            return _cuda().shared_prefix_attn(q, k, v, own_k, own_v, prefix_lens, own_rows, scale)
+    return ref.shared_prefix_attention(q, k, v, own_k, own_v, prefix_lens, own_rows, scale)
 
 
 class _QKVAttnFn(torch.autograd.Function):

@@ -117,6 +117,85 @@ def attention(
     return out
 
 
+def shared_prefix_attention(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    own_k: torch.Tensor,
+    own_v: torch.Tensor,
+    prefix_lens: torch.Tensor | None = None,
+    own_rows: torch.Tensor | None = None,
+    scale: float | None = None,
+) -> torch.Tensor:
+    """One new token of each of W continuations of B prompts.  q (B, W, H, hd); k, v (B, P, Hkv, hd) and own_k, own_v
+    (B, W, S, Hkv, hd); ``own_rows[b, w, s]``: the continuation whose own cache holds position s of continuation w (a value that is
+    none: nowhere).  What is not visible takes no part, whatever it holds; a row that sees nothing is zero."""
+    b, w, h, hd = q.shape
+    p, hkv, s = k.shape[1], k.shape[2], own_k.shape[2]
+    scale = 1.0 / math.sqrt(hd) if scale is None else scale
+    qf = _wide(q).reshape(b, w, hkv, h // hkv, hd)
+    kf, vf, okf, ovf = _wide(k), _wide(v), _wide(own_k), _wide(own_v)
+    sees = torch.ones(b, 1, 1, 1, p, dtype=torch.bool, device=q.device)
+    if prefix_lens is not None:
+        sees = (torch.arange(p, device=q.device) < prefix_lens[:, None])[:, None, None, None]
+        vf = torch.where(sees[:, 0, 0, 0, :, None, None], vf, 0.0)
+    own_sees = torch.ones(b, w, 1, 1, s, dtype=torch.bool, device=q.device)
+    if own_rows is not None:
+        own_sees = (own_rows < w)[:, :, None, None]
+        at = torch.arange(b, device=q.device)[:, None, None], own_rows.long().clamp_max(w - 1), torch.arange(s, device=q.device)
+        okf, ovf = okf[at], torch.where(own_sees[:, :, 0, 0, :, None, None], ovf[at], 0.0)
+    scores = torch.cat([torch.einsum("bwkgd,bpkd->bwkgp", qf, kf).masked_fill(~sees, float("-inf")),
+                        torch.einsum("bwkgd,bwskd->bwkgs", qf, okf).masked_fill(~own_sees, float("-inf"))], dim=-1) * scale
+    some = torch.cat([sees.expand(b, w, 1, 1, p), own_sees], dim=-1).any(-1, keepdim=True)
+    probs = torch.softmax(scores, dim=-1) if p + s else scores
+    probs = torch.where(some, probs, 0.0)
+    out = torch.einsum("bwkgp,bpkd->bwkgd", probs[..., :p], vf) + torch.einsum("bwkgs,bwskd->bwkgd", probs[..., p:], ovf)
+    return out.reshape(b, w, h, hd).to(q.dtype)
+
+
+# --------------------------------------------------------------------------- beam search
+def beam_select(logits: torch.Tensor, scores: torch.Tensor, finished: torch.Tensor | None, eos_id: int, pad_id: int):
+    """(scores, parents, tokens, finished), each (B, W): the W best of a prompt's candidates, in 64 bits.  A beam's candidates are ordered
+    by logit, then by token; all by score, then by beam.  NaN logits count as -inf, +inf as the type's largest number."""
+    b, w, vocab = logits.shape
+    x = logits.double()
+    x = torch.where(x > float("-inf"), x.clamp_max(torch.finfo(logits.dtype).max), float("-inf"))
+    top = x.amax(-1, keepdim=True)
+    shifted = torch.where(x > float("-inf"), x - top, float("-inf"))
+    lse = top + shifted.exp().sum(-1, keepdim=True).log()
+    x, token = torch.sort(x, dim=-1, descending=True, stable=True)
+    x, token = x[..., :w], token[..., :w]
+    total = torch.where(x > float("-inf"), scores.double()[..., None] + (x - lse), float("-inf"))
+    done = torch.zeros_like(scores, dtype=torch.bool) if finished is None else finished
+    only = torch.full_like(total, float("-inf"))
+    only[..., 0] = scores.double()
+    total = torch.where(done[..., None], only, total)
+    total = torch.where((scores > float("-inf"))[..., None], total, float("-inf"))
+    token = torch.where(done[..., None], pad_id, token)
+    width = total.shape[-1]
+    total, at = torch.sort(total.flatten(1), dim=-1, descending=True, stable=True)
+    if width < w:   # fewer tokens than beams
+        total, at = (torch.nn.functional.pad(t, (0, max(0, w - t.shape[1])), value=fill) for t, fill in ((total, float("-inf")), (at, 0)))
+    total, at = total[:, :w], at[:, :w]
+    none = total == float("-inf")
+    parents = torch.where(none, torch.arange(w, device=logits.device), at // width)
+    tokens = torch.where(none, pad_id, torch.gather(token.flatten(1), 1, at))
+    ended = torch.gather(done, 1, parents)
+    return total.float(), parents, tokens, ~none & (ended | (tokens == eos_id))
+
+
+def beam_reorder(states, parents: torch.Tensor, length: int | None, out) -> None:
+    """out[b, w, :length] = state[b, parents[b, w], :length]; where the parent is no beam, out stays."""
+    w = parents.shape[1]
+    ok = (parents >= 0) & (parents < w)
+    rows = torch.arange(parents.shape[0], device=parents.device)[:, None]
+    for x, y in zip(states, out):
+        n = x.shape[2] if length is None and x.dim() > 2 else length
+        src, dst = (x, y) if n is None else (x[:, :, :n], y[:, :, :n])
+        new = src[rows, parents.clamp(0, w - 1).long()]
+        dst.copy_(torch.where(ok.view(*ok.shape, *([1] * (x.dim() - 2))), new, dst))
+
+
 # --------------------------------------------------------------------------- mlp
 def swiglu(gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor:
     return F.silu(gate) * up
