@@ -1,6 +1,6 @@
 """Model zoo: decoder-only transformer (dense / MoE) and the vision-language wrappers."""
 
-from kempnerforge_b200.models.attention import Attention, KVCache
+from kempnerforge_b200.models.attention import Attention, KVCache, SharedPrefixCache
 from kempnerforge_b200.models.embedding import OutputHead, TokenEmbedding
 from kempnerforge_b200.models.init import init_weights
 from kempnerforge_b200.models.mlp import StandardMLP, SwiGLUMLP, build_mlp

@@ -46,6 +46,48 @@ class KVCache:
         self.seq_len = 0
 
 
+class SharedPrefixCache:
+    """Keys and values of ``width`` continuations of each prompt of a batch: the prompts' own, once, and those of each continuation's
+    tokens, (batch, width, position, kv_head, head_dim).  A generation step over it has batch x width rows, the continuations of a
+    prompt side by side.
+
+    ``rows`` (batch, width, position) uint8, shared by all layers: in which continuation's cache a position lies.  Beams are exchanged by
+    :func:`kempnerforge_b200.ops.beam.reorder` of the rows alone; the keys stay where they are.
+    """
+
+    def __init__(self, prefix: KVCache, width: int, max_new: int, rows: torch.Tensor | None = None) -> None:
+        n = prefix.seq_len
+        self.k, self.v = prefix.k[:, :n], prefix.v[:, :n]
+        shape = (self.k.shape[0], width, max_new, *self.k.shape[2:])
+        self.own_k = torch.zeros(shape, dtype=self.k.dtype, device=self.k.device)
+        self.own_v = torch.zeros(shape, dtype=self.v.dtype, device=self.v.device)
+        self.rows, self.width, self.prefix_len, self.seq_len = rows, width, n, n
+
+    @staticmethod
+    def new_rows(batch: int, width: int, max_new: int, device) -> torch.Tensor:
+        """Every position in its own continuation's cache."""
+        if width > 256:
+            raise ValueError(f"{width} continuations: their numbers are bytes")
+        room = -(-max_new // 16) * 16   # beams on 16 bytes, which a reordering moves in one word
+        own = torch.arange(width, device=device, dtype=torch.uint8)[None, :, None]
+        return own.expand(batch, width, room).contiguous()[:, :, :max_new]
+
+    def attend(self, q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor) -> torch.Tensor:
+        """Append one position (batch x width, 1, kv_head, head_dim) and attend to all: q (batch x width, 1, heads, head_dim)."""
+        at, b, w = self.seq_len - self.prefix_len, self.k.shape[0], self.width
+        if q.shape[0] != b * w or q.shape[1] != 1 or k_new.shape[:2] != q.shape[:2]:
+            raise ValueError(f"one new token for each of {b} x {w} continuations, not {tuple(q.shape[:2])}")
+        if at >= self.own_k.shape[2]:
+            raise ValueError(f"KV cache overflow: {at + 1} > {self.own_k.shape[2]} new tokens")
+        self.own_k[:, :, at] = k_new.reshape(b, w, *k_new.shape[2:])
+        self.own_v[:, :, at] = v_new.reshape(b, w, *v_new.shape[2:])
+        self.seq_len += 1
+        rows = None if self.rows is None else self.rows[:, :, : at + 1]
+        out = F.shared_prefix_attention(q.view(b, w, *q.shape[2:]), self.k, self.v, self.own_k[:, :, : at + 1], self.own_v[:, :, : at + 1],
+                                        own_rows=rows)
+        return out.view(q.shape)
+
+
 class Attention(nn.Module):
     def __init__(
         self,
@@ -78,7 +120,7 @@ class Attention(nn.Module):
         x: torch.Tensor,
         rope_cos: torch.Tensor,
         rope_sin: torch.Tensor,
-        kv_cache: KVCache | None = None,
+        kv_cache: KVCache | SharedPrefixCache | None = None,
         doc_ids: torch.Tensor | None = None,
         key_padding_mask: torch.Tensor | None = None,
         qkv: torch.Tensor | None = None,
@@ -108,10 +150,15 @@ class Attention(nn.Module):
             )
         qkv = F.rope(qkv, rope_cos, rope_sin, n_rot_heads=h + hkv)
         q, k, v = qkv[:, :, :h], qkv[:, :, h : h + hkv], qkv[:, :, h + hkv :]
-        if kv_cache is not None:
+        shared = isinstance(kv_cache, SharedPrefixCache)
+        if shared and (doc_ids is not None or key_padding_mask is not None or self.capture_attention_weights):
+            raise ValueError("a step over a shared prefix takes no masks and keeps no attention weights")
+        if kv_cache is not None and not shared:
             k, v = kv_cache.update(k, v)
         causal = kv_cache is None or s > 1
-        if self.capture_attention_weights:
+        if shared:
+            out = kv_cache.attend(q, k, v)
+        elif self.capture_attention_weights:
             out, probs = ref.attention(q, k, v, causal, doc_ids, key_padding_mask, return_weights=True)
             self.last_attention_weights = probs.detach()
         else:

@@ -2,15 +2,17 @@
 
 ``sample``: temperature -> top-k -> top-p (nucleus) -> multinomial; temperature 0 is greedy.
 ``generate``: one prefill pass over the prompt, then one token per step against the caches.
+``beam_search``: the most likely continuations; the beams of a prompt share its cache and exchange no keys.
 
-Parity: kempnerforge/model/generate.py:15-131.
+Parity: kempnerforge/model/generate.py:15-131 (``beam_search`` has no counterpart there).
 """
 
 from __future__ import annotations
 
 import torch
 
-from kempnerforge_b200.models.attention import KVCache
+from kempnerforge_b200.models.attention import KVCache, SharedPrefixCache
+from kempnerforge_b200.ops import beam
 
 
 def sample(logits: torch.Tensor, temperature: float = 1.0, top_k: int = 0, top_p: float = 1.0,
@@ -66,3 +68,59 @@ def generate(model, prompt_tokens: torch.Tensor, max_new_tokens: int, temperatur
     if was_training:
         model.train()
     return out
+
+
+@torch.no_grad()
+def beam_search(model, prompt_tokens: torch.Tensor, max_new_tokens: int, num_beams: int = 4, eos_token_id: int | None = None,
+                length_penalty: float = 1.0) -> tuple[torch.Tensor, torch.Tensor]:
+    """The ``num_beams`` best continuations that a beam search finds for each prompt (batch, prompt length): (token ids
+    (batch, num_beams, prompt length + new), scores (batch, num_beams) fp32), best first.
+
+    A score is the sum of the new tokens' log-probabilities divided by their number to the power ``length_penalty`` (an
+    ``eos_token_id`` counts, what follows it does not, and is filled with it).  During the search beams compete by their sums; a finished
+    one keeps its place as long as its sum does.  The search ends when all beams have finished or at ``max_new_tokens``.
+    """
+    cfg = model.config
+    b, plen = prompt_tokens.shape
+    w, total = int(num_beams), plen + max_new_tokens
+    if w < 1 or w > 256:
+        raise ValueError(f"num_beams {num_beams} is not between 1 and 256")
+    if plen < 1:
+        raise ValueError("a search needs a prompt of at least one token")
+    if total > cfg.max_seq_len:
+        raise ValueError(f"prompt ({plen}) + max_new_tokens ({max_new_tokens}) = {total} exceeds model max_seq_len "
+                         f"({cfg.max_seq_len})")
+    dev = prompt_tokens.device
+    if max_new_tokens <= 0 or b == 0:
+        return prompt_tokens[:, None].expand(b, w, plen).clone(), torch.zeros(b, w, device=dev)
+    param = next(model.parameters())
+    hd = cfg.head_dim
+    caches = [KVCache(b, plen, layer.attention.k_proj.weight.shape[0] // hd, hd, param.dtype, param.device)
+              for layer in model.layers.values()]
+    was_training = model.training
+    model.eval()
+    logits = model(prompt_tokens, kv_caches=caches)[:, -1:].expand(b, w, -1)
+    rows = SharedPrefixCache.new_rows(b, w, max_new_tokens, dev)
+    caches = [SharedPrefixCache(c, w, max_new_tokens, rows) for c in caches]
+    pad = 0 if eos_token_id is None else eos_token_id
+    scores = torch.full((b, w), float("-inf"), device=dev)
+    scores[:, 0] = 0.0   # the beams of a prompt are one until the first choice
+    finished = torch.zeros(b, w, dtype=torch.bool, device=dev)
+    tokens = torch.full((b, w, max_new_tokens), pad, dtype=torch.int64, device=dev)
+    for n in range(max_new_tokens):
+        step = beam.select(logits, scores, finished, eos_token_id, pad)
+        if n:
+            beam.reorder([tokens, rows], step.parents, n)
+        tokens[:, :, n] = step.tokens
+        scores, finished = step.scores, step.finished
+        if n + 1 == max_new_tokens or (eos_token_id is not None and bool(finished.all())):
+            break
+        logits = model(step.tokens.view(b * w, 1), kv_caches=caches)[:, -1].view(b, w, -1)
+    if was_training:
+        model.train()
+    tokens = tokens[:, :, : n + 1]
+    ends = (tokens == eos_token_id) if eos_token_id is not None else torch.zeros_like(tokens, dtype=torch.bool)
+    lengths = (ends.cumsum(2) - ends.long() == 0).sum(2)
+    scores, order = (scores / lengths**length_penalty).sort(dim=1, descending=True, stable=True)
+    tokens = tokens.gather(1, order[:, :, None].expand_as(tokens))
+    return torch.cat([prompt_tokens[:, None].expand(b, w, plen), tokens], dim=2), scores

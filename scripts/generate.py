@@ -5,7 +5,7 @@
     python scripts/generate.py cfg.toml --checkpoint ... --interactive
 
 Same contract as the reference's scripts/generate.py:42-151 (DCP ``{"model": ...}`` load, prompt or REPL,
-temperature / top-k / top-p sampling).  Without a tokenizer path the prompt is read as space-separated token ids.
+temperature / top-k / top-p sampling), and ``--num-beams`` for a beam search.  Without a tokenizer path the prompt is read as space-separated token ids.
 """
 
 from __future__ import annotations
@@ -21,7 +21,7 @@ import torch.distributed.checkpoint as dcp  # noqa: E402
 
 from kempnerforge_b200.config import load_config  # noqa: E402
 from kempnerforge_b200.models import Transformer  # noqa: E402
-from kempnerforge_b200.models.generate import generate  # noqa: E402
+from kempnerforge_b200.models.generate import beam_search, generate  # noqa: E402
 
 
 def load_model(cfg, checkpoint: str | None, device: torch.device) -> Transformer:
@@ -47,6 +47,8 @@ def main(argv=None) -> int:
     ap.add_argument("--top-k", "--top_k", dest="top_k", type=int, default=0)
     ap.add_argument("--top-p", "--top_p", dest="top_p", type=float, default=1.0)
     ap.add_argument("--seed", type=int, default=0)
+    ap.add_argument("--num-beams", type=int, default=0, help="beam search over this many beams instead of sampling (0: sample)")
+    ap.add_argument("--length-penalty", type=float, default=1.0, help="beams are ranked by log-probability / length ** this")
     ap.add_argument("--interactive", action="store_true")
     ap.add_argument("--device", default=None, help="default: cuda when available")
     ap.add_argument("--dtype", default=None, choices=["float32", "bfloat16", "float16"])
@@ -69,6 +71,10 @@ def main(argv=None) -> int:
         room = cfg.model.max_seq_len - len(ids)
         if room <= 0:
             raise SystemExit(f"the prompt has {len(ids)} tokens; the model's context is {cfg.model.max_seq_len}")
+        if args.num_beams > 0:
+            out = beam_search(model, x, min(args.max_new_tokens, room), args.num_beams, tok.eos_token_id if tok else None, args.length_penalty)[0][0, 0]
+            new = out.tolist()
+            return tok.decode(new) if tok else " ".join(map(str, new))
         out = generate(model, x, min(args.max_new_tokens, room), args.temperature, args.top_k, args.top_p,
                        eos_token_id=tok.eos_token_id if tok else None,
                        generator=None if device.type == "cuda" else gen)
