@@ -2,30 +2,36 @@
 //
 // kf_beam_select.  Of each prompt's W beams with scores s_w and logits l_w (V values each) the W best pairs (w, t) by
 //     s_w + l_w[t] - log sum_t' exp(l_w[t']) .
-// Within a beam the order of candidates is that of its logits, so W tokens of each beam are all that can be among the best, and one pass
-// over the logits finds them together with the sum: kf_beam_rows.  Every warp keeps the W largest logits that it has met, one per lane,
-// as 64-bit keys (the logit's bits in an order-preserving form, then the complement of its index: of equal logits the lowest index is
-// the largest key).  A vector of logits costs a packed maximum and a compare with the warp's W-th largest; only what is above it is
-// inserted, W ln(n / W) times for n values in random order.  The sum runs over exp(x - m) with m the largest so far, in fp32 per thread
-// (at most a few hundred terms each) and in 64 bits from there on, because candidates of different beams may lie close together.  The
-// difference is taken before the factor log2 e: rows of the type's lowest value have exponents of zero like any others, and no product
-// overflows.
-// What bounds it: the logits are read once.  A row is split over blocks so that a few rows fill the GPU too; kf_beam_merge, one block a
-// prompt, joins the splits, one warp a beam, and picks W times the best of the beams' heads.
+// Within a beam the order of candidates is that of its logits, so W tokens of each beam are all that can be among the best.  One cluster
+// of CTAs a prompt; the logits of its beams, one after the other, are dealt out to the CTAs in equal ranges.
+//   * One pass over the logits: a thread keeps the largest of its logits and the sum of exp(x - largest), in fp32 over at most a few hundred
+//     terms and in 64 bits from there on, because candidates of different beams may lie close together.  The difference is taken before the
+//     factor log2 e: rows of the type's lowest value have exponents of zero like any others, and no product overflows.
+//   * The W-th largest of the threads' largest logits is at most the W-th largest logit, so only threads whose largest is not below it
+//     can hold one of the W best: about W of them, whose logits are read again (out of L2).  A list that every warp kept on the way, which
+//     costs an insertion for each of W ln(n / W) logits, took 98 us where this takes 24 (64 x 8 x 128 256 bf16).
+//   * Candidates are 64-bit keys: the logit's bits in an order-preserving form, then the complement of its index, so that of equal
+//     logits the lowest index is the largest key; sorted by a warp, and joined over the cluster through distributed shared memory.
+// What bounds it: the logits are read once.
 //
 // kf_beam_reorder.  state[b, w] = state[b, parent[b, w]] for all states in one launch.  A thread owns 16 bytes of a column: it reads
 // the column's W values and then writes them, so that parents may be any selection of beams, also in place, without a second buffer.
 #include "common.cuh"
-#include "skinny_common.cuh"
+#include "decode_common.cuh"
 
 #include <cuda_fp16.h>
 
 namespace kf {
 namespace beam {
 
+using decode::mapa_shared;
+
 constexpr int MAX_BEAMS = 32;   // a warp's list is one key per lane
 constexpr int WARPS = 8;
 constexpr int THREADS = WARPS * 32;
+constexpr int MIN_CTAS = 8;     // of a cluster
+constexpr int MAX_PARTS = MAX_BEAMS / MIN_CTAS + 1;   // rows that a CTA's range meets
+constexpr int ROOM = WARPS * MAX_BEAMS;       // candidates that a CTA sorts; more (equal logits) go through lists
 constexpr double LOG2E_D = 1.44269504088896340736;
 
 typedef unsigned long long Key;
@@ -59,7 +65,7 @@ __device__ __forceinline__ float min_of(float a, float b) {
   return r;
 }
 
-// The largest `width` keys that a warp has met, lane i the i-th (0 = none).
+// Key by key: the largest `width` that a warp has met, lane i the i-th (0 = none).
 struct TopList {
   Key mine = 0, worst = 0;
   // All lanes call; each offers a key (0 = nothing).
@@ -79,20 +85,29 @@ struct TopList {
   }
 };
 
-// What a block leaves of its part of a row: the largest logit m and the sum of exp(x - m) over the part; its keys lie beside.
-struct Part {
-  double sum, m;
-};
-// Of the kernel before this one (see ld_after_wait).
-__device__ __forceinline__ Part load_part(const Part* p) {
-  Part v;
-  asm volatile("ld.global.v2.f64 {%0, %1}, [%2];" : "=d"(v.sum), "=d"(v.m) : "l"(p) : "memory");
-  return v;
+// One step of a warp's sorting network: lanes `j` apart, the larger one to the lower lane where `down`.
+template <typename K>
+__device__ __forceinline__ K exchange(K k, int j, bool down) {
+  const K other = __shfl_xor_sync(0xffffffffu, k, j);
+  const bool larger = ((threadIdx.x & j) == 0) == down;
+  return (k > other) == larger ? k : other;
 }
-__device__ __forceinline__ Key load_key(const Key* p) {
-  Key v;
-  asm volatile("ld.global.u64 %0, [%1];" : "=l"(v) : "l"(p) : "memory");
-  return v;
+// A warp's keys, largest first.
+template <typename K>
+__device__ __forceinline__ K sorted(K k) {
+#pragma unroll
+  for (int n = 2; n <= 32; n *= 2)
+#pragma unroll
+    for (int j = n / 2; j > 0; j /= 2) k = exchange(k, j, (threadIdx.x & n & 31) == 0);
+  return k;
+}
+// The 32 largest of two sorted lists.
+__device__ __forceinline__ Key merged(Key a, Key b) {
+  const Key other = __shfl_sync(0xffffffffu, b, 31 - (threadIdx.x & 31));
+  Key k = a > other ? a : other;
+#pragma unroll
+  for (int j = 16; j > 0; j /= 2) k = exchange(k, j, true);
+  return k;
 }
 
 // Logits as floats: 16 bytes of them.  NaN counts as -inf, +inf as the type's largest number.
@@ -140,172 +155,299 @@ struct Logits<__half> {
   static __device__ __forceinline__ float one(const __half* p) { return clean(__half2float(*p)); }
 };
 
-// A beam that has candidates: a score above -inf (not NaN).  A finished one has a single candidate and needs no pass over its logits.
-__device__ __forceinline__ bool alive(const float* scores, long long row) { return scores[row] > -INFINITY; }
+__device__ __forceinline__ double max_double(double a, double b) { return a > b ? a : b; }
 
-template <typename T>
-__global__ void __launch_bounds__(THREADS)
-kf_beam_rows(const T* __restrict__ logits, long long stride_b, long long stride_w, const float* __restrict__ scores,
-             const uint8_t* __restrict__ finished, int W, int V, int splits, int chunk, Part* __restrict__ parts, Key* __restrict__ keys) {
-  constexpr int N = Logits<T>::N;
-  constexpr float LOG2E = 1.4426950408889634f;
-  __shared__ Key lists[WARPS][MAX_BEAMS];
-  __shared__ float ms[WARPS];
-  __shared__ double sums[WARPS];
-  grid_dep_launch();
-  const long long row = blockIdx.x / splits;
-  const int split = int(blockIdx.x % splits);
-  if (!alive(scores, row) || (finished && finished[row])) return;   // kf_beam_merge asks nothing of this row's parts
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const T* x0 = logits + (row / W) * stride_b + (row % W) * stride_w;
-
-  TopList top;
-  float m = -INFINITY, sum = 0.f;
-  auto add = [&](float x) {   // one value (lanes without one pass -inf)
-    const float mn = fmaxf(m, x);
-    if (mn == -INFINITY) return;
-    sum = (m == -INFINITY ? 0.f : sum * exp2_fast((m - mn) * LOG2E)) + exp2_fast((x - mn) * LOG2E);
-    m = mn;
-  };
-  // the row from its first 16-byte boundary on in vectors; what is left at both ends is the first split's
-  const int head = min(V, int((16 - (reinterpret_cast<uintptr_t>(x0) & 15)) & 15) / int(sizeof(T)));
-  const int vectors = (V - head) / N;
-  const int tail0 = head + vectors * N;
-  if (split == 0 && warp == 0) {
-    int i = -1;
-    if (lane < head) i = lane;
-    else if (lane >= 16 && tail0 + lane - 16 < V) i = tail0 + lane - 16;
-    const float x = i >= 0 ? Logits<T>::one(x0 + i) : -INFINITY;
-    add(x);
-    top.offer(x > -INFINITY ? make_key(x, uint32_t(i)) : 0, W);
-  }
-  const uint4* vec = reinterpret_cast<const uint4*>(x0 + head);
-  const int v0 = split * chunk, v1 = min(vectors, v0 + chunk);
-  constexpr int UNROLL = 4;
-  for (int base = v0 + warp * 32; base < v1; base += THREADS * UNROLL) {
-    uint4 raw[UNROLL];
-#pragma unroll
-    for (int u = 0; u < UNROLL; ++u) {
-      const int i = base + u * THREADS + lane;
-      if (i < v1) raw[u] = __ldcs(vec + i);
-    }
-#pragma unroll
-    for (int u = 0; u < UNROLL; ++u) {
-      const int i = base + u * THREADS + lane;
-      float x[N];
-      if (i < v1) {
-        Logits<T>::load(raw[u], x);
-      } else {
-#pragma unroll
-        for (int j = 0; j < N; ++j) x[j] = -INFINITY;
-      }
-      float mx = x[0];
-#pragma unroll
-      for (int j = 1; j < N; ++j) mx = max_of(mx, x[j]);
-      if (mx > m) {
-        sum *= m == -INFINITY ? 0.f : exp2_fast((m - mx) * LOG2E);
-        m = mx;
-      }
-      const float b = m == -INFINITY ? 0.f : m;
-#pragma unroll
-      for (int j = 0; j < N; ++j) sum += exp2_fast((x[j] - b) * LOG2E);
-      if (__any_sync(0xffffffffu, mx > -INFINITY && ordered(mx) >= uint32_t(top.worst >> 32))) {
-#pragma unroll
-        for (int j = 0; j < N; ++j) top.offer(x[j] > -INFINITY ? make_key(x[j], uint32_t(head + i * N + j)) : 0, W);
-      }
-    }
-  }
-
-  // the warp's sum, then the block's
-  float wm = m;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) wm = fmaxf(wm, __shfl_xor_sync(0xffffffffu, wm, o));
-  double ws = m == -INFINITY ? 0.0 : double(sum) * exp2((double(m) - double(wm)) * LOG2E_D);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) ws += __shfl_xor_sync(0xffffffffu, ws, o);
-  if (lane == 0) ms[warp] = wm, sums[warp] = ws;
-  lists[warp][lane] = top.mine;
-  __syncthreads();
-  if (warp != 0) return;
-  for (int i = 1; i < WARPS; ++i) top.offer(lists[i][lane], W);
-  if (lane < W) keys[(long long)blockIdx.x * W + lane] = top.mine;
-  if (lane == 0) {
-    float bm = -INFINITY;
-    for (int i = 0; i < WARPS; ++i) bm = fmaxf(bm, ms[i]);
-    double bs = 0.0;
-    for (int i = 0; i < WARPS; ++i)
-      if (ms[i] > -INFINITY) bs += sums[i] * exp2((double(ms[i]) - double(bm)) * LOG2E_D);
-    parts[blockIdx.x] = Part{bs, double(bm)};
-  }
+__device__ __forceinline__ unsigned long long ld_cluster_u64(uint32_t addr) {
+  unsigned long long v;
+  asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(addr) : "memory");
+  return v;
 }
 
-// One block a prompt, one warp a beam.
-__global__ void kf_beam_merge(const Part* parts, const Key* keys, const float* __restrict__ scores,
-                              const uint8_t* __restrict__ finished, int W, int splits, long long eos, long long pad,
-                              float* __restrict__ out_scores, long long* __restrict__ out_parents, long long* __restrict__ out_tokens,
-                              uint8_t* __restrict__ out_finished) {
-  extern __shared__ __align__(8) uint8_t smem[];
-  double* total = reinterpret_cast<double*>(smem);                        // [W][W], best first, -inf: none
-  uint32_t* token = reinterpret_cast<uint32_t*>(total + W * W);           // [W][W]
-  const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const long long row = (long long)blockIdx.x * W + w;
-  grid_dep_wait();
-  const double NONE = -INFINITY;
-  const bool done = finished && finished[row];
-  if (alive(scores, row) && !done) {
-    const Part* p = parts + row * splits;
-    const Key* k = keys + row * splits * W;
-    double m = -INFINITY;
-    for (int i = lane; i < splits; i += 32) m = fmax(m, load_part(p + i).m);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmax(m, __shfl_xor_sync(0xffffffffu, m, o));
-    double sum = 0.0;
-    for (int i = lane; i < splits; i += 32) {
-      const Part x = load_part(p + i);
-      if (x.m > -INFINITY) sum += x.sum * exp2((x.m - m) * LOG2E_D);
+// The order of doubles as unsigned integers, and back.
+__device__ __forceinline__ Key ordered(double x) {
+  const Key u = Key(__double_as_longlong(x == 0.0 ? 0.0 : x));
+  return (u >> 63) ? ~u : u | (1ull << 63);
+}
+__device__ __forceinline__ double unordered(Key o) { return __longlong_as_double((o >> 63) ? (long long)(o & ~(1ull << 63)) : (long long)~o); }
+
+template <typename T>
+__global__ void __launch_bounds__(THREADS, 4)
+kf_beam_select(const T* __restrict__ logits, long long stride_b, long long stride_w, const float* __restrict__ scores,
+               const uint8_t* __restrict__ finished, int W, int V, long long eos, long long pad, float* __restrict__ out_scores,
+               long long* __restrict__ out_parents, long long* __restrict__ out_tokens, uint8_t* __restrict__ out_finished) {
+  constexpr int N = Logits<T>::N;
+  constexpr float LOG2E = 1.4426950408889634f;
+  constexpr int UNROLL = 8;
+  struct Part {
+    double m, sum;
+    Key keys[MAX_BEAMS];
+  };
+  __shared__ Part parts[MAX_PARTS];
+  __shared__ uint32_t tops[WARPS][MAX_BEAMS];      // each warp's threads by their largest logit
+  __shared__ double ms[WARPS], sums[WARPS];
+  __shared__ uint32_t bound;
+  __shared__ int n_readers, n_found;
+  __shared__ uint16_t readers[THREADS];
+  __shared__ Key found[WARPS * MAX_BEAMS];         // ROOM candidates, or the warps' lists
+  __shared__ double total[MAX_BEAMS * MAX_BEAMS];  // [W][W], best first, -inf: none
+  __shared__ uint32_t token[MAX_BEAMS * MAX_BEAMS];
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tid = threadIdx.x;
+  const int ctas = int(cluster_nctaid()), rank = int(cluster_ctarank());
+  const long long b = blockIdx.x / ctas, first = b * W;
+  // Beams whose logits count.  One without a score above -inf (or with NaN) has no candidates, a finished one has itself.
+  const bool alive = lane < W && scores[first + lane] > -INFINITY;
+  const bool done = lane < W && finished != nullptr && finished[first + lane];
+  const uint32_t live = __ballot_sync(0xffffffffu, alive && !done);
+  const int per = V / N + 1;                       // vectors of a row, at most
+  const long long all = (long long)__popc(live) * per;
+  const int working = all < ctas ? int(all) : ctas;   // CTAs that have a range, and one that is not empty
+  const long long r0 = rank < working ? all * rank / working : 0, r1 = rank < working ? all * (rank + 1) / working : 0;
+
+  int part = 0;
+  for (long long pos = r0; pos < r1; ++part) {
+    const int nth = int(pos / per), v0 = int(pos % per);
+    const int v_end = int(r1 - pos < per - v0 ? v0 + (r1 - pos) : per);
+    pos += v_end - v0;
+    const int w = __fns(live, 0, nth + 1);
+    const T* x0 = logits + b * stride_b + w * stride_w;
+    // vectors from the row's first 16-byte boundary on; what is left at both ends goes with the first vector, a value a thread
+    const int misaligned = int(reinterpret_cast<uintptr_t>(x0) & 15) / int(sizeof(T));
+    const int head = misaligned ? min(V, N - misaligned) : 0;
+    const int vectors = (V - head) / N, tail0 = head + vectors * N;
+    const int v1 = min(v_end, vectors);
+    const uint4* vec = reinterpret_cast<const uint4*>(x0 + head);
+    auto single = [&](int t) { return v0 != 0 ? -1 : t < head ? t : t >= N && t - N < V - tail0 ? tail0 + t - N : -1; };
+
+    float m = -INFINITY, sum = 0.f;
+    if (tid < 2 * N) {
+      const int i = single(tid);
+      const float x = i >= 0 ? Logits<T>::one(x0 + i) : -INFINITY;
+      if (x > -INFINITY) m = x, sum = 1.f;
     }
+    for (int base = v0 + tid; base < v1; base += THREADS * UNROLL) {
+      uint4 raw[UNROLL];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    const double lse = m + log(sum);
-    TopList top;
-    for (int i = 0; i < splits * W; i += 32) top.offer(i + lane < splits * W ? load_key(k + i + lane) : 0, W);
+      for (int u = 0; u < UNROLL; ++u)
+        if (base + u * THREADS < v1) raw[u] = vec[base + u * THREADS];
+#pragma unroll
+      for (int u = 0; u < UNROLL; ++u) {
+        if (base + u * THREADS >= v1) break;
+        float x[N];
+        Logits<T>::load(raw[u], x);
+        float mx = x[0];
+#pragma unroll
+        for (int j = 1; j < N; ++j) mx = max_of(mx, x[j]);
+        if (mx > m) {
+          sum = m == -INFINITY ? 0.f : sum * exp2_fast((m - mx) * LOG2E);
+          m = mx;
+        } else {
+          m = max_of(m, mx);   // apart where both are below the smallest normal number, which the compare takes for zeros
+        }
+        const float from = m == -INFINITY ? 0.f : m;
+        float s[2] = {0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < N; ++j) s[j & 1] += exp2_fast((x[j] - from) * LOG2E);
+        sum += s[0] + s[1];
+      }
+    }
+
+    // ---- the sum, and each warp's threads in order
+    double wm = double(m), ws = double(sum);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) wm = max_double(wm, __shfl_xor_sync(0xffffffffu, wm, o));
+    if (m > -INFINITY) ws *= double(exp2_fast(float(double(m) - wm) * LOG2E));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) ws += __shfl_xor_sync(0xffffffffu, ws, o);
+    if (lane == 0) ms[warp] = wm, sums[warp] = ws;
+    const uint32_t best = m > -INFINITY ? ordered(m) : 0u;   // 0: none
+    const uint32_t in_order = sorted(best);
+    tops[warp][lane] = in_order;
+    if (tid == 0) n_readers = n_found = 0;
+    __syncthreads();
+    // ---- the W-th largest of the threads' largest: that with W - 1 before it (equal ones in the order of the warps)
     if (lane < W) {
-      total[w * W + lane] = top.mine ? double(scores[row]) + (double(key_value(top.mine)) - lse) : NONE;
-      token[w * W + lane] = key_index(top.mine);
+      int before = lane;
+      for (int x = 0; x < WARPS; ++x) {
+        if (x == warp) continue;
+        // the lists are sorted: how many of the first W come before mine
+        for (int i = 0; i < W; ++i) {
+          const uint32_t other = tops[x][i];
+          if (other < in_order || (other == in_order && x > warp)) break;
+          ++before;
+        }
+      }
+      if (before == W - 1) bound = in_order;
     }
-  } else if (lane < W) {
-    total[w * W + lane] = done && lane == 0 && alive(scores, row) ? double(scores[row]) : NONE;
+    __syncthreads();
+    if (best != 0u && best >= bound) readers[atomicAdd(&n_readers, 1)] = uint16_t(tid);
+    __syncthreads();
+    // ---- the logits of these threads again
+    const int n = n_readers;
+    const uint32_t least = bound;
+    for (int i = warp; i < n; i += WARPS) {
+      const int t = readers[i];
+      for (int base = v0 + t; base < v1; base += THREADS * 32) {
+        const int at = base + lane * THREADS;
+        if (at < v1) {
+          float x[N];
+          Logits<T>::load(vec[at], x);
+#pragma unroll
+          for (int j = 0; j < N; ++j)
+            if (x[j] > -INFINITY && ordered(x[j]) >= least) {
+              const int to = atomicAdd(&n_found, 1);
+              if (to < ROOM) found[to] = make_key(x[j], uint32_t(head + at * N + j));
+            }
+        }
+      }
+      if (lane == 0 && t < 2 * N && single(t) >= 0) {
+        const float x = Logits<T>::one(x0 + single(t));
+        if (x > -INFINITY && ordered(x) >= least) {
+          const int to = atomicAdd(&n_found, 1);
+          if (to < ROOM) found[to] = make_key(x, uint32_t(single(t)));
+        }
+      }
+    }
+    __syncthreads();
+    const int candidates = n_found;
+    Key mine = 0;
+    if (candidates <= ROOM) {
+      if (warp == 0)
+        for (int i = 0; i < candidates; i += 32) {
+          const Key k = sorted(i + lane < candidates ? found[i + lane] : 0);
+          mine = i ? merged(mine, k) : k;
+        }
+    } else {
+      // so many equal logits that there is no room: every warp through the whole of its vectors
+      TopList top;
+      for (int base = v0 + warp * 32; base < v1; base += THREADS) {
+        const int at = base + lane;
+        float x[N];
+        if (at < v1) Logits<T>::load(vec[at], x);
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+          top.offer(at < v1 && x[j] > -INFINITY && ordered(x[j]) >= least ? make_key(x[j], uint32_t(head + at * N + j)) : 0, W);
+      }
+      if (warp == 0) {
+        const int i = lane < 2 * N ? single(lane) : -1;
+        const float x = i >= 0 ? Logits<T>::one(x0 + i) : -INFINITY;
+        top.offer(x > -INFINITY ? make_key(x, uint32_t(i)) : 0, W);
+      }
+      found[warp * MAX_BEAMS + lane] = top.mine;
+      __syncthreads();
+      if (warp == 0)
+        for (int i = 0; i < WARPS; ++i) mine = i ? merged(mine, found[i * MAX_BEAMS + lane]) : found[lane];
+    }
+    if (warp == 0) {
+      parts[part].keys[lane] = mine;
+      double pm = lane < WARPS ? ms[lane] : -INFINITY;
+      const double own = pm;
+#pragma unroll
+      for (int o = WARPS / 2; o > 0; o >>= 1) pm = max_double(pm, __shfl_xor_sync(0xffffffffu, pm, o));
+      double ps = lane < WARPS && own > -INFINITY ? sums[lane] * exp2((own - pm) * LOG2E_D) : 0.0;
+#pragma unroll
+      for (int o = WARPS / 2; o > 0; o >>= 1) ps += __shfl_xor_sync(0xffffffffu, ps, o);
+      if (lane == 0) parts[part].m = pm, parts[part].sum = ps;
+    }
+    __syncthreads();
+  }
+
+  cluster_sync_all();
+  // ---- the first CTA joins what the cluster found, a warp a beam
+  const double NONE = -INFINITY;
+  if (rank == 0) {
+    for (int w = warp; w < W; w += WARPS) {
+      const bool w_alive = scores[first + w] > -INFINITY;
+      if ((live >> w) & 1u) {
+        const int nth = __popc(live & ((1u << w) - 1u));
+        const long long u0 = (long long)nth * per, u1 = u0 + per - 1;
+        const int c0 = int(((u0 + 1) * working - 1) / all), c1 = int(((u1 + 1) * working - 1) / all);   // CTAs that hold its first and last vector
+        auto part_of = [&](int c) {
+          const long long begin = all * c / working;
+          return mapa_shared(smem_u32(&parts[nth - int(begin / per)]), uint32_t(c));
+        };
+        double m = NONE, sum = 0.0, own_m = NONE, own_sum = 0.0;
+        if (lane <= c1 - c0) {
+          const uint32_t at = part_of(c0 + lane);
+          own_m = __longlong_as_double((long long)ld_cluster_u64(at));
+          own_sum = __longlong_as_double((long long)ld_cluster_u64(at + 8));
+        }
+        m = own_m;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) m = max_double(m, __shfl_xor_sync(0xffffffffu, m, o));
+        sum = own_m > NONE ? own_sum * exp2((own_m - m) * LOG2E_D) : 0.0;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        const double lse = m + log(sum);
+        Key mine = 0;
+        const int count = (c1 - c0 + 1) * W;
+        for (int i = 0; i < count; i += 32) {
+          Key k = 0;
+          if (i + lane < count) k = ld_cluster_u64(part_of(c0 + (i + lane) / W) + 16 + 8 * ((i + lane) % W));
+          k = sorted(k);
+          mine = i ? merged(mine, k) : k;
+        }
+        if (lane < W) {
+          total[w * W + lane] = mine ? double(scores[first + w]) + (double(key_value(mine)) - lse) : NONE;
+          token[w * W + lane] = key_index(mine);
+        }
+      } else if (lane < W) {
+        total[w * W + lane] = lane == 0 && w_alive ? double(scores[first + w]) : NONE;   // finished, or nothing
+      }
+    }
   }
   __syncthreads();
-  if (w != 0) return;
-  // lane = beam; its best candidate that is not taken yet
-  int at = 0, parent = lane, place = -1;
-  double mine = lane < W ? total[lane * W] : NONE, score = NONE;
-  for (int r = 0; r < W; ++r) {
-    double best = mine;
-    int who = lane;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const double other = __shfl_xor_sync(0xffffffffu, best, o);
-      const int whose = __shfl_xor_sync(0xffffffffu, who, o);
-      if (other > best || (other == best && whose < who)) best = other, who = whose;
+  if (rank == 0 && warp == 0) {
+    // lane = beam; its best candidate that is not taken yet.  The score in two halves: the larger, of equal ones the lower beam.
+    int at = 0, parent = lane, place = -1;
+    const Key none = ordered(NONE);
+    Key mine = lane < W ? ordered(total[lane * W]) : none, score = none;
+    for (int r = 0; r < W; ++r) {
+      const uint32_t hi = __reduce_max_sync(0xffffffffu, uint32_t(mine >> 32));
+      const uint32_t lo = __reduce_max_sync(0xffffffffu, uint32_t(mine >> 32) == hi ? uint32_t(mine) : 0u);
+      const Key best = (Key(hi) << 32) | lo;
+      if (best <= none) break;
+      const int who = __ffs(__ballot_sync(0xffffffffu, mine == best)) - 1;
+      const int taken = __shfl_sync(0xffffffffu, at, who);
+      if (lane == r) score = best, parent = who, place = taken;
+      if (lane == who) {
+        ++at;
+        mine = at < W ? ordered(total[lane * W + at]) : none;
+      }
     }
-    if (best == NONE) break;
-    const int taken = __shfl_sync(0xffffffffu, at, who);
-    if (lane == r) score = best, parent = who, place = taken;
-    if (lane == who) {
-      ++at;
-      mine = at < W ? total[lane * W + at] : NONE;
+    const uint32_t ends = __ballot_sync(0xffffffffu, done);
+    if (lane < W) {
+      const bool ended = place >= 0 && ((ends >> parent) & 1u);
+      const long long t = place < 0 || ended ? pad : (long long)token[parent * W + place];
+      out_scores[first + lane] = float(unordered(score));
+      out_parents[first + lane] = parent;
+      out_tokens[first + lane] = t;
+      out_finished[first + lane] = ended || (place >= 0 && t == eos);
     }
   }
-  if (lane >= W) return;
-  const long long first = (long long)blockIdx.x * W, to = first + lane;
-  const bool ended = place >= 0 && finished && finished[first + parent];
-  const long long t = place < 0 || ended ? pad : (long long)token[parent * W + place];
-  out_scores[to] = float(score);
-  out_parents[to] = parent;
-  out_tokens[to] = t;
-  out_finished[to] = ended || (place >= 0 && t == eos);
+  cluster_sync_all();   // no CTA leaves while the first reads its shared memory
+}
+
+template <typename T>
+static int launch_select(const void* logits, long long stride_b, long long stride_w, const float* scores, const uint8_t* finished, int B, int W, int V,
+                         long long eos, long long pad, float* out_scores, long long* out_parents, long long* out_tokens, uint8_t* out_finished,
+                         int num_sms, cudaStream_t stream) {
+  auto kern = kf_beam_select<T>;
+  cudaLaunchConfig_t cfg = {};
+  const int ctas = MIN_CTAS;
+  if ((long long)B * ctas > 0x7fffffffLL) return 6;
+  cfg.gridDim = dim3((unsigned)(B * ctas));
+  cfg.blockDim = dim3(THREADS);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)ctas;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kern, (const T*)logits, stride_b, stride_w, scores, finished, W, V, eos, pad, out_scores, out_parents,
+                                     out_tokens, out_finished);
+  return e == cudaSuccess ? 0 : 500 + (int)e;
 }
 
 // ------------------------------------------------------------------ reorder
@@ -389,55 +531,21 @@ static void launch_reorder(const States& st, int n, int beams, const void* paren
 
 extern "C" {
 
-// How many blocks share a row of V logits.
-int kf_beam_splits(long long rows, int V, int size, int num_sms) {
-  // eight blocks an SM at most; a block has at least one vector of 16 bytes for each of its threads
-  const long long most = ((long long)V * size + 16 * kf::beam::THREADS - 1) / (16 * kf::beam::THREADS);
-  long long s = (8LL * num_sms) / (rows > 0 ? rows : 1);
-  if (s > most) s = most;
-  return s < 1 ? 1 : (int)s;
-}
-
 // logits (B, W, V) with strides in elements and V side by side; type 0 bf16, 1 fp32, 2 fp16.  scores (B, W) fp32, finished (B, W) bytes
-// or null.  parts: splits * B * W * (16 + 8 W) bytes of scratch, on 16.  Writes scores, parents, tokens and finished (B, W).
+// or null.  Writes scores, parents, tokens and finished (B, W).
 int kf_beam_select(const void* logits, int type, long long stride_b, long long stride_w, const void* scores, const void* finished, int B, int W,
-                   int V, long long eos, long long pad, void* parts, int splits, void* out_scores, void* out_parents, void* out_tokens,
-                   void* out_finished, void* stream) {
+                   int V, long long eos, long long pad, void* out_scores, void* out_parents, void* out_tokens, void* out_finished, int num_sms,
+                   void* stream) {
   using namespace kf::beam;
-  const long long rows = (long long)B * W;
-  if (B < 1 || W < 1 || W > MAX_BEAMS || V < 1 || splits < 1 || rows * splits > 0x7fffffffLL) return 3;
-  cudaStream_t st = (cudaStream_t)stream;
-  const int size = type == 1 ? 4 : 2, per = 16 / size;
-  const int vectors = V / per + 1;
-  const int chunk = (vectors + splits - 1) / splits;
-  Part* p = (Part*)parts;
-  Key* k = (Key*)(p + rows * splits);
-  const unsigned grid = (unsigned)(rows * splits);
-  const float* sc = (const float*)scores;
-  const uint8_t* fin = (const uint8_t*)finished;
-  if (type == 0)
-    kf_beam_rows<__nv_bfloat16><<<grid, THREADS, 0, st>>>((const __nv_bfloat16*)logits, stride_b, stride_w, sc, fin, W, V, splits, chunk, p, k);
-  else if (type == 1)
-    kf_beam_rows<float><<<grid, THREADS, 0, st>>>((const float*)logits, stride_b, stride_w, sc, fin, W, V, splits, chunk, p, k);
-  else if (type == 2)
-    kf_beam_rows<__half><<<grid, THREADS, 0, st>>>((const __half*)logits, stride_b, stride_w, sc, fin, W, V, splits, chunk, p, k);
-  else
-    return 4;
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return 400 + (int)e;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)B);
-  cfg.blockDim = dim3((unsigned)W * 32);
-  cfg.dynamicSmemBytes = size_t(W) * W * 12;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  e = cudaLaunchKernelEx(&cfg, kf_beam_merge, (const Part*)p, (const Key*)k, sc, fin, W, splits, eos, pad, (float*)out_scores,
-                         (long long*)out_parents, (long long*)out_tokens, (uint8_t*)out_finished);
-  return e == cudaSuccess ? 0 : 500 + (int)e;
+  if (B < 1 || W < 1 || W > MAX_BEAMS || V < 1) return 3;
+  auto go = [&](auto launch) {
+    return launch(logits, stride_b, stride_w, (const float*)scores, (const uint8_t*)finished, B, W, V, eos, pad, (float*)out_scores,
+                  (long long*)out_parents, (long long*)out_tokens, (uint8_t*)out_finished, num_sms, (cudaStream_t)stream);
+  };
+  if (type == 0) return go(launch_select<__nv_bfloat16>);
+  if (type == 1) return go(launch_select<float>);
+  if (type == 2) return go(launch_select<__half>);
+  return 4;
 }
 
 int kf_beam_max_states() { return kf::beam::MAX_STATES; }

@@ -13,9 +13,8 @@
 namespace {
 
 struct Beam {
-  int (*splits)(long long, int, int, int) = nullptr;
-  int (*select)(const void*, int, long long, long long, const void*, const void*, int, int, int, long long, long long, void*, int, void*, void*, void*,
-                void*, void*) = nullptr;
+  int (*select)(const void*, int, long long, long long, const void*, const void*, int, int, int, long long, long long, void*, void*, void*, void*, int,
+                void*) = nullptr;
   int (*reorder)(const long long*, int, int, int, const void*, int, int, void*) = nullptr;
   long long (*scratch)(int, int, int, int, int, int, int) = nullptr;
   int (*attention)(const void*, const void*, const void*, const void*, const void*, const void*, const void*, void*, void*, int, int, int, int, int, int,
@@ -50,14 +49,12 @@ PyObject* beam_select(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
       (f && (f->scalar_type() != at::kBool || f->sizes() != s->sizes() || !f->is_contiguous())))
     Py_RETURN_NONE;
   HANDLE_TH_ERRORS
-  const int splits = bm.splits(b * w, int(v), int(x->element_size()), int(sms));
   const at::TensorOptions o = s->options();
-  const at::Tensor scratch = at::empty({splits * b * w * (16 + 8 * w)}, o.dtype(at::kByte));
   at::Tensor scores = at::empty({b, w}, o), parents = at::empty({b, w}, o.dtype(at::kLong)), tokens = at::empty({b, w}, o.dtype(at::kLong));
   at::Tensor finished = at::empty({b, w}, o.dtype(at::kBool));
   const int rc = issued([&] {
     return bm.select(x->const_data_ptr(), type, x->stride(0), x->stride(1), s->const_data_ptr(), f ? f->const_data_ptr() : nullptr, int(b), int(w),
-                     int(v), eos, pad, at_(scratch), splits, at_(scores), at_(parents), at_(tokens), at_(finished), stream);
+                     int(v), eos, pad, at_(scores), at_(parents), at_(tokens), at_(finished), int(sms), stream);
   });
   if (rc) return PyLong_FromLong(rc);
   return Py_BuildValue("(NNNN)", wrap(std::move(scores)), wrap(std::move(parents)), wrap(std::move(tokens)), wrap(std::move(finished)));
@@ -192,13 +189,12 @@ PyObject* shared_prefix_attn(PyObject*, PyObject* const* args, Py_ssize_t nargs)
   END_HANDLE_TH_ERRORS
 }
 
-// beam_configure(addresses of kf_beam_splits, kf_beam_select, kf_beam_reorder, kf_shared_prefix_scratch, kf_shared_prefix_attn_bf16, beams and
+// beam_configure(addresses of kf_beam_select, kf_beam_reorder, kf_shared_prefix_scratch, kf_shared_prefix_attn_bf16, beams and
 // states that the kernels take at most)
 PyObject* beam_configure(PyObject*, PyObject* args) {
-  unsigned long long splits = 0, select = 0, reorder = 0, scratch = 0, attention = 0;
+  unsigned long long select = 0, reorder = 0, scratch = 0, attention = 0;
   Beam c;
-  if (!PyArg_ParseTuple(args, "KKKKKii", &splits, &select, &reorder, &scratch, &attention, &c.max_beams, &c.max_states)) return nullptr;
-  c.splits = reinterpret_cast<decltype(c.splits)>(splits);
+  if (!PyArg_ParseTuple(args, "KKKKii", &select, &reorder, &scratch, &attention, &c.max_beams, &c.max_states)) return nullptr;
   c.select = reinterpret_cast<decltype(c.select)>(select);
   c.reorder = reinterpret_cast<decltype(c.reorder)>(reorder);
   c.scratch = reinterpret_cast<decltype(c.scratch)>(scratch);

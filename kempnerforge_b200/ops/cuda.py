@@ -141,8 +141,7 @@ def _declare(L: ctypes.CDLL) -> None:
         "kf_gemm_gather_bf16": [i, vp, vp, vp, i, i, i, i, i, i, vp, i, i, i, vp, vp, vp, vp, vp, vp, i, i, i, i, vp],
         "kf_shared_prefix_scratch": [i] * 7,
         "kf_shared_prefix_attn_bf16": [vp] * 9 + [i] * 7 + [vp, f, i, vp],
-        "kf_beam_splits": [ll, i, i, i],
-        "kf_beam_select": [vp, i, ll, ll, vp, vp, i, i, i, ll, ll, vp, i, vp, vp, vp, vp, vp],
+        "kf_beam_select": [vp, i, ll, ll, vp, vp, i, i, i, ll, ll, vp, vp, vp, vp, i, vp],
         "kf_beam_max_states": [],
         "kf_beam_reorder": [vp, i, i, i, vp, i, i, vp],
         "kf_read_status": [],
@@ -515,7 +514,7 @@ def _load_steps():
         "kf_gemm_fp8_blocks", "kf_add_rmsnorm_fp8_blocks", "kf_fp8_blocks_cast_bf16", "kf_fp8_blocks_values_bf16",
         "kf_norm_grads_f32", "kf_norm_grads_blocks")))
     mod.beam_configure(*(ctypes.cast(getattr(lib(), name), c_void_p).value for name in (
-        "kf_beam_splits", "kf_beam_select", "kf_beam_reorder", "kf_shared_prefix_scratch", "kf_shared_prefix_attn_bf16")),
+        "kf_beam_select", "kf_beam_reorder", "kf_shared_prefix_scratch", "kf_shared_prefix_attn_bf16")),
         BEAMS, lib().kf_beam_max_states())
     _steps = mod
     return mod
@@ -1126,7 +1125,7 @@ _LOGITS = {torch.bfloat16: 0, torch.float32: 1, torch.float16: 2}
 
 def beam_select_call(logits, scores, finished, eos_id: int, pad_id: int):
     """:func:`beam_select`, checked as well; None where Python's checks have to look."""
-    return _step("beam_select", logits, scores, finished, eos_id, pad_id, sm_count(), launches=2)
+    return _step("beam_select", logits, scores, finished, eos_id, pad_id, sm_count())
 
 
 def beam_reorder_call(states: list, parents, length, out: list | None) -> bool:
@@ -1151,13 +1150,10 @@ def beam_select_supported(logits: torch.Tensor) -> bool:
 def beam_select(logits: torch.Tensor, scores: torch.Tensor, finished: torch.Tensor | None, eos_id: int, pad_id: int):
     """(scores, parents, tokens, finished), (B, W) each, of logits (B, W, V) whose last dimension is dense; the others are contiguous."""
     b, w, v = logits.shape
-    L, rows = lib(), b * w
-    splits = L.kf_beam_splits(rows, v, logits.element_size(), sm_count())
-    scratch = torch.empty(splits * rows * (16 + 8 * w), dtype=torch.uint8, device=logits.device)
     out = (torch.empty_like(scores), torch.empty((b, w), dtype=torch.int64, device=logits.device),
            torch.empty((b, w), dtype=torch.int64, device=logits.device), torch.empty((b, w), dtype=torch.bool, device=logits.device))
-    _check(L.kf_beam_select(logits.data_ptr(), _LOGITS[logits.dtype], logits.stride(0), logits.stride(1), scores.data_ptr(), _ptr(finished),
-                            b, w, v, eos_id, pad_id, scratch.data_ptr(), splits, *(t.data_ptr() for t in out), _stream()), "kf_beam_select", 2)
+    _check(lib().kf_beam_select(logits.data_ptr(), _LOGITS[logits.dtype], logits.stride(0), logits.stride(1), scores.data_ptr(), _ptr(finished),
+                                b, w, v, eos_id, pad_id, *(t.data_ptr() for t in out), sm_count(), _stream()), "kf_beam_select")
     return out
 
 

@@ -70,8 +70,8 @@ def test_search_in_bf16(native_lib, dim, heads, kv):
     prompt = torch.randint(0, 500, (3, 100), device="cuda")
     before = native_lib.LAUNCH_COUNT
     tokens, scores = beam_search(model, prompt, 12, 5)
-    # 12 choices of two kernels, 11 reorderings, 11 steps of two layers of two attention kernels, and the models' own
-    assert native_lib.LAUNCH_COUNT - before >= 24 + 11 + 44
+    # 12 choices, 11 reorderings, 11 steps of two layers of two attention kernels, and the models' own
+    assert native_lib.LAUNCH_COUNT - before >= 12 + 11 + 44
     assert tokens.shape == (3, 5, 112) and torch.isfinite(scores).all() and (scores[:, :-1] >= scores[:, 1:]).all()
     assert all(len({tuple(row) for row in t.tolist()}) == 5 for t in tokens)
     # The scores are those of the sequences.  A logit is a sum over `dim` of a normed state, off by some 30 roundings of 2^-8 in all,
