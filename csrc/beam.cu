@@ -4,19 +4,24 @@
 //     s_w + l_w[t] - log sum_t' exp(l_w[t']) .
 // Within a beam the order of candidates is that of its logits, so W tokens of each beam are all that can be among the best.  One cluster
 // of CTAs a prompt; the logits of its beams, one after the other, are dealt out to the CTAs in equal ranges.
-//   * One pass over the logits: a thread keeps the largest of its logits and the sum of exp(x - largest), in fp32 over at most a few hundred
-//     terms and in 64 bits from there on, because candidates of different beams may lie close together.  The difference is taken before the
-//     factor log2 e: rows of the type's lowest value have exponents of zero like any others, and no product overflows.
-//   * The W-th largest of the threads' largest logits is at most the W-th largest logit, so only threads whose largest is not below it
-//     can hold one of the W best: about W of them, whose logits are read again (out of L2).  A list that every warp kept on the way, which
-//     costs an insertion for each of W ln(n / W) logits, took 98 us where this takes 24 (64 x 8 x 128 256 bf16).
+//   * One pass over the logits: a thread keeps the largest of its logits and the sum of exp(x - r), with r the largest of its first round; in
+//     fp32 over at most a few hundred terms and in 64 bits from there on, because candidates of different beams may lie close together.
+//     r moves only when a logit is 27 above it: moved with every new maximum, it cost a branch in most vectors.  The difference is taken
+//     before the factor log2 e: large logits lose nothing, and rows of the type's lowest value have exponents of zero like any others.
+//   * Each of a CTA's 8 warps has ceil(W / 8) threads whose largest logit is at least the warp's ceil(W / 8)-th largest.  So at least W logits
+//     reach the least of these over the warps, a bound that costs a warp-wide maximum or a few.  Taken after each thread's first four
+//     vectors, which lie spread over the range, it leaves about 22 * rounds / 4 vectors of 8 beams that reach it and are noted; taken
+//     again at the end, about 22, which are read once more (out of L2).  A list that every warp kept on the way, with an insertion
+//     for each of W ln(n / W) logits, took 98 us for 64 x 8 x 128 256 in bf16; reading all vectors of the threads that reach the bound 92.
 //   * Candidates are 64-bit keys: the logit's bits in an order-preserving form, then the complement of its index, so that of equal
-//     logits the lowest index is the largest key; sorted by a warp, and joined over the cluster through distributed shared memory.
+//     logits the lowest index is the largest key.  There are few, so a candidate's place is how many are larger, counted; the cluster's
+//     CTAs put theirs into the first one's shared memory.
 // What bounds it: the logits are read once.
 //
 // kf_beam_reorder.  state[b, w] = state[b, parent[b, w]] for all states in one launch.  A thread owns 16 bytes of a column: it reads
 // the column's W values and then writes them, so that parents may be any selection of beams, also in place, without a second buffer.
 #include "common.cuh"
+#include "attention_common.cuh"
 #include "decode_common.cuh"
 
 #include <cuda_fp16.h>
@@ -24,15 +29,16 @@
 namespace kf {
 namespace beam {
 
+using namespace kf::attn;   // two-wide arithmetic
 using decode::mapa_shared;
 
 constexpr int MAX_BEAMS = 32;   // a warp's list is one key per lane
 constexpr int WARPS = 8;
 constexpr int THREADS = WARPS * 32;
-constexpr int MIN_CTAS = 8;     // of a cluster
-constexpr int MAX_PARTS = MAX_BEAMS / MIN_CTAS + 1;   // rows that a CTA's range meets
-constexpr int ROOM = WARPS * MAX_BEAMS;       // candidates that a CTA sorts; more (equal logits) go through lists
-constexpr double LOG2E_D = 1.44269504088896340736;
+constexpr int CTAS = 8;         // of a cluster
+constexpr int MAX_PARTS = MAX_BEAMS / CTAS + 1;       // rows that a CTA's range meets
+constexpr int NOTES = 1024;     // vectors that a CTA notes; more (logits in rising order, equal ones) go through lists
+constexpr int ROOM = 512;             // candidates that a CTA sorts, likewise
 
 typedef unsigned long long Key;
 
@@ -85,90 +91,65 @@ struct TopList {
   }
 };
 
-// One step of a warp's sorting network: lanes `j` apart, the larger one to the lower lane where `down`.
-template <typename K>
-__device__ __forceinline__ K exchange(K k, int j, bool down) {
-  const K other = __shfl_xor_sync(0xffffffffu, k, j);
-  const bool larger = ((threadIdx.x & j) == 0) == down;
-  return (k > other) == larger ? k : other;
+// Logits as floats: 16 bytes of them, and their maximum, which is NaN where one of them is.
+__device__ __forceinline__ float max_or_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
 }
-// A warp's keys, largest first.
-template <typename K>
-__device__ __forceinline__ K sorted(K k) {
-#pragma unroll
-  for (int n = 2; n <= 32; n *= 2)
-#pragma unroll
-    for (int j = n / 2; j > 0; j /= 2) k = exchange(k, j, (threadIdx.x & n & 31) == 0);
-  return k;
-}
-// The 32 largest of two sorted lists.
-__device__ __forceinline__ Key merged(Key a, Key b) {
-  const Key other = __shfl_sync(0xffffffffu, b, 31 - (threadIdx.x & 31));
-  Key k = a > other ? a : other;
-#pragma unroll
-  for (int j = 16; j > 0; j /= 2) k = exchange(k, j, true);
-  return k;
-}
-
-// Logits as floats: 16 bytes of them.  NaN counts as -inf, +inf as the type's largest number.
 template <typename T>
 struct Logits;
 template <>
 struct Logits<float> {
+  static constexpr uint32_t NONE = 0xff800000u;   // -inf in all of a word
   static constexpr int N = 4;
-  static __device__ __forceinline__ float clean(float x) { return min_of(max_of(x, -INFINITY), 3.402823466e38f); }
-  static __device__ __forceinline__ void load(const uint4& v, float (&x)[N]) {
-    x[0] = clean(__uint_as_float(v.x)), x[1] = clean(__uint_as_float(v.y)), x[2] = clean(__uint_as_float(v.z)), x[3] = clean(__uint_as_float(v.w));
+  static __device__ __forceinline__ float one(const float* p) { return *p; }
+  static __device__ __forceinline__ float load(const uint4& v, float (&x)[N]) {
+    x[0] = __uint_as_float(v.x), x[1] = __uint_as_float(v.y), x[2] = __uint_as_float(v.z), x[3] = __uint_as_float(v.w);
+    return max_or_nan(max_or_nan(x[0], x[1]), max_or_nan(x[2], x[3]));
   }
-  static __device__ __forceinline__ float one(const float* p) { return clean(*p); }
 };
 template <>
 struct Logits<__nv_bfloat16> {
+  static constexpr uint32_t NONE = 0xff80ff80u;   // -inf in all of a word
   static constexpr int N = 8;
-  static __device__ __forceinline__ uint32_t clean2(uint32_t u) {
+  static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
     uint32_t r;
-    asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(u), "r"(0xff80ff80u));
-    asm("min.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(r), "r"(0x7f7f7f7fu));
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
     return r;
   }
-  static __device__ __forceinline__ void load(const uint4& v, float (&x)[N]) {
-    const uint32_t u[4] = {clean2(v.x), clean2(v.y), clean2(v.z), clean2(v.w)};
+  static __device__ __forceinline__ float one(const __nv_bfloat16* p) { return __uint_as_float(uint32_t(*reinterpret_cast<const uint16_t*>(p)) << 16); }
+  static __device__ __forceinline__ float load(const uint4& v, float (&x)[N]) {
+    const uint32_t u[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) x[2 * i] = __uint_as_float(u[i] << 16), x[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
-  }
-  static __device__ __forceinline__ float one(const __nv_bfloat16* p) {
-    return __uint_as_float(clean2(uint32_t(*reinterpret_cast<const uint16_t*>(p))) << 16);
+    const uint32_t m = max2(max2(v.x, v.y), max2(v.z, v.w));
+    return max_or_nan(__uint_as_float(m << 16), __uint_as_float(m & 0xffff0000u));
   }
 };
 template <>
 struct Logits<__half> {
+  static constexpr uint32_t NONE = 0xfc00fc00u;   // -inf in all of a word
   static constexpr int N = 8;
-  static __device__ __forceinline__ float clean(float x) { return fminf(fmaxf(x, -INFINITY), 65504.f); }
-  static __device__ __forceinline__ void load(const uint4& v, float (&x)[N]) {
+  static __device__ __forceinline__ float one(const __half* p) { return __half2float(*p); }
+  static __device__ __forceinline__ float load(const uint4& v, float (&x)[N]) {
     const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+    float m = -INFINITY;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u[i]));
-      x[2 * i] = clean(f.x), x[2 * i + 1] = clean(f.y);
+      x[2 * i] = f.x, x[2 * i + 1] = f.y;
+      m = max_or_nan(m, max_or_nan(f.x, f.y));
     }
+    return m;
   }
-  static __device__ __forceinline__ float one(const __half* p) { return clean(__half2float(*p)); }
 };
+// NaN counts as -inf, +inf as the largest number.
+__device__ __forceinline__ float clean(float x) { return min_of(max_of(x, -INFINITY), 3.402823466e38f); }
 
-__device__ __forceinline__ double max_double(double a, double b) { return a > b ? a : b; }
-
-__device__ __forceinline__ unsigned long long ld_cluster_u64(uint32_t addr) {
-  unsigned long long v;
-  asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(addr) : "memory");
-  return v;
+__device__ __forceinline__ void st_cluster_u64(uint32_t addr, unsigned long long v) {
+  asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(addr), "l"(v) : "memory");
 }
-
-// The order of doubles as unsigned integers, and back.
-__device__ __forceinline__ Key ordered(double x) {
-  const Key u = Key(__double_as_longlong(x == 0.0 ? 0.0 : x));
-  return (u >> 63) ? ~u : u | (1ull << 63);
-}
-__device__ __forceinline__ double unordered(Key o) { return __longlong_as_double((o >> 63) ? (long long)(o & ~(1ull << 63)) : (long long)~o); }
 
 template <typename T>
 __global__ void __launch_bounds__(THREADS, 4)
@@ -176,40 +157,49 @@ kf_beam_select(const T* __restrict__ logits, long long stride_b, long long strid
                const uint8_t* __restrict__ finished, int W, int V, long long eos, long long pad, float* __restrict__ out_scores,
                long long* __restrict__ out_parents, long long* __restrict__ out_tokens, uint8_t* __restrict__ out_finished) {
   constexpr int N = Logits<T>::N;
-  constexpr float LOG2E = 1.4426950408889634f;
-  constexpr int UNROLL = 8;
+  constexpr float LOG2E = 1.4426950408889634f, HIGH = 27.f;
+  constexpr int UNROLL = 4;
+  // What a CTA found in its part of a row, in the first CTA's memory.  Part (nth row, CTA) has number nth + CTA: along the vectors every
+  // step raises one of the two.
   struct Part {
-    double m, sum;
+    double r, sum;
     Key keys[MAX_BEAMS];
   };
-  __shared__ Part parts[MAX_PARTS];
-  __shared__ uint32_t tops[WARPS][MAX_BEAMS];      // each warp's threads by their largest logit
-  __shared__ double ms[WARPS], sums[WARPS];
-  __shared__ uint32_t bound;
-  __shared__ int n_readers, n_found;
-  __shared__ uint16_t readers[THREADS];
-  __shared__ Key found[WARPS * MAX_BEAMS];         // ROOM candidates, or the warps' lists
-  __shared__ double total[MAX_BEAMS * MAX_BEAMS];  // [W][W], best first, -inf: none
-  __shared__ uint32_t token[MAX_BEAMS * MAX_BEAMS];
+  __shared__ Part parts[MAX_BEAMS + CTAS];
+  __shared__ float rs[2][WARPS];
+  __shared__ double sums[2][WARPS];
+  __shared__ uint32_t reach[2][WARPS];             // after the first round, at the end
+  __shared__ int n_found[MAX_PARTS], n_notes[MAX_PARTS];
+  __shared__ Key notes[NOTES];                     // (largest logit, vector)
+  __shared__ Key found[ROOM];                      // candidates, or the warps' lists
+  __shared__ int winner[MAX_BEAMS];                // of each place: which candidate
+  double* total = reinterpret_cast<double*>(notes);   // [W][W], best first, -inf: none
+  uint32_t* token = reinterpret_cast<uint32_t*>(found);
+  static_assert(sizeof(notes) >= MAX_BEAMS * MAX_BEAMS * 8 && sizeof(found) >= MAX_BEAMS * MAX_BEAMS * 4, "");
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tid = threadIdx.x;
-  const int ctas = int(cluster_nctaid()), rank = int(cluster_ctarank());
-  const long long b = blockIdx.x / ctas, first = b * W;
+  const int rank = int(cluster_ctarank());
+  const long long b = blockIdx.x / CTAS, first = b * W;
+  if (tid < MAX_PARTS) n_found[tid] = n_notes[tid] = 0;
+  if (tid < MAX_BEAMS) winner[tid] = -1;
   // Beams whose logits count.  One without a score above -inf (or with NaN) has no candidates, a finished one has itself.
-  const bool alive = lane < W && scores[first + lane] > -INFINITY;
+  const float score = lane < W ? scores[first + lane] : -INFINITY;
+  const bool alive = score > -INFINITY;
   const bool done = lane < W && finished != nullptr && finished[first + lane];
   const uint32_t live = __ballot_sync(0xffffffffu, alive && !done);
-  const int per = V / N + 1;                       // vectors of a row, at most
-  const long long all = (long long)__popc(live) * per;
-  const int working = all < ctas ? int(all) : ctas;   // CTAs that have a range, and one that is not empty
-  const long long r0 = rank < working ? all * rank / working : 0, r1 = rank < working ? all * (rank + 1) / working : 0;
+  const uint32_t per = (max(1u, uint32_t(V) / N) + CTAS - 1) / CTAS * CTAS;   // vectors of a row, at most; so that CTAs meet eighths of rows
+  const uint32_t all = uint32_t(__popc(live)) * per;
+  const uint32_t chunk = all / CTAS;
+  const uint32_t r1 = chunk * (rank + 1);
+  cluster_sync_all();   // the first CTA is there to be written to
 
   int part = 0;
-  for (long long pos = r0; pos < r1; ++part) {
-    const int nth = int(pos / per), v0 = int(pos % per);
-    const int v_end = int(r1 - pos < per - v0 ? v0 + (r1 - pos) : per);
+  for (uint32_t pos = chunk * rank; pos < r1; ++part) {
+    const uint32_t nth = pos / per;
+    const int v0 = int(pos - nth * per), v_end = int(min(r1 - pos, per - v0)) + v0;
     pos += v_end - v0;
-    const int w = __fns(live, 0, nth + 1);
+    // the nth live beam
+    const int w = __ffs(__ballot_sync(0xffffffffu, ((live >> lane) & 1u) && __popc(live & ((1u << lane) - 1u)) == int(nth))) - 1;
     const T* x0 = logits + b * stride_b + w * stride_w;
     // vectors from the row's first 16-byte boundary on; what is left at both ends goes with the first vector, a value a thread
     const int misaligned = int(reinterpret_cast<uintptr_t>(x0) & 15) / int(sizeof(T));
@@ -217,215 +207,251 @@ kf_beam_select(const T* __restrict__ logits, long long stride_b, long long strid
     const int vectors = (V - head) / N, tail0 = head + vectors * N;
     const int v1 = min(v_end, vectors);
     const uint4* vec = reinterpret_cast<const uint4*>(x0 + head);
-    auto single = [&](int t) { return v0 != 0 ? -1 : t < head ? t : t >= N && t - N < V - tail0 ? tail0 + t - N : -1; };
-
-    float m = -INFINITY, sum = 0.f;
-    if (tid < 2 * N) {
-      const int i = single(tid);
-      const float x = i >= 0 ? Logits<T>::one(x0 + i) : -INFINITY;
-      if (x > -INFINITY) m = x, sum = 1.f;
-    }
-    for (int base = v0 + tid; base < v1; base += THREADS * UNROLL) {
-      uint4 raw[UNROLL];
+    const int single = v0 != 0 || tid >= 2 * N ? -1 : tid < head ? tid : tid >= N && tid - N < V - tail0 ? tail0 + tid - N : -1;
+    // Four streams of rounds through the range, a vector a thread each; four vectors under way while four are worked on.
+    const int rounds = v1 > v0 ? (v1 - v0 + THREADS - 1) / THREADS : 0, quarter = (rounds + UNROLL - 1) / UNROLL;
+    const int own_rounds = v1 - v0 > tid ? (v1 - v0 - tid + THREADS - 1) / THREADS : 0;
+    const uint4* mine0 = vec + v0 + tid;
+    auto fetch = [&](int round) {   // vectors that are not there hold -inf
+      uint4 v = make_uint4(Logits<T>::NONE, Logits<T>::NONE, Logits<T>::NONE, Logits<T>::NONE);
+      if (round < own_rounds) v = mine0[round * THREADS];
+      return v;
+    };
+    uint4 now[UNROLL], next[UNROLL];
 #pragma unroll
-      for (int u = 0; u < UNROLL; ++u)
-        if (base + u * THREADS < v1) raw[u] = vec[base + u * THREADS];
+    for (int u = 0; u < UNROLL; ++u) now[u] = fetch(quarter > 0 ? u * quarter : own_rounds);
+    const float alone = single >= 0 ? clean(Logits<T>::one(x0 + single)) : -INFINITY;
+
+    // ---- the first round's largest
+    float m = alone;
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+      float x[N];
+      float mx = Logits<T>::load(now[u], x);
+      if (!(mx < INFINITY)) {
+        mx = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < N; ++j) mx = max_of(mx, clean(x[j]));
+      }
+      m = max_of(m, mx);
+    }
+    // what ceil(W / warps) of the warp's threads reach, of `full` warps that have a vector a thread (0: fewer have a logit)
+    const int full = max(1, min(WARPS, (v1 - v0) / 32));
+    auto reached = [&]() {
+      uint32_t left = m > -INFINITY ? ordered(m) : 0u, top = __reduce_max_sync(0xffffffffu, left);
+      for (int i = full; i < W; i += full) {   // the next largest: one thread less each time
+        if (lane == __ffs(__ballot_sync(0xffffffffu, left == top)) - 1) left = 0u;
+        top = __reduce_max_sync(0xffffffffu, left);
+      }
+      return top;
+    };
+    auto least_of = [&](const uint32_t (&of)[WARPS]) {
+      uint32_t least = of[0];
+      for (int i = 1; i < full; ++i) least = min(least, of[i]);
+      return least;
+    };
+    float least_f = -INFINITY;
+    auto bound = [&]() {
+      const uint32_t top = reached();
+      if (lane == 0) reach[0][warp] = top;
+      __syncthreads();
+      const uint32_t least = least_of(reach[0]);
+      if (least) least_f = unordered(least);
+    };
+    bound();
+
+    // ---- the pass: exp(x - r); limit: the logit that is HIGH above r
+    float r = m > -INFINITY ? m : 0.f, limit = m > -INFINITY ? r + HIGH : -INFINITY;
+    float usual = fminf(least_f, limit);   // vectors whose largest is below only add to the sum
+    uint64_t sum2[2] = {pack2(alone > -INFINITY ? exp2_fast((alone - r) * LOG2E) : 0.f, 0.f), 0ull};
+#pragma unroll 1
+    for (int j = 0; j < quarter; ++j) {
+#pragma unroll
+      for (int u = 0; u < UNROLL; ++u) next[u] = fetch(j + 1 < quarter ? u * quarter + j + 1 : own_rounds);
 #pragma unroll
       for (int u = 0; u < UNROLL; ++u) {
-        if (base + u * THREADS >= v1) break;
         float x[N];
-        Logits<T>::load(raw[u], x);
-        float mx = x[0];
+        float mx = Logits<T>::load(now[u], x);
+        if (!(mx < usual)) {
+          if (!(mx < INFINITY)) {
+            mx = -INFINITY;
 #pragma unroll
-        for (int j = 1; j < N; ++j) mx = max_of(mx, x[j]);
-        if (mx > m) {
-          sum = m == -INFINITY ? 0.f : sum * exp2_fast((m - mx) * LOG2E);
-          m = mx;
-        } else {
-          m = max_of(m, mx);   // apart where both are below the smallest normal number, which the compare takes for zeros
+            for (int e = 0; e < N; ++e) mx = max_of(mx, x[e] = clean(x[e]));
+          }
+          if (mx > limit) {
+            const float f = limit == -INFINITY ? 0.f : exp2_fast((r - mx) * LOG2E);
+            sum2[0] = fmul2(sum2[0], pack2(f, f));
+            sum2[1] = fmul2(sum2[1], pack2(f, f));
+            r = mx;
+            limit = r + HIGH;
+          }
+          if (mx >= least_f && mx > -INFINITY) {
+            const int to = atomicAdd(&n_notes[part], 1);
+            if (to < NOTES) notes[to] = make_key(mx, uint32_t(v0 + (u * quarter + j) * THREADS + tid));
+          }
+          usual = fminf(least_f, limit);
         }
-        const float from = m == -INFINITY ? 0.f : m;
-        float s[2] = {0.f, 0.f};
+        m = max_of(m, mx);
+        const uint64_t r2 = pack2(-r, -r), log2e2 = pack2(LOG2E, LOG2E);
 #pragma unroll
-        for (int j = 0; j < N; ++j) s[j & 1] += exp2_fast((x[j] - from) * LOG2E);
-        sum += s[0] + s[1];
+        for (int e = 0; e < N; e += 2) {
+          float a, c;
+          unpack2(fmul2(fadd2(pack2(x[e], x[e + 1]), r2), log2e2), a, c);
+          sum2[(e >> 1) & 1] = fadd2(sum2[(e >> 1) & 1], pack2(exp2_fast(a), exp2_fast(c)));
+        }
       }
+      if (j == quarter / 4 && j > 0) {   // of a quarter of the range
+        __syncthreads();                 // nobody reads the first bound any more
+        bound();
+        usual = fminf(least_f, limit);
+      }
+#pragma unroll
+      for (int u = 0; u < UNROLL; ++u) now[u] = next[u];
     }
 
-    // ---- the sum, and each warp's threads in order
-    double wm = double(m), ws = double(sum);
+    // ---- the warp's sum, and the bound again
+    {
+      float a, c;
+      unpack2(fadd2(sum2[0], sum2[1]), a, c);
+      const float own_r = m > -INFINITY ? r : -INFINITY;
+      float wr = own_r;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) wm = max_double(wm, __shfl_xor_sync(0xffffffffu, wm, o));
-    if (m > -INFINITY) ws *= double(exp2_fast(float(double(m) - wm) * LOG2E));
+      for (int o = 16; o > 0; o >>= 1) wr = max_of(wr, __shfl_xor_sync(0xffffffffu, wr, o));
+      double ws = m > -INFINITY ? double(a + c) * double(exp2_fast((own_r - wr) * LOG2E)) : 0.0;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) ws += __shfl_xor_sync(0xffffffffu, ws, o);
-    if (lane == 0) ms[warp] = wm, sums[warp] = ws;
-    const uint32_t best = m > -INFINITY ? ordered(m) : 0u;   // 0: none
-    const uint32_t in_order = sorted(best);
-    tops[warp][lane] = in_order;
-    if (tid == 0) n_readers = n_found = 0;
-    __syncthreads();
-    // ---- the W-th largest of the threads' largest: that with W - 1 before it (equal ones in the order of the warps)
-    if (lane < W) {
-      int before = lane;
-      for (int x = 0; x < WARPS; ++x) {
-        if (x == warp) continue;
-        // the lists are sorted: how many of the first W come before mine
-        for (int i = 0; i < W; ++i) {
-          const uint32_t other = tops[x][i];
-          if (other < in_order || (other == in_order && x > warp)) break;
-          ++before;
-        }
-      }
-      if (before == W - 1) bound = in_order;
+      for (int o = 16; o > 0; o >>= 1) ws += __shfl_xor_sync(0xffffffffu, ws, o);
+      const uint32_t top = reached();
+      if (lane == 0) rs[part & 1][warp] = wr, sums[part & 1][warp] = ws, reach[1][warp] = top;
     }
     __syncthreads();
-    if (best != 0u && best >= bound) readers[atomicAdd(&n_readers, 1)] = uint16_t(tid);
-    __syncthreads();
-    // ---- the logits of these threads again
-    const int n = n_readers;
-    const uint32_t least = bound;
-    for (int i = warp; i < n; i += WARPS) {
-      const int t = readers[i];
-      for (int base = v0 + t; base < v1; base += THREADS * 32) {
-        const int at = base + lane * THREADS;
-        if (at < v1) {
-          float x[N];
-          Logits<T>::load(vec[at], x);
-#pragma unroll
-          for (int j = 0; j < N; ++j)
-            if (x[j] > -INFINITY && ordered(x[j]) >= least) {
-              const int to = atomicAdd(&n_found, 1);
-              if (to < ROOM) found[to] = make_key(x[j], uint32_t(head + at * N + j));
-            }
-        }
+    const uint32_t least = least_of(reach[1]);
+    // ---- the vectors that reach it once more
+    auto take = [&](float x, int i) {
+      if (x > -INFINITY && ordered(x) >= least) {
+        const int to = atomicAdd(&n_found[part], 1);
+        if (to < ROOM) found[to] = make_key(x, uint32_t(i));
       }
-      if (lane == 0 && t < 2 * N && single(t) >= 0) {
-        const float x = Logits<T>::one(x0 + single(t));
-        if (x > -INFINITY && ordered(x) >= least) {
-          const int to = atomicAdd(&n_found, 1);
-          if (to < ROOM) found[to] = make_key(x, uint32_t(single(t)));
-        }
-      }
-    }
-    __syncthreads();
-    const int candidates = n_found;
-    Key mine = 0;
-    if (candidates <= ROOM) {
-      if (warp == 0)
-        for (int i = 0; i < candidates; i += 32) {
-          const Key k = sorted(i + lane < candidates ? found[i + lane] : 0);
-          mine = i ? merged(mine, k) : k;
-        }
-    } else {
-      // so many equal logits that there is no room: every warp through the whole of its vectors
-      TopList top;
-      for (int base = v0 + warp * 32; base < v1; base += THREADS) {
-        const int at = base + lane;
+    };
+    const int noted = n_notes[part];
+    take(alone, single);
+    for (int e = tid; e < min(noted, NOTES); e += THREADS) {
+      const Key n = notes[e];
+      if (uint32_t(n >> 32) >= least) {
+        const int at = head + int(key_index(n)) * N;
         float x[N];
-        if (at < v1) Logits<T>::load(vec[at], x);
+        Logits<T>::load(*reinterpret_cast<const uint4*>(x0 + at), x);
 #pragma unroll
-        for (int j = 0; j < N; ++j)
-          top.offer(at < v1 && x[j] > -INFINITY && ordered(x[j]) >= least ? make_key(x[j], uint32_t(head + at * N + j)) : 0, W);
+        for (int j = 0; j < N; ++j) take(clean(x[j]), at + j);
       }
-      if (warp == 0) {
-        const int i = lane < 2 * N ? single(lane) : -1;
-        const float x = i >= 0 ? Logits<T>::one(x0 + i) : -INFINITY;
-        top.offer(x > -INFINITY ? make_key(x, uint32_t(i)) : 0, W);
+    }
+    __syncthreads();
+    // ---- the W largest and the sum, into the first CTA
+    const uint32_t to = mapa_shared(smem_u32(&parts[nth + rank]), 0);
+    const int candidates = n_found[part];
+    if (candidates <= ROOM && noted <= NOTES) {
+      if (tid < W && tid >= candidates) st_cluster_u64(to + 16 + 8 * tid, 0ull);
+      for (int e = tid; e < candidates; e += THREADS) {
+        const Key mine = found[e];
+        int larger = 0;
+        for (int i = 0; i < candidates; ++i) larger += found[i] > mine;
+        if (larger < W) st_cluster_u64(to + 16 + 8 * larger, mine);
       }
-      found[warp * MAX_BEAMS + lane] = top.mine;
+    } else {
+      // rising or equal logits: every warp through the whole of its vectors
+      TopList list;
+      for (int base = v0 + warp * 32; base < v1; base += THREADS) {
+        const int i = base + lane;
+        float x[N], mx = -INFINITY;
+        if (i < v1) Logits<T>::load(vec[i], x);
+#pragma unroll
+        for (int j = 0; j < N; ++j) mx = max_of(mx, x[j] = i < v1 ? clean(x[j]) : -INFINITY);
+        if (!__any_sync(0xffffffffu, mx > -INFINITY && ordered(mx) >= max(least, uint32_t(list.worst >> 32)))) continue;
+#pragma unroll 1
+        for (int j = 0; j < N; ++j) list.offer(x[j] > -INFINITY ? make_key(x[j], uint32_t(head + i * N + j)) : 0, W);
+      }
+      if (warp == 0) list.offer(alone > -INFINITY ? make_key(alone, uint32_t(single)) : 0, W);
+      found[warp * MAX_BEAMS + lane] = list.mine;
       __syncthreads();
-      if (warp == 0)
-        for (int i = 0; i < WARPS; ++i) mine = i ? merged(mine, found[i * MAX_BEAMS + lane]) : found[lane];
+      if (warp == 0) {
+        for (int i = 1; i < WARPS; ++i) list.offer(found[i * MAX_BEAMS + lane], W);
+        if (lane < W) st_cluster_u64(to + 16 + 8 * lane, list.mine);
+      }
     }
     if (warp == 0) {
-      parts[part].keys[lane] = mine;
-      double pm = lane < WARPS ? ms[lane] : -INFINITY;
-      const double own = pm;
+      const float own = lane < WARPS ? rs[part & 1][lane] : -INFINITY;
+      float pr = own;
 #pragma unroll
-      for (int o = WARPS / 2; o > 0; o >>= 1) pm = max_double(pm, __shfl_xor_sync(0xffffffffu, pm, o));
-      double ps = lane < WARPS && own > -INFINITY ? sums[lane] * exp2((own - pm) * LOG2E_D) : 0.0;
+      for (int o = WARPS / 2; o > 0; o >>= 1) pr = max_of(pr, __shfl_xor_sync(0xffffffffu, pr, o));
+      double ps = own > -INFINITY ? sums[part & 1][lane] * double(exp2_fast((own - pr) * LOG2E)) : 0.0;
 #pragma unroll
       for (int o = WARPS / 2; o > 0; o >>= 1) ps += __shfl_xor_sync(0xffffffffu, ps, o);
-      if (lane == 0) parts[part].m = pm, parts[part].sum = ps;
+      if (lane == 0) {
+        st_cluster_u64(to, (unsigned long long)__double_as_longlong(double(pr)));
+        st_cluster_u64(to + 8, (unsigned long long)__double_as_longlong(ps));
+      }
     }
-    __syncthreads();
   }
 
   cluster_sync_all();
   // ---- the first CTA joins what the cluster found, a warp a beam
+  if (rank != 0) return;
   const double NONE = -INFINITY;
-  if (rank == 0) {
-    for (int w = warp; w < W; w += WARPS) {
-      const bool w_alive = scores[first + w] > -INFINITY;
-      if ((live >> w) & 1u) {
-        const int nth = __popc(live & ((1u << w) - 1u));
-        const long long u0 = (long long)nth * per, u1 = u0 + per - 1;
-        const int c0 = int(((u0 + 1) * working - 1) / all), c1 = int(((u1 + 1) * working - 1) / all);   // CTAs that hold its first and last vector
-        auto part_of = [&](int c) {
-          const long long begin = all * c / working;
-          return mapa_shared(smem_u32(&parts[nth - int(begin / per)]), uint32_t(c));
-        };
-        double m = NONE, sum = 0.0, own_m = NONE, own_sum = 0.0;
-        if (lane <= c1 - c0) {
-          const uint32_t at = part_of(c0 + lane);
-          own_m = __longlong_as_double((long long)ld_cluster_u64(at));
-          own_sum = __longlong_as_double((long long)ld_cluster_u64(at + 8));
-        }
-        m = own_m;
+  for (int w = warp; w < W; w += WARPS) {
+    const double own_score = double(__shfl_sync(0xffffffffu, score, w));
+    if (lane < W) total[w * W + lane] = NONE;
+    __syncwarp();
+    if ((live >> w) & 1u) {
+      const uint32_t nth = uint32_t(__popc(live & ((1u << w) - 1u)));
+      const int c0 = int(nth * per / chunk), count = int((nth * per + per - 1) / chunk) - c0 + 1;   // CTAs that hold its vectors
+      const Part* p = parts + nth + c0;
+      const double own_r = lane < count ? p[lane].r : NONE;
+      double r = own_r;
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) m = max_double(m, __shfl_xor_sync(0xffffffffu, m, o));
-        sum = own_m > NONE ? own_sum * exp2((own_m - m) * LOG2E_D) : 0.0;
+      for (int o = CTAS / 2; o > 0; o >>= 1) r = fmax(r, __shfl_xor_sync(0xffffffffu, r, o));
+      double sum = own_r > NONE ? p[lane].sum * double(exp2_fast(float(own_r - r) * LOG2E)) : 0.0;
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        const double lse = m + log(sum);
-        Key mine = 0;
-        const int count = (c1 - c0 + 1) * W;
-        for (int i = 0; i < count; i += 32) {
-          Key k = 0;
-          if (i + lane < count) k = ld_cluster_u64(part_of(c0 + (i + lane) / W) + 16 + 8 * ((i + lane) % W));
-          k = sorted(k);
-          mine = i ? merged(mine, k) : k;
+      for (int o = CTAS / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      const double lse = __shfl_sync(0xffffffffu, r + log(sum), 0);
+      for (int i = lane; i < count * W; i += 32) {
+        const Key mine = p[i / W].keys[i % W];
+        int larger = 0;
+        for (int c = 0; c < count; ++c)
+          for (int j = 0; j < W; ++j) larger += p[c].keys[j] > mine;
+        if (mine && larger < W) {
+          total[w * W + larger] = own_score + (double(key_value(mine)) - lse);
+          token[w * W + larger] = key_index(mine);
         }
-        if (lane < W) {
-          total[w * W + lane] = mine ? double(scores[first + w]) + (double(key_value(mine)) - lse) : NONE;
-          token[w * W + lane] = key_index(mine);
-        }
-      } else if (lane < W) {
-        total[w * W + lane] = lane == 0 && w_alive ? double(scores[first + w]) : NONE;   // finished, or nothing
       }
+    } else if (lane == 0 && own_score > NONE) {
+      total[w * W] = own_score;   // finished
     }
   }
   __syncthreads();
-  if (rank == 0 && warp == 0) {
-    // lane = beam; its best candidate that is not taken yet.  The score in two halves: the larger, of equal ones the lower beam.
-    int at = 0, parent = lane, place = -1;
-    const Key none = ordered(NONE);
-    Key mine = lane < W ? ordered(total[lane * W]) : none, score = none;
-    for (int r = 0; r < W; ++r) {
-      const uint32_t hi = __reduce_max_sync(0xffffffffu, uint32_t(mine >> 32));
-      const uint32_t lo = __reduce_max_sync(0xffffffffu, uint32_t(mine >> 32) == hi ? uint32_t(mine) : 0u);
-      const Key best = (Key(hi) << 32) | lo;
-      if (best <= none) break;
-      const int who = __ffs(__ballot_sync(0xffffffffu, mine == best)) - 1;
-      const int taken = __shfl_sync(0xffffffffu, at, who);
-      if (lane == r) score = best, parent = who, place = taken;
-      if (lane == who) {
-        ++at;
-        mine = at < W ? ordered(total[lane * W + at]) : none;
+  // a candidate's place: how many come before it, its own beam's better ones, others' better ones, lower beams' equal ones
+  for (int i = tid; i < W * W; i += THREADS) {
+    const double mine = total[i];
+    const int w = i / W;
+    int before = mine > NONE ? i - w * W : W;
+    for (int x = 0; x < W && before < W; ++x) {
+      if (x == w) continue;
+      for (int j = x * W; j < x * W + W; ++j) {
+        if (!(total[j] > mine || (total[j] == mine && x < w))) break;
+        if (++before == W) break;
       }
     }
-    const uint32_t ends = __ballot_sync(0xffffffffu, done);
-    if (lane < W) {
-      const bool ended = place >= 0 && ((ends >> parent) & 1u);
-      const long long t = place < 0 || ended ? pad : (long long)token[parent * W + place];
-      out_scores[first + lane] = float(unordered(score));
-      out_parents[first + lane] = parent;
-      out_tokens[first + lane] = t;
-      out_finished[first + lane] = ended || (place >= 0 && t == eos);
-    }
+    if (before < W) winner[before] = i;
   }
-  cluster_sync_all();   // no CTA leaves while the first reads its shared memory
+  __syncthreads();
+  const uint32_t ends = __ballot_sync(0xffffffffu, done);
+  if (tid < W) {
+    const int i = winner[tid], parent = i < 0 ? tid : i / W;
+    const bool ended = i >= 0 && ((ends >> parent) & 1u);
+    const long long t = i < 0 || ended ? pad : (long long)token[i];
+    out_scores[first + tid] = i < 0 ? -INFINITY : float(total[i]);
+    out_parents[first + tid] = parent;
+    out_tokens[first + tid] = t;
+    out_finished[first + tid] = ended || (i >= 0 && t == eos);
+  }
 }
 
 template <typename T>
@@ -434,7 +460,7 @@ static int launch_select(const void* logits, long long stride_b, long long strid
                          int num_sms, cudaStream_t stream) {
   auto kern = kf_beam_select<T>;
   cudaLaunchConfig_t cfg = {};
-  const int ctas = MIN_CTAS;
+  const int ctas = CTAS;
   if ((long long)B * ctas > 0x7fffffffLL) return 6;
   cfg.gridDim = dim3((unsigned)(B * ctas));
   cfg.blockDim = dim3(THREADS);
@@ -537,7 +563,7 @@ int kf_beam_select(const void* logits, int type, long long stride_b, long long s
                    int V, long long eos, long long pad, void* out_scores, void* out_parents, void* out_tokens, void* out_finished, int num_sms,
                    void* stream) {
   using namespace kf::beam;
-  if (B < 1 || W < 1 || W > MAX_BEAMS || V < 1) return 3;
+  if (B < 1 || W < 1 || W > MAX_BEAMS || V < 1 || V > 1 << 28) return 3;   // vectors of 32 rows are counted in 32 bits
   auto go = [&](auto launch) {
     return launch(logits, stride_b, stride_w, (const float*)scores, (const uint8_t*)finished, B, W, V, eos, pad, (float*)out_scores,
                   (long long*)out_parents, (long long*)out_tokens, (uint8_t*)out_finished, num_sms, (cudaStream_t)stream);

@@ -44,7 +44,7 @@ PyObject* beam_select(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   const int64_t b = x->size(0), w = x->size(1), v = x->size(2);
   const at::ScalarType t = x->scalar_type();
   const int type = t == at::kBFloat16 ? 0 : t == at::kFloat ? 1 : t == at::kHalf ? 2 : -1;
-  if (type < 0 || b < 1 || w < 1 || v < 1 || w > bm.max_beams || v > kLargest || b * w >= 1 << 27 || (x->stride(2) != 1 && v > 1) ||
+  if (type < 0 || b < 1 || w < 1 || v < 1 || w > bm.max_beams || v > 1 << 28 || b * w >= 1 << 27 || (x->stride(2) != 1 && v > 1) ||
       s->scalar_type() != at::kFloat || s->size(0) != b || s->size(1) != w || !s->is_contiguous() ||
       (f && (f->scalar_type() != at::kBool || f->sizes() != s->sizes() || !f->is_contiguous())))
     Py_RETURN_NONE;

@@ -50,7 +50,7 @@ def select(logits: torch.Tensor, scores: torch.Tensor, finished: torch.Tensor | 
     """The W best continuations of each prompt's W beams: logits (B, W, V), scores (B, W) fp32, finished (B, W) bool.
 
     A beam's candidates are its tokens, with its score plus the token's log-probability, computed in 64 bits and rounded to 32; logits of
-    -inf or NaN are no candidates, +inf counts as the largest number of the logits' type.  A finished beam has one candidate: itself, with
+    -inf or NaN are no candidates, +inf counts as the largest fp32 number.  A finished beam has one candidate: itself, with
     ``pad_id`` and its score; a beam whose score is -inf or NaN has none (a search starts with the scores 0, -inf, -inf, ..).  Best first;
     ties go to the lower beam, then to the lower token.  A beam that takes ``eos_id`` is finished.  Where there are fewer than W candidates
     the places left have the score -inf, their own beam as parent and ``pad_id``.

@@ -1143,7 +1143,7 @@ def beam_reorder_call(states: list, parents, length, out: list | None) -> bool:
 
 
 def beam_select_supported(logits: torch.Tensor) -> bool:
-    return (logits.dtype in _LOGITS and logits.shape[1] <= BEAMS and logits.stride(2) == 1 and logits.shape[2] < 2**31 - 2**16
+    return (logits.dtype in _LOGITS and logits.shape[1] <= BEAMS and logits.stride(2) == 1 and logits.shape[2] <= 2**28
             and logits.shape[0] * logits.shape[1] < 2**27)
 
 

@@ -156,10 +156,10 @@ def shared_prefix_attention(
 # --------------------------------------------------------------------------- beam search
 def beam_select(logits: torch.Tensor, scores: torch.Tensor, finished: torch.Tensor | None, eos_id: int, pad_id: int):
     """(scores, parents, tokens, finished), each (B, W): the W best of a prompt's candidates, in 64 bits.  A beam's candidates are ordered
-    by logit, then by token; all by score, then by beam.  NaN logits count as -inf, +inf as the type's largest number."""
+    by logit, then by token; all by score, then by beam.  NaN logits count as -inf, +inf as the largest fp32 number."""
     b, w, vocab = logits.shape
     x = logits.double()
-    x = torch.where(x > float("-inf"), x.clamp_max(torch.finfo(logits.dtype).max), float("-inf"))
+    x = torch.where(x > float("-inf"), x.clamp_max(torch.finfo(torch.float32).max), float("-inf"))
     top = x.amax(-1, keepdim=True)
     shifted = torch.where(x > float("-inf"), x - top, float("-inf"))
     lse = top + shifted.exp().sum(-1, keepdim=True).log()

@@ -13,7 +13,7 @@ NONE = float("-inf")
 def by_hand(logits, scores, finished, eos, pad):
     """Candidate by candidate in Python floats."""
     b, w, vocab = logits.shape
-    largest = torch.finfo(logits.dtype).max
+    largest = torch.finfo(torch.float32).max
     rows = []
     for i in range(b):
         found = []
