@@ -3,10 +3,11 @@
 // What a continuation has written itself is its own, so these keys are read by its group of query heads only: a stream as in the generation
 // step of single sequences.  In a beam search the cache of a continuation does not move when beams are exchanged; own_rows says in whose
 // cache each position lies.  Beams share most of their ancestors, so most of these keys come out of L2 for all beams but the first.
-//   * one cluster per (continuation, key head): the group's query heads are the 16 rows of an m16n8k16 MMA, the keys are split over the
-//     cluster's CTAs (up to 8) and over the four warps of each;
-//   * tiles of 64 keys move through a three-stage cp.async ring, 16-byte chunks XOR-swizzled, so that ldmatrix is free of bank conflicts;
-//   * the partial (max, sum, output) triples of the warps, the CTAs and the prompt's partial results are joined in a fixed order.
+//   * a unit is a continuation's key head; its query heads are the 16 rows of an m16n8k16 MMA, its keys are dealt out to 1 to 32 warps, as
+//     many as it takes to have eight warps on every SM: few units need all of them for one, many (a batch of short continuations) one each;
+//   * every warp streams tiles of 16 keys through a cp.async ring of its own, two tiles ahead, without a barrier; 16-byte chunks are
+//     XOR-swizzled, so that ldmatrix is free of bank conflicts;
+//   * the (max, sum, output) triples of the warps, of the CTAs of a cluster and of the prompt are joined in a fixed order.
 // All of it up to that last step runs without the prompt's kernel, and starts on the SMs that it leaves (programmatic launch).
 #include "decode_common.cuh"
 #include "shared_prefix.cuh"
@@ -16,21 +17,20 @@ namespace shared_prefix {
 
 using namespace kf::decode;
 
-constexpr int OWN_THREADS = 128;
-constexpr int OWN_TILE = 64;     // keys per ring stage, 16 per warp
-constexpr int OWN_STAGES = 3;
-constexpr int OWN_ROWS = 16;     // query heads per cluster (MMA rows)
+constexpr int OWN_WARPS = 4, OWN_THREADS = OWN_WARPS * 32;
+constexpr int OWN_TILE = 16;       // keys per ring stage of a warp
+constexpr int OWN_ROWS = 16;       // query heads per unit (MMA rows)
+constexpr int OWN_RING = 24 << 10; // bytes of a warp's ring: two CTAs an SM, 128 KB of it under way
 
 template <int HD>
 struct OwnCfg {
   static constexpr int TILE_BYTES = OWN_TILE * HD * 2;
-  static constexpr int RING = OWN_STAGES * 2 * TILE_BYTES;
-  static constexpr int PART = 4 * OWN_ROWS * HD * 4;                 // per-warp partial outputs, alias the ring
-  static constexpr int BODY = RING > PART ? RING : PART;
-  static constexpr int MERGED = OWN_ROWS * HD * 4;                   // the CTA's merged partial
-  static constexpr int STATS = (4 + 1) * OWN_ROWS * 2 * 4;           // (max, sum) per warp and merged
-  static constexpr int SEEN = OWN_STAGES * OWN_TILE;                 // per ring row: holds a visible key
-  static constexpr size_t SMEM = size_t(BODY) + MERGED + STATS + SEEN;
+  static constexpr int STAGES = OWN_RING / (2 * TILE_BYTES);         // 3 for a head dim of 128, 6 for 64
+  static constexpr int PART = OWN_ROWS * HD * 4;                     // a warp's partial output, over its ring
+  static_assert(PART <= OWN_RING, "");
+  static constexpr int STATS = OWN_WARPS * OWN_ROWS * 2 * 4;         // (max, sum) per warp and row
+  static constexpr int SEEN = OWN_WARPS * 8 * 4;                     // per stage: which of its keys are visible
+  static constexpr size_t SMEM = size_t(OWN_WARPS) * OWN_RING + STATS + SEEN;
 };
 
 struct Own {
@@ -43,55 +43,66 @@ struct Own {
   float scale_log2;
 };
 
-template <int HD>
+// WPU: warps of a CTA that share a unit.  Clusters of more than one CTA (WPU = 4) share one too.
+template <int HD, int WPU>
 __global__ void __launch_bounds__(OWN_THREADS)
-kf_shared_prefix_own(const Own a, const Layout lay, const float* part_o, const float2* part_ml) {
+kf_shared_prefix_own(const Own a, const Layout lay, const float* part_o, const float2* part_ml, const long long units) {
   using C = OwnCfg<HD>;
   extern __shared__ __align__(128) uint8_t smem_raw[];
-  const uint32_t ring = smem_u32(smem_raw);
-  float* part = reinterpret_cast<float*>(smem_raw);
-  float* merged = reinterpret_cast<float*>(smem_raw + C::BODY);
-  float* stats = reinterpret_cast<float*>(smem_raw + C::BODY + C::MERGED);  // [5][ROWS][2]
-  uint8_t* seen = smem_raw + C::BODY + C::MERGED + C::STATS;
-
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int splits = int(cluster_nctaid()), rank = int(cluster_ctarank());
+  const int splits = WPU == OWN_WARPS ? int(cluster_nctaid()) : 1, rank = WPU == OWN_WARPS ? int(cluster_ctarank()) : 0;
+  const int way = rank * WPU + warp % WPU, ways = splits * WPU;     // which share of the unit's keys
+  const uint32_t ring = smem_u32(smem_raw) + warp * OWN_RING;
+  float* stats = reinterpret_cast<float*>(smem_raw + OWN_WARPS * OWN_RING);                            // [warp][row][2]
+  volatile uint32_t* seen = reinterpret_cast<uint32_t*>(smem_raw + OWN_WARPS * OWN_RING + C::STATS) + warp * 8;
+
+  const long long unit0 = blockIdx.x / splits * (OWN_WARPS / WPU) + warp / WPU;
+  const bool there = unit0 < units;
+  long long unit = there ? unit0 : 0;
+  const int w = int(unit % lay.W);   // continuations of a prompt side by side: their common keys are in L2, some in L1
+  unit /= lay.W;
   const int blocks_per_kv = (a.group + OWN_ROWS - 1) / OWN_ROWS;
-  long long unit = blockIdx.x / splits;
   const int hb = int(unit % blocks_per_kv);
   unit /= blocks_per_kv;
-  const int hk = int(unit % a.Hkv);
-  unit /= a.Hkv;
-  const int w = int(unit % lay.W), b = int(unit / lay.W);
-  const int n_heads = min(OWN_ROWS, a.group - hb * OWN_ROWS);     // query heads of this cluster
+  const int hk = int(unit % a.Hkv), b = int(unit / a.Hkv);
+  const int n_heads = there ? min(OWN_ROWS, a.group - hb * OWN_ROWS) : 0;     // query heads of this unit
   const int h0 = hk * a.group + hb * OWN_ROWS;
 
-  const int n_tiles = (a.S + OWN_TILE - 1) / OWN_TILE;
-  const int t0 = int((long long)n_tiles * rank / splits), t1 = int((long long)n_tiles * (rank + 1) / splits);
+  const int n_tiles = there ? (a.S + OWN_TILE - 1) / OWN_TILE : 0;
+  const int t0 = int((long long)n_tiles * way / ways), t1 = int((long long)n_tiles * (way + 1) / ways);
   const __nv_bfloat16* kb = a.k + b * a.k_b + hk * a.k_h;
   const __nv_bfloat16* vb = a.v + b * a.v_b + hk * a.v_h;
   const uint8_t* table = a.rows ? a.rows + b * a.r_b + w * a.r_w : nullptr;
 
   constexpr int CHUNKS = HD / 8;                        // 16-byte chunks per row
-  auto issue = [&](int t) {
-    const int st = (t - t0) % OWN_STAGES;
+  // whose cache holds the lane's key of tile t (lay.W: nobody's)
+  auto slot_of = [&](int t) {
+    const int pos = t * OWN_TILE + (lane & 15);
+    return t >= t1 || pos >= a.S ? lay.W : table ? int(table[pos]) : w;
+  };
+  auto issue = [&](int t, int slot) {
+    const int st = (t - t0) % C::STAGES;
     const uint32_t ks = ring + uint32_t(st) * 2u * C::TILE_BYTES, vs = ks + C::TILE_BYTES;
+    const uint32_t mask = __ballot_sync(0xffffffffu, slot < lay.W);
+    if (lane == 0) seen[st] = mask;
 #pragma unroll
-    for (int i = 0; i < OWN_TILE * CHUNKS / OWN_THREADS; ++i) {
-      const int idx = threadIdx.x + i * OWN_THREADS, r = idx / CHUNKS, c = idx % CHUNKS;
-      const int pos = t * OWN_TILE + r;
-      const int slot = pos >= a.S ? lay.W : table ? int(table[pos]) : w;
-      const bool in = slot < lay.W;
-      const long long ko = in ? slot * a.k_w + pos * a.k_s + c * 8 : 0, vo = in ? slot * a.v_w + pos * a.v_s + c * 8 : 0;
+    for (int i = 0; i < OWN_TILE * CHUNKS / 32; ++i) {
+      const int idx = lane + i * 32, r = idx / CHUNKS, c = idx % CHUNKS;
+      const int sl = __shfl_sync(0xffffffffu, slot, r);
+      const bool in = (mask >> r) & 1u;
+      const long long pos = t * OWN_TILE + r;
+      const long long ko = in ? sl * a.k_w + pos * a.k_s + c * 8 : 0, vo = in ? sl * a.v_w + pos * a.v_s + c * 8 : 0;
       const uint32_t dst = uint32_t(r * HD * 2 + ((c ^ (r & 7)) << 4));
       cp_async16(ks + dst, kb + ko, in);
       cp_async16(vs + dst, vb + vo, in);
-      if (c == 0) seen[st * OWN_TILE + r] = in;
     }
   };
-  for (int t = t0; t < t0 + OWN_STAGES - 1; ++t) {
-    if (t < t1) issue(t);
+  int slot = slot_of(t0);
+  for (int t = t0; t < t0 + C::STAGES - 1; ++t) {
+    const int after = slot_of(t + 1);
+    if (t < t1) issue(t, slot);
     cp_commit();
+    slot = after;
   }
 
   // query rows as MMA A fragments (rows past the group are zero)
@@ -114,18 +125,18 @@ kf_shared_prefix_own(const Own a, const Layout lay, const float* part_o, const f
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 
   for (int t = t0; t < t1; ++t) {
-    cp_wait<OWN_STAGES - 2>();
-    __syncthreads();  // tile t has landed for every thread, and the stage refilled below has been consumed
-    if (t + OWN_STAGES - 1 < t1) issue(t + OWN_STAGES - 1);
+    cp_wait<C::STAGES - 2>();
+    __syncwarp();   // tile t has landed for every lane, and the stage refilled below has been consumed
+    const int after = slot_of(t + C::STAGES);
+    if (t + C::STAGES - 1 < t1) issue(t + C::STAGES - 1, slot);
     cp_commit();
-    if (t * OWN_TILE + warp * 16 >= a.S) continue;
-    const int st = (t - t0) % OWN_STAGES;
+    slot = after;
+    const int st = (t - t0) % C::STAGES;
     const uint32_t ks = ring + uint32_t(st) * 2u * C::TILE_BYTES, vs = ks + C::TILE_BYTES;
     const int mi = lane >> 3, lr = lane & 7;
     float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
     {
-      const int r = warp * 16 + lr + (mi >> 1) * 8;
-      const uint32_t row = ks + uint32_t(r * HD * 2);
+      const uint32_t row = ks + uint32_t((lr + (mi >> 1) * 8) * HD * 2);
 #pragma unroll
       for (int kk = 0; kk < HD / 16; ++kk) {
         uint32_t f[4];
@@ -134,11 +145,11 @@ kf_shared_prefix_own(const Own a, const Layout lay, const float* part_o, const f
         mma16816(s[1], qa[kk], f[2], f[3]);
       }
     }
-    const uint8_t* sees = seen + st * OWN_TILE + warp * 16 + (lane & 3) * 2;
+    const uint32_t sees = seen[st] >> ((lane & 3) * 2);
 #pragma unroll
     for (int n = 0; n < 2; ++n)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s[n][e] = sees[n * 8 + (e & 1)] ? s[n][e] * a.scale_log2 : -INFINITY;
+      for (int e = 0; e < 4; ++e) s[n][e] = (sees >> (n * 8 + (e & 1))) & 1u ? s[n][e] * a.scale_log2 : -INFINITY;
     uint32_t pa[4];
 #pragma unroll
     for (int hf = 0; hf < 2; ++hf) {
@@ -167,8 +178,7 @@ kf_shared_prefix_own(const Own a, const Layout lay, const float* part_o, const f
       }
     }
     {
-      const int r = warp * 16 + lr + (mi & 1) * 8;
-      const uint32_t row = vs + uint32_t(r * HD * 2);
+      const uint32_t row = vs + uint32_t((lr + (mi & 1) * 8) * HD * 2);
 #pragma unroll
       for (int d = 0; d < HD / 16; ++d) {
         uint32_t f[4];
@@ -179,79 +189,66 @@ kf_shared_prefix_own(const Own a, const Layout lay, const float* part_o, const f
     }
   }
   cp_wait<0>();
-  __syncthreads();  // the ring is idle: it becomes the partial buffer
-
-  // ---- the warps of this CTA
+  __syncwarp();  // the ring is idle: the warp's partial result takes its place
+  float* part = reinterpret_cast<float*>(smem_raw + warp * OWN_RING);
 #pragma unroll
   for (int hf = 0; hf < 2; ++hf) {
     l[hf] += __shfl_xor_sync(0xffffffffu, l[hf], 1);
     l[hf] += __shfl_xor_sync(0xffffffffu, l[hf], 2);
     const int r = (lane >> 2) + hf * 8;
-    if ((lane & 3) == 0) {
-      stats[(warp * OWN_ROWS + r) * 2] = m[hf];
-      stats[(warp * OWN_ROWS + r) * 2 + 1] = l[hf];
-    }
     if (r < n_heads) {
-      float* dst = part + (warp * OWN_ROWS + r) * HD + (lane & 3) * 2;
+      if ((lane & 3) == 0) {
+        stats[(warp * OWN_ROWS + r) * 2] = m[hf];
+        stats[(warp * OWN_ROWS + r) * 2 + 1] = l[hf];
+      }
+      float* dst = part + r * HD + (lane & 3) * 2;
 #pragma unroll
       for (int i = 0; i < HD / 8; ++i) *reinterpret_cast<float2*>(dst + i * 8) = make_float2(o[i][2 * hf], o[i][2 * hf + 1]);
     }
   }
-  __syncthreads();
-  for (int i = threadIdx.x; i < n_heads * (HD / 4); i += OWN_THREADS) {
-    const int r = i / (HD / 4), d = (i % (HD / 4)) * 4;
-    float top = -INFINITY;
-#pragma unroll
-    for (int x = 0; x < 4; ++x) top = fmaxf(top, stats[(x * OWN_ROWS + r) * 2]);
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    float sum = 0.f;
-#pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      const float f = weight(stats[(x * OWN_ROWS + r) * 2], top);
-      const float4 v = *reinterpret_cast<const float4*>(part + (x * OWN_ROWS + r) * HD + d);
-      acc.x += f * v.x; acc.y += f * v.y; acc.z += f * v.z; acc.w += f * v.w;
-      sum += f * stats[(x * OWN_ROWS + r) * 2 + 1];
-    }
-    *reinterpret_cast<float4*>(merged + r * HD + d) = acc;
-    if (d == 0) {
-      stats[(4 * OWN_ROWS + r) * 2] = top;
-      stats[(4 * OWN_ROWS + r) * 2 + 1] = sum;
-    }
-  }
   // ---- the prompt's partial results: which there are
-  long long before = 0, total = 0;
-  if (part_o != nullptr) {
-    before = tiles_before(lay, b);
-    total = tiles_before(lay, lay.B);
-  }
-  cluster_sync_all();
-  grid_dep_wait();
+  int c0 = 0, parts = 0;
   const int u = hk * lay.row_tiles + w / lay.wt;
-  const int nt = part_o != nullptr ? tiles_of(length(lay, b)) : 0;
-  int c0 = 0, c1 = -1;
-  if (nt > 0) {
-    const int ctas = working(lay, total);
-    c0 = cta_of(total, before + (long long)u * nt, ctas);
-    c1 = cta_of(total, before + (long long)(u + 1) * nt - 1, ctas);
+  if (part_o != nullptr) {
+    const long long before = tiles_before(lay, b), total = tiles_before(lay, lay.B);
+    const int nt = there ? tiles_of(length(lay, b)) : 0;
+    if (nt > 0) {
+      const int ctas = working(lay, total);
+      c0 = cta_of(total, before + (long long)u * nt, ctas);
+      parts = cta_of(total, before + (long long)(u + 1) * nt - 1, ctas) - c0 + 1;
+    }
   }
+  if (WPU == 1) __syncwarp();
+  else if (splits == 1) __syncthreads();
+  else cluster_sync_all();
+  grid_dep_wait();
   const long long slot0 = ((long long)b * lay.per_prompt + u + c0) * TILE_ROWS + (w % lay.wt) * a.group + hb * OWN_ROWS;
-  // ---- the CTAs of the cluster and the prompt, each CTA its share of the output
-  const uint32_t merged_a = ring + C::BODY, stats_a = ring + C::BODY + C::MERGED + 4 * OWN_ROWS * 2 * 4;
-  for (int i = rank * OWN_THREADS + threadIdx.x; i < n_heads * (HD / 4); i += splits * OWN_THREADS) {
+  // ---- each warp of the unit its share of the output
+  const int warp0 = warp / WPU * WPU;
+  for (int i = way * 32 + lane; i < n_heads * (HD / 4); i += ways * 32) {
     const int r = i / (HD / 4), d = (i % (HD / 4)) * 4;
     const float2* ml = part_ml + slot0 + r;
+    const uint32_t stats_a = smem_u32(stats + (warp0 * OWN_ROWS + r) * 2), part_a = smem_u32(smem_raw) + warp0 * OWN_RING + uint32_t(r * HD + d) * 4u;
     float top = -INFINITY;
-    for (int c = 0; c < splits; ++c) top = fmaxf(top, ld_cluster_f1(mapa_shared(stats_a + r * 8, c)));
-    for (int c = 0; c <= c1 - c0; ++c) top = fmaxf(top, ld_after_wait(ml + (long long)c * TILE_ROWS).x);
+    for (int c = 0; c < splits; ++c)
+#pragma unroll
+      for (int x = 0; x < WPU; ++x) {
+        const uint32_t at = stats_a + x * OWN_ROWS * 8;
+        top = fmaxf(top, ld_cluster_f1(splits > 1 ? mapa_shared(at, c) : at));
+      }
+    for (int c = 0; c < parts; ++c) top = fmaxf(top, ld_after_wait(ml + (long long)c * TILE_ROWS).x);
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     float sum = 0.f;
-    for (int c = 0; c < splits; ++c) {
-      const float f = weight(ld_cluster_f1(mapa_shared(stats_a + r * 8, c)), top);
-      const float4 v = ld_cluster_f4(mapa_shared(merged_a + uint32_t(r * HD + d) * 4u, c));
-      acc.x += f * v.x; acc.y += f * v.y; acc.z += f * v.z; acc.w += f * v.w;
-      sum += f * ld_cluster_f1(mapa_shared(stats_a + r * 8 + 4, c));
-    }
-    for (int c = 0; c <= c1 - c0; ++c) {
+    for (int c = 0; c < splits; ++c)
+#pragma unroll
+      for (int x = 0; x < WPU; ++x) {
+        const uint32_t at = stats_a + x * OWN_ROWS * 8, from = part_a + x * OWN_RING;
+        const float f = weight(ld_cluster_f1(splits > 1 ? mapa_shared(at, c) : at), top);
+        const float4 v = ld_cluster_f4(splits > 1 ? mapa_shared(from, c) : from);
+        acc.x += f * v.x; acc.y += f * v.y; acc.z += f * v.z; acc.w += f * v.w;
+        sum += f * ld_cluster_f1(splits > 1 ? mapa_shared(at + 4, c) : at + 4);
+      }
+    for (int c = 0; c < parts; ++c) {
       const float2 x = ld_after_wait(ml + (long long)c * TILE_ROWS);
       const float f = weight(x.x, top);
       const float4 v = ld_after_wait(reinterpret_cast<const float4*>(part_o + (slot0 + r + (long long)c * TILE_ROWS) * HD + d));
@@ -264,13 +261,13 @@ kf_shared_prefix_own(const Own a, const Layout lay, const float* part_o, const f
     out.y = pack_bf16(acc.z * inv, acc.w * inv);
     *reinterpret_cast<uint2*>(a.o + (((long long)b * lay.W + w) * a.Hkv * a.group + h0 + r) * HD + d) = out;
   }
-  cluster_sync_all();   // no CTA leaves while another reads its shared memory
+  if (splits > 1) cluster_sync_all();   // no CTA leaves while another reads its shared memory
 }
 
-template <int HD>
-static int launch_own(const Own& a, const Layout& l, const float* part_o, const float2* part_ml, int num_sms, cudaStream_t stream) {
+template <int HD, int WPU>
+static int launch_ways(const Own& a, const Layout& l, const float* part_o, const float2* part_ml, long long units, int splits, cudaStream_t stream) {
   using C = OwnCfg<HD>;
-  auto kern = kf_shared_prefix_own<HD>;
+  auto kern = kf_shared_prefix_own<HD, WPU>;
   static bool attr_set[16] = {};
   int dev = 0;
   cudaGetDevice(&dev);
@@ -279,13 +276,11 @@ static int launch_own(const Own& a, const Layout& l, const float* part_o, const 
     if (e != cudaSuccess) return 300 + (int)e;
     if (dev < 16) attr_set[dev] = true;
   }
-  const long long units = (long long)l.B * l.W * a.Hkv * ((a.group + OWN_ROWS - 1) / OWN_ROWS);
-  // two CTAs per SM, at least one tile per CTA
-  int splits = 1;
-  while (splits < 8 && units * splits * 2 <= 2LL * num_sms && a.S > splits * OWN_TILE) splits *= 2;
-  if (units * splits > 0x7fffffffLL) return 6;
+  const int per_cta = OWN_WARPS / WPU;
+  const long long ctas = (units + per_cta - 1) / per_cta * splits;
+  if (ctas > 0x7fffffffLL) return 6;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(units * splits));
+  cfg.gridDim = dim3((unsigned)ctas);
   cfg.blockDim = dim3(OWN_THREADS);
   cfg.dynamicSmemBytes = C::SMEM;
   cfg.stream = stream;
@@ -297,8 +292,20 @@ static int launch_own(const Own& a, const Layout& l, const float* part_o, const 
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = part_o != nullptr ? 2 : 1;
-  cudaError_t e = cudaLaunchKernelEx(&cfg, kern, a, l, part_o, part_ml);
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kern, a, l, part_o, part_ml, units);
   return e == cudaSuccess ? 0 : 500 + (int)e;
+}
+
+template <int HD>
+static int launch_own(const Own& a, const Layout& l, const float* part_o, const float2* part_ml, int num_sms, cudaStream_t stream) {
+  const long long units = (long long)l.B * l.W * a.Hkv * ((a.group + OWN_ROWS - 1) / OWN_ROWS);
+  // as many warps a unit as fill eight on every SM, of which each has a tile at least
+  const int tiles = (a.S + OWN_TILE - 1) / OWN_TILE;
+  int ways = 1;
+  while (ways < 32 && units * ways * 2 <= 8LL * num_sms && tiles >= ways * 2) ways *= 2;
+  if (ways == 1) return launch_ways<HD, 1>(a, l, part_o, part_ml, units, 1, stream);
+  if (ways == 2) return launch_ways<HD, 2>(a, l, part_o, part_ml, units, 1, stream);
+  return launch_ways<HD, 4>(a, l, part_o, part_ml, units, ways / 4, stream);
 }
 
 int launch_prefix(const void* q, const void* k, const void* v, const Layout& l, int H, int Hkv, int hd, const long long* qs, const long long* ks,
