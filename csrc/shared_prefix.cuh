@@ -23,17 +23,14 @@ struct Layout {
 __host__ __device__ __forceinline__ int tiles_of(int len) { return (len + TILE_KEYS - 1) / TILE_KEYS; }
 __device__ __forceinline__ int length(const Layout& l, int b) { return l.lens ? min(max(l.lens[b], 0), l.P) : l.P; }
 
-// CTAs that have work: with fewer tiles than CTAs one tile each, so that no CTA between two others has none.
-__device__ __forceinline__ int working(const Layout& l, long long total) { return total < l.ctas ? int(total) : l.ctas; }
-// First tile of the range of one of `ctas` CTAs that all have work; the ranges follow one another.
-__device__ __forceinline__ long long range_begin(long long total, int cta, int ctas) { return total * cta / ctas; }
-// The CTA whose range holds tile t: the last one with range_begin <= t.
-__device__ __forceinline__ int cta_of(long long total, long long t, int ctas) { return int(((t + 1) * ctas - 1) / total); }
+// Tiles of a CTA's range: as few as cover all with the CTAs there are.  Counts of tiles have 32 bits (kf_shared_prefix_scratch), and
+// CTAs without work are the last ones, so that none lies between two parts of a unit.
+__device__ __forceinline__ uint32_t range(uint32_t total, int ctas) { return (total + ctas - 1) / ctas; }
 
 // Tiles of the prompts before b (all: b = B), by one warp; every lane has the result.
-__device__ __forceinline__ long long tiles_before(const Layout& l, int b) {
-  if (!l.lens) return (long long)tiles_of(l.P) * l.per_prompt * b;
-  long long n = 0;
+__device__ __forceinline__ uint32_t tiles_before(const Layout& l, int b) {
+  if (!l.lens) return uint32_t(tiles_of(l.P)) * l.per_prompt * b;
+  uint32_t n = 0;
   for (int i = threadIdx.x & 31; i < b; i += 32) n += tiles_of(length(l, i));
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);

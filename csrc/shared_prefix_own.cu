@@ -6,7 +6,8 @@
 //   * a unit is a continuation's key head; its query heads are the 16 rows of an m16n8k16 MMA, its keys are dealt out to 1 to 32 warps, as
 //     many as it takes to have eight warps on every SM: few units need all of them for one, many (a batch of short continuations) one each;
 //   * every warp streams tiles of 16 keys through a cp.async ring of its own, two tiles ahead, without a barrier; 16-byte chunks are
-//     XOR-swizzled, so that ldmatrix is free of bank conflicts;
+//     XOR-swizzled, so that ldmatrix is free of bank conflicts; where there is a warp for every tile, the ring is one tile, and the CTAs are
+//     small enough to run beside those of the prompt's kernel;
 //   * the (max, sum, output) triples of the warps, of the CTAs of a cluster and of the prompt are joined in a fixed order.
 // All of it up to that last step runs without the prompt's kernel, and starts on the SMs that it leaves (programmatic launch).
 #include "decode_common.cuh"
@@ -20,17 +21,18 @@ using namespace kf::decode;
 constexpr int OWN_WARPS = 4, OWN_THREADS = OWN_WARPS * 32;
 constexpr int OWN_TILE = 16;       // keys per ring stage of a warp
 constexpr int OWN_ROWS = 16;       // query heads per unit (MMA rows)
-constexpr int OWN_RING = 24 << 10; // bytes of a warp's ring: two CTAs an SM, 128 KB of it under way
 
-template <int HD>
+// ONE: a warp has one tile at most.  Else its ring has 24 KB: two CTAs an SM, 128 KB of it under way.
+template <int HD, bool ONE>
 struct OwnCfg {
   static constexpr int TILE_BYTES = OWN_TILE * HD * 2;
-  static constexpr int STAGES = OWN_RING / (2 * TILE_BYTES);         // 3 for a head dim of 128, 6 for 64
+  static constexpr int STAGES = ONE ? 1 : (24 << 10) / (2 * TILE_BYTES);   // 3 for a head dim of 128, 6 for 64
+  static constexpr int RING = STAGES * 2 * TILE_BYTES;
   static constexpr int PART = OWN_ROWS * HD * 4;                     // a warp's partial output, over its ring
-  static_assert(PART <= OWN_RING, "");
+  static_assert(PART <= RING, "");
   static constexpr int STATS = OWN_WARPS * OWN_ROWS * 2 * 4;         // (max, sum) per warp and row
   static constexpr int SEEN = OWN_WARPS * 8 * 4;                     // per stage: which of its keys are visible
-  static constexpr size_t SMEM = size_t(OWN_WARPS) * OWN_RING + STATS + SEEN;
+  static constexpr size_t SMEM = size_t(OWN_WARPS) * RING + STATS + SEEN;
 };
 
 struct Own {
@@ -44,32 +46,33 @@ struct Own {
 };
 
 // WPU: warps of a CTA that share a unit.  Clusters of more than one CTA (WPU = 4) share one too.
-template <int HD, int WPU>
+template <int HD, int WPU, bool ONE>
 __global__ void __launch_bounds__(OWN_THREADS)
-kf_shared_prefix_own(const Own a, const Layout lay, const float* part_o, const float2* part_ml, const long long units) {
-  using C = OwnCfg<HD>;
+kf_shared_prefix_own(const Own a, const Layout lay, const float* part_o, const float2* part_ml, const uint32_t units) {
+  using C = OwnCfg<HD, ONE>;
   extern __shared__ __align__(128) uint8_t smem_raw[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int splits = WPU == OWN_WARPS ? int(cluster_nctaid()) : 1, rank = WPU == OWN_WARPS ? int(cluster_ctarank()) : 0;
   const int way = rank * WPU + warp % WPU, ways = splits * WPU;     // which share of the unit's keys
-  const uint32_t ring = smem_u32(smem_raw) + warp * OWN_RING;
-  float* stats = reinterpret_cast<float*>(smem_raw + OWN_WARPS * OWN_RING);                            // [warp][row][2]
-  volatile uint32_t* seen = reinterpret_cast<uint32_t*>(smem_raw + OWN_WARPS * OWN_RING + C::STATS) + warp * 8;
+  const uint32_t ring = smem_u32(smem_raw) + warp * C::RING;
+  float* stats = reinterpret_cast<float*>(smem_raw + OWN_WARPS * C::RING);                            // [warp][row][2]
+  volatile uint32_t* seen = reinterpret_cast<uint32_t*>(smem_raw + OWN_WARPS * C::RING + C::STATS) + warp * 8;
 
-  const long long unit0 = blockIdx.x / splits * (OWN_WARPS / WPU) + warp / WPU;
+  const uint32_t unit0 = blockIdx.x / uint32_t(splits) * (OWN_WARPS / WPU) + warp / WPU;
   const bool there = unit0 < units;
-  long long unit = there ? unit0 : 0;
-  const int w = int(unit % lay.W);   // continuations of a prompt side by side: their common keys are in L2, some in L1
-  unit /= lay.W;
-  const int blocks_per_kv = (a.group + OWN_ROWS - 1) / OWN_ROWS;
-  const int hb = int(unit % blocks_per_kv);
-  unit /= blocks_per_kv;
-  const int hk = int(unit % a.Hkv), b = int(unit / a.Hkv);
+  uint32_t unit = there ? unit0 : 0u;
+  uint32_t next = unit / lay.W;
+  const int w = int(unit - next * lay.W);   // continuations of a prompt side by side: their common keys are in L2, some in L1
+  unit = next;
+  const uint32_t blocks_per_kv = (a.group + OWN_ROWS - 1) / OWN_ROWS;
+  next = blocks_per_kv > 1 ? unit / blocks_per_kv : unit;
+  const int hb = int(unit - next * blocks_per_kv);
+  const int b = int(next / a.Hkv), hk = int(next - uint32_t(b) * a.Hkv);
   const int n_heads = there ? min(OWN_ROWS, a.group - hb * OWN_ROWS) : 0;     // query heads of this unit
   const int h0 = hk * a.group + hb * OWN_ROWS;
 
   const int n_tiles = there ? (a.S + OWN_TILE - 1) / OWN_TILE : 0;
-  const int t0 = int((long long)n_tiles * way / ways), t1 = int((long long)n_tiles * (way + 1) / ways);
+  const int each = (n_tiles + ways - 1) / ways, t0 = min(n_tiles, each * way), t1 = min(n_tiles, t0 + each);
   const __nv_bfloat16* kb = a.k + b * a.k_b + hk * a.k_h;
   const __nv_bfloat16* vb = a.v + b * a.v_b + hk * a.v_h;
   const uint8_t* table = a.rows ? a.rows + b * a.r_b + w * a.r_w : nullptr;
@@ -98,8 +101,8 @@ kf_shared_prefix_own(const Own a, const Layout lay, const float* part_o, const f
     }
   };
   int slot = slot_of(t0);
-  for (int t = t0; t < t0 + C::STAGES - 1; ++t) {
-    const int after = slot_of(t + 1);
+  for (int t = t0; t < t0 + max(1, C::STAGES - 1); ++t) {
+    const int after = ONE ? 0 : slot_of(t + 1);
     if (t < t1) issue(t, slot);
     cp_commit();
     slot = after;
@@ -125,12 +128,14 @@ kf_shared_prefix_own(const Own a, const Layout lay, const float* part_o, const f
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 
   for (int t = t0; t < t1; ++t) {
-    cp_wait<C::STAGES - 2>();
+    cp_wait<ONE ? 0 : C::STAGES - 2>();
     __syncwarp();   // tile t has landed for every lane, and the stage refilled below has been consumed
-    const int after = slot_of(t + C::STAGES);
-    if (t + C::STAGES - 1 < t1) issue(t + C::STAGES - 1, slot);
-    cp_commit();
-    slot = after;
+    if (!ONE) {
+      const int after = slot_of(t + C::STAGES);
+      if (t + C::STAGES - 1 < t1) issue(t + C::STAGES - 1, slot);
+      cp_commit();
+      slot = after;
+    }
     const int st = (t - t0) % C::STAGES;
     const uint32_t ks = ring + uint32_t(st) * 2u * C::TILE_BYTES, vs = ks + C::TILE_BYTES;
     const int mi = lane >> 3, lr = lane & 7;
@@ -190,7 +195,7 @@ kf_shared_prefix_own(const Own a, const Layout lay, const float* part_o, const f
   }
   cp_wait<0>();
   __syncwarp();  // the ring is idle: the warp's partial result takes its place
-  float* part = reinterpret_cast<float*>(smem_raw + warp * OWN_RING);
+  float* part = reinterpret_cast<float*>(smem_raw + warp * C::RING);
 #pragma unroll
   for (int hf = 0; hf < 2; ++hf) {
     l[hf] += __shfl_xor_sync(0xffffffffu, l[hf], 1);
@@ -210,52 +215,74 @@ kf_shared_prefix_own(const Own a, const Layout lay, const float* part_o, const f
   int c0 = 0, parts = 0;
   const int u = hk * lay.row_tiles + w / lay.wt;
   if (part_o != nullptr) {
-    const long long before = tiles_before(lay, b), total = tiles_before(lay, lay.B);
+    const uint32_t first = tiles_before(lay, b), chunk = range(tiles_before(lay, lay.B), lay.ctas);
     const int nt = there ? tiles_of(length(lay, b)) : 0;
     if (nt > 0) {
-      const int ctas = working(lay, total);
-      c0 = cta_of(total, before + (long long)u * nt, ctas);
-      parts = cta_of(total, before + (long long)(u + 1) * nt - 1, ctas) - c0 + 1;
+      c0 = int((first + uint32_t(u) * nt) / chunk);
+      parts = int((first + uint32_t(u + 1) * nt - 1) / chunk) - c0 + 1;
     }
   }
   if (WPU == 1) __syncwarp();
   else if (splits == 1) __syncthreads();
   else cluster_sync_all();
   grid_dep_wait();
+  grid_dep_launch();
   const long long slot0 = ((long long)b * lay.per_prompt + u + c0) * TILE_ROWS + (w % lay.wt) * a.group + hb * OWN_ROWS;
-  // ---- each warp of the unit its share of the output
   const int warp0 = warp / WPU * WPU;
-  for (int i = way * 32 + lane; i < n_heads * (HD / 4); i += ways * 32) {
-    const int r = i / (HD / 4), d = (i % (HD / 4)) * 4;
-    const float2* ml = part_ml + slot0 + r;
-    const uint32_t stats_a = smem_u32(stats + (warp0 * OWN_ROWS + r) * 2), part_a = smem_u32(smem_raw) + warp0 * OWN_RING + uint32_t(r * HD + d) * 4u;
-    float top = -INFINITY;
-    for (int c = 0; c < splits; ++c)
-#pragma unroll
-      for (int x = 0; x < WPU; ++x) {
-        const uint32_t at = stats_a + x * OWN_ROWS * 8;
-        top = fmaxf(top, ld_cluster_f1(splits > 1 ? mapa_shared(at, c) : at));
+  const uint32_t stats_a = smem_u32(stats + warp0 * OWN_ROWS * 2), part_a = smem_u32(smem_raw) + warp0 * C::RING;
+  auto own_at = [&](uint32_t base, int s, int step) {   // of the unit's s-th warp
+    const uint32_t at = base + (s % WPU) * step;
+    return splits > 1 ? mapa_shared(at, s / WPU) : at;
+  };
+  // ---- each row's largest score and sum: a few lanes a row, each some of the warps and of the prompt's parts
+  const int spread = n_heads <= 1 ? 1 : 1 << (32 - __clz(n_heads - 1)), lanes = 32 / spread;
+  float top = -INFINITY, sum = 0.f;
+  {
+    const int r = lane / lanes, sub = lane % lanes;
+    if (r < n_heads) {
+      for (int s = sub; s < ways + parts; s += lanes) {
+        float2 x;
+        if (s < ways) {
+          const uint32_t at = own_at(stats_a + r * 8, s, OWN_ROWS * 8);
+          x = make_float2(ld_cluster_f1(at), ld_cluster_f1(at + 4));
+        } else {
+          x = ld_after_wait(part_ml + slot0 + r + (long long)(s - ways) * TILE_ROWS);
+        }
+        const float higher = fmaxf(top, x.x);
+        sum = sum * weight(top, higher) + x.y * weight(x.x, higher);
+        top = higher;
       }
-    for (int c = 0; c < parts; ++c) top = fmaxf(top, ld_after_wait(ml + (long long)c * TILE_ROWS).x);
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    float sum = 0.f;
-    for (int c = 0; c < splits; ++c)
-#pragma unroll
-      for (int x = 0; x < WPU; ++x) {
-        const uint32_t at = stats_a + x * OWN_ROWS * 8, from = part_a + x * OWN_RING;
-        const float f = weight(ld_cluster_f1(splits > 1 ? mapa_shared(at, c) : at), top);
-        const float4 v = ld_cluster_f4(splits > 1 ? mapa_shared(from, c) : from);
-        acc.x += f * v.x; acc.y += f * v.y; acc.z += f * v.z; acc.w += f * v.w;
-        sum += f * ld_cluster_f1(splits > 1 ? mapa_shared(at + 4, c) : at + 4);
-      }
-    for (int c = 0; c < parts; ++c) {
-      const float2 x = ld_after_wait(ml + (long long)c * TILE_ROWS);
-      const float f = weight(x.x, top);
-      const float4 v = ld_after_wait(reinterpret_cast<const float4*>(part_o + (slot0 + r + (long long)c * TILE_ROWS) * HD + d));
-      acc.x += f * v.x; acc.y += f * v.y; acc.z += f * v.z; acc.w += f * v.w;
-      sum += f * x.y;
     }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;   // nothing visible: zeros
+    for (int o = lanes / 2; o > 0; o >>= 1) {
+      const float x = __shfl_xor_sync(0xffffffffu, top, o), y = __shfl_xor_sync(0xffffffffu, sum, o);
+      const float higher = fmaxf(top, x);
+      sum = sum * weight(top, higher) + y * weight(x, higher);
+      top = higher;
+    }
+  }
+  // ---- each warp of the unit its share of the output
+  for (int base = way * 32; base < n_heads * (HD / 4); base += ways * 32) {
+    const int i = base + lane, r = i / (HD / 4), d = (i % (HD / 4)) * 4;
+    const float row_top = __shfl_sync(0xffffffffu, top, (r * lanes) & 31), row_sum = __shfl_sync(0xffffffffu, sum, (r * lanes) & 31);
+    if (r >= n_heads) continue;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    auto add = [&](float f, const float4& v) { acc.x += f * v.x; acc.y += f * v.y; acc.z += f * v.z; acc.w += f * v.w; };
+    constexpr int AT_ONCE = 4;
+    const float2* ml = part_ml + slot0 + r;
+    const float4* po = reinterpret_cast<const float4*>(part_o + (slot0 + r) * HD + d);
+    for (int c = 0; c < parts; c += AT_ONCE) {
+      float2 x[AT_ONCE];
+      float4 v[AT_ONCE];
+#pragma unroll
+      for (int e = 0; e < AT_ONCE; ++e)
+        if (c + e < parts) x[e] = ld_after_wait(ml + (long long)(c + e) * TILE_ROWS), v[e] = ld_after_wait(po + (long long)(c + e) * TILE_ROWS * (HD / 4));
+#pragma unroll
+      for (int e = 0; e < AT_ONCE; ++e)
+        if (c + e < parts) add(weight(x[e].x, row_top), v[e]);
+    }
+    for (int s = 0; s < ways; ++s)
+      add(weight(ld_cluster_f1(own_at(stats_a + r * 8, s, OWN_ROWS * 8)), row_top), ld_cluster_f4(own_at(part_a + uint32_t(r * HD + d) * 4u, s, C::RING)));
+    const float inv = row_sum == 0.f ? 0.f : 1.f / row_sum;   // nothing visible: zeros
     uint2 out;
     out.x = pack_bf16(acc.x * inv, acc.y * inv);
     out.y = pack_bf16(acc.z * inv, acc.w * inv);
@@ -264,10 +291,10 @@ kf_shared_prefix_own(const Own a, const Layout lay, const float* part_o, const f
   if (splits > 1) cluster_sync_all();   // no CTA leaves while another reads its shared memory
 }
 
-template <int HD, int WPU>
+template <int HD, int WPU, bool ONE>
 static int launch_ways(const Own& a, const Layout& l, const float* part_o, const float2* part_ml, long long units, int splits, cudaStream_t stream) {
-  using C = OwnCfg<HD>;
-  auto kern = kf_shared_prefix_own<HD, WPU>;
+  using C = OwnCfg<HD, ONE>;
+  auto kern = kf_shared_prefix_own<HD, WPU, ONE>;
   static bool attr_set[16] = {};
   int dev = 0;
   cudaGetDevice(&dev);
@@ -292,20 +319,28 @@ static int launch_ways(const Own& a, const Layout& l, const float* part_o, const
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = part_o != nullptr ? 2 : 1;
-  cudaError_t e = cudaLaunchKernelEx(&cfg, kern, a, l, part_o, part_ml, units);
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kern, a, l, part_o, part_ml, (uint32_t)units);
   return e == cudaSuccess ? 0 : 500 + (int)e;
 }
 
 template <int HD>
 static int launch_own(const Own& a, const Layout& l, const float* part_o, const float2* part_ml, int num_sms, cudaStream_t stream) {
   const long long units = (long long)l.B * l.W * a.Hkv * ((a.group + OWN_ROWS - 1) / OWN_ROWS);
-  // as many warps a unit as fill eight on every SM, of which each has a tile at least
+  // A warp for every tile where that leaves no more than 24 on an SM, which is what its memory holds of them; else as many warps a unit as
+  // fill eight on every SM, of which each has a tile at least.
   const int tiles = (a.S + OWN_TILE - 1) / OWN_TILE;
   int ways = 1;
+  while (ways < tiles && ways < 32) ways *= 2;
+  if (ways >= tiles && units * ways <= 24LL * num_sms) {
+    if (ways == 1) return launch_ways<HD, 1, true>(a, l, part_o, part_ml, units, 1, stream);
+    if (ways == 2) return launch_ways<HD, 2, true>(a, l, part_o, part_ml, units, 1, stream);
+    return launch_ways<HD, 4, true>(a, l, part_o, part_ml, units, ways / 4, stream);
+  }
+  ways = 1;
   while (ways < 32 && units * ways * 2 <= 8LL * num_sms && tiles >= ways * 2) ways *= 2;
-  if (ways == 1) return launch_ways<HD, 1>(a, l, part_o, part_ml, units, 1, stream);
-  if (ways == 2) return launch_ways<HD, 2>(a, l, part_o, part_ml, units, 1, stream);
-  return launch_ways<HD, 4>(a, l, part_o, part_ml, units, ways / 4, stream);
+  if (ways == 1) return launch_ways<HD, 1, false>(a, l, part_o, part_ml, units, 1, stream);
+  if (ways == 2) return launch_ways<HD, 2, false>(a, l, part_o, part_ml, units, 1, stream);
+  return launch_ways<HD, 4, false>(a, l, part_o, part_ml, units, ways / 4, stream);
 }
 
 int launch_prefix(const void* q, const void* k, const void* v, const Layout& l, int H, int Hkv, int hd, const long long* qs, const long long* ks,
@@ -317,7 +352,7 @@ static bool make_layout(Layout& l, const void* lens, int B, int W, int P, int gr
   const int row_tiles = (W + wt - 1) / wt;
   const long long tiles = (long long)tiles_of(P) * Hkv * row_tiles * B;
   l = Layout{(const int*)lens, B, W, P, Hkv * row_tiles, row_tiles, wt, (int)(tiles < num_sms ? tiles : num_sms)};
-  return (long long)Hkv * row_tiles * B < 0x7fffff00LL;
+  return tiles < 0x7fff0000LL && (long long)B * W * Hkv * group < 1LL << 27;   // counts of tiles and units in 32 bits
 }
 
 }  // namespace shared_prefix

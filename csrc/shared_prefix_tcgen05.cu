@@ -5,6 +5,7 @@
 // What bounds it: the keys and values, 4 hd bytes per position and head.  A tile of 128 keys of 128 values is 64 KB, which is 2700 cycles
 // of an SM's share of HBM; its two products take 512, its 16 384 exponentials 1024.  So rows that are not there (a tile is always 128)
 // cost nothing, and all that counts is to keep the copies in flight: three stages each of K and V (192 KB) run ahead of the products.
+// A CTA of one or two tiles takes only their memory, and leaves the rest of its SM to the second kernel, which starts meanwhile.
 //
 //   warp 0     : TMA producer of Q and K
 //   warp 1     : MMA issuer
@@ -28,7 +29,7 @@ using namespace kf::attn;
 constexpr int THREADS = 384;
 constexpr int REGS_ISSUE = 72, REGS_SOFTMAX = 216;  // per thread; 72 + 2 * 216 = 3 * 168, what the launch gets
 constexpr int TMEM_COLS = 512;
-constexpr int STAGES = 3;
+constexpr int STAGES = 3;                           // of K and of V at most; a CTA with fewer tiles takes less memory
 constexpr float RESCALE_THRESHOLD = 8.0f;           // P up to 2^8 before the accumulator is scaled again
 
 template <int HD>
@@ -36,16 +37,15 @@ struct Cfg {
   static constexpr int BLOCKS = HD / 64;
   static constexpr int TILE_BYTES = TILE_KEYS * HD * 2;
   static constexpr int BLOCK_BYTES = TILE_KEYS * 128;
-  static constexpr int TILES = 1 + 2 * STAGES;      // Q, K ring, V ring
   static constexpr int STATS = 2 * TILE_ROWS * 8;   // (max, sum) of each group's rows
   static constexpr int HEAD = 3 * 1024;             // STATS and the barriers, before the tiles, which start on 1024 bytes
-  static constexpr size_t SMEM = HEAD + TILES * size_t(TILE_BYTES);   // all of the 227 KB of a CTA at a head dim of 128
+  static constexpr size_t smem(int stages) { return HEAD + (1 + 2 * size_t(stages)) * TILE_BYTES; }   // Q, K ring, V ring: up to 227 KB
 };
 
 // Where a CTA is in its range.
 struct Walk {
   int b, u, j, nt;      // prompt, unit of the prompt, tile of the unit, tiles of a unit of this prompt
-  long long left;       // tiles of the range that are still to come
+  int left;             // tiles of the range that are still to come
 };
 
 __device__ __forceinline__ void advance(const Layout& l, Walk& w, int n) {
@@ -61,30 +61,30 @@ __device__ __forceinline__ void advance(const Layout& l, Walk& w, int n) {
   }
 }
 
-__device__ __forceinline__ int segment(const Walk& w) { return int(w.left < w.nt - w.j ? w.left : w.nt - w.j); }
+__device__ __forceinline__ int segment(const Walk& w) { return min(w.left, w.nt - w.j); }
 
 // Start of this CTA's range, by one warp.
 __device__ Walk locate(const Layout& l) {
   Walk w;
-  const long long total = tiles_before(l, l.B);
-  const int ctas = working(l, total), cta = int(blockIdx.x);
-  const long long t0 = cta < ctas ? range_begin(total, cta, ctas) : 0;
-  w.left = cta < ctas ? range_begin(total, cta + 1, ctas) - t0 : 0;
+  const uint32_t total = tiles_before(l, l.B), chunk = range(total, l.ctas);
+  const uint32_t t0 = chunk * blockIdx.x;
+  w.left = t0 < total ? int(min(chunk, total - t0)) : 0;
   w.b = w.u = w.j = 0;
   w.nt = 1;
   if (w.left <= 0) return w;
-  long long before = 0;
+  uint32_t before = 0;
   if (!l.lens) {
-    w.b = int(t0 / ((long long)tiles_of(l.P) * l.per_prompt));
-    before = (long long)tiles_of(l.P) * l.per_prompt * w.b;
+    const uint32_t each = uint32_t(tiles_of(l.P)) * l.per_prompt;
+    w.b = int(t0 / each);
+    before = each * w.b;
   } else {
     const int lane = threadIdx.x & 31;
     for (int base = 0; base < l.B; base += 32) {
-      const long long own = base + lane < l.B ? (long long)tiles_of(length(l, base + lane)) * l.per_prompt : 0;
-      long long upto = own;
+      const uint32_t own = base + lane < l.B ? uint32_t(tiles_of(length(l, base + lane))) * l.per_prompt : 0u;
+      uint32_t upto = own;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const long long v = __shfl_up_sync(0xffffffffu, upto, o);
+        const uint32_t v = __shfl_up_sync(0xffffffffu, upto, o);
         if (lane >= o) upto += v;
       }
       const uint32_t past = __ballot_sync(0xffffffffu, before + upto > t0);
@@ -103,16 +103,31 @@ __device__ Walk locate(const Layout& l) {
   return w;
 }
 
+// Stage and phase of a ring's next use.
+struct Turn {
+  int st = 0;
+  uint32_t phase = 0;
+  __device__ __forceinline__ void next(int stages) {
+    if (++st == stages) st = 0, phase ^= 1u;
+  }
+};
+
 template <int N>
 __device__ __forceinline__ void regs_give() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N>
 __device__ __forceinline__ void regs_take() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 
+__device__ __forceinline__ void st_global_v8(float* p, const float (&v)[8]) {
+  asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]),
+               "f"(v[6]), "f"(v[7])
+               : "memory");
+}
+
 template <int HD>
 __global__ void __launch_bounds__(THREADS, 1)
 kf_shared_prefix_tcgen05(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
-                         const __grid_constant__ CUtensorMap map_v, const Layout lay, int group, float scale_log2, float* __restrict__ part_o,
-                         float2* __restrict__ part_ml, int* status) {
+                         const __grid_constant__ CUtensorMap map_v, const Layout lay, int group, int stages, float scale_log2,
+                         float* __restrict__ part_o, float2* __restrict__ part_ml, int* status) {
   using C = Cfg<HD>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   const uint32_t smem_base = smem_u32(smem_raw) + C::HEAD;
@@ -121,7 +136,7 @@ kf_shared_prefix_tcgen05(const __grid_constant__ CUtensorMap map_q, const __grid
     if (threadIdx.x == 0) atomicCAS(status, 0, int(KF_ERR_WAIT_DRAIN));
     return;
   }
-  const uint32_t q_smem = smem_base, k_smem = q_smem + C::TILE_BYTES, v_smem = k_smem + STAGES * C::TILE_BYTES;
+  const uint32_t q_smem = smem_base, k_smem = q_smem + C::TILE_BYTES, v_smem = k_smem + stages * C::TILE_BYTES;
   float2* stats = reinterpret_cast<float2*>(smem_raw);
   uint8_t* bar_generic = smem_raw + C::STATS;
   const uint32_t bar_base = smem_u32(bar_generic);
@@ -167,6 +182,7 @@ kf_shared_prefix_tcgen05(const __grid_constant__ CUtensorMap map_q, const __grid
     tmem_alloc(smem_u32(const_cast<uint32_t*>(tmem_slot_ptr)), TMEM_COLS);
     tmem_relinquish();
   }
+  grid_dep_wait();
   if (warp == 2) {
     const Walk w = locate(lay);
     if (lane == 0) *start = w;
@@ -186,7 +202,8 @@ kf_shared_prefix_tcgen05(const __grid_constant__ CUtensorMap map_q, const __grid
       // ------------------------------------------------------------ TMA producer of Q and K
       if (elect_one()) {
         bool ok = true;
-        int i = 0, seg = 0, issued = 0, q_issued = 0;   // i, seg: tiles and units so far
+        int seg = 0, issued = 0, q_issued = 0;   // units and tiles so far
+        Turn turn;
         while (wk.left > 0 && ok) {
           const int n = segment(wk), hk = wk.u / lay.row_tiles, rt = wk.u % lay.row_tiles;
           if (seg > 0 && !mbar_wait(q_empty, (seg - 1) & 1, status, KF_ERR_WAIT_EMPTY)) { ok = false; break; }
@@ -195,13 +212,12 @@ kf_shared_prefix_tcgen05(const __grid_constant__ CUtensorMap map_q, const __grid
           for (int c = 0; c < C::BLOCKS; ++c)
             tma_load_4d(q_smem + c * C::BLOCK_BYTES, &map_q, q_full, 64 * c, hk * group, rt * lay.wt, wk.b);
           ++q_issued;
-          for (int j = wk.j; j < wk.j + n; ++j, ++i) {
-            const int st = i % STAGES, use = i / STAGES;
-            if (use > 0 && !mbar_wait(k_empty(st), (use - 1) & 1, status, KF_ERR_WAIT_EMPTY)) { ok = false; break; }
-            mbar_expect_tx(k_full(st), C::TILE_BYTES);
+          for (int j = wk.j; j < wk.j + n; ++j, turn.next(stages)) {
+            if (issued >= stages && !mbar_wait(k_empty(turn.st), turn.phase ^ 1u, status, KF_ERR_WAIT_EMPTY)) { ok = false; break; }
+            mbar_expect_tx(k_full(turn.st), C::TILE_BYTES);
 #pragma unroll
             for (int c = 0; c < C::BLOCKS; ++c)
-              tma_load_4d(k_smem + st * C::TILE_BYTES + c * C::BLOCK_BYTES, &map_k, k_full(st), 64 * c, hk, j * TILE_KEYS, wk.b);
+              tma_load_4d(k_smem + turn.st * C::TILE_BYTES + c * C::BLOCK_BYTES, &map_k, k_full(turn.st), 64 * c, hk, j * TILE_KEYS, wk.b);
             ++issued;
           }
           advance(lay, wk, n);
@@ -209,29 +225,29 @@ kf_shared_prefix_tcgen05(const __grid_constant__ CUtensorMap map_q, const __grid
         }
         if (!ok) {
           if (q_issued > 0) mbar_wait(q_full, (q_issued - 1) & 1, status, KF_ERR_WAIT_DRAIN);
-          for (int j = max(0, issued - STAGES); j < issued; ++j) mbar_wait(k_full(j % STAGES), (j / STAGES) & 1, status, KF_ERR_WAIT_DRAIN);
+          for (int j = max(0, issued - stages); j < issued; ++j) mbar_wait(k_full(j % stages), (j / stages) & 1, status, KF_ERR_WAIT_DRAIN);
         }
       }
     } else if (warp == 2) {
       // ------------------------------------------------------------ TMA producer of V
       if (elect_one()) {
         bool ok = true;
-        int i = 0, issued = 0;
+        int issued = 0;
+        Turn turn;
         while (wk.left > 0 && ok) {
           const int n = segment(wk), hk = wk.u / lay.row_tiles;
-          for (int j = wk.j; j < wk.j + n; ++j, ++i) {
-            const int st = i % STAGES, use = i / STAGES;
-            if (use > 0 && !mbar_wait(v_empty(st), (use - 1) & 1, status, KF_ERR_WAIT_EMPTY)) { ok = false; break; }
-            mbar_expect_tx(v_full(st), C::TILE_BYTES);
+          for (int j = wk.j; j < wk.j + n; ++j, turn.next(stages)) {
+            if (issued >= stages && !mbar_wait(v_empty(turn.st), turn.phase ^ 1u, status, KF_ERR_WAIT_EMPTY)) { ok = false; break; }
+            mbar_expect_tx(v_full(turn.st), C::TILE_BYTES);
 #pragma unroll
             for (int c = 0; c < C::BLOCKS; ++c)
-              tma_load_4d(v_smem + st * C::TILE_BYTES + c * C::BLOCK_BYTES, &map_v, v_full(st), 64 * c, hk, j * TILE_KEYS, wk.b);
+              tma_load_4d(v_smem + turn.st * C::TILE_BYTES + c * C::BLOCK_BYTES, &map_v, v_full(turn.st), 64 * c, hk, j * TILE_KEYS, wk.b);
             ++issued;
           }
           advance(lay, wk, n);
         }
         if (!ok)
-          for (int j = max(0, issued - STAGES); j < issued; ++j) mbar_wait(v_full(j % STAGES), (j / STAGES) & 1, status, KF_ERR_WAIT_DRAIN);
+          for (int j = max(0, issued - stages); j < issued; ++j) mbar_wait(v_full(j % stages), (j / stages) & 1, status, KF_ERR_WAIT_DRAIN);
       }
     } else if (warp == 1) {
       // ------------------------------------------------------------ MMA issuer
@@ -239,12 +255,13 @@ kf_shared_prefix_tcgen05(const __grid_constant__ CUtensorMap map_q, const __grid
         constexpr uint32_t idesc_s = umma_idesc_bf16(TILE_ROWS, TILE_KEYS, false, false);
         constexpr uint32_t idesc_o = umma_idesc_bf16(TILE_ROWS, HD, false, true);
         bool ok = true;
-        int first = 0, seg = 0;        // tiles before this unit, units
+        int seg = 0;                   // units so far
         int done[2] = {0, 0};          // tiles of each group whose P has been read
-        // S_g = Q K^T of the i-th tile of the range
-        auto issue_s = [&](int g, int i) {
-          const int st = i % STAGES;
-          if (!mbar_wait(k_full(st), (i / STAGES) & 1, status, KF_ERR_WAIT_FULL)) return false;
+        Turn kt, vt;
+        // S_g = Q K^T of the next tile of the range
+        auto issue_s = [&](int g) {
+          const int st = kt.st;
+          if (!mbar_wait(k_full(st), kt.phase, status, KF_ERR_WAIT_FULL)) return false;
           tc_fence_after();
 #pragma unroll
           for (int kk = 0; kk < HD / 16; ++kk) {
@@ -254,19 +271,20 @@ kf_shared_prefix_tcgen05(const __grid_constant__ CUtensorMap map_q, const __grid
           }
           tc_commit(s_full(g));
           tc_commit(k_empty(st));
+          kt.next(stages);
           return true;
         };
         while (wk.left > 0 && ok) {
           const int n = segment(wk);
           ok = mbar_wait(q_full, seg & 1, status, KF_ERR_WAIT_FULL);
           if (ok) tc_fence_after();
-          for (int i = 0; i < min(n, 2) && ok; ++i) ok = issue_s(i, first + i);
+          for (int i = 0; i < min(n, 2) && ok; ++i) ok = issue_s(i);
           if (ok && n <= 2) tc_commit(q_empty);
           // the accumulators of the unit before have been read
           if (ok && seg > 0) ok = mbar_wait(o_free, (seg - 1) & 1, status, KF_ERR_WAIT_TMEM_EMPTY);
-          for (int i = 0; i < n && ok; ++i) {
-            const int g = i & 1, st = (first + i) % STAGES;
-            if (!mbar_wait(v_full(st), ((first + i) / STAGES) & 1, status, KF_ERR_WAIT_FULL)) { ok = false; break; }
+          for (int i = 0; i < n && ok; ++i, vt.next(stages)) {
+            const int g = i & 1, st = vt.st;
+            if (!mbar_wait(v_full(st), vt.phase, status, KF_ERR_WAIT_FULL)) { ok = false; break; }
             // O_g += P_g V: A = P from tensor memory, B = V with the head dim contiguous, in two halves of the keys
             if (!mbar_wait(p_half(g), done[g] & 1, status, KF_ERR_WAIT_TMEM_EMPTY)) { ok = false; break; }
             tc_fence_after();
@@ -286,11 +304,10 @@ kf_shared_prefix_tcgen05(const __grid_constant__ CUtensorMap map_q, const __grid
             if (i + 1 == n) tc_commit(o_final);
             // the group's next scores follow at once: the products just issued have read its P before they are written
             if (i + 2 < n) {
-              ok = issue_s(g, first + i + 2);
+              ok = issue_s(g);
               if (ok && i + 3 == n) tc_commit(q_empty);
             }
           }
-          first += n;
           ++seg;
           advance(lay, wk, n);
         }
@@ -323,14 +340,14 @@ kf_shared_prefix_tcgen05(const __grid_constant__ CUtensorMap map_q, const __grid
         tc_fence_after();
         if (n0 + TILE_KEYS > len && len < lay.P) {
           // positions behind the prompt hold anything, and 0 times that need not be 0: their values become zeros
-          const int st = (first + i) % STAGES;
-          if (ok && !mbar_wait(v_full(st), ((first + i) / STAGES) & 1, status, KF_ERR_WAIT_FULL)) ok = false;
+          const int st = (first + i) % stages;
+          if (ok && !mbar_wait(v_full(st), ((first + i) / stages) & 1, status, KF_ERR_WAIT_FULL)) ok = false;
           if (ok && n0 + row >= len) {
 #pragma unroll
             for (int c = 0; c < C::BLOCKS; ++c)
 #pragma unroll
               for (int e = 0; e < 8; ++e)
-                *reinterpret_cast<uint4*>(smem + (1 + STAGES + st) * C::TILE_BYTES + c * C::BLOCK_BYTES + row * 128 + e * 16) = make_uint4(0, 0, 0, 0);
+                *reinterpret_cast<uint4*>(smem + (1 + stages + st) * C::TILE_BYTES + c * C::BLOCK_BYTES + row * 128 + e * 16) = make_uint4(0, 0, 0, 0);
           }
           fence_async_smem();
         }
@@ -435,14 +452,14 @@ kf_shared_prefix_tcgen05(const __grid_constant__ CUtensorMap map_q, const __grid
           tmem_ld_wait();
           if (row < rows) {
 #pragma unroll
-            for (int k = 0; k < 32; k += 4) {
-              float v[4];
+            for (int k = 0; k < 32; k += 8) {
+              float v[8];
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
+              for (int e = 0; e < 8; ++e) {
                 v[e] = f0 * __uint_as_float(o0[k + e]);
                 if (n > 1) v[e] = __fmaf_rn(f1, __uint_as_float(o1[k + e]), v[e]);
               }
-              *reinterpret_cast<float4*>(dst + col + k) = make_float4(v[0], v[1], v[2], v[3]);
+              st_global_v8(dst + col + k, v);   // whole sectors: every lane writes a row of its own
             }
           }
         }
@@ -487,12 +504,23 @@ static int launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMa
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev >= 16 || !attr_set[dev]) {
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Cfg<HD>::SMEM);
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Cfg<HD>::smem(STAGES));
     if (e != cudaSuccess) return 300 + (int)e;
     if (dev < 16) attr_set[dev] = true;
   }
-  kern<<<(unsigned)l.ctas, THREADS, Cfg<HD>::SMEM, stream>>>(mq, mk, mv, l, group, scale * 1.4426950408889634f, part_o, part_ml, status);
-  cudaError_t e = cudaGetLastError();
+  const long long tiles = (long long)tiles_of(l.P) * l.per_prompt * l.B, each = (tiles + l.ctas - 1) / l.ctas;   // most tiles of a CTA
+  const int stages = each < STAGES ? (int)each : STAGES;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)l.ctas);
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = Cfg<HD>::smem(stages);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kern, mq, mk, mv, l, group, stages, scale * 1.4426950408889634f, part_o, part_ml, status);
   return e == cudaSuccess ? 0 : 400 + (int)e;
 }
 

@@ -1097,7 +1097,7 @@ def shared_prefix_call(q, k, v, own_k, own_v, prefix_lens, own_rows, scale) -> t
 
 def shared_prefix_supported(q: torch.Tensor, k: torch.Tensor) -> bool:
     b, w, h, hd = q.shape
-    return hd in (64, 128) and h // k.shape[2] <= 128 and b * w * h < 2**27 and k.shape[1] < 2**31 - 2**16
+    return k.shape[1] < 2**31 - 2**16 and b * w * h < 2**27 and lib().kf_shared_prefix_scratch(b, w, k.shape[1], h, k.shape[2], hd, sm_count()) >= 0
 
 
 def shared_prefix_attn(q, k, v, own_k, own_v, prefix_lens, own_rows, scale: float) -> torch.Tensor:
