@@ -239,25 +239,29 @@ kf_shared_prefix_own(const Own a, const Layout lay, const float* part_o, const f
   float top = -INFINITY, sum = 0.f;
   {
     const int r = lane / lanes, sub = lane % lanes;
+    auto join = [&](float x, float y) {
+      const float higher = fmaxf(top, x);
+      sum = sum * weight(top, higher) + y * weight(x, higher);
+      top = higher;
+    };
     if (r < n_heads) {
-      for (int s = sub; s < ways + parts; s += lanes) {
-        float2 x;
-        if (s < ways) {
-          const uint32_t at = own_at(stats_a + r * 8, s, OWN_ROWS * 8);
-          x = make_float2(ld_cluster_f1(at), ld_cluster_f1(at + 4));
-        } else {
-          x = ld_after_wait(part_ml + slot0 + r + (long long)(s - ways) * TILE_ROWS);
-        }
-        const float higher = fmaxf(top, x.x);
-        sum = sum * weight(top, higher) + x.y * weight(x.x, higher);
-        top = higher;
+      for (int c = sub; c < parts; c += 4 * lanes) {
+        float2 x[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (c + e * lanes < parts) x[e] = ld_after_wait(part_ml + slot0 + r + (long long)(c + e * lanes) * TILE_ROWS);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (c + e * lanes < parts) join(x[e].x, x[e].y);
+      }
+      for (int s = sub; s < ways; s += lanes) {
+        const uint32_t at = own_at(stats_a + r * 8, s, OWN_ROWS * 8);
+        join(ld_cluster_f1(at), ld_cluster_f1(at + 4));
       }
     }
     for (int o = lanes / 2; o > 0; o >>= 1) {
       const float x = __shfl_xor_sync(0xffffffffu, top, o), y = __shfl_xor_sync(0xffffffffu, sum, o);
-      const float higher = fmaxf(top, x);
-      sum = sum * weight(top, higher) + y * weight(x, higher);
-      top = higher;
+      join(x, y);
     }
   }
   // ---- each warp of the unit its share of the output
@@ -267,7 +271,7 @@ kf_shared_prefix_own(const Own a, const Layout lay, const float* part_o, const f
     if (r >= n_heads) continue;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     auto add = [&](float f, const float4& v) { acc.x += f * v.x; acc.y += f * v.y; acc.z += f * v.z; acc.w += f * v.w; };
-    constexpr int AT_ONCE = 4;
+    constexpr int AT_ONCE = 8;
     const float2* ml = part_ml + slot0 + r;
     const float4* po = reinterpret_cast<const float4*>(part_o + (slot0 + r) * HD + d);
     for (int c = 0; c < parts; c += AT_ONCE) {
