@@ -3,15 +3,16 @@
 // What a continuation has written itself is its own, so these keys are read by its group of query heads only: a stream as in the generation
 // step of single sequences.  In a beam search the cache of a continuation does not move when beams are exchanged; own_rows says in whose
 // cache each position lies.  Beams share most of their ancestors, so most of these keys come out of L2 for all beams but the first.
-//   * a unit is a continuation's key head; its query heads are the 16 rows of an m16n8k16 MMA, its keys are dealt out to 1 to 32 warps, as
-//     many as it takes to have eight warps on every SM: few units need all of them for one, many (a batch of short continuations) one each;
+//   * a unit is a continuation's key head; its query heads are the 16 rows of an m16n8k16 MMA, its keys are dealt out to 1 to 32 warps:
+//     few units need many warps for one, many (a batch of short continuations) one each;
 //   * every warp streams tiles of 16 keys through a cp.async ring of its own, two tiles ahead, without a barrier; 16-byte chunks are
-//     XOR-swizzled, so that ldmatrix is free of bank conflicts; where there is a warp for every tile, the ring is one tile, and the CTAs are
-//     small enough to run beside those of the prompt's kernel;
+//     XOR-swizzled, so that ldmatrix is free of bank conflicts; a warp of one or two tiles has them all under way at once;
 //   * the (max, sum, output) triples of the warps, of the CTAs of a cluster and of the prompt are joined in a fixed order.
 // All of it up to that last step runs without the prompt's kernel, and starts on the SMs that it leaves (programmatic launch).
 #include "decode_common.cuh"
 #include "shared_prefix.cuh"
+
+#include <type_traits>
 
 namespace kf {
 namespace shared_prefix {
@@ -22,11 +23,14 @@ constexpr int OWN_WARPS = 4, OWN_THREADS = OWN_WARPS * 32;
 constexpr int OWN_TILE = 16;       // keys per ring stage of a warp
 constexpr int OWN_ROWS = 16;       // query heads per unit (MMA rows)
 
-// ONE: a warp has one tile at most.  Else its ring has 24 KB: two CTAs an SM, 128 KB of it under way.
-template <int HD, bool ONE>
+// RING: tiles in a warp's ring, up to which it has them all under way at once.  0: it streams through 24 KB (two CTAs an SM, 128 KB of it
+// under way).
+template <int HD, int RING_TILES>
 struct OwnCfg {
   static constexpr int TILE_BYTES = OWN_TILE * HD * 2;
-  static constexpr int STAGES = ONE ? 1 : (24 << 10) / (2 * TILE_BYTES);   // 3 for a head dim of 128, 6 for 64
+  static constexpr bool STREAM = RING_TILES == 0;
+  static constexpr int STAGES = STREAM ? (24 << 10) / (2 * TILE_BYTES) : RING_TILES;   // 3 for a head dim of 128, 6 for 64
+  static constexpr int AHEAD = STREAM ? STAGES - 1 : STAGES;         // tiles under way before the first is read
   static constexpr int RING = STAGES * 2 * TILE_BYTES;
   static constexpr int PART = OWN_ROWS * HD * 4;                     // a warp's partial output, over its ring
   static_assert(PART <= RING, "");
@@ -46,10 +50,10 @@ struct Own {
 };
 
 // WPU: warps of a CTA that share a unit.  Clusters of more than one CTA (WPU = 4) share one too.
-template <int HD, int WPU, bool ONE>
+template <int HD, int WPU, int RING_TILES>
 __global__ void __launch_bounds__(OWN_THREADS)
 kf_shared_prefix_own(const Own a, const Layout lay, const float* part_o, const float2* part_ml, const uint32_t units) {
-  using C = OwnCfg<HD, ONE>;
+  using C = OwnCfg<HD, RING_TILES>;
   extern __shared__ __align__(128) uint8_t smem_raw[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int splits = WPU == OWN_WARPS ? int(cluster_nctaid()) : 1, rank = WPU == OWN_WARPS ? int(cluster_ctarank()) : 0;
@@ -101,13 +105,6 @@ kf_shared_prefix_own(const Own a, const Layout lay, const float* part_o, const f
     }
   };
   int slot = slot_of(t0);
-  for (int t = t0; t < t0 + max(1, C::STAGES - 1); ++t) {
-    const int after = ONE ? 0 : slot_of(t + 1);
-    if (t < t1) issue(t, slot);
-    cp_commit();
-    slot = after;
-  }
-
   // query rows as MMA A fragments (rows past the group are zero)
   uint32_t qa[HD / 16][4];
   {
@@ -122,15 +119,22 @@ kf_shared_prefix_own(const Own a, const Layout lay, const float* part_o, const f
       qa[kk][3] = g + 8 < n_heads ? *reinterpret_cast<const uint32_t*>(q1 + kk * 16 + 8 + c) : 0u;
     }
   }
+  for (int t = t0; t < t0 + C::AHEAD; ++t) {
+    const int after = slot_of(t + 1);
+    if (t < t1) issue(t, slot);
+    cp_commit();
+    slot = after;
+  }
+
   float o[HD / 8][4];
 #pragma unroll
   for (int i = 0; i < HD / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 
   for (int t = t0; t < t1; ++t) {
-    cp_wait<ONE ? 0 : C::STAGES - 2>();
+    cp_wait<C::STREAM ? C::STAGES - 2 : 0>();
     __syncwarp();   // tile t has landed for every lane, and the stage refilled below has been consumed
-    if (!ONE) {
+    if (C::STREAM) {
       const int after = slot_of(t + C::STAGES);
       if (t + C::STAGES - 1 < t1) issue(t + C::STAGES - 1, slot);
       cp_commit();
@@ -234,59 +238,50 @@ kf_shared_prefix_own(const Own a, const Layout lay, const float* part_o, const f
     const uint32_t at = base + (s % WPU) * step;
     return splits > 1 ? mapa_shared(at, s / WPU) : at;
   };
-  // ---- each row's largest score and sum: a few lanes a row, each some of the warps and of the prompt's parts
-  const int spread = n_heads <= 1 ? 1 : 1 << (32 - __clz(n_heads - 1)), lanes = 32 / spread;
-  float top = -INFINITY, sum = 0.f;
-  {
-    const int r = lane / lanes, sub = lane % lanes;
-    auto join = [&](float x, float y) {
-      const float higher = fmaxf(top, x);
-      sum = sum * weight(top, higher) + y * weight(x, higher);
-      top = higher;
-    };
-    if (r < n_heads) {
-      for (int c = sub; c < parts; c += 4 * lanes) {
-        float2 x[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (c + e * lanes < parts) x[e] = ld_after_wait(part_ml + slot0 + r + (long long)(c + e * lanes) * TILE_ROWS);
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (c + e * lanes < parts) join(x[e].x, x[e].y);
-      }
-      for (int s = sub; s < ways; s += lanes) {
-        const uint32_t at = own_at(stats_a + r * 8, s, OWN_ROWS * 8);
-        join(ld_cluster_f1(at), ld_cluster_f1(at + 4));
-      }
-    }
-    for (int o = lanes / 2; o > 0; o >>= 1) {
-      const float x = __shfl_xor_sync(0xffffffffu, top, o), y = __shfl_xor_sync(0xffffffffu, sum, o);
-      join(x, y);
-    }
-  }
-  // ---- each warp of the unit its share of the output
-  for (int base = way * 32; base < n_heads * (HD / 4); base += ways * 32) {
-    const int i = base + lane, r = i / (HD / 4), d = (i % (HD / 4)) * 4;
-    const float row_top = __shfl_sync(0xffffffffu, top, (r * lanes) & 31), row_sum = __shfl_sync(0xffffffffu, sum, (r * lanes) & 31);
-    if (r >= n_heads) continue;
+  // ---- each warp of the unit its share of the output: a lane four values of a row, over the prompt's parts and the unit's warps
+  for (int i = way * 32 + lane; i < n_heads * (HD / 4); i += ways * 32) {
+    const int r = i / (HD / 4), d = (i % (HD / 4)) * 4;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    auto add = [&](float f, const float4& v) { acc.x += f * v.x; acc.y += f * v.y; acc.z += f * v.z; acc.w += f * v.w; };
+    float top = -INFINITY, sum = 0.f;
     constexpr int AT_ONCE = 8;
+    float2 x[AT_ONCE];
+    float4 v[AT_ONCE];
+    auto join = [&](int n) {   // the first n of them
+      float higher = top;
+#pragma unroll
+      for (int e = 0; e < AT_ONCE; ++e)
+        if (e < n) higher = fmaxf(higher, x[e].x);
+      const float f = weight(top, higher);
+      acc.x *= f; acc.y *= f; acc.z *= f; acc.w *= f;
+      sum *= f;
+      top = higher;
+#pragma unroll
+      for (int e = 0; e < AT_ONCE; ++e)
+        if (e < n) {
+          const float g = weight(x[e].x, top);
+          acc.x += g * v[e].x; acc.y += g * v[e].y; acc.z += g * v[e].z; acc.w += g * v[e].w;
+          sum += g * x[e].y;
+        }
+    };
     const float2* ml = part_ml + slot0 + r;
     const float4* po = reinterpret_cast<const float4*>(part_o + (slot0 + r) * HD + d);
     for (int c = 0; c < parts; c += AT_ONCE) {
-      float2 x[AT_ONCE];
-      float4 v[AT_ONCE];
 #pragma unroll
       for (int e = 0; e < AT_ONCE; ++e)
         if (c + e < parts) x[e] = ld_after_wait(ml + (long long)(c + e) * TILE_ROWS), v[e] = ld_after_wait(po + (long long)(c + e) * TILE_ROWS * (HD / 4));
+      join(parts - c);
+    }
+    for (int s = 0; s < ways; s += AT_ONCE) {
 #pragma unroll
       for (int e = 0; e < AT_ONCE; ++e)
-        if (c + e < parts) add(weight(x[e].x, row_top), v[e]);
+        if (s + e < ways) {
+          const uint32_t at = own_at(stats_a + r * 8, s + e, OWN_ROWS * 8);
+          x[e] = make_float2(ld_cluster_f1(at), ld_cluster_f1(at + 4));
+          v[e] = ld_cluster_f4(own_at(part_a + uint32_t(r * HD + d) * 4u, s + e, C::RING));
+        }
+      join(ways - s);
     }
-    for (int s = 0; s < ways; ++s)
-      add(weight(ld_cluster_f1(own_at(stats_a + r * 8, s, OWN_ROWS * 8)), row_top), ld_cluster_f4(own_at(part_a + uint32_t(r * HD + d) * 4u, s, C::RING)));
-    const float inv = row_sum == 0.f ? 0.f : 1.f / row_sum;   // nothing visible: zeros
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;   // nothing visible: zeros
     uint2 out;
     out.x = pack_bf16(acc.x * inv, acc.y * inv);
     out.y = pack_bf16(acc.z * inv, acc.w * inv);
@@ -295,10 +290,10 @@ kf_shared_prefix_own(const Own a, const Layout lay, const float* part_o, const f
   if (splits > 1) cluster_sync_all();   // no CTA leaves while another reads its shared memory
 }
 
-template <int HD, int WPU, bool ONE>
+template <int HD, int WPU, int RING_TILES>
 static int launch_ways(const Own& a, const Layout& l, const float* part_o, const float2* part_ml, long long units, int splits, cudaStream_t stream) {
-  using C = OwnCfg<HD, ONE>;
-  auto kern = kf_shared_prefix_own<HD, WPU, ONE>;
+  using C = OwnCfg<HD, RING_TILES>;
+  auto kern = kf_shared_prefix_own<HD, WPU, RING_TILES>;
   static bool attr_set[16] = {};
   int dev = 0;
   cudaGetDevice(&dev);
@@ -330,21 +325,25 @@ static int launch_ways(const Own& a, const Layout& l, const float* part_o, const
 template <int HD>
 static int launch_own(const Own& a, const Layout& l, const float* part_o, const float2* part_ml, int num_sms, cudaStream_t stream) {
   const long long units = (long long)l.B * l.W * a.Hkv * ((a.group + OWN_ROWS - 1) / OWN_ROWS);
-  // A warp for every tile where that leaves no more than 24 on an SM, which is what its memory holds of them; else as many warps a unit as
-  // fill eight on every SM, of which each has a tile at least.
   const int tiles = (a.S + OWN_TILE - 1) / OWN_TILE;
-  int ways = 1;
-  while (ways < tiles && ways < 32) ways *= 2;
-  if (ways >= tiles && units * ways <= 24LL * num_sms) {
-    if (ways == 1) return launch_ways<HD, 1, true>(a, l, part_o, part_ml, units, 1, stream);
-    if (ways == 2) return launch_ways<HD, 2, true>(a, l, part_o, part_ml, units, 1, stream);
-    return launch_ways<HD, 4, true>(a, l, part_o, part_ml, units, ways / 4, stream);
+  auto go = [&](auto ring, int ways) {
+    constexpr int R = decltype(ring)::value;
+    if (ways == 1) return launch_ways<HD, 1, R>(a, l, part_o, part_ml, units, 1, stream);
+    if (ways == 2) return launch_ways<HD, 2, R>(a, l, part_o, part_ml, units, 1, stream);
+    return launch_ways<HD, 4, R>(a, l, part_o, part_ml, units, ways / 4, stream);
+  };
+  // One or two tiles a warp, where that takes a CTA a unit at most and no more than 16 warps on an SM, which is what registers and
+  // memory hold: everything is under way at once, and nothing crosses CTAs (8 x 5 continuations of 65 keys: 27.2 -> 23 us, 1 x 8 of 96
+  // 15.6 -> 13).  Else as many warps a unit as fill eight on every SM, of which each has a tile at least.
+  for (int ring = 1; ring <= 2; ++ring) {
+    int ways = 1;
+    while (ways < 4 && ways * ring < tiles) ways *= 2;
+    if (ways * ring >= tiles && units * ways <= 16LL * num_sms)
+      return ring == 1 ? go(std::integral_constant<int, 1>(), ways) : go(std::integral_constant<int, 2>(), ways);
   }
-  ways = 1;
+  int ways = 1;
   while (ways < 32 && units * ways * 2 <= 8LL * num_sms && tiles >= ways * 2) ways *= 2;
-  if (ways == 1) return launch_ways<HD, 1, false>(a, l, part_o, part_ml, units, 1, stream);
-  if (ways == 2) return launch_ways<HD, 2, false>(a, l, part_o, part_ml, units, 1, stream);
-  return launch_ways<HD, 4, false>(a, l, part_o, part_ml, units, ways / 4, stream);
+  return go(std::integral_constant<int, 0>(), ways);
 }
 
 int launch_prefix(const void* q, const void* k, const void* v, const Layout& l, int H, int Hkv, int hd, const long long* qs, const long long* ks,

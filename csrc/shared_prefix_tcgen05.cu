@@ -4,8 +4,8 @@
 // once for all and S = Q K^T and O += P V are 128-row products on the tensor cores; one kernel per continuation reads it W times.
 // What bounds it: the keys and values, 4 hd bytes per position and head.  A tile of 128 keys of 128 values is 64 KB, which is 2700 cycles
 // of an SM's share of HBM; its two products take 512, its 16 384 exponentials 1024.  So rows that are not there (a tile is always 128)
-// cost nothing, and all that counts is to keep the copies in flight: three stages each of K and V (192 KB) run ahead of the products.
-// A CTA of one or two tiles takes only their memory, and leaves the rest of its SM to the second kernel, which starts meanwhile.
+// cost nothing, and all that counts is to keep the copies in flight: two stages each of K and V (128 KB) run ahead of the products.  Three
+// were slower (4 x 32 768 keys, 64 heads of 128, with the second kernel: 102 and 98 us).
 //
 //   warp 0     : TMA producer of Q and K
 //   warp 1     : MMA issuer
@@ -29,7 +29,6 @@ using namespace kf::attn;
 constexpr int THREADS = 384;
 constexpr int REGS_ISSUE = 72, REGS_SOFTMAX = 216;  // per thread; 72 + 2 * 216 = 3 * 168, what the launch gets
 constexpr int TMEM_COLS = 512;
-constexpr int STAGES = 3;                           // of K and of V at most; a CTA with fewer tiles takes less memory
 constexpr float RESCALE_THRESHOLD = 8.0f;           // P up to 2^8 before the accumulator is scaled again
 
 template <int HD>
@@ -37,6 +36,7 @@ struct Cfg {
   static constexpr int BLOCKS = HD / 64;
   static constexpr int TILE_BYTES = TILE_KEYS * HD * 2;
   static constexpr int BLOCK_BYTES = TILE_KEYS * 128;
+  static constexpr int STAGES = HD == 128 ? 2 : 3;  // of K and of V at most; a CTA with fewer tiles takes less memory
   static constexpr int STATS = 2 * TILE_ROWS * 8;   // (max, sum) of each group's rows
   static constexpr int HEAD = 3 * 1024;             // STATS and the barriers, before the tiles, which start on 1024 bytes
   static constexpr size_t smem(int stages) { return HEAD + (1 + 2 * size_t(stages)) * TILE_BYTES; }   // Q, K ring, V ring: up to 227 KB
@@ -156,7 +156,7 @@ kf_shared_prefix_tcgen05(const __grid_constant__ CUtensorMap map_q, const __grid
   const int warp = warp_index();
   const int lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < STAGES; ++i) {
+    for (int i = 0; i < 3; ++i) {
       mbar_init(k_full(i), 1);
       mbar_init(k_empty(i), 1);
       mbar_init(v_full(i), 1);
@@ -504,12 +504,12 @@ static int launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMa
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev >= 16 || !attr_set[dev]) {
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Cfg<HD>::smem(STAGES));
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Cfg<HD>::smem(Cfg<HD>::STAGES));
     if (e != cudaSuccess) return 300 + (int)e;
     if (dev < 16) attr_set[dev] = true;
   }
   const long long tiles = (long long)tiles_of(l.P) * l.per_prompt * l.B, each = (tiles + l.ctas - 1) / l.ctas;   // most tiles of a CTA
-  const int stages = each < STAGES ? (int)each : STAGES;
+  const int stages = each < Cfg<HD>::STAGES ? (int)each : Cfg<HD>::STAGES;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)l.ctas);
   cfg.blockDim = dim3(THREADS);
