@@ -33,10 +33,10 @@ struct OwnCfg {
   static constexpr int AHEAD = STREAM ? STAGES - 1 : STAGES;         // tiles under way before the first is read
   static constexpr int RING = STAGES * 2 * TILE_BYTES;
   static constexpr int PART = OWN_ROWS * HD * 4;                     // a warp's partial output, over its ring
-  static_assert(PART <= RING, "");
-  static constexpr int STATS = OWN_WARPS * OWN_ROWS * 2 * 4;         // (max, sum) per warp and row
-  static constexpr int SEEN = OWN_WARPS * 8 * 4;                     // per stage: which of its keys are visible
-  static constexpr size_t SMEM = size_t(OWN_WARPS) * RING + STATS + SEEN;
+  static constexpr int STATS = OWN_ROWS * 2 * 4;                     // (max, sum) of its rows, behind it
+  static constexpr int SEEN = STREAM ? OWN_WARPS * 8 * 4 : 0;        // per stage: which of its keys are visible
+  static constexpr int WARP = RING > PART + STATS ? RING : PART + STATS;
+  static constexpr size_t SMEM = size_t(OWN_WARPS) * WARP + SEEN;
 };
 
 struct Own {
@@ -51,16 +51,15 @@ struct Own {
 
 // WPU: warps of a CTA that share a unit.  Clusters of more than one CTA (WPU = 4) share one too.
 template <int HD, int WPU, int RING_TILES>
-__global__ void __launch_bounds__(OWN_THREADS)
+__global__ void __launch_bounds__(OWN_THREADS, RING_TILES == 0 ? 3 : 4)   // 4: 128 registers, so that more CTAs fit
 kf_shared_prefix_own(const Own a, const Layout lay, const float* part_o, const float2* part_ml, const uint32_t units) {
   using C = OwnCfg<HD, RING_TILES>;
   extern __shared__ __align__(128) uint8_t smem_raw[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int splits = WPU == OWN_WARPS ? int(cluster_nctaid()) : 1, rank = WPU == OWN_WARPS ? int(cluster_ctarank()) : 0;
   const int way = rank * WPU + warp % WPU, ways = splits * WPU;     // which share of the unit's keys
-  const uint32_t ring = smem_u32(smem_raw) + warp * C::RING;
-  float* stats = reinterpret_cast<float*>(smem_raw + OWN_WARPS * C::RING);                            // [warp][row][2]
-  volatile uint32_t* seen = reinterpret_cast<uint32_t*>(smem_raw + OWN_WARPS * C::RING + C::STATS) + warp * 8;
+  const uint32_t ring = smem_u32(smem_raw) + warp * C::WARP;
+  volatile uint32_t* seen = reinterpret_cast<uint32_t*>(smem_raw + OWN_WARPS * C::WARP) + warp * 8;
 
   const uint32_t unit0 = blockIdx.x / uint32_t(splits) * (OWN_WARPS / WPU) + warp / WPU;
   const bool there = unit0 < units;
@@ -81,30 +80,40 @@ kf_shared_prefix_own(const Own a, const Layout lay, const float* part_o, const f
   const __nv_bfloat16* vb = a.v + b * a.v_b + hk * a.v_h;
   const uint8_t* table = a.rows ? a.rows + b * a.r_b + w * a.r_w : nullptr;
 
-  constexpr int CHUNKS = HD / 8;                        // 16-byte chunks per row
-  // whose cache holds the lane's key of tile t (lay.W: nobody's)
-  auto slot_of = [&](int t) {
-    const int pos = t * OWN_TILE + (lane & 15);
-    return t >= t1 || pos >= a.S ? lay.W : table ? int(table[pos]) : w;
+  // whose cache holds the lane's key of the two tiles from t on (lay.W: nobody's)
+  auto slots_of = [&](int t) {
+    const int pos = t * OWN_TILE + lane;
+    return t + (lane >> 4) >= t1 || pos >= a.S ? lay.W : table ? int(table[pos]) : w;
   };
-  auto issue = [&](int t, int slot) {
-    const int st = (t - t0) % C::STAGES;
+  int slots = slots_of(t0), ahead = t0 + 2 < t1 ? slots_of(t0 + 2) : lay.W;   // of the tiles issued next and the two after them
+  // Four lanes a key: 64 bytes side by side at a time, of keys lane / 4 and that + 8.  The 16-byte chunk c of row r lies at c ^ (r & 7).
+  const int row0 = lane >> 2;
+  const uint32_t dst0 = uint32_t(row0 * HD * 2 + (((lane & 3) ^ row0) << 4));   // bit 6 of it turned over by row0's bit 2
+  uint32_t masks[C::STREAM ? 1 : C::STAGES];
+  auto issue = [&](int t) {
+    const int st = (t - t0) % C::STAGES, half = ((t - t0) & 1) * 16;
     const uint32_t ks = ring + uint32_t(st) * 2u * C::TILE_BYTES, vs = ks + C::TILE_BYTES;
-    const uint32_t mask = __ballot_sync(0xffffffffu, slot < lay.W);
-    if (lane == 0) seen[st] = mask;
+    const uint32_t mask = __ballot_sync(0xffffffffu, slots < lay.W) >> half;
+    if (!C::STREAM) masks[st % (C::STREAM ? 1 : C::STAGES)] = mask;
+    else if (lane == 0) seen[st] = mask;
 #pragma unroll
-    for (int i = 0; i < OWN_TILE * CHUNKS / 32; ++i) {
-      const int idx = lane + i * 32, r = idx / CHUNKS, c = idx % CHUNKS;
-      const int sl = __shfl_sync(0xffffffffu, slot, r);
+    for (int h = 0; h < 2; ++h) {
+      const int r = row0 + h * 8, sl = __shfl_sync(0xffffffffu, slots, half + r);
       const bool in = (mask >> r) & 1u;
-      const long long pos = t * OWN_TILE + r;
-      const long long ko = in ? sl * a.k_w + pos * a.k_s + c * 8 : 0, vo = in ? sl * a.v_w + pos * a.v_s + c * 8 : 0;
-      const uint32_t dst = uint32_t(r * HD * 2 + ((c ^ (r & 7)) << 4));
-      cp_async16(ks + dst, kb + ko, in);
-      cp_async16(vs + dst, vb + vo, in);
+      const long long pos = in ? t * OWN_TILE + r : 0, of = in ? sl : 0;
+      const __nv_bfloat16 *kp = kb + of * a.k_w + pos * a.k_s + (lane & 3) * 8, *vp = vb + of * a.v_w + pos * a.v_s + (lane & 3) * 8;
+#pragma unroll
+      for (int c = 0; c < HD / 32; ++c) {
+        const uint32_t dst = (dst0 ^ uint32_t(c * 64)) + uint32_t(h * 8 * HD * 2);
+        cp_async16(ks + dst, kp + c * 32, in);
+        cp_async16(vs + dst, vp + c * 32, in);
+      }
+    }
+    if (half) {
+      slots = ahead;
+      ahead = t + 3 < t1 ? slots_of(t + 3) : lay.W;
     }
   };
-  int slot = slot_of(t0);
   // query rows as MMA A fragments (rows past the group are zero)
   uint32_t qa[HD / 16][4];
   {
@@ -119,11 +128,10 @@ kf_shared_prefix_own(const Own a, const Layout lay, const float* part_o, const f
       qa[kk][3] = g + 8 < n_heads ? *reinterpret_cast<const uint32_t*>(q1 + kk * 16 + 8 + c) : 0u;
     }
   }
-  for (int t = t0; t < t0 + C::AHEAD; ++t) {
-    const int after = slot_of(t + 1);
-    if (t < t1) issue(t, slot);
+#pragma unroll
+  for (int i = 0; i < C::AHEAD; ++i) {
+    if (t0 + i < t1) issue(t0 + i);
     cp_commit();
-    slot = after;
   }
 
   float o[HD / 8][4];
@@ -131,16 +139,17 @@ kf_shared_prefix_own(const Own a, const Layout lay, const float* part_o, const f
   for (int i = 0; i < HD / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 
-  for (int t = t0; t < t1; ++t) {
+#pragma unroll(C::STREAM ? 1 : C::STAGES)
+  for (int i = 0; i < (C::STREAM ? t1 - t0 : C::STAGES); ++i) {
+    const int t = t0 + i;
+    if (t >= t1) break;
     cp_wait<C::STREAM ? C::STAGES - 2 : 0>();
     __syncwarp();   // tile t has landed for every lane, and the stage refilled below has been consumed
     if (C::STREAM) {
-      const int after = slot_of(t + C::STAGES);
-      if (t + C::STAGES - 1 < t1) issue(t + C::STAGES - 1, slot);
+      if (t + C::STAGES - 1 < t1) issue(t + C::STAGES - 1);
       cp_commit();
-      slot = after;
     }
-    const int st = (t - t0) % C::STAGES;
+    const int st = C::STREAM ? i % C::STAGES : i;
     const uint32_t ks = ring + uint32_t(st) * 2u * C::TILE_BYTES, vs = ks + C::TILE_BYTES;
     const int mi = lane >> 3, lr = lane & 7;
     float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
@@ -154,7 +163,7 @@ kf_shared_prefix_own(const Own a, const Layout lay, const float* part_o, const f
         mma16816(s[1], qa[kk], f[2], f[3]);
       }
     }
-    const uint32_t sees = seen[st] >> ((lane & 3) * 2);
+    const uint32_t sees = (C::STREAM ? seen[st] : masks[st % (C::STREAM ? 1 : C::STAGES)]) >> ((lane & 3) * 2);
 #pragma unroll
     for (int n = 0; n < 2; ++n)
 #pragma unroll
@@ -199,7 +208,7 @@ kf_shared_prefix_own(const Own a, const Layout lay, const float* part_o, const f
   }
   cp_wait<0>();
   __syncwarp();  // the ring is idle: the warp's partial result takes its place
-  float* part = reinterpret_cast<float*>(smem_raw + warp * C::RING);
+  float *part = reinterpret_cast<float*>(smem_raw + warp * C::WARP), *stats = part + C::PART / 4;
 #pragma unroll
   for (int hf = 0; hf < 2; ++hf) {
     l[hf] += __shfl_xor_sync(0xffffffffu, l[hf], 1);
@@ -207,8 +216,8 @@ kf_shared_prefix_own(const Own a, const Layout lay, const float* part_o, const f
     const int r = (lane >> 2) + hf * 8;
     if (r < n_heads) {
       if ((lane & 3) == 0) {
-        stats[(warp * OWN_ROWS + r) * 2] = m[hf];
-        stats[(warp * OWN_ROWS + r) * 2 + 1] = l[hf];
+        stats[r * 2] = m[hf];
+        stats[r * 2 + 1] = l[hf];
       }
       float* dst = part + r * HD + (lane & 3) * 2;
 #pragma unroll
@@ -233,9 +242,9 @@ kf_shared_prefix_own(const Own a, const Layout lay, const float* part_o, const f
   grid_dep_launch();
   const long long slot0 = ((long long)b * lay.per_prompt + u + c0) * TILE_ROWS + (w % lay.wt) * a.group + hb * OWN_ROWS;
   const int warp0 = warp / WPU * WPU;
-  const uint32_t stats_a = smem_u32(stats + warp0 * OWN_ROWS * 2), part_a = smem_u32(smem_raw) + warp0 * C::RING;
-  auto own_at = [&](uint32_t base, int s, int step) {   // of the unit's s-th warp
-    const uint32_t at = base + (s % WPU) * step;
+  const uint32_t part_a = smem_u32(smem_raw) + warp0 * C::WARP, stats_a = part_a + C::PART;
+  auto own_at = [&](uint32_t base, int s) {   // of the unit's s-th warp
+    const uint32_t at = base + (s % WPU) * C::WARP;
     return splits > 1 ? mapa_shared(at, s / WPU) : at;
   };
   // ---- each warp of the unit its share of the output: a lane four values of a row, over the prompt's parts and the unit's warps
@@ -275,9 +284,9 @@ kf_shared_prefix_own(const Own a, const Layout lay, const float* part_o, const f
 #pragma unroll
       for (int e = 0; e < AT_ONCE; ++e)
         if (s + e < ways) {
-          const uint32_t at = own_at(stats_a + r * 8, s + e, OWN_ROWS * 8);
+          const uint32_t at = own_at(stats_a + r * 8, s + e);
           x[e] = make_float2(ld_cluster_f1(at), ld_cluster_f1(at + 4));
-          v[e] = ld_cluster_f4(own_at(part_a + uint32_t(r * HD + d) * 4u, s + e, C::RING));
+          v[e] = ld_cluster_f4(own_at(part_a + uint32_t(r * HD + d) * 4u, s + e));
         }
       join(ways - s);
     }
@@ -299,6 +308,8 @@ static int launch_ways(const Own& a, const Layout& l, const float* part_o, const
   cudaGetDevice(&dev);
   if (dev >= 16 || !attr_set[dev]) {
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::SMEM);
+    // all of the SM's memory as shared memory: CTAs of both kernels side by side
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
     if (e != cudaSuccess) return 300 + (int)e;
     if (dev < 16) attr_set[dev] = true;
   }

@@ -6,6 +6,9 @@
 // of an SM's share of HBM; its two products take 512, its 16 384 exponentials 1024.  So rows that are not there (a tile is always 128)
 // cost nothing, and all that counts is to keep the copies in flight: two stages each of K and V (128 KB) run ahead of the products.  Three
 // were slower (4 x 32 768 keys, 64 heads of 128, with the second kernel: 102 and 98 us).
+// Where a CTA has two tiles at most, what counts is that the second kernel does its own part meanwhile, beside it on the same SM: LEAN, in 96
+// registers a thread, with scores taken from tensor memory twice, 32 at a time, for the maximum and for the exponentials, and at most
+// 162 KB.  1 x 8 x 4000: 14.2 -> 11.7 us; but 24 x 8 x 512 (three tiles) 15.9 -> 16.4, 2 x 64 x 8000 59 -> 66.
 //
 //   warp 0     : TMA producer of Q and K
 //   warp 1     : MMA issuer
@@ -28,6 +31,8 @@ using namespace kf::attn;
 
 constexpr int THREADS = 384;
 constexpr int REGS_ISSUE = 72, REGS_SOFTMAX = 216;  // per thread; 72 + 2 * 216 = 3 * 168, what the launch gets
+constexpr int LEAN_BOUND = 608;                     // threads that a block might have: 96 registers each
+constexpr int LEAN_TILES = 2;
 constexpr int TMEM_COLS = 512;
 constexpr float RESCALE_THRESHOLD = 8.0f;           // P up to 2^8 before the accumulator is scaled again
 
@@ -37,9 +42,9 @@ struct Cfg {
   static constexpr int TILE_BYTES = TILE_KEYS * HD * 2;
   static constexpr int BLOCK_BYTES = TILE_KEYS * 128;
   static constexpr int STAGES = HD == 128 ? 2 : 3;  // of K and of V at most; a CTA with fewer tiles takes less memory
-  static constexpr int STATS = 2 * TILE_ROWS * 8;   // (max, sum) of each group's rows
-  static constexpr int HEAD = 3 * 1024;             // STATS and the barriers, before the tiles, which start on 1024 bytes
-  static constexpr size_t smem(int stages) { return HEAD + (1 + 2 * size_t(stages)) * TILE_BYTES; }   // Q, K ring, V ring: up to 227 KB
+  static constexpr int STATS = 3 * TILE_ROWS * 4;   // each group's maxima, the odd one's sums
+  // Q, K ring, V ring, STATS, barriers: up to 162 KB, which leaves 64 KB for a CTA of the second kernel
+  static constexpr size_t smem(int stages) { return (1 + 2 * size_t(stages)) * TILE_BYTES + STATS + 256; }
 };
 
 // Where a CTA is in its range.
@@ -123,22 +128,22 @@ __device__ __forceinline__ void st_global_v8(float* p, const float (&v)[8]) {
                : "memory");
 }
 
-template <int HD>
-__global__ void __launch_bounds__(THREADS, 1)
+template <int HD, bool LEAN>
+__global__ void __launch_bounds__(LEAN ? LEAN_BOUND : THREADS, 1)
 kf_shared_prefix_tcgen05(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                          const __grid_constant__ CUtensorMap map_v, const Layout lay, int group, int stages, float scale_log2,
                          float* __restrict__ part_o, float2* __restrict__ part_ml, int* status) {
   using C = Cfg<HD>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  const uint32_t smem_base = smem_u32(smem_raw) + C::HEAD;
-  uint8_t* smem = smem_raw + C::HEAD;
+  const uint32_t smem_base = smem_u32(smem_raw);
+  uint8_t* smem = smem_raw;
   if (smem_base & 1023u) {   // not as declared: nothing is touched
     if (threadIdx.x == 0) atomicCAS(status, 0, int(KF_ERR_WAIT_DRAIN));
     return;
   }
   const uint32_t q_smem = smem_base, k_smem = q_smem + C::TILE_BYTES, v_smem = k_smem + stages * C::TILE_BYTES;
-  float2* stats = reinterpret_cast<float2*>(smem_raw);
-  uint8_t* bar_generic = smem_raw + C::STATS;
+  float* stats = reinterpret_cast<float*>(smem + (1 + 2 * stages) * C::TILE_BYTES);
+  uint8_t* bar_generic = reinterpret_cast<uint8_t*>(stats) + C::STATS;
   const uint32_t bar_base = smem_u32(bar_generic);
   auto k_full = [&](int st) { return bar_base + 8u * st; };
   auto k_empty = [&](int st) { return bar_base + 8u * (3 + st); };
@@ -197,7 +202,7 @@ kf_shared_prefix_tcgen05(const __grid_constant__ CUtensorMap map_q, const __grid
   auto o_col = [&](int g) { return tmem_base + uint32_t(256 + g * 128); };
 
   if (warp < 4) {
-    regs_give<REGS_ISSUE>();
+    if (!LEAN) regs_give<REGS_ISSUE>();
     if (warp == 0) {
       // ------------------------------------------------------------ TMA producer of Q and K
       if (elect_one()) {
@@ -319,7 +324,7 @@ kf_shared_prefix_tcgen05(const __grid_constant__ CUtensorMap map_q, const __grid
     }
   } else {
     // ------------------------------------------------------------ softmax: warps 4-7 even tiles, 8-11 odd tiles
-    regs_take<REGS_SOFTMAX>();
+    if (!LEAN) regs_take<REGS_SOFTMAX>();
     const int g = (warp >> 2) - 1;
     const int quarter = warp & 3;
     const int row = quarter * 32 + lane;
@@ -361,22 +366,29 @@ kf_shared_prefix_tcgen05(const __grid_constant__ CUtensorMap map_q, const __grid
           }
           continue;
         }
-        uint32_t sv[TILE_KEYS];
+        // the scores: all at once, or (LEAN) in pieces, twice; what lies behind the prompt is hidden
+        constexpr int PIECE = LEAN ? 32 : TILE_KEYS;
+        const int visible = len - n0;
+        auto scores = [&](uint32_t* x, int k0, int n) {
 #pragma unroll
-        for (int c = 0; c < TILE_KEYS / 32; ++c) tmem_ld_32x32_at(t_s + c * 32, sv + c * 32);
-        tmem_ld_wait();
-        if (n0 + TILE_KEYS > len) {
+          for (int c = 0; c < n; c += 32) tmem_ld_32x32_at(t_s + k0 + c, x + c);
+          tmem_ld_wait();
+          if (visible < k0 + n) {
 #pragma unroll
-          for (int k = 0; k < TILE_KEYS; ++k) sv[k] = n0 + k < len ? sv[k] : __float_as_uint(NEG_INF);
-        }
-        float mx;
-        {
-          float mx4[4] = {NEG_INF, NEG_INF, NEG_INF, NEG_INF};
+            for (int k = 0; k < n; ++k) x[k] = k0 + k < visible ? x[k] : __float_as_uint(NEG_INF);
+          }
+        };
+        uint32_t sv[PIECE];
+        float mx = NEG_INF;
+#pragma unroll(LEAN ? 1 : TILE_KEYS / PIECE)
+        for (int k0 = 0; k0 < TILE_KEYS; k0 += PIECE) {
+          scores(sv, k0, PIECE);
+          float mx4[4] = {mx, NEG_INF, NEG_INF, NEG_INF};
 #pragma unroll
-          for (int k = 0; k < TILE_KEYS; k += 8)
+          for (int k = 0; k < PIECE; k += 8)
 #pragma unroll
             for (int q = 0; q < 4; ++q) mx4[q] = fmax3(mx4[q], __uint_as_float(sv[k + 2 * q]), __uint_as_float(sv[k + 2 * q + 1]));
-          mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
+          mx = fmax3(fmaxf(mx4[0], mx4[1]), mx4[2], mx4[3]);
         }
         const float m_new = fmaxf(m_run, mx * scale_log2);
         const bool grow = m_new > m_run + RESCALE_THRESHOLD;
@@ -403,12 +415,14 @@ kf_shared_prefix_tcgen05(const __grid_constant__ CUtensorMap map_q, const __grid
         const float m_use = m_run == NEG_INF ? 0.f : m_run;
         const uint64_t scale2 = pack2(scale_log2, scale_log2), neg_m2 = pack2(-m_use, -m_use);
         uint64_t lsum[4] = {0ull, 0ull, 0ull, 0ull};
-#pragma unroll
+#pragma unroll(LEAN ? 1 : TILE_KEYS / 32)
         for (int c = 0; c < TILE_KEYS / 32; ++c) {
-          uint32_t pk[16];
+          uint32_t again[LEAN ? 32 : 1], pk[16];
+          if (LEAN) scores(again, c * 32, LEAN ? 32 : 0);   // the weights go over scores that have been taken
+          const uint32_t* x = LEAN ? again : sv + c * 32;
 #pragma unroll
           for (int k = 0; k < 16; ++k) {
-            const uint64_t x2 = ffma2(pack2(__uint_as_float(sv[c * 32 + 2 * k]), __uint_as_float(sv[c * 32 + 2 * k + 1])), scale2, neg_m2);
+            const uint64_t x2 = ffma2(pack2(__uint_as_float(x[2 * k]), __uint_as_float(x[2 * k + 1])), scale2, neg_m2);
             float x0, x1;
             unpack2(x2, x0, x1);
             const float e0 = fast_exp2(x0), e1 = fast_exp2(x1);
@@ -416,27 +430,24 @@ kf_shared_prefix_tcgen05(const __grid_constant__ CUtensorMap map_q, const __grid
             pk[k] = pack_bf16(e0, e1);
           }
           tmem_st_32x16(t_s + c * 16, pk);
-          if (c == 1) {
+          if (c & 1) {   // half of the keys are in place
             tmem_st_wait();
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(p_half(g));
+            if (lane == 0) mbar_arrive(c == 1 ? p_half(g) : p_full(g));
           }
         }
         float a0, a1;
         unpack2(fadd2(fadd2(lsum[0], lsum[1]), fadd2(lsum[2], lsum[3])), a0, a1);
         l_run += a0 + a1;
-        tmem_st_wait();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(p_full(g));
       }
       // ---- the unit's partial result: both groups' rows joined, each group writes half of the columns
-      stats[g * TILE_ROWS + row] = make_float2(m_run, l_run);
+      stats[g * TILE_ROWS + row] = m_run;
+      if (g == 1) stats[2 * TILE_ROWS + row] = l_run;
       asm volatile("bar.sync 1, 256;" ::: "memory");
-      const float2 other = stats[(1 - g) * TILE_ROWS + row];
-      const float top = fmaxf(m_run, other.x);
-      const float f_mine = m_run == NEG_INF ? 0.f : fast_exp2(m_run - top), f_other = other.x == NEG_INF ? 0.f : fast_exp2(other.x - top);
+      const float m_other = stats[(1 - g) * TILE_ROWS + row];
+      const float top = fmaxf(m_run, m_other);
+      const float f_mine = m_run == NEG_INF ? 0.f : fast_exp2(m_run - top), f_other = m_other == NEG_INF ? 0.f : fast_exp2(m_other - top);
       const float f0 = g == 0 ? f_mine : f_other, f1 = g == 0 ? f_other : f_mine;
       if (ok && !mbar_wait(o_final, seg & 1, status, KF_ERR_WAIT_TMEM_FULL)) ok = false;
       tc_fence_after();
@@ -463,7 +474,7 @@ kf_shared_prefix_tcgen05(const __grid_constant__ CUtensorMap map_q, const __grid
             }
           }
         }
-        if (g == 0 && row < rows) part_ml[slot * TILE_ROWS + row] = make_float2(top, f_mine * l_run + f_other * other.y);
+        if (g == 0 && row < rows) part_ml[slot * TILE_ROWS + row] = make_float2(top, f0 * l_run + f1 * stats[2 * TILE_ROWS + row]);
       }
       tc_fence_before();
       // the accumulators may be written again, and stats by the next unit
@@ -496,20 +507,20 @@ static int make_map_4d(CUtensorMap* map, const void* base, const uint64_t (&size
   return r == CUDA_SUCCESS ? 0 : (int)r;
 }
 
-template <int HD>
-static int launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const Layout& l, int group, float scale, float* part_o,
-                  float2* part_ml, int* status, cudaStream_t stream) {
-  auto kern = kf_shared_prefix_tcgen05<HD>;
+template <int HD, bool LEAN>
+static int launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const Layout& l, int group, int stages, float scale,
+                  float* part_o, float2* part_ml, int* status, cudaStream_t stream) {
+  auto kern = kf_shared_prefix_tcgen05<HD, LEAN>;
   static bool attr_set[16] = {};
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev >= 16 || !attr_set[dev]) {
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Cfg<HD>::smem(Cfg<HD>::STAGES));
+    // all of the SM's memory as shared memory: CTAs of both kernels side by side
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
     if (e != cudaSuccess) return 300 + (int)e;
     if (dev < 16) attr_set[dev] = true;
   }
-  const long long tiles = (long long)tiles_of(l.P) * l.per_prompt * l.B, each = (tiles + l.ctas - 1) / l.ctas;   // most tiles of a CTA
-  const int stages = each < Cfg<HD>::STAGES ? (int)each : Cfg<HD>::STAGES;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)l.ctas);
   cfg.blockDim = dim3(THREADS);
@@ -524,6 +535,15 @@ static int launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMa
   return e == cudaSuccess ? 0 : 400 + (int)e;
 }
 
+template <int HD>
+static int launch_hd(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const Layout& l, int group, float scale, float* part_o,
+                     float2* part_ml, int* status, cudaStream_t stream) {
+  const long long tiles = (long long)tiles_of(l.P) * l.per_prompt * l.B, each = (tiles + l.ctas - 1) / l.ctas;   // most tiles of a CTA
+  const int stages = each < Cfg<HD>::STAGES ? (int)each : Cfg<HD>::STAGES;
+  return each <= LEAN_TILES ? launch<HD, true>(mq, mk, mv, l, group, stages, scale, part_o, part_ml, status, stream)
+                            : launch<HD, false>(mq, mk, mv, l, group, stages, scale, part_o, part_ml, status, stream);
+}
+
 // Steps in elements: q prompt, continuation, head; k and v prompt, position, head.
 int launch_prefix(const void* q, const void* k, const void* v, const Layout& l, int H, int Hkv, int hd, const long long* qs, const long long* ks,
                   const long long* vs, float scale, float* part_o, float2* part_ml, int* status, cudaStream_t stream) {
@@ -536,8 +556,8 @@ int launch_prefix(const void* q, const void* k, const void* v, const Layout& l, 
   if (rc) return 2000 + rc;
   rc = make_map_4d(&mv, v, {(uint64_t)hd, (uint64_t)Hkv, (uint64_t)l.P, (uint64_t)l.B}, {vs[2], vs[1], vs[0]}, {64u, 1u, (uint32_t)TILE_KEYS, 1u});
   if (rc) return 3000 + rc;
-  return hd == 128 ? launch<128>(mq, mk, mv, l, group, scale, part_o, part_ml, status, stream)
-                   : launch<64>(mq, mk, mv, l, group, scale, part_o, part_ml, status, stream);
+  return hd == 128 ? launch_hd<128>(mq, mk, mv, l, group, scale, part_o, part_ml, status, stream)
+                   : launch_hd<64>(mq, mk, mv, l, group, scale, part_o, part_ml, status, stream);
 }
 
 }  // namespace shared_prefix
