@@ -247,54 +247,76 @@ kf_shared_prefix_own(const Own a, const Layout lay, const float* part_o, const f
     const uint32_t at = base + (s % WPU) * C::WARP;
     return splits > 1 ? mapa_shared(at, s / WPU) : at;
   };
-  // ---- each warp of the unit its share of the output: a lane four values of a row, over the prompt's parts and the unit's warps
-  for (int i = way * 32 + lane; i < n_heads * (HD / 4); i += ways * 32) {
-    const int r = i / (HD / 4), d = (i % (HD / 4)) * 4;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    float top = -INFINITY, sum = 0.f;
-    constexpr int AT_ONCE = 8;
-    float2 x[AT_ONCE];
-    float4 v[AT_ONCE];
+  // ---- each warp of the unit its share of the output: a lane four values of a row, over the prompt's parts and the unit's warps; several
+  // rows at once where a warp has several, with eight loads of parts under way
+  constexpr int ITEMS = WPU == 1 ? 4 : WPU == 2 ? 2 : 1, AT_ONCE = 8 / ITEMS;
+  const int n_items = n_heads * (HD / 4);
+  for (int i0 = way * 32 + lane; i0 < n_items; i0 += ways * 32 * ITEMS) {
+    float4 acc[ITEMS];
+    float top[ITEMS], sum[ITEMS];
+    float2 x[ITEMS][AT_ONCE];
+    float4 v[ITEMS][AT_ONCE];
+    int r[ITEMS], d[ITEMS];
+#pragma unroll
+    for (int j = 0; j < ITEMS; ++j) {
+      const int i = min(i0 + j * ways * 32, n_items - 1);   // one too many is worked on with the others, and not written
+      r[j] = i / (HD / 4), d[j] = (i % (HD / 4)) * 4;
+      acc[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+      top[j] = -INFINITY, sum[j] = 0.f;
+    }
     auto join = [&](int n) {   // the first n of them
-      float higher = top;
 #pragma unroll
-      for (int e = 0; e < AT_ONCE; ++e)
-        if (e < n) higher = fmaxf(higher, x[e].x);
-      const float f = weight(top, higher);
-      acc.x *= f; acc.y *= f; acc.z *= f; acc.w *= f;
-      sum *= f;
-      top = higher;
+      for (int j = 0; j < ITEMS; ++j) {
+        float higher = top[j];
 #pragma unroll
-      for (int e = 0; e < AT_ONCE; ++e)
-        if (e < n) {
-          const float g = weight(x[e].x, top);
-          acc.x += g * v[e].x; acc.y += g * v[e].y; acc.z += g * v[e].z; acc.w += g * v[e].w;
-          sum += g * x[e].y;
-        }
+        for (int e = 0; e < AT_ONCE; ++e)
+          if (e < n) higher = fmaxf(higher, x[j][e].x);
+        const float f = weight(top[j], higher);
+        acc[j].x *= f; acc[j].y *= f; acc[j].z *= f; acc[j].w *= f;
+        sum[j] *= f;
+        top[j] = higher;
+#pragma unroll
+        for (int e = 0; e < AT_ONCE; ++e)
+          if (e < n) {
+            const float g = weight(x[j][e].x, higher);
+            acc[j].x += g * v[j][e].x; acc[j].y += g * v[j][e].y; acc[j].z += g * v[j][e].z; acc[j].w += g * v[j][e].w;
+            sum[j] += g * x[j][e].y;
+          }
+      }
     };
-    const float2* ml = part_ml + slot0 + r;
-    const float4* po = reinterpret_cast<const float4*>(part_o + (slot0 + r) * HD + d);
     for (int c = 0; c < parts; c += AT_ONCE) {
 #pragma unroll
       for (int e = 0; e < AT_ONCE; ++e)
-        if (c + e < parts) x[e] = ld_after_wait(ml + (long long)(c + e) * TILE_ROWS), v[e] = ld_after_wait(po + (long long)(c + e) * TILE_ROWS * (HD / 4));
+#pragma unroll
+        for (int j = 0; j < ITEMS; ++j)
+          if (c + e < parts) {
+            const long long at = slot0 + r[j] + (long long)(c + e) * TILE_ROWS;
+            x[j][e] = ld_after_wait(part_ml + at);
+            v[j][e] = ld_after_wait(reinterpret_cast<const float4*>(part_o + at * HD + d[j]));
+          }
       join(parts - c);
     }
     for (int s = 0; s < ways; s += AT_ONCE) {
 #pragma unroll
       for (int e = 0; e < AT_ONCE; ++e)
-        if (s + e < ways) {
-          const uint32_t at = own_at(stats_a + r * 8, s + e);
-          x[e] = make_float2(ld_cluster_f1(at), ld_cluster_f1(at + 4));
-          v[e] = ld_cluster_f4(own_at(part_a + uint32_t(r * HD + d) * 4u, s + e));
-        }
+#pragma unroll
+        for (int j = 0; j < ITEMS; ++j)
+          if (s + e < ways) {
+            const uint32_t at = own_at(stats_a + r[j] * 8, s + e);
+            x[j][e] = make_float2(ld_cluster_f1(at), ld_cluster_f1(at + 4));
+            v[j][e] = ld_cluster_f4(own_at(part_a + uint32_t(r[j] * HD + d[j]) * 4u, s + e));
+          }
       join(ways - s);
     }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;   // nothing visible: zeros
-    uint2 out;
-    out.x = pack_bf16(acc.x * inv, acc.y * inv);
-    out.y = pack_bf16(acc.z * inv, acc.w * inv);
-    *reinterpret_cast<uint2*>(a.o + (((long long)b * lay.W + w) * a.Hkv * a.group + h0 + r) * HD + d) = out;
+#pragma unroll
+    for (int j = 0; j < ITEMS; ++j) {
+      if (i0 + j * ways * 32 >= n_items) break;
+      const float inv = sum[j] == 0.f ? 0.f : 1.f / sum[j];   // nothing visible: zeros
+      uint2 out;
+      out.x = pack_bf16(acc[j].x * inv, acc[j].y * inv);
+      out.y = pack_bf16(acc[j].z * inv, acc[j].w * inv);
+      *reinterpret_cast<uint2*>(a.o + (((long long)b * lay.W + w) * a.Hkv * a.group + h0 + r[j]) * HD + d[j]) = out;
+    }
   }
   if (splits > 1) cluster_sync_all();   // no CTA leaves while another reads its shared memory
 }
