@@ -11,7 +11,7 @@
 //   * Each of a CTA's 8 warps has ceil(W / 8) threads whose largest logit is at least the warp's ceil(W / 8)-th largest.  So at least W logits
 //     reach the least of these over the warps, a bound that costs a warp-wide maximum or a few.  Taken after each thread's first four
 //     vectors, which lie spread over the range, it leaves about 22 * rounds / 4 vectors of 8 beams that reach it and are noted; taken
-//     again at the end, about 22, which are read once more (out of L2).  A list that every warp kept on the way, with an insertion
+//     again at the end, about 22.  A list that every warp kept on the way, with an insertion
 //     for each of W ln(n / W) logits, took 98 us for 64 x 8 x 128 256 in bf16; reading all vectors of the threads that reach the bound 92.
 //   * Candidates are 64-bit keys: the logit's bits in an order-preserving form, then the complement of its index, so that of equal
 //     logits the lowest index is the largest key.  There are few, so a candidate's place is how many are larger, counted; the cluster's
@@ -37,7 +37,7 @@ constexpr int WARPS = 8;
 constexpr int THREADS = WARPS * 32;
 constexpr int CTAS = 8;         // of a cluster
 constexpr int MAX_PARTS = MAX_BEAMS / CTAS + 1;       // rows that a CTA's range meets
-constexpr int NOTES = 1024;     // vectors that a CTA notes; more (logits in rising order, equal ones) go through lists
+constexpr int NOTES = 1024;     // vectors that a CTA notes (24 KB); more (logits in rising order, equal ones) go through lists
 constexpr int ROOM = 512;             // candidates that a CTA sorts, likewise
 
 typedef unsigned long long Key;
@@ -171,6 +171,7 @@ kf_beam_select(const T* __restrict__ logits, long long stride_b, long long strid
   __shared__ uint32_t reach[2][WARPS];             // after the first round, at the end
   __shared__ int n_found[MAX_PARTS], n_notes[MAX_PARTS];
   __shared__ Key notes[NOTES];                     // (largest logit, vector)
+  __shared__ uint4 noted_raw[NOTES];               // the vector
   __shared__ Key found[ROOM];                      // candidates, or the warps' lists
   __shared__ int winner[MAX_BEAMS];                // of each place: which candidate
   double* total = reinterpret_cast<double*>(notes);   // [W][W], best first, -inf: none
@@ -208,7 +209,7 @@ kf_beam_select(const T* __restrict__ logits, long long stride_b, long long strid
     const int v1 = min(v_end, vectors);
     const uint4* vec = reinterpret_cast<const uint4*>(x0 + head);
     const int single = v0 != 0 || tid >= 2 * N ? -1 : tid < head ? tid : tid >= N && tid - N < V - tail0 ? tail0 + tid - N : -1;
-    // Four streams of rounds through the range, a vector a thread each; four vectors under way while four are worked on.
+    // Four streams of rounds through the range, a vector a thread each; a vector is asked for as the one before it is taken.
     const int rounds = v1 > v0 ? (v1 - v0 + THREADS - 1) / THREADS : 0, quarter = (rounds + UNROLL - 1) / UNROLL;
     const int own_rounds = v1 - v0 > tid ? (v1 - v0 - tid + THREADS - 1) / THREADS : 0;
     const uint4* mine0 = vec + v0 + tid;
@@ -217,7 +218,7 @@ kf_beam_select(const T* __restrict__ logits, long long stride_b, long long strid
       if (round < own_rounds) v = mine0[round * THREADS];
       return v;
     };
-    uint4 now[UNROLL], next[UNROLL];
+    uint4 now[UNROLL];
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u) now[u] = fetch(quarter > 0 ? u * quarter : own_rounds);
     const float alone = single >= 0 ? clean(Logits<T>::one(x0 + single)) : -INFINITY;
@@ -267,8 +268,6 @@ kf_beam_select(const T* __restrict__ logits, long long stride_b, long long strid
 #pragma unroll 1
     for (int j = 0; j < quarter; ++j) {
 #pragma unroll
-      for (int u = 0; u < UNROLL; ++u) next[u] = fetch(j + 1 < quarter ? u * quarter + j + 1 : own_rounds);
-#pragma unroll
       for (int u = 0; u < UNROLL; ++u) {
         float x[N];
         float mx = Logits<T>::load(now[u], x);
@@ -287,10 +286,11 @@ kf_beam_select(const T* __restrict__ logits, long long stride_b, long long strid
           }
           if (mx >= least_f && mx > -INFINITY) {
             const int to = atomicAdd(&n_notes[part], 1);
-            if (to < NOTES) notes[to] = make_key(mx, uint32_t(v0 + (u * quarter + j) * THREADS + tid));
+            if (to < NOTES) notes[to] = make_key(mx, uint32_t(v0 + (u * quarter + j) * THREADS + tid)), noted_raw[to] = now[u];
           }
           usual = fminf(least_f, limit);
         }
+        now[u] = fetch(j + 1 < quarter ? u * quarter + j + 1 : own_rounds);
         m = max_of(m, mx);
         const uint64_t r2 = pack2(-r, -r), log2e2 = pack2(LOG2E, LOG2E);
 #pragma unroll
@@ -305,8 +305,6 @@ kf_beam_select(const T* __restrict__ logits, long long stride_b, long long strid
         bound();
         usual = fminf(least_f, limit);
       }
-#pragma unroll
-      for (int u = 0; u < UNROLL; ++u) now[u] = next[u];
     }
 
     // ---- the warp's sum, and the bound again
@@ -325,7 +323,7 @@ kf_beam_select(const T* __restrict__ logits, long long stride_b, long long strid
     }
     __syncthreads();
     const uint32_t least = least_of(reach[1]);
-    // ---- the vectors that reach it once more
+    // ---- the noted vectors that reach it
     auto take = [&](float x, int i) {
       if (x > -INFINITY && ordered(x) >= least) {
         const int to = atomicAdd(&n_found[part], 1);
@@ -338,10 +336,9 @@ kf_beam_select(const T* __restrict__ logits, long long stride_b, long long strid
       const Key n = notes[e];
       if (uint32_t(n >> 32) >= least) {
         const int at = head + int(key_index(n)) * N;
-        float x[N];
-        Logits<T>::load(*reinterpret_cast<const uint4*>(x0 + at), x);
-#pragma unroll
-        for (int j = 0; j < N; ++j) take(clean(x[j]), at + j);
+        const T* x = reinterpret_cast<const T*>(&noted_raw[e]);
+#pragma unroll 2
+        for (int j = 0; j < N; ++j) take(clean(Logits<T>::one(x + j)), at + j);
       }
     }
     __syncthreads();
