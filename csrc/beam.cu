@@ -192,7 +192,7 @@ kf_beam_select(const T* __restrict__ logits, long long stride_b, long long strid
   const uint32_t all = uint32_t(__popc(live)) * per;
   const uint32_t chunk = all / CTAS;
   const uint32_t r1 = chunk * (rank + 1);
-  cluster_sync_all();   // the first CTA is there to be written to
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");   // waited for below: the first CTA is there to be written to
 
   int part = 0;
   for (uint32_t pos = chunk * rank; pos < r1; ++part) {
@@ -331,18 +331,26 @@ kf_beam_select(const T* __restrict__ logits, long long stride_b, long long strid
       }
     };
     const int noted = n_notes[part];
+    const float reached_f = least ? unordered(least) : -INFINITY;
     take(alone, single);
     for (int e = tid; e < min(noted, NOTES); e += THREADS) {
       const Key n = notes[e];
       if (uint32_t(n >> 32) >= least) {
         const int at = head + int(key_index(n)) * N;
-        const T* x = reinterpret_cast<const T*>(&noted_raw[e]);
-#pragma unroll 2
-        for (int j = 0; j < N; ++j) take(clean(Logits<T>::one(x + j)), at + j);
+        float x[N];
+        Logits<T>::load(noted_raw[e], x);
+        uint32_t hits = 0;   // as floats: those below the smallest normal number are all alike, and looked at again
+#pragma unroll
+        for (int j = 0; j < N; ++j) hits |= uint32_t(!(clean(x[j]) < reached_f)) << j;
+        for (; hits; hits &= hits - 1) {
+          const int j = __ffs(hits) - 1;
+          take(clean(Logits<T>::one(reinterpret_cast<const T*>(&noted_raw[e]) + j)), at + j);
+        }
       }
     }
     __syncthreads();
     // ---- the W largest and the sum, into the first CTA
+    if (part == 0) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
     const uint32_t to = mapa_shared(smem_u32(&parts[nth + rank]), 0);
     const int candidates = n_found[part];
     if (candidates <= ROOM && noted <= NOTES) {
@@ -389,6 +397,7 @@ kf_beam_select(const T* __restrict__ logits, long long stride_b, long long strid
     }
   }
 
+  if (part == 0) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");   // this CTA had nothing to write
   cluster_sync_all();
   // ---- the first CTA joins what the cluster found, a warp a beam
   if (rank != 0) return;

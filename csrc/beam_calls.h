@@ -30,6 +30,14 @@ const at::Tensor* on_device(PyObject* o, long rank, long device) {
 
 bool wants_gradient(const at::Tensor& t) { return t.requires_grad() && at::GradMode::is_enabled(); }
 
+// A dense tensor in `base`'s memory from byte `at` on; an allocation of its own takes 1 us.
+at::Tensor within(const at::Tensor& base, at::ScalarType type, int64_t at, at::IntArrayRef sizes) {
+  auto impl = c10::make_intrusive<c10::TensorImpl>(c10::Storage(base.storage()), base.key_set(), c10::scalarTypeToTypeMeta(type));
+  impl->set_sizes_contiguous(sizes);
+  impl->set_storage_offset(at / static_cast<int64_t>(c10::elementSize(type)));
+  return at::Tensor(std::move(impl));
+}
+
 // beam_select(logits, scores, finished or None, eos, pad, sms, device, stream) -> (scores, parents, tokens, finished)
 PyObject* beam_select(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   long device = 0;
@@ -49,9 +57,10 @@ PyObject* beam_select(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
       (f && (f->scalar_type() != at::kBool || f->sizes() != s->sizes() || !f->is_contiguous())))
     Py_RETURN_NONE;
   HANDLE_TH_ERRORS
-  const at::TensorOptions o = s->options();
-  at::Tensor scores = at::empty({b, w}, o), parents = at::empty({b, w}, o.dtype(at::kLong)), tokens = at::empty({b, w}, o.dtype(at::kLong));
-  at::Tensor finished = at::empty({b, w}, o.dtype(at::kBool));
+  const int64_t n = b * w;
+  const at::Tensor all = at::empty({n * 21}, s->options().dtype(at::kByte));
+  at::Tensor parents = within(all, at::kLong, 0, {b, w}), tokens = within(all, at::kLong, 8 * n, {b, w});
+  at::Tensor scores = within(all, at::kFloat, 16 * n, {b, w}), finished = within(all, at::kBool, 20 * n, {b, w});
   const int rc = issued([&] {
     return bm.select(x->const_data_ptr(), type, x->stride(0), x->stride(1), s->const_data_ptr(), f ? f->const_data_ptr() : nullptr, int(b), int(w),
                      int(v), eos, pad, at_(scores), at_(parents), at_(tokens), at_(finished), int(sms), stream);
