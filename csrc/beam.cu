@@ -489,73 +489,76 @@ struct State {
   long long src_b, src_w, dst_b, dst_w;   // bytes
   long long bytes;                        // of a beam that follow it
 };
-constexpr int MAX_STATES = 56;            // with the rest of the arguments below 4 KB
+constexpr int MAX_STATES = 60;            // with the rest of the arguments below 4 KB
 struct States {
   State s[MAX_STATES];
-  long long first[MAX_STATES + 1];        // prefix sums of columns x prompts
 };
 
-// T: the widest word that all addresses and steps are multiples of.  A column is one word; the last column of a state may hold fewer
-// bytes than a word and is moved byte by byte.
-template <typename T, int W>
+// T: the widest word that all addresses and steps are multiples of.  A column is one word of all W beams; the last column of a state may
+// hold fewer bytes than a word and is moved byte by byte.  Block (x, prompt, state); a thread moves COLS columns, whose words are all
+// under way at once: W * COLS of 16 bytes are what fills a GPU's memory with threads enough.
+template <typename T, int W, int COLS>
 __global__ void __launch_bounds__(256)
-kf_beam_reorder(const __grid_constant__ States st, int n, int beams, const void* __restrict__ parents, int wide) {
-  const long long total = st.first[n];
-  int s = 0;
-  for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (long long)gridDim.x * blockDim.x) {
-    while (i >= st.first[s + 1]) ++s;
-    const State& a = st.s[s];
-    const long long columns = (a.bytes + sizeof(T) - 1) / (long long)sizeof(T);
-    const long long b = (i - st.first[s]) / columns, off = (i - st.first[s]) % columns * (long long)sizeof(T);
-    const uint8_t* src = a.src + b * a.src_b + off;
-    uint8_t* dst = a.dst + b * a.dst_b + off;
-    const bool in_place = a.src == a.dst;
-    const int left = int(a.bytes - off < (long long)sizeof(T) ? a.bytes - off : (long long)sizeof(T));
-    T v[W];
-    bool move[W];
+kf_beam_reorder(const __grid_constant__ States st, int beams, const void* __restrict__ parents, int wide) {
+  const State& a = st.s[blockIdx.z];
+  const long long b = blockIdx.y;
+  const long long off0 = ((long long)blockIdx.x * (256 * COLS) + threadIdx.x) * (long long)sizeof(T);
+  if ((long long)blockIdx.x * (256 * COLS) * (long long)sizeof(T) >= a.bytes) return;
+  const uint8_t* src = a.src + b * a.src_b;
+  uint8_t* dst = a.dst + b * a.dst_b;
+  int from[W];   // a parent that is no beam, or in place the beam itself: it stays as it is (-1)
 #pragma unroll
-    for (int w = 0; w < W; ++w) {
-      move[w] = false;
-      if (w < beams) {
-        const long long p = wide ? reinterpret_cast<const long long*>(parents)[b * beams + w]
-                                 : (long long)reinterpret_cast<const int*>(parents)[b * beams + w];
-        // a parent that is no beam: the state stays as it is
-        move[w] = p >= 0 && p < beams && !(in_place && p == w);
-        if (move[w]) {
-          const uint8_t* from = src + p * a.src_w;
-          if (left == (int)sizeof(T)) {
-            v[w] = *reinterpret_cast<const T*>(from);
-          } else {
-            uint8_t* bytes = reinterpret_cast<uint8_t*>(&v[w]);
-            for (int j = 0; j < (int)sizeof(T); ++j)
-              if (j < left) bytes[j] = from[j];
-          }
-        }
+  for (int w = 0; w < W; ++w) {
+    from[w] = -1;
+    if (w < beams) {
+      const long long p = wide ? reinterpret_cast<const long long*>(parents)[b * beams + w] : (long long)reinterpret_cast<const int*>(parents)[b * beams + w];
+      if (p >= 0 && p < beams && !(a.src == a.dst && p == w)) from[w] = int(p);
+    }
+  }
+  T v[COLS][W];
+#pragma unroll
+  for (int c = 0; c < COLS; ++c) {
+    const long long off = off0 + c * 256 * (long long)sizeof(T), left = a.bytes - off;
+    if (left >= (long long)sizeof(T)) {
+#pragma unroll
+      for (int w = 0; w < W; ++w)
+        if (from[w] >= 0) v[c][w] = *reinterpret_cast<const T*>(src + from[w] * a.src_w + off);
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < COLS; ++c) {
+    const long long off = off0 + c * 256 * (long long)sizeof(T), left = a.bytes - off;
+    if (left >= (long long)sizeof(T)) {
+#pragma unroll
+      for (int w = 0; w < W; ++w)
+        if (from[w] >= 0) *reinterpret_cast<T*>(dst + w * a.dst_w + off) = v[c][w];
+    } else if (left > 0) {
+      for (int j = 0; j < int(left); ++j) {   // a byte of all beams at a time
+        uint8_t byte[W];
+#pragma unroll
+        for (int w = 0; w < W; ++w)
+          if (from[w] >= 0) byte[w] = src[from[w] * a.src_w + off + j];
+#pragma unroll
+        for (int w = 0; w < W; ++w)
+          if (from[w] >= 0) dst[w * a.dst_w + off + j] = byte[w];
       }
     }
-#pragma unroll
-    for (int w = 0; w < W; ++w)
-      if (move[w]) {
-        uint8_t* to = dst + w * a.dst_w;
-        if (left == (int)sizeof(T)) {
-          *reinterpret_cast<T*>(to) = v[w];
-        } else {
-          const uint8_t* bytes = reinterpret_cast<const uint8_t*>(&v[w]);
-          for (int j = 0; j < (int)sizeof(T); ++j)
-            if (j < left) to[j] = bytes[j];
-        }
-      }
   }
 }
 
+template <typename T, int W, int COLS>
+static void launch_columns(const States& st, int n, int B, int beams, const void* parents, int wide, long long bytes, cudaStream_t stream) {
+  const long long step = 256LL * COLS * sizeof(T);
+  const dim3 grid((unsigned)((bytes + step - 1) / step), (unsigned)B, (unsigned)n);
+  kf_beam_reorder<T, W, COLS><<<grid, 256, 0, stream>>>(st, beams, parents, wide);
+}
+
 template <typename T>
-static void launch_reorder(const States& st, int n, int beams, const void* parents, int wide, int num_sms, cudaStream_t stream) {
-  const long long need = (st.first[n] + 255) / 256;
-  const unsigned grid = (unsigned)(need < 8LL * num_sms ? need : 8LL * num_sms);
-  if (beams <= 4) kf_beam_reorder<T, 4><<<grid, 256, 0, stream>>>(st, n, beams, parents, wide);
-  else if (beams <= 8) kf_beam_reorder<T, 8><<<grid, 256, 0, stream>>>(st, n, beams, parents, wide);
-  else if (beams <= 16) kf_beam_reorder<T, 16><<<grid, 256, 0, stream>>>(st, n, beams, parents, wide);
-  else kf_beam_reorder<T, 32><<<grid, 256, 0, stream>>>(st, n, beams, parents, wide);
+static void launch_reorder(const States& st, int n, int B, int beams, const void* parents, int wide, long long bytes, cudaStream_t stream) {
+  if (beams <= 4) launch_columns<T, 4, 2>(st, n, B, beams, parents, wide, bytes, stream);
+  else if (beams <= 8) launch_columns<T, 8, 1>(st, n, B, beams, parents, wide, bytes, stream);
+  else if (beams <= 16) launch_columns<T, 16, 1>(st, n, B, beams, parents, wide, bytes, stream);
+  else launch_columns<T, 32, 1>(st, n, B, beams, parents, wide, bytes, stream);
 }
 
 }  // namespace beam
@@ -584,27 +587,27 @@ int kf_beam_max_states() { return kf::beam::MAX_STATES; }
 
 // table: 7 numbers a state (src, dst, and in bytes: steps of src and dst from prompt to prompt and beam to beam as src_b, src_w, dst_b,
 // dst_w, and the length that moves).  parents (B, beams), int64 or (wide == 0) int32.  dst is src itself or does not overlap it.
-int kf_beam_reorder(const long long* table, int n, int B, int beams, const void* parents, int wide, int num_sms, void* stream) {
+int kf_beam_reorder(const long long* table, int n, int B, int beams, const void* parents, int wide, void* stream) {
   using namespace kf::beam;
-  if (n < 1 || n > MAX_STATES || B < 1 || beams < 1 || beams > MAX_BEAMS) return 3;
+  if (n < 1 || n > MAX_STATES || B < 1 || B > 65535 || beams < 1 || beams > MAX_BEAMS) return 3;
   States st;
   unsigned long long all = 0;
+  long long most = 0;
   for (int i = 0; i < n; ++i) {
     const long long* t = table + 7 * i;
     st.s[i] = State{(const uint8_t*)t[0], (uint8_t*)t[1], t[2], t[3], t[4], t[5], t[6]};
     if (t[6] < 0) return 3;
+    if (t[6] > most) most = t[6];
     for (int j = 0; j < 6; ++j) all |= (unsigned long long)t[j];
   }
-  const int word = !(all & 15) ? 16 : !(all & 7) ? 8 : !(all & 3) ? 4 : !(all & 1) ? 2 : 1;
-  st.first[0] = 0;
-  for (int i = 0; i < n; ++i) st.first[i + 1] = st.first[i] + (st.s[i].bytes + word - 1) / word * B;
-  if (st.first[n] == 0) return 0;
+  if (most == 0) return 0;
+  if (most > 1LL << 37) return 6;   // blocks of 256 bytes are counted in 31 bits
   cudaStream_t s = (cudaStream_t)stream;
-  if (word == 16) launch_reorder<uint4>(st, n, beams, parents, wide, num_sms, s);
-  else if (word == 8) launch_reorder<unsigned long long>(st, n, beams, parents, wide, num_sms, s);
-  else if (word == 4) launch_reorder<uint32_t>(st, n, beams, parents, wide, num_sms, s);
-  else if (word == 2) launch_reorder<uint16_t>(st, n, beams, parents, wide, num_sms, s);
-  else launch_reorder<uint8_t>(st, n, beams, parents, wide, num_sms, s);
+  if (!(all & 15)) launch_reorder<uint4>(st, n, B, beams, parents, wide, most, s);
+  else if (!(all & 7)) launch_reorder<unsigned long long>(st, n, B, beams, parents, wide, most, s);
+  else if (!(all & 3)) launch_reorder<uint32_t>(st, n, B, beams, parents, wide, most, s);
+  else if (!(all & 1)) launch_reorder<uint16_t>(st, n, B, beams, parents, wide, most, s);
+  else launch_reorder<uint8_t>(st, n, B, beams, parents, wide, most, s);
   cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? 0 : 400 + (int)e;
 }

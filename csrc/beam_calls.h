@@ -15,7 +15,7 @@ namespace {
 struct Beam {
   int (*select)(const void*, int, long long, long long, const void*, const void*, int, int, int, long long, long long, void*, void*, void*, void*, int,
                 void*) = nullptr;
-  int (*reorder)(const long long*, int, int, int, const void*, int, int, void*) = nullptr;
+  int (*reorder)(const long long*, int, int, int, const void*, int, void*) = nullptr;
   long long (*scratch)(int, int, int, int, int, int, int) = nullptr;
   int (*attention)(const void*, const void*, const void*, const void*, const void*, const void*, const void*, void*, void*, int, int, int, int, int, int,
                    int, const long long*, float, int, void*) = nullptr;
@@ -70,21 +70,20 @@ PyObject* beam_select(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
-// beam_reorder(states, parents, length or None, out or None, sms, device, stream) -> launches; states and out are lists
+// beam_reorder(states, parents, length or None, out or None, device, stream) -> launches; states and out are lists
 PyObject* beam_reorder(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   long device = 0;
   void* stream = nullptr;
-  if (nargs != 7 || !bm.reorder || !where(args + 5, &device, &stream)) return none();
+  if (nargs != 6 || !bm.reorder || !where(args + 4, &device, &stream)) return none();
   const bool whole = args[2] == Py_None, in_place = args[3] == Py_None;
   if (!PyList_Check(args[0]) || (!in_place && (!PyList_Check(args[3]) || PyList_GET_SIZE(args[3]) != PyList_GET_SIZE(args[0])))) Py_RETURN_NONE;
   const long long length = whole ? 0 : PyLong_AsLongLong(args[2]);
-  const long sms = PyErr_Occurred() ? 0 : PyLong_AsLong(args[4]);
   if (PyErr_Occurred()) return nullptr;
   const at::Tensor* p = on_device(args[1], 2, device);
   if (!p || !p->is_contiguous() || (p->scalar_type() != at::kLong && p->scalar_type() != at::kInt) || (!whole && length < 1)) Py_RETURN_NONE;
   const int64_t b = p->size(0), w = p->size(1);
   const Py_ssize_t n = PyList_GET_SIZE(args[0]);
-  if (b < 1 || w < 1 || w > bm.max_beams || b > kLargest || n < 1) Py_RETURN_NONE;
+  if (b < 1 || w < 1 || w > bm.max_beams || b > 65535 || n < 1) Py_RETURN_NONE;
   HANDLE_TH_ERRORS
   struct Span {
     long long begin, end;
@@ -117,6 +116,7 @@ PyObject* beam_reorder(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     }
     const long long inner = x->dim() > 2 ? x->size(2) : 1;
     const long long beam = x->numel() / (b * w) / inner * (whole ? inner : length) * size;
+    if (beam > 1LL << 37) Py_RETURN_NONE;
     const long long row[7] = {reinterpret_cast<long long>(x->const_data_ptr()), reinterpret_cast<long long>(at_(*y)), x->stride(0) * size,
                               x->stride(1) * size, y->stride(0) * size, y->stride(1) * size, beam};
     table.insert(table.end(), row, row + 7);
@@ -133,7 +133,7 @@ PyObject* beam_reorder(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   for (Py_ssize_t i = 0; i < n; i += bm.max_states, ++launches) {
     const int rc = issued([&] {
       return bm.reorder(table.data() + 7 * i, int(std::min<Py_ssize_t>(bm.max_states, n - i)), int(b), int(w), p->const_data_ptr(),
-                        p->scalar_type() == at::kLong, int(sms), stream);
+                        p->scalar_type() == at::kLong, stream);
     });
     if (rc) return PyLong_FromLong(-rc);
   }

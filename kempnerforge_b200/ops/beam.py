@@ -145,7 +145,7 @@ def reorder(states: list[torch.Tensor], parents: torch.Tensor, length: int | Non
     if parents.numel() == 0 or not states:
         return to
     with torch.no_grad():
-        if not (_native(parents) and parents.shape[1] <= 32):
+        if not (_native(parents) and parents.shape[1] <= 32 and parents.shape[0] <= 65535):
             ref.beam_reorder(states, parents, length, to)
         else:
             _reorder_native(states, parents, length, to)
@@ -160,7 +160,7 @@ def _reorder_native(states, parents, length, to):
         if x.numel() == 0:
             continue
         inner = x[0, 0].numel()
-        if not _dense_beams(x) or not _dense_beams(y) or not _apart(y) or min(x.stride(0), x.stride(1), y.stride(0), y.stride(1)) < 0:
+        if inner * x.element_size() > 1 << 37 or not _dense_beams(x) or not _dense_beams(y) or not _apart(y) or min(x.stride(0), x.stride(1), y.stride(0), y.stride(1)) < 0:
             later.append((x, y))
             continue
         moves.append((x, y, inner * x.element_size()))

@@ -143,7 +143,7 @@ def _declare(L: ctypes.CDLL) -> None:
         "kf_shared_prefix_attn_bf16": [vp] * 9 + [i] * 7 + [vp, f, i, vp],
         "kf_beam_select": [vp, i, ll, ll, vp, vp, i, i, i, ll, ll, vp, vp, vp, vp, i, vp],
         "kf_beam_max_states": [],
-        "kf_beam_reorder": [vp, i, i, i, vp, i, i, vp],
+        "kf_beam_reorder": [vp, i, i, i, vp, i, vp],
         "kf_read_status": [],
         "kf_clear_status": [],
         "kf_status_device_ptr": [],
@@ -1133,7 +1133,7 @@ def beam_reorder_call(states: list, parents, length, out: list | None) -> bool:
     global LAUNCH_COUNT
     steps = _load_steps() if _steps is None else _steps
     device = torch._C._cuda_getDevice()
-    n = steps.beam_reorder(states, parents, length, out, sm_count(), device, torch._C._cuda_getCurrentRawStream(device)) if steps else None
+    n = steps.beam_reorder(states, parents, length, out, device, torch._C._cuda_getCurrentRawStream(device)) if steps else None
     if n is None:
         return False
     if n < 0:
@@ -1158,7 +1158,8 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, finished: torch.Tens
 
 
 def beam_reorder(moves, parents: torch.Tensor) -> None:
-    """``moves``: (source, destination, bytes of a beam that move) of states whose beams are dense; the same tensor, or no overlap."""
+    """``moves``: (source, destination, bytes of a beam that move) of states whose beams are dense; the same tensor, or no overlap.  Up to
+    65 535 prompts, ``BEAMS`` beams and 2^37 bytes of a beam."""
     b, w = parents.shape
     L = lib()
     most = L.kf_beam_max_states()
@@ -1169,8 +1170,8 @@ def beam_reorder(moves, parents: torch.Tensor) -> None:
             size = src.element_size()
             table.extend((src.data_ptr(), dst.data_ptr(), src.stride(0) * size, src.stride(1) * size, dst.stride(0) * size,
                           dst.stride(1) * size, n))
-        _check(L.kf_beam_reorder(table.buffer_info()[0], len(part), b, w, parents.data_ptr(), int(parents.dtype == torch.int64), sm_count(),
-                                 _stream()), "kf_beam_reorder")
+        _check(L.kf_beam_reorder(table.buffer_info()[0], len(part), b, w, parents.data_ptr(), int(parents.dtype == torch.int64), _stream()),
+               "kf_beam_reorder")
 
 
 # --------------------------------------------------------------------------- Lion / schedule-free AdamW
