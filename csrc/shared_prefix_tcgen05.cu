@@ -6,20 +6,10 @@
 // of an SM's share of HBM; its two products take 512, its 16 384 exponentials 1024.  So rows that are not there (a tile is always 128)
 // cost nothing, and all that counts is to keep the copies in flight: two stages each of K and V (128 KB) run ahead of the products.  Three
 // were slower (4 x 32 768 keys, 64 heads of 128, with the second kernel: 102 and 98 us).
-// Where a CTA has two tiles at most, what counts is that the second kernel does its own part meanwhile, beside it on the same SM: LEAN, in 96
-// registers a thread, with scores taken from tensor memory twice, 32 at a time, for the maximum and for the exponentials, and at most
-// 162 KB.  1 x 8 x 4000: 14.2 -> 11.7 us; but 24 x 8 x 512 (three tiles) 15.9 -> 16.4, 2 x 64 x 8000 59 -> 66.
-//
-//   warp 0     : TMA producer of Q and K
-//   warp 1     : MMA issuer
-//   warp 2     : TMA producer of V (warp 3 only makes the first warpgroup whole)
-//   warps 4-7  : softmax of the even tiles of a unit, one thread per row
-//   warps 8-11 : softmax of the odd tiles
-//   TMEM       : S_even | S_odd | O_even | O_odd   (128 fp32 columns each; bf16 P over the start of its S)
-// The two softmax groups have maxima, sums and accumulators of their own, so neither waits for the other; they are joined where a unit ends.
-//
-// P is rounded to bf16 for the second product (2^-9 of each weight, and the sum of the weights is that of the unrounded ones);
-// maxima, sums and O are fp32, and so are the partial results.
+// Where a CTA has three tiles at most, what counts is that the second kernel does its own part meanwhile, beside it on the same SM: LEAN, in
+// 96 registers a thread, with scores taken from tensor memory twice, 32 at a time, for the maximum and for the exponentials, and at most
+// 162 KB.  Not LEAN / LEAN, us: 1 x 8 x 4000 (two tiles) 14.2 / 11.3, 24 x 8 x 512 (three) 15.4 / 14.9, 16 x 4 x 800 (four) 13.8 / 15.0,
+// 8 x 5 x 1777 (seven) 21.3 / 22.5.
 #include "attention_common.cuh"
 #include "shared_prefix.cuh"
 #include "skinny_common.cuh"
@@ -32,7 +22,7 @@ using namespace kf::attn;
 constexpr int THREADS = 384;
 constexpr int REGS_ISSUE = 72, REGS_SOFTMAX = 216;  // per thread; 72 + 2 * 216 = 3 * 168, what the launch gets
 constexpr int LEAN_BOUND = 608;                     // threads that a block might have: 96 registers each
-constexpr int LEAN_TILES = 2;
+constexpr int LEAN_TILES = 3;
 constexpr int TMEM_COLS = 512;
 constexpr float RESCALE_THRESHOLD = 8.0f;           // P up to 2^8 before the accumulator is scaled again
 
@@ -239,6 +229,8 @@ kf_shared_prefix_tcgen05(const __grid_constant__ CUtensorMap map_q, const __grid
         bool ok = true;
         int issued = 0;
         Turn turn;
+        // the first K before the first V: the scores can begin
+        if (wk.left > 0) ok = mbar_wait(k_full(0), 0, status, KF_ERR_WAIT_FULL);
         while (wk.left > 0 && ok) {
           const int n = segment(wk), hk = wk.u / lay.row_tiles;
           for (int j = wk.j; j < wk.j + n; ++j, turn.next(stages)) {
