@@ -9,8 +9,8 @@
 //     r moves only when a logit is 27 above it: moved with every new maximum, it cost a branch in most vectors.  The difference is taken
 //     before the factor log2 e: large logits lose nothing, and rows of the type's lowest value have exponents of zero like any others.
 //   * Each of a CTA's 8 warps has ceil(W / 8) threads whose largest logit is at least the warp's ceil(W / 8)-th largest.  So at least W logits
-//     reach the least of these over the warps, a bound that costs a warp-wide maximum or a few.  Taken after each thread's first four
-//     vectors, which lie spread over the range, it leaves about 22 * rounds / 4 vectors of 8 beams that reach it and are noted; taken
+//     reach the least of these over the warps, a bound that costs a warp-wide maximum or a few.  Taken after each thread's first two
+//     vectors, and whenever there are twice as many, it leaves about a hundred vectors for 8 beams that reach it and are noted; taken
 //     again at the end, about 22.  A list that every warp kept on the way, with an insertion
 //     for each of W ln(n / W) logits, took 98 us for 64 x 8 x 128 256 in bf16; reading all vectors of the threads that reach the bound 92.
 //   * Candidates are 64-bit keys: the logit's bits in an order-preserving form, then the complement of its index, so that of equal
@@ -37,7 +37,7 @@ constexpr int WARPS = 8;
 constexpr int THREADS = WARPS * 32;
 constexpr int CTAS = 8;         // of a cluster
 constexpr int MAX_PARTS = MAX_BEAMS / CTAS + 1;       // rows that a CTA's range meets
-constexpr int NOTES = 1024;     // vectors that a CTA notes (24 KB); more (logits in rising order, equal ones) go through lists
+constexpr int NOTES = 512;      // vectors that a CTA notes (20 KB); more (logits in rising order, equal ones) go through lists
 constexpr int ROOM = 512;             // candidates that a CTA sorts, likewise
 
 typedef unsigned long long Key;
@@ -91,53 +91,66 @@ struct TopList {
   }
 };
 
-// Logits as floats: 16 bytes of them, and their maximum, which is NaN where one of them is.
+// 32 bytes of logits, on 32 bytes: the widest load there is.
+struct Raw {
+  uint32_t w[8];
+};
+__device__ __forceinline__ Raw load_raw(const Raw* p) {
+  Raw v;
+  asm("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+      : "=r"(v.w[0]), "=r"(v.w[1]), "=r"(v.w[2]), "=r"(v.w[3]), "=r"(v.w[4]), "=r"(v.w[5]), "=r"(v.w[6]), "=r"(v.w[7])
+      : "l"(p));
+  return v;
+}
 __device__ __forceinline__ float max_or_nan(float a, float b) {
   float r;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
+// Them as floats, and their maximum, which is NaN where one of them is.
 template <typename T>
 struct Logits;
 template <>
 struct Logits<float> {
   static constexpr uint32_t NONE = 0xff800000u;   // -inf in all of a word
-  static constexpr int N = 4;
+  static constexpr int N = 8;
   static __device__ __forceinline__ float one(const float* p) { return *p; }
-  static __device__ __forceinline__ float load(const uint4& v, float (&x)[N]) {
-    x[0] = __uint_as_float(v.x), x[1] = __uint_as_float(v.y), x[2] = __uint_as_float(v.z), x[3] = __uint_as_float(v.w);
-    return max_or_nan(max_or_nan(x[0], x[1]), max_or_nan(x[2], x[3]));
+  static __device__ __forceinline__ float load(const Raw& v, float (&x)[N]) {
+    float m[4];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(v.w[i]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m[i] = max_or_nan(x[2 * i], x[2 * i + 1]);
+    return max_or_nan(max_or_nan(m[0], m[1]), max_or_nan(m[2], m[3]));
   }
 };
 template <>
 struct Logits<__nv_bfloat16> {
-  static constexpr uint32_t NONE = 0xff80ff80u;   // -inf in all of a word
-  static constexpr int N = 8;
+  static constexpr uint32_t NONE = 0xff80ff80u;
+  static constexpr int N = 16;
   static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
     uint32_t r;
     asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
     return r;
   }
   static __device__ __forceinline__ float one(const __nv_bfloat16* p) { return __uint_as_float(uint32_t(*reinterpret_cast<const uint16_t*>(p)) << 16); }
-  static __device__ __forceinline__ float load(const uint4& v, float (&x)[N]) {
-    const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+  static __device__ __forceinline__ float load(const Raw& v, float (&x)[N]) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[2 * i] = __uint_as_float(u[i] << 16), x[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
-    const uint32_t m = max2(max2(v.x, v.y), max2(v.z, v.w));
+    for (int i = 0; i < 8; ++i) x[2 * i] = __uint_as_float(v.w[i] << 16), x[2 * i + 1] = __uint_as_float(v.w[i] & 0xffff0000u);
+    const uint32_t m = max2(max2(max2(v.w[0], v.w[1]), max2(v.w[2], v.w[3])), max2(max2(v.w[4], v.w[5]), max2(v.w[6], v.w[7])));
     return max_or_nan(__uint_as_float(m << 16), __uint_as_float(m & 0xffff0000u));
   }
 };
 template <>
 struct Logits<__half> {
-  static constexpr uint32_t NONE = 0xfc00fc00u;   // -inf in all of a word
-  static constexpr int N = 8;
+  static constexpr uint32_t NONE = 0xfc00fc00u;
+  static constexpr int N = 16;
   static __device__ __forceinline__ float one(const __half* p) { return __half2float(*p); }
-  static __device__ __forceinline__ float load(const uint4& v, float (&x)[N]) {
-    const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+  static __device__ __forceinline__ float load(const Raw& v, float (&x)[N]) {
     float m = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u[i]));
+    for (int i = 0; i < 8; ++i) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&v.w[i]));
       x[2 * i] = f.x, x[2 * i + 1] = f.y;
       m = max_or_nan(m, max_or_nan(f.x, f.y));
     }
@@ -158,7 +171,7 @@ kf_beam_select(const T* __restrict__ logits, long long stride_b, long long strid
                long long* __restrict__ out_parents, long long* __restrict__ out_tokens, uint8_t* __restrict__ out_finished) {
   constexpr int N = Logits<T>::N;
   constexpr float LOG2E = 1.4426950408889634f, HIGH = 27.f;
-  constexpr int UNROLL = 4;
+  constexpr int UNROLL = 2;
   // What a CTA found in its part of a row, in the first CTA's memory.  Part (nth row, CTA) has number nth + CTA: along the vectors every
   // step raises one of the two.
   struct Part {
@@ -171,12 +184,12 @@ kf_beam_select(const T* __restrict__ logits, long long stride_b, long long strid
   __shared__ uint32_t reach[2][WARPS];             // after the first round, at the end
   __shared__ int n_found[MAX_PARTS], n_notes[MAX_PARTS];
   __shared__ Key notes[NOTES];                     // (largest logit, vector)
-  __shared__ uint4 noted_raw[NOTES];               // the vector
+  __shared__ Raw noted_raw[NOTES];                 // the vector
   __shared__ Key found[ROOM];                      // candidates, or the warps' lists
   __shared__ int winner[MAX_BEAMS];                // of each place: which candidate
-  double* total = reinterpret_cast<double*>(notes);   // [W][W], best first, -inf: none
+  double* total = reinterpret_cast<double*>(noted_raw);   // [W][W], best first, -inf: none
   uint32_t* token = reinterpret_cast<uint32_t*>(found);
-  static_assert(sizeof(notes) >= MAX_BEAMS * MAX_BEAMS * 8 && sizeof(found) >= MAX_BEAMS * MAX_BEAMS * 4, "");
+  static_assert(sizeof(noted_raw) >= MAX_BEAMS * MAX_BEAMS * 8 && sizeof(found) >= MAX_BEAMS * MAX_BEAMS * 4, "");
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tid = threadIdx.x;
   const int rank = int(cluster_ctarank());
@@ -202,25 +215,29 @@ kf_beam_select(const T* __restrict__ logits, long long stride_b, long long strid
     // the nth live beam
     const int w = __ffs(__ballot_sync(0xffffffffu, ((live >> lane) & 1u) && __popc(live & ((1u << lane) - 1u)) == int(nth))) - 1;
     const T* x0 = logits + b * stride_b + w * stride_w;
-    // vectors from the row's first 16-byte boundary on; what is left at both ends goes with the first vector, a value a thread
-    const int misaligned = int(reinterpret_cast<uintptr_t>(x0) & 15) / int(sizeof(T));
+    // vectors from the row's first 32-byte boundary on; what is left at both ends goes with the first vector, a value a thread
+    const int misaligned = int(reinterpret_cast<uintptr_t>(x0) & 31) / int(sizeof(T));
     const int head = misaligned ? min(V, N - misaligned) : 0;
     const int vectors = (V - head) / N, tail0 = head + vectors * N;
     const int v1 = min(v_end, vectors);
-    const uint4* vec = reinterpret_cast<const uint4*>(x0 + head);
+    const Raw* vec = reinterpret_cast<const Raw*>(x0 + head);
     const int single = v0 != 0 || tid >= 2 * N ? -1 : tid < head ? tid : tid >= N && tid - N < V - tail0 ? tail0 + tid - N : -1;
-    // Four streams of rounds through the range, a vector a thread each; a vector is asked for as the one before it is taken.
-    const int rounds = v1 > v0 ? (v1 - v0 + THREADS - 1) / THREADS : 0, quarter = (rounds + UNROLL - 1) / UNROLL;
-    const int own_rounds = v1 - v0 > tid ? (v1 - v0 - tid + THREADS - 1) / THREADS : 0;
-    const uint4* mine0 = vec + v0 + tid;
-    auto fetch = [&](int round) {   // vectors that are not there hold -inf
-      uint4 v = make_uint4(Logits<T>::NONE, Logits<T>::NONE, Logits<T>::NONE, Logits<T>::NONE);
-      if (round < own_rounds) v = mine0[round * THREADS];
+    // Rounds of a vector a thread: two streams, the whole rounds' first and second half, and a last turn with what is left; a vector is
+    // asked for as the one before it is taken.
+    const int n_vec = v1 > v0 ? v1 - v0 : 0, half = n_vec / THREADS / UNROLL;
+    const Raw* mine0 = vec + v0 + tid;
+    auto round_of = [&](int u, int j) { return j < half ? u * half + j : UNROLL * half + u; };
+    auto fetch = [&](int u, int j) {
+      if (j < half) return load_raw(mine0 + (u * half + j) * THREADS);
+      Raw v;   // vectors that are not there hold -inf
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v.w[e] = Logits<T>::NONE;
+      if (j == half && (UNROLL * half + u) * THREADS + tid < n_vec) v = load_raw(mine0 + (UNROLL * half + u) * THREADS);
       return v;
     };
-    uint4 now[UNROLL];
+    Raw now[UNROLL];
 #pragma unroll
-    for (int u = 0; u < UNROLL; ++u) now[u] = fetch(quarter > 0 ? u * quarter : own_rounds);
+    for (int u = 0; u < UNROLL; ++u) now[u] = fetch(u, 0);
     const float alone = single >= 0 ? clean(Logits<T>::one(x0 + single)) : -INFINITY;
 
     // ---- the first round's largest
@@ -251,14 +268,19 @@ kf_beam_select(const T* __restrict__ logits, long long stride_b, long long strid
       for (int i = 1; i < full; ++i) least = min(least, of[i]);
       return least;
     };
-    float least_f = -INFINITY;
-    auto bound = [&]() {
+    volatile uint32_t* so_far = reach[0];
+    auto publish = [&]() {
       const uint32_t top = reached();
-      if (lane == 0) reach[0][warp] = top;
-      __syncthreads();
-      const uint32_t least = least_of(reach[0]);
+      if (lane == 0) so_far[warp] = top;
+    };
+    float least_f = -INFINITY;
+    auto bound = [&]() {   // what a warp reaches only grows: an older value of another one is a bound as well
+      uint32_t least = so_far[0];
+      for (int i = 1; i < full; ++i) least = min(least, so_far[i]);
       if (least) least_f = unordered(least);
     };
+    publish();
+    __syncthreads();
     bound();
 
     // ---- the pass: exp(x - r); limit: the logit that is HIGH above r
@@ -266,7 +288,7 @@ kf_beam_select(const T* __restrict__ logits, long long stride_b, long long strid
     float usual = fminf(least_f, limit);   // vectors whose largest is below only add to the sum
     uint64_t sum2[2] = {pack2(alone > -INFINITY ? exp2_fast((alone - r) * LOG2E) : 0.f, 0.f), 0ull};
 #pragma unroll 1
-    for (int j = 0; j < quarter; ++j) {
+    for (int j = 0; j <= half; ++j) {
 #pragma unroll
       for (int u = 0; u < UNROLL; ++u) {
         float x[N];
@@ -286,11 +308,11 @@ kf_beam_select(const T* __restrict__ logits, long long stride_b, long long strid
           }
           if (mx >= least_f && mx > -INFINITY) {
             const int to = atomicAdd(&n_notes[part], 1);
-            if (to < NOTES) notes[to] = make_key(mx, uint32_t(v0 + (u * quarter + j) * THREADS + tid)), noted_raw[to] = now[u];
+            if (to < NOTES) notes[to] = make_key(mx, uint32_t(v0 + round_of(u, j) * THREADS + tid)), noted_raw[to] = now[u];
           }
           usual = fminf(least_f, limit);
         }
-        now[u] = fetch(j + 1 < quarter ? u * quarter + j + 1 : own_rounds);
+        now[u] = fetch(u, j + 1);
         m = max_of(m, mx);
         const uint64_t r2 = pack2(-r, -r), log2e2 = pack2(LOG2E, LOG2E);
 #pragma unroll
@@ -300,8 +322,9 @@ kf_beam_select(const T* __restrict__ logits, long long stride_b, long long strid
           sum2[(e >> 1) & 1] = fadd2(sum2[(e >> 1) & 1], pack2(exp2_fast(a), exp2_fast(c)));
         }
       }
-      if (j == quarter / 4 && j > 0) {   // of a quarter of the range
-        __syncthreads();                 // nobody reads the first bound any more
+      if (j > 0 && (j & (j - 1)) == 0) {   // of twice as many vectors
+        publish();
+        __syncwarp();
         bound();
         usual = fminf(least_f, limit);
       }
@@ -367,7 +390,7 @@ kf_beam_select(const T* __restrict__ logits, long long stride_b, long long strid
       for (int base = v0 + warp * 32; base < v1; base += THREADS) {
         const int i = base + lane;
         float x[N], mx = -INFINITY;
-        if (i < v1) Logits<T>::load(vec[i], x);
+        if (i < v1) Logits<T>::load(load_raw(vec + i), x);
 #pragma unroll
         for (int j = 0; j < N; ++j) mx = max_of(mx, x[j] = i < v1 ? clean(x[j]) : -INFINITY);
         if (!__any_sync(0xffffffffu, mx > -INFINITY && ordered(mx) >= max(least, uint32_t(list.worst >> 32)))) continue;
