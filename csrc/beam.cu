@@ -16,7 +16,8 @@
 //   * Candidates are 64-bit keys: the logit's bits in an order-preserving form, then the complement of its index, so that of equal
 //     logits the lowest index is the largest key.  There are few, so a candidate's place is how many are larger, counted; the cluster's
 //     CTAs put theirs into the first one's shared memory.
-// What bounds it: the logits are read once.
+// What bounds it: the logits are read once.  Launches are joined to the one before (programmatic launch): by itself a launch of clusters began
+// 2.4 us later.
 //
 // kf_beam_reorder.  state[b, w] = state[b, parent[b, w]] for all states in one launch.  A thread owns 16 bytes of a column: it reads
 // the column's W values and then writes them, so that parents may be any selection of beams, also in place, without a second buffer.
@@ -35,8 +36,9 @@ using decode::mapa_shared;
 constexpr int MAX_BEAMS = 32;   // a warp's list is one key per lane
 constexpr int WARPS = 8;
 constexpr int THREADS = WARPS * 32;
-constexpr int CTAS = 8;         // of a cluster
-constexpr int MAX_PARTS = MAX_BEAMS / CTAS + 1;       // rows that a CTA's range meets
+// CTAs of a cluster: 16 where all clusters' CTAs have an SM each, which few prompts need (1 x 8 x 128 256: 20.7 -> 16.6 us), else 8.
+constexpr int CTAS_FEW = 16, CTAS_MANY = 8;
+constexpr int MAX_PARTS = MAX_BEAMS / CTAS_MANY + 1;  // rows that a CTA's range meets
 constexpr int NOTES = 512;      // vectors that a CTA notes (20 KB); more (logits in rising order, equal ones) go through lists
 constexpr int ROOM = 512;             // candidates that a CTA sorts, likewise
 
@@ -178,7 +180,7 @@ kf_beam_select(const T* __restrict__ logits, long long stride_b, long long strid
     double r, sum;
     Key keys[MAX_BEAMS];
   };
-  __shared__ Part parts[MAX_BEAMS + CTAS];
+  __shared__ Part parts[MAX_BEAMS + CTAS_FEW];
   __shared__ float rs[2][WARPS];
   __shared__ double sums[2][WARPS];
   __shared__ uint32_t reach[2][WARPS];             // after the first round, at the end
@@ -192,18 +194,21 @@ kf_beam_select(const T* __restrict__ logits, long long stride_b, long long strid
   static_assert(sizeof(noted_raw) >= MAX_BEAMS * MAX_BEAMS * 8 && sizeof(found) >= MAX_BEAMS * MAX_BEAMS * 4, "");
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tid = threadIdx.x;
+  const uint32_t ctas = cluster_nctaid();
   const int rank = int(cluster_ctarank());
-  const long long b = blockIdx.x / CTAS, first = b * W;
+  const long long b = blockIdx.x / ctas, first = b * W;
   if (tid < MAX_PARTS) n_found[tid] = n_notes[tid] = 0;
   if (tid < MAX_BEAMS) winner[tid] = -1;
+  grid_dep_wait();
+  grid_dep_launch();
   // Beams whose logits count.  One without a score above -inf (or with NaN) has no candidates, a finished one has itself.
   const float score = lane < W ? scores[first + lane] : -INFINITY;
   const bool alive = score > -INFINITY;
   const bool done = lane < W && finished != nullptr && finished[first + lane];
   const uint32_t live = __ballot_sync(0xffffffffu, alive && !done);
-  const uint32_t per = (max(1u, uint32_t(V) / N) + CTAS - 1) / CTAS * CTAS;   // vectors of a row, at most; so that CTAs meet eighths of rows
+  const uint32_t per = (max(1u, uint32_t(V) / N) + CTAS_FEW - 1) / CTAS_FEW * CTAS_FEW;   // vectors of a row, at most; so that CTAs meet eighths of rows
   const uint32_t all = uint32_t(__popc(live)) * per;
-  const uint32_t chunk = all / CTAS;
+  const uint32_t chunk = all / ctas;
   const uint32_t r1 = chunk * (rank + 1);
   asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");   // waited for below: the first CTA is there to be written to
 
@@ -436,10 +441,10 @@ kf_beam_select(const T* __restrict__ logits, long long stride_b, long long strid
       const double own_r = lane < count ? p[lane].r : NONE;
       double r = own_r;
 #pragma unroll
-      for (int o = CTAS / 2; o > 0; o >>= 1) r = fmax(r, __shfl_xor_sync(0xffffffffu, r, o));
+      for (int o = CTAS_FEW / 2; o > 0; o >>= 1) r = fmax(r, __shfl_xor_sync(0xffffffffu, r, o));
       double sum = own_r > NONE ? p[lane].sum * double(exp2_fast(float(own_r - r) * LOG2E)) : 0.0;
 #pragma unroll
-      for (int o = CTAS / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      for (int o = CTAS_FEW / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
       const double lse = __shfl_sync(0xffffffffu, r + log(sum), 0);
       for (int i = lane; i < count * W; i += 32) {
         const Key mine = p[i / W].keys[i % W];
@@ -488,18 +493,28 @@ static int launch_select(const void* logits, long long stride_b, long long strid
                          long long eos, long long pad, float* out_scores, long long* out_parents, long long* out_tokens, uint8_t* out_finished,
                          int num_sms, cudaStream_t stream) {
   auto kern = kf_beam_select<T>;
+  static bool attr_set[16] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev >= 16 || !attr_set[dev]) {
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e != cudaSuccess) return 300 + (int)e;
+    if (dev < 16) attr_set[dev] = true;
+  }
   cudaLaunchConfig_t cfg = {};
-  const int ctas = CTAS;
+  const int ctas = (long long)B * CTAS_FEW <= num_sms ? CTAS_FEW : CTAS_MANY;
   if ((long long)B * ctas > 0x7fffffffLL) return 6;
   cfg.gridDim = dim3((unsigned)(B * ctas));
   cfg.blockDim = dim3(THREADS);
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = (unsigned)ctas;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = 2;
   cudaError_t e = cudaLaunchKernelEx(&cfg, kern, (const T*)logits, stride_b, stride_w, scores, finished, W, V, eos, pad, out_scores, out_parents,
                                      out_tokens, out_finished);
   return e == cudaSuccess ? 0 : 500 + (int)e;
@@ -523,6 +538,8 @@ struct States {
 template <typename T, int W, int COLS>
 __global__ void __launch_bounds__(256)
 kf_beam_reorder(const __grid_constant__ States st, int beams, const void* __restrict__ parents, int wide) {
+  grid_dep_wait();
+  grid_dep_launch();
   const State& a = st.s[blockIdx.z];
   const long long b = blockIdx.y;
   const long long off0 = ((long long)blockIdx.x * (256 * COLS) + threadIdx.x) * (long long)sizeof(T);
@@ -572,8 +589,16 @@ kf_beam_reorder(const __grid_constant__ States st, int beams, const void* __rest
 template <typename T, int W, int COLS>
 static void launch_columns(const States& st, int n, int B, int beams, const void* parents, int wide, long long bytes, cudaStream_t stream) {
   const long long step = 256LL * COLS * sizeof(T);
-  const dim3 grid((unsigned)((bytes + step - 1) / step), (unsigned)B, (unsigned)n);
-  kf_beam_reorder<T, W, COLS><<<grid, 256, 0, stream>>>(st, beams, parents, wide);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)((bytes + step - 1) / step), (unsigned)B, (unsigned)n);
+  cfg.blockDim = dim3(256);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cudaLaunchKernelEx(&cfg, kf_beam_reorder<T, W, COLS>, st, beams, parents, wide);   // the caller asks for the last error
 }
 
 template <typename T>
