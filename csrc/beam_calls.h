@@ -16,9 +16,9 @@ struct Beam {
   int (*select)(const void*, int, long long, long long, const void*, const void*, int, int, int, long long, long long, void*, void*, void*, void*, int,
                 void*) = nullptr;
   int (*reorder)(const long long*, int, int, int, const void*, int, void*) = nullptr;
-  long long (*scratch)(int, int, int, int, int, int, int) = nullptr;
+  long long (*scratch)(int, int, int, int, int, int, int, int) = nullptr;
   int (*attention)(const void*, const void*, const void*, const void*, const void*, const void*, const void*, void*, void*, int, int, int, int, int, int,
-                   int, const long long*, float, int, void*) = nullptr;
+                   int, const long long*, float, int, int, void*) = nullptr;
   int max_beams = 0, max_states = 0;
 } bm;
 
@@ -154,7 +154,7 @@ bool steps_of(const at::Tensor& t, long long*& steps) {
   return true;
 }
 
-// shared_prefix_attn(q, k, v, own_k, own_v, prefix_lens or None, own_rows or None, scale or None, sms, device, stream) -> (B, W, H, hd)
+// shared_prefix_attn(q, k, v, own_k, own_v, prefix_lens or None, own_rows or None, scale or None, sms, device, stream) -> ((B, W, H, hd), launches)
 PyObject* shared_prefix_attn(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   long device = 0;
   void* stream = nullptr;
@@ -185,16 +185,16 @@ PyObject* shared_prefix_attn(PyObject*, PyObject* const* args, Py_ssize_t nargs)
   steps[17] = rows ? rows->stride(0) : 0;
   steps[18] = rows ? rows->stride(1) : 0;
   HANDLE_TH_ERRORS
-  const long long bytes = bm.scratch(int(b), int(w), int(p), int(h), int(hkv), int(hd), int(sms));
+  const long long bytes = bm.scratch(int(b), int(w), int(p), int(h), int(hkv), int(hd), -1, int(sms));
   if (bytes < 0) Py_RETURN_NONE;
   at::Tensor scratch, out = at::empty({b, w, h, hd}, q.options());
   if (bytes) scratch = at::empty({bytes}, q.options().dtype(at::kByte));
   const int rc = issued([&] {
     return bm.attention(q.const_data_ptr(), k.const_data_ptr(), t[2]->const_data_ptr(), ok.const_data_ptr(), t[4]->const_data_ptr(),
                         lens ? lens->const_data_ptr() : nullptr, rows ? rows->const_data_ptr() : nullptr, at_(out), bytes ? at_(scratch) : nullptr,
-                        int(b), int(w), int(p), int(s), int(h), int(hkv), int(hd), steps, float(scale), int(sms), stream);
+                        int(b), int(w), int(p), int(s), int(h), int(hkv), int(hd), steps, float(scale), -1, int(sms), stream);
   });
-  return rc ? PyLong_FromLong(rc) : THPVariable_Wrap(std::move(out));
+  return rc ? PyLong_FromLong(rc) : Py_BuildValue("(Ni)", wrap(std::move(out)), bytes ? 2 : 1);
   END_HANDLE_TH_ERRORS
 }
 

@@ -9,6 +9,9 @@
 //     XOR-swizzled, so that ldmatrix is free of bank conflicts; a warp of one or two tiles has them all under way at once;
 //   * the (max, sum, output) triples of the warps, of the CTAs of a cluster and of the prompt are joined in a fixed order.
 // All of it up to that last step runs without the prompt's kernel, and starts on the SMs that it leaves (programmatic launch).
+//
+// Where the prompts are short, this kernel alone reads them too, for every continuation again (out of L2), as the tiles before those of its
+// own: `direct`.  What that costs is traffic, what it saves a launch, the partial results and the wait between the kernels.
 #include "decode_common.cuh"
 #include "shared_prefix.cuh"
 
@@ -44,6 +47,9 @@ struct Own {
   __nv_bfloat16* o;
   const uint8_t* rows;                                       // [B][W][S] or null
   int S, Hkv, group;
+  const __nv_bfloat16 *pk, *pv;                              // the prompts, where they are read here
+  int direct;
+  long long pk_b, pk_s, pk_h, pv_b, pv_s, pv_h;
   long long q_b, q_w, q_h, k_b, k_w, k_s, k_h, v_b, v_w, v_s, v_h;   // elements
   long long r_b, r_w;
   float scale_log2;
@@ -74,16 +80,20 @@ kf_shared_prefix_own(const Own a, const Layout lay, const float* part_o, const f
   const int n_heads = there ? min(OWN_ROWS, a.group - hb * OWN_ROWS) : 0;     // query heads of this unit
   const int h0 = hk * a.group + hb * OWN_ROWS;
 
-  const int n_tiles = there ? (a.S + OWN_TILE - 1) / OWN_TILE : 0;
+  const int plen = a.direct ? length(lay, b) : 0, prompt_tiles = (plen + OWN_TILE - 1) / OWN_TILE;
+  const int n_tiles = there ? prompt_tiles + (a.S + OWN_TILE - 1) / OWN_TILE : 0;
   const int each = (n_tiles + ways - 1) / ways, t0 = min(n_tiles, each * way), t1 = min(n_tiles, t0 + each);
   const __nv_bfloat16* kb = a.k + b * a.k_b + hk * a.k_h;
   const __nv_bfloat16* vb = a.v + b * a.v_b + hk * a.v_h;
+  const __nv_bfloat16 *pkb = a.pk + b * a.pk_b + hk * a.pk_h, *pvb = a.pv + b * a.pv_b + hk * a.pv_h;
   const uint8_t* table = a.rows ? a.rows + b * a.r_b + w * a.r_w : nullptr;
 
-  // whose cache holds the lane's key of the two tiles from t on (lay.W: nobody's)
+  // whose cache holds the lane's key of the two tiles from t on (-1: the prompt's, lay.W: nobody's)
   auto slots_of = [&](int t) {
-    const int pos = t * OWN_TILE + lane;
-    return t + (lane >> 4) >= t1 || pos >= a.S ? lay.W : table ? int(table[pos]) : w;
+    const int tile = t + (lane >> 4), pos = t * OWN_TILE + lane, own = pos - prompt_tiles * OWN_TILE;
+    if (tile >= t1) return lay.W;
+    if (tile < prompt_tiles) return pos < plen ? -1 : lay.W;
+    return own >= a.S ? lay.W : table ? int(table[own]) : w;
   };
   int slots = slots_of(t0), ahead = t0 + 2 < t1 ? slots_of(t0 + 2) : lay.W;   // of the tiles issued next and the two after them
   // Four lanes a key: 64 bytes side by side at a time, of keys lane / 4 and that + 8.  The 16-byte chunk c of row r lies at c ^ (r & 7).
@@ -100,8 +110,9 @@ kf_shared_prefix_own(const Own a, const Layout lay, const float* part_o, const f
     for (int h = 0; h < 2; ++h) {
       const int r = row0 + h * 8, sl = __shfl_sync(0xffffffffu, slots, half + r);
       const bool in = (mask >> r) & 1u;
-      const long long pos = in ? t * OWN_TILE + r : 0, of = in ? sl : 0;
-      const __nv_bfloat16 *kp = kb + of * a.k_w + pos * a.k_s + (lane & 3) * 8, *vp = vb + of * a.v_w + pos * a.v_s + (lane & 3) * 8;
+      const long long of = in ? sl : 0, pos = in ? (t - (of < 0 ? 0 : prompt_tiles)) * OWN_TILE + r : 0;
+      const __nv_bfloat16* kp = (of < 0 ? pkb + pos * a.pk_s : kb + of * a.k_w + pos * a.k_s) + (lane & 3) * 8;
+      const __nv_bfloat16* vp = (of < 0 ? pvb + pos * a.pv_s : vb + of * a.v_w + pos * a.v_s) + (lane & 3) * 8;
 #pragma unroll
       for (int c = 0; c < HD / 32; ++c) {
         const uint32_t dst = (dst0 ^ uint32_t(c * 64)) + uint32_t(h * 8 * HD * 2);
@@ -364,20 +375,21 @@ static int launch_ways(const Own& a, const Layout& l, const float* part_o, const
 template <int HD>
 static int launch_own(const Own& a, const Layout& l, const float* part_o, const float2* part_ml, int num_sms, cudaStream_t stream) {
   const long long units = (long long)l.B * l.W * a.Hkv * ((a.group + OWN_ROWS - 1) / OWN_ROWS);
-  const int tiles = (a.S + OWN_TILE - 1) / OWN_TILE;
+  const int tiles = (a.S + OWN_TILE - 1) / OWN_TILE + (a.direct ? (l.P + OWN_TILE - 1) / OWN_TILE : 0);
   auto go = [&](auto ring, int ways) {
     constexpr int R = decltype(ring)::value;
     if (ways == 1) return launch_ways<HD, 1, R>(a, l, part_o, part_ml, units, 1, stream);
     if (ways == 2) return launch_ways<HD, 2, R>(a, l, part_o, part_ml, units, 1, stream);
     return launch_ways<HD, 4, R>(a, l, part_o, part_ml, units, ways / 4, stream);
   };
-  // One or two tiles a warp, where that takes a CTA a unit at most and no more than 16 warps on an SM, which is what registers and
+  // One or two tiles a warp, where that takes a CTA a unit at most and no more than 16 or 12 warps on an SM, which is what registers or
   // memory hold: everything is under way at once, and nothing crosses CTAs (8 x 5 continuations of 65 keys: 27.2 -> 23 us, 1 x 8 of 96
-  // 15.6 -> 13).  Else as many warps a unit as fill eight on every SM, of which each has a tile at least.
+  // 15.6 -> 13; but 8 x 8 of 65, 14 warps an SM, 17.8, and streaming 12.9).  Else as many warps a unit as fill eight on every SM, of which
+  // each has a tile at least.
   for (int ring = 1; ring <= 2; ++ring) {
     int ways = 1;
     while (ways < 4 && ways * ring < tiles) ways *= 2;
-    if (ways * ring >= tiles && units * ways <= 16LL * num_sms)
+    if (ways * ring >= tiles && units * ways <= (ring == 1 ? 16LL : 12LL) * num_sms)
       return ring == 1 ? go(std::integral_constant<int, 1>(), ways) : go(std::integral_constant<int, 2>(), ways);
   }
   int ways = 1;
@@ -397,6 +409,14 @@ static bool make_layout(Layout& l, const void* lens, int B, int W, int P, int gr
   return tiles < 0x7fff0000LL && (long long)B * W * Hkv * group < 1LL << 27;   // counts of tiles and units in 32 bits
 }
 
+// Bytes of the prompts, once for every continuation, up to which one kernel reads them all.  In a graph, direct / two kernels, us:
+// 3.5 MB (1 x 4 x 300, 12 heads of 64) 6.4 / 6.8, 16 MB (1 x 8 x 500, 8 heads of 128) 10.0 / 7.5; eager, 3.5 MB, 8.2 / 10.9: a launch
+// and an allocation less for the host.
+constexpr long long DIRECT_BYTES = 4LL << 20;
+static bool is_direct(int direct, int B, int W, int P, int Hkv, int hd) {
+  return P > 0 && (direct < 0 ? 4LL * B * W * P * Hkv * hd <= DIRECT_BYTES : direct != 0);
+}
+
 }  // namespace shared_prefix
 }  // namespace kf
 
@@ -404,12 +424,13 @@ extern "C" void* kf_status_device_ptr();
 
 extern "C" {
 
-// Bytes of scratch that kf_shared_prefix_attn_bf16 needs for these sizes (0: none), negative where it does not take them.
-long long kf_shared_prefix_scratch(int B, int W, int P, int H, int Hkv, int hd, int num_sms) {
+// Bytes of scratch that kf_shared_prefix_attn_bf16 needs for these sizes (0: none, and one launch), negative where it does not take them.
+// direct: whether the prompts are read for every continuation again; below 0: where that is the faster way.
+long long kf_shared_prefix_scratch(int B, int W, int P, int H, int Hkv, int hd, int direct, int num_sms) {
   using namespace kf::shared_prefix;
   Layout l;
   if (B < 1 || W < 1 || P < 0 || Hkv < 1 || H % Hkv || (hd != 64 && hd != 128) || !make_layout(l, nullptr, B, W, P, H / Hkv, Hkv, num_sms)) return -1;
-  return P == 0 ? 0 : slots(l) * TILE_ROWS * (hd * 4 + 8);
+  return P == 0 || is_direct(direct, B, W, P, Hkv, hd) ? 0 : slots(l) * TILE_ROWS * (hd * 4 + 8);
 }
 
 // o (B, W, H, hd), dense = attention of q (B, W, H, hd) over k, v (B, P, Hkv, hd), of which lens[b] positions count (null: all), and over
@@ -418,23 +439,24 @@ long long kf_shared_prefix_scratch(int B, int W, int P, int H, int Hkv, int hd, 
 // head) and rows (prompt, continuation): 19 numbers.  Head dim 64 or 128, dense; steps multiples of 8 and bases on 16 bytes (rows: any).
 int kf_shared_prefix_attn_bf16(const void* q, const void* k, const void* v, const void* own_k, const void* own_v, const void* lens,
                                const void* rows, void* o, void* scratch, int B, int W, int P, int S, int H, int Hkv, int hd,
-                               const long long* steps, float scale, int num_sms, void* stream) {
+                               const long long* steps, float scale, int direct, int num_sms, void* stream) {
   using namespace kf::shared_prefix;
   Layout l;
-  if (kf_shared_prefix_scratch(B, W, P, H, Hkv, hd, num_sms) < 0 || S < 0 || !(scale > 0.f)) return 3;
+  if (kf_shared_prefix_scratch(B, W, P, H, Hkv, hd, direct, num_sms) < 0 || S < 0 || !(scale > 0.f)) return 3;
   make_layout(l, lens, B, W, P, H / Hkv, Hkv, num_sms);
   const long long *qs = steps, *ks = steps + 3, *vs = steps + 6, *oks = steps + 9, *ovs = steps + 13, *rs = steps + 17;
   for (int i = 0; i < 17; ++i)
     if (steps[i] & 7) return 5;
   cudaStream_t st = (cudaStream_t)stream;
-  float* part_o = P > 0 ? (float*)scratch : nullptr;
-  float2* part_ml = P > 0 ? (float2*)(part_o + slots(l) * TILE_ROWS * hd) : nullptr;
-  if (P > 0) {
+  const bool alone = P == 0 || is_direct(direct, B, W, P, Hkv, hd);
+  float* part_o = alone ? nullptr : (float*)scratch;
+  float2* part_ml = alone ? nullptr : (float2*)(part_o + slots(l) * TILE_ROWS * hd);
+  if (!alone) {
     const int rc = launch_prefix(q, k, v, l, H, Hkv, hd, qs, ks, vs, scale, part_o, part_ml, (int*)kf_status_device_ptr(), st);
     if (rc) return rc;
   }
   const Own a{(const __nv_bfloat16*)q, (const __nv_bfloat16*)own_k, (const __nv_bfloat16*)own_v, (__nv_bfloat16*)o, (const uint8_t*)rows, S, Hkv,
-              H / Hkv, qs[0], qs[1], qs[2], oks[0], oks[1], oks[2], oks[3], ovs[0], ovs[1], ovs[2], ovs[3], rs[0], rs[1],
+              H / Hkv, (const __nv_bfloat16*)k, (const __nv_bfloat16*)v, alone && P > 0, ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], qs[0], qs[1], qs[2], oks[0], oks[1], oks[2], oks[3], ovs[0], ovs[1], ovs[2], ovs[3], rs[0], rs[1],
               scale * 1.4426950408889634f};
   return hd == 128 ? launch_own<128>(a, l, part_o, part_ml, num_sms, st) : launch_own<64>(a, l, part_o, part_ml, num_sms, st);
 }

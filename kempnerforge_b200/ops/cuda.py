@@ -139,8 +139,8 @@ def _declare(L: ctypes.CDLL) -> None:
         "kf_symm_pull_bf16": [vp, i, i, vp, vp, vp, vp, i, vp],
         "kf_symm_rs_shard_bf16": [vp, vp, i, i, i, vp, vp, vp, vp, i, i, vp],
         "kf_gemm_gather_bf16": [i, vp, vp, vp, i, i, i, i, i, i, vp, i, i, i, vp, vp, vp, vp, vp, vp, i, i, i, i, vp],
-        "kf_shared_prefix_scratch": [i] * 7,
-        "kf_shared_prefix_attn_bf16": [vp] * 9 + [i] * 7 + [vp, f, i, vp],
+        "kf_shared_prefix_scratch": [i] * 8,
+        "kf_shared_prefix_attn_bf16": [vp] * 9 + [i] * 7 + [vp, f, i, i, vp],
         "kf_beam_select": [vp, i, ll, ll, vp, vp, i, i, i, ll, ll, vp, vp, vp, vp, i, vp],
         "kf_beam_max_states": [],
         "kf_beam_reorder": [vp, i, i, i, vp, i, vp],
@@ -1089,32 +1089,34 @@ def _copies_ok(t: torch.Tensor) -> torch.Tensor:
 def shared_prefix_call(q, k, v, own_k, own_v, prefix_lens, own_rows, scale) -> torch.Tensor | None:
     """:func:`shared_prefix_attn`, checked as well; None where Python's checks have to look."""
     global LAUNCH_COUNT
-    out = _step("shared_prefix_attn", q, k, v, own_k, own_v, prefix_lens, own_rows, scale, sm_count())
-    if out is not None and k.shape[1]:
-        LAUNCH_COUNT += 1   # the kernel over the prompts
-    return out
+    r = _step("shared_prefix_attn", q, k, v, own_k, own_v, prefix_lens, own_rows, scale, sm_count(), launches=0)
+    if r is None:
+        return None
+    LAUNCH_COUNT += r[1]
+    return r[0]
 
 
 def shared_prefix_supported(q: torch.Tensor, k: torch.Tensor) -> bool:
     b, w, h, hd = q.shape
-    return k.shape[1] < 2**31 - 2**16 and b * w * h < 2**27 and lib().kf_shared_prefix_scratch(b, w, k.shape[1], h, k.shape[2], hd, sm_count()) >= 0
+    return k.shape[1] < 2**31 - 2**16 and b * w * h < 2**27 and lib().kf_shared_prefix_scratch(b, w, k.shape[1], h, k.shape[2], hd, -1, sm_count()) >= 0
 
 
-def shared_prefix_attn(q, k, v, own_k, own_v, prefix_lens, own_rows, scale: float) -> torch.Tensor:
-    """q (B, W, H, hd), k / v (B, P, Hkv, hd), own_k / own_v (B, W, S, Hkv, hd) bf16, prefix_lens (B,) int32, own_rows (B, W, S) uint8."""
+def shared_prefix_attn(q, k, v, own_k, own_v, prefix_lens, own_rows, scale: float, direct: int = -1) -> torch.Tensor:
+    """q (B, W, H, hd), k / v (B, P, Hkv, hd), own_k / own_v (B, W, S, Hkv, hd) bf16, prefix_lens (B,) int32, own_rows (B, W, S) uint8.
+    ``direct``: 1 reads the prompts for every continuation again, in one kernel, 0 once for all, in two; -1: the faster way."""
     q, k, v, own_k, own_v = (_copies_ok(t) for t in (q, k, v, own_k, own_v))
     b, w, h, hd = q.shape
     p, hkv, s = k.shape[1], k.shape[2], own_k.shape[2]
     if own_rows is not None and own_rows.stride(2) != 1:
         own_rows = own_rows.contiguous()
     L, sms = lib(), sm_count()
-    scratch = torch.empty(L.kf_shared_prefix_scratch(b, w, p, h, hkv, hd, sms), dtype=torch.uint8, device=q.device)
+    scratch = torch.empty(L.kf_shared_prefix_scratch(b, w, p, h, hkv, hd, direct, sms), dtype=torch.uint8, device=q.device)
     out = torch.empty((b, w, h, hd), dtype=q.dtype, device=q.device)
     rows = own_rows.stride()[:2] if own_rows is not None else (0, 0)
     steps = array("q", (*_steps_of(q), *_steps_of(k), *_steps_of(v), *_steps_of(own_k), *_steps_of(own_v), *rows))
     _check(L.kf_shared_prefix_attn_bf16(q.data_ptr(), k.data_ptr(), v.data_ptr(), own_k.data_ptr(), own_v.data_ptr(), _ptr(prefix_lens),
                                         _ptr(own_rows), out.data_ptr(), scratch.data_ptr(), b, w, p, s, h, hkv, hd, steps.buffer_info()[0],
-                                        float(scale), sms, _stream()), "kf_shared_prefix_attn_bf16", 2 if p else 1)
+                                        float(scale), direct, sms, _stream()), "kf_shared_prefix_attn_bf16", 2 if scratch.numel() else 1)
     return out
 
 

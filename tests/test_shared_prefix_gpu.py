@@ -36,9 +36,13 @@ def test_sizes(native_lib, b, w, p, s, h, hkv, hd, table, ragged):
     args = make(b, w, p, s, h, hkv, hd, torch.bfloat16, table, ragged, seed=p + s, device="cuda")
     before = native_lib.LAUNCH_COUNT
     got = F.shared_prefix_attention(*args)
-    assert native_lib.LAUNCH_COUNT == before + (2 if p else 1)
+    assert native_lib.LAUNCH_COUNT > before
     near(got, args)
     assert torch.equal(got, F.shared_prefix_attention(*args))
+    for direct in (0, 1):   # the prompts once for all, and for every continuation again
+        got = native_lib.shared_prefix_attn(*args, hd**-0.5, direct)
+        near(got, args)
+        assert torch.equal(got, native_lib.shared_prefix_attn(*args, hd**-0.5, direct))
     assert native_lib.read_status() == 0
 
 
@@ -51,6 +55,8 @@ def test_lengths(native_lib):
         k[i, n:], v[i, n:] = NAN, float("inf")
     for kind in (torch.int32, torch.int64):
         near(F.shared_prefix_attention(q, k, v, ok, ov, lens.to(kind)), (q, k, v, ok, ov, lens))
+    for direct in (0, 1):
+        near(native_lib.shared_prefix_attn(q, k, v, ok, ov, lens.int(), None, 128**-0.5, direct), (q, k, v, ok, ov, lens))
     # lengths that are none are taken to the nearest one
     past = torch.tensor([-5, 1, 4000, 128, -1, 0, 129, 256, 5], device="cuda", dtype=torch.int32)
     near(F.shared_prefix_attention(q, k, v, ok, ov, past), (q, k, v, ok, ov, lens))
@@ -62,6 +68,8 @@ def test_all_prompts_empty(native_lib):
     near(F.shared_prefix_attention(*args), args)
     args[6] = torch.full((3, 2, 3), 255, dtype=torch.uint8, device="cuda")
     assert (F.shared_prefix_attention(*args) == 0).all()
+    for direct in (0, 1):
+        assert (native_lib.shared_prefix_attn(*args, 0.125, direct) == 0).all()
 
 
 def test_what_is_hidden_may_hold_anything(native_lib):
@@ -77,18 +85,21 @@ def test_what_is_hidden_may_hold_anything(native_lib):
     for t in (ok, ov):
         t[:, 2] = NAN
         t[:, 1, :3] = NAN
-    got = F.shared_prefix_attention(q, k, v, ok, ov, lens, rows)
-    near(got, (q, k, v, ok, ov, lens, rows))
-    assert (got[1, 2] == 0).all()
+    calls = [F.shared_prefix_attention] + [lambda *a, d=d: native_lib.shared_prefix_attn(*a, 128**-0.5, d) for d in (0, 1)]
+    for call in calls:
+        got = call(q, k, v, ok, ov, lens, rows)
+        near(got, (q, k, v, ok, ov, lens, rows))
+        assert (got[1, 2] == 0).all()
     # what one continuation sees stays with it
     ov[0, 1, 10] = NAN
-    got = F.shared_prefix_attention(q, k, v, ok, ov, lens, rows)
-    assert torch.isnan(got[0, 1]).all() and torch.isfinite(got[0, 0]).all() and torch.isfinite(got[0, 2]).all() and torch.isfinite(got[1]).all()
+    for call in calls:
+        got = call(q, k, v, ok, ov, lens, rows)
+        assert torch.isnan(got[0, 1]).all() and torch.isfinite(got[0, 0]).all() and torch.isfinite(got[0, 2]).all() and torch.isfinite(got[1]).all()
 
 
 def test_large_scores(native_lib):
     """Scores of hundreds, in rising order, so that maxima move from tile to tile."""
-    args = make(1, 4, 700, 150, 4, 2, 128, torch.bfloat16, device="cuda")
+    args = make(1, 40, 700, 150, 4, 2, 128, torch.bfloat16, device="cuda")   # so many that the prompt is read once for all
     ramp = torch.linspace(0.2, 30.0, 700, device="cuda")[None, :, None, None]
     args[1] = (args[1].float().abs() * ramp).bfloat16()
     args[0] = args[0].abs()
