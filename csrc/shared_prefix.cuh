@@ -1,8 +1,9 @@
 // Attention of many continuations of one prompt: how the work over the prompts' keys is laid out.  Both kernels go by it.
 //
-// A unit is (prompt b, key head, row tile): up to 128 query rows, wt continuations times the query heads of the key head.  Its keys come in
-// tiles of 128.  The tiles of all units, one after the other, are dealt out to the CTAs in equal ranges, so that every SM has the same
-// share whatever the lengths of the prompts; a CTA leaves one partial result for every unit that its range meets.
+// A unit is (prompt b, key head, one or two row tiles): a row tile is up to 128 query rows, wt continuations times the query heads of the
+// key head, and with more rows than that two of them may share the keys.  Keys come in tiles of 128.  The tiles of all units, one after the
+// other, are dealt out to the CTAs in equal ranges, so that every SM has the same share whatever the lengths of the prompts; a CTA leaves
+// one partial result for every unit that its range meets.
 #pragma once
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -15,8 +16,9 @@ constexpr int TILE_KEYS = 128, TILE_ROWS = 128;
 struct Layout {
   const int* lens;     // keys of each prompt, or null: P for all
   int B, W, P;
-  int per_prompt;      // units of a prompt: key heads x row tiles
-  int row_tiles, wt;   // row tiles of a key head, continuations per row tile
+  int per_prompt;      // units of a prompt: key heads x row_units
+  int row_units;       // units of a key head
+  int pair, wt;        // row tiles of a unit, 1 or 2; continuations per row tile
   int ctas;
 };
 

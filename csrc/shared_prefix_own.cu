@@ -237,7 +237,7 @@ kf_shared_prefix_own(const Own a, const Layout lay, const float* part_o, const f
   }
   // ---- the prompt's partial results: which there are
   int c0 = 0, parts = 0;
-  const int u = hk * lay.row_tiles + w / lay.wt;
+  const int u = hk * lay.row_units + w / (lay.wt * lay.pair), slot_rows = TILE_ROWS * lay.pair;
   if (part_o != nullptr) {
     const uint32_t first = tiles_before(lay, b), chunk = range(tiles_before(lay, lay.B), lay.ctas);
     const int nt = there ? tiles_of(length(lay, b)) : 0;
@@ -251,7 +251,8 @@ kf_shared_prefix_own(const Own a, const Layout lay, const float* part_o, const f
   else cluster_sync_all();
   grid_dep_wait();
   grid_dep_launch();
-  const long long slot0 = ((long long)b * lay.per_prompt + u + c0) * TILE_ROWS + (w % lay.wt) * a.group + hb * OWN_ROWS;
+  const long long slot0 =
+      ((long long)b * lay.per_prompt + u + c0) * slot_rows + (w / lay.wt % lay.pair) * TILE_ROWS + (w % lay.wt) * a.group + hb * OWN_ROWS;
   const int warp0 = warp / WPU * WPU;
   const uint32_t part_a = smem_u32(smem_raw) + warp0 * C::WARP, stats_a = part_a + C::PART;
   auto own_at = [&](uint32_t base, int s) {   // of the unit's s-th warp
@@ -301,7 +302,7 @@ kf_shared_prefix_own(const Own a, const Layout lay, const float* part_o, const f
 #pragma unroll
         for (int j = 0; j < ITEMS; ++j)
           if (c + e < parts) {
-            const long long at = slot0 + r[j] + (long long)(c + e) * TILE_ROWS;
+            const long long at = slot0 + r[j] + (long long)(c + e) * slot_rows;
             x[j][e] = ld_after_wait(part_ml + at);
             v[j][e] = ld_after_wait(reinterpret_cast<const float4*>(part_o + at * HD + d[j]));
           }
@@ -400,12 +401,18 @@ static int launch_own(const Own& a, const Layout& l, const float* part_o, const 
 int launch_prefix(const void* q, const void* k, const void* v, const Layout& l, int H, int Hkv, int hd, const long long* qs, const long long* ks,
                   const long long* vs, float scale, float* part_o, float2* part_ml, int* status, cudaStream_t stream);
 
-static bool make_layout(Layout& l, const void* lens, int B, int W, int P, int group, int Hkv, int num_sms) {
+// Prompts of this many bytes outlast L2 (126 MB): two row tiles share a key.  Otherwise the second finds it there, and units of one tile
+// deal out more evenly and join both groups.  Alone / shared, us: 8 x 64 x 4000 (131 MB) 64.2 / 68.8, 1 x 32 x 32 768 (134 MB) 46.2 / 50.7,
+// 1 x 32 x 40 000 (164 MB) 55.0 / 56.6, 10 x 64 x 4000 (164 MB) 108.8 / 109.0, 12 x 64 x 4000 (197 MB) 133.9 / 127.4, 2 x 32 x 24 000
+// (197 MB) 76.3 / 61.4, 2 x 32 x 32 768 (268 MB) 98 / 76, 4 x 32 x 32 768 (537 MB) 184 / 142.
+constexpr long long PAIR_BYTES = 168LL << 20;
+
+static bool make_layout(Layout& l, const void* lens, int B, int W, int P, int group, int Hkv, int hd, int num_sms) {
   if (group > TILE_ROWS) return false;
   const int wt = TILE_ROWS / group < W ? TILE_ROWS / group : W;
-  const int row_tiles = (W + wt - 1) / wt;
-  const long long tiles = (long long)tiles_of(P) * Hkv * row_tiles * B;
-  l = Layout{(const int*)lens, B, W, P, Hkv * row_tiles, row_tiles, wt, (int)(tiles < num_sms ? tiles : num_sms)};
+  const int pair = wt < W && 4LL * B * P * Hkv * hd > PAIR_BYTES ? 2 : 1, row_units = (W + wt * pair - 1) / (wt * pair);
+  const long long tiles = (long long)tiles_of(P) * Hkv * row_units * B;
+  l = Layout{(const int*)lens, B, W, P, Hkv * row_units, row_units, pair, wt, (int)(tiles < num_sms ? tiles : num_sms)};
   return tiles < 0x7fff0000LL && (long long)B * W * Hkv * group < 1LL << 27;   // counts of tiles and units in 32 bits
 }
 
@@ -429,8 +436,9 @@ extern "C" {
 long long kf_shared_prefix_scratch(int B, int W, int P, int H, int Hkv, int hd, int direct, int num_sms) {
   using namespace kf::shared_prefix;
   Layout l;
-  if (B < 1 || W < 1 || P < 0 || Hkv < 1 || H % Hkv || (hd != 64 && hd != 128) || !make_layout(l, nullptr, B, W, P, H / Hkv, Hkv, num_sms)) return -1;
-  return P == 0 || is_direct(direct, B, W, P, Hkv, hd) ? 0 : slots(l) * TILE_ROWS * (hd * 4 + 8);
+  if (B < 1 || W < 1 || P < 0 || Hkv < 1 || H % Hkv || (hd != 64 && hd != 128)) return -1;
+  if (!make_layout(l, nullptr, B, W, P, H / Hkv, Hkv, hd, num_sms)) return -1;
+  return P == 0 || is_direct(direct, B, W, P, Hkv, hd) ? 0 : slots(l) * l.pair * TILE_ROWS * (hd * 4 + 8);
 }
 
 // o (B, W, H, hd), dense = attention of q (B, W, H, hd) over k, v (B, P, Hkv, hd), of which lens[b] positions count (null: all), and over
@@ -443,20 +451,21 @@ int kf_shared_prefix_attn_bf16(const void* q, const void* k, const void* v, cons
   using namespace kf::shared_prefix;
   Layout l;
   if (kf_shared_prefix_scratch(B, W, P, H, Hkv, hd, direct, num_sms) < 0 || S < 0 || !(scale > 0.f)) return 3;
-  make_layout(l, lens, B, W, P, H / Hkv, Hkv, num_sms);
+  make_layout(l, lens, B, W, P, H / Hkv, Hkv, hd, num_sms);
   const long long *qs = steps, *ks = steps + 3, *vs = steps + 6, *oks = steps + 9, *ovs = steps + 13, *rs = steps + 17;
   for (int i = 0; i < 17; ++i)
     if (steps[i] & 7) return 5;
   cudaStream_t st = (cudaStream_t)stream;
   const bool alone = P == 0 || is_direct(direct, B, W, P, Hkv, hd);
   float* part_o = alone ? nullptr : (float*)scratch;
-  float2* part_ml = alone ? nullptr : (float2*)(part_o + slots(l) * TILE_ROWS * hd);
+  float2* part_ml = alone ? nullptr : (float2*)(part_o + slots(l) * l.pair * TILE_ROWS * hd);
   if (!alone) {
     const int rc = launch_prefix(q, k, v, l, H, Hkv, hd, qs, ks, vs, scale, part_o, part_ml, (int*)kf_status_device_ptr(), st);
     if (rc) return rc;
   }
-  const Own a{(const __nv_bfloat16*)q, (const __nv_bfloat16*)own_k, (const __nv_bfloat16*)own_v, (__nv_bfloat16*)o, (const uint8_t*)rows, S, Hkv,
-              H / Hkv, (const __nv_bfloat16*)k, (const __nv_bfloat16*)v, alone && P > 0, ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], qs[0], qs[1], qs[2], oks[0], oks[1], oks[2], oks[3], ovs[0], ovs[1], ovs[2], ovs[3], rs[0], rs[1],
+  const Own a{(const __nv_bfloat16*)q, (const __nv_bfloat16*)own_k, (const __nv_bfloat16*)own_v, (__nv_bfloat16*)o, (const uint8_t*)rows,
+              S, Hkv, H / Hkv, (const __nv_bfloat16*)k, (const __nv_bfloat16*)v, alone && P > 0, ks[0], ks[1], ks[2], vs[0], vs[1], vs[2],
+              qs[0], qs[1], qs[2], oks[0], oks[1], oks[2], oks[3], ovs[0], ovs[1], ovs[2], ovs[3], rs[0], rs[1],
               scale * 1.4426950408889634f};
   return hd == 128 ? launch_own<128>(a, l, part_o, part_ml, num_sms, st) : launch_own<64>(a, l, part_o, part_ml, num_sms, st);
 }

@@ -3,9 +3,10 @@
 // The W continuations of a prompt and the query heads of a key head are the rows of one tile, up to 128 of them, so that a key is read
 // once for all and S = Q K^T and O += P V are 128-row products on the tensor cores; one kernel per continuation reads it W times.
 // What bounds it: the keys and values, 4 hd bytes per position and head.  A tile of 128 keys of 128 values is 64 KB, which is 2700 cycles
-// of an SM's share of HBM; its two products take 512, its 16 384 exponentials 1024.  So rows that are not there (a tile is always 128)
+// of an SM's share of HBM; its two products take 1040, its 16 384 exponentials 1024.  So rows that are not there (a tile is always 128)
 // cost nothing, and all that counts is to keep the copies in flight: two stages each of K and V (128 KB) run ahead of the products.  Three
-// were slower (4 x 32 768 keys, 64 heads of 128, with the second kernel: 102 and 98 us).
+// were slower (4 x 32 768 keys, 64 heads of 128, with the second kernel: 102 and 98 us).  Prompts that L2 holds (64 continuations of 8000
+// keys: four row tiles read them) are bound by the chain scores - weights - products of a row tile, 1450 cycles a tile with two under way.
 // Where a CTA has three tiles at most, what counts is that the second kernel does its own part meanwhile, beside it on the same SM: LEAN, in
 // 96 registers a thread, with scores taken from tensor memory twice, 32 at a time, for the maximum and for the exponentials, and at most
 // 162 KB.  Not LEAN / LEAN, us: 1 x 8 x 4000 (two tiles) 14.2 / 11.3, 24 x 8 x 512 (three) 15.4 / 14.9, 16 x 4 x 800 (four) 13.8 / 15.0,
@@ -33,8 +34,8 @@ struct Cfg {
   static constexpr int BLOCK_BYTES = TILE_KEYS * 128;
   static constexpr int STAGES = HD == 128 ? 2 : 3;  // of K and of V at most; a CTA with fewer tiles takes less memory
   static constexpr int STATS = 3 * TILE_ROWS * 4;   // each group's maxima, the odd one's sums
-  // Q, K ring, V ring, STATS, barriers: up to 162 KB, which leaves 64 KB for a CTA of the second kernel
-  static constexpr size_t smem(int stages) { return (1 + 2 * size_t(stages)) * TILE_BYTES + STATS + 256; }
+  // Q, K ring, V ring, STATS, barriers: with one row tile up to 162 KB, which leaves 64 KB for a CTA of the second kernel
+  static constexpr size_t smem(int stages, int q_tiles) { return (q_tiles + 2 * size_t(stages)) * TILE_BYTES + STATS + 256; }
 };
 
 // Where a CTA is in its range.
@@ -118,7 +119,7 @@ __device__ __forceinline__ void st_global_v8(float* p, const float (&v)[8]) {
                : "memory");
 }
 
-template <int HD, bool LEAN>
+template <int HD, bool LEAN, bool PAIR>
 __global__ void __launch_bounds__(LEAN ? LEAN_BOUND : THREADS, 1)
 kf_shared_prefix_tcgen05(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                          const __grid_constant__ CUtensorMap map_v, const Layout lay, int group, int stages, float scale_log2,
@@ -131,8 +132,9 @@ kf_shared_prefix_tcgen05(const __grid_constant__ CUtensorMap map_q, const __grid
     if (threadIdx.x == 0) atomicCAS(status, 0, int(KF_ERR_WAIT_DRAIN));
     return;
   }
-  const uint32_t q_smem = smem_base, k_smem = q_smem + C::TILE_BYTES, v_smem = k_smem + stages * C::TILE_BYTES;
-  float* stats = reinterpret_cast<float*>(smem + (1 + 2 * stages) * C::TILE_BYTES);
+  constexpr int Q_TILES = PAIR ? 2 : 1;
+  const uint32_t q_smem = smem_base, k_smem = q_smem + Q_TILES * C::TILE_BYTES, v_smem = k_smem + stages * C::TILE_BYTES;
+  float* stats = reinterpret_cast<float*>(smem + (Q_TILES + 2 * stages) * C::TILE_BYTES);
   uint8_t* bar_generic = reinterpret_cast<uint8_t*>(stats) + C::STATS;
   const uint32_t bar_base = smem_u32(bar_generic);
   auto k_full = [&](int st) { return bar_base + 8u * st; };
@@ -189,6 +191,8 @@ kf_shared_prefix_tcgen05(const __grid_constant__ CUtensorMap map_q, const __grid
   const uint32_t tmem_base = *tmem_slot_ptr;
   Walk wk = *start;
   auto s_col = [&](int g) { return tmem_base + uint32_t(g * 128); };
+  // query rows of a unit's tile g (none: not there)
+  auto rows_of = [&](const Walk& w, int g) { return min(lay.wt, lay.W - (w.u % lay.row_units * Q_TILES + g) * lay.wt) * group; };
   auto o_col = [&](int g) { return tmem_base + uint32_t(256 + g * 128); };
 
   if (warp < 4) {
@@ -200,12 +204,14 @@ kf_shared_prefix_tcgen05(const __grid_constant__ CUtensorMap map_q, const __grid
         int seg = 0, issued = 0, q_issued = 0;   // units and tiles so far
         Turn turn;
         while (wk.left > 0 && ok) {
-          const int n = segment(wk), hk = wk.u / lay.row_tiles, rt = wk.u % lay.row_tiles;
+          const int n = segment(wk), hk = wk.u / lay.row_units, tiles = PAIR && rows_of(wk, 1) > 0 ? 2 : 1;
           if (seg > 0 && !mbar_wait(q_empty, (seg - 1) & 1, status, KF_ERR_WAIT_EMPTY)) { ok = false; break; }
-          mbar_expect_tx(q_full, uint32_t(group * lay.wt * HD * 2));
+          mbar_expect_tx(q_full, uint32_t(tiles * group * lay.wt * HD * 2));
+          for (int g = 0; g < tiles; ++g)
 #pragma unroll
-          for (int c = 0; c < C::BLOCKS; ++c)
-            tma_load_4d(q_smem + c * C::BLOCK_BYTES, &map_q, q_full, 64 * c, hk * group, rt * lay.wt, wk.b);
+            for (int c = 0; c < C::BLOCKS; ++c)
+              tma_load_4d(q_smem + g * C::TILE_BYTES + c * C::BLOCK_BYTES, &map_q, q_full, 64 * c, hk * group,
+                          (wk.u % lay.row_units * Q_TILES + g) * lay.wt, wk.b);
           ++q_issued;
           for (int j = wk.j; j < wk.j + n; ++j, turn.next(stages)) {
             if (issued >= stages && !mbar_wait(k_empty(turn.st), turn.phase ^ 1u, status, KF_ERR_WAIT_EMPTY)) { ok = false; break; }
@@ -232,7 +238,7 @@ kf_shared_prefix_tcgen05(const __grid_constant__ CUtensorMap map_q, const __grid
         // the first K before the first V: the scores can begin
         if (wk.left > 0) ok = mbar_wait(k_full(0), 0, status, KF_ERR_WAIT_FULL);
         while (wk.left > 0 && ok) {
-          const int n = segment(wk), hk = wk.u / lay.row_tiles;
+          const int n = segment(wk), hk = wk.u / lay.row_units;
           for (int j = wk.j; j < wk.j + n; ++j, turn.next(stages)) {
             if (issued >= stages && !mbar_wait(v_empty(turn.st), turn.phase ^ 1u, status, KF_ERR_WAIT_EMPTY)) { ok = false; break; }
             mbar_expect_tx(v_full(turn.st), C::TILE_BYTES);
@@ -255,7 +261,7 @@ kf_shared_prefix_tcgen05(const __grid_constant__ CUtensorMap map_q, const __grid
         int seg = 0;                   // units so far
         int done[2] = {0, 0};          // tiles of each group whose P has been read
         Turn kt, vt;
-        // S_g = Q K^T of the next tile of the range
+        // S_g = Q K^T with the tile of keys whose turn it is
         auto issue_s = [&](int g) {
           const int st = kt.st;
           if (!mbar_wait(k_full(st), kt.phase, status, KF_ERR_WAIT_FULL)) return false;
@@ -263,46 +269,62 @@ kf_shared_prefix_tcgen05(const __grid_constant__ CUtensorMap map_q, const __grid
 #pragma unroll
           for (int kk = 0; kk < HD / 16; ++kk) {
             const uint32_t off = (kk / 4) * C::BLOCK_BYTES + (kk % 4) * 32;
-            tc_mma_f16(s_col(g), umma_desc_sw128(q_smem + off, 16, 1024), umma_desc_sw128(k_smem + st * C::TILE_BYTES + off, 16, 1024),
-                       idesc_s, kk != 0);
+            tc_mma_f16(s_col(g), umma_desc_sw128(q_smem + (PAIR ? g * C::TILE_BYTES : 0) + off, 16, 1024),
+                       umma_desc_sw128(k_smem + st * C::TILE_BYTES + off, 16, 1024), idesc_s, kk != 0);
           }
           tc_commit(s_full(g));
-          tc_commit(k_empty(st));
+          return true;
+        };
+        auto k_read = [&]() {   // every S that wants the tile has been issued
+          tc_commit(k_empty(kt.st));
           kt.next(stages);
+        };
+        // O_g += P_g V: A = P from tensor memory, B = V with the head dim contiguous, in two halves of the keys
+        auto issue_o = [&](int g, bool start) {
+          const int st = vt.st;
+          if (!mbar_wait(v_full(st), vt.phase, status, KF_ERR_WAIT_FULL)) return false;
+          if (!mbar_wait(p_half(g), done[g] & 1, status, KF_ERR_WAIT_TMEM_EMPTY)) return false;
+          tc_fence_after();
+#pragma unroll
+          for (int kk = 0; kk < TILE_KEYS / 32; ++kk)
+            tc_mma_f16_ts(o_col(g), s_col(g) + kk * 8, umma_desc_sw128(v_smem + st * C::TILE_BYTES + kk * 2048, C::BLOCK_BYTES, 1024), idesc_o,
+                          !start || kk != 0);
+          if (!mbar_wait(p_full(g), done[g] & 1, status, KF_ERR_WAIT_TMEM_EMPTY)) return false;
+          tc_fence_after();
+#pragma unroll
+          for (int kk = TILE_KEYS / 32; kk < TILE_KEYS / 16; ++kk)
+            tc_mma_f16_ts(o_col(g), s_col(g) + kk * 8, umma_desc_sw128(v_smem + st * C::TILE_BYTES + kk * 2048, C::BLOCK_BYTES, 1024), idesc_o, 1u);
+          tc_commit(pv_done(g));
+          ++done[g];
           return true;
         };
         while (wk.left > 0 && ok) {
-          const int n = segment(wk);
+          const int n = segment(wk), groups = !PAIR || rows_of(wk, 1) > 0 ? 2 : 1;
           ok = mbar_wait(q_full, seg & 1, status, KF_ERR_WAIT_FULL);
           if (ok) tc_fence_after();
-          for (int i = 0; i < min(n, 2) && ok; ++i) ok = issue_s(i);
-          if (ok && n <= 2) tc_commit(q_empty);
+          // the first scores of both groups: of the unit's first two tiles, or (PAIR) of its first tile with both row tiles
+          const int ahead = PAIR ? 1 : 2;
+          for (int g = 0; g < (PAIR ? groups : min(n, 2)) && ok; ++g) {
+            ok = issue_s(g);
+            if (ok && (!PAIR || g + 1 == groups)) k_read();
+          }
+          if (ok && n <= ahead) tc_commit(q_empty);
           // the accumulators of the unit before have been read
           if (ok && seg > 0) ok = mbar_wait(o_free, (seg - 1) & 1, status, KF_ERR_WAIT_TMEM_EMPTY);
           for (int i = 0; i < n && ok; ++i, vt.next(stages)) {
-            const int g = i & 1, st = vt.st;
-            if (!mbar_wait(v_full(st), vt.phase, status, KF_ERR_WAIT_FULL)) { ok = false; break; }
-            // O_g += P_g V: A = P from tensor memory, B = V with the head dim contiguous, in two halves of the keys
-            if (!mbar_wait(p_half(g), done[g] & 1, status, KF_ERR_WAIT_TMEM_EMPTY)) { ok = false; break; }
-            tc_fence_after();
-#pragma unroll
-            for (int kk = 0; kk < TILE_KEYS / 32; ++kk)
-              tc_mma_f16_ts(o_col(g), s_col(g) + kk * 8, umma_desc_sw128(v_smem + st * C::TILE_BYTES + kk * 2048, C::BLOCK_BYTES, 1024),
-                            idesc_o, i >= 2 || kk != 0);
-            if (!mbar_wait(p_full(g), done[g] & 1, status, KF_ERR_WAIT_TMEM_EMPTY)) { ok = false; break; }
-            tc_fence_after();
-#pragma unroll
-            for (int kk = TILE_KEYS / 32; kk < TILE_KEYS / 16; ++kk)
-              tc_mma_f16_ts(o_col(g), s_col(g) + kk * 8, umma_desc_sw128(v_smem + st * C::TILE_BYTES + kk * 2048, C::BLOCK_BYTES, 1024),
-                            idesc_o, 1u);
-            tc_commit(pv_done(g));
-            tc_commit(v_empty(st));
-            ++done[g];
-            if (i + 1 == n) tc_commit(o_final);
-            // the group's next scores follow at once: the products just issued have read its P before they are written
-            if (i + 2 < n) {
-              ok = issue_s(g);
-              if (ok && i + 3 == n) tc_commit(q_empty);
+            for (int g = PAIR ? 0 : i & 1; g < (PAIR ? groups : (i & 1) + 1) && ok; ++g) {
+              const bool last = !PAIR || g + 1 == groups;
+              ok = issue_o(g, i < ahead);
+              if (ok && last) tc_commit(v_empty(vt.st));
+              if (ok && last && i + 1 == n) tc_commit(o_final);
+              // the group's next scores follow at once: the products just issued have read its P before they are written
+              if (ok && i + ahead < n) {
+                ok = issue_s(g);
+                if (ok && last) {
+                  k_read();
+                  if (i + ahead + 1 == n) tc_commit(q_empty);
+                }
+              }
             }
           }
           ++seg;
@@ -326,16 +348,15 @@ kf_shared_prefix_tcgen05(const __grid_constant__ CUtensorMap map_q, const __grid
     bool ok = true;
     int first = 0, seg = 0, mine = 0;   // tiles before this unit, units, tiles of this group
     while (wk.left > 0) {
-      const int n = segment(wk), rt = wk.u % lay.row_tiles;
-      const int rows = min(lay.wt, lay.W - rt * lay.wt) * group;
+      const int n = segment(wk), rows = rows_of(wk, PAIR ? g : 0);
       const bool active = quarter * 32 < rows;   // the warp has rows at all
       const int len = length(lay, wk.b);
       float m_run = NEG_INF, l_run = 0.f;
-      for (int i = g; i < n; i += 2, ++mine) {
+      for (int i = PAIR ? (rows > 0 ? 0 : n) : g; i < n; i += PAIR ? 1 : 2, ++mine) {
         const int n0 = (wk.j + i) * TILE_KEYS;
         if (ok && !mbar_wait(s_full(g), mine & 1, status, KF_ERR_WAIT_TMEM_FULL)) ok = false;
         tc_fence_after();
-        if (n0 + TILE_KEYS > len && len < lay.P) {
+        if (n0 + TILE_KEYS > len && len < lay.P && (!PAIR || g == 0)) {   // PAIR: the products of group 0 come first
           // positions behind the prompt hold anything, and 0 times that need not be 0: their values become zeros
           const int st = (first + i) % stages;
           if (ok && !mbar_wait(v_full(st), ((first + i) / stages) & 1, status, KF_ERR_WAIT_FULL)) ok = false;
@@ -344,7 +365,8 @@ kf_shared_prefix_tcgen05(const __grid_constant__ CUtensorMap map_q, const __grid
             for (int c = 0; c < C::BLOCKS; ++c)
 #pragma unroll
               for (int e = 0; e < 8; ++e)
-                *reinterpret_cast<uint4*>(smem + (1 + stages + st) * C::TILE_BYTES + c * C::BLOCK_BYTES + row * 128 + e * 16) = make_uint4(0, 0, 0, 0);
+                *reinterpret_cast<uint4*>(smem + (Q_TILES + stages + st) * C::TILE_BYTES + c * C::BLOCK_BYTES + row * 128 + e * 16) =
+                    make_uint4(0, 0, 0, 0);
           }
           fence_async_smem();
         }
@@ -386,7 +408,7 @@ kf_shared_prefix_tcgen05(const __grid_constant__ CUtensorMap map_q, const __grid
         const bool grow = m_new > m_run + RESCALE_THRESHOLD;
         if (__any_sync(0xffffffffu, grow)) {
           const float alpha = grow ? (m_run == NEG_INF ? 0.f : fast_exp2(m_run - m_new)) : 1.f;
-          if (i >= 2) {
+          if (i >= (PAIR ? 1 : 2)) {
             if (ok && !mbar_wait(pv_done(g), (mine - 1) & 1, status, KF_ERR_WAIT_TMEM_FULL)) ok = false;
             tc_fence_after();
 #pragma unroll 1
@@ -433,44 +455,70 @@ kf_shared_prefix_tcgen05(const __grid_constant__ CUtensorMap map_q, const __grid
         unpack2(fadd2(fadd2(lsum[0], lsum[1]), fadd2(lsum[2], lsum[3])), a0, a1);
         l_run += a0 + a1;
       }
-      // ---- the unit's partial result: both groups' rows joined, each group writes half of the columns
-      stats[g * TILE_ROWS + row] = m_run;
-      if (g == 1) stats[2 * TILE_ROWS + row] = l_run;
-      asm volatile("bar.sync 1, 256;" ::: "memory");
-      const float m_other = stats[(1 - g) * TILE_ROWS + row];
-      const float top = fmaxf(m_run, m_other);
-      const float f_mine = m_run == NEG_INF ? 0.f : fast_exp2(m_run - top), f_other = m_other == NEG_INF ? 0.f : fast_exp2(m_other - top);
-      const float f0 = g == 0 ? f_mine : f_other, f1 = g == 0 ? f_other : f_mine;
-      if (ok && !mbar_wait(o_final, seg & 1, status, KF_ERR_WAIT_TMEM_FULL)) ok = false;
-      tc_fence_after();
-      if (ok && active) {
-        const long long slot = (long long)wk.b * lay.per_prompt + wk.u + blockIdx.x;
-        float* dst = part_o + (slot * TILE_ROWS + row) * HD;
+      const long long slot = ((long long)wk.b * lay.per_prompt + wk.u + blockIdx.x) * Q_TILES + (PAIR ? g : 0);
+      float* dst = part_o + (slot * TILE_ROWS + row) * HD;
+      if (PAIR) {
+        // ---- the row tile's partial result
+        if (ok && !mbar_wait(o_final, seg & 1, status, KF_ERR_WAIT_TMEM_FULL)) ok = false;
+        tc_fence_after();
+        if (ok && active) {
 #pragma unroll 1
-        for (int c = 0; c < HD / 64; ++c) {
-          const int col = g * (HD / 2) + c * 32;
-          uint32_t o0[32], o1[32];
-          tmem_ld_32x32_at(o_col(0) + lane_off + col, o0);
-          if (n > 1) tmem_ld_32x32_at(o_col(1) + lane_off + col, o1);
-          tmem_ld_wait();
-          if (row < rows) {
+          for (int c = 0; c < HD; c += 32) {
+            uint32_t o[32];
+            tmem_ld_32x32_at(t_o + c, o);
+            tmem_ld_wait();
+            if (row < rows) {
 #pragma unroll
-            for (int k = 0; k < 32; k += 8) {
-              float v[8];
+              for (int k = 0; k < 32; k += 8) {
+                float v[8];
 #pragma unroll
-              for (int e = 0; e < 8; ++e) {
-                v[e] = f0 * __uint_as_float(o0[k + e]);
-                if (n > 1) v[e] = __fmaf_rn(f1, __uint_as_float(o1[k + e]), v[e]);
+                for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(o[k + e]);
+                st_global_v8(dst + c + k, v);   // whole sectors: every lane writes a row of its own
               }
-              st_global_v8(dst + col + k, v);   // whole sectors: every lane writes a row of its own
             }
           }
+          if (row < rows) part_ml[slot * TILE_ROWS + row] = make_float2(m_run, l_run);
         }
-        if (g == 0 && row < rows) part_ml[slot * TILE_ROWS + row] = make_float2(top, f0 * l_run + f1 * stats[2 * TILE_ROWS + row]);
+        tc_fence_before();
+        __syncwarp();
+      } else {
+        // ---- the unit's partial result: both groups' rows joined, each group writes half of the columns
+        stats[g * TILE_ROWS + row] = m_run;
+        if (g == 1) stats[2 * TILE_ROWS + row] = l_run;
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        const float m_other = stats[(1 - g) * TILE_ROWS + row];
+        const float top = fmaxf(m_run, m_other);
+        const float f_mine = m_run == NEG_INF ? 0.f : fast_exp2(m_run - top), f_other = m_other == NEG_INF ? 0.f : fast_exp2(m_other - top);
+        const float f0 = g == 0 ? f_mine : f_other, f1 = g == 0 ? f_other : f_mine;
+        if (ok && !mbar_wait(o_final, seg & 1, status, KF_ERR_WAIT_TMEM_FULL)) ok = false;
+        tc_fence_after();
+        if (ok && active) {
+#pragma unroll 1
+          for (int c = 0; c < HD / 64; ++c) {
+            const int col = g * (HD / 2) + c * 32;
+            uint32_t o0[32], o1[32];
+            tmem_ld_32x32_at(o_col(0) + lane_off + col, o0);
+            if (n > 1) tmem_ld_32x32_at(o_col(1) + lane_off + col, o1);
+            tmem_ld_wait();
+            if (row < rows) {
+#pragma unroll
+              for (int k = 0; k < 32; k += 8) {
+                float v[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                  v[e] = f0 * __uint_as_float(o0[k + e]);
+                  if (n > 1) v[e] = __fmaf_rn(f1, __uint_as_float(o1[k + e]), v[e]);
+                }
+                st_global_v8(dst + col + k, v);   // whole sectors: every lane writes a row of its own
+              }
+            }
+          }
+          if (g == 0 && row < rows) part_ml[slot * TILE_ROWS + row] = make_float2(top, f0 * l_run + f1 * stats[2 * TILE_ROWS + row]);
+        }
+        tc_fence_before();
+        // the accumulators may be written again, and stats by the next unit
+        asm volatile("bar.sync 1, 256;" ::: "memory");
       }
-      tc_fence_before();
-      // the accumulators may be written again, and stats by the next unit
-      asm volatile("bar.sync 1, 256;" ::: "memory");
       if (lane == 0) mbar_arrive(o_free);
       first += n;
       ++seg;
@@ -499,15 +547,15 @@ static int make_map_4d(CUtensorMap* map, const void* base, const uint64_t (&size
   return r == CUDA_SUCCESS ? 0 : (int)r;
 }
 
-template <int HD, bool LEAN>
+template <int HD, bool LEAN, bool PAIR>
 static int launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const Layout& l, int group, int stages, float scale,
                   float* part_o, float2* part_ml, int* status, cudaStream_t stream) {
-  auto kern = kf_shared_prefix_tcgen05<HD, LEAN>;
+  auto kern = kf_shared_prefix_tcgen05<HD, LEAN, PAIR>;
   static bool attr_set[16] = {};
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev >= 16 || !attr_set[dev]) {
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Cfg<HD>::smem(Cfg<HD>::STAGES));
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Cfg<HD>::smem(Cfg<HD>::STAGES, PAIR ? 2 : 1));
     // all of the SM's memory as shared memory: CTAs of both kernels side by side
     if (e == cudaSuccess) e = cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
     if (e != cudaSuccess) return 300 + (int)e;
@@ -516,7 +564,7 @@ static int launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMa
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)l.ctas);
   cfg.blockDim = dim3(THREADS);
-  cfg.dynamicSmemBytes = Cfg<HD>::smem(stages);
+  cfg.dynamicSmemBytes = Cfg<HD>::smem(stages, PAIR ? 2 : 1);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -532,8 +580,9 @@ static int launch_hd(const CUtensorMap& mq, const CUtensorMap& mk, const CUtenso
                      float2* part_ml, int* status, cudaStream_t stream) {
   const long long tiles = (long long)tiles_of(l.P) * l.per_prompt * l.B, each = (tiles + l.ctas - 1) / l.ctas;   // most tiles of a CTA
   const int stages = each < Cfg<HD>::STAGES ? (int)each : Cfg<HD>::STAGES;
-  return each <= LEAN_TILES ? launch<HD, true>(mq, mk, mv, l, group, stages, scale, part_o, part_ml, status, stream)
-                            : launch<HD, false>(mq, mk, mv, l, group, stages, scale, part_o, part_ml, status, stream);
+  if (l.pair == 2) return launch<HD, false, true>(mq, mk, mv, l, group, stages, scale, part_o, part_ml, status, stream);
+  return each <= LEAN_TILES ? launch<HD, true, false>(mq, mk, mv, l, group, stages, scale, part_o, part_ml, status, stream)
+                            : launch<HD, false, false>(mq, mk, mv, l, group, stages, scale, part_o, part_ml, status, stream);
 }
 
 // Steps in elements: q prompt, continuation, head; k and v prompt, position, head.

@@ -184,3 +184,23 @@ def test_prompts_behind_4_gb(native_lib):
     room[:, :p] = k
     got = F.shared_prefix_attention(q, room[:, :p], v, ok, ov)
     near(got, (q, k, v, ok, ov))
+
+
+# prompts of over 168 MB, which two row tiles read together: two tiles, three, an odd one of one row, lengths that end in any tile
+@pytest.mark.parametrize("b,w,p,h,hkv,hd,lens", [
+    (1, 17, 43_011, 64, 8, 128, None), (3, 40, 14_500, 32, 8, 128, [14_499, 1, 9000]), (3, 33, 14_500, 64, 8, 128, [0, 14_337, 130]),
+    (5, 129, 58_000, 3, 3, 64, [58_000, 3, 0, 129, 10_001]),
+])
+def test_prompts_that_outlast_the_cache(native_lib, b, w, p, h, hkv, hd, lens):
+    args = make(b, w, p, 5, h, hkv, hd, torch.bfloat16, device="cuda")
+    if lens is not None:
+        for i, n in enumerate(lens):
+            args[1][i, n:], args[2][i, n:] = NAN, float("inf")
+        args[5] = torch.tensor(lens, device="cuda", dtype=torch.int32)
+    got = F.shared_prefix_attention(*args)
+    # a prompt at a time, by what of it counts: the whole in 64 bits would be large
+    for i in range(b):
+        n = p if lens is None else lens[i]
+        near(got[i : i + 1], (args[0][i : i + 1], args[1][i : i + 1, :n], args[2][i : i + 1, :n], args[3][i : i + 1], args[4][i : i + 1], None, None))
+    assert torch.equal(got, F.shared_prefix_attention(*args))
+    assert native_lib.read_status() == 0
