@@ -8,19 +8,22 @@
 //     fp32 over at most a few hundred terms and in 64 bits from there on, because candidates of different beams may lie close together.
 //     r moves only when a logit is 27 above it: moved with every new maximum, it cost a branch in most vectors.  The difference is taken
 //     before the factor log2 e: large logits lose nothing, and rows of the type's lowest value have exponents of zero like any others.
-//   * Each of a CTA's 8 warps has ceil(W / 8) threads whose largest logit is at least the warp's ceil(W / 8)-th largest.  So at least W logits
-//     reach the least of these over the warps, a bound that costs a warp-wide maximum or a few.  Taken after each thread's first two
+//   * Each of a CTA's 8 warps has ceil(W / 8) threads whose largest logit is at least the warp's ceil(W / 8)-th largest.  So at least W
+//     logits reach the least of these over the warps, a bound that costs a warp-wide maximum or a few.  Taken after each thread's first two
 //     vectors, and whenever there are twice as many, it leaves about a hundred vectors for 8 beams that reach it and are noted; taken
-//     again at the end, about 22.  A list that every warp kept on the way, with an insertion
-//     for each of W ln(n / W) logits, took 98 us for 64 x 8 x 128 256 in bf16; reading all vectors of the threads that reach the bound 92.
+//     again at the end, about 22.  Lists that every warp kept on the way, with an insertion for each of W ln(n / W) logits, took 98 us for
+//     64 x 8 x 128 256 in bf16, reading all vectors of the threads that reach the bound again 92, the notes 41.
 //   * Candidates are 64-bit keys: the logit's bits in an order-preserving form, then the complement of its index, so that of equal
 //     logits the lowest index is the largest key.  There are few, so a candidate's place is how many are larger, counted; the cluster's
 //     CTAs put theirs into the first one's shared memory.
-// What bounds it: the logits are read once.  Launches are joined to the one before (programmatic launch): by itself a launch of clusters began
-// 2.4 us later.
+// What bounds it: many prompts, the logits, which are read once (64 x 8 x 128 256 in bf16, an eighth finished: 115 MB in 41 us, 2.8 TB/s: the
+// pass at 75 to 80 % of a copy's rate, and behind it, in every CTA at the same time, bounds, candidates and sums); few prompts, these steps and the launch
+// (1 x 4 x 32 000: 7.5 us).  Launches are joined to the one before (programmatic launch): by itself a launch of clusters began 2.4 us later.
 //
 // kf_beam_reorder.  state[b, w] = state[b, parent[b, w]] for all states in one launch.  A thread owns 16 bytes of a column: it reads
 // the column's W values and then writes them, so that parents may be any selection of beams, also in place, without a second buffer.
+// What bounds it: a read and a write of what moves (4 x 8 beams' caches of a 7B model, 1.7 GB: 255 us, 104 % of a copy's rate, since beams
+// that keep their place move nothing); small states, the launch and the host's work for it (16 x 8 histories: 5.5 us).
 #include "common.cuh"
 #include "attention_common.cuh"
 #include "decode_common.cuh"
@@ -39,8 +42,8 @@ constexpr int THREADS = WARPS * 32;
 // CTAs of a cluster: 16 where all clusters' CTAs have an SM each, which few prompts need (1 x 8 x 128 256: 20.7 -> 16.6 us), else 8.
 constexpr int CTAS_FEW = 16, CTAS_MANY = 8;
 constexpr int MAX_PARTS = MAX_BEAMS / CTAS_MANY + 1;  // rows that a CTA's range meets
-constexpr int NOTES = 512;      // vectors that a CTA notes (20 KB); more (logits in rising order, equal ones) go through lists
-constexpr int ROOM = 512;             // candidates that a CTA sorts, likewise
+constexpr int NOTES = 512;                            // vectors that a CTA notes (20 KB); more (rising logits, equal ones) go through lists
+constexpr int ROOM = 512;                             // candidates that a CTA sorts, likewise
 
 typedef unsigned long long Key;
 
@@ -135,7 +138,9 @@ struct Logits<__nv_bfloat16> {
     asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
     return r;
   }
-  static __device__ __forceinline__ float one(const __nv_bfloat16* p) { return __uint_as_float(uint32_t(*reinterpret_cast<const uint16_t*>(p)) << 16); }
+  static __device__ __forceinline__ float one(const __nv_bfloat16* p) {
+    return __uint_as_float(uint32_t(*reinterpret_cast<const uint16_t*>(p)) << 16);
+  }
   static __device__ __forceinline__ float load(const Raw& v, float (&x)[N]) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[2 * i] = __uint_as_float(v.w[i] << 16), x[2 * i + 1] = __uint_as_float(v.w[i] & 0xffff0000u);
@@ -168,9 +173,8 @@ __device__ __forceinline__ void st_cluster_u64(uint32_t addr, unsigned long long
 
 template <typename T>
 __global__ void __launch_bounds__(THREADS, 4)
-kf_beam_select(const T* __restrict__ logits, long long stride_b, long long stride_w, const float* __restrict__ scores,
-               const uint8_t* __restrict__ finished, int W, int V, long long eos, long long pad, float* __restrict__ out_scores,
-               long long* __restrict__ out_parents, long long* __restrict__ out_tokens, uint8_t* __restrict__ out_finished) {
+kf_beam_select(const T* logits, long long stride_b, long long stride_w, const float* scores, const uint8_t* finished, int W, int V,
+               long long eos, long long pad, float* out_scores, long long* out_parents, long long* out_tokens, uint8_t* out_finished) {
   constexpr int N = Logits<T>::N;
   constexpr float LOG2E = 1.4426950408889634f, HIGH = 27.f;
   constexpr int UNROLL = 2;
@@ -201,12 +205,14 @@ kf_beam_select(const T* __restrict__ logits, long long stride_b, long long strid
   if (tid < MAX_BEAMS) winner[tid] = -1;
   grid_dep_wait();
   grid_dep_launch();
+  // No pointer is __restrict__: loads of what it says is constant may move ahead of the wait.
   // Beams whose logits count.  One without a score above -inf (or with NaN) has no candidates, a finished one has itself.
   const float score = lane < W ? scores[first + lane] : -INFINITY;
   const bool alive = score > -INFINITY;
   const bool done = lane < W && finished != nullptr && finished[first + lane];
   const uint32_t live = __ballot_sync(0xffffffffu, alive && !done);
-  const uint32_t per = (max(1u, uint32_t(V) / N) + CTAS_FEW - 1) / CTAS_FEW * CTAS_FEW;   // vectors of a row, at most; so that CTAs meet eighths of rows
+  // vectors of a row, at most, so that CTAs meet eighths of rows
+  const uint32_t per = (max(1u, uint32_t(V) / N) + CTAS_FEW - 1) / CTAS_FEW * CTAS_FEW;
   const uint32_t all = uint32_t(__popc(live)) * per;
   const uint32_t chunk = all / ctas;
   const uint32_t r1 = chunk * (rank + 1);
@@ -489,9 +495,9 @@ kf_beam_select(const T* __restrict__ logits, long long stride_b, long long strid
 }
 
 template <typename T>
-static int launch_select(const void* logits, long long stride_b, long long stride_w, const float* scores, const uint8_t* finished, int B, int W, int V,
-                         long long eos, long long pad, float* out_scores, long long* out_parents, long long* out_tokens, uint8_t* out_finished,
-                         int num_sms, cudaStream_t stream) {
+static int launch_select(const void* logits, long long stride_b, long long stride_w, const float* scores, const uint8_t* finished, int B, int W,
+                         int V, long long eos, long long pad, float* out_scores, long long* out_parents, long long* out_tokens,
+                         uint8_t* out_finished, int num_sms, cudaStream_t stream) {
   auto kern = kf_beam_select<T>;
   static bool attr_set[16] = {};
   int dev = 0;
@@ -537,7 +543,7 @@ struct States {
 // under way at once: W * COLS of 16 bytes are what fills a GPU's memory with threads enough.
 template <typename T, int W, int COLS>
 __global__ void __launch_bounds__(256)
-kf_beam_reorder(const __grid_constant__ States st, int beams, const void* __restrict__ parents, int wide) {
+kf_beam_reorder(const __grid_constant__ States st, int beams, const void* parents, int wide) {
   grid_dep_wait();
   grid_dep_launch();
   const State& a = st.s[blockIdx.z];
@@ -551,7 +557,8 @@ kf_beam_reorder(const __grid_constant__ States st, int beams, const void* __rest
   for (int w = 0; w < W; ++w) {
     from[w] = -1;
     if (w < beams) {
-      const long long p = wide ? reinterpret_cast<const long long*>(parents)[b * beams + w] : (long long)reinterpret_cast<const int*>(parents)[b * beams + w];
+      const long long at = b * beams + w;
+      const long long p = wide ? reinterpret_cast<const long long*>(parents)[at] : (long long)reinterpret_cast<const int*>(parents)[at];
       if (p >= 0 && p < beams && !(a.src == a.dst && p == w)) from[w] = int(p);
     }
   }

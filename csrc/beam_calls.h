@@ -13,12 +13,12 @@
 namespace {
 
 struct Beam {
-  int (*select)(const void*, int, long long, long long, const void*, const void*, int, int, int, long long, long long, void*, void*, void*, void*, int,
-                void*) = nullptr;
+  int (*select)(const void*, int, long long, long long, const void*, const void*, int, int, int, long long, long long, void*, void*, void*,
+                void*, int, void*) = nullptr;
   int (*reorder)(const long long*, int, int, int, const void*, int, void*) = nullptr;
   long long (*scratch)(int, int, int, int, int, int, int, int) = nullptr;
-  int (*attention)(const void*, const void*, const void*, const void*, const void*, const void*, const void*, void*, void*, int, int, int, int, int, int,
-                   int, const long long*, float, int, int, void*) = nullptr;
+  int (*attention)(const void*, const void*, const void*, const void*, const void*, const void*, const void*, void*, void*, int, int, int,
+                   int, int, int, int, const long long*, float, int, int, void*) = nullptr;
   int max_beams = 0, max_states = 0;
 } bm;
 
@@ -27,6 +27,8 @@ const at::Tensor* on_device(PyObject* o, long rank, long device) {
   const at::Tensor* t = tensor(o);
   return t && t->is_cuda() && t->get_device() == device && t->dim() == rank && !t->is_conj() && !t->is_neg() ? t : nullptr;
 }
+
+constexpr double kScales[2] = {0x1p-100, 0x1p100};   // of an attention: beyond, products with scores leave 32 bits
 
 bool wants_gradient(const at::Tensor& t) { return t.requires_grad() && at::GradMode::is_enabled(); }
 
@@ -90,9 +92,11 @@ PyObject* beam_reorder(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     bool written;
   };
   std::vector<long long> table;
-  std::vector<Span> spans;
+  std::vector<Span> spans;   // of what is read and written: parents too
   std::vector<const at::Tensor*> to;
   table.reserve(size_t(n) * 7);
+  const auto first = reinterpret_cast<long long>(p->const_data_ptr());
+  spans.push_back({first, first + b * w * static_cast<long long>(p->element_size()), false});
   for (Py_ssize_t i = 0; i < n; ++i) {
     const at::Tensor *x = tensor(PyList_GET_ITEM(args[0], i)), *y = in_place ? x : tensor(PyList_GET_ITEM(args[3], i));
     if (!x || !y || x->dim() < 2 || wants_gradient(*x) || wants_gradient(*y)) Py_RETURN_NONE;
@@ -175,10 +179,11 @@ PyObject* shared_prefix_attn(PyObject*, PyObject* const* args, Py_ssize_t nargs)
       (hd != 64 && hd != 128) || h / hkv > 128 || p > kLargest || s > kLargest || k.size(0) != b || k.size(3) != hd || k.sizes() != t[2]->sizes() ||
       ok.size(0) != b || ok.size(1) != w || ok.size(3) != hkv || ok.size(4) != hd || ok.sizes() != t[4]->sizes() ||
       (lens && (lens->scalar_type() != at::kInt || lens->size(0) != b || !lens->is_contiguous())) ||
-      (rows && (rows->scalar_type() != at::kByte || rows->size(0) != b || rows->size(1) != w || rows->size(2) != s || (s > 1 && rows->stride(2) != 1))))
+      (rows && (rows->scalar_type() != at::kByte || rows->size(0) != b || rows->size(1) != w || rows->size(2) != s ||
+                (s > 1 && rows->stride(2) != 1))))
     Py_RETURN_NONE;
   if (args[7] == Py_None) scale = 1.0 / std::sqrt(static_cast<double>(hd));
-  if (!(scale > 0.0) || std::isinf(scale)) Py_RETURN_NONE;
+  if (!(scale >= kScales[0] && scale <= kScales[1])) Py_RETURN_NONE;
   long long steps[19], *next = steps;
   for (int i = 0; i < 5; ++i)
     if (!steps_of(*t[i], next)) Py_RETURN_NONE;

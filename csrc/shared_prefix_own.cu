@@ -110,9 +110,10 @@ kf_shared_prefix_own(const Own a, const Layout lay, const float* part_o, const f
     for (int h = 0; h < 2; ++h) {
       const int r = row0 + h * 8, sl = __shfl_sync(0xffffffffu, slots, half + r);
       const bool in = (mask >> r) & 1u;
-      const long long of = in ? sl : 0, pos = in ? (t - (of < 0 ? 0 : prompt_tiles)) * OWN_TILE + r : 0;
-      const __nv_bfloat16* kp = (of < 0 ? pkb + pos * a.pk_s : kb + of * a.k_w + pos * a.k_s) + (lane & 3) * 8;
-      const __nv_bfloat16* vp = (of < 0 ? pvb + pos * a.pv_s : vb + of * a.v_w + pos * a.v_s) + (lane & 3) * 8;
+      const bool prompt = t < prompt_tiles;   // of the whole tile, so that a hidden key's address is in the same tensor
+      const long long of = in ? sl : 0, pos = in ? (t - (prompt ? 0 : prompt_tiles)) * OWN_TILE + r : 0;
+      const __nv_bfloat16* kp = (prompt ? pkb + pos * a.pk_s : kb + of * a.k_w + pos * a.k_s) + (lane & 3) * 8;
+      const __nv_bfloat16* vp = (prompt ? pvb + pos * a.pv_s : vb + of * a.v_w + pos * a.v_s) + (lane & 3) * 8;
 #pragma unroll
       for (int c = 0; c < HD / 32; ++c) {
         const uint32_t dst = (dst0 ^ uint32_t(c * 64)) + uint32_t(h * 8 * HD * 2);

@@ -65,13 +65,13 @@ def select(logits: torch.Tensor, scores: torch.Tensor, finished: torch.Tensor | 
     if scores.shape != logits.shape[:2] or scores.dtype != torch.float32 or scores.device != logits.device:
         raise ValueError(f"scores are fp32 {tuple(logits.shape[:2])} on {logits.device}, not {scores.dtype} {tuple(scores.shape)} on {scores.device}")
     if finished is not None and (finished.shape != scores.shape or finished.dtype != torch.bool or finished.device != logits.device):
-        raise ValueError(f"finished is bool {tuple(scores.shape)} on {logits.device}, not {finished.dtype} {tuple(finished.shape)} on {finished.device}")
+        raise ValueError(f"finished is bool {tuple(scores.shape)} on {logits.device}, not {finished.dtype} {tuple(finished.shape)} on "
+                         f"{finished.device}")
     logits, scores = logits.detach(), scores.detach().contiguous()
     finished = None if finished is None else finished.contiguous()
-    if logits.shape[0] and _native(logits):
-        if _cuda().beam_select_supported(logits):
-            with _on(logits):
-                return Selected(*_cuda().beam_select(logits, scores, finished, eos, pad))
+    if logits.shape[0] and _native(logits) and _cuda().beam_select_supported(logits):
+        with _on(logits):
+            return Selected(*_cuda().beam_select(logits, scores, finished, eos, pad))
     return Selected(*ref.beam_select(logits, scores, finished, eos, pad))
 
 
@@ -110,6 +110,7 @@ def reorder(states: list[torch.Tensor], parents: torch.Tensor, length: int | Non
     """state[b, w] = state[b, parents[b, w]] for states (B, W, ..) of any types, in place, or into ``out``: tensors like the states that
     share no memory with them.
 
+    States that are written share no memory with each other or with ``parents``.
     ``length``: only the first ``length`` entries of the third dimension move, and what lies behind them stays as it is.  parents (B, W)
     int64 or int32, any selection of beams; where one is no beam (outside 0 .. W - 1) that place stays as it is.  Returns what was written.
     """
@@ -132,16 +133,18 @@ def reorder(states: list[torch.Tensor], parents: torch.Tensor, length: int | Non
             raise ValueError(f"what is written for a state is {tuple(x.shape)} {x.dtype} on {x.device}, not {tuple(y.shape)} {y.dtype} on {y.device}")
         if torch.is_grad_enabled() and (x.requires_grad or y.requires_grad):
             raise ValueError("no gradient passes through a reordering: call it under no_grad")
-    spans = [(*_span(y), 1, i) for i, y in enumerate(to) if y.numel()]
+    spans = [(*_span(y), 1, y) for y in to if y.numel()]
     if out is not None:
-        spans += [(*_span(x), 0, i) for i, x in enumerate(states) if x.numel()]
-    spans.sort()
-    for n, (_, end, writes, i) in enumerate(spans):
-        for begin, _, written, j in spans[n + 1 :]:
+        spans += [(*_span(x), 0, x) for x in states if x.numel()]
+    if parents.numel():
+        spans.append((*_span(parents), 0, parents))
+    spans.sort(key=lambda s: s[0])
+    for n, (_, end, writes, x) in enumerate(spans):
+        for begin, _, written, y in spans[n + 1 :]:
             if begin >= end:
                 break
-            if (writes or written) and not _interleaved((to if writes else states)[i], (to if written else states)[j]):
-                raise ValueError("a state that is written shares memory with another")
+            if (writes or written) and not _interleaved(x, y):
+                raise ValueError("a state that is written shares memory with another or with the parents")
     if parents.numel() == 0 or not states:
         return to
     with torch.no_grad():
@@ -160,7 +163,7 @@ def _reorder_native(states, parents, length, to):
         if x.numel() == 0:
             continue
         inner = x[0, 0].numel()
-        if inner * x.element_size() > 1 << 37 or not _dense_beams(x) or not _dense_beams(y) or not _apart(y) or min(x.stride(0), x.stride(1), y.stride(0), y.stride(1)) < 0:
+        if inner * x.element_size() > 1 << 37 or not _dense_beams(x) or not _dense_beams(y) or not _apart(y):
             later.append((x, y))
             continue
         moves.append((x, y, inner * x.element_size()))

@@ -897,7 +897,8 @@ def gemm_fp8_swiglu_bwd(a8: torch.Tensor, b8: torch.Tensor, sa: torch.Tensor, sb
 
 # --------------------------------------------------------------------------- fp8 with a scale for each block of 128 (ops/fp8_blocks.py)
 def _step(name: str, *args, launches: int = 1):
-    """The answer of a call of ``csrc/fp8_blocks_calls.h`` or ``csrc/beam_calls.h`` on the current device's stream; None where the call is not plainly covered."""
+    """The answer of a call of ``csrc/fp8_blocks_calls.h`` or ``csrc/beam_calls.h`` on the current device's stream; None where the call is
+    not plainly covered."""
     global LAUNCH_COUNT
     steps = _load_steps() if _steps is None else _steps
     if not steps:
@@ -1096,9 +1097,11 @@ def shared_prefix_call(q, k, v, own_k, own_v, prefix_lens, own_rows, scale) -> t
     return r[0]
 
 
-def shared_prefix_supported(q: torch.Tensor, k: torch.Tensor) -> bool:
+def shared_prefix_supported(q: torch.Tensor, k: torch.Tensor, scale: float) -> bool:
     b, w, h, hd = q.shape
-    return k.shape[1] < 2**31 - 2**16 and b * w * h < 2**27 and lib().kf_shared_prefix_scratch(b, w, k.shape[1], h, k.shape[2], hd, -1, sm_count()) >= 0
+    p, hkv = k.shape[1:3]
+    return (p < 2**31 - 2**16 and b * w * h < 2**27 and 2.0**-100 <= scale <= 2.0**100
+            and lib().kf_shared_prefix_scratch(b, w, p, h, hkv, hd, -1, sm_count()) >= 0)
 
 
 def shared_prefix_attn(q, k, v, own_k, own_v, prefix_lens, own_rows, scale: float, direct: int = -1) -> torch.Tensor:

@@ -364,15 +364,16 @@ def shared_prefix_attention(
     prompt, which lets beams be exchanged without moving their caches; a value that is no continuation hides the position.
     A continuation that sees nothing gives zeros.  ``scale`` is positive.
 
-    bf16 with heads of 64 or 128 runs ``csrc/shared_prefix_tcgen05.cu`` and ``csrc/shared_prefix_own.cu``; other types and sizes, calls
-    that want gradients, and CPU tensors the formulas of ``ops.ref``.
+    bf16 with heads of 64 or 128 runs ``csrc/shared_prefix_tcgen05.cu`` and ``csrc/shared_prefix_own.cu`` (short prompts the latter
+    alone); other types and sizes, calls that want gradients, and CPU tensors the formulas of ``ops.ref``.
     """
     if q.is_cuda and not _FORCE_REF and _cuda().attn_policy() == "native":
         out = _cuda().shared_prefix_call(q, k, v, own_k, own_v, prefix_lens, own_rows, scale)
         if out is not None:
             return out
     if q.dim() != 4 or k.dim() != 4 or own_k.dim() != 5:
-        raise ValueError(f"q is (B, W, H, hd), k (B, P, Hkv, hd), own_k (B, W, S, Hkv, hd), not {tuple(q.shape)}, {tuple(k.shape)}, {tuple(own_k.shape)}")
+        raise ValueError(f"q is (B, W, H, hd), k (B, P, Hkv, hd), own_k (B, W, S, Hkv, hd), not {tuple(q.shape)}, {tuple(k.shape)}, "
+                         f"{tuple(own_k.shape)}")
     b, w, h, hd = q.shape
     hkv, s = k.shape[2], own_k.shape[2]
     if (v.shape != k.shape or own_v.shape != own_k.shape or k.shape[0] != b or k.shape[3] != hd or own_k.shape != (b, w, s, hkv, hd)
@@ -382,15 +383,18 @@ def shared_prefix_attention(
     for t in (k, v, own_k, own_v):
         if t.dtype != q.dtype or t.device != q.device:
             raise ValueError(f"q is {q.dtype} on {q.device}, a cache {t.dtype} on {t.device}")
-    if prefix_lens is not None and (prefix_lens.shape != (b,) or prefix_lens.dtype not in (torch.int32, torch.int64) or prefix_lens.device != q.device):
-        raise ValueError(f"prefix_lens is ({b},) int32 or int64 on {q.device}, not {tuple(prefix_lens.shape)} {prefix_lens.dtype} on {prefix_lens.device}")
+    if prefix_lens is not None and (prefix_lens.shape != (b,) or prefix_lens.dtype not in (torch.int32, torch.int64)
+                                    or prefix_lens.device != q.device):
+        raise ValueError(f"prefix_lens is ({b},) int32 or int64 on {q.device}, not {tuple(prefix_lens.shape)} {prefix_lens.dtype} on "
+                         f"{prefix_lens.device}")
     if own_rows is not None and (own_rows.shape != (b, w, s) or own_rows.dtype != torch.uint8 or own_rows.device != q.device):
-        raise ValueError(f"own_rows is {(b, w, s)} uint8 on {q.device}, not {tuple(own_rows.shape)} {own_rows.dtype} on {own_rows.device}")
+        raise ValueError(f"own_rows is {(b, w, s)} uint8 on {q.device}, not {tuple(own_rows.shape)} {own_rows.dtype} on "
+                         f"{own_rows.device}")
     scale = 1.0 / math.sqrt(hd) if scale is None else float(scale)
     if not 0.0 < scale < math.inf:
         raise ValueError(f"scale {scale} is not positive")
     needs_grad = torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, own_k, own_v))
-    if b * w and use_native(q) and not needs_grad and _cuda().attn_policy() == "native" and _cuda().shared_prefix_supported(q, k):
+    if b * w and use_native(q) and not needs_grad and _cuda().attn_policy() == "native" and _cuda().shared_prefix_supported(q, k, scale):
         with _on_device(q):
             if prefix_lens is not None:
                 if prefix_lens.dtype != torch.int32:

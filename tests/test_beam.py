@@ -158,3 +158,15 @@ def test_reorder_moves_the_version():
     before = x._version
     beam.reorder([x], torch.tensor([[1, 0]]))
     assert x._version > before
+
+
+@pytest.mark.parametrize("dtype", [torch.int64, torch.int32])
+def test_reorder_refuses_to_write_its_parents(dtype):
+    parents = torch.tensor([[1, 0, 2]], dtype=dtype)
+    room = torch.tensor([[0, 2, 1, 1]], dtype=dtype)
+    for bad in (lambda: beam.reorder([parents], parents), lambda: beam.reorder([torch.zeros(1, 3), room[:, 1:]], room[:, :3]),
+                lambda: beam.reorder([torch.zeros(1, 3, dtype=dtype)], parents, out=[parents])):
+        with pytest.raises(ValueError):
+            bad()
+    assert parents.tolist() == [[1, 0, 2]]
+    assert beam.reorder([parents], parents, out=[torch.zeros(1, 3, dtype=dtype)])[0].tolist() == [[0, 1, 2]]

@@ -162,3 +162,31 @@ def test_reorder_captured_and_behind_4_gb(native_lib):
     want = big[0, [2, 0, 1], -40:].clone()
     beam.reorder([big], torch.tensor([[2, 0, 1]], device="cuda"))
     assert torch.equal(big[0, :, -40:], want)
+
+
+@pytest.mark.parametrize("dtype", [torch.int64, torch.int32])
+def test_reorder_refuses_to_write_its_parents(native_lib, dtype):
+    parents = torch.tensor([[1, 0, 2]], dtype=dtype, device="cuda")
+    room = torch.tensor([[0, 2, 1, 1]], dtype=dtype, device="cuda")
+    for bad in (lambda: beam.reorder([parents], parents), lambda: beam.reorder([torch.zeros(1, 3, device="cuda"), room[:, 1:]], room[:, :3]),
+                lambda: beam.reorder([torch.zeros_like(parents)], parents, out=[parents])):
+        with pytest.raises(ValueError):
+            bad()
+    assert parents.tolist() == [[1, 0, 2]]
+    assert beam.reorder([parents], parents, out=[torch.zeros_like(parents)])[0].tolist() == [[0, 1, 2]]
+
+
+def test_in_inference_mode(native_lib):
+    logits = torch.randn(2, 3, 1000, device="cuda")
+    scores = torch.randn(2, 3, device="cuda")
+    history = torch.randint(0, 99, (2, 3, 8), device="cuda")
+    want = beam.select(logits, scores, eos_id=5)
+    moved = torch.stack([history[i, want.parents[i]] for i in range(2)])
+    with torch.inference_mode():
+        for x in (history.clone(), history):
+            got = beam.select(logits, scores, eos_id=5)
+            assert all(torch.equal(a, b) for a, b in zip(got, want)) and got.scores.is_inference()
+            got.scores.add_(1.0)
+            assert torch.equal(got.parents, want.parents)
+            beam.reorder([x], got.parents)
+            assert torch.equal(x, moved)

@@ -204,3 +204,15 @@ def test_prompts_that_outlast_the_cache(native_lib, b, w, p, h, hkv, hd, lens):
         near(got[i : i + 1], (args[0][i : i + 1], args[1][i : i + 1, :n], args[2][i : i + 1, :n], args[3][i : i + 1], args[4][i : i + 1], None, None))
     assert torch.equal(got, F.shared_prefix_attention(*args))
     assert native_lib.read_status() == 0
+
+
+@pytest.mark.parametrize("p,s", [(130, 0), (0, 130), (5, 17)])
+def test_scales_that_leave_32_bits_take_the_formulas(native_lib, p, s):
+    args = make(1, 2, p, s, 4, 2, 64, torch.bfloat16, device="cuda")
+    before = native_lib.LAUNCH_COUNT
+    near(F.shared_prefix_attention(*args, scale=1e-50), args, scale=1e-50)
+    assert native_lib.LAUNCH_COUNT == before
+    with torch.inference_mode():
+        got = F.shared_prefix_attention(*args, scale=2.0**-100)
+        near(got, args, scale=2.0**-100)
+    assert native_lib.LAUNCH_COUNT > before
