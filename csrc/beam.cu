@@ -12,13 +12,13 @@
 //     logits reach the least of these over the warps, a bound that costs a warp-wide maximum or a few.  Taken after each thread's first two
 //     vectors, and whenever there are twice as many, it leaves about a hundred vectors for 8 beams that reach it and are noted; taken
 //     again at the end, about 22.  Lists that every warp kept on the way, with an insertion for each of W ln(n / W) logits, took 98 us for
-//     64 x 8 x 128 256 in bf16, reading all vectors of the threads that reach the bound again 92, the notes 41.
+//     64 x 8 x 128 256 in bf16, reading all vectors of the threads that reach the bound again 92, the notes 40.
 //   * Candidates are 64-bit keys: the logit's bits in an order-preserving form, then the complement of its index, so that of equal
 //     logits the lowest index is the largest key.  There are few, so a candidate's place is how many are larger, counted; the cluster's
 //     CTAs put theirs into the first one's shared memory.
-// What bounds it: many prompts, the logits, which are read once (64 x 8 x 128 256 in bf16, an eighth finished: 115 MB in 41 us, 2.8 TB/s: the
+// What bounds it: many prompts, the logits, which are read once (64 x 8 x 128 256 in bf16, an eighth finished: 115 MB in 40 us, 2.9 TB/s: the
 // pass at 75 to 80 % of a copy's rate, and behind it, in every CTA at the same time, bounds, candidates and sums); few prompts, these steps and the launch
-// (1 x 4 x 32 000: 7.5 us).  Launches are joined to the one before (programmatic launch): by itself a launch of clusters began 2.4 us later.
+// (1 x 4 x 32 000: 7.4 us).  Launches are joined to the one before (programmatic launch): by itself a launch of clusters began 2.4 us later.
 //
 // kf_beam_reorder.  state[b, w] = state[b, parent[b, w]] for all states in one launch.  A thread owns 16 bytes of a column: it reads
 // the column's W values and then writes them, so that parents may be any selection of beams, also in place, without a second buffer.
@@ -39,20 +39,29 @@ using decode::mapa_shared;
 constexpr int MAX_BEAMS = 32;   // a warp's list is one key per lane
 constexpr int WARPS = 8;
 constexpr int THREADS = WARPS * 32;
-// CTAs of a cluster: 16 where all clusters' CTAs have an SM each, which few prompts need (1 x 8 x 128 256: 20.7 -> 16.6 us), else 8.
+// CTAs of a cluster: 16 where all clusters' CTAs have an SM each, which few prompts need (1 x 8 x 128 256: 20.7 -> 16.1 us), else 8.
 constexpr int CTAS_FEW = 16, CTAS_MANY = 8;
+// Vectors that a CTA reads in the time that bounds and candidates of a second row take it.  Rows dealt out in equal shares / a whole number of
+// CTAs each, us: 3 x 5 x 50 257 12.8 / 10.4, 2 x 6 x 128 256 16.0 / 14.0, 2 x 12 x 50 257 19.1 / 16.6, 4 x 7 x 30 000 13.6 / 9.4.
+constexpr uint32_t SPARE = 2048;
 constexpr int MAX_PARTS = MAX_BEAMS / CTAS_MANY + 1;  // rows that a CTA's range meets
 constexpr int NOTES = 512;                            // vectors that a CTA notes (20 KB); more (rising logits, equal ones) go through lists
 constexpr int ROOM = 512;                             // candidates that a CTA sorts, likewise
 
 typedef unsigned long long Key;
 
-// The order of floats as unsigned integers; -0 counts as +0.
+// The order of floats as unsigned integers (of numbers none is 0); -0 counts as +0.
 __device__ __forceinline__ uint32_t ordered(float x) {
   uint32_t u = __float_as_uint(x);
   if (u == 0x80000000u) u = 0u;
   return (u & 0x80000000u) ? ~u : u | 0x80000000u;
 }
+__device__ __forceinline__ Key ordered(double x) {
+  Key u = Key(__double_as_longlong(x));
+  if (u == 1ull << 63) u = 0;
+  return (u >> 63) ? ~u : u | 1ull << 63;
+}
+__device__ __forceinline__ double unordered(Key o) { return __longlong_as_double((long long)((o >> 63) ? o & ~(1ull << 63) : ~o)); }
 __device__ __forceinline__ float unordered(uint32_t o) { return __uint_as_float((o & 0x80000000u) ? o & 0x7fffffffu : ~o); }
 __device__ __forceinline__ Key make_key(float x, uint32_t index) { return (Key(ordered(x)) << 32) | (0xffffffffu - index); }
 __device__ __forceinline__ float key_value(Key k) { return unordered(uint32_t(k >> 32)); }
@@ -95,6 +104,13 @@ struct TopList {
     }
   }
 };
+
+// Over eight lanes side by side.
+__device__ __forceinline__ int sum_of_8(int x) {
+#pragma unroll
+  for (int o = 4; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+  return x;
+}
 
 // 32 bytes of logits, on 32 bytes: the widest load there is.
 struct Raw {
@@ -193,9 +209,10 @@ kf_beam_select(const T* logits, long long stride_b, long long stride_w, const fl
   __shared__ Raw noted_raw[NOTES];                 // the vector
   __shared__ Key found[ROOM];                      // candidates, or the warps' lists
   __shared__ int winner[MAX_BEAMS];                // of each place: which candidate
-  double* total = reinterpret_cast<double*>(noted_raw);   // [W][W], best first, -inf: none
+  Key* total = reinterpret_cast<Key*>(noted_raw);  // [W][totals]: scores in the order of integers, best first, 0: none
+  const int totals = (W + 7) / 8 * 8 + 1;          // an odd number spreads the beams' over the banks
   uint32_t* token = reinterpret_cast<uint32_t*>(found);
-  static_assert(sizeof(noted_raw) >= MAX_BEAMS * MAX_BEAMS * 8 && sizeof(found) >= MAX_BEAMS * MAX_BEAMS * 4, "");
+  static_assert(sizeof(noted_raw) >= MAX_BEAMS * (MAX_BEAMS + 1) * 8 && sizeof(found) >= MAX_BEAMS * MAX_BEAMS * 4, "");
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tid = threadIdx.x;
   const uint32_t ctas = cluster_nctaid();
@@ -212,10 +229,14 @@ kf_beam_select(const T* logits, long long stride_b, long long stride_w, const fl
   const bool done = lane < W && finished != nullptr && finished[first + lane];
   const uint32_t live = __ballot_sync(0xffffffffu, alive && !done);
   // vectors of a row, at most, so that CTAs meet eighths of rows
-  const uint32_t per = (max(1u, uint32_t(V) / N) + CTAS_FEW - 1) / CTAS_FEW * CTAS_FEW;
-  const uint32_t all = uint32_t(__popc(live)) * per;
-  const uint32_t chunk = all / ctas;
-  const uint32_t r1 = chunk * (rank + 1);
+  uint32_t per = (max(1u, uint32_t(V) / N) + CTAS_FEW - 1) / CTAS_FEW * CTAS_FEW;
+  const uint32_t lives = __popc(live);
+  uint32_t chunk = lives * per / ctas;
+  if (ctas == CTAS_FEW && lives > 2 && lives <= CTAS_FEW) {   // few prompts: no CTA with parts of two rows, if that is no more than SPARE more
+    const uint32_t ways = CTAS_FEW / lives, each = (per + ways - 1) / ways;
+    if (each <= chunk + SPARE) chunk = each, per = each * ways;
+  }
+  const uint32_t r1 = min(chunk * (rank + 1), lives * per);
   asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");   // waited for below: the first CTA is there to be written to
 
   int part = 0;
@@ -389,11 +410,14 @@ kf_beam_select(const T* logits, long long stride_b, long long stride_w, const fl
     const int candidates = n_found[part];
     if (candidates <= ROOM && noted <= NOTES) {
       if (tid < W && tid >= candidates) st_cluster_u64(to + 16 + 8 * tid, 0ull);
-      for (int e = tid; e < candidates; e += THREADS) {
-        const Key mine = found[e];
+      for (int e0 = warp * 4; e0 < candidates; e0 += WARPS * 4) {   // eight lanes a candidate
+        const int e = e0 + lane / 8;
+        const Key mine = found[min(e, candidates - 1)];
         int larger = 0;
-        for (int i = 0; i < candidates; ++i) larger += found[i] > mine;
-        if (larger < W) st_cluster_u64(to + 16 + 8 * larger, mine);
+#pragma unroll 4
+        for (int i = lane & 7; i < candidates; i += 8) larger += found[i] > mine;
+        larger = sum_of_8(larger);
+        if ((lane & 7) == 0 && e < candidates && larger < W) st_cluster_u64(to + 16 + 8 * larger, mine);
       }
     } else {
       // rising or equal logits: every warp through the whole of its vectors
@@ -416,7 +440,7 @@ kf_beam_select(const T* logits, long long stride_b, long long stride_w, const fl
         if (lane < W) st_cluster_u64(to + 16 + 8 * lane, list.mine);
       }
     }
-    if (warp == 0) {
+    if (warp == WARPS - 1) {   // it has the fewest candidates
       const float own = lane < WARPS ? rs[part & 1][lane] : -INFINITY;
       float pr = own;
 #pragma unroll
@@ -438,7 +462,7 @@ kf_beam_select(const T* logits, long long stride_b, long long stride_w, const fl
   const double NONE = -INFINITY;
   for (int w = warp; w < W; w += WARPS) {
     const double own_score = double(__shfl_sync(0xffffffffu, score, w));
-    if (lane < W) total[w * W + lane] = NONE;
+    if (lane < totals - 1) total[w * totals + lane] = 0;
     __syncwarp();
     if ((live >> w) & 1u) {
       const uint32_t nth = uint32_t(__popc(live & ((1u << w) - 1u)));
@@ -458,36 +482,43 @@ kf_beam_select(const T* logits, long long stride_b, long long stride_w, const fl
         for (int c = 0; c < count; ++c)
           for (int j = 0; j < W; ++j) larger += p[c].keys[j] > mine;
         if (mine && larger < W) {
-          total[w * W + larger] = own_score + (double(key_value(mine)) - lse);
+          total[w * totals + larger] = ordered(own_score + (double(key_value(mine)) - lse));
           token[w * W + larger] = key_index(mine);
         }
       }
     } else if (lane == 0 && own_score > NONE) {
-      total[w * W] = own_score;   // finished
+      total[w * totals] = ordered(own_score);   // finished
     }
   }
   __syncthreads();
-  // a candidate's place: how many come before it, its own beam's better ones, others' better ones, lower beams' equal ones
-  for (int i = tid; i < W * W; i += THREADS) {
-    const double mine = total[i];
-    const int w = i / W;
-    int before = mine > NONE ? i - w * W : W;
-    for (int x = 0; x < W && before < W; ++x) {
-      if (x == w) continue;
-      for (int j = x * W; j < x * W + W; ++j) {
-        if (!(total[j] > mine || (total[j] == mine && x < w))) break;
-        if (++before == W) break;
+  // a candidate's place: how many come before it, its own beam's better ones, others' better ones, lower beams' equal ones; a warp a beam,
+  // eight lanes a candidate
+  for (int w = warp; w < W; w += WARPS)
+    for (int j0 = 0; j0 < W; j0 += 4) {
+      const int j = j0 + lane / 8;
+      const Key mine = j < W ? total[w * totals + j] : 0;
+      int before = 0;
+      for (int x = lane & 7; x < W; x += 8) {
+        const Key* of = total + x * totals;
+        const Key limit = mine - (x < w);
+        int n = 0;
+        for (int k = 0; k < W; k += 8)   // zeros behind the last one
+#pragma unroll
+          for (int e = 0; e < 8; ++e) n += of[k + e] > limit;
+        before += x == w ? j : n;
       }
+      before = sum_of_8(before);
+      const bool among = mine && before < W;
+      if (among && (lane & 7) == 0) winner[before] = w * W + j;
+      if (!__any_sync(0xffffffffu, among)) break;   // nor are those behind
     }
-    if (before < W) winner[before] = i;
-  }
   __syncthreads();
   const uint32_t ends = __ballot_sync(0xffffffffu, done);
   if (tid < W) {
     const int i = winner[tid], parent = i < 0 ? tid : i / W;
     const bool ended = i >= 0 && ((ends >> parent) & 1u);
     const long long t = i < 0 || ended ? pad : (long long)token[i];
-    out_scores[first + tid] = i < 0 ? -INFINITY : float(total[i]);
+    out_scores[first + tid] = i < 0 ? -INFINITY : float(unordered(total[parent * totals + i - parent * W]));
     out_parents[first + tid] = parent;
     out_tokens[first + tid] = t;
     out_finished[first + tid] = ended || (i >= 0 && t == eos);
