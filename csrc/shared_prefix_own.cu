@@ -5,7 +5,7 @@
 // cache each position lies.  Beams share most of their ancestors, so most of these keys come out of L2 for all beams but the first.
 //   * a unit is a continuation's key head; its query heads are the 16 rows of an m16n8k16 MMA, its keys are dealt out to 1 to 32 warps:
 //     few units need many warps for one, many (a batch of short continuations) one each;
-//   * every warp streams tiles of 16 keys through a cp.async ring of its own, two tiles ahead, without a barrier; 16-byte chunks are
+//   * every warp streams tiles of 16 keys through a cp.async ring of its own, without a barrier; 16-byte chunks are
 //     XOR-swizzled, so that ldmatrix is free of bank conflicts; a warp of one or two tiles has them all under way at once;
 //   * the (max, sum, output) triples of the warps, of the CTAs of a cluster and of the prompt are joined in a fixed order.
 // All of it up to that last step runs without the prompt's kernel, and starts on the SMs that it leaves (programmatic launch).
@@ -26,14 +26,13 @@ constexpr int OWN_WARPS = 4, OWN_THREADS = OWN_WARPS * 32;
 constexpr int OWN_TILE = 16;       // keys per ring stage of a warp
 constexpr int OWN_ROWS = 16;       // query heads per unit (MMA rows)
 
-// RING: tiles in a warp's ring, up to which it has them all under way at once.  0: it streams through 24 KB (two CTAs an SM, 128 KB of it
-// under way).
+// RING: tiles in a warp's ring, up to which it has them all under way at once.  0: it streams through 24 KB (two CTAs an SM, 192 KB
+// under way; refilled before a tile is worked on, with a stage less under way, it was 1 to 4 % slower).
 template <int HD, int RING_TILES>
 struct OwnCfg {
   static constexpr int TILE_BYTES = OWN_TILE * HD * 2;
   static constexpr bool STREAM = RING_TILES == 0;
   static constexpr int STAGES = STREAM ? (24 << 10) / (2 * TILE_BYTES) : RING_TILES;   // 3 for a head dim of 128, 6 for 64
-  static constexpr int AHEAD = STREAM ? STAGES - 1 : STAGES;         // tiles under way before the first is read
   static constexpr int RING = STAGES * 2 * TILE_BYTES;
   static constexpr int PART = OWN_ROWS * HD * 4;                     // a warp's partial output, over its ring
   static constexpr int STATS = OWN_ROWS * 2 * 4;                     // (max, sum) of its rows, behind it
@@ -141,7 +140,7 @@ kf_shared_prefix_own(const Own a, const Layout lay, const float* part_o, const f
     }
   }
 #pragma unroll
-  for (int i = 0; i < C::AHEAD; ++i) {
+  for (int i = 0; i < C::STAGES; ++i) {
     if (t0 + i < t1) issue(t0 + i);
     cp_commit();
   }
@@ -155,12 +154,8 @@ kf_shared_prefix_own(const Own a, const Layout lay, const float* part_o, const f
   for (int i = 0; i < (C::STREAM ? t1 - t0 : C::STAGES); ++i) {
     const int t = t0 + i;
     if (t >= t1) break;
-    cp_wait<C::STREAM ? C::STAGES - 2 : 0>();
-    __syncwarp();   // tile t has landed for every lane, and the stage refilled below has been consumed
-    if (C::STREAM) {
-      if (t + C::STAGES - 1 < t1) issue(t + C::STAGES - 1);
-      cp_commit();
-    }
+    cp_wait<C::STREAM ? C::STAGES - 1 : 0>();
+    __syncwarp();   // tile t has landed for every lane
     const int st = C::STREAM ? i % C::STAGES : i;
     const uint32_t ks = ring + uint32_t(st) * 2u * C::TILE_BYTES, vs = ks + C::TILE_BYTES;
     const int mi = lane >> 3, lr = lane & 7;
@@ -216,6 +211,11 @@ kf_shared_prefix_own(const Own a, const Layout lay, const float* part_o, const f
         mma16816(o[2 * d], pa, f[0], f[1]);
         mma16816(o[2 * d + 1], pa, f[2], f[3]);
       }
+    }
+    if (C::STREAM) {
+      __syncwarp();   // every lane has read the stage
+      if (t + C::STAGES < t1) issue(t + C::STAGES);
+      cp_commit();
     }
   }
   cp_wait<0>();
