@@ -60,6 +60,11 @@ __global__ void __launch_bounds__(OWN_THREADS, RING_TILES == 0 ? 3 : 4)   // 4: 
 kf_shared_prefix_own(const Own a, const Layout lay, const float* part_o, const float2* part_ml, const uint32_t units) {
   using C = OwnCfg<HD, RING_TILES>;
   extern __shared__ __align__(128) uint8_t smem_raw[];
+  // Behind the prompt's kernel everything but its results is there at the start, because it has waited itself; alone nothing is.
+  if (part_o == nullptr) {
+    grid_dep_wait();
+    grid_dep_launch();
+  }
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int splits = WPU == OWN_WARPS ? int(cluster_nctaid()) : 1, rank = WPU == OWN_WARPS ? int(cluster_ctarank()) : 0;
   const int way = rank * WPU + warp % WPU, ways = splits * WPU;     // which share of the unit's keys
@@ -250,8 +255,10 @@ kf_shared_prefix_own(const Own a, const Layout lay, const float* part_o, const f
   if (WPU == 1) __syncwarp();
   else if (splits == 1) __syncthreads();
   else cluster_sync_all();
-  grid_dep_wait();
-  grid_dep_launch();
+  if (part_o != nullptr) {
+    grid_dep_wait();
+    grid_dep_launch();
+  }
   const long long slot0 =
       ((long long)b * lay.per_prompt + u + c0) * slot_rows + (w / lay.wt % lay.pair) * TILE_ROWS + (w % lay.wt) * a.group + hb * OWN_ROWS;
   const int warp0 = warp / WPU * WPU;
@@ -365,11 +372,9 @@ static int launch_ways(const Own& a, const Layout& l, const float* part_o, const
     attr[cfg.numAttrs].val.clusterDim.y = attr[cfg.numAttrs].val.clusterDim.z = 1;
     ++cfg.numAttrs;
   }
-  if (part_o != nullptr) {
-    attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
-    ++cfg.numAttrs;
-  }
+  attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
+  ++cfg.numAttrs;
   cudaError_t e = cudaLaunchKernelEx(&cfg, kern, a, l, part_o, part_ml, (uint32_t)units);
   return e == cudaSuccess ? 0 : 500 + (int)e;
 }
@@ -386,12 +391,13 @@ static int launch_own(const Own& a, const Layout& l, const float* part_o, const 
   };
   // One or two tiles a warp, where that takes a CTA a unit at most and no more than 16 or 12 warps on an SM, which is what registers or
   // memory hold: everything is under way at once, and nothing crosses CTAs (8 x 5 continuations of 65 keys: 27.2 -> 23 us, 1 x 8 of 96
-  // 15.6 -> 13; but 8 x 8 of 65, 14 warps an SM, 17.8, and streaming 12.9).  Else as many warps a unit as fill eight on every SM, of which
-  // each has a tile at least.
+  // 15.6 -> 13; but 8 x 8 of 65, 14 warps an SM, 17.8, and streaming 12.9).  Units of one tile so however many they are (64 x 8 of 16 keys:
+  // streaming 18.6, so 11.6; two tiles, of 30, 20.9 and 24.9).  Else as many warps a unit as fill eight on every SM, of which each has a
+  // tile at least.
   for (int ring = 1; ring <= 2; ++ring) {
     int ways = 1;
     while (ways < 4 && ways * ring < tiles) ways *= 2;
-    if (ways * ring >= tiles && units * ways <= (ring == 1 ? 16LL : 12LL) * num_sms)
+    if (ways * ring >= tiles && (units * ways <= (ring == 1 ? 16LL : 12LL) * num_sms || ring * ways == 1))
       return ring == 1 ? go(std::integral_constant<int, 1>(), ways) : go(std::integral_constant<int, 2>(), ways);
   }
   int ways = 1;
@@ -417,12 +423,17 @@ static bool make_layout(Layout& l, const void* lens, int B, int W, int P, int gr
   return tiles < 0x7fff0000LL && (long long)B * W * Hkv * group < 1LL << 27;   // counts of tiles and units in 32 bits
 }
 
-// Bytes of the prompts, once for every continuation, up to which one kernel reads them all.  In a graph, direct / two kernels, us:
-// 3.5 MB (1 x 4 x 300, 12 heads of 64) 6.4 / 6.8, 16 MB (1 x 8 x 500, 8 heads of 128) 10.0 / 7.5; eager, 3.5 MB, 8.2 / 10.9: a launch
-// and an allocation less for the host.
-constexpr long long DIRECT_BYTES = 4LL << 20;
-static bool is_direct(int direct, int B, int W, int P, int Hkv, int hd) {
-  return P > 0 && (direct < 0 ? 4LL * B * W * P * Hkv * hd <= DIRECT_BYTES : direct != 0);
+// Whether one kernel reads the prompts for every continuation again.  Up to 4 MB of them that is a launch and an allocation less for the host
+// (1 x 4 x 300, 12 heads of 64: eager 10.9 -> 7.7 us); beyond, a warp's chain of tiles is longer than what two kernels take.  Prompts of one
+// tile of 128 keys have no chain: up to 12 MB, and up to 64 where the other kernel's tiles are for few keys or continuations.  One kernel / two,
+// in a graph, us: 6 MB (1 x 4 x 375) 7.8 / 7.0, 8 MB (1 x 4 x 500) 11.5 / 7.2; one tile, 8 MB (1 x 32 x 64) 7.1 / 8.8, 20 MB in 24 tiles
+// (3 x 32 x 52) 25.6 / 22.9, 34 in 128 (16 x 8 x 64) 11.0 / 11.7, 67 in 512 (64 x 8 x 32) 29.4 / 37.3, 134 in 256 (32 x 8 x 128) 28.8 / 21.2.
+constexpr long long DIRECT_BYTES = 4LL << 20, DIRECT_SHORT = 12LL << 20, DIRECT_MOST = 64LL << 20, DIRECT_OF_A_TILE = 256LL << 10;
+static bool is_direct(int direct, const Layout& l, int Hkv, int hd) {
+  const long long bytes = 4LL * l.B * l.W * l.P * Hkv * hd, tiles = (long long)l.per_prompt * l.B;
+  if (l.P == 0 || direct >= 0) return l.P > 0 && direct != 0;
+  if (l.P > TILE_KEYS) return bytes <= DIRECT_BYTES;
+  return bytes <= DIRECT_SHORT || (bytes <= DIRECT_MOST && bytes <= tiles * DIRECT_OF_A_TILE);
 }
 
 }  // namespace shared_prefix
@@ -439,7 +450,7 @@ long long kf_shared_prefix_scratch(int B, int W, int P, int H, int Hkv, int hd, 
   Layout l;
   if (B < 1 || W < 1 || P < 0 || Hkv < 1 || H % Hkv || (hd != 64 && hd != 128)) return -1;
   if (!make_layout(l, nullptr, B, W, P, H / Hkv, Hkv, hd, num_sms)) return -1;
-  return P == 0 || is_direct(direct, B, W, P, Hkv, hd) ? 0 : slots(l) * l.pair * TILE_ROWS * (hd * 4 + 8);
+  return P == 0 || is_direct(direct, l, Hkv, hd) ? 0 : slots(l) * l.pair * TILE_ROWS * (hd * 4 + 8);
 }
 
 // o (B, W, H, hd), dense = attention of q (B, W, H, hd) over k, v (B, P, Hkv, hd), of which lens[b] positions count (null: all), and over
@@ -457,7 +468,7 @@ int kf_shared_prefix_attn_bf16(const void* q, const void* k, const void* v, cons
   for (int i = 0; i < 17; ++i)
     if (steps[i] & 7) return 5;
   cudaStream_t st = (cudaStream_t)stream;
-  const bool alone = P == 0 || is_direct(direct, B, W, P, Hkv, hd);
+  const bool alone = P == 0 || is_direct(direct, l, Hkv, hd);
   float* part_o = alone ? nullptr : (float*)scratch;
   float2* part_ml = alone ? nullptr : (float2*)(part_o + slots(l) * l.pair * TILE_ROWS * hd);
   if (!alone) {
