@@ -26,13 +26,14 @@ constexpr int OWN_WARPS = 4, OWN_THREADS = OWN_WARPS * 32;
 constexpr int OWN_TILE = 16;       // keys per ring stage of a warp
 constexpr int OWN_ROWS = 16;       // query heads per unit (MMA rows)
 
-// RING: tiles in a warp's ring, up to which it has them all under way at once.  0: it streams through 24 KB (two CTAs an SM, 192 KB
-// under way; refilled before a tile is worked on, with a stage less under way, it was 1 to 4 % slower).
+// RING_TILES: tiles in a warp's ring, up to which it has them all under way at once.  WIDE, NARROW: it streams through 24 KB (two CTAs an SM,
+// 192 KB under way; refilled before a tile is worked on, with a stage less under way, it was 1 to 4 % slower) or 16 KB (three CTAs).
+constexpr int WIDE = 0, NARROW = -1;
 template <int HD, int RING_TILES>
 struct OwnCfg {
   static constexpr int TILE_BYTES = OWN_TILE * HD * 2;
-  static constexpr bool STREAM = RING_TILES == 0;
-  static constexpr int STAGES = STREAM ? (24 << 10) / (2 * TILE_BYTES) : RING_TILES;   // 3 for a head dim of 128, 6 for 64
+  static constexpr bool STREAM = RING_TILES <= 0;
+  static constexpr int STAGES = STREAM ? ((RING_TILES == WIDE ? 24 : 16) << 10) / (2 * TILE_BYTES) : RING_TILES;   // of 128: 3 or 2
   static constexpr int RING = STAGES * 2 * TILE_BYTES;
   static constexpr int PART = OWN_ROWS * HD * 4;                     // a warp's partial output, over its ring
   static constexpr int STATS = OWN_ROWS * 2 * 4;                     // (max, sum) of its rows, behind it
@@ -56,7 +57,7 @@ struct Own {
 
 // WPU: warps of a CTA that share a unit.  Clusters of more than one CTA (WPU = 4) share one too.
 template <int HD, int WPU, int RING_TILES>
-__global__ void __launch_bounds__(OWN_THREADS, RING_TILES == 0 ? 3 : 4)   // 4: 128 registers, so that more CTAs fit
+__global__ void __launch_bounds__(OWN_THREADS, RING_TILES <= 0 ? 3 : 4)   // 4: 128 registers, so that more CTAs fit
 kf_shared_prefix_own(const Own a, const Layout lay, const float* part_o, const float2* part_ml, const uint32_t units) {
   using C = OwnCfg<HD, RING_TILES>;
   extern __shared__ __align__(128) uint8_t smem_raw[];
@@ -392,8 +393,9 @@ static int launch_own(const Own& a, const Layout& l, const float* part_o, const 
   // One or two tiles a warp, where that takes a CTA a unit at most and no more than 16 or 12 warps on an SM, which is what registers or
   // memory hold: everything is under way at once, and nothing crosses CTAs (8 x 5 continuations of 65 keys: 27.2 -> 23 us, 1 x 8 of 96
   // 15.6 -> 13; but 8 x 8 of 65, 14 warps an SM, 17.8, and streaming 12.9).  Units of one tile so however many they are (64 x 8 of 16 keys:
-  // streaming 18.6, so 11.6; two tiles, of 30, 20.9 and 24.9).  Else as many warps a unit as fill eight on every SM, of which each has a
-  // tile at least.
+  // streaming 18.6, so 11.6; two tiles, of 30, 20.9 and 24.9).  Else as many warps a unit as fit on the SMs at once, each with a
+  // tile at least: up to eight an SM with wide rings, or twelve with narrow ones (3 x 32 of 240 keys, 5.2 warps an SM / 10.4, 20.9 / 15.2;
+  // 8 x 16 of 128, 12 heads of 64, 10.4 warps with wide / narrow rings 15.6 / 10.2).
   for (int ring = 1; ring <= 2; ++ring) {
     int ways = 1;
     while (ways < 4 && ways * ring < tiles) ways *= 2;
@@ -401,8 +403,9 @@ static int launch_own(const Own& a, const Layout& l, const float* part_o, const 
       return ring == 1 ? go(std::integral_constant<int, 1>(), ways) : go(std::integral_constant<int, 2>(), ways);
   }
   int ways = 1;
-  while (ways < 32 && units * ways * 2 <= 8LL * num_sms && tiles >= ways * 2) ways *= 2;
-  return go(std::integral_constant<int, 0>(), ways);
+  while (ways < 32 && units * ways * 2 <= 12LL * num_sms && tiles >= ways * 2) ways *= 2;
+  const bool narrow = units * ways > 8LL * num_sms && units * ways <= 12LL * num_sms;
+  return narrow ? go(std::integral_constant<int, NARROW>(), ways) : go(std::integral_constant<int, WIDE>(), ways);
 }
 
 int launch_prefix(const void* q, const void* k, const void* v, const Layout& l, int H, int Hkv, int hd, const long long* qs, const long long* ks,
