@@ -408,8 +408,8 @@ static int launch_own(const Own& a, const Layout& l, const float* part_o, const 
   return narrow ? go(std::integral_constant<int, NARROW>(), ways) : go(std::integral_constant<int, WIDE>(), ways);
 }
 
-int launch_prefix(const void* q, const void* k, const void* v, const Layout& l, int H, int Hkv, int hd, const long long* qs, const long long* ks,
-                  const long long* vs, float scale, float* part_o, float2* part_ml, int* status, cudaStream_t stream);
+int launch_prefix(const void* q, const void* k, const void* v, const Layout& l, int H, int Hkv, int hd, bool few, const long long* qs,
+                  const long long* ks, const long long* vs, float scale, float* part_o, float2* part_ml, int* status, cudaStream_t stream);
 
 // Prompts of this many bytes outlast L2 (126 MB): two row tiles share a key.  Otherwise the second finds it there, and units of one tile
 // deal out more evenly and join both groups.  Alone / shared, us: 8 x 64 x 4000 (131 MB) 64.2 / 68.8, 1 x 32 x 32 768 (134 MB) 46.2 / 50.7,
@@ -475,7 +475,7 @@ int kf_shared_prefix_attn_bf16(const void* q, const void* k, const void* v, cons
   float* part_o = alone ? nullptr : (float*)scratch;
   float2* part_ml = alone ? nullptr : (float2*)(part_o + slots(l) * l.pair * TILE_ROWS * hd);
   if (!alone) {
-    const int rc = launch_prefix(q, k, v, l, H, Hkv, hd, qs, ks, vs, scale, part_o, part_ml, (int*)kf_status_device_ptr(), st);
+    const int rc = launch_prefix(q, k, v, l, H, Hkv, hd, S <= 2 * OWN_WARPS * OWN_TILE, qs, ks, vs, scale, part_o, part_ml, (int*)kf_status_device_ptr(), st);
     if (rc) return rc;
   }
   const Own a{(const __nv_bfloat16*)q, (const __nv_bfloat16*)own_k, (const __nv_bfloat16*)own_v, (__nv_bfloat16*)o, (const uint8_t*)rows,

@@ -7,10 +7,12 @@
 // cost nothing, and all that counts is to keep the copies in flight: two stages each of K and V (128 KB) run ahead of the products.  Three
 // were slower (4 x 32 768 keys, 64 heads of 128, with the second kernel: 102 and 98 us).  Prompts that L2 holds (64 continuations of 8000
 // keys: four row tiles read them) are bound by the chain scores - weights - products of a row tile, 1450 cycles a tile with two under way.
-// Where a CTA has three tiles at most, what counts is that the second kernel does its own part meanwhile, beside it on the same SM: LEAN, in
-// 96 registers a thread, with scores taken from tensor memory twice, 32 at a time, for the maximum and for the exponentials, and at most
-// 162 KB.  Not LEAN / LEAN, us: 1 x 8 x 4000 (two tiles) 14.2 / 11.3, 24 x 8 x 512 (three) 15.4 / 14.9, 16 x 4 x 800 (four) 13.8 / 15.0,
-// 8 x 5 x 1777 (seven) 21.3 / 22.5.
+// Where the softmax does not take the time it is LEAN: 96 registers a thread, with scores taken from tensor memory twice, 32 at a time, for
+// the maximum and for the weights, and at most 162 KB, so that the second kernel does its own part meanwhile, beside it on the same SM.  That
+// is up to three tiles a CTA, and with heads of 128 (of 64 there are twice the scores per byte) wherever one row tile reads the keys and the
+// second kernel's rings are small.  Not LEAN / LEAN, us: 1 x 8 x 4000 (two tiles) 14.2 / 11.3, 1 x 8 x 16 000 of 96 own (seven) 23.6 / 21.5,
+// 4 x 8 x 32 768 of 20 own (56) 94.8 / 93.0; of 200 own 106.9 / 109.8, 8 x 8 x 4000, 12 heads of 64, 29.5 / 32.9, 2 x 64 x 8000 (two row
+// tiles) 31.3 / 32.9.
 #include "attention_common.cuh"
 #include "shared_prefix.cuh"
 #include "skinny_common.cuh"
@@ -576,18 +578,19 @@ static int launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMa
 }
 
 template <int HD>
-static int launch_hd(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const Layout& l, int group, float scale, float* part_o,
-                     float2* part_ml, int* status, cudaStream_t stream) {
+static int launch_hd(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const Layout& l, int group, bool few, float scale,
+                     float* part_o, float2* part_ml, int* status, cudaStream_t stream) {
   const long long tiles = (long long)tiles_of(l.P) * l.per_prompt * l.B, each = (tiles + l.ctas - 1) / l.ctas;   // most tiles of a CTA
   const int stages = each < Cfg<HD>::STAGES ? (int)each : Cfg<HD>::STAGES;
   if (l.pair == 2) return launch<HD, false, true>(mq, mk, mv, l, group, stages, scale, part_o, part_ml, status, stream);
-  return each <= LEAN_TILES ? launch<HD, true, false>(mq, mk, mv, l, group, stages, scale, part_o, part_ml, status, stream)
-                            : launch<HD, false, false>(mq, mk, mv, l, group, stages, scale, part_o, part_ml, status, stream);
+  const bool lean = each <= LEAN_TILES || (HD == 128 && l.row_units == 1 && few);
+  return lean ? launch<HD, true, false>(mq, mk, mv, l, group, stages, scale, part_o, part_ml, status, stream)
+              : launch<HD, false, false>(mq, mk, mv, l, group, stages, scale, part_o, part_ml, status, stream);
 }
 
-// Steps in elements: q prompt, continuation, head; k and v prompt, position, head.
-int launch_prefix(const void* q, const void* k, const void* v, const Layout& l, int H, int Hkv, int hd, const long long* qs, const long long* ks,
-                  const long long* vs, float scale, float* part_o, float2* part_ml, int* status, cudaStream_t stream) {
+// Steps in elements: q prompt, continuation, head; k and v prompt, position, head.  few: the second kernel's own keys are.
+int launch_prefix(const void* q, const void* k, const void* v, const Layout& l, int H, int Hkv, int hd, bool few, const long long* qs,
+                  const long long* ks, const long long* vs, float scale, float* part_o, float2* part_ml, int* status, cudaStream_t stream) {
   const int group = H / Hkv;
   CUtensorMap mq, mk, mv;
   int rc = make_map_4d(&mq, q, {(uint64_t)hd, (uint64_t)H, (uint64_t)l.W, (uint64_t)l.B}, {qs[2], qs[1], qs[0]},
@@ -597,8 +600,8 @@ int launch_prefix(const void* q, const void* k, const void* v, const Layout& l, 
   if (rc) return 2000 + rc;
   rc = make_map_4d(&mv, v, {(uint64_t)hd, (uint64_t)Hkv, (uint64_t)l.P, (uint64_t)l.B}, {vs[2], vs[1], vs[0]}, {64u, 1u, (uint32_t)TILE_KEYS, 1u});
   if (rc) return 3000 + rc;
-  return hd == 128 ? launch_hd<128>(mq, mk, mv, l, group, scale, part_o, part_ml, status, stream)
-                   : launch_hd<64>(mq, mk, mv, l, group, scale, part_o, part_ml, status, stream);
+  return hd == 128 ? launch_hd<128>(mq, mk, mv, l, group, few, scale, part_o, part_ml, status, stream)
+                   : launch_hd<64>(mq, mk, mv, l, group, few, scale, part_o, part_ml, status, stream);
 }
 
 }  // namespace shared_prefix
