@@ -17,8 +17,8 @@
 //     logits the lowest index is the largest key.  There are few, so a candidate's place is how many are larger, counted; the cluster's
 //     CTAs put theirs into the first one's shared memory.
 // What bounds it: many prompts, the logits, which are read once (64 x 8 x 128 256 in bf16, an eighth finished: 115 MB in 40 us, 2.9 TB/s: the
-// pass at 75 to 80 % of a copy's rate, and behind it, in every CTA at the same time, bounds, candidates and sums); few prompts, these steps and the launch
-// (1 x 4 x 32 000: 7.4 us).  Launches are joined to the one before (programmatic launch): by itself a launch of clusters began 2.4 us later.
+// pass at 75 to 80 % of a copy's rate, and behind it, in every CTA at the same time, bounds, candidates and sums); few prompts, these steps
+// and the launch (1 x 4 x 32 000: 7.4 us).  Launches are joined to the one before (programmatic launch): by itself a launch of clusters began 2.4 us later.
 //
 // kf_beam_reorder.  state[b, w] = state[b, parent[b, w]] for all states in one launch.  A thread owns 16 bytes of a column: it reads
 // the column's W values and then writes them, so that parents may be any selection of beams, also in place, without a second buffer.

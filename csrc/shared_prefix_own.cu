@@ -475,7 +475,8 @@ int kf_shared_prefix_attn_bf16(const void* q, const void* k, const void* v, cons
   float* part_o = alone ? nullptr : (float*)scratch;
   float2* part_ml = alone ? nullptr : (float2*)(part_o + slots(l) * l.pair * TILE_ROWS * hd);
   if (!alone) {
-    const int rc = launch_prefix(q, k, v, l, H, Hkv, hd, S <= 2 * OWN_WARPS * OWN_TILE, qs, ks, vs, scale, part_o, part_ml, (int*)kf_status_device_ptr(), st);
+    const bool few = S <= 2 * OWN_WARPS * OWN_TILE;   // rings of one or two tiles
+    const int rc = launch_prefix(q, k, v, l, H, Hkv, hd, few, qs, ks, vs, scale, part_o, part_ml, (int*)kf_status_device_ptr(), st);
     if (rc) return rc;
   }
   const Own a{(const __nv_bfloat16*)q, (const __nv_bfloat16*)own_k, (const __nv_bfloat16*)own_v, (__nv_bfloat16*)o, (const uint8_t*)rows,

@@ -5,7 +5,8 @@
     python scripts/generate.py cfg.toml --checkpoint ... --interactive
 
 Same contract as the reference's scripts/generate.py:42-151 (DCP ``{"model": ...}`` load, prompt or REPL,
-temperature / top-k / top-p sampling), and ``--num-beams`` for a beam search.  Without a tokenizer path the prompt is read as space-separated token ids.
+temperature / top-k / top-p sampling), and ``--num-beams`` for a beam search.  Without a tokenizer path the prompt is read as
+space-separated token ids.
 """
 
 from __future__ import annotations
@@ -72,8 +73,9 @@ def main(argv=None) -> int:
         if room <= 0:
             raise SystemExit(f"the prompt has {len(ids)} tokens; the model's context is {cfg.model.max_seq_len}")
         if args.num_beams > 0:
-            out = beam_search(model, x, min(args.max_new_tokens, room), args.num_beams, tok.eos_token_id if tok else None, args.length_penalty)[0][0, 0]
-            new = out.tolist()
+            best, _ = beam_search(model, x, min(args.max_new_tokens, room), args.num_beams, tok.eos_token_id if tok else None,
+                                  args.length_penalty)
+            new = best[0, 0].tolist()
             return tok.decode(new) if tok else " ".join(map(str, new))
         out = generate(model, x, min(args.max_new_tokens, room), args.temperature, args.top_k, args.top_p,
                        eos_token_id=tok.eos_token_id if tok else None,

@@ -216,3 +216,19 @@ def test_scales_that_leave_32_bits_take_the_formulas(native_lib, p, s):
         got = F.shared_prefix_attention(*args, scale=2.0**-100)
         near(got, args, scale=2.0**-100)
     assert native_lib.LAUNCH_COUNT > before
+
+
+# sizes at which the kernels take other forms: narrow rings (10 warps an SM) with and without the prompts, many tiles of keys a CTA in few
+# and in many registers, prompts of one tile by one kernel where they are many, and by two
+@pytest.mark.parametrize("b,w,p,s,h,hkv,hd", [
+    (3, 32, 20, 70, 16, 8, 128), (8, 16, 140, 40, 12, 12, 64), (1, 2, 40_001, 9, 8, 8, 128), (1, 2, 40_001, 140, 8, 8, 128),
+    (40, 4, 60, 17, 16, 8, 128), (9, 16, 128, 17, 8, 8, 128), (70, 8, 3, 16, 4, 4, 64),
+])
+def test_forms(native_lib, b, w, p, s, h, hkv, hd):
+    args = make(b, w, p, s, h, hkv, hd, torch.bfloat16, table=True, ragged=b > 1, seed=s, device="cuda")
+    before = native_lib.LAUNCH_COUNT
+    got = F.shared_prefix_attention(*args)
+    assert native_lib.LAUNCH_COUNT > before
+    near(got, args)
+    assert torch.equal(got, F.shared_prefix_attention(*args))
+    assert native_lib.read_status() == 0
