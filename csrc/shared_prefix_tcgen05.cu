@@ -6,7 +6,8 @@
 // of an SM's share of HBM; its two products take 1040, its 16 384 exponentials 1024.  So rows that are not there (a tile is always 128)
 // cost nothing, and all that counts is to keep the copies in flight: two stages each of K and V (128 KB) run ahead of the products.  Three
 // were slower (4 x 32 768 keys, 64 heads of 128, with the second kernel: 102 and 98 us).  Prompts that L2 holds (64 continuations of 8000
-// keys: four row tiles read them) are bound by the chain scores - weights - products of a row tile, 1450 cycles a tile with two under way.
+// keys: two row tiles of each key head read them) are bound by what L2 gives, 258 MB in 25 us, and where row tiles share a key by the chain
+// scores - weights - products, 1450 cycles a tile with two under way, which is no faster.
 // Where the softmax does not take the time it is LEAN: 96 registers a thread, with scores taken from tensor memory twice, 32 at a time, for
 // the maximum and for the weights, and at most 162 KB, so that the second kernel does its own part meanwhile, beside it on the same SM.  That
 // is up to three tiles a CTA, and with heads of 128 (of 64 there are twice the scores per byte) wherever one row tile reads the keys and the
