@@ -4,6 +4,10 @@
 // key head, and with more rows than that two of them may share the keys.  Keys come in tiles of 128.  The tiles of all units, one after the
 // other, are dealt out to the CTAs in equal ranges, so that every SM has the same share whatever the lengths of the prompts; a CTA leaves
 // one partial result for every unit that its range meets.
+//
+// Without lens, and where that makes the ranges no more than SPARE tiles longer, a unit counts for a whole number of ranges: a CTA that ends a
+// unit and begins another one has two results to write, 5800 cycles each, and waits for first keys twice.  Equal ranges / whole numbers, us:
+// 2 x 30 x 8254 (32 heads on 8) 27.5 / 24.1, 6 x 16 x 1568 (16 on 4) 15.6 / 13.1, 4 x 3 x 6522 (40 on 8) 29.3 / 26.6, 2 x 64 x 8000 32.3 / 28.4.
 #pragma once
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -12,6 +16,7 @@ namespace kf {
 namespace shared_prefix {
 
 constexpr int TILE_KEYS = 128, TILE_ROWS = 128;
+constexpr int SPARE = 3;
 
 struct Layout {
   const int* lens;     // keys of each prompt, or null: P for all
@@ -19,7 +24,8 @@ struct Layout {
   int per_prompt;      // units of a prompt: key heads x row_units
   int row_units;       // units of a key head
   int pair, wt;        // row tiles of a unit, 1 or 2; continuations per row tile
-  int ctas;
+  int ctas, most;      // how many are launched; how many might be, whatever the lengths
+  int span;            // without lens: tiles that a unit counts for
 };
 
 __host__ __device__ __forceinline__ int tiles_of(int len) { return (len + TILE_KEYS - 1) / TILE_KEYS; }
@@ -31,7 +37,7 @@ __device__ __forceinline__ uint32_t range(uint32_t total, int ctas) { return (to
 
 // Tiles of the prompts before b (all: b = B), by one warp; every lane has the result.
 __device__ __forceinline__ uint32_t tiles_before(const Layout& l, int b) {
-  if (!l.lens) return uint32_t(tiles_of(l.P)) * l.per_prompt * b;
+  if (!l.lens) return uint32_t(l.span) * l.per_prompt * b;
   uint32_t n = 0;
   for (int i = threadIdx.x & 31; i < b; i += 32) n += tiles_of(length(l, i));
 #pragma unroll
@@ -40,7 +46,7 @@ __device__ __forceinline__ uint32_t tiles_before(const Layout& l, int b) {
 }
 
 // A partial result of unit u by CTA c lies in slot u + c: along the tiles every step raises one of the two, so no two share one.
-__host__ __device__ __forceinline__ long long slots(const Layout& l) { return (long long)l.B * l.per_prompt + l.ctas; }
+__host__ __device__ __forceinline__ long long slots(const Layout& l) { return (long long)l.B * l.per_prompt + l.most; }
 
 }  // namespace shared_prefix
 }  // namespace kf

@@ -249,8 +249,9 @@ kf_shared_prefix_own(const Own a, const Layout lay, const float* part_o, const f
     const uint32_t first = tiles_before(lay, b), chunk = range(tiles_before(lay, lay.B), lay.ctas);
     const int nt = there ? tiles_of(length(lay, b)) : 0;
     if (nt > 0) {
-      c0 = int((first + uint32_t(u) * nt) / chunk);
-      parts = int((first + uint32_t(u + 1) * nt - 1) / chunk) - c0 + 1;
+      const uint32_t begin = first + uint32_t(u) * (lay.lens ? nt : lay.span);
+      c0 = int(begin / chunk);
+      parts = int((begin + nt - 1) / chunk) - c0 + 1;
     }
   }
   if (WPU == 1) __syncwarp();
@@ -422,7 +423,13 @@ static bool make_layout(Layout& l, const void* lens, int B, int W, int P, int gr
   const int wt = TILE_ROWS / group < W ? TILE_ROWS / group : W;
   const int pair = wt < W && 4LL * B * P * Hkv * hd > PAIR_BYTES ? 2 : 1, row_units = (W + wt * pair - 1) / (wt * pair);
   const long long tiles = (long long)tiles_of(P) * Hkv * row_units * B;
-  l = Layout{(const int*)lens, B, W, P, Hkv * row_units, row_units, pair, wt, (int)(tiles < num_sms ? tiles : num_sms)};
+  const int most = (int)(tiles < num_sms ? tiles : num_sms);
+  l = Layout{(const int*)lens, B, W, P, Hkv * row_units, row_units, pair, wt, most, most, tiles_of(P)};
+  const long long units = (long long)B * l.per_prompt;
+  if (!lens && P > 0 && units <= num_sms) {
+    const int ways = num_sms / (int)units, each = (l.span + ways - 1) / ways, whole = (l.span + each - 1) / each;
+    if (each <= (tiles + most - 1) / most + SPARE) l.ctas = (int)units * whole, l.span = whole * each;
+  }
   return tiles < 0x7fff0000LL && (long long)B * W * Hkv * group < 1LL << 27;   // counts of tiles and units in 32 bits
 }
 

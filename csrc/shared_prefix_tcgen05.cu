@@ -5,9 +5,9 @@
 // What bounds it: the keys and values, 4 hd bytes per position and head.  A tile of 128 keys of 128 values is 64 KB, which is 2700 cycles
 // of an SM's share of HBM; its two products take 1040, its 16 384 exponentials 1024.  So rows that are not there (a tile is always 128)
 // cost nothing, and all that counts is to keep the copies in flight: two stages each of K and V (128 KB) run ahead of the products.  Three
-// were slower (4 x 32 768 keys, 64 heads of 128, with the second kernel: 102 and 98 us).  Prompts that L2 holds (64 continuations of 8000
-// keys: two row tiles of each key head read them) are bound by what L2 gives, 258 MB in 25 us, and where row tiles share a key by the chain
-// scores - weights - products, 1450 cycles a tile with two under way, which is no faster.
+// were slower (4 x 32 768 keys, 64 heads of 128, with the second kernel: 102 and 98 us).  With more rows (64 continuations of 8000 keys:
+// two row tiles of each key head) the chain scores - weights - products of a row tile, 3000 cycles with two of them under way, is what takes
+// the time; first keys (6000 cycles) and a unit's partial result (5800) come on top.
 // Where the softmax does not take the time it is LEAN: 96 registers a thread, with scores taken from tensor memory twice, 32 at a time, for
 // the maximum and for the weights, and at most 162 KB, so that the second kernel does its own part meanwhile, beside it on the same SM.  That
 // is up to three tiles a CTA, and with heads of 128 (of 64 there are twice the scores per byte) wherever one row tile reads the keys and the
@@ -73,7 +73,7 @@ __device__ Walk locate(const Layout& l) {
   if (w.left <= 0) return w;
   uint32_t before = 0;
   if (!l.lens) {
-    const uint32_t each = uint32_t(tiles_of(l.P)) * l.per_prompt;
+    const uint32_t each = uint32_t(l.span) * l.per_prompt;
     w.b = int(t0 / each);
     before = each * w.b;
   } else {
@@ -97,8 +97,10 @@ __device__ Walk locate(const Layout& l) {
     }
   }
   w.nt = tiles_of(length(l, w.b));
-  w.u = int((t0 - before) / w.nt);
-  w.j = int((t0 - before) % w.nt);
+  const int span = l.lens ? w.nt : l.span;
+  w.u = int((t0 - before) / span);
+  w.j = int((t0 - before) % span);
+  if (span > w.nt) w.left = min(w.left, w.nt - w.j);   // one unit, whose last range may be shorter
   return w;
 }
 
