@@ -152,8 +152,10 @@ kf_shared_prefix_tcgen05(const __grid_constant__ CUtensorMap map_q, const __grid
   auto pv_done = [&](int g) { return bar_base + 8u * (18 + g); };
   const uint32_t q_full = bar_base + 8u * 20, q_empty = bar_base + 8u * 21;
   const uint32_t o_final = bar_base + 8u * 22, o_free = bar_base + 8u * 23, drain_bar = bar_base + 8u * 24;
-  volatile uint32_t* tmem_slot_ptr = reinterpret_cast<volatile uint32_t*>(bar_generic + 8 * 25);
-  Walk* start = reinterpret_cast<Walk*>(bar_generic + 8 * 26);
+  const uint32_t v_begun = bar_base + 8u * 25;   // V's producer has seen the first K
+  volatile uint32_t* tmem_slot_ptr = reinterpret_cast<volatile uint32_t*>(bar_generic + 8 * 26);
+  Walk* start = reinterpret_cast<Walk*>(bar_generic + 8 * 27);
+  static_assert(8 * 27 + sizeof(Walk) <= 256, "what Cfg::smem has for barriers");
 
   const int warp = warp_index();
   const int lane = threadIdx.x & 31;
@@ -175,6 +177,7 @@ kf_shared_prefix_tcgen05(const __grid_constant__ CUtensorMap map_q, const __grid
     mbar_init(o_final, 1);
     mbar_init(o_free, 8);
     mbar_init(drain_bar, 1);
+    mbar_init(v_begun, 1);
     mbar_fence_init();
     tma_prefetch_desc(&map_q);
     tma_prefetch_desc(&map_k);
@@ -219,6 +222,9 @@ kf_shared_prefix_tcgen05(const __grid_constant__ CUtensorMap map_q, const __grid
                           (wk.u % lay.row_units * Q_TILES + g) * lay.wt, wk.b);
           ++q_issued;
           for (int j = wk.j; j < wk.j + n; ++j, turn.next(stages)) {
+            // A wait knows a phase by its parity alone.  Nothing else that comes before a second K in the first stage waits for V, and after it V's
+            // producer would not see the first any more.
+            if (issued == stages && !mbar_wait(v_begun, 0, status, KF_ERR_WAIT_EMPTY)) { ok = false; break; }
             if (issued >= stages && !mbar_wait(k_empty(turn.st), turn.phase ^ 1u, status, KF_ERR_WAIT_EMPTY)) { ok = false; break; }
             mbar_expect_tx(k_full(turn.st), C::TILE_BYTES);
 #pragma unroll
@@ -242,6 +248,7 @@ kf_shared_prefix_tcgen05(const __grid_constant__ CUtensorMap map_q, const __grid
         Turn turn;
         // the first K before the first V: the scores can begin
         if (wk.left > 0) ok = mbar_wait(k_full(0), 0, status, KF_ERR_WAIT_FULL);
+        mbar_arrive(v_begun);
         while (wk.left > 0 && ok) {
           const int n = segment(wk), hk = wk.u / lay.row_units;
           for (int j = wk.j; j < wk.j + n; ++j, turn.next(stages)) {
