@@ -5,9 +5,12 @@
 // Within a beam the order of candidates is that of its logits, so W tokens of each beam are all that can be among the best.  One cluster
 // of CTAs a prompt; the logits of its beams, one after the other, are dealt out to the CTAs in equal ranges.
 //   * One pass over the logits: a thread keeps the largest of its logits and the sum of exp(x - r), with r the largest of its first round; in
-//     fp32 over at most a few hundred terms and in 64 bits from there on, because candidates of different beams may lie close together.
-//     r moves only when a logit is 27 above it: moved with every new maximum, it cost a branch in most vectors.  The difference is taken
+//     fp32 over a vector and in 64 bits from there on, because candidates of different beams may lie close together.
+//     r moves only when a logit is 8 above it: moved with every new maximum, it cost a branch in most vectors.  The difference is taken
 //     before the factor log2 e: large logits lose nothing, and rows of the type's lowest value have exponents of zero like any others.
+//   * What a row's sum comes to depends on where the row begins and which threads read it, in the last bits.  So where candidates of different
+//     beams are so close that this could decide (NEAR), the first CTA takes these beams' sums again in 64 bits, in the order of the values,
+//     and counts places again: equal rows with equal scores tie, whatever their places in memory.
 //   * Each of a CTA's 8 warps has ceil(W / 8) threads whose largest logit is at least the warp's ceil(W / 8)-th largest.  So at least W
 //     logits reach the least of these over the warps, a bound that costs a warp-wide maximum or a few.  Taken after each thread's first two
 //     vectors, and whenever there are twice as many, it leaves about a hundred vectors for 8 beams that reach it and are noted; taken
@@ -34,6 +37,7 @@ namespace kf {
 namespace beam {
 
 using namespace kf::attn;   // two-wide arithmetic
+using decode::fast_exp2;
 using decode::mapa_shared;
 
 constexpr int MAX_BEAMS = 32;   // a warp's list is one key per lane
@@ -67,12 +71,6 @@ __device__ __forceinline__ Key make_key(float x, uint32_t index) { return (Key(o
 __device__ __forceinline__ float key_value(Key k) { return unordered(uint32_t(k >> 32)); }
 __device__ __forceinline__ uint32_t key_index(Key k) { return 0xffffffffu - uint32_t(k); }
 
-__device__ __forceinline__ float exp2_fast(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 // Maximum and minimum that keep numbers below the smallest normal one (the build's fast math would make them zeros) and ignore NaN.
 __device__ __forceinline__ float max_of(float a, float b) {
   float r;
@@ -84,6 +82,25 @@ __device__ __forceinline__ float min_of(float a, float b) {
   asm("min.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
+
+// e^d for d <= 0, the difference of two references, with an error that does not grow with d: the whole part of d log2 e goes into the
+// exponent, and log2 e has 48 bits.  Below -80 is nothing beside a sum of 1.
+__device__ __forceinline__ float exp_between(float d) {
+  constexpr float LOG2E = 1.4426950408889634f, REST = float(1.4426950408889634 - double(LOG2E));
+  d = max_of(d, -80.f);
+  const float whole = rintf(__fmul_rn(d, LOG2E)), part = __fmaf_rn(d, REST, __fmaf_rn(d, LOG2E, -whole));
+  return __fmul_rn(fast_exp2(part), __int_as_float((int(whole) + 127) << 23));
+}
+
+// What the one pass leaves in a logarithm of a sum, at most.  The relative error of a sum is the mean of its terms' errors, which are
+//   * of an exponential: 2^-22; of its argument: |d| (2^-24 + 2^-24 + 2^-26), from the difference, the factor and log2 e.  The mean of |d|
+//     is at most HIGH + 1 above the reference, and below, with a term next to the reference among n of them, the a - 1 for which
+//     a + log(a - 1) = log n + 1/2: 4.3 for 500 of a thread, 11 for the 2^20 that it may have.  So 2.4e-7 + 11 * 1.4e-7;
+//   * of the additions: 6 in 32 bits behind a term, 3.6e-7, the rest is in 64;
+//   * of exp_between: 2^-22 + 2^-24, at three joins, and with a reference that moves: what has moved three times counts for nothing.
+// That is 4e-6.  Where candidates of different beams are no further apart than twice as much, the sums are taken again in 64 bits.
+constexpr float HIGH = 8.f;   // a reference moves where a logit is this far above it
+constexpr double NEAR = 8e-6;
 
 // Key by key: the largest `width` that a warp has met, lane i the i-th (0 = none).
 struct TopList {
@@ -187,12 +204,141 @@ __device__ __forceinline__ void st_cluster_u64(uint32_t addr, unsigned long long
   asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(addr), "l"(v) : "memory");
 }
 
+// e^d for d <= 0 in 64 bits, without a branch, so that several are under way: 2^n e^r with |r| <= log(2) / 2 and the exponential's series up to
+// r^12 / 12!, of which r^13 / 13! = 2e-16 is left.  What is below e^-700 counts for nothing beside the 1 of the largest.
+__device__ __forceinline__ double exp_below(double d) {
+  constexpr double LN2 = 0.6931471805599453, LN2_REST = 2.3190468138462996e-17;   // log 2 in 106 bits
+  d = fmax(d, -700.0);
+  const double n = rint(d * 1.4426950408889634), r = fma(-n, LN2_REST, fma(-n, LN2, d));
+  double y = fma(1.0 / 479001600.0, r, 1.0 / 39916800.0);
+  y = fma(y, r, 1.0 / 3628800.0), y = fma(y, r, 1.0 / 362880.0), y = fma(y, r, 1.0 / 40320.0), y = fma(y, r, 1.0 / 5040.0);
+  y = fma(y, r, 1.0 / 720.0), y = fma(y, r, 1.0 / 120.0), y = fma(y, r, 1.0 / 24.0), y = fma(y, r, 1.0 / 6.0);
+  y = fma(y, r, 0.5), y = fma(y, r, 1.0), y = fma(y, r, 1.0);
+  return y * __hiloint2double((1023 + int(n)) << 20, 0);
+}
+
+template <typename T>
+struct Call {
+  const T* logits;
+  long long stride_b, stride_w;
+  const float* scores;
+  const uint8_t* finished;
+  int W, V;
+  long long eos, pad;
+  float* out_scores;
+  long long *out_parents, *out_tokens;
+  uint8_t* out_finished;
+};
+
+// The candidates of a prompt's beams and their places, in shared memory.  The pointers are kept for choose_again: as registers they are spilled.
+struct Choice {
+  Key* total;                // [W][totals]: scores in the order of integers, best first, 0: none
+  uint32_t* token;           // [W][W]
+  int totals;
+  int winner[MAX_BEAMS];     // of each place: which candidate, beam * MAX_BEAMS + its rank there, or -1
+  Key best[MAX_BEAMS];       // its score
+  Key next[MAX_BEAMS];       // of each beam: its best candidate without a place, 0: none
+};
+
+// A candidate's place: how many come before it, its own beam's better ones, others' better ones, lower beams' equal ones; a warp a beam,
+// eight lanes a candidate.
+__device__ __forceinline__ void find_places(Choice& c, const Key* total, int totals, int W) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int w = warp; w < W; w += WARPS)
+    for (int j0 = 0; j0 < W; j0 += 4) {
+      const int j = j0 + lane / 8;
+      const Key mine = j < W ? total[w * totals + j] : 0;
+      int before = 0;
+      for (int x = lane & 7; x < W; x += 8) {
+        const Key* of = total + x * totals;
+        const Key limit = mine - (x < w);
+        int n = 0;
+        for (int k = 0; k < W; k += 8)   // zeros behind the last one
+#pragma unroll
+          for (int e = 0; e < 8; ++e) n += of[k + e] > limit;
+        before += x == w ? j : n;
+      }
+      before = sum_of_8(before);
+      const bool among = mine && before < W;
+      const bool ahead = __shfl_up_sync(0xffffffffu, int(among), 8) || lane < 8;   // the one before it has a place
+      if ((lane & 7) == 0 && mine) {
+        if (among) c.winner[before] = w * MAX_BEAMS + j, c.best[before] = mine;
+        else if (ahead) c.next[w] = mine;
+      }
+      if (!__all_sync(0xffffffffu, among)) break;   // nor are those behind
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ void write_places(const Call<T>& a, const Choice& c, const uint32_t* token, long long first, uint32_t ends, int W) {
+  const int tid = threadIdx.x;
+  if (tid >= W) return;
+  const int i = c.winner[tid], parent = i < 0 ? tid : i / MAX_BEAMS;
+  const bool ended = i >= 0 && ((ends >> parent) & 1u);
+  const long long t = i < 0 || ended ? a.pad : (long long)token[parent * W + i % MAX_BEAMS];
+  a.out_scores[first + tid] = i < 0 ? -INFINITY : float(unordered(c.best[tid]));
+  a.out_parents[first + tid] = parent;
+  a.out_tokens[first + tid] = t;
+  a.out_finished[first + tid] = ended || (i >= 0 && t == a.eos);
+}
+
+// Places once more, with the scores of some beams (`near`, those of `live` among them with logits) from sums in 64 bits: value i by thread
+// i % THREADS, so that equal rows have equal sums wherever they lie.  Where all rows are equal one sum will do, whatever its last bits.
+// Nothing follows this, so that the pass keeps no registers for it; that, and not a call (0.1 to 0.5 us for every selection).
+template <typename T>
+__device__ __forceinline__ void choose_again(const Call<T>& a, Choice& c, long long b, uint32_t near, uint32_t live, uint32_t ends, double* of_warps) {
+  constexpr int AT_ONCE = 8;
+  const int tid = threadIdx.x, W = a.W;
+  const int lead = __ffs(near & live) - 1;
+  const T* x0 = a.logits + b * a.stride_b + lead * a.stride_w;
+  int same = (near & ~live) == 0;
+  for (uint32_t left = near & live & ~(1u << lead); same && left; left &= left - 1) {
+    const T* x = a.logits + b * a.stride_b + (__ffs(left) - 1) * a.stride_w;
+#pragma unroll 1
+    for (int i0 = tid; i0 < a.V; i0 += AT_ONCE * THREADS)
+#pragma unroll
+      for (int e = 0; e < AT_ONCE; ++e)
+        if (i0 + e * THREADS < a.V) same &= clean(Logits<T>::one(x + i0 + e * THREADS)) == clean(Logits<T>::one(x0 + i0 + e * THREADS));
+    same = __syncthreads_and(same);
+  }
+  double lse = clean(Logits<T>::one(x0 + c.token[lead * W])) - (unordered(c.total[lead * c.totals]) - double(a.scores[b * W + lead]));
+  __syncthreads();   // the total has been read
+  for (uint32_t left = near & live; left; left &= left - 1) {
+    const int w = __ffs(left) - 1;
+    const T* x = a.logits + b * a.stride_b + w * a.stride_w;
+    if (!same) {
+      const double top = clean(Logits<T>::one(x + c.token[w * W]));
+      double sum = 0.0;
+#pragma unroll 1
+      for (int i0 = tid; i0 < a.V; i0 += AT_ONCE * THREADS) {
+        float v[AT_ONCE];
+#pragma unroll
+        for (int e = 0; e < AT_ONCE; ++e) v[e] = i0 + e * THREADS < a.V ? clean(Logits<T>::one(x + i0 + e * THREADS)) : -INFINITY;
+#pragma unroll
+        for (int e = 0; e < AT_ONCE; ++e) sum += exp_below(double(v[e]) - top);
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      if ((tid & 31) == 0) of_warps[tid >> 5] = sum;
+      __syncthreads();
+      sum = of_warps[0];
+      for (int i = 1; i < WARPS; ++i) sum += of_warps[i];
+      lse = top + log(sum);
+    }
+    Key* mine = c.total + w * c.totals + tid;
+    if (tid < W && *mine) *mine = ordered(double(a.scores[b * W + w]) + (double(clean(Logits<T>::one(x + c.token[w * W + tid]))) - lse));
+    __syncthreads();   // of_warps has been read
+  }
+  find_places(c, c.total, c.totals, W);
+  __syncthreads();
+  write_places(a, c, c.token, b * W, ends, W);
+}
+
 template <typename T>
 __global__ void __launch_bounds__(THREADS, 4)
-kf_beam_select(const T* logits, long long stride_b, long long stride_w, const float* scores, const uint8_t* finished, int W, int V,
-               long long eos, long long pad, float* out_scores, long long* out_parents, long long* out_tokens, uint8_t* out_finished) {
+kf_beam_select(const __grid_constant__ Call<T> a) {
   constexpr int N = Logits<T>::N;
-  constexpr float LOG2E = 1.4426950408889634f, HIGH = 27.f;
+  constexpr float LOG2E = 1.4426950408889634f;
   constexpr int UNROLL = 2;
   // What a CTA found in its part of a row, in the first CTA's memory.  Part (nth row, CTA) has number nth + CTA: along the vectors every
   // step raises one of the two.
@@ -208,8 +354,10 @@ kf_beam_select(const T* logits, long long stride_b, long long stride_w, const fl
   __shared__ Key notes[NOTES];                     // (largest logit, vector)
   __shared__ Raw noted_raw[NOTES];                 // the vector
   __shared__ Key found[ROOM];                      // candidates, or the warps' lists
-  __shared__ int winner[MAX_BEAMS];                // of each place: which candidate
-  Key* total = reinterpret_cast<Key*>(noted_raw);  // [W][totals]: scores in the order of integers, best first, 0: none
+  __shared__ Choice choice;
+  __shared__ uint32_t again;                       // beams that choose_again looks at
+  const int W = a.W, V = a.V;
+  Key* total = reinterpret_cast<Key*>(noted_raw);
   const int totals = (W + 7) / 8 * 8 + 1;          // an odd number spreads the beams' over the banks
   uint32_t* token = reinterpret_cast<uint32_t*>(found);
   static_assert(sizeof(noted_raw) >= MAX_BEAMS * (MAX_BEAMS + 1) * 8 && sizeof(found) >= MAX_BEAMS * MAX_BEAMS * 4, "");
@@ -219,14 +367,15 @@ kf_beam_select(const T* logits, long long stride_b, long long stride_w, const fl
   const int rank = int(cluster_ctarank());
   const long long b = blockIdx.x / ctas, first = b * W;
   if (tid < MAX_PARTS) n_found[tid] = n_notes[tid] = 0;
-  if (tid < MAX_BEAMS) winner[tid] = -1;
+  if (tid < MAX_BEAMS) choice.winner[tid] = -1, choice.next[tid] = 0;
+  if (tid == 0) choice.total = total, choice.token = token, choice.totals = totals;
   grid_dep_wait();
   grid_dep_launch();
   // No pointer is __restrict__: loads of what it says is constant may move ahead of the wait.
   // Beams whose logits count.  One without a score above -inf (or with NaN) has no candidates, a finished one has itself.
-  const float score = lane < W ? scores[first + lane] : -INFINITY;
+  const float score = lane < W ? a.scores[first + lane] : -INFINITY;
   const bool alive = score > -INFINITY;
-  const bool done = lane < W && finished != nullptr && finished[first + lane];
+  const bool done = lane < W && a.finished != nullptr && a.finished[first + lane];
   const uint32_t live = __ballot_sync(0xffffffffu, alive && !done);
   // vectors of a row, at most, so that CTAs meet eighths of rows
   uint32_t per = (max(1u, uint32_t(V) / N) + CTAS_FEW - 1) / CTAS_FEW * CTAS_FEW;
@@ -246,7 +395,7 @@ kf_beam_select(const T* logits, long long stride_b, long long stride_w, const fl
     pos += v_end - v0;
     // the nth live beam
     const int w = __ffs(__ballot_sync(0xffffffffu, ((live >> lane) & 1u) && __popc(live & ((1u << lane) - 1u)) == int(nth))) - 1;
-    const T* x0 = logits + b * stride_b + w * stride_w;
+    const T* x0 = a.logits + b * a.stride_b + w * a.stride_w;
     // vectors from the row's first 32-byte boundary on; what is left at both ends goes with the first vector, a value a thread
     const int misaligned = int(reinterpret_cast<uintptr_t>(x0) & 31) / int(sizeof(T));
     const int head = misaligned ? min(V, N - misaligned) : 0;
@@ -316,9 +465,10 @@ kf_beam_select(const T* logits, long long stride_b, long long stride_w, const fl
     bound();
 
     // ---- the pass: exp(x - r); limit: the logit that is HIGH above r
-    float r = m > -INFINITY ? m : 0.f, limit = m > -INFINITY ? r + HIGH : -INFINITY;
+    // Whole numbers, so that differences of references are exact (those beyond 2^24 differ by nothing, or by so much that it does not matter).
+    float r = m > -INFINITY ? rintf(m) : 0.f, limit = m > -INFINITY ? r + HIGH : -INFINITY;
     float usual = fminf(least_f, limit);   // vectors whose largest is below only add to the sum
-    uint64_t sum2[2] = {pack2(alone > -INFINITY ? exp2_fast((alone - r) * LOG2E) : 0.f, 0.f), 0ull};
+    double sum = alone > -INFINITY ? double(fast_exp2((alone - r) * LOG2E)) : 0.0;
 #pragma unroll 1
     for (int j = 0; j <= half; ++j) {
 #pragma unroll
@@ -332,10 +482,9 @@ kf_beam_select(const T* logits, long long stride_b, long long stride_w, const fl
             for (int e = 0; e < N; ++e) mx = max_of(mx, x[e] = clean(x[e]));
           }
           if (mx > limit) {
-            const float f = limit == -INFINITY ? 0.f : exp2_fast((r - mx) * LOG2E);
-            sum2[0] = fmul2(sum2[0], pack2(f, f));
-            sum2[1] = fmul2(sum2[1], pack2(f, f));
-            r = mx;
+            const float to = rintf(mx);
+            if (limit > -INFINITY) sum *= double(exp_between(r - to));
+            r = to;
             limit = r + HIGH;
           }
           if (mx >= least_f && mx > -INFINITY) {
@@ -347,12 +496,17 @@ kf_beam_select(const T* logits, long long stride_b, long long stride_w, const fl
         now[u] = fetch(u, j + 1);
         m = max_of(m, mx);
         const uint64_t r2 = pack2(-r, -r), log2e2 = pack2(LOG2E, LOG2E);
+        uint64_t sum2[2];   // of the vector: 32 bits take few terms, and 64 what they come to
 #pragma unroll
         for (int e = 0; e < N; e += 2) {
-          float a, c;
-          unpack2(fmul2(fadd2(pack2(x[e], x[e + 1]), r2), log2e2), a, c);
-          sum2[(e >> 1) & 1] = fadd2(sum2[(e >> 1) & 1], pack2(exp2_fast(a), exp2_fast(c)));
+          float y0, y1;
+          unpack2(fmul2(fadd2(pack2(x[e], x[e + 1]), r2), log2e2), y0, y1);
+          const uint64_t terms = pack2(fast_exp2(y0), fast_exp2(y1));
+          sum2[(e >> 1) & 1] = e < 4 ? terms : fadd2(sum2[(e >> 1) & 1], terms);
         }
+        float even, odd;
+        unpack2(fadd2(sum2[0], sum2[1]), even, odd);
+        sum += double(even + odd);
       }
       if (j > 0 && (j & (j - 1)) == 0) {   // of twice as many vectors
         publish();
@@ -364,13 +518,11 @@ kf_beam_select(const T* logits, long long stride_b, long long stride_w, const fl
 
     // ---- the warp's sum, and the bound again
     {
-      float a, c;
-      unpack2(fadd2(sum2[0], sum2[1]), a, c);
       const float own_r = m > -INFINITY ? r : -INFINITY;
       float wr = own_r;
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) wr = max_of(wr, __shfl_xor_sync(0xffffffffu, wr, o));
-      double ws = m > -INFINITY ? double(a + c) * double(exp2_fast((own_r - wr) * LOG2E)) : 0.0;
+      double ws = m > -INFINITY ? sum * double(exp_between(own_r - wr)) : 0.0;
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) ws += __shfl_xor_sync(0xffffffffu, ws, o);
       const uint32_t top = reached();
@@ -445,7 +597,7 @@ kf_beam_select(const T* logits, long long stride_b, long long stride_w, const fl
       float pr = own;
 #pragma unroll
       for (int o = WARPS / 2; o > 0; o >>= 1) pr = max_of(pr, __shfl_xor_sync(0xffffffffu, pr, o));
-      double ps = own > -INFINITY ? sums[part & 1][lane] * double(exp2_fast((own - pr) * LOG2E)) : 0.0;
+      double ps = own > -INFINITY ? sums[part & 1][lane] * double(exp_between(own - pr)) : 0.0;
 #pragma unroll
       for (int o = WARPS / 2; o > 0; o >>= 1) ps += __shfl_xor_sync(0xffffffffu, ps, o);
       if (lane == 0) {
@@ -472,7 +624,7 @@ kf_beam_select(const T* logits, long long stride_b, long long stride_w, const fl
       double r = own_r;
 #pragma unroll
       for (int o = CTAS_FEW / 2; o > 0; o >>= 1) r = fmax(r, __shfl_xor_sync(0xffffffffu, r, o));
-      double sum = own_r > NONE ? p[lane].sum * double(exp2_fast(float(own_r - r) * LOG2E)) : 0.0;
+      double sum = own_r > NONE ? p[lane].sum * double(exp_between(float(own_r - r))) : 0.0;
 #pragma unroll
       for (int o = CTAS_FEW / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
       const double lse = __shfl_sync(0xffffffffu, r + log(sum), 0);
@@ -491,44 +643,29 @@ kf_beam_select(const T* logits, long long stride_b, long long stride_w, const fl
     }
   }
   __syncthreads();
-  // a candidate's place: how many come before it, its own beam's better ones, others' better ones, lower beams' equal ones; a warp a beam,
-  // eight lanes a candidate
-  for (int w = warp; w < W; w += WARPS)
-    for (int j0 = 0; j0 < W; j0 += 4) {
-      const int j = j0 + lane / 8;
-      const Key mine = j < W ? total[w * totals + j] : 0;
-      int before = 0;
-      for (int x = lane & 7; x < W; x += 8) {
-        const Key* of = total + x * totals;
-        const Key limit = mine - (x < w);
-        int n = 0;
-        for (int k = 0; k < W; k += 8)   // zeros behind the last one
-#pragma unroll
-          for (int e = 0; e < 8; ++e) n += of[k + e] > limit;
-        before += x == w ? j : n;
-      }
-      before = sum_of_8(before);
-      const bool among = mine && before < W;
-      if (among && (lane & 7) == 0) winner[before] = w * W + j;
-      if (!__any_sync(0xffffffffu, among)) break;   // nor are those behind
-    }
-  __syncthreads();
   const uint32_t ends = __ballot_sync(0xffffffffu, done);
-  if (tid < W) {
-    const int i = winner[tid], parent = i < 0 ? tid : i / W;
-    const bool ended = i >= 0 && ((ends >> parent) & 1u);
-    const long long t = i < 0 || ended ? pad : (long long)token[i];
-    out_scores[first + tid] = i < 0 ? -INFINITY : float(unordered(total[parent * totals + i - parent * W]));
-    out_parents[first + tid] = parent;
-    out_tokens[first + tid] = t;
-    out_finished[first + tid] = ended || (i >= 0 && t == eos);
+  find_places(choice, total, totals, W);
+  __syncthreads();
+  write_places(a, choice, token, first, ends, W);
+  // ---- meanwhile: candidates of different beams that may have changed places, neighbours that are NEAR, the last one and any beam's next
+  if (warp == 1) {
+    const int parent = lane < W ? choice.winner[lane] >> 5 : -1, above_parent = lane > 0 && lane < W ? choice.winner[lane - 1] >> 5 : -1;
+    const int last_parent = choice.winner[W - 1] >> 5;
+    uint32_t beams = 0;
+    if (parent >= 0 && above_parent >= 0 && parent != above_parent && unordered(choice.best[lane - 1]) - unordered(choice.best[lane]) <= NEAR)
+      beams = 1u << parent | 1u << above_parent;
+    const Key behind = choice.next[lane];
+    if (behind && last_parent >= 0 && lane != last_parent && unordered(choice.best[W - 1]) - unordered(behind) <= NEAR)
+      beams |= 1u << lane | 1u << last_parent;
+    beams = __reduce_or_sync(0xffffffffu, beams);
+    if (lane == 0) again = beams & live ? beams : 0u;
   }
+  __syncthreads();
+  if (again) choose_again(a, choice, b, again, live, ends, sums[0]);
 }
 
 template <typename T>
-static int launch_select(const void* logits, long long stride_b, long long stride_w, const float* scores, const uint8_t* finished, int B, int W,
-                         int V, long long eos, long long pad, float* out_scores, long long* out_parents, long long* out_tokens,
-                         uint8_t* out_finished, int num_sms, cudaStream_t stream) {
+static int launch_select(const Call<T>& call, int B, int num_sms, cudaStream_t stream) {
   auto kern = kf_beam_select<T>;
   static bool attr_set[16] = {};
   int dev = 0;
@@ -552,8 +689,7 @@ static int launch_select(const void* logits, long long stride_b, long long strid
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  cudaError_t e = cudaLaunchKernelEx(&cfg, kern, (const T*)logits, stride_b, stride_w, scores, finished, W, V, eos, pad, out_scores, out_parents,
-                                     out_tokens, out_finished);
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kern, call);
   return e == cudaSuccess ? 0 : 500 + (int)e;
 }
 
@@ -659,13 +795,15 @@ int kf_beam_select(const void* logits, int type, long long stride_b, long long s
                    void* stream) {
   using namespace kf::beam;
   if (B < 1 || W < 1 || W > MAX_BEAMS || V < 1 || V > 1 << 28) return 3;   // vectors of 32 rows are counted in 32 bits
-  auto go = [&](auto launch) {
-    return launch(logits, stride_b, stride_w, (const float*)scores, (const uint8_t*)finished, B, W, V, eos, pad, (float*)out_scores,
-                  (long long*)out_parents, (long long*)out_tokens, (uint8_t*)out_finished, num_sms, (cudaStream_t)stream);
+  auto go = [&](auto first) {
+    using T = decltype(first);
+    return launch_select(Call<T>{(const T*)logits, stride_b, stride_w, (const float*)scores, (const uint8_t*)finished, W, V, eos, pad, (float*)out_scores,
+                                 (long long*)out_parents, (long long*)out_tokens, (uint8_t*)out_finished},
+                         B, num_sms, (cudaStream_t)stream);
   };
-  if (type == 0) return go(launch_select<__nv_bfloat16>);
-  if (type == 1) return go(launch_select<float>);
-  if (type == 2) return go(launch_select<__half>);
+  if (type == 0) return go(__nv_bfloat16());
+  if (type == 1) return go(float());
+  if (type == 2) return go(__half());
   return 4;
 }
 

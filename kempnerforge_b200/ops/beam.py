@@ -49,11 +49,15 @@ def select(logits: torch.Tensor, scores: torch.Tensor, finished: torch.Tensor | 
            pad_id: int = 0) -> Selected:
     """The W best continuations of each prompt's W beams: logits (B, W, V), scores (B, W) fp32, finished (B, W) bool.
 
-    A beam's candidates are its tokens, with its score plus the token's log-probability, computed in 64 bits and rounded to 32; logits of
-    -inf or NaN are no candidates, +inf counts as the largest fp32 number.  A finished beam has one candidate: itself, with
-    ``pad_id`` and its score; a beam whose score is -inf or NaN has none (a search starts with the scores 0, -inf, -inf, ..).  Best first;
-    ties go to the lower beam, then to the lower token.  A beam that takes ``eos_id`` is finished.  Where there are fewer than W candidates
-    the places left have the score -inf, their own beam as parent and ``pad_id``.
+    A beam's candidates are its tokens, with its score plus the token's log-probability; logits of -inf or NaN are no candidates, +inf
+    counts as the largest fp32 number.  A finished beam has one candidate: itself, with ``pad_id`` and its score; a beam whose score is
+    -inf or NaN has none (a search starts with the scores 0, -inf, -inf, ..).  Best first; ties go to the lower beam, then to the lower
+    token.  A beam that takes ``eos_id`` is finished.  Where there are fewer than W candidates the places left have the score -inf, their
+    own beam as parent and ``pad_id``.
+
+    The order is that of scores in 64 bits.  On a GPU exponentials have 32, which leaves up to 4e-6 in a score before it is rounded to 32
+    bits.  Where candidates of different beams are closer than that can tell, these beams' sums are taken again in 64: one prompt's
+    beams of 128 256 tokens take 57 us longer each, or 28 if their logits are the same.
     """
     eos, pad = -1 if eos_id is None else int(eos_id), int(pad_id)
     if logits.is_cuda and not F._FORCE_REF:
