@@ -176,11 +176,13 @@ kf_shared_prefix_own(const Own a, const Layout lay, const float* part_o, const f
         mma16816(s[1], qa[kk], f[2], f[3]);
       }
     }
+    // Rounded by itself, so that the largest is its own maximum: fused with the difference below, a product of over 2^31 would be off from the
+    // maximum by its rounding, more than an exponent holds.
     const uint32_t sees = (C::STREAM ? seen[st] : masks[st % (C::STREAM ? 1 : C::STAGES)]) >> ((lane & 3) * 2);
 #pragma unroll
     for (int n = 0; n < 2; ++n)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s[n][e] = (sees >> (n * 8 + (e & 1))) & 1u ? s[n][e] * a.scale_log2 : -INFINITY;
+      for (int e = 0; e < 4; ++e) s[n][e] = (sees >> (n * 8 + (e & 1))) & 1u ? __fmul_rn(s[n][e], a.scale_log2) : -INFINITY;
     uint32_t pa[4];
 #pragma unroll
     for (int hf = 0; hf < 2; ++hf) {

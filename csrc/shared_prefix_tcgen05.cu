@@ -29,6 +29,7 @@ constexpr int LEAN_BOUND = 608;                     // threads that a block migh
 constexpr int LEAN_TILES = 3;
 constexpr int TMEM_COLS = 512;
 constexpr float RESCALE_THRESHOLD = 8.0f;           // P up to 2^8 before the accumulator is scaled again
+constexpr float FAR = 0x1p30f;
 
 template <int HD>
 struct Cfg {
@@ -357,13 +358,17 @@ kf_shared_prefix_tcgen05(const __grid_constant__ CUtensorMap map_q, const __grid
     const uint32_t lane_off = uint32_t(quarter * 32) << 16;
     const uint32_t t_s = s_col(g) + lane_off, t_o = o_col(g) + lane_off;
     const float NEG_INF = -INFINITY;
+    // Weights are 2^(x scale - m), fused, so the largest score's is 2 to the rounding of m.  All of a row share that factor, but beyond 2^31 it is
+    // more than an exponent holds.  From 2^30 on a power of two serves as the scale: its products are exact, and scores that differ at all
+    // differ by 32 or more in the exponent, so that with either scale nothing counts but the largest.
+    const float rough_scale = __uint_as_float(__float_as_uint(scale_log2) & 0xff800000u);
     bool ok = true;
     int first = 0, seg = 0, mine = 0;   // tiles before this unit, units, tiles of this group
     while (wk.left > 0) {
       const int n = segment(wk), rows = rows_of(wk, PAIR ? g : 0);
       const bool active = quarter * 32 < rows;   // the warp has rows at all
       const int len = length(lay, wk.b);
-      float m_run = NEG_INF, l_run = 0.f;
+      float m_run = NEG_INF, l_run = 0.f, factor = scale_log2, less = 0.f;
       for (int i = PAIR ? (rows > 0 ? 0 : n) : g; i < n; i += PAIR ? 1 : 2, ++mine) {
         const int n0 = (wk.j + i) * TILE_KEYS;
         if (ok && !mbar_wait(s_full(g), mine & 1, status, KF_ERR_WAIT_TMEM_FULL)) ok = false;
@@ -436,10 +441,12 @@ kf_shared_prefix_tcgen05(const __grid_constant__ CUtensorMap map_q, const __grid
           if (grow) {
             l_run *= alpha;
             m_run = m_new;
+            const bool far = fabsf(m_new) >= FAR;
+            factor = far ? rough_scale : scale_log2;
+            less = far ? -(mx * rough_scale) : -m_new;
           }
         }
-        const float m_use = m_run == NEG_INF ? 0.f : m_run;
-        const uint64_t scale2 = pack2(scale_log2, scale_log2), neg_m2 = pack2(-m_use, -m_use);
+        const uint64_t scale2 = pack2(factor, factor), neg_m2 = pack2(less, less);
         uint64_t lsum[4] = {0ull, 0ull, 0ull, 0ull};
 #pragma unroll(LEAN ? 1 : TILE_KEYS / 32)
         for (int c = 0; c < TILE_KEYS / 32; ++c) {
