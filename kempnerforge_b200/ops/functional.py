@@ -344,6 +344,12 @@ def _on_device(t: torch.Tensor):
     return contextlib.nullcontext() if t.device.index == torch._C._cuda_getDevice() else torch.cuda.device(t.device)
 
 
+def _plain(*tensors: torch.Tensor | None) -> bool:
+    """What a kernel may be given: tensors with memory, no wrappers of a transform, and no tangents that it would drop."""
+    return torch.autograd.forward_ad._current_level < 0 and not any(
+        t is not None and torch._C._functorch.is_functorch_wrapped_tensor(t) for t in tensors)
+
+
 def shared_prefix_attention(
     q: torch.Tensor,
     k: torch.Tensor,
@@ -365,9 +371,10 @@ def shared_prefix_attention(
     A continuation that sees nothing gives zeros.  ``scale`` is positive.
 
     bf16 with heads of 64 or 128 runs ``csrc/shared_prefix_tcgen05.cu`` and ``csrc/shared_prefix_own.cu`` (short prompts the latter
-    alone); other types and sizes, calls that want gradients, and CPU tensors the formulas of ``ops.ref``.
+    alone); other types and sizes, calls that want gradients, in forward mode or under a transform (``vmap``), and CPU tensors the formulas
+    of ``ops.ref``.
     """
-    if q.is_cuda and not _FORCE_REF and _cuda().attn_policy() == "native":
+    if q.is_cuda and not _FORCE_REF and torch.autograd.forward_ad._current_level < 0 and _cuda().attn_policy() == "native":
         out = _cuda().shared_prefix_call(q, k, v, own_k, own_v, prefix_lens, own_rows, scale)
         if out is not None:
             return out
@@ -394,7 +401,8 @@ def shared_prefix_attention(
     if not 0.0 < scale < math.inf:
         raise ValueError(f"scale {scale} is not positive")
     needs_grad = torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, own_k, own_v))
-    if b * w and use_native(q) and not needs_grad and _cuda().attn_policy() == "native" and _cuda().shared_prefix_supported(q, k, scale):
+    if (b * w and use_native(q) and not needs_grad and _plain(q, k, v, own_k, own_v, prefix_lens, own_rows)
+            and _cuda().attn_policy() == "native" and _cuda().shared_prefix_supported(q, k, scale)):
         with _on_device(q):
             if prefix_lens is not None:
                 if prefix_lens.dtype != torch.int32:
