@@ -138,12 +138,12 @@ def shared_prefix_attention(
     sees = torch.ones(b, 1, 1, 1, p, dtype=torch.bool, device=q.device)
     if prefix_lens is not None:
         sees = (torch.arange(p, device=q.device) < prefix_lens[:, None])[:, None, None, None]
-        vf = torch.where(sees[:, 0, 0, 0, :, None, None], vf, 0.0)
+        kf, vf = (torch.where(sees[:, 0, 0, 0, :, None, None], t, 0.0) for t in (kf, vf))   # gradients multiply by what keys hold, too
     own_sees = torch.ones(b, w, 1, 1, s, dtype=torch.bool, device=q.device)
     if own_rows is not None:
         own_sees = (own_rows < w)[:, :, None, None]
         at = torch.arange(b, device=q.device)[:, None, None], own_rows.long().clamp_max(w - 1), torch.arange(s, device=q.device)
-        okf, ovf = okf[at], torch.where(own_sees[:, :, 0, 0, :, None, None], ovf[at], 0.0)
+        okf, ovf = (torch.where(own_sees[:, :, 0, 0, :, None, None], t[at], 0.0) for t in (okf, ovf))
     scores = torch.cat([torch.einsum("bwkgd,bpkd->bwkgp", qf, kf).masked_fill(~sees, float("-inf")),
                         torch.einsum("bwkgd,bwskd->bwkgs", qf, okf).masked_fill(~own_sees, float("-inf"))], dim=-1) * scale
     some = torch.cat([sees.expand(b, w, 1, 1, p), own_sees], dim=-1).any(-1, keepdim=True)
