@@ -103,7 +103,8 @@ PyObject* beam_reorder(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     if (!whole && (x->dim() < 3 || x->size(2) < length)) Py_RETURN_NONE;
     if (y->sizes() != x->sizes() || y->scalar_type() != x->scalar_type()) Py_RETURN_NONE;
     const long long size = x->element_size();
-    for (const at::Tensor* t : {x, y}) {
+    for (int j = in_place ? 1 : 0; j < 2; ++j) {   // in place the two are one, and one span
+      const at::Tensor* t = j ? y : x;
       if (!t->is_cuda() || t->get_device() != device || t->size(0) != b || t->size(1) != w || t->is_conj() || t->is_neg()) Py_RETURN_NONE;
       long long step = 1;   // what a beam holds is dense, beams do not overlap
       for (int64_t d = t->dim() - 1; d >= 2; --d) {
@@ -113,16 +114,15 @@ PyObject* beam_reorder(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
       if (step < 1 || (w > 1 && t->stride(1) < step) || (b > 1 && t->stride(0) < step) ||
           (b > 1 && w > 1 && t->stride(0) < w * t->stride(1) && t->stride(1) < b * t->stride(0)))
         Py_RETURN_NONE;
-      if (t == y || !in_place) {
-        const auto base = reinterpret_cast<long long>(t->const_data_ptr());
-        spans.push_back({base, base + ((b - 1) * t->stride(0) + (w - 1) * t->stride(1) + step) * size, t == y});
-      }
+      const auto base = reinterpret_cast<long long>(t->const_data_ptr());
+      spans.push_back({base, base + ((b - 1) * t->stride(0) + (w - 1) * t->stride(1) + step) * size, j == 1});
     }
     const long long inner = x->dim() > 2 ? x->size(2) : 1;
     const long long beam = x->numel() / (b * w) / inner * (whole ? inner : length) * size;
     if (beam > 1LL << 37) Py_RETURN_NONE;
-    const long long row[7] = {reinterpret_cast<long long>(x->const_data_ptr()), reinterpret_cast<long long>(at_(*y)), x->stride(0) * size,
-                              x->stride(1) * size, y->stride(0) * size, y->stride(1) * size, beam};
+    const auto dst = reinterpret_cast<long long>(at_(*y));   // first: memory that a lazy clone shares is y's own after this
+    const long long row[7] = {in_place ? dst : reinterpret_cast<long long>(x->const_data_ptr()), dst, x->stride(0) * size, x->stride(1) * size,
+                              y->stride(0) * size, y->stride(1) * size, beam};
     table.insert(table.end(), row, row + 7);
     to.push_back(y);
   }
