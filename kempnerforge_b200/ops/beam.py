@@ -73,7 +73,7 @@ def select(logits: torch.Tensor, scores: torch.Tensor, finished: torch.Tensor | 
                          f"{finished.device}")
     logits, scores = logits.detach(), scores.detach().contiguous()
     finished = None if finished is None else finished.contiguous()
-    if logits.shape[0] and _native(logits) and _cuda().beam_select_supported(logits):
+    if logits.shape[0] and _native(logits) and F._plain(logits, scores, finished) and _cuda().beam_select_supported(logits):
         with _on(logits):
             return Selected(*_cuda().beam_select(logits, scores, finished, eos, pad))
     return Selected(*ref.beam_select(logits, scores, finished, eos, pad))
