@@ -119,7 +119,8 @@ def reorder(states: list[torch.Tensor], parents: torch.Tensor, length: int | Non
     int64 or int32, any selection of beams; where one is no beam (outside 0 .. W - 1) that place stays as it is.  Returns what was written.
     """
     states, to = list(states), None if out is None else list(out)
-    if parents.is_cuda and not F._FORCE_REF and _cuda().beam_reorder_call(states, parents, length, to):
+    native = _native(parents) and torch.autograd.forward_ad._current_level < 0   # the formulas move tangents with the states
+    if native and _cuda().beam_reorder_call(states, parents, length, to):
         return states if to is None else to
     if parents.dim() != 2 or parents.dtype not in (torch.int64, torch.int32):
         raise ValueError(f"parents are (prompts, beams) in int64 or int32, not {tuple(parents.shape)} {parents.dtype}")
@@ -152,7 +153,7 @@ def reorder(states: list[torch.Tensor], parents: torch.Tensor, length: int | Non
     if parents.numel() == 0 or not states:
         return to
     with torch.no_grad():
-        if not (_native(parents) and parents.shape[1] <= 32 and parents.shape[0] <= 65535):
+        if not (native and parents.shape[1] <= 32 and parents.shape[0] <= 65535):
             ref.beam_reorder(states, parents, length, to)
         else:
             _reorder_native(states, parents, length, to)
