@@ -101,12 +101,22 @@ def _span(t: torch.Tensor) -> tuple[int, int]:
 
 
 def _interleaved(a: torch.Tensor, b: torch.Tensor) -> bool:
-    """Tensors of one shape and stepping whose beams lie between each other's."""
-    if a.shape != b.shape or a.stride() != b.stride() or a.element_size() != b.element_size() or not _dense_beams(a):
+    """Tensors of one shape and stepping whose values lie between each other's: no value of the one shares memory with one of the other."""
+    if a.shape != b.shape or a.stride() != b.stride() or a.element_size() != b.element_size():
         return False
-    steps = [s * a.element_size() for n, s in zip(a.shape[:2], a.stride()[:2]) if n > 1]
-    own, apart = a[0, 0].numel() * a.element_size(), abs(a.data_ptr() - b.data_ptr())
-    return own <= apart and all(s >= apart + own for s in steps)
+    size = a.element_size()
+    steps = sorted(((s * size, n) for n, s in zip(a.shape, a.stride()) if n > 1), reverse=True)
+    if any(s < (inner[0] * inner[1] if inner else size) for (s, _), inner in zip(steps, [*steps[1:], None])):
+        return False   # a step that is shorter than what it steps over: not looked into
+
+    def met(apart: int, level: int) -> bool:
+        """Whether steps from `level` on, so many forwards or backwards as there are entries, come within a value's size of `apart`."""
+        if level == len(steps):
+            return abs(apart) < size
+        s, n = steps[level]   # what is left is less than a step
+        return any(abs(k) < n and met(apart - k * s, level + 1) for k in (apart // s, apart // s + 1))
+
+    return not met(a.data_ptr() - b.data_ptr(), 0)
 
 
 def reorder(states: list[torch.Tensor], parents: torch.Tensor, length: int | None = None,
