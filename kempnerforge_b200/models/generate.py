@@ -78,7 +78,7 @@ def beam_search(model, prompt_tokens: torch.Tensor, max_new_tokens: int, num_bea
 
     A score is the sum of the new tokens' log-probabilities divided by their number to the power ``length_penalty`` (an
     ``eos_token_id`` counts, what follows it does not, and is filled with it).  During the search beams compete by their sums; a finished
-    one keeps its place as long as its sum does.  The search ends when all beams have finished or at ``max_new_tokens``.
+    one keeps its place as long as its sum does.  The search ends when all beams that there are have finished, or at ``max_new_tokens``.
     """
     cfg = model.config
     b, plen = prompt_tokens.shape
@@ -113,7 +113,8 @@ def beam_search(model, prompt_tokens: torch.Tensor, max_new_tokens: int, num_bea
             beam.reorder([tokens, rows], step.parents, n)
         tokens[:, :, n] = step.tokens
         scores, finished = step.scores, step.finished
-        if n + 1 == max_new_tokens or (eos_token_id is not None and bool(finished.all())):
+        # a place without a continuation stays one: where the others have finished, nothing can come
+        if n + 1 == max_new_tokens or (eos_token_id is not None and bool((finished | scores.isneginf()).all())):
             break
         logits = model(step.tokens.view(b * w, 1), kv_caches=caches)[:, -1].view(b, w, -1)
     if was_training:
