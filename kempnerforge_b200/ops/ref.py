@@ -174,8 +174,6 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, finished: torch.Tens
     token = torch.where(done[..., None], pad_id, token)
     width = total.shape[-1]
     total, at = torch.sort(total.flatten(1), dim=-1, descending=True, stable=True)
-    if width < w:   # fewer tokens than beams
-        total, at = (torch.nn.functional.pad(t, (0, max(0, w - t.shape[1])), value=fill) for t, fill in ((total, float("-inf")), (at, 0)))
     total, at = total[:, :w], at[:, :w]
     none = total == float("-inf")
     parents = torch.where(none, torch.arange(w, device=logits.device), at // width)
