@@ -162,6 +162,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, finished: torch.Tens
     x = torch.where(x > float("-inf"), x.clamp_max(torch.finfo(torch.float32).max), float("-inf"))
     top = x.amax(-1, keepdim=True)
     shifted = torch.where(x > float("-inf"), x - top, float("-inf"))
+    shifted = torch.nn.functional.pad(shifted, (0, -vocab % 16), value=float("-inf"))   # rows that begin alike are added up alike
     lse = top + shifted.exp().sum(-1, keepdim=True).log()
     x, token = torch.sort(x, dim=-1, descending=True, stable=True)
     x, token = x[..., :w], token[..., :w]
