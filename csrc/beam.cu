@@ -130,7 +130,7 @@ __device__ __forceinline__ int sum_of_8(int x) {
 }
 
 // 32 bytes of logits, on 32 bytes: the widest load there is.
-struct Raw {
+struct alignas(32) Raw {
   uint32_t w[8];
 };
 __device__ __forceinline__ Raw load_raw(const Raw* p) {
@@ -353,14 +353,16 @@ kf_beam_select(const __grid_constant__ Call<T> a) {
   __shared__ int n_found[MAX_PARTS], n_notes[MAX_PARTS];
   __shared__ Key notes[NOTES];                     // (largest logit, vector)
   __shared__ Raw noted_raw[NOTES];                 // the vector
-  __shared__ Key found[ROOM];                      // candidates, or the warps' lists
+  __shared__ Key found[ROOM];                      // candidates, or the warps' lists; later the candidates' tokens
   __shared__ Choice choice;
   __shared__ uint32_t again;                       // beams that choose_again looks at
   const int W = a.W, V = a.V;
   Key* total = reinterpret_cast<Key*>(noted_raw);
   const int totals = (W + 7) / 8 * 8 + 1;          // an odd number spreads the beams' over the banks
   uint32_t* token = reinterpret_cast<uint32_t*>(found);
-  static_assert(sizeof(noted_raw) >= MAX_BEAMS * (MAX_BEAMS + 1) * 8 && sizeof(found) >= MAX_BEAMS * MAX_BEAMS * 4, "");
+  static_assert(sizeof(noted_raw) >= MAX_BEAMS * (MAX_BEAMS + 1) * sizeof(Key) && alignof(Raw) >= alignof(Key) &&
+                    sizeof(found) >= MAX_BEAMS * MAX_BEAMS * sizeof(uint32_t) && alignof(Key) >= alignof(uint32_t),
+                "what `total` and `token` lie in");
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tid = threadIdx.x;
   const uint32_t ctas = cluster_nctaid();
