@@ -147,12 +147,12 @@ PyObject* beam_reorder(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
-// A cache or a query as 16-byte copies take it; its steps are appended.
-bool steps_of(const at::Tensor& t, long long*& steps) {
+// A cache or a query as 16-byte copies take it; its steps are appended.  `one`: the first may be 0.
+bool steps_of(const at::Tensor& t, bool one, long long*& steps) {
   const int64_t last = t.dim() - 1;
   if (t.numel() > 0 && ((t.stride(last) != 1) || !address(t))) return false;
   for (int64_t d = 0; d < last; ++d) {
-    if (t.size(d) > 1 && t.numel() > 0 && (t.stride(d) <= 0 || t.stride(d) % 8)) return false;
+    if (t.size(d) > 1 && t.numel() > 0 && (t.stride(d) < (one && d == 0 ? 0 : 1) || t.stride(d) % 8)) return false;
     *steps++ = t.size(d) > 1 && t.numel() > 0 ? t.stride(d) : 0;
   }
   return true;
@@ -186,7 +186,7 @@ PyObject* shared_prefix_attn(PyObject*, PyObject* const* args, Py_ssize_t nargs)
   if (!(scale >= kScales[0] && scale <= kScales[1])) Py_RETURN_NONE;
   long long steps[19], *next = steps;
   for (int i = 0; i < 5; ++i)
-    if (!steps_of(*t[i], next)) Py_RETURN_NONE;
+    if (!steps_of(*t[i], i == 1 || i == 2, next)) Py_RETURN_NONE;
   steps[17] = rows ? rows->stride(0) : 0;
   steps[18] = rows ? rows->stride(1) : 0;
   HANDLE_TH_ERRORS

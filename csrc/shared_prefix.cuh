@@ -26,6 +26,7 @@ struct Layout {
   int pair, wt;        // row tiles of a unit, 1 or 2; continuations per row tile
   int ctas, most;      // how many are launched; how many might be, whatever the lengths
   int span;            // without lens: tiles that a unit counts for
+  int k_step, v_step;  // 0: all prompts have the first one's keys, or values
 };
 
 __host__ __device__ __forceinline__ int tiles_of(int len) { return (len + TILE_KEYS - 1) / TILE_KEYS; }

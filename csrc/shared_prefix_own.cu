@@ -426,7 +426,7 @@ static bool make_layout(Layout& l, const void* lens, int B, int W, int P, int gr
   const int pair = wt < W && 4LL * B * P * Hkv * hd > PAIR_BYTES ? 2 : 1, row_units = (W + wt * pair - 1) / (wt * pair);
   const long long tiles = (long long)tiles_of(P) * Hkv * row_units * B;
   const int most = (int)(tiles < num_sms ? tiles : num_sms);
-  l = Layout{(const int*)lens, B, W, P, Hkv * row_units, row_units, pair, wt, most, most, tiles_of(P)};
+  l = Layout{(const int*)lens, B, W, P, Hkv * row_units, row_units, pair, wt, most, most, tiles_of(P), 1, 1};
   const long long units = (long long)B * l.per_prompt;
   if (!lens && P > 0 && units <= num_sms) {
     const int ways = num_sms / (int)units, each = (l.span + ways - 1) / ways, whole = (l.span + each - 1) / each;
@@ -468,7 +468,8 @@ long long kf_shared_prefix_scratch(int B, int W, int P, int H, int Hkv, int hd, 
 // o (B, W, H, hd), dense = attention of q (B, W, H, hd) over k, v (B, P, Hkv, hd), of which lens[b] positions count (null: all), and over
 // own_k, own_v (B, W, S, Hkv, hd), where position s of continuation w lies in the cache of continuation rows[b][w][s] (null: w).
 // steps: in elements, of q (prompt, continuation, head), k and v (prompt, position, head), own_k and own_v (prompt, continuation, position,
-// head) and rows (prompt, continuation): 19 numbers.  Head dim 64 or 128, dense; steps multiples of 8 and bases on 16 bytes (rows: any).
+// head) and rows (prompt, continuation): 19 numbers.  Head dim 64 or 128, dense; steps multiples of 8 and bases on 16 bytes (rows: any).  Of k and v
+// the step from prompt to prompt may be 0; other steps are of dimensions of one entry where they are.
 int kf_shared_prefix_attn_bf16(const void* q, const void* k, const void* v, const void* own_k, const void* own_v, const void* lens,
                                const void* rows, void* o, void* scratch, int B, int W, int P, int S, int H, int Hkv, int hd,
                                const long long* steps, float scale, int direct, int num_sms, void* stream) {
@@ -476,6 +477,8 @@ int kf_shared_prefix_attn_bf16(const void* q, const void* k, const void* v, cons
   Layout l;
   if (kf_shared_prefix_scratch(B, W, P, H, Hkv, hd, direct, num_sms) < 0 || S < 0 || !(scale > 0.f)) return 3;
   make_layout(l, lens, B, W, P, H / Hkv, Hkv, hd, num_sms);
+  l.k_step = steps[3] != 0;
+  l.v_step = steps[6] != 0;
   const long long *qs = steps, *ks = steps + 3, *vs = steps + 6, *oks = steps + 9, *ovs = steps + 13, *rs = steps + 17;
   for (int i = 0; i < 17; ++i)
     if (steps[i] & 7) return 5;

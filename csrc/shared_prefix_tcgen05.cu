@@ -230,7 +230,8 @@ kf_shared_prefix_tcgen05(const __grid_constant__ CUtensorMap map_q, const __grid
             mbar_expect_tx(k_full(turn.st), C::TILE_BYTES);
 #pragma unroll
             for (int c = 0; c < C::BLOCKS; ++c)
-              tma_load_4d(k_smem + turn.st * C::TILE_BYTES + c * C::BLOCK_BYTES, &map_k, k_full(turn.st), 64 * c, hk, j * TILE_KEYS, wk.b);
+              tma_load_4d(k_smem + turn.st * C::TILE_BYTES + c * C::BLOCK_BYTES, &map_k, k_full(turn.st), 64 * c, hk, j * TILE_KEYS,
+                          wk.b * lay.k_step);
             ++issued;
           }
           advance(lay, wk, n);
@@ -257,7 +258,8 @@ kf_shared_prefix_tcgen05(const __grid_constant__ CUtensorMap map_q, const __grid
             mbar_expect_tx(v_full(turn.st), C::TILE_BYTES);
 #pragma unroll
             for (int c = 0; c < C::BLOCKS; ++c)
-              tma_load_4d(v_smem + turn.st * C::TILE_BYTES + c * C::BLOCK_BYTES, &map_v, v_full(turn.st), 64 * c, hk, j * TILE_KEYS, wk.b);
+              tma_load_4d(v_smem + turn.st * C::TILE_BYTES + c * C::BLOCK_BYTES, &map_v, v_full(turn.st), 64 * c, hk, j * TILE_KEYS,
+                          wk.b * lay.v_step);
             ++issued;
           }
           advance(lay, wk, n);
@@ -613,9 +615,11 @@ int launch_prefix(const void* q, const void* k, const void* v, const Layout& l, 
   int rc = make_map_4d(&mq, q, {(uint64_t)hd, (uint64_t)H, (uint64_t)l.W, (uint64_t)l.B}, {qs[2], qs[1], qs[0]},
                        {64u, (uint32_t)group, (uint32_t)l.wt, 1u});
   if (rc) return 1000 + rc;
-  rc = make_map_4d(&mk, k, {(uint64_t)hd, (uint64_t)Hkv, (uint64_t)l.P, (uint64_t)l.B}, {ks[2], ks[1], ks[0]}, {64u, 1u, (uint32_t)TILE_KEYS, 1u});
+  rc = make_map_4d(&mk, k, {(uint64_t)hd, (uint64_t)Hkv, (uint64_t)l.P, (uint64_t)(l.k_step ? l.B : 1)}, {ks[2], ks[1], ks[0]},
+                   {64u, 1u, (uint32_t)TILE_KEYS, 1u});
   if (rc) return 2000 + rc;
-  rc = make_map_4d(&mv, v, {(uint64_t)hd, (uint64_t)Hkv, (uint64_t)l.P, (uint64_t)l.B}, {vs[2], vs[1], vs[0]}, {64u, 1u, (uint32_t)TILE_KEYS, 1u});
+  rc = make_map_4d(&mv, v, {(uint64_t)hd, (uint64_t)Hkv, (uint64_t)l.P, (uint64_t)(l.v_step ? l.B : 1)}, {vs[2], vs[1], vs[0]},
+                   {64u, 1u, (uint32_t)TILE_KEYS, 1u});
   if (rc) return 3000 + rc;
   return hd == 128 ? launch_hd<128>(mq, mk, mv, l, group, few, scale, part_o, part_ml, status, stream)
                    : launch_hd<64>(mq, mk, mv, l, group, few, scale, part_o, part_ml, status, stream);

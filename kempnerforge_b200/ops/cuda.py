@@ -1079,10 +1079,12 @@ def _steps_of(t: torch.Tensor) -> list[int]:
     return [s if n > 1 else 0 for n, s in zip(t.shape[:-1], t.stride()[:-1])]
 
 
-def _copies_ok(t: torch.Tensor) -> torch.Tensor:
-    """`t` where 16-byte copies can take it: a dense last dimension, steps and base on 16 bytes; else a copy that is so."""
+def _copies_ok(t: torch.Tensor, one: bool = False) -> torch.Tensor:
+    """`t` where 16-byte copies can take it: a dense last dimension, steps and base on 16 bytes; else a copy that is so.  `one`: the first
+    step may be 0."""
     if (t.numel() == 0 or t.stride(-1) == 1 and t.data_ptr() % 16 == 0
-            and all(n == 1 or (s > 0 and s % 8 == 0) for n, s in zip(t.shape[:-1], t.stride()[:-1]))):
+            and all(n == 1 or (s >= (0 if one and d == 0 else 1) and s % 8 == 0)
+                    for d, (n, s) in enumerate(zip(t.shape[:-1], t.stride()[:-1])))):
         return t
     return t.clone(memory_format=torch.contiguous_format)
 
@@ -1107,7 +1109,7 @@ def shared_prefix_supported(q: torch.Tensor, k: torch.Tensor, scale: float) -> b
 def shared_prefix_attn(q, k, v, own_k, own_v, prefix_lens, own_rows, scale: float, direct: int = -1) -> torch.Tensor:
     """q (B, W, H, hd), k / v (B, P, Hkv, hd), own_k / own_v (B, W, S, Hkv, hd) bf16, prefix_lens (B,) int32, own_rows (B, W, S) uint8.
     ``direct``: 1 reads the prompts for every continuation again, in one kernel, 0 once for all, in two; -1: the faster way."""
-    q, k, v, own_k, own_v = (_copies_ok(t) for t in (q, k, v, own_k, own_v))
+    q, k, v, own_k, own_v = _copies_ok(q), _copies_ok(k, one=True), _copies_ok(v, one=True), _copies_ok(own_k), _copies_ok(own_v)
     b, w, h, hd = q.shape
     p, hkv, s = k.shape[1], k.shape[2], own_k.shape[2]
     if own_rows is not None and own_rows.stride(2) != 1:

@@ -362,8 +362,9 @@ def shared_prefix_attention(
 ) -> torch.Tensor:
     """One new token for each of W continuations of B prompts: softmax(q [K | own K]ᵀ * scale) [V | own V] -> (B, W, H, hd).
 
-    q (B, W, H, hd); k, v (B, P, Hkv, hd): the prompts' keys and values, read once for all continuations; own_k, own_v
-    (B, W, S, Hkv, hd): those of each continuation's own tokens, the new one's included.  P or S may be 0.
+    q (B, W, H, hd); k, v (B, P, Hkv, hd): the prompts' keys and values, read once for all continuations (and where they lie, if one prompt is
+    expanded over the batch); own_k, own_v (B, W, S, Hkv, hd): those of each continuation's own tokens, the new one's included.  P or S may
+    be 0.
 
     ``prefix_lens`` (B,) int32 or int64: how many positions of each prompt count, 0 .. P; what lies behind them is not looked at.
     ``own_rows`` (B, W, S) uint8: position s of continuation w lies in the own cache of continuation ``own_rows[b, w, s]`` of the same
