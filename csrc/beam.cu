@@ -21,7 +21,8 @@
 //     CTAs put theirs into the first one's shared memory.
 // What bounds it: many prompts, the logits, which are read once (64 x 8 x 128 256 in bf16, an eighth finished: 115 MB in 40 us, 2.9 TB/s: the
 // pass at 75 to 80 % of a copy's rate, and behind it, in every CTA at the same time, bounds, candidates and sums); few prompts, these steps
-// and the launch (1 x 4 x 32 000: 7.4 us).  Launches are joined to the one before (programmatic launch): by itself a launch of clusters began 2.4 us later.
+// and the launch (1 x 4 x 32 000: 7.2 us).  Launches are joined to the one before (programmatic launch): by itself a launch of clusters began
+// 2.4 us later.
 //
 // kf_beam_reorder.  state[b, w] = state[b, parent[b, w]] for all states in one launch.  A thread owns 16 bytes of a column: it reads
 // the column's W values and then writes them, so that parents may be any selection of beams, also in place, without a second buffer.
@@ -43,10 +44,10 @@ using decode::mapa_shared;
 constexpr int MAX_BEAMS = 32;   // a warp's list is one key per lane
 constexpr int WARPS = 8;
 constexpr int THREADS = WARPS * 32;
-// CTAs of a cluster: 16 where all clusters' CTAs have an SM each, which few prompts need (1 x 8 x 128 256: 20.7 -> 16.1 us), else 8.
+// CTAs of a cluster: 16 where all clusters' CTAs have an SM each, which few prompts need (1 x 8 x 128 256: 18.2 -> 13.4 us), else 8.
 constexpr int CTAS_FEW = 16, CTAS_MANY = 8;
 // Vectors that a CTA reads in the time that bounds and candidates of a second row take it.  Rows dealt out in equal shares / a whole number of
-// CTAs each, us: 3 x 5 x 50 257 12.8 / 10.4, 2 x 6 x 128 256 16.0 / 14.0, 2 x 12 x 50 257 19.1 / 16.6, 4 x 7 x 30 000 13.6 / 9.4.
+// CTAs each, us: 3 x 5 x 50 257 12.8 / 10.6, 2 x 6 x 128 256 14.7 / 13.5, 2 x 12 x 50 257 18.3 / 15.8, 4 x 7 x 30 000 11.9 / 9.0.
 constexpr uint32_t SPARE = 2048;
 constexpr int MAX_PARTS = MAX_BEAMS / CTAS_MANY + 1;  // rows that a CTA's range meets
 constexpr int NOTES = 512;                            // vectors that a CTA notes (20 KB); more (rising logits, equal ones) go through lists
@@ -286,7 +287,8 @@ __device__ __forceinline__ void write_places(const Call<T>& a, const Choice& c, 
 // i % THREADS, so that equal rows have equal sums wherever they lie.  Where all rows are equal one sum will do, whatever its last bits.
 // Nothing follows this, so that the pass keeps no registers for it; that, and not a call (0.1 to 0.5 us for every selection).
 template <typename T>
-__device__ __forceinline__ void choose_again(const Call<T>& a, Choice& c, long long b, uint32_t near, uint32_t live, uint32_t ends, double* of_warps) {
+__device__ __forceinline__ void choose_again(const Call<T>& a, Choice& c, long long b, uint32_t near, uint32_t live, uint32_t ends,
+                                             double* of_warps) {
   constexpr int AT_ONCE = 8;
   const int tid = threadIdx.x, W = a.W;
   const int lead = __ffs(near & live) - 1;
@@ -334,6 +336,8 @@ __device__ __forceinline__ void choose_again(const Call<T>& a, Choice& c, long l
   write_places(a, c, c.token, b * W, ends, W);
 }
 
+// Four CTAs an SM, which is 64 registers: with logits of 16 bits 80 bytes are spilled and 130 read back.  With three and none, us:
+// 1 x 8 x 128 256 13.4 / 12.8, 40 x 8 x 50 257 22.3 / 18.0, but 64 x 8 x 128 256 40.1 / 49.2, 64 x 8 x 32 000 in fp32 21.9 / 27.7.
 template <typename T>
 __global__ void __launch_bounds__(THREADS, 4)
 kf_beam_select(const __grid_constant__ Call<T> a) {
@@ -799,9 +803,9 @@ int kf_beam_select(const void* logits, int type, long long stride_b, long long s
   if (B < 1 || W < 1 || W > MAX_BEAMS || V < 1 || V > 1 << 28) return 3;   // vectors of 32 rows are counted in 32 bits
   auto go = [&](auto first) {
     using T = decltype(first);
-    return launch_select(Call<T>{(const T*)logits, stride_b, stride_w, (const float*)scores, (const uint8_t*)finished, W, V, eos, pad, (float*)out_scores,
-                                 (long long*)out_parents, (long long*)out_tokens, (uint8_t*)out_finished},
-                         B, num_sms, (cudaStream_t)stream);
+    const Call<T> call{(const T*)logits, stride_b, stride_w, (const float*)scores, (const uint8_t*)finished, W, V, eos, pad, (float*)out_scores,
+                       (long long*)out_parents, (long long*)out_tokens, (uint8_t*)out_finished};
+    return launch_select(call, B, num_sms, (cudaStream_t)stream);
   };
   if (type == 0) return go(__nv_bfloat16());
   if (type == 1) return go(float());

@@ -8,6 +8,15 @@
 // Without lens, and where that makes the ranges no more than SPARE tiles longer, a unit counts for a whole number of ranges: a CTA that ends a
 // unit and begins another one has two results to write, 5800 cycles each, and waits for first keys twice.  Equal ranges / whole numbers, us:
 // 2 x 30 x 8254 (32 heads on 8) 27.5 / 24.1, 6 x 16 x 1568 (16 on 4) 15.6 / 13.1, 4 x 3 x 6522 (40 on 8) 29.3 / 26.6, 2 x 64 x 8000 32.3 / 28.4.
+//
+// Which form a call takes, in this order (kf_shared_prefix_attn_bf16, launch_own, launch_hd):
+//   prompts      the second kernel alone (is_direct): up to 4 MB times continuations, prompts of one tile up to 64;
+//                else the first kernel, two row tiles a unit (make_layout) where a key head has over 128 rows and the prompts 168 MB or more;
+//                else one row tile, LEAN up to three tiles a CTA, or with heads of 128, one row tile a key head and at most 128 own keys;
+//                else one row tile with all scores in registers.
+//   own keys     (launch_own; tiles of 16, the prompts' among them where this kernel is alone) rings of one, then of two tiles, with 1, 2 or 4
+//                warps a unit, where these hold all tiles and no more warps come to an SM than fit at once;
+//                else 1 to 32 warps a unit that stream, as many as fit, through 16 KB each where 8 to 12 come to an SM, else through 24.
 #pragma once
 #include <cuda_runtime.h>
 #include <stdint.h>

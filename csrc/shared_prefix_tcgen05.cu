@@ -24,7 +24,7 @@ namespace shared_prefix {
 using namespace kf::attn;
 
 constexpr int THREADS = 384;
-constexpr int REGS_ISSUE = 72, REGS_SOFTMAX = 216;  // per thread; 72 + 2 * 216 = 3 * 168, what the launch gets
+constexpr int REGS_ISSUE = 72, REGS_SOFTMAX = 216;  // per thread; 72 + 2 * 216 = 3 * 168, what the launch gets (68 bytes are spilled)
 constexpr int LEAN_BOUND = 608;                     // threads that a block might have: 96 registers each
 constexpr int LEAN_TILES = 3;
 constexpr int TMEM_COLS = 512;
@@ -462,7 +462,7 @@ kf_shared_prefix_tcgen05(const __grid_constant__ CUtensorMap map_q, const __grid
             unpack2(x2, x0, x1);
             const float e0 = fast_exp2(x0), e1 = fast_exp2(x1);
             lsum[k & 3] = fadd2(lsum[k & 3], pack2(e0, e1));
-            pk[k] = pack_bf16(e0, e1);
+            pk[k] = pack_bf16(e0, e1);   // as V is, which the product asks for; the sum is of the unrounded weights
           }
           tmem_st_32x16(t_s + c * 16, pk);
           if (c & 1) {   // half of the keys are in place
