@@ -55,8 +55,9 @@ def select(logits: torch.Tensor, scores: torch.Tensor, finished: torch.Tensor | 
     token.  A beam that takes ``eos_id`` is finished.  Where there are fewer than W candidates the places left have the score -inf, their
     own beam as parent and ``pad_id``.
 
-    The order is that of scores in 64 bits.  On a GPU exponentials have 32, which leaves up to 4e-6 in a score before it is rounded to 32
-    bits.  Where candidates of different beams are closer than that can tell, these beams' sums are taken again in 64: one prompt's
+    The order is that of scores in 64 bits, s + (x - (top + log of the sum)).  (Beside logits of 1e16 and more 64 bits hold no logarithm: all of
+    a row of the lowest fp32 value have the log-probability 0.)  On a GPU exponentials have 32, which leaves up to 4e-6 in a score before it
+    is rounded to 32 bits.  Where candidates of different beams are closer than that can tell, these beams' sums are taken again in 64: one prompt's
     beams of 128 256 tokens take 57 us longer each, or 28 if their logits are the same.
     """
     eos, pad = -1 if eos_id is None else int(eos_id), int(pad_id)
